@@ -41,6 +41,7 @@ _STATUS_NAMES = {
 
 # name -> (restype, argtypes); mirrors include/flash_sinkhorn_b200.h one to one.
 _P = c_void_p
+_L = ctypes.c_longlong
 SIGNATURES = {
     "fs_version": (c_int, []),
     "fs_last_error": (c_char_p, []),
@@ -143,6 +144,18 @@ SIGNATURES = {
         [_P, _P, c_int, c_int, c_int, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_float, c_float, c_int,
          c_float, c_float, c_int, _P, c_size_t, _P],
     ),
+    "fs_route_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "fs_route": (
+        c_int, [_P, c_int, _L, c_int, c_int, c_int, _P, _P, c_int, _P, _P, _P, _P, _P, _P, _P, c_size_t, _P]),
+    "fs_route_grad": (c_int, [_P, c_int, _L, c_int, c_int, c_int, _P, _P, c_int, _P, _P, _P, _P, _P]),
+    "fs_grouped_mm": (
+        c_int, [_P, _L, c_int, _P, c_int, _P, _L, _L, _L, c_int, c_int, c_int, _P, _P, _L, c_int, _P]),
+    "fs_grouped_mm_wgrad": (
+        c_int, [_P, _L, c_int, _P, _P, _L, c_int, _P, c_int, c_int, c_int, c_int, _P, _P, c_int, _P]),
+    "fs_gated_act": (c_int, [_P, c_int, _L, c_int, c_int, _P, _P, _P, _P, _P, _P]),
+    "fs_gated_act_grad": (c_int, [_P, _L, _P, _P, c_int, c_int, c_int, _P, _P, _P, _P, _L, _P, _P, _P, _P]),
+    "fs_combine": (c_int, [_P, c_int, _L, c_int, c_int, c_int, _P, _P, _P, _P]),
+    "fs_combine_grad": (c_int, [_P, c_int, _L, c_int, c_int, c_int, _P, _P, _P, _P, _L, _P, _P, _P]),
 }
 
 _lib: Optional[ctypes.CDLL] = None

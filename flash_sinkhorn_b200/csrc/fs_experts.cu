@@ -1,0 +1,789 @@
+// Routed experts around their matrix products: the choice of experts and the order of the rows, the gated activation
+// with its 8-bit checkpoint, and the sum of the experts' rows back into tokens. All of it is bound by memory traffic (the
+// routing of a large batch by instruction issue); every value is read once and nothing is kept between calls.
+#include "fs_experts.cuh"
+
+namespace fs {
+namespace ex {
+namespace {
+
+constexpr unsigned kAll = 0xffffffffu;
+
+// ---------------------------------------------------------------------------------------------------------------
+// Routing
+// ---------------------------------------------------------------------------------------------------------------
+// Token t goes to the k experts with the largest score = logit + bias (fp32; ties to the lower expert), among those that
+// are on: logit and bias above -inf, token not masked. Its gates are the soft-max of the LOGITS over the chosen experts or
+// over all that are on. The (token, slot) pairs of an expert keep their order, so the result is the same in every run.
+//
+// One warp per token, expert j in lane j % 32. Two kernels of at most kMaxBlocks CTAs, CTA b with tokens [b c, (b + 1) c):
+// the first selects and counts the CTA's pairs per expert, the second adds up the counts of the CTAs before it (every CTA
+// for itself: E x kMaxBlocks words from L2, cheaper than a third launch or CTAs that wait for one another) and numbers
+// its own pairs. Batches of one CTA do both in one launch.
+
+constexpr int kRouteWarps = 16;
+constexpr int kMaxBlocks = 296;    // two CTAs on each of 148 SMs
+constexpr int kMaxExperts = 1024;  // 32 per lane
+constexpr int kMaxK = 32;          // one slot per lane
+
+struct RouteArgs {
+  const void* logits;
+  long long ld;
+  int T, E, k, chunk, blocks;
+  const float* bias;
+  const uint8_t* mask;
+  int over_all;
+  float* gates;
+  int *experts, *offsets, *pairs, *rows, *position;
+  int* counts;  // [E, blocks]
+  // gradient
+  const float *gates_in, *grad;
+  const int* experts_in;
+  void* out;
+};
+
+// Unsigned keys in the order of the scores: 0 for an expert that is off, NaN above everything (it then shows in the gates).
+__device__ __forceinline__ unsigned score_key(float s) {
+  if (s != s) return 0xffffffffu;
+  const unsigned b = __float_as_uint(s + 0.f);  // -0 becomes +0: they tie
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+  return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kAll, v, o));
+  return v;
+}
+
+template <typename T, int PER>
+__device__ __forceinline__ void load_logits(const RouteArgs& a, int t, int lane, float (&l)[PER], bool (&on)[PER]) {
+  const T* row = static_cast<const T*>(a.logits) + (long long)t * a.ld;
+  const bool token_on = !a.mask || a.mask[t];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int j = i * 32 + lane;
+    l[i] = j < a.E ? to_f32(row[j]) : -INFINITY;
+    on[i] = token_on && l[i] != -INFINITY && (!a.bias || j >= a.E || a.bias[j] != -INFINITY);
+  }
+}
+// Largest logit of the experts that are on, and the sum of exp(logit - largest) over them.
+template <int PER>
+__device__ __forceinline__ void soft_max_over(const float (&l)[PER], const bool (&on)[PER], float& top, float& sum) {
+  top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) top = on[i] ? fmaxf(top, l[i]) : top;
+  top = warp_max(top);
+  sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) sum += on[i] ? expf(l[i] - top) : 0.f;
+  sum = warp_sum(sum);
+}
+
+template <typename T, int PER>
+__device__ __forceinline__ void select_tokens(const RouteArgs& a, int* count) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int t0 = blockIdx.x * a.chunk, t1 = min(t0 + a.chunk, a.T);
+  for (int t = t0 + warp; t < t1; t += kRouteWarps) {
+    float l[PER];
+    bool on[PER];
+    load_logits<T, PER>(a, t, lane, l, on);
+    unsigned key[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int j = i * 32 + lane;
+      key[i] = on[i] ? score_key(a.bias ? l[i] + a.bias[j] : l[i]) : 0u;
+    }
+    int expert = -1;       // of slot `lane`
+    float chosen = 0.f;    // its logit
+    for (int s = 0; s < a.k; ++s) {
+      unsigned best = key[0];
+#pragma unroll
+      for (int i = 1; i < PER; ++i) best = max(best, key[i]);
+      best = __reduce_max_sync(kAll, best);
+      if (best == 0u) break;
+      int at = 0x7fffffff;
+#pragma unroll
+      for (int i = PER - 1; i >= 0; --i) at = key[i] == best ? i * 32 + lane : at;
+      at = __reduce_min_sync(kAll, at);
+      float mine = 0.f;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        if (i == at >> 5) {
+          mine = l[i];
+          if (lane == (at & 31)) key[i] = 0u;
+        }
+      }
+      mine = __shfl_sync(kAll, mine, at & 31);
+      if (lane == s) {
+        expert = at;
+        chosen = mine;
+      }
+    }
+    float top, sum;
+    if (a.over_all) {
+      soft_max_over<PER>(l, on, top, sum);
+    } else {
+      const float one[1] = {chosen};
+      const bool has[1] = {expert >= 0};
+      soft_max_over<1>(one, has, top, sum);
+    }
+    if (lane < a.k) {
+      const long long p = (long long)t * a.k + lane;
+      a.gates[p] = expert >= 0 ? expf(chosen - top) / sum : 0.f;
+      a.experts[p] = expert;
+      if (expert >= 0) atomicAdd(count + expert, 1);
+    }
+  }
+}
+
+// Exclusive prefix over v[0 .. n) in shared memory, by all threads of the CTA; the total comes back.
+__device__ __forceinline__ int scan_in_place(int* v, int n, int* scratch) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int base = 0;
+  for (int c = 0; c < n; c += kRouteWarps * 32) {
+    const int j = c + threadIdx.x, x = j < n ? v[j] : 0;
+    int inc = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(kAll, inc, o);
+      inc += lane >= o ? y : 0;
+    }
+    if (lane == 31) scratch[warp] = inc;
+    __syncthreads();
+    int before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < kRouteWarps; ++w) {
+      before += w < warp ? scratch[w] : 0;
+      total += scratch[w];
+    }
+    if (j < n) v[j] = base + before + inc - x;
+    base += total;
+    __syncthreads();
+  }
+  return base;
+}
+
+// Rows of this CTA's pairs. first[e]: row of its first pair of expert e. hist: [kRouteWarps, E].
+__device__ __forceinline__ void number_pairs(const RouteArgs& a, int* first, int* hist, int total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int j = threadIdx.x; j < kRouteWarps * a.E; j += kRouteWarps * 32) hist[j] = 0;
+  __syncthreads();
+  const long long p0 = (long long)blockIdx.x * a.chunk * a.k;
+  const long long p1 = min((long long)a.T, (long long)(blockIdx.x + 1) * a.chunk) * a.k;
+  const long long share = ((p1 - p0 + kRouteWarps - 1) / kRouteWarps + 31) / 32 * 32;  // pairs of a warp, in order
+  const long long w0 = p0 + warp * share, w1 = min(p1, w0 + share);
+  int* mine = hist + warp * a.E;
+  for (long long p = w0 + lane; p - lane < w1; p += 32) {
+    const int e = p < w1 ? a.experts[p] : -1;
+    const unsigned same = __match_any_sync(kAll, e);
+    if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
+    __syncwarp();
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < a.E; e += kRouteWarps * 32) {
+    int at = first[e];
+#pragma unroll
+    for (int w = 0; w < kRouteWarps; ++w) {
+      const int c = hist[w * a.E + e];
+      hist[w * a.E + e] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+  for (long long p = w0 + lane; p - lane < w1; p += 32) {
+    const int e = p < w1 ? a.experts[p] : -1;
+    const unsigned same = __match_any_sync(kAll, e);
+    const int rank = __popc(same & ((1u << lane) - 1u));
+    const int at = e >= 0 ? mine[e] + rank : -1;
+    __syncwarp();
+    if (e >= 0 && rank == 0) mine[e] += __popc(same);
+    __syncwarp();
+    if (p < w1) {
+      a.position[p] = at;
+      if (at >= 0) {
+        a.pairs[at] = (int)p;
+        a.rows[at] = (int)(p / a.k);
+      }
+      if (p >= total) a.pairs[p] = a.rows[p] = -1;  // rows after the last one that is routed
+    }
+  }
+}
+
+template <typename T, int PER>
+__global__ void __launch_bounds__(kRouteWarps * 32) route_select_kernel(const RouteArgs a) {
+  extern __shared__ int sm[];
+  __shared__ int scratch[kRouteWarps];
+  int* count = sm;  // [E], then the histograms of the warps
+  for (int e = threadIdx.x; e < a.E; e += kRouteWarps * 32) count[e] = 0;
+  __syncthreads();
+  select_tokens<T, PER>(a, count);
+  __syncthreads();
+  if (a.blocks > 1) {
+    for (int e = threadIdx.x; e < a.E; e += kRouteWarps * 32) a.counts[e * a.blocks + blockIdx.x] = count[e];
+    return;
+  }
+  const int total = scan_in_place(count, a.E, scratch);
+  __syncthreads();
+  for (int e = threadIdx.x; e < a.E; e += kRouteWarps * 32) a.offsets[e] = count[e];
+  if (threadIdx.x == 0) a.offsets[a.E] = total;
+  number_pairs(a, count, sm + a.E, total);
+}
+
+__global__ void __launch_bounds__(kRouteWarps * 32) route_order_kernel(const RouteArgs a) {
+  extern __shared__ int sm[];
+  __shared__ int scratch[kRouteWarps];
+  int *all = sm, *before = sm + a.E;  // pairs of expert e in all CTAs, in the CTAs before this one
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int e = warp; e < a.E; e += kRouteWarps) {
+    int n = 0, b = 0;
+#pragma unroll 4
+    for (int c = lane; c < a.blocks; c += 32) {
+      const int v = a.counts[e * a.blocks + c];
+      n += v;
+      b += c < (int)blockIdx.x ? v : 0;
+    }
+    n = __reduce_add_sync(kAll, n);
+    b = __reduce_add_sync(kAll, b);
+    if (lane == 0) {
+      all[e] = n;
+      before[e] = b;
+    }
+  }
+  __syncthreads();
+  const int total = scan_in_place(all, a.E, scratch);
+  for (int e = threadIdx.x; e < a.E; e += kRouteWarps * 32) {
+    if (blockIdx.x == 0) a.offsets[e] = all[e];
+    before[e] += all[e];
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.offsets[a.E] = total;
+  __syncthreads();
+  number_pairs(a, before, sm + 2 * a.E, total);
+}
+
+// d logit_j = [j chosen as slot s] g_s dg_s - p_j sum_s g_s dg_s, p = the soft-max that the gates were taken from.
+template <typename T, int PER>
+__global__ void __launch_bounds__(kRouteWarps * 32) route_grad_kernel(const RouteArgs a) {
+  const int lane = threadIdx.x & 31;
+  for (long long t = (long long)blockIdx.x * kRouteWarps + (threadIdx.x >> 5); t < a.T; t += (long long)gridDim.x * kRouteWarps) {
+    const long long p = t * a.k + lane;
+    const int expert = lane < a.k ? a.experts_in[p] : -1;
+    const float gate = expert >= 0 ? a.gates_in[p] : 0.f;
+    const float own = expert >= 0 ? gate * a.grad[p] : 0.f, inner = warp_sum(own);
+    float v[PER];
+    if (a.over_all) {
+      float l[PER], top, sum;
+      bool on[PER];
+      load_logits<T, PER>(a, (int)t, lane, l, on);
+      soft_max_over<PER>(l, on, top, sum);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) v[i] = on[i] ? -inner * (expf(l[i] - top) / sum) : 0.f;
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) v[i] = 0.f;
+    }
+    const float add = a.over_all ? own : own - gate * inner;
+    for (int s = 0; s < a.k; ++s) {
+      const int e = __shfl_sync(kAll, expert, s);
+      const float g = __shfl_sync(kAll, add, s);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) v[i] += e == i * 32 + lane ? g : 0.f;
+    }
+    T* row = static_cast<T*>(a.out) + t * a.E;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (i * 32 + lane < a.E) row[i * 32 + lane] = from_f32<T>(v[i]);
+  }
+}
+
+// Tokens per CTA: a whole number of rounds of its warps, and at most kMaxBlocks CTAs. Small batches (16 tokens a warp)
+// stay in one CTA and one launch: 256 tokens of 64 experts take less time there than a second launch does.
+void plan_route(int T, int& chunk, int& blocks) {
+  chunk = (T + kMaxBlocks - 1) / kMaxBlocks;
+  chunk = (chunk + kRouteWarps - 1) / kRouteWarps * kRouteWarps;
+  if (T <= 16 * kRouteWarps) chunk = 16 * kRouteWarps;
+  blocks = T > 0 ? (T + chunk - 1) / chunk : 1;
+}
+
+template <typename K>
+int allow_smem(K kernel, size_t bytes) {
+  if (bytes <= 48 * 1024) return FS_OK;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  return e == cudaSuccess ? FS_OK : report_error(FS_ERR_CUDA, cudaGetErrorString(e));
+}
+
+template <typename T, int PER>
+int launch_route(const RouteArgs& a, bool grad, cudaStream_t st) {
+  if (grad) {
+    const long long want = ((long long)a.T + kRouteWarps - 1) / kRouteWarps;
+    route_grad_kernel<T, PER><<<(int)(want < 592 ? want : 592), kRouteWarps * 32, 0, st>>>(a);
+    return launched(1);
+  }
+  const size_t one = (size_t)(a.blocks > 1 ? 1 : 1 + kRouteWarps) * a.E * 4, two = (size_t)(2 + kRouteWarps) * a.E * 4;
+  int s = allow_smem(route_select_kernel<T, PER>, one);
+  if (s != FS_OK) return s;
+  if (a.blocks > 1 && (s = allow_smem(route_order_kernel, two)) != FS_OK) return s;
+  route_select_kernel<T, PER><<<a.blocks, kRouteWarps * 32, one, st>>>(a);
+  if (a.blocks > 1) route_order_kernel<<<a.blocks, kRouteWarps * 32, two, st>>>(a);
+  return launched(a.blocks > 1 ? 2 : 1);
+}
+template <typename T>
+int launch_route(const RouteArgs& a, bool grad, cudaStream_t st) {
+  const int per = (a.E + 31) / 32;
+  if (per <= 1) return launch_route<T, 1>(a, grad, st);
+  if (per <= 2) return launch_route<T, 2>(a, grad, st);
+  if (per <= 4) return launch_route<T, 4>(a, grad, st);
+  if (per <= 8) return launch_route<T, 8>(a, grad, st);
+  if (per <= 16) return launch_route<T, 16>(a, grad, st);
+  return launch_route<T, 32>(a, grad, st);
+}
+int launch_route(const RouteArgs& a, int type, bool grad, cudaStream_t st) {
+  if (type == FS_TYPE_F32) return launch_route<float>(a, grad, st);
+  if (type == FS_TYPE_F16) return launch_route<__half>(a, grad, st);
+  return launch_route<__nv_bfloat16>(a, grad, st);
+}
+
+int check_route(const void* logits, int type, long long ld, int T, int E, int k) {
+  if (type < 0 || type > 2) return report_error(FS_ERR_BAD_ARG, "type must be FS_TYPE_F32, FS_TYPE_F16 or FS_TYPE_BF16");
+  if (T < 0 || E < 1 || E > kMaxExperts) return report_error(FS_ERR_BAD_ARG, "T must be >= 0 and E in [1, 1024]");
+  if (k < 1 || k > kMaxK || k > E) return report_error(FS_ERR_BAD_ARG, "k must be in [1, min(E, 32)]");
+  if ((long long)T * k > 0x7fffffffll) return report_error(FS_ERR_BAD_ARG, "T * k must be below 2^31");
+  if (ld < E || (T > 0 && !logits)) return report_error(FS_ERR_BAD_ARG, "logits must have rows of at least E values");
+  return check_device();
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Gated activation and its checkpoint
+// ---------------------------------------------------------------------------------------------------------------
+// h = p silu(g) v of rows u = [g | v], p = the gate of the row's pair (1 without a routing). The backward pass needs g and
+// v; the checkpoint holds them in blocks of 32 along the row as integers in [-127, 127] times 2^e, e the smallest exponent
+// at which the block's largest magnitude rounds to 127 at most: 8.25 bits instead of 16, an error of at most half a step
+// = 2^-7 of the block's maximum (a quarter of that of an 8-bit float with 3 bits of fraction at the same size), and since
+// scaling by a power of two is exact the codes do not depend on how the quotient is rounded. A block with an infinity or
+// a NaN has exponent code 255 and stands for NaN throughout.
+//
+// A warp per row (or per part of a row, where there are few), VEC values of each half per lane and step: 16-byte loads for
+// 16-bit types. 32 / VEC neighbouring lanes share a block.
+
+constexpr int kActWarps = 8;
+
+struct ActArgs {
+  const void* u;
+  long long ldu;
+  int R, F, parts;
+  const float* gates;
+  const int* pairs;
+  void* h;  // forward: the result; backward (may be null): the result recomputed from the checkpoint
+  int8_t* codes;
+  uint8_t* scales;
+  // backward
+  const int* position;
+  const void* dh;
+  long long lddh;
+  void* du;
+  float* dgates;
+};
+
+__device__ __forceinline__ unsigned block_exponent(unsigned amax_bits) {
+  if (amax_bits >= 0x7f800000u) return 255u;
+  const int e = (int)(amax_bits >> 23), m = (int)(amax_bits & 0x7fffffu);
+  const int code = e - (m < 0x7f0000 ? 6 : 5);  // magnitude * 2^(127 - code) is in [64, 127.5)
+  return (unsigned)(code < 1 ? 1 : code);
+}
+__device__ __forceinline__ float block_scale(unsigned code) {
+  return code == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(code << 23);
+}
+// Codes of this lane's values (whole warps; 32 / VEC lanes hold a block); the exponent code of the block comes back.
+template <int VEC>
+__device__ __forceinline__ unsigned encode(const float (&x)[VEC], int8_t (&q)[VEC]) {
+  unsigned top = 0u;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+#pragma unroll
+  for (int o = 16 / VEC; o; o >>= 1) top = max(top, __shfl_xor_sync(kAll, top, o));
+  const unsigned code = block_exponent(top);
+  const float inv = code == 255u ? 0.f : __uint_as_float((254u - code) << 23);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) q[i] = code == 255u ? (int8_t)0 : (int8_t)__float2int_rn(x[i] * inv);
+  return code;
+}
+
+__device__ __forceinline__ float row_gate(const ActArgs& a, int r, bool& routed) {
+  routed = true;
+  if (!a.pairs) return 1.f;
+  const int p = a.pairs[r];
+  routed = p >= 0 && p < a.R;  // as many pairs as rows
+  return routed ? a.gates[p] : 0.f;
+}
+__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kActWarps * 32) act_kernel(const ActArgs a) {
+  const int lane = threadIdx.x & 31;
+  constexpr int kLanes = 32 / VEC;  // of a block
+  const int steps = (a.F + 32 * VEC - 1) / (32 * VEC), share = (steps + a.parts - 1) / a.parts;
+  const int nb = (a.F + 31) / 32;
+  const long long items = (long long)a.R * a.parts;
+  for (long long it = (long long)blockIdx.x * kActWarps + (threadIdx.x >> 5); it < items; it += (long long)gridDim.x * kActWarps) {
+    const int r = (int)(it / a.parts), s0 = (int)(it - (long long)r * a.parts) * share, s1 = min(s0 + share, steps);
+    bool routed;
+    const float p = row_gate(a, r, routed);
+    const T* row = static_cast<const T*>(a.u) + (long long)r * a.ldu;
+    T* out = static_cast<T*>(a.h) + (long long)r * a.F;
+#pragma unroll 2
+    for (int s = s0; s < s1; ++s) {
+      const int c = (s * 32 + lane) * VEC;
+      const bool in = c < a.F;
+      float g[VEC], v[VEC], h[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) g[i] = v[i] = h[i] = 0.f;
+      if (routed) {
+        if (in) {
+          load_f32<T, VEC>(row + c, g);
+          load_f32<T, VEC>(row + a.F + c, v);
+        }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) h[i] = p * (g[i] * sigmoid(g[i])) * v[i];
+        if (a.codes) {
+          Pack<int8_t, VEC> q[2];
+          const unsigned eg = encode<VEC>(g, q[0].v), ev = encode<VEC>(v, q[1].v);
+          if (in) {
+            int8_t* codes = a.codes + (long long)r * 2 * a.F + c;
+            *reinterpret_cast<Pack<int8_t, VEC>*>(codes) = q[0];
+            *reinterpret_cast<Pack<int8_t, VEC>*>(codes + a.F) = q[1];
+            if (lane % kLanes == 0) {
+              uint8_t* sc = a.scales + (long long)r * 2 * nb + c / 32;
+              sc[0] = (uint8_t)eg;
+              sc[nb] = (uint8_t)ev;
+            }
+          }
+        }
+      }
+      if (in) store_f32<T, VEC>(out + c, h);
+    }
+  }
+}
+
+// du = [p dh v s (1 + g (1 - s)) | p dh g s] with s = sigmoid(g), and d p = sum dh g s v, from the checkpoint (CODES) or
+// from u as it was. One warp per row: the sum over the row stays in the warp.
+template <typename T, int VEC, bool CODES>
+__global__ void __launch_bounds__(kActWarps * 32) act_grad_kernel(const ActArgs a) {
+  const int lane = threadIdx.x & 31, nb = (a.F + 31) / 32;
+  for (int r = blockIdx.x * kActWarps + (threadIdx.x >> 5); r < a.R; r += gridDim.x * kActWarps) {
+    bool routed;
+    const float p = row_gate(a, r, routed);
+    T *du = static_cast<T*>(a.du) + (long long)r * 2 * a.F, *hr = a.h ? static_cast<T*>(a.h) + (long long)r * a.F : nullptr;
+    float dp = 0.f;
+#pragma unroll 2
+    for (int c = lane * VEC; c < a.F; c += 32 * VEC) {
+      float dg[VEC], dv[VEC], h[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) dg[i] = dv[i] = h[i] = 0.f;
+      if (routed) {
+        float g[VEC], v[VEC], d[VEC];
+        if (CODES) {
+          const int8_t* codes = a.codes + (long long)r * 2 * a.F + c;
+          const uint8_t* sc = a.scales + (long long)r * 2 * nb + c / 32;
+          const Pack<int8_t, VEC> qg = *reinterpret_cast<const Pack<int8_t, VEC>*>(codes);
+          const Pack<int8_t, VEC> qv = *reinterpret_cast<const Pack<int8_t, VEC>*>(codes + a.F);
+          const float sg = block_scale(sc[0]), sv = block_scale(sc[nb]);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            g[i] = sg * (float)qg.v[i];
+            v[i] = sv * (float)qv.v[i];
+          }
+        } else {
+          const T* row = static_cast<const T*>(a.u) + (long long)r * a.ldu + c;
+          load_f32<T, VEC>(row, g);
+          load_f32<T, VEC>(row + a.F, v);
+        }
+        load_f32<T, VEC>(static_cast<const T*>(a.dh) + (long long)r * a.lddh + c, d);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float s = sigmoid(g[i]), gs = g[i] * s, pd = p * d[i];
+          dv[i] = pd * gs;
+          dg[i] = pd * v[i] * (s + gs * (1.f - s));
+          dp += d[i] * gs * v[i];
+          h[i] = p * gs * v[i];
+        }
+      }
+      store_f32<T, VEC>(du + c, dg);
+      store_f32<T, VEC>(du + a.F + c, dv);
+      if (hr) store_f32<T, VEC>(hr + c, h);
+    }
+    if (a.dgates) {
+      dp = warp_sum(dp);
+      if (lane == 0) {
+        if (routed) a.dgates[a.pairs[r]] = dp;
+        if (a.position[r] < 0) a.dgates[r] = 0.f;  // r as a pair: one that has no row
+      }
+    }
+  }
+}
+
+// Values a lane takes at a time: the most (8, 4 or 1) that divides the widths and that all pointers are aligned to.
+template <typename... P>
+int lane_values(int F, int bytes, long long ld0, long long ld1, P... ptrs) {
+  for (int v : {8, 4}) {
+    const size_t a = (size_t)v * bytes < 16 ? (size_t)v * bytes : 16;
+    if (F % v == 0 && ld0 % v == 0 && ld1 % v == 0 && (aligned(ptrs, a) && ...)) return v;
+  }
+  return 1;
+}
+
+// Parts of a row, where the rows alone do not give every SM some warps.
+int row_parts(long long rows, int width, int vec) {
+  const int steps = (width + 32 * vec - 1) / (32 * vec);
+  const long long want = rows > 0 ? (148 * 16 + rows - 1) / rows : 1;
+  return (int)(want < 1 ? 1 : want > steps ? steps : want);
+}
+int row_blocks(long long items) {
+  const long long b = (items + kActWarps - 1) / kActWarps;
+  return (int)(b < 1 ? 1 : b > 148 * 64 ? 148 * 64 : b);
+}
+
+template <typename T, int VEC>
+int launch_act(ActArgs a, bool grad, cudaStream_t st) {
+  if (!grad) {
+    a.parts = row_parts(a.R, a.F, VEC);
+    act_kernel<T, VEC><<<row_blocks((long long)a.R * a.parts), kActWarps * 32, 0, st>>>(a);
+  } else if (a.codes) {
+    act_grad_kernel<T, VEC, true><<<row_blocks(a.R), kActWarps * 32, 0, st>>>(a);
+  } else {
+    act_grad_kernel<T, VEC, false><<<row_blocks(a.R), kActWarps * 32, 0, st>>>(a);
+  }
+  return launched(1);
+}
+template <typename T>
+int launch_act(const ActArgs& a, bool grad, int vec, cudaStream_t st) {
+  if (vec == 8) return launch_act<T, 8>(a, grad, st);
+  if (vec == 4) return launch_act<T, 4>(a, grad, st);
+  return launch_act<T, 1>(a, grad, st);
+}
+int launch_act(const ActArgs& a, int type, bool grad, int vec, cudaStream_t st) {
+  if (type == FS_TYPE_F32) return launch_act<float>(a, grad, vec, st);
+  if (type == FS_TYPE_F16) return launch_act<__half>(a, grad, vec, st);
+  return launch_act<__nv_bfloat16>(a, grad, vec, st);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Rows back into tokens
+// ---------------------------------------------------------------------------------------------------------------
+// y_t = sum_s w_ts o[position_ts] over the slots that are routed, w = the gates or 1, summed in fp32 in slot order and
+// rounded once. A warp per token (or part of one), all its rows' loads in flight together.
+
+struct CombineArgs {
+  const void* o;
+  long long ldo;
+  int T, k, D, parts;
+  const float* gates;  // null: weights of 1
+  const int *position, *pairs;
+  void* y;
+  const void* dy;
+  long long lddy;
+  void* d_o;
+  float* dgates;
+};
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kActWarps * 32) combine_kernel(const CombineArgs a) {
+  const int lane = threadIdx.x & 31, n = a.T * a.k;
+  const int steps = (a.D + 32 * VEC - 1) / (32 * VEC), share = (steps + a.parts - 1) / a.parts;
+  const long long items = (long long)a.T * a.parts;
+  for (long long it = (long long)blockIdx.x * kActWarps + (threadIdx.x >> 5); it < items; it += (long long)gridDim.x * kActWarps) {
+    const int t = (int)(it / a.parts), s0 = (int)(it - (long long)t * a.parts) * share, s1 = min(s0 + share, steps);
+    const long long pair = (long long)t * a.k + lane;
+    const int at = lane < a.k ? a.position[pair] : -1;
+    const float w = lane < a.k && a.gates ? a.gates[pair] : 1.f;
+    for (int s = s0; s < s1; ++s) {
+      const int c = (s * 32 + lane) * VEC;
+      float y[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) y[i] = 0.f;
+#pragma unroll 4
+      for (int j = 0; j < a.k; ++j) {
+        const int row = __shfl_sync(kAll, at, j);
+        const float wj = __shfl_sync(kAll, w, j);
+        if (row >= 0 && row < n && c < a.D) {
+          float o[VEC];
+          load_f32<T, VEC>(static_cast<const T*>(a.o) + (long long)row * a.ldo + c, o);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) y[i] += wj * o[i];
+        }
+      }
+      if (c < a.D) store_f32<T, VEC>(static_cast<T*>(a.y) + (long long)t * a.D + c, y);
+    }
+  }
+}
+
+// do_i = w dy_t and d w = <dy_t, o_i> for the row i of a pair; rows of no pair get zeros, pairs of no row a zero gradient.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kActWarps * 32) combine_grad_kernel(const CombineArgs a) {
+  const int lane = threadIdx.x & 31, n = a.T * a.k;
+  for (int r = blockIdx.x * kActWarps + (threadIdx.x >> 5); r < n; r += gridDim.x * kActWarps) {
+    const int pair = a.pairs[r];
+    const bool routed = pair >= 0 && pair < n;
+    const float w = routed ? (a.gates ? a.gates[pair] : 1.f) : 0.f;
+    const T* dy = static_cast<const T*>(a.dy) + (long long)(routed ? pair / a.k : 0) * a.lddy;
+    const T* o = static_cast<const T*>(a.o) + (long long)r * a.ldo;
+    T* out = static_cast<T*>(a.d_o) + (long long)r * a.D;
+    float dw = 0.f;
+#pragma unroll 2
+    for (int c = lane * VEC; c < a.D; c += 32 * VEC) {
+      float g[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) g[i] = 0.f;
+      if (routed) {
+        load_f32<T, VEC>(dy + c, g);
+        if (a.dgates) {
+          float x[VEC];
+          load_f32<T, VEC>(o + c, x);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) dw += g[i] * x[i];
+        }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) g[i] *= w;
+      }
+      store_f32<T, VEC>(out + c, g);
+    }
+    if (a.dgates) {
+      dw = warp_sum(dw);
+      if (lane == 0) {
+        if (routed) a.dgates[pair] = dw;
+        if (a.position[r] < 0) a.dgates[r] = 0.f;  // r as a pair: one that has no row
+      }
+    }
+  }
+}
+
+template <typename T, int VEC>
+int launch_combine(CombineArgs a, bool grad, cudaStream_t st) {
+  a.parts = row_parts(a.T, a.D, VEC);
+  if (!grad) combine_kernel<T, VEC><<<row_blocks((long long)a.T * a.parts), kActWarps * 32, 0, st>>>(a);
+  else combine_grad_kernel<T, VEC><<<row_blocks((long long)a.T * a.k), kActWarps * 32, 0, st>>>(a);
+  return launched(1);
+}
+template <typename T>
+int launch_combine(const CombineArgs& a, bool grad, int vec, cudaStream_t st) {
+  if (vec == 8) return launch_combine<T, 8>(a, grad, st);
+  if (vec == 4) return launch_combine<T, 4>(a, grad, st);
+  return launch_combine<T, 1>(a, grad, st);
+}
+int launch_combine(const CombineArgs& a, int type, bool grad, int vec, cudaStream_t st) {
+  if (type == FS_TYPE_F32) return launch_combine<float>(a, grad, vec, st);
+  if (type == FS_TYPE_F16) return launch_combine<__half>(a, grad, vec, st);
+  return launch_combine<__nv_bfloat16>(a, grad, vec, st);
+}
+
+int check_rows(int type, int rows, int width) {
+  if (type < 0 || type > 2) return report_error(FS_ERR_BAD_ARG, "type must be FS_TYPE_F32, FS_TYPE_F16 or FS_TYPE_BF16");
+  if (rows < 0 || width < 1 || width > (1 << 28)) return report_error(FS_ERR_BAD_ARG, "rows must be >= 0 and the width in [1, 2^28]");
+  return check_device();
+}
+
+}  // namespace
+}  // namespace ex
+}  // namespace fs
+
+using namespace fs;
+using namespace fs::ex;
+
+extern "C" {
+
+size_t fs_route_bytes(int T, int E, int k) {
+  (void)k;
+  if (T < 0 || E < 1 || E > kMaxExperts) return 0;
+  int chunk, blocks;
+  plan_route(T, chunk, blocks);
+  return blocks > 1 ? (size_t)E * blocks * sizeof(int) : 0;
+}
+
+int fs_route(const void* logits, int type, long long ld, int T, int E, int k, const float* bias, const uint8_t* mask,
+             int over_all, float* gates, int* experts, int* offsets, int* pairs, int* rows, int* position, void* ws,
+             size_t ws_bytes, void* stream) {
+  int s = check_route(logits, type, ld, T, E, k);
+  if (s != FS_OK) return s;
+  if (!offsets || (T > 0 && (!gates || !experts || !pairs || !rows || !position)))
+    return report_error(FS_ERR_BAD_ARG, "null argument");
+  if (ws_bytes < fs_route_bytes(T, E, k) || (fs_route_bytes(T, E, k) > 0 && !ws))
+    return report_error(FS_ERR_WORKSPACE, "workspace smaller than fs_route_bytes()");
+  RouteArgs a{};
+  a.logits = logits; a.ld = ld; a.T = T; a.E = E; a.k = k; a.bias = bias; a.mask = mask; a.over_all = over_all;
+  a.gates = gates; a.experts = experts; a.offsets = offsets; a.pairs = pairs; a.rows = rows; a.position = position;
+  a.counts = static_cast<int*>(ws);
+  plan_route(T, a.chunk, a.blocks);
+  return launch_route(a, type, false, static_cast<cudaStream_t>(stream));
+}
+
+int fs_route_grad(const void* logits, int type, long long ld, int T, int E, int k, const float* bias, const uint8_t* mask,
+                  int over_all, const float* gates, const int* experts, const float* grad, void* out, void* stream) {
+  int s = check_route(logits, type, ld, T, E, k);
+  if (s != FS_OK || T == 0) return s;
+  if (!gates || !experts || !grad || !out) return report_error(FS_ERR_BAD_ARG, "null argument");
+  RouteArgs a{};
+  a.logits = logits; a.ld = ld; a.T = T; a.E = E; a.k = k; a.bias = bias; a.mask = mask; a.over_all = over_all;
+  a.gates_in = gates; a.experts_in = experts; a.grad = grad; a.out = out;
+  return launch_route(a, type, true, static_cast<cudaStream_t>(stream));
+}
+
+int fs_gated_act(const void* u, int type, long long ldu, int R, int F, const float* gates, const int* pairs, void* h,
+                 int8_t* codes, uint8_t* scales, void* stream) {
+  int s = check_rows(type, R, F);
+  if (s != FS_OK || R == 0) return s;
+  if (!u || !h || ldu < 2 * (long long)F || (pairs && !gates) || (codes && !scales))
+    return report_error(FS_ERR_BAD_ARG, "null argument, or rows of u shorter than 2 F");
+  ActArgs a{};
+  a.u = u; a.ldu = ldu; a.R = R; a.F = F; a.gates = gates; a.pairs = pairs; a.h = h;
+  a.codes = codes; a.scales = scales;
+  // the codes' alignment is that of their first byte and the width: 8 values of a lane are one store
+  int vec = lane_values(F, type_bytes(type), ldu, 0, u, h);
+  while (codes && vec > 1 && !aligned(codes, vec)) vec = vec == 8 ? 4 : 1;
+  return launch_act(a, type, false, vec, static_cast<cudaStream_t>(stream));
+}
+
+int fs_gated_act_grad(const void* u, long long ldu, const int8_t* codes, const uint8_t* scales, int type, int R, int F,
+                      const float* gates, const int* pairs, const int* position, const void* dh, long long lddh, void* du,
+                      float* dgates, void* h, void* stream) {
+  int s = check_rows(type, R, F);
+  if (s != FS_OK || R == 0) return s;
+  if ((!u && !codes) || (codes && !scales) || !dh || !du || lddh < F || (u && !codes && ldu < 2 * (long long)F) ||
+      (pairs && !gates) || (dgates && (!pairs || !position)))
+    return report_error(FS_ERR_BAD_ARG, "null argument, or rows shorter than their width");
+  ActArgs a{};
+  a.u = u; a.ldu = ldu; a.R = R; a.F = F; a.gates = gates; a.pairs = pairs; a.position = position; a.h = h;
+  a.codes = const_cast<int8_t*>(codes); a.scales = const_cast<uint8_t*>(scales);
+  a.dh = dh; a.lddh = lddh; a.du = du; a.dgates = dgates;
+  int vec = lane_values(F, type_bytes(type), codes ? 0 : ldu, lddh, codes ? nullptr : u, dh, du, static_cast<const void*>(h));
+  while (codes && vec > 1 && !aligned(codes, vec)) vec = vec == 8 ? 4 : 1;
+  return launch_act(a, type, true, vec, static_cast<cudaStream_t>(stream));
+}
+
+int fs_combine(const void* o, int type, long long ldo, int T, int k, int D, const float* gates, const int* position, void* y,
+               void* stream) {
+  int s = check_rows(type, T, D);
+  if (s != FS_OK || T == 0) return s;
+  if (k < 1 || k > kMaxK || (long long)T * k > 0x7fffffffll) return report_error(FS_ERR_BAD_ARG, "k must be in [1, 32], T * k below 2^31");
+  if (!o || !position || !y || ldo < D) return report_error(FS_ERR_BAD_ARG, "null argument, or rows shorter than D");
+  CombineArgs a{};
+  a.o = o; a.ldo = ldo; a.T = T; a.k = k; a.D = D; a.gates = gates; a.position = position; a.y = y;
+  return launch_combine(a, type, false, lane_values(D, type_bytes(type), ldo, 0, o, y), static_cast<cudaStream_t>(stream));
+}
+
+int fs_combine_grad(const void* o, int type, long long ldo, int T, int k, int D, const float* gates, const int* position,
+                    const int* pairs, const void* dy, long long lddy, void* d_o, float* dgates, void* stream) {
+  int s = check_rows(type, T, D);
+  if (s != FS_OK || T == 0) return s;
+  if (k < 1 || k > kMaxK || (long long)T * k > 0x7fffffffll) return report_error(FS_ERR_BAD_ARG, "k must be in [1, 32], T * k below 2^31");
+  if (!position || !pairs || !dy || !d_o || lddy < D || (dgates && (!o || !gates || ldo < D)))
+    return report_error(FS_ERR_BAD_ARG, "null argument, or rows shorter than D");
+  CombineArgs a{};
+  a.o = o; a.ldo = ldo; a.T = T; a.k = k; a.D = D; a.gates = gates; a.position = position; a.pairs = pairs;
+  a.dy = dy; a.lddy = lddy; a.d_o = d_o; a.dgates = dgates;
+  return launch_combine(a, type, true, lane_values(D, type_bytes(type), o ? ldo : 0, lddy, o, dy, d_o), static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

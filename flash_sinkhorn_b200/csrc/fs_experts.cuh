@@ -1,0 +1,67 @@
+// What the kernels of routed experts share (fs_experts.cu: routing, gated activation, sums back into tokens;
+// fs_group.cu: matrix products grouped by expert): loads and stores of 16- and 32-bit values, checks of the host side.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/flash_sinkhorn_b200.h"
+
+namespace fs {
+int report_error(int code, const char* msg);  // fs_api.cu: records the calling thread's error text
+void count_launches(int k);                   // fs_api.cu: adds to the count behind fs_launch_count()
+
+namespace ex {
+namespace {
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// N consecutive values as one load or store of up to 16 bytes each; the pointer is aligned to N values (at most 16 bytes).
+template <typename T, int N>
+struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Pack {
+  T v[N];
+};
+template <typename T, int N>
+__device__ __forceinline__ void load_f32(const T* p, float (&out)[N]) {
+  const Pack<T, N> q = *reinterpret_cast<const Pack<T, N>*>(p);
+#pragma unroll
+  for (int i = 0; i < N; ++i) out[i] = to_f32(q.v[i]);
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_f32(T* p, const float (&in)[N]) {
+  Pack<T, N> q;
+#pragma unroll
+  for (int i = 0; i < N; ++i) q.v[i] = from_f32<T>(in[i]);
+  *reinterpret_cast<Pack<T, N>*>(p) = q;
+}
+
+inline bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+inline int type_bytes(int type) { return type == FS_TYPE_F32 ? 4 : 2; }
+
+inline int check_device() {
+  const int arch = fs_device_arch();
+  if (arch < 0) return report_error(FS_ERR_CUDA, "cannot query the current CUDA device");
+  if (arch / 10 != 10) return report_error(FS_ERR_UNSUPPORTED, "this library is built for sm_100a only");
+  return FS_OK;
+}
+inline int launched(int kernels) {
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return report_error(FS_ERR_CUDA, cudaGetErrorString(e));
+  count_launches(kernels);
+  return FS_OK;
+}
+
+}  // namespace
+}  // namespace ex
+}  // namespace fs

@@ -473,6 +473,67 @@ int fs_plan_session_cg(const float* x, const float* y, int n, int m, int d,
                        float eps, float cost_scale, int max_iter, float rtol, float atol, int prec,
                        void* ws, size_t ws_bytes, void* stream);
 
+/* ---- Routed experts -------------------------------------------------------------------------------------
+ * No counterpart in the reference. T tokens go to k experts each; the T * k (token, slot) pairs that are routed are put
+ * in the order of their experts, pairs of one expert in their own order. With a routing
+ *   offsets [E + 1]   rows [offsets[e], offsets[e + 1]) belong to expert e; offsets[E] rows are routed
+ *   pairs   [T * k]   pair (t * k + slot) of each row, -1 for the rows after the last one that is routed
+ *   rows    [T * k]   its token t, or -1
+ *   position [T, k]   row of each pair, or -1
+ * Matrices are of one of the types below, rows `ld` values apart, columns adjacent. Sums are held in fp32 and rounded
+ * once. Nothing is allocated, nothing synchronises, and the results are the same in every run. */
+enum { FS_TYPE_F32 = 0, FS_TYPE_F16 = 1, FS_TYPE_BF16 = 2 };
+
+/* Scratch of fs_route (0: none). */
+size_t fs_route_bytes(int T, int E, int k);
+
+/* Chooses k <= 32 of E <= 1024 experts for every token: the largest logit + bias (bias may be null), ties to the lower
+ * expert, NaN first. An expert is off where its logit or bias is -inf, or mask[t] is 0 (mask may be null); slots without
+ * an expert have expert -1 and gate 0. gates [T, k]: soft-max of the logits over the chosen experts (over_all == 0) or
+ * over all that are on. */
+int fs_route(const void* logits, int type, long long ld, int T, int E, int k, const float* bias, const uint8_t* mask,
+             int over_all, float* gates, int* experts, int* offsets, int* pairs, int* rows, int* position, void* ws,
+             size_t ws_bytes, void* stream);
+
+/* Gradient of the gates to the logits: out [T, E], densely packed, from grad [T, k] and what fs_route gave. */
+int fs_route_grad(const void* logits, int type, long long ld, int T, int E, int k, const float* bias, const uint8_t* mask,
+                  int over_all, const float* gates, const int* experts, const float* grad, void* out, void* stream);
+
+/* Products grouped by expert: out[i, :] = W_e x[row(i), :] for the rows i of expert e, zeros for the rows of none. x has
+ * M rows of K values; row(i) = rows[i] (rows [R]) or i (rows null, M >= R; rows outside [0, M) count as zeros). W_e is
+ * N x K with element (n, k) at w[e * w_expert + n * w_row + k * w_col]; w_row or w_col is 1. out is R x N. FS_TYPE_F16
+ * and FS_TYPE_BF16. offsets that decrease or leave [0, R] are taken as their running maximum within it. */
+int fs_grouped_mm(const void* x, long long ldx, int M, const int* rows, int R, const void* w, long long w_expert,
+                  long long w_row, long long w_col, int E, int N, int K, const int* offsets, void* out, long long ldo,
+                  int type, void* stream);
+
+/* Its gradient to the weights: dw[e, n, k] = sum over the rows i of expert e of dy[dy_row(i), n] x[x_row(i), k], zeros for
+ * an expert without rows; dw is E x N x K, densely packed. */
+int fs_grouped_mm_wgrad(const void* dy, long long lddy, int M_dy, const int* dy_rows, const void* x, long long ldx, int M_x,
+                        const int* x_rows, int R, int E, int N, int K, const int* offsets, void* dw, int type,
+                        void* stream);
+
+/* Gated activation of R rows u = [g | v] of 2 F values: h = p g sigmoid(g) v, p = gates[pairs[i]] (1 without pairs; rows
+ * of no pair give zeros). codes [R, 2 F] and scales [R, 2 ceil(F / 32)] (or null) receive u in 8 bits: blocks of 32 along
+ * each half as integers times 2^(scale - 127), scale 255 for a block with an infinity or NaN. */
+int fs_gated_act(const void* u, int type, long long ldu, int R, int F, const float* gates, const int* pairs, void* h,
+                 int8_t* codes, uint8_t* scales, void* stream);
+
+/* Its gradients from codes and scales, or from u where codes is null: du [R, 2 F] densely packed, dgates (or null) one for
+ * each pair, and in h (or null) the activation recomputed from what the gradient used. */
+int fs_gated_act_grad(const void* u, long long ldu, const int8_t* codes, const uint8_t* scales, int type, int R, int F,
+                      const float* gates, const int* pairs, const int* position, const void* dh, long long lddh, void* du,
+                      float* dgates, void* h, void* stream);
+
+/* Rows back into tokens: y[t, :] = sum over the slots s with a row of gates[t, s] o[position[t, s], :] (gates null:
+ * weights of 1). o has T * k rows of D values, y is T x D, densely packed. */
+int fs_combine(const void* o, int type, long long ldo, int T, int k, int D, const float* gates, const int* position, void* y,
+               void* stream);
+
+/* Its gradients: d_o [T * k, D] densely packed, and dgates [T, k] (or null; then o may be null too). */
+int fs_combine_grad(const void* o, int type, long long ldo, int T, int k, int D, const float* gates, const int* position,
+                    const int* pairs, const void* dy, long long lddy, void* d_o, float* dgates, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
