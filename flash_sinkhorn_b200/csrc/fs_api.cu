@@ -527,6 +527,10 @@ namespace fs {
 int report_error(int code, const char* msg) { return fail(code, "%s", msg); }
 // Lets them add the kernels they enqueue themselves to the count behind fs_launch_count().
 void count_launches(int k) { g_launches.fetch_add(k, std::memory_order_relaxed); }
+namespace ex {  // fs_group.cu
+int group_error_flag();
+int clear_group_error_flag();
+}  // namespace ex
 }  // namespace fs
 
 using namespace fs;
@@ -538,13 +542,13 @@ int fs_version(void) { return 200; }  // 0.2.0
 long long fs_launch_count(void) { return g_launches.load(std::memory_order_relaxed); }
 
 int fs_device_error(void) {
-  const int a = tc::read_error_flag(), b = sym::read_error_flag();
-  return a < 0 || b < 0 ? -1 : (a | b);
+  const int a = tc::read_error_flag(), b = sym::read_error_flag(), c = ex::group_error_flag();
+  return a < 0 || b < 0 || c < 0 ? -1 : (a | b | c);
 }
 
 int fs_clear_device_error(void) {
-  const int a = tc::clear_error_flag(), b = sym::clear_error_flag();
-  return a ? a : b;
+  const int a = tc::clear_error_flag(), b = sym::clear_error_flag(), c = ex::clear_group_error_flag();
+  return a ? a : b ? b : c;
 }
 
 size_t fs_apply_mat_plan_bytes(int n, int m, int d, int dv, int prec) {

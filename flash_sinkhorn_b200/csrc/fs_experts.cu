@@ -589,7 +589,7 @@ struct CombineArgs {
   float* dgates;
 };
 
-template <typename T, int VEC>
+template <typename T, typename Y, int VEC>
 __global__ void __launch_bounds__(kActWarps * 32) combine_kernel(const CombineArgs a) {
   const int lane = threadIdx.x & 31, n = a.T * a.k;
   const int steps = (a.D + 32 * VEC - 1) / (32 * VEC), share = (steps + a.parts - 1) / a.parts;
@@ -615,7 +615,7 @@ __global__ void __launch_bounds__(kActWarps * 32) combine_kernel(const CombineAr
           for (int i = 0; i < VEC; ++i) y[i] += wj * o[i];
         }
       }
-      if (c < a.D) store_f32<T, VEC>(static_cast<T*>(a.y) + (long long)t * a.D + c, y);
+      if (c < a.D) store_f32<Y, VEC>(static_cast<Y*>(a.y) + (long long)t * a.D + c, y);
     }
   }
 }
@@ -660,23 +660,25 @@ __global__ void __launch_bounds__(kActWarps * 32) combine_grad_kernel(const Comb
   }
 }
 
-template <typename T, int VEC>
+template <typename T, typename Y, int VEC>
 int launch_combine(CombineArgs a, bool grad, cudaStream_t st) {
   a.parts = row_parts(a.T, a.D, VEC);
-  if (!grad) combine_kernel<T, VEC><<<row_blocks((long long)a.T * a.parts), kActWarps * 32, 0, st>>>(a);
+  if (!grad) combine_kernel<T, Y, VEC><<<row_blocks((long long)a.T * a.parts), kActWarps * 32, 0, st>>>(a);
   else combine_grad_kernel<T, VEC><<<row_blocks((long long)a.T * a.k), kActWarps * 32, 0, st>>>(a);
   return launched(1);
 }
-template <typename T>
+template <typename T, typename Y>
 int launch_combine(const CombineArgs& a, bool grad, int vec, cudaStream_t st) {
-  if (vec == 8) return launch_combine<T, 8>(a, grad, st);
-  if (vec == 4) return launch_combine<T, 4>(a, grad, st);
-  return launch_combine<T, 1>(a, grad, st);
+  if (vec == 8) return launch_combine<T, Y, 8>(a, grad, st);
+  if (vec == 4) return launch_combine<T, Y, 4>(a, grad, st);
+  return launch_combine<T, Y, 1>(a, grad, st);
 }
-int launch_combine(const CombineArgs& a, int type, bool grad, int vec, cudaStream_t st) {
-  if (type == FS_TYPE_F32) return launch_combine<float>(a, grad, vec, st);
-  if (type == FS_TYPE_F16) return launch_combine<__half>(a, grad, vec, st);
-  return launch_combine<__nv_bfloat16>(a, grad, vec, st);
+int launch_combine(const CombineArgs& a, int type, int y_type, bool grad, int vec, cudaStream_t st) {
+  if (type == FS_TYPE_F16) return launch_combine<__half, __half>(a, grad, vec, st);
+  if (type == FS_TYPE_BF16) return launch_combine<__nv_bfloat16, __nv_bfloat16>(a, grad, vec, st);
+  if (y_type == FS_TYPE_F16) return launch_combine<float, __half>(a, grad, vec, st);
+  if (y_type == FS_TYPE_BF16) return launch_combine<float, __nv_bfloat16>(a, grad, vec, st);
+  return launch_combine<float, float>(a, grad, vec, st);
 }
 
 int check_rows(int type, int rows, int width) {
@@ -763,14 +765,15 @@ int fs_gated_act_grad(const void* u, long long ldu, const int8_t* codes, const u
 }
 
 int fs_combine(const void* o, int type, long long ldo, int T, int k, int D, const float* gates, const int* position, void* y,
-               void* stream) {
+               int y_type, void* stream) {
   int s = check_rows(type, T, D);
   if (s != FS_OK || T == 0) return s;
   if (k < 1 || k > kMaxK || (long long)T * k > 0x7fffffffll) return report_error(FS_ERR_BAD_ARG, "k must be in [1, 32], T * k below 2^31");
-  if (!o || !position || !y || ldo < D) return report_error(FS_ERR_BAD_ARG, "null argument, or rows shorter than D");
+  if (!o || !position || !y || ldo < D || y_type < 0 || y_type > 2 || (y_type != type && type != FS_TYPE_F32))
+    return report_error(FS_ERR_BAD_ARG, "null argument, rows shorter than D, or a wrong type of the result");
   CombineArgs a{};
   a.o = o; a.ldo = ldo; a.T = T; a.k = k; a.D = D; a.gates = gates; a.position = position; a.y = y;
-  return launch_combine(a, type, false, lane_values(D, type_bytes(type), ldo, 0, o, y), static_cast<cudaStream_t>(stream));
+  return launch_combine(a, type, y_type, false, lane_values(D, type_bytes(type), ldo, 0, o, y), static_cast<cudaStream_t>(stream));
 }
 
 int fs_combine_grad(const void* o, int type, long long ldo, int T, int k, int D, const float* gates, const int* position,
@@ -783,7 +786,7 @@ int fs_combine_grad(const void* o, int type, long long ldo, int T, int k, int D,
   CombineArgs a{};
   a.o = o; a.ldo = ldo; a.T = T; a.k = k; a.D = D; a.gates = gates; a.position = position; a.pairs = pairs;
   a.dy = dy; a.lddy = lddy; a.d_o = d_o; a.dgates = dgates;
-  return launch_combine(a, type, true, lane_values(D, type_bytes(type), o ? ldo : 0, lddy, o, dy, d_o), static_cast<cudaStream_t>(stream));
+  return launch_combine(a, type, type, true, lane_values(D, type_bytes(type), o ? ldo : 0, lddy, o, dy, d_o), static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -1,120 +1,602 @@
-// Matrix products grouped by expert, with groups of any size.
+// Matrix products grouped by expert on the 5th-generation tensor cores, with groups of any size.
+//
+//   rows     out[i, n] = sum_k W_e[n, k] x[row(i), k]           (forward, and the gradient to x with W transposed)
+//   weights  dw_e[n, k] = sum_i dy[dy_row(i), n] x[x_row(i), k]  (i over the rows of expert e)
+//
+// In the rows form the FEATURES are the M side of the tensor-core instruction (128 lanes of TMEM per CTA) and the rows of a
+// group its N side: N goes in steps of 16 at run time, so the last, partial tile of a group costs what it holds, and a
+// group of one row costs 16 columns rather than 128. The rows of the next group that a tile load may bring along are other
+// columns of the accumulator; they are not written. In the weights form the rows are the contraction, so those of
+// another group must not be read: a block of 64 rows that a group ends in, and every block of gathered rows, comes by
+// loads of four rows each (tile::gather4) whose row numbers are set past the end of the tensor where there is no row -
+// such rows arrive as zeros, in both operands, so that no infinity of a neighbour meets a zero.
+//
+// One persistent CTA per SM, or a pair of CTAs on neighbouring SMs that share a 256 x 256 tile (each holds 128 features and
+// fetches half of the rows: two thirds of the bytes per product of 128 x 256 tiles). Warp 4 fetches (TMA into a ring of
+// stages of 64 contraction values), warp 5 issues the products into one of two TMEM accumulators, warps 0 to 3 write the
+// other one out. Group boundaries are read by the kernel itself; every CTA takes every n-th tile, features fastest, so that
+// the CTAs working at one time share a group's weights and rows in L2.
 #include "fs_experts.cuh"
+#include "fs_ptx.cuh"
+#include "fs_tc.cuh"
+
+#include <cudaTypedefs.h>
+
+#include <mutex>
 
 namespace fs {
 namespace ex {
 namespace {
 
-constexpr int kTile = 64, kDepth = 16;
+using namespace fs::tc;
+
+__device__ int g_group_error = 0;  // non-zero once a bounded wait gave up (read by fs_device_error)
+
+enum Form { ROWS_K, ROWS_MN, WEIGHTS };  // rows with W contiguous along the contraction; along the features
+
+constexpr int kThreads = 192;
+constexpr uint32_t kHalfTile = 64 * 128;  // 64 rows of 128 bytes
+constexpr int kMaxGroups = 1024;
 
 struct GroupArgs {
-  const void* x;  // forward: the rows; gradient to the weights: the rows that give the columns of dw
-  long long ldx;
-  int M;
-  const int* rows;
-  const void* y;  // gradient to the weights: the rows that give the rows of dw
-  long long ldy;
-  int My;
-  const int* yrows;
-  const void* w;
-  long long w_expert, w_row, w_col;
+  const int* offsets;
+  const int *arows, *brows;  // row numbers of the M and N operands (null: in order)
+  int Ma, Mb;                // rows of those operands
+  int R, E, N, K;
   void* out;
   long long ldo;
-  int R, E, N, K;
-  const int* offsets;
+  int type, out_type;  // FS_TYPE_*
+  int nstage;
 };
 
-// Group and first row of row tile `tile`; rows of no expert come last, as group E.
-__device__ bool find_tile(const GroupArgs& a, int tile, int& e, int& lo, int& hi) {
-  int end = 0;
-  for (e = 0; e <= a.E; ++e) {
-    const int begin = end;
-    end = e < a.E ? max(begin, min(a.offsets[e + 1], a.R)) : a.R;
-    const int tiles = (end - begin + kTile - 1) / kTile;
-    if (tile < tiles) {
-      lo = begin + tile * kTile;
-      hi = end;
-      return true;
+// ------------------------------------------------------------------ PTX of CTA pairs and gathered loads
+__device__ __forceinline__ uint32_t cta_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t in_leader(uint32_t addr) {  // the same shared-memory address in CTA 0 of the cluster
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool try_wait_cluster(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, 2000;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Bounded, as mbar_wait, for barriers that the other CTA of the pair arrives on.
+__device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  const long long t0 = clock64();
+  while (!try_wait_cluster(bar, parity)) {
+    if (*abort_flag) return false;
+    if (clock64() - t0 > kSpinLimit) {
+      *abort_flag = 1;
+      return false;
     }
-    tile -= tiles;
   }
-  return false;
+  return true;
 }
 
-template <typename T>
-__device__ __forceinline__ float row_value(const void* base, long long ld, int M, const int* rows, int i, int c, int width) {
-  const int r = rows ? rows[i] : i;
-  return r >= 0 && r < M && c < width ? to_f32(static_cast<const T*>(base)[(long long)r * ld + c]) : 0.f;
+template <int CG>
+__device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+  if (CG == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
+  else
+    tma_load_2d(dst, map, c0, c1, bar);
+}
+template <int CG>
+__device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+  if (CG == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void load_rows4(uint32_t dst, const CUtensorMap* map, int c0, const int (&r)[4], uint32_t bar) {
+  if (CG == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, "
+        "%4, %5, %6, %7}], [%2];"
+        ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, "
+        "%7}], [%2];"
+        ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if (CG == 2)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void commit(uint32_t bar) {  // arrives at this barrier of every CTA of the pair
+  if (CG == 2)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+        ::"r"(bar), "h"((uint16_t)3) : "memory");
+  else
+    umma_commit(bar);
+}
+template <int CG>
+__device__ __forceinline__ void alloc_columns(uint32_t slot, uint32_t n) {
+  if (CG == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(n) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    tmem_alloc(slot, n);
+    tmem_relinquish();
+  }
+}
+template <int CG>
+__device__ __forceinline__ void free_columns(uint32_t addr, uint32_t n) {
+  if (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(n) : "memory");
+  else tmem_dealloc(addr, n);
 }
 
-// 64 x 64 outputs per CTA, 4 x 4 per thread, fp32 throughout.
-template <typename T>
-__global__ void __launch_bounds__(256) group_rows_kernel(const GroupArgs a) {
-  __shared__ float xs[kDepth][kTile + 1], ws[kDepth][kTile + 1];
-  int e, lo, hi;
-  if (!find_tile(a, blockIdx.y, e, lo, hi)) return;
-  const int n0 = blockIdx.x * kTile, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float acc[4][4] = {};
-  if (e < a.E) {
-    const T* w = static_cast<const T*>(a.w) + e * a.w_expert;
-    for (int k0 = 0; k0 < a.K; k0 += kDepth) {
-      for (int i = threadIdx.x; i < kTile * kDepth; i += 256) {
-        const int r = i / kDepth, c = i % kDepth, k = k0 + c;
-        xs[c][r] = lo + r < hi ? row_value<T>(a.x, a.ldx, a.M, a.rows, lo + r, k, a.K) : 0.f;
-        ws[c][r] = n0 + r < a.N && k < a.K ? to_f32(w[(n0 + r) * a.w_row + k * a.w_col]) : 0.f;
+// Shared-memory operands, 128-byte swizzle. K-major: rows of 64 contraction values, groups of 8 rows 1024 bytes apart; a step
+// of 16 values is 32 bytes on. MN-major: 64 rows (contraction) of 64 features, the next 64 features one half tile on (the
+// leading offset), groups of 8 contraction rows 1024 bytes apart; a step of 16 contraction rows is 2048 bytes on.
+template <bool MN>
+__device__ __forceinline__ uint32_t operand_lo(uint32_t addr) {
+  return ((addr & 0x3FFFFu) >> 4) | ((MN ? kHalfTile >> 4 : 1u) << 16);
+}
+__host__ __device__ constexpr uint32_t step_of(bool mn) { return mn ? 2048u >> 4 : 32u >> 4; }
+
+// ------------------------------------------------------------------ tiles
+struct Tile {
+  int e, m0;     // expert, first feature
+  int lo, hi;    // rows form: rows of the tile; weights form: rows of the expert
+  int n0, cols;  // weights form: first column and columns; rows form: columns = rows
+  int blocks;    // of 64 contraction values
+};
+
+template <int FORM, int CG, int BN>
+struct Tiles {
+  const GroupArgs& a;
+  const int *gs, *ts;  // first row and first tile of every group
+  int mt, nt, e = 0;
+  __device__ Tiles(const GroupArgs& args, const int* rows, const int* tiles) : a(args), gs(rows), ts(tiles) {
+    mt = (a.N + 128 * CG - 1) / (128 * CG);
+    nt = (a.K + BN - 1) / BN;
+  }
+  __device__ int total() const { return FORM == WEIGHTS ? a.E * mt * nt : ts[a.E + 1]; }
+  __device__ Tile at(int tile) {  // in increasing order
+    Tile t;
+    if (FORM == WEIGHTS) {
+      t.e = tile / (mt * nt);
+      const int rest = tile - t.e * mt * nt, n = rest / mt;
+      t.m0 = (rest - n * mt) * 128 * CG;
+      t.n0 = n * BN;
+      t.cols = min(BN, a.K - t.n0);
+      t.lo = gs[t.e];
+      t.hi = gs[t.e + 1];
+      t.blocks = (t.hi - t.lo + 63) / 64;
+    } else {
+      while (tile >= ts[e + 1]) ++e;
+      const int rest = tile - ts[e], n = rest / mt;
+      t.e = e;
+      t.m0 = (rest - n * mt) * 128 * CG;
+      t.lo = gs[e] + n * BN;
+      t.hi = min(t.lo + BN, gs[e + 1]);
+      t.n0 = 0;
+      t.cols = t.hi - t.lo;
+      t.blocks = e < a.E ? (a.K + 63) / 64 : 0;  // group E: the rows of no expert
+    }
+    return t;
+  }
+};
+
+// First rows of the groups (running maximum of the offsets within [0, R]), of the rows of no expert (gs[E]) and the end
+// (gs[E + 1]); with TILES the number of tiles before each of them. One warp.
+template <bool TILES>
+__device__ void read_groups(const GroupArgs& a, int* gs, int* ts, int per_column, int bn) {
+  const int lane = threadIdx.x & 31;
+  int top = 0, sum = 0;
+  if (lane == 0) gs[0] = 0;
+  for (int c = 0; c <= a.E; c += 32) {
+    const int j = c + lane;
+    int end = j < a.E ? min(max(a.offsets[j + 1], 0), a.R) : a.R;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, end, o);
+      end = lane >= o ? max(end, v) : end;
+    }
+    end = max(end, top);
+    const int before = __shfl_up_sync(0xffffffffu, end, 1), begin = lane ? before : top;
+    if (j <= a.E) gs[j + 1] = end;
+    top = __shfl_sync(0xffffffffu, end, 31);
+    if (TILES) {
+      int n = j <= a.E ? (end - begin + bn - 1) / bn * per_column : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, n, o);
+        n += lane >= o ? v : 0;
       }
-      __syncthreads();
-      for (int c = 0; c < kDepth; ++c)
-        for (int i = 0; i < 4; ++i)
-          for (int j = 0; j < 4; ++j) acc[i][j] += xs[c][ty * 4 + i] * ws[c][tx * 4 + j];
-      __syncthreads();
+      if (j <= a.E) ts[j + 1] = sum + n;
+      sum += __shfl_sync(0xffffffffu, n, 31);
     }
   }
-  T* out = static_cast<T*>(a.out);
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j)
-      if (lo + ty * 4 + i < hi && n0 + tx * 4 + j < a.N)
-        out[(long long)(lo + ty * 4 + i) * a.ldo + n0 + tx * 4 + j] = from_f32<T>(acc[i][j]);
+  if (TILES && lane == 0) ts[0] = 0;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) group_weights_kernel(const GroupArgs a) {
-  __shared__ float ys[kDepth][kTile + 1], xs[kDepth][kTile + 1];
-  const int e = blockIdx.z, n0 = blockIdx.y * kTile, c0 = blockIdx.x * kTile, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  int lo = 0, hi = 0;
-  for (int g = 0; g <= e; ++g) {
-    lo = hi;
-    hi = max(lo, min(a.offsets[g + 1], a.R));
+__device__ __forceinline__ void store_one(void* out, long long at, float v, int type) {
+  if (type == FS_TYPE_BF16) static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
+  else if (type == FS_TYPE_F16) static_cast<__half*>(out)[at] = __float2half_rn(v);
+  else static_cast<float*>(out)[at] = v;
+}
+__device__ __forceinline__ uint32_t pack_two(float lo, float hi, int type) {
+  if (type == FS_TYPE_BF16) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&p);
   }
-  float acc[4][4] = {};
-  for (int r0 = lo; r0 < hi; r0 += kDepth) {
-    for (int i = threadIdx.x; i < kTile * kDepth; i += 256) {
-      const int r = i / kTile, c = i % kTile;
-      ys[r][c] = r0 + r < hi ? row_value<T>(a.y, a.ldy, a.My, a.yrows, r0 + r, n0 + c, a.N) : 0.f;
-      xs[r][c] = r0 + r < hi ? row_value<T>(a.x, a.ldx, a.M, a.rows, r0 + r, c0 + c, a.K) : 0.f;
+  const __half2 p = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+
+// Row numbers of four rows of an operand from row `i` on: past the end of the tensor (rows of zeros) where there is none.
+__device__ __forceinline__ void four_rows(const int* rows, int M, int i, int hi, int (&r)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    int v = i + j < hi ? (rows ? rows[i + j] : i + j) : M;
+    r[j] = v >= 0 && v < M ? v : M;
+  }
+}
+
+template <int FORM, int CG, int BN>
+__global__ void __launch_bounds__(kThreads, 1)
+group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapA4,
+             const __grid_constant__ CUtensorMap mapB, const __grid_constant__ CUtensorMap mapB4) {
+  constexpr int BNC = BN / CG;                         // columns whose operand this CTA fetches
+  constexpr uint32_t kA = 2 * kHalfTile, kB = BNC * 128, kStage = kA + kB;
+  constexpr bool A_MN = FORM != ROWS_K, B_MN = FORM == WEIGHTS;
+  constexpr uint32_t kColumns = 2 * BN;
+  static_assert(kColumns >= 32 && kColumns <= 512 && kStage % 1024 == 0, "tile");
+  extern __shared__ uint8_t raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + (size_t)a.nstage * kStage);
+  const int FULL = 0, EMPTY = a.nstage, ACC_FULL = 2 * a.nstage, ACC_EMPTY = ACC_FULL + 2, DRAIN = ACC_EMPTY + 2;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(bars + DRAIN + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(slot + 1);
+  int *gs = reinterpret_cast<int*>(slot + 2), *ts = gs + a.E + 2;
+  auto bar = [&](int i) { return smem_u32(bars + i); };
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = CG == 2 ? (int)cta_rank() : 0;
+  const int first = blockIdx.x / CG, stride = gridDim.x / CG;
+
+  if (warp == 0) {
+    read_groups<FORM != WEIGHTS>(a, gs, ts, (a.N + 128 * CG - 1) / (128 * CG), BN);
+  } else if (warp == 4 && lane == 0) {
+    for (int s = 0; s < a.nstage; ++s) {
+      mbar_init(bar(FULL + s), 1);
+      mbar_init(bar(EMPTY + s), 1);
     }
-    __syncthreads();
-    for (int r = 0; r < kDepth; ++r)
-      for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) acc[i][j] += ys[r][ty * 4 + i] * xs[r][tx * 4 + j];
-    __syncthreads();
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(ACC_FULL + i), 1);
+      mbar_init(bar(ACC_EMPTY + i), 4 * CG);  // one arrive per epilogue warp of the pair
+    }
+    mbar_init(bar(DRAIN), 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  } else if (warp == 5) {
+    alloc_columns<CG>(smem_u32(slot), kColumns);
   }
-  T* out = static_cast<T*>(a.out) + (long long)e * a.N * a.K;
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j)
-      if (n0 + ty * 4 + i < a.N && c0 + tx * 4 + j < a.K)
-        out[(long long)(n0 + ty * 4 + i) * a.K + c0 + tx * 4 + j] = from_f32<T>(acc[i][j]);
+  tc_fence_before();
+  __syncthreads();
+  if (CG == 2) cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem = *slot;
+  Tiles<FORM, CG, BN> tiles(a, gs, ts);
+  const int total = tiles.total();
+
+  if (warp == 4) {
+    // ===================== loads =====================
+    int s = 0, issued = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (int it = first; ok && it < total; it += stride) {
+      const Tile t = tiles.at(it);
+      const int np = (t.cols + 16 * CG - 1) / (16 * CG) * (16 * CG), npc = np / CG;  // columns of the product, of this CTA
+      const int m0 = t.m0 + rank * 128, r0 = t.lo + rank * npc;
+      int rb[4];
+      const bool gathered = FORM != WEIGHTS && a.brows && t.blocks;
+      if (gathered) four_rows(a.brows, a.Mb, r0 + 4 * lane, t.hi, rb);
+      for (int kb = 0; kb < t.blocks; ++kb) {
+        if (!__all_sync(0xffffffffu, mbar_wait(bar(EMPTY + s), ph ^ 1, abort_flag, 2000))) {
+          ok = false;
+          break;
+        }
+        const uint32_t full = CG == 2 ? in_leader(bar(FULL + s)) : bar(FULL + s);
+        const uint32_t dst = smem_u32(ring + (size_t)s * kStage);
+        if (FORM == WEIGHTS) {
+          const int i0 = t.lo + kb * 64;
+          const bool part = i0 + 64 > t.hi;  // other rows follow
+          if (lane == 0 && rank == 0) mbar_expect_tx(bar(FULL + s), CG * kStage);
+          __syncwarp();
+          if (a.arows || part) {
+            int r[4];
+            four_rows(a.arows, a.Ma, i0 + 4 * (lane & 15), t.hi, r);
+            load_rows4<CG>(dst + (lane >> 4) * kHalfTile + (lane & 15) * 512, &mapA4, m0 + (lane >> 4) * 64, r, full);
+          } else if (lane < 2) {
+            load_2d<CG>(dst + lane * kHalfTile, &mapA, m0 + lane * 64, i0, full);
+          }
+          const int n0 = t.n0 + rank * npc;
+          if (a.brows || part) {
+            int r[4];
+            four_rows(a.brows, a.Mb, i0 + 4 * (lane & 15), t.hi, r);
+#pragma unroll
+            for (int c = 0; c < BNC / 64; c += 2)
+              if (c + (lane >> 4) < BNC / 64)
+                load_rows4<CG>(dst + kA + (c + (lane >> 4)) * kHalfTile + (lane & 15) * 512, &mapB4, n0 + (c + (lane >> 4)) * 64, r, full);
+          } else if (lane < BNC / 64) {
+            load_2d<CG>(dst + kA + lane * kHalfTile, &mapB, n0 + lane * 64, i0, full);
+          }
+        } else {
+          if (lane == 0) {
+            if (rank == 0) mbar_expect_tx(bar(FULL + s), CG * kA + (gathered ? np * 128 : CG * kB));
+            if (FORM == ROWS_K) {
+              load_3d<CG>(dst, &mapA, kb * 64, m0, t.e, full);
+            } else {
+              load_3d<CG>(dst, &mapA, m0, kb * 64, t.e, full);
+              load_3d<CG>(dst + kHalfTile, &mapA, m0 + 64, kb * 64, t.e, full);
+            }
+            if (!gathered) load_2d<CG>(dst + kA, &mapB, kb * 64, r0, full);
+          }
+          __syncwarp();
+          if (gathered && 4 * lane < npc) load_rows4<CG>(dst + kA + lane * 512, &mapB4, kb * 64, rb, full);
+        }
+        __syncwarp();
+        ++issued;
+        if (++s == a.nstage) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+    }
+    // let the copies in flight land (in CTA 0 also the other one's; it stays until the pair has met)
+    if (*abort_flag && lane == 0 && rank == 0)
+      for (int j = issued > a.nstage ? issued - a.nstage : 0; j < issued; ++j)
+        mbar_wait_quiet(bar(FULL + j % a.nstage), (j / a.nstage) & 1);
+  } else if (warp == 5) {
+    // ===================== products =====================
+    if (rank == 0) {
+      const uint32_t type = a.type == FS_TYPE_BF16 ? 1u : 0u;
+      const uint32_t idesc0 = (1u << 4) | (type << 7) | (type << 10) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) |
+                              ((uint32_t)(128 * CG >> 4) << 24);
+      int s = 0, n = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int it = first; ok && it < total; it += stride) {
+        const Tile t = tiles.at(it);
+        if (t.blocks == 0) continue;
+        const int np = (t.cols + 16 * CG - 1) / (16 * CG) * (16 * CG);
+        const uint32_t idesc = idesc0 | ((uint32_t)(np >> 3) << 17);
+        const int buf = n & 1;
+        if (!__all_sync(0xffffffffu, wait_cluster(bar(ACC_EMPTY + buf), ((n >> 1) & 1) ^ 1, abort_flag))) break;
+        ++n;
+        tc_fence_after();
+        const uint32_t d = tmem + buf * BN;
+        for (int kb = 0; kb < t.blocks; ++kb) {
+          if (!__all_sync(0xffffffffu, wait_cluster(bar(FULL + s), ph, abort_flag))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t base = smem_u32(ring + (size_t)s * kStage);
+          const uint32_t al = operand_lo<A_MN>(base), bl = operand_lo<B_MN>(base + kA);
+          const int left = FORM == WEIGHTS ? t.hi - t.lo - kb * 64 : a.K - kb * 64;  // contraction values from here on
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+            if (ks * 16 < left && elect_one())
+              mma_f16<CG>(d, pack_desc(al + ks * step_of(A_MN), kDescHi128), pack_desc(bl + ks * step_of(B_MN), kDescHi128), idesc,
+                          kb | ks);
+          if (elect_one()) commit<CG>(bar(EMPTY + s));
+          __syncwarp();
+          if (++s == a.nstage) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+        if (!ok) break;
+        if (elect_one()) commit<CG>(bar(ACC_FULL + buf));
+        __syncwarp();
+      }
+      if (*abort_flag && elect_one()) {  // every product issued here ends before TMEM is freed
+        commit<CG>(bar(DRAIN));
+        mbar_wait_quiet(bar(DRAIN), 0);
+      }
+    }
+  } else {
+    // ===================== results =====================
+    const int q = warp;  // quarter of the TMEM lanes that this warp may read
+    int n = 0;
+    for (int it = first; it < total; it += stride) {
+      const Tile t = tiles.at(it);
+      const int f = t.m0 + rank * 128 + q * 32 + lane;  // this thread's feature
+      const int buf = n & 1;
+      if (t.blocks) {
+        if (!__all_sync(0xffffffffu, wait_cluster(bar(ACC_FULL + buf), (n >> 1) & 1, abort_flag))) break;
+        ++n;
+        tc_fence_after();
+      }
+      for (int c = 0; c < t.cols; c += 32) {
+        float v[32];
+        if (t.blocks) {
+          tmem_ld32(tmem + buf * BN + c + ((uint32_t)(q * 32) << 16), v);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = 0.f;
+        }
+        if (FORM == WEIGHTS) {
+          if (f < a.N) {
+            const long long at = ((long long)t.e * a.N + f) * a.K + t.n0 + c;
+            if (a.K % 8 == 0) {
+              uint4* p = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + at);
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (c + 8 * j < t.cols)
+                  p[j] = make_uint4(pack_two(v[8 * j], v[8 * j + 1], a.out_type), pack_two(v[8 * j + 2], v[8 * j + 3], a.out_type),
+                                    pack_two(v[8 * j + 4], v[8 * j + 5], a.out_type), pack_two(v[8 * j + 6], v[8 * j + 7], a.out_type));
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (c + j < t.cols) store_one(a.out, at + j, v[j], a.out_type);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (c + j < t.cols && f < a.N) store_one(a.out, (long long)(t.lo + c + j) * a.ldo + f, v[j], a.out_type);
+        }
+      }
+      if (t.blocks) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (CG == 2) arrive_cluster(in_leader(bar(ACC_EMPTY + buf)));
+          else mbar_arrive(bar(ACC_EMPTY + buf));
+        }
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (CG == 2) cluster_sync_all();
+  tc_fence_after();
+  if (warp == 5) free_columns<CG>(tmem, kColumns);
+  if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_group_error, 1);
+}
+
+// ------------------------------------------------------------------ host side
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* sym = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &found) == cudaSuccess &&
+        found == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(sym);
+  });
+  return fn;
+}
+
+// 16-bit tensor of 2 or 3 dimensions, contiguous along the first; boxes of 64 x box_rows.
+bool encode(CUtensorMap* map, int type, const void* base, int dims, const long long (&size)[3], const long long (&stride)[2],
+            int box_rows) {
+  const cuuint64_t sizes[3] = {(cuuint64_t)size[0], (cuuint64_t)size[1], (cuuint64_t)size[2]};
+  const cuuint64_t strides[2] = {(cuuint64_t)stride[0] * 2, (cuuint64_t)stride[1] * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1}, ones[3] = {1, 1, 1};
+  const auto fn = encoder();
+  return fn && fn(map, type == FS_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, dims,
+                  const_cast<void*>(base), sizes, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+bool encode_rows(CUtensorMap* map, int type, const void* base, long long cols, long long rows, long long ld, int box_rows) {
+  return encode(map, type, base, 2, {cols, rows, 1}, {ld, 0}, box_rows);
+}
+
+int no_map() { return report_error(FS_ERR_CUDA, "cuTensorMapEncodeTiled failed"); }
+
+template <int FORM, int CG, int BN>
+int launch_group(GroupArgs a, const CUtensorMap (&maps)[4], long long most_tiles, cudaStream_t st) {
+  constexpr size_t kStage = 2 * kHalfTile + BN / CG * 128;
+  const size_t fixed = 1024 + 8 * (2 * 12 + 5) + 8 + 8 * ((size_t)a.E + 2);
+  a.nstage = (int)((kSmemMax - fixed) / kStage);
+  if (a.nstage > 12) a.nstage = 12;
+  size_t smem = fixed + a.nstage * kStage;
+  if (smem < (size_t)kSmemMin) smem = kSmemMin;
+  const auto kernel = group_kernel<FORM, CG, BN>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return report_error(FS_ERR_CUDA, cudaGetErrorString(e));
+  if (most_tiles > 0x3fffffffll) return report_error(FS_ERR_UNSUPPORTED, "more than 2^30 tiles");
+  long long grid = detail::free_ctas() / CG;
+  if (grid > most_tiles) grid = most_tiles;
+  if (grid < 1) grid = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)grid * CG);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = CG;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kernel, a, maps[0], maps[1], maps[2], maps[3]);
+  if (e != cudaSuccess) return report_error(FS_ERR_CUDA, cudaGetErrorString(e));
+  count_launches(1);
+  return FS_OK;
+}
+
+template <int CG, int BN>
+int launch_rows(const GroupArgs& a, bool k_major, CUtensorMap (&maps)[4], const void* x, long long ldx, cudaStream_t st) {
+  if (!encode_rows(&maps[2], a.type, x, a.K, a.Mb, ldx, BN / CG)) return no_map();
+  const long long tiles = (long long)((a.R + BN - 1) / BN + a.E + 1) * ((a.N + 128 * CG - 1) / (128 * CG));
+  return k_major ? launch_group<ROWS_K, CG, BN>(a, maps, tiles, st) : launch_group<ROWS_MN, CG, BN>(a, maps, tiles, st);
 }
 
 int check_group(int type, int R, int E, int N, int K, const int* offsets) {
   if (type != FS_TYPE_F16 && type != FS_TYPE_BF16) return report_error(FS_ERR_BAD_ARG, "type must be FS_TYPE_F16 or FS_TYPE_BF16");
-  if (R < 0 || E < 1 || E > 1024 || N < 1 || K < 1 || N > (1 << 22) || K > (1 << 22))
+  if (R < 0 || E < 1 || E > kMaxGroups || N < 1 || K < 1 || N > (1 << 22) || K > (1 << 22))
     return report_error(FS_ERR_BAD_ARG, "R must be >= 0, E in [1, 1024], N and K in [1, 2^22]");
   if (!offsets) return report_error(FS_ERR_BAD_ARG, "null argument");
+  // A thread that has launched nothing yet (autograd's) has no current context, which the encoding of tensor maps needs;
+  // setting the device that is current binds it.
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess)
+    return report_error(FS_ERR_CUDA, "cannot make the current CUDA device's context current");
   return check_device();
+}
+// What tensor loads ask of an operand.
+bool loadable(const void* p, long long ld) { return aligned(p, 16) && ld % 8 == 0; }
+int not_loadable() {
+  return report_error(FS_ERR_BAD_ARG, "operands must be aligned to 16 bytes, their rows and experts multiples of 8 values apart");
 }
 
 }  // namespace
+
+int group_error_flag() {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_group_error, sizeof(int)) != cudaSuccess) return -1;
+  return v ? 1 : 0;
+}
+int clear_group_error_flag() {
+  const int zero = 0;
+  return cudaMemcpyToSymbol(g_group_error, &zero, sizeof(int)) == cudaSuccess ? 0 : -1;
+}
+
 }  // namespace ex
 }  // namespace fs
 
@@ -124,19 +606,30 @@ using namespace fs::ex;
 extern "C" {
 
 int fs_grouped_mm(const void* x, long long ldx, int M, const int* rows, int R, const void* w, long long w_expert,
-                  long long w_row, long long w_col, int E, int N, int K, const int* offsets, void* out, long long ldo,
-                  int type, void* stream) {
+                  long long w_row, long long w_col, int E, int N, int K, const int* offsets, void* out, int out_type,
+                  long long ldo, int type, void* stream) {
   int s = check_group(type, R, E, N, K, offsets);
   if (s != FS_OK || R == 0) return s;
-  if (!x || !w || !out || ldx < K || ldo < N || M < 0 || (!rows && M < R)) return report_error(FS_ERR_BAD_ARG, "null argument, or too few rows or columns");
+  if (!x || !w || !out || ldx < K || ldo < N || M < 1 || (!rows && M < R) || (out_type != type && out_type != FS_TYPE_F32))
+    return report_error(FS_ERR_BAD_ARG, "null argument, too few rows or columns, or a wrong type of the result");
+  const bool k_major = w_col == 1;
+  const long long w_ld = k_major ? w_row : w_col;
+  if (!k_major && w_row != 1) return report_error(FS_ERR_BAD_ARG, "w_row or w_col must be 1");
+  if (w_ld < (k_major ? K : N) || w_expert < 0 || (w_expert == 0 && E > 1))
+    return report_error(FS_ERR_BAD_ARG, "rows or experts of w overlap");
+  if (!loadable(x, ldx) || !loadable(w, w_ld) || w_expert % 8) return not_loadable();
   GroupArgs a{};
-  a.x = x; a.ldx = ldx; a.M = M; a.rows = rows; a.R = R; a.w = w; a.w_expert = w_expert; a.w_row = w_row; a.w_col = w_col;
-  a.E = E; a.N = N; a.K = K; a.offsets = offsets; a.out = out; a.ldo = ldo;
-  const dim3 grid((N + kTile - 1) / kTile, (R + kTile - 1) / kTile + E + 1);
+  a.offsets = offsets; a.brows = rows; a.Mb = M; a.R = R; a.E = E; a.N = N; a.K = K;
+  a.out = out; a.ldo = ldo; a.type = type; a.out_type = out_type;
+  CUtensorMap maps[4] = {};
+  if (!encode(&maps[0], type, w, 3, {k_major ? K : N, k_major ? N : K, E}, {w_ld, w_expert ? w_expert : w_ld}, k_major ? 128 : 64))
+    return no_map();
+  if (!encode_rows(&maps[3], type, x, K, M, ldx, 1)) return no_map();
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (type == FS_TYPE_F16) group_rows_kernel<__half><<<grid, 256, 0, st>>>(a);
-  else group_rows_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a);
-  return launched(1);
+  const int mean = R / E;
+  if (mean >= 96 && N > 128) return launch_rows<2, 256>(a, k_major, maps, x, ldx, st);
+  if (mean >= 48) return launch_rows<1, 128>(a, k_major, maps, x, ldx, st);
+  return launch_rows<1, 32>(a, k_major, maps, x, ldx, st);
 }
 
 int fs_grouped_mm_wgrad(const void* dy, long long lddy, int M_dy, const int* dy_rows, const void* x, long long ldx, int M_x,
@@ -144,16 +637,23 @@ int fs_grouped_mm_wgrad(const void* dy, long long lddy, int M_dy, const int* dy_
                         void* stream) {
   int s = check_group(type, R, E, N, K, offsets);
   if (s != FS_OK) return s;
-  if (!dw || (R > 0 && (!dy || !x)) || lddy < N || ldx < K || M_dy < 0 || M_x < 0 || (!dy_rows && M_dy < R) || (!x_rows && M_x < R))
+  if (!dw || (R > 0 && (!dy || !x || M_dy < 1 || M_x < 1)) || lddy < N || ldx < K || (!dy_rows && M_dy < R) || (!x_rows && M_x < R))
     return report_error(FS_ERR_BAD_ARG, "null argument, or too few rows or columns");
-  GroupArgs a{};
-  a.y = dy; a.ldy = lddy; a.My = M_dy; a.yrows = dy_rows; a.x = x; a.ldx = ldx; a.M = M_x; a.rows = x_rows;
-  a.R = R; a.E = E; a.N = N; a.K = K; a.offsets = offsets; a.out = dw;
-  const dim3 grid((K + kTile - 1) / kTile, (N + kTile - 1) / kTile, E);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (type == FS_TYPE_F16) group_weights_kernel<__half><<<grid, 256, 0, st>>>(a);
-  else group_weights_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a);
-  return launched(1);
+  if (R == 0) {
+    const cudaError_t e = cudaMemsetAsync(dw, 0, (size_t)E * N * K * 2, st);
+    return e == cudaSuccess ? FS_OK : report_error(FS_ERR_CUDA, cudaGetErrorString(e));
+  }
+  if (!loadable(dy, lddy) || !loadable(x, ldx) || (K % 8 == 0 && !aligned(dw, 16))) return not_loadable();
+  GroupArgs a{};
+  a.offsets = offsets; a.arows = dy_rows; a.Ma = M_dy; a.brows = x_rows; a.Mb = M_x; a.R = R; a.E = E; a.N = N; a.K = K;
+  a.out = dw; a.type = a.out_type = type;
+  CUtensorMap maps[4] = {};
+  if (!encode_rows(&maps[0], type, dy, N, M_dy, lddy, 64) || !encode_rows(&maps[1], type, dy, N, M_dy, lddy, 1) ||
+      !encode_rows(&maps[2], type, x, K, M_x, ldx, 64) || !encode_rows(&maps[3], type, x, K, M_x, ldx, 1))
+    return no_map();
+  if (N > 128 && K > 128) return launch_group<WEIGHTS, 2, 256>(a, maps, (long long)E * ((N + 255) / 256) * ((K + 255) / 256), st);
+  return launch_group<WEIGHTS, 1, 128>(a, maps, (long long)E * ((N + 127) / 128) * ((K + 127) / 128), st);
 }
 
 }  // extern "C"

@@ -162,29 +162,44 @@ def route_tokens(logits: torch.Tensor, k: int, *, bias: Optional[torch.Tensor] =
 # ---------------------------------------------------------------------------------------------------------------
 
 
-def _weights_of(w: torch.Tensor) -> torch.Tensor:
-    """``w [E, N, K]`` itself where one of its two matrix dimensions is contiguous, else a copy."""
-    _, n, k = w.shape
+def _loadable_rows(t: torch.Tensor) -> torch.Tensor:
+    """``t [R, C]`` as the tensor loads of the products take it: rows a multiple of 16 bytes apart, the first one aligned to
+    16 bytes; ``t`` itself, or a copy with padded rows."""
+    if t.stride(1) == 1 and t.stride(0) >= t.shape[1] and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t
+    r, c = t.shape
+    out = torch.empty((r, -(-c // 8) * 8), dtype=t.dtype, device=t.device)[:, :c]
+    return out.copy_(t)
+
+
+def _loadable_weights(w: torch.Tensor) -> torch.Tensor:
+    """``w [E, N, K]`` itself where one of its two matrix dimensions is contiguous and the other strides are multiples of 16
+    bytes, else a copy. Weights whose last dimension is a multiple of 8 are never copied."""
+    e, n, k = w.shape
     se, sn, sk = w.stride()
-    if (sk == 1 and sn >= k or sn == 1 and sk >= n) and se >= 0:
-        return w
-    return w.contiguous()
+    if w.data_ptr() % 16 == 0 and se % 8 == 0 and (se > 0 or e == 1):
+        if sk == 1 and sn >= k and sn % 8 == 0 or sn == 1 and sk >= n and sk % 8 == 0:
+            return w
+    out = torch.empty((e, n, -(-k // 8) * 8), dtype=w.dtype, device=w.device)[:, :, :k]
+    return out.copy_(w)
 
 
-def _mm(x, rows, count, w, offsets, transposed=False):
+def _mm(x, rows, count, w, offsets, transposed=False, dtype=None):
     """``[count, N]``: rows of x (through ``rows``, if given) times their expert's matrix, or its transpose."""
     dev, (e, n, k) = x.device, w.shape
+    x, w = _loadable_rows(x), _loadable_weights(w)
     strides = w.stride()
     if transposed:
         n, k, strides = k, n, (strides[0], strides[2], strides[1])
-    out = torch.empty((count, n), dtype=x.dtype, device=dev)
+    out = torch.empty((count, n), dtype=dtype or x.dtype, device=dev)
     _lib.call("fs_grouped_mm", dev, _lib.ptr(x), _ld(x), x.shape[0], _lib.ptr(rows), count, _lib.ptr(w), *strides, e, n, k,
-              _lib.ptr(offsets), _lib.ptr(out), n, _TYPES[x.dtype], _lib.stream_ptr(dev))
+              _lib.ptr(offsets), _lib.ptr(out), _TYPES[out.dtype], n, _TYPES[x.dtype], _lib.stream_ptr(dev))
     return out
 
 
 def _wgrad(dy, dy_rows, x, x_rows, count, offsets):
     dev, e = x.device, offsets.shape[0] - 1
+    dy, x = _loadable_rows(dy), _loadable_rows(x)
     out = torch.empty((e, dy.shape[1], x.shape[1]), dtype=x.dtype, device=dev)
     _lib.call("fs_grouped_mm_wgrad", dev, _lib.ptr(dy), _ld(dy), dy.shape[0], _lib.ptr(dy_rows), _lib.ptr(x), _ld(x),
               x.shape[0], _lib.ptr(x_rows), count, e, dy.shape[1], x.shape[1], _lib.ptr(offsets), _lib.ptr(out),
@@ -203,12 +218,14 @@ class _GroupedMmFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         x, w, offsets, rows, position = ctx.saved_tensors
-        dy = _rows_of(dy)
+        dy = _loadable_rows(dy)
         dx = dw = None
         if ctx.needs_input_grad[0]:
-            dx = _mm(dy, None, ctx.count, w, offsets, transposed=True)
-            if rows is not None:
-                dx = _combine(dx, None, position)
+            if rows is None:
+                dx = _mm(dy, None, ctx.count, w, offsets, transposed=True)
+            else:  # rows in fp32, so that the sum over a token's rows is rounded once
+                dx = _mm(dy, None, ctx.count, w, offsets, transposed=True, dtype=torch.float32)
+                dx = _combine(dx, None, position, x.dtype)
         if ctx.needs_input_grad[1]:
             dw = _wgrad(dy, None, x, rows, ctx.count, offsets)
         return dx, dw, None, None, None, None
@@ -222,8 +239,8 @@ def grouped_mm(x: torch.Tensor, weight: torch.Tensor, groups: Union[Routing, tor
     ``offsets[e + 1]``; any sizes, zero among them). ``weight [E, N, K]`` as a linear layer holds it, or the transposed
     view of ``[E, K, N]``. ``x [R, K]`` in the order of the groups; with ``gather`` (and a routing) ``x [T, K]`` is in the
     order of the tokens and row ``i`` reads token ``routing.rows[i]``, without a copy. fp16 or bf16, both the same; sums in
-    fp32, one rounding. Differentiable in both: the gradient of a gathered token is the sum over its rows (each rounded
-    to the type, the sum in fp32).
+    fp32, one rounding. Differentiable in both. Operands that tensor loads do not take (16 bytes of alignment, rows and
+    experts a multiple of 8 values apart) are copied in every call: keep weights padded to a multiple of 8.
     """
     if x.ndim != 2 or weight.ndim != 3:
         raise ValueError(f"x must be 2D and weight 3D [E, N, K], got shapes {tuple(x.shape)} and {tuple(weight.shape)}")
@@ -250,7 +267,7 @@ def grouped_mm(x: torch.Tensor, weight: torch.Tensor, groups: Union[Routing, tor
         raise ValueError(f"x must have {want} rows, got {x.shape[0]}")
     if offsets.shape[0] != e + 1 or e > MAX_EXPERTS:
         raise ValueError(f"groups must have as many experts as weight ({e}, at most {MAX_EXPERTS}), got {offsets.shape[0] - 1}")
-    x, weight = _rows_of(x), _weights_of(weight)
+    x, weight = _loadable_rows(x), _loadable_weights(weight)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         return _GroupedMmFunction.apply(x, weight, offsets, rows, position, count)
     return _mm(x, rows, count, weight, offsets)
@@ -329,11 +346,11 @@ def gated_act(u: torch.Tensor, routing: Optional[Routing] = None, *, checkpoint:
 # ---------------------------------------------------------------------------------------------------------------
 
 
-def _combine(o, gates, position):
+def _combine(o, gates, position, dtype=None):
     dev, (t, k), d = o.device, position.shape, o.shape[1]
-    y = torch.empty((t, d), dtype=o.dtype, device=dev)
+    y = torch.empty((t, d), dtype=dtype or o.dtype, device=dev)
     _lib.call("fs_combine", dev, _lib.ptr(o), _TYPES[o.dtype], _ld(o), t, k, d, _lib.ptr(gates), _lib.ptr(position),
-              _lib.ptr(y), _lib.stream_ptr(dev))
+              _lib.ptr(y), _TYPES[y.dtype], _lib.stream_ptr(dev))
     return y
 
 
@@ -400,7 +417,7 @@ class _ExpertMlpFunction(torch.autograd.Function):
     def backward(ctx, dy):
         x, w_in, w_out, gates, offsets, pairs, rows, position, u, codes, scales = ctx.saved_tensors
         need_x, need_in, need_out, need_gates = ctx.needs_input_grad[:4]
-        dy, count = _rows_of(dy), pairs.shape[0]
+        dy, count = _loadable_rows(dy), pairs.shape[0]
         dh = _mm(dy, rows, count, w_out, offsets, transposed=True)
         du, dgates, h = _act_grad(u, codes, scales, gates, pairs, position, dh, need_gates, need_out)
         dx = _combine(_mm(du, None, count, w_in, offsets, transposed=True), None, position) if need_x else None
@@ -430,7 +447,7 @@ def expert_mlp(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, routing
         raise ValueError(f"w_in must be [E, 2 F, {d}] and w_out [E, {d}, F], got {tuple(w_in.shape)} and {tuple(w_out.shape)}")
     if routing.position.shape[0] != t or routing.offsets.shape[0] != e + 1 or routing.position.shape[1] > MAX_K:
         raise ValueError(f"routing must be of {t} tokens and {e} experts, at most {MAX_K} for a token")
-    x, w_in, w_out = _rows_of(x), _weights_of(w_in), _weights_of(w_out)
+    x, w_in, w_out = _loadable_rows(x), _loadable_weights(w_in), _loadable_weights(w_out)
     r = routing
     if torch.is_grad_enabled() and any(v.requires_grad for v in (x, w_in, w_out, r.gates)):
         return _ExpertMlpFunction.apply(x, w_in, w_out, r.gates, r.offsets, r.pairs, r.rows, r.position, bool(checkpoint))

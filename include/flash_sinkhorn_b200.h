@@ -500,15 +500,17 @@ int fs_route_grad(const void* logits, int type, long long ld, int T, int E, int 
                   int over_all, const float* gates, const int* experts, const float* grad, void* out, void* stream);
 
 /* Products grouped by expert: out[i, :] = W_e x[row(i), :] for the rows i of expert e, zeros for the rows of none. x has
- * M rows of K values; row(i) = rows[i] (rows [R]) or i (rows null, M >= R; rows outside [0, M) count as zeros). W_e is
- * N x K with element (n, k) at w[e * w_expert + n * w_row + k * w_col]; w_row or w_col is 1. out is R x N. FS_TYPE_F16
- * and FS_TYPE_BF16. offsets that decrease or leave [0, R] are taken as their running maximum within it. */
+ * M >= 1 rows of K values; row(i) = rows[i] (rows [R]; numbers outside [0, M) are rows of zeros) or i (rows null, M >= R).
+ * W_e is N x K with element (n, k) at w[e * w_expert + n * w_row + k * w_col]; w_row or w_col is 1. out is R x N, of the type
+ * of x and w (FS_TYPE_F16 or FS_TYPE_BF16) or FS_TYPE_F32. x and w are aligned to 16 bytes, ldx, w_expert and the other
+ * stride of w multiples of 8. offsets[0] is taken as 0; offsets that decrease or leave [0, R] are taken as their running
+ * maximum within it. E <= 1024. */
 int fs_grouped_mm(const void* x, long long ldx, int M, const int* rows, int R, const void* w, long long w_expert,
-                  long long w_row, long long w_col, int E, int N, int K, const int* offsets, void* out, long long ldo,
-                  int type, void* stream);
+                  long long w_row, long long w_col, int E, int N, int K, const int* offsets, void* out, int out_type,
+                  long long ldo, int type, void* stream);
 
 /* Its gradient to the weights: dw[e, n, k] = sum over the rows i of expert e of dy[dy_row(i), n] x[x_row(i), k], zeros for
- * an expert without rows; dw is E x N x K, densely packed. */
+ * an expert without rows; dw is E x N x K, densely packed. dy and x aligned and strided as x above, dw to 16 bytes. */
 int fs_grouped_mm_wgrad(const void* dy, long long lddy, int M_dy, const int* dy_rows, const void* x, long long ldx, int M_x,
                         const int* x_rows, int R, int E, int N, int K, const int* offsets, void* dw, int type,
                         void* stream);
@@ -526,9 +528,10 @@ int fs_gated_act_grad(const void* u, long long ldu, const int8_t* codes, const u
                       float* dgates, void* h, void* stream);
 
 /* Rows back into tokens: y[t, :] = sum over the slots s with a row of gates[t, s] o[position[t, s], :] (gates null:
- * weights of 1). o has T * k rows of D values, y is T x D, densely packed. */
+ * weights of 1). o has T * k rows of D values, y is T x D, densely packed, of the type of o or, where that is FS_TYPE_F32,
+ * of any. */
 int fs_combine(const void* o, int type, long long ldo, int T, int k, int D, const float* gates, const int* position, void* y,
-               void* stream);
+               int y_type, void* stream);
 
 /* Its gradients: d_o [T * k, D] densely packed, and dgates [T, k] (or null; then o may be null too). */
 int fs_combine_grad(const void* o, int type, long long ldo, int T, int k, int D, const float* gates, const int* position,

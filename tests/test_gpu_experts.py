@@ -294,14 +294,14 @@ def test_grouped_mm_of_gathered_rows(ex, k, n, tokens, slots, e, dtype):
     check_mm(ex, dyt, w.transpose(1, 2), routing.offsets, routing.rows)
     check_wgrad(ex, dyt, routing.rows, normal(g, r, k, dtype=dtype), None, r, routing.offsets)
 
-    # through the public call: the gradient of a token is the sum over its rows, each rounded once
+    # through the public call: the gradient of a token is the sum over its rows in fp32, rounded once
     xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
     y = ex.grouped_mm(xl, wl, routing, gather=True)
     dx, dw = torch.autograd.grad(y, (xl, wl), dy)
     assert torch.equal(y, ex._mm(x, routing.rows, r, w, routing.offsets))
     assert torch.equal(dw, ex._wgrad(dy, None, x, routing.rows, r, routing.offsets))
     pos = routing.position.long()
-    part = ex._mm(dy, None, r, w, routing.offsets, transposed=True).double()[pos.clamp_min(0)] * (pos >= 0)[..., None]
+    part = ex._mm(dy, None, r, w, routing.offsets, transposed=True, dtype=FP32).double()[pos.clamp_min(0)] * (pos >= 0)[..., None]
     within(dx, part.sum(1), ULP[dtype] * part.sum(1).abs() + ACC * part.abs().sum(1) + TINY[dtype])
 
 
