@@ -7,15 +7,16 @@
 // group its N side: N goes in steps of 16 at run time, so the last, partial tile of a group costs what it holds, and a
 // group of one row costs 16 columns rather than 128. The rows of the next group that a tile load may bring along are other
 // columns of the accumulator; they are not written. In the weights form the rows are the contraction, so those of
-// another group must not be read: a block of 64 rows that a group ends in, and every block of gathered rows, comes by
-// loads of four rows each (tile::gather4) whose row numbers are set past the end of the tensor where there is no row -
-// such rows arrive as zeros, in both operands, so that no infinity of a neighbour meets a zero.
+// another group must not be read: the block of 64 rows that a group ends in is filled up with zeros, in both operands, so
+// that no infinity of a neighbour meets a zero.
 //
 // One persistent CTA per SM, or a pair of CTAs on neighbouring SMs that share a 256 x 256 tile (each holds 128 features and
-// fetches half of the rows: two thirds of the bytes per product of 128 x 256 tiles). Warp 4 fetches (TMA into a ring of
-// stages of 64 contraction values), warp 5 issues the products into one of two TMEM accumulators, warps 0 to 3 write the
-// other one out. Group boundaries are read by the kernel itself; every CTA takes every n-th tile, features fastest, so that
-// the CTAs working at one time share a group's weights and rows in L2.
+// fetches half of the rows: two thirds of the bytes per product of 128 x 256 tiles). Warp 4 fetches whole tiles (TMA into a
+// ring of stages of 64 contraction values), warp 5 issues the products into one of two TMEM accumulators, warps 0 to 3
+// write the other one out. Rows in another order and blocks that end inside are fetched by warps 6 to 9, 16 bytes a lane
+// (cp.async; a lane keeps four stages in flight): TMA's loads of four rows each took 75 clocks apiece, 2.6 times the time
+// of the whole product. Group boundaries are read by the kernel itself; every CTA takes every n-th tile, features fastest,
+// so that the CTAs working at one time share a group's weights and rows in L2.
 #include "fs_experts.cuh"
 #include "fs_ptx.cuh"
 #include "fs_tc.cuh"
@@ -34,7 +35,7 @@ __device__ int g_group_error = 0;  // non-zero once a bounded wait gave up (read
 
 enum Form { ROWS_K, ROWS_MN, WEIGHTS };  // rows with W contiguous along the contraction; along the features
 
-constexpr int kThreads = 192;
+constexpr int kCopyWarps = 4, kCopyDepth = 4;  // warps that fetch single rows; stages that each has in flight
 constexpr uint32_t kHalfTile = 64 * 128;  // 64 rows of 128 bytes
 constexpr int kMaxGroups = 1024;
 
@@ -46,7 +47,11 @@ struct GroupArgs {
   void* out;
   long long ldo;
   int type, out_type;  // FS_TYPE_*
+  int out_vec;         // values of a store: 8, 2 or 1
   int nstage;
+  // operands as plain memory, for rows that are fetched one by one
+  const void *aptr, *bptr;
+  long long lda, ldb;
 };
 
 // ------------------------------------------------------------------ PTX of CTA pairs and gathered loads
@@ -64,32 +69,8 @@ __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ bool try_wait_cluster(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, 2000;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// Bounded, as mbar_wait, for barriers that the other CTA of the pair arrives on.
-__device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-  const long long t0 = clock64();
-  while (!try_wait_cluster(bar, parity)) {
-    if (*abort_flag) return false;
-    if (clock64() - t0 > kSpinLimit) {
-      *abort_flag = 1;
-      return false;
-    }
-  }
-  return true;
-}
-
 template <int CG>
 __device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
   if (CG == 2)
@@ -110,19 +91,16 @@ __device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, in
         "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
         ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
 }
-template <int CG>
-__device__ __forceinline__ void load_rows4(uint32_t dst, const CUtensorMap* map, int c0, const int (&r)[4], uint32_t bar) {
-  if (CG == 2)
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, "
-        "%4, %5, %6, %7}], [%2];"
-        ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
-  else
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, "
-        "%7}], [%2];"
-        ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+__device__ __forceinline__ void expect_cluster(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
+// 16 bytes, of which those past the first `valid` become zeros (the source is not read for them).
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 template <int CG>
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   if (CG == 2)
@@ -247,11 +225,6 @@ __device__ void read_groups(const GroupArgs& a, int* gs, int* ts, int per_column
   if (TILES && lane == 0) ts[0] = 0;
 }
 
-__device__ __forceinline__ void store_one(void* out, long long at, float v, int type) {
-  if (type == FS_TYPE_BF16) static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
-  else if (type == FS_TYPE_F16) static_cast<__half*>(out)[at] = __float2half_rn(v);
-  else static_cast<float*>(out)[at] = v;
-}
 __device__ __forceinline__ uint32_t pack_two(float lo, float hi, int type) {
   if (type == FS_TYPE_BF16) {
     const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
@@ -261,27 +234,96 @@ __device__ __forceinline__ uint32_t pack_two(float lo, float hi, int type) {
   return *reinterpret_cast<const uint32_t*>(&p);
 }
 
-// Row numbers of four rows of an operand from row `i` on: past the end of the tensor (rows of zeros) where there is none.
-__device__ __forceinline__ void four_rows(const int* rows, int M, int i, int hi, int (&r)[4]) {
+// 32 lanes x 32 columns of an accumulator as 16-bit values into a warp's staging tile of 32 rows of 64 bytes, whose 16-byte
+// chunks are exchanged so that neither side meets bank conflicts. FLIP: rows are columns of the accumulator.
+__device__ __forceinline__ uint32_t staged(uint32_t base, int row, int chunk) {
+  return base + row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
+}
+template <bool FLIP>
+__device__ __forceinline__ void stage_block(uint32_t tmem, uint32_t base, int lane, int type) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    int v = i + j < hi ? (rows ? rows[i + j] : i + j) : M;
-    r[j] = v >= 0 && v < M ? v : M;
+  for (int h = 0; h < 2; ++h) {  // 16 lanes of TMEM at a time
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(tmem + ((uint32_t)(16 * h) << 16))
+        : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+    // a lane holds columns 8 i + 2 (lane % 4) and the next one of rows lane / 4 (g = 0) and lane / 4 + 8 (g = 1)
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      uint32_t m[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        m[i] = pack_two(__uint_as_float(r[4 * i + 2 * g]), __uint_as_float(r[4 * i + 2 * g + 1]), type);
+      if (FLIP)
+        asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(staged(base, lane, 2 * h + g)),
+                     "r"(m[0]), "r"(m[1]), "r"(m[2]), "r"(m[3])
+                     : "memory");
+      else
+        asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};"
+                     ::"r"(staged(base, 16 * h + 8 * g + (lane & 7), lane >> 3)), "r"(m[0]), "r"(m[1]), "r"(m[2]), "r"(m[3])
+                     : "memory");
+    }
+  }
+}
+// rows x cols values (at most 32 x 32) of the staging tile, or zeros, to out, rows ld values apart.
+__device__ __forceinline__ void write_block(uint16_t* out, long long ld, int rows, int cols, int vec, bool zero, uint32_t base, int lane) {
+  if (vec == 8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 8 * i + (lane >> 2), c = lane & 3;
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (!zero) asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(staged(base, r, c)));
+      if (r < rows && 8 * c < cols) *reinterpret_cast<uint4*>(out + r * ld + 8 * c) = v;
+    }
+  } else if (vec == 2) {
+#pragma unroll 4
+    for (int i = 0; i < 16; ++i) {
+      const int r = 2 * i + (lane >> 4), c = 2 * (lane & 15);
+      uint32_t v = 0u;
+      if (!zero) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(staged(base, r, c >> 3) + (c & 7) * 2));
+      if (r < rows && c < cols) *reinterpret_cast<uint32_t*>(out + r * ld + c) = v;
+    }
+  } else {
+#pragma unroll 4
+    for (int r = 0; r < 32; ++r) {
+      uint16_t v = 0;
+      if (!zero) asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(staged(base, r, lane >> 3) + (lane & 7) * 2));
+      if (r < rows && lane < cols) out[r * ld + lane] = v;
+    }
   }
 }
 
-template <int FORM, int CG, int BN>
-__global__ void __launch_bounds__(kThreads, 1)
-group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapA4,
-             const __grid_constant__ CUtensorMap mapB, const __grid_constant__ CUtensorMap mapB4) {
+// One lane's part of an operand block that comes row by row: 16-byte chunk `chunk` of row i of the operand (through `rows`, if
+// given; zeros where i is not below hi or the number is not that of a row), its first value being column c of `width`.
+__device__ __forceinline__ void copy_chunk(uint32_t dst, const void* base, long long ld, const int* rows, int M, int i, int hi, int c,
+                                           int width) {
+  int r = i < hi ? (rows ? __ldg(rows + i) : i) : -1;
+  int valid = r >= 0 && r < M ? (width - c) * 2 : 0;
+  valid = min(max(valid, 0), 16);
+  copy16(dst, static_cast<const uint16_t*>(base) + (valid ? r * ld + c : 0), valid);
+}
+
+// COPY: rows of the N operand come one by one (rows form); the weights form always has warps for that.
+template <int FORM, int CG, int BN, bool COPY>
+__global__ void __launch_bounds__(COPY ? 192 + 32 * kCopyWarps : 192, 1)
+group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB) {
   constexpr int BNC = BN / CG;                         // columns whose operand this CTA fetches
   constexpr uint32_t kA = 2 * kHalfTile, kB = BNC * 128, kStage = kA + kB;
   constexpr bool A_MN = FORM != ROWS_K, B_MN = FORM == WEIGHTS;
   constexpr uint32_t kColumns = 2 * BN;
-  static_assert(kColumns >= 32 && kColumns <= 512 && kStage % 1024 == 0, "tile");
+  static_assert(kColumns >= 32 && kColumns <= 512 && kStage % 1024 == 0 && (COPY || FORM != WEIGHTS), "tile");
   extern __shared__ uint8_t raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + (size_t)a.nstage * kStage);
+  uint8_t* staging = ring + (size_t)a.nstage * kStage;  // 2 KB for each of warps 0 to 3
+  uint64_t* bars = reinterpret_cast<uint64_t*>(staging + 8192);
   const int FULL = 0, EMPTY = a.nstage, ACC_FULL = 2 * a.nstage, ACC_EMPTY = ACC_FULL + 2, DRAIN = ACC_EMPTY + 2;
   uint32_t* slot = reinterpret_cast<uint32_t*>(bars + DRAIN + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(slot + 1);
@@ -296,12 +338,12 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
     read_groups<FORM != WEIGHTS>(a, gs, ts, (a.N + 128 * CG - 1) / (128 * CG), BN);
   } else if (warp == 4 && lane == 0) {
     for (int s = 0; s < a.nstage; ++s) {
-      mbar_init(bar(FULL + s), 1);
+      mbar_init(bar(FULL + s), CG * (COPY ? 1 + kCopyWarps : 1));  // in CTA 0: every fetching warp of the pair
       mbar_init(bar(EMPTY + s), 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar(ACC_FULL + i), 1);
-      mbar_init(bar(ACC_EMPTY + i), 4 * CG);  // one arrive per epilogue warp of the pair
+      mbar_init(bar(ACC_EMPTY + i), 4 * CG);  // in CTA 0: every warp of the pair that writes results
     }
     mbar_init(bar(DRAIN), 1);
     *abort_flag = 0;
@@ -317,75 +359,57 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
   const uint32_t tmem = *slot;
   Tiles<FORM, CG, BN> tiles(a, gs, ts);
   const int total = tiles.total();
+  auto full_bar = [&](int s) { return CG == 2 ? in_leader(bar(FULL + s)) : bar(FULL + s); };
 
   if (warp == 4) {
-    // ===================== loads =====================
+    // ===================== whole tiles =====================
     int s = 0, issued = 0;
     uint32_t ph = 0;
     bool ok = true;
-    for (int it = first; ok && it < total; it += stride) {
-      const Tile t = tiles.at(it);
-      const int np = (t.cols + 16 * CG - 1) / (16 * CG) * (16 * CG), npc = np / CG;  // columns of the product, of this CTA
-      const int m0 = t.m0 + rank * 128, r0 = t.lo + rank * npc;
-      int rb[4];
-      const bool gathered = FORM != WEIGHTS && a.brows && t.blocks;
-      if (gathered) four_rows(a.brows, a.Mb, r0 + 4 * lane, t.hi, rb);
-      for (int kb = 0; kb < t.blocks; ++kb) {
-        if (!__all_sync(0xffffffffu, mbar_wait(bar(EMPTY + s), ph ^ 1, abort_flag, 2000))) {
-          ok = false;
-          break;
-        }
-        const uint32_t full = CG == 2 ? in_leader(bar(FULL + s)) : bar(FULL + s);
-        const uint32_t dst = smem_u32(ring + (size_t)s * kStage);
-        if (FORM == WEIGHTS) {
+    if (lane == 0) {
+      for (int it = first; ok && it < total; it += stride) {
+        const Tile t = tiles.at(it);
+        const int npc = (t.cols + 16 * CG - 1) / (16 * CG) * 16;  // columns of the product that this CTA fetches
+        const int m0 = t.m0 + rank * 128;
+        for (int kb = 0; kb < t.blocks; ++kb) {
+          if (!mbar_wait(bar(EMPTY + s), ph ^ 1, abort_flag, 2000)) {
+            ok = false;
+            break;
+          }
+          const uint32_t full = full_bar(s), dst = smem_u32(ring + (size_t)s * kStage);
           const int i0 = t.lo + kb * 64;
-          const bool part = i0 + 64 > t.hi;  // other rows follow
-          if (lane == 0 && rank == 0) mbar_expect_tx(bar(FULL + s), CG * kStage);
-          __syncwarp();
-          if (a.arows || part) {
-            int r[4];
-            four_rows(a.arows, a.Ma, i0 + 4 * (lane & 15), t.hi, r);
-            load_rows4<CG>(dst + (lane >> 4) * kHalfTile + (lane & 15) * 512, &mapA4, m0 + (lane >> 4) * 64, r, full);
-          } else if (lane < 2) {
-            load_2d<CG>(dst + lane * kHalfTile, &mapA, m0 + lane * 64, i0, full);
+          const bool part = FORM == WEIGHTS && i0 + 64 > t.hi;  // rows of another group follow
+          const bool load_a = !(FORM == WEIGHTS && (a.arows || part)), load_b = !(COPY && (FORM != WEIGHTS || a.brows || part));
+          expect_cluster(full, (load_a ? kA : 0u) + (load_b ? kB : 0u));
+          if (FORM == ROWS_K) {
+            load_3d<CG>(dst, &mapA, kb * 64, m0, t.e, full);
+          } else if (FORM == ROWS_MN) {
+            load_3d<CG>(dst, &mapA, m0, kb * 64, t.e, full);
+            load_3d<CG>(dst + kHalfTile, &mapA, m0 + 64, kb * 64, t.e, full);
+          } else if (load_a) {
+            load_2d<CG>(dst, &mapA, m0, i0, full);
+            load_2d<CG>(dst + kHalfTile, &mapA, m0 + 64, i0, full);
           }
-          const int n0 = t.n0 + rank * npc;
-          if (a.brows || part) {
-            int r[4];
-            four_rows(a.brows, a.Mb, i0 + 4 * (lane & 15), t.hi, r);
+          if (load_b) {
+            if (FORM == WEIGHTS) {
 #pragma unroll
-            for (int c = 0; c < BNC / 64; c += 2)
-              if (c + (lane >> 4) < BNC / 64)
-                load_rows4<CG>(dst + kA + (c + (lane >> 4)) * kHalfTile + (lane & 15) * 512, &mapB4, n0 + (c + (lane >> 4)) * 64, r, full);
-          } else if (lane < BNC / 64) {
-            load_2d<CG>(dst + kA + lane * kHalfTile, &mapB, n0 + lane * 64, i0, full);
-          }
-        } else {
-          if (lane == 0) {
-            if (rank == 0) mbar_expect_tx(bar(FULL + s), CG * kA + (gathered ? np * 128 : CG * kB));
-            if (FORM == ROWS_K) {
-              load_3d<CG>(dst, &mapA, kb * 64, m0, t.e, full);
+              for (int c = 0; c < BNC / 64; ++c) load_2d<CG>(dst + kA + c * kHalfTile, &mapB, t.n0 + rank * npc + c * 64, i0, full);
             } else {
-              load_3d<CG>(dst, &mapA, m0, kb * 64, t.e, full);
-              load_3d<CG>(dst + kHalfTile, &mapA, m0 + 64, kb * 64, t.e, full);
+              load_2d<CG>(dst + kA, &mapB, kb * 64, t.lo + rank * npc, full);
             }
-            if (!gathered) load_2d<CG>(dst + kA, &mapB, kb * 64, r0, full);
           }
-          __syncwarp();
-          if (gathered && 4 * lane < npc) load_rows4<CG>(dst + kA + lane * 512, &mapB4, kb * 64, rb, full);
-        }
-        __syncwarp();
-        ++issued;
-        if (++s == a.nstage) {
-          s = 0;
-          ph ^= 1;
+          ++issued;
+          if (++s == a.nstage) {
+            s = 0;
+            ph ^= 1;
+          }
         }
       }
+      // let the copies in flight land (in CTA 0 also the other one's; it stays until the pair has met)
+      if (*abort_flag && rank == 0)
+        for (int j = issued > a.nstage ? issued - a.nstage : 0; j < issued; ++j)
+          mbar_wait_quiet(bar(FULL + j % a.nstage), (j / a.nstage) & 1);
     }
-    // let the copies in flight land (in CTA 0 also the other one's; it stays until the pair has met)
-    if (*abort_flag && lane == 0 && rank == 0)
-      for (int j = issued > a.nstage ? issued - a.nstage : 0; j < issued; ++j)
-        mbar_wait_quiet(bar(FULL + j % a.nstage), (j / a.nstage) & 1);
   } else if (warp == 5) {
     // ===================== products =====================
     if (rank == 0) {
@@ -401,12 +425,12 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
         const int np = (t.cols + 16 * CG - 1) / (16 * CG) * (16 * CG);
         const uint32_t idesc = idesc0 | ((uint32_t)(np >> 3) << 17);
         const int buf = n & 1;
-        if (!__all_sync(0xffffffffu, wait_cluster(bar(ACC_EMPTY + buf), ((n >> 1) & 1) ^ 1, abort_flag))) break;
+        if (!__all_sync(0xffffffffu, mbar_wait(bar(ACC_EMPTY + buf), ((n >> 1) & 1) ^ 1, abort_flag, 2000))) break;
         ++n;
         tc_fence_after();
         const uint32_t d = tmem + buf * BN;
         for (int kb = 0; kb < t.blocks; ++kb) {
-          if (!__all_sync(0xffffffffu, wait_cluster(bar(FULL + s), ph, abort_flag))) {
+          if (!__all_sync(0xffffffffu, mbar_wait(bar(FULL + s), ph, abort_flag, 2000))) {
             ok = false;
             break;
           }
@@ -435,50 +459,48 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
         mbar_wait_quiet(bar(DRAIN), 0);
       }
     }
-  } else {
+  } else if (warp < 4) {
     // ===================== results =====================
     const int q = warp;  // quarter of the TMEM lanes that this warp may read
+    const uint32_t stage = smem_u32(staging + 2048 * q);
     int n = 0;
     for (int it = first; it < total; it += stride) {
       const Tile t = tiles.at(it);
-      const int f = t.m0 + rank * 128 + q * 32 + lane;  // this thread's feature
+      const int f = t.m0 + rank * 128 + q * 32;  // first of this warp's features
       const int buf = n & 1;
-      if (t.blocks) {
-        if (!__all_sync(0xffffffffu, wait_cluster(bar(ACC_FULL + buf), (n >> 1) & 1, abort_flag))) break;
+      const bool zero = t.blocks == 0;
+      if (!zero) {
+        if (!__all_sync(0xffffffffu, mbar_wait(bar(ACC_FULL + buf), (n >> 1) & 1, abort_flag, 2000))) break;
         ++n;
         tc_fence_after();
       }
-      for (int c = 0; c < t.cols; c += 32) {
-        float v[32];
-        if (t.blocks) {
-          tmem_ld32(tmem + buf * BN + c + ((uint32_t)(q * 32) << 16), v);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = 0.f;
-        }
-        if (FORM == WEIGHTS) {
-          if (f < a.N) {
-            const long long at = ((long long)t.e * a.N + f) * a.K + t.n0 + c;
-            if (a.K % 8 == 0) {
-              uint4* p = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + at);
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (c + 8 * j < t.cols)
-                  p[j] = make_uint4(pack_two(v[8 * j], v[8 * j + 1], a.out_type), pack_two(v[8 * j + 2], v[8 * j + 3], a.out_type),
-                                    pack_two(v[8 * j + 4], v[8 * j + 5], a.out_type), pack_two(v[8 * j + 6], v[8 * j + 7], a.out_type));
-            } else {
+      const uint32_t acc = tmem + buf * BN + ((uint32_t)(q * 32) << 16);
+      if (f < a.N) {
+        for (int c = 0; c < t.cols; c += 32) {
+          if (FORM != WEIGHTS && a.out_type == FS_TYPE_F32) {
+            float v[32];
+            if (!zero) tmem_ld32(acc + c, v);
+            float* p = static_cast<float*>(a.out) + (long long)(t.lo + c) * a.ldo + f + lane;
+            if (f + lane < a.N) {
 #pragma unroll
               for (int j = 0; j < 32; ++j)
-                if (c + j < t.cols) store_one(a.out, at + j, v[j], a.out_type);
+                if (c + j < t.cols) p[j * a.ldo] = zero ? 0.f : v[j];
             }
+            continue;
           }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (c + j < t.cols && f < a.N) store_one(a.out, (long long)(t.lo + c + j) * a.ldo + f, v[j], a.out_type);
+          if (!zero) {
+            stage_block<FORM != WEIGHTS>(acc + c, stage, lane, a.out_type);
+            __syncwarp();
+          }
+          uint16_t* out = static_cast<uint16_t*>(a.out);
+          if (FORM == WEIGHTS)
+            write_block(out + ((long long)t.e * a.N + f) * a.K + t.n0 + c, a.K, a.N - f, t.cols - c, a.out_vec, zero, stage, lane);
+          else
+            write_block(out + (long long)(t.lo + c) * a.ldo + f, a.ldo, t.cols - c, a.N - f, a.out_vec, zero, stage, lane);
+          __syncwarp();
         }
       }
-      if (t.blocks) {
+      if (!zero) {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
@@ -487,6 +509,78 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
         }
       }
     }
+  } else if (COPY) {
+    // ===================== single rows =====================
+    // Chunk ch of rows r, r + 16, ... of every half tile (64 rows of 128 bytes, chunk exchanged with its row as the 128-byte
+    // swizzle has it). A stage is reported full when the copies of kCopyDepth - 1 stages later are under way; at once if
+    // nothing of it is copied here.
+    const int id = threadIdx.x - 192, r = id >> 3, ch = id & 7;
+    const uint32_t at = r * 128 + ((ch ^ (r & 7)) << 4);  // 16 rows on: 2048 bytes
+    int s = 0;
+    uint32_t ph = 0, copied = 0;  // bit i: the stage i before the last one has copies that are not reported
+    bool ok = true;
+    auto report = [&](int stage, bool copies) {
+      if (copies) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) arrive_cluster(full_bar(stage));
+    };
+    auto stage_before = [&](int n) { return s >= n ? s - n : s - n + a.nstage; };
+    for (int it = first; ok && it < total; it += stride) {
+      const Tile t = tiles.at(it);
+      const int npc = (t.cols + 16 * CG - 1) / (16 * CG) * 16, m0 = t.m0 + rank * 128;
+      const uint16_t* src[8];
+      if (FORM != WEIGHTS && t.blocks) {
+#pragma unroll
+        for (int j = 0; j < BNC / 16; ++j) {
+          const int i = t.lo + rank * npc + r + 16 * j, v = i < t.hi && r + 16 * j < npc ? __ldg(a.brows + i) : -1;
+          src[j] = v >= 0 && v < a.Mb ? static_cast<const uint16_t*>(a.bptr) + v * a.ldb + ch * 8 : nullptr;
+        }
+      }
+      for (int kb = 0; kb < t.blocks; ++kb) {
+        if (!__all_sync(0xffffffffu, mbar_wait(bar(EMPTY + s), ph ^ 1, abort_flag, 2000))) {
+          ok = false;
+          break;
+        }
+        const uint32_t dst = smem_u32(ring + (size_t)s * kStage) + at;
+        bool copies = true;
+        if (FORM == WEIGHTS) {
+          const int i0 = t.lo + kb * 64;
+          const bool part = i0 + 64 > t.hi;
+          copies = part || a.arows || a.brows;
+          if (a.arows || part) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              copy_chunk(dst + j * 2048, a.aptr, a.lda, a.arows, a.Ma, i0 + r + 16 * (j & 3), t.hi, m0 + (j >> 2) * 64 + ch * 8, a.N);
+          }
+          if (a.brows || part) {
+#pragma unroll
+            for (int j = 0; j < BNC / 16; ++j)
+              copy_chunk(dst + kA + j * 2048, a.bptr, a.ldb, a.brows, a.Mb, i0 + r + 16 * (j & 3), t.hi,
+                         t.n0 + rank * npc + (j >> 2) * 64 + ch * 8, a.K);
+          }
+        } else {
+          const int valid = min(max((a.K - kb * 64 - ch * 8) * 2, 0), 16);
+#pragma unroll
+          for (int j = 0; j < BNC / 16; ++j)
+            copy16(dst + kA + j * 2048, src[j] && valid ? src[j] + kb * 64 : a.bptr, src[j] ? valid : 0);
+        }
+        copy_commit();
+        copied = copied << 1 | (copies ? 1u : 0u);
+        if (!copies) report(s, false);
+        if (copied >> (kCopyDepth - 1) & 1u) {
+          copy_wait<kCopyDepth - 1>();
+          report(stage_before(kCopyDepth - 1), true);
+        }
+        if (++s == a.nstage) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+    }
+    copy_wait<0>();
+    if (ok)
+      for (int i = kCopyDepth - 2; i >= 0; --i)
+        if (copied >> i & 1u) report(stage_before(i + 1), true);  // s is one past the last stage here
   }
   __syncwarp();
   tc_fence_before();
@@ -528,15 +622,16 @@ bool encode_rows(CUtensorMap* map, int type, const void* base, long long cols, l
 
 int no_map() { return report_error(FS_ERR_CUDA, "cuTensorMapEncodeTiled failed"); }
 
-template <int FORM, int CG, int BN>
-int launch_group(GroupArgs a, const CUtensorMap (&maps)[4], long long most_tiles, cudaStream_t st) {
+template <int FORM, int CG, int BN, bool COPY>
+int launch_group(GroupArgs a, const CUtensorMap& mapA, const CUtensorMap& mapB, long long most_tiles, cudaStream_t st) {
   constexpr size_t kStage = 2 * kHalfTile + BN / CG * 128;
-  const size_t fixed = 1024 + 8 * (2 * 12 + 5) + 8 + 8 * ((size_t)a.E + 2);
+  const size_t fixed = 1024 + 8192 + 8 * (2 * 12 + 5) + 8 + 8 * ((size_t)a.E + 2);
   a.nstage = (int)((kSmemMax - fixed) / kStage);
+  static_assert((kSmemMax - 1024 - 8192 - 248 - 8 * (kMaxGroups + 2)) / kStage > kCopyDepth, "stages");
   if (a.nstage > 12) a.nstage = 12;
   size_t smem = fixed + a.nstage * kStage;
   if (smem < (size_t)kSmemMin) smem = kSmemMin;
-  const auto kernel = group_kernel<FORM, CG, BN>;
+  const auto kernel = group_kernel<FORM, CG, BN, COPY>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return report_error(FS_ERR_CUDA, cudaGetErrorString(e));
   if (most_tiles > 0x3fffffffll) return report_error(FS_ERR_UNSUPPORTED, "more than 2^30 tiles");
@@ -545,7 +640,7 @@ int launch_group(GroupArgs a, const CUtensorMap (&maps)[4], long long most_tiles
   if (grid < 1) grid = 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)grid * CG);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(COPY ? 192 + 32 * kCopyWarps : 192);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr{};
@@ -554,17 +649,26 @@ int launch_group(GroupArgs a, const CUtensorMap (&maps)[4], long long most_tiles
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kernel, a, maps[0], maps[1], maps[2], maps[3]);
+  e = cudaLaunchKernelEx(&cfg, kernel, a, mapA, mapB);
   if (e != cudaSuccess) return report_error(FS_ERR_CUDA, cudaGetErrorString(e));
   count_launches(1);
   return FS_OK;
 }
 
 template <int CG, int BN>
-int launch_rows(const GroupArgs& a, bool k_major, CUtensorMap (&maps)[4], const void* x, long long ldx, cudaStream_t st) {
-  if (!encode_rows(&maps[2], a.type, x, a.K, a.Mb, ldx, BN / CG)) return no_map();
-  const long long tiles = (long long)((a.R + BN - 1) / BN + a.E + 1) * ((a.N + 128 * CG - 1) / (128 * CG));
-  return k_major ? launch_group<ROWS_K, CG, BN>(a, maps, tiles, st) : launch_group<ROWS_MN, CG, BN>(a, maps, tiles, st);
+int launch_rows(const GroupArgs& a, bool k_major, const CUtensorMap& mapA, cudaStream_t st) {
+  CUtensorMap mapB = {};
+  if (!a.brows && !encode_rows(&mapB, a.type, a.bptr, a.K, a.Mb, a.ldb, BN / CG)) return no_map();
+  const long long tiles = ((a.R + BN - 1ll) / BN + a.E + 1) * ((a.N + 128 * CG - 1) / (128 * CG));
+  if (a.brows)
+    return k_major ? launch_group<ROWS_K, CG, BN, true>(a, mapA, mapB, tiles, st) : launch_group<ROWS_MN, CG, BN, true>(a, mapA, mapB, tiles, st);
+  return k_major ? launch_group<ROWS_K, CG, BN, false>(a, mapA, mapB, tiles, st) : launch_group<ROWS_MN, CG, BN, false>(a, mapA, mapB, tiles, st);
+}
+
+// Values of a 16-bit store: all rows start at multiples of it, and it divides the width.
+int store_values(const void* out, long long ld, int width) {
+  if (ld % 8 == 0 && width % 8 == 0 && aligned(out, 16)) return 8;
+  return ld % 2 == 0 && width % 2 == 0 && aligned(out, 4) ? 2 : 1;
 }
 
 int check_group(int type, int R, int E, int N, int K, const int* offsets) {
@@ -620,16 +724,16 @@ int fs_grouped_mm(const void* x, long long ldx, int M, const int* rows, int R, c
   if (!loadable(x, ldx) || !loadable(w, w_ld) || w_expert % 8) return not_loadable();
   GroupArgs a{};
   a.offsets = offsets; a.brows = rows; a.Mb = M; a.R = R; a.E = E; a.N = N; a.K = K;
-  a.out = out; a.ldo = ldo; a.type = type; a.out_type = out_type;
-  CUtensorMap maps[4] = {};
-  if (!encode(&maps[0], type, w, 3, {k_major ? K : N, k_major ? N : K, E}, {w_ld, w_expert ? w_expert : w_ld}, k_major ? 128 : 64))
+  a.out = out; a.ldo = ldo; a.type = type; a.out_type = out_type; a.bptr = x; a.ldb = ldx;
+  a.out_vec = store_values(out, ldo, N);
+  CUtensorMap mapA = {};
+  if (!encode(&mapA, type, w, 3, {k_major ? K : N, k_major ? N : K, E}, {w_ld, w_expert ? w_expert : w_ld}, k_major ? 128 : 64))
     return no_map();
-  if (!encode_rows(&maps[3], type, x, K, M, ldx, 1)) return no_map();
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int mean = R / E;
-  if (mean >= 96 && N > 128) return launch_rows<2, 256>(a, k_major, maps, x, ldx, st);
-  if (mean >= 48) return launch_rows<1, 128>(a, k_major, maps, x, ldx, st);
-  return launch_rows<1, 32>(a, k_major, maps, x, ldx, st);
+  if (mean >= 96 && N > 128) return launch_rows<2, 256>(a, k_major, mapA, st);
+  if (mean >= 48) return launch_rows<1, 128>(a, k_major, mapA, st);
+  return launch_rows<1, 32>(a, k_major, mapA, st);
 }
 
 int fs_grouped_mm_wgrad(const void* dy, long long lddy, int M_dy, const int* dy_rows, const void* x, long long ldx, int M_x,
@@ -644,16 +748,15 @@ int fs_grouped_mm_wgrad(const void* dy, long long lddy, int M_dy, const int* dy_
     const cudaError_t e = cudaMemsetAsync(dw, 0, (size_t)E * N * K * 2, st);
     return e == cudaSuccess ? FS_OK : report_error(FS_ERR_CUDA, cudaGetErrorString(e));
   }
-  if (!loadable(dy, lddy) || !loadable(x, ldx) || (K % 8 == 0 && !aligned(dw, 16))) return not_loadable();
+  if (!loadable(dy, lddy) || !loadable(x, ldx)) return not_loadable();
   GroupArgs a{};
   a.offsets = offsets; a.arows = dy_rows; a.Ma = M_dy; a.brows = x_rows; a.Mb = M_x; a.R = R; a.E = E; a.N = N; a.K = K;
-  a.out = dw; a.type = a.out_type = type;
-  CUtensorMap maps[4] = {};
-  if (!encode_rows(&maps[0], type, dy, N, M_dy, lddy, 64) || !encode_rows(&maps[1], type, dy, N, M_dy, lddy, 1) ||
-      !encode_rows(&maps[2], type, x, K, M_x, ldx, 64) || !encode_rows(&maps[3], type, x, K, M_x, ldx, 1))
-    return no_map();
-  if (N > 128 && K > 128) return launch_group<WEIGHTS, 2, 256>(a, maps, (long long)E * ((N + 255) / 256) * ((K + 255) / 256), st);
-  return launch_group<WEIGHTS, 1, 128>(a, maps, (long long)E * ((N + 127) / 128) * ((K + 127) / 128), st);
+  a.out = dw; a.type = a.out_type = type; a.out_vec = store_values(dw, K, K);
+  a.aptr = dy; a.lda = lddy; a.bptr = x; a.ldb = ldx;
+  CUtensorMap mapA = {}, mapB = {};
+  if (!encode_rows(&mapA, type, dy, N, M_dy, lddy, 64) || !encode_rows(&mapB, type, x, K, M_x, ldx, 64)) return no_map();
+  if (N > 128 && K > 128) return launch_group<WEIGHTS, 2, 256, true>(a, mapA, mapB, (long long)E * ((N + 255) / 256) * ((K + 255) / 256), st);
+  return launch_group<WEIGHTS, 1, 128, true>(a, mapA, mapB, (long long)E * ((N + 127) / 128) * ((K + 127) / 128), st);
 }
 
 }  // extern "C"

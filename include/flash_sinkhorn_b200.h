@@ -510,7 +510,7 @@ int fs_grouped_mm(const void* x, long long ldx, int M, const int* rows, int R, c
                   long long ldo, int type, void* stream);
 
 /* Its gradient to the weights: dw[e, n, k] = sum over the rows i of expert e of dy[dy_row(i), n] x[x_row(i), k], zeros for
- * an expert without rows; dw is E x N x K, densely packed. dy and x aligned and strided as x above, dw to 16 bytes. */
+ * an expert without rows; dw is E x N x K, densely packed. dy and x are aligned and strided as x above. */
 int fs_grouped_mm_wgrad(const void* dy, long long lddy, int M_dy, const int* dy_rows, const void* x, long long ldx, int M_x,
                         const int* x_rows, int R, int E, int N, int K, const int* offsets, void* dw, int type,
                         void* stream);
