@@ -579,7 +579,7 @@ int launch_act(const ActArgs& a, int type, bool grad, int vec, cudaStream_t st) 
 struct CombineArgs {
   const void* o;
   long long ldo;
-  int T, k, D, parts;
+  int M, T, k, D, parts;
   const float* gates;  // null: weights of 1
   const int *position, *pairs;
   void* y;
@@ -591,7 +591,7 @@ struct CombineArgs {
 
 template <typename T, typename Y, int VEC>
 __global__ void __launch_bounds__(kActWarps * 32) combine_kernel(const CombineArgs a) {
-  const int lane = threadIdx.x & 31, n = a.T * a.k;
+  const int lane = threadIdx.x & 31;
   const int steps = (a.D + 32 * VEC - 1) / (32 * VEC), share = (steps + a.parts - 1) / a.parts;
   const long long items = (long long)a.T * a.parts;
   for (long long it = (long long)blockIdx.x * kActWarps + (threadIdx.x >> 5); it < items; it += (long long)gridDim.x * kActWarps) {
@@ -608,7 +608,7 @@ __global__ void __launch_bounds__(kActWarps * 32) combine_kernel(const CombineAr
       for (int j = 0; j < a.k; ++j) {
         const int row = __shfl_sync(kAll, at, j);
         const float wj = __shfl_sync(kAll, w, j);
-        if (row >= 0 && row < n && c < a.D) {
+        if (row >= 0 && row < a.M && c < a.D) {
           float o[VEC];
           load_f32<T, VEC>(static_cast<const T*>(a.o) + (long long)row * a.ldo + c, o);
 #pragma unroll
@@ -764,15 +764,15 @@ int fs_gated_act_grad(const void* u, long long ldu, const int8_t* codes, const u
   return launch_act(a, type, true, vec, static_cast<cudaStream_t>(stream));
 }
 
-int fs_combine(const void* o, int type, long long ldo, int T, int k, int D, const float* gates, const int* position, void* y,
-               int y_type, void* stream) {
+int fs_combine(const void* o, int type, long long ldo, int M, int T, int k, int D, const float* gates, const int* position,
+               void* y, int y_type, void* stream) {
   int s = check_rows(type, T, D);
   if (s != FS_OK || T == 0) return s;
   if (k < 1 || k > kMaxK || (long long)T * k > 0x7fffffffll) return report_error(FS_ERR_BAD_ARG, "k must be in [1, 32], T * k below 2^31");
-  if (!o || !position || !y || ldo < D || y_type < 0 || y_type > 2 || (y_type != type && type != FS_TYPE_F32))
+  if (!o || M < 0 || !position || !y || ldo < D || y_type < 0 || y_type > 2 || (y_type != type && type != FS_TYPE_F32))
     return report_error(FS_ERR_BAD_ARG, "null argument, rows shorter than D, or a wrong type of the result");
   CombineArgs a{};
-  a.o = o; a.ldo = ldo; a.T = T; a.k = k; a.D = D; a.gates = gates; a.position = position; a.y = y;
+  a.o = o; a.ldo = ldo; a.M = M; a.T = T; a.k = k; a.D = D; a.gates = gates; a.position = position; a.y = y;
   return launch_combine(a, type, y_type, false, lane_values(D, type_bytes(type), ldo, 0, o, y), static_cast<cudaStream_t>(stream));
 }
 

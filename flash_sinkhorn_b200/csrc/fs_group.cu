@@ -1,22 +1,23 @@
 // Matrix products grouped by expert on the 5th-generation tensor cores, with groups of any size.
 //
 //   rows     out[i, n] = sum_k W_e[n, k] x[row(i), k]           (forward, and the gradient to x with W transposed)
-//   weights  dw_e[n, k] = sum_i dy[dy_row(i), n] x[x_row(i), k]  (i over the rows of expert e)
+//   weights  dw_e[n, k] = sum_i dy[i, n] x[i, k]                 (i over the rows of expert e)
 //
 // In the rows form the FEATURES are the M side of the tensor-core instruction (128 lanes of TMEM per CTA) and the rows of a
 // group its N side: N goes in steps of 16 at run time, so the last, partial tile of a group costs what it holds, and a
 // group of one row costs 16 columns rather than 128. The rows of the next group that a tile load may bring along are other
 // columns of the accumulator; they are not written. In the weights form the rows are the contraction, so those of
-// another group must not be read: the block of 64 rows that a group ends in is filled up with zeros, in both operands, so
-// that no infinity of a neighbour meets a zero.
+// another group must not be read: a group ends at a step of 16 of the contraction, and where its rows end inside of one,
+// the rest of that step is overwritten with zeros in shared memory, in both operands, so that no infinity of a neighbour
+// meets a zero.
 //
 // One persistent CTA per SM, or a pair of CTAs on neighbouring SMs that share a 256 x 256 tile (each holds 128 features and
 // fetches half of the rows: two thirds of the bytes per product of 128 x 256 tiles). Warp 4 fetches whole tiles (TMA into a
 // ring of stages of 64 contraction values), warp 5 issues the products into one of two TMEM accumulators, warps 0 to 3
-// write the other one out. Rows in another order and blocks that end inside are fetched by warps 6 to 9, 16 bytes a lane
-// (cp.async; a lane keeps four stages in flight): TMA's loads of four rows each took 75 clocks apiece, 2.6 times the time
-// of the whole product. Group boundaries are read by the kernel itself; every CTA takes every n-th tile, features fastest,
-// so that the CTAs working at one time share a group's weights and rows in L2.
+// write the other one out. Rows in another order are fetched by warps 7 to 10, 16 bytes a lane (cp.async): TMA's loads of
+// four rows each took 75 clocks apiece, 2.6 times the time of the whole product. Group boundaries are read by the kernel
+// itself; every CTA takes every n-th tile, features fastest, so that the CTAs working at one time share a group's weights
+// and rows in L2.
 #include "fs_experts.cuh"
 #include "fs_ptx.cuh"
 #include "fs_tc.cuh"
@@ -35,23 +36,23 @@ __device__ int g_group_error = 0;  // non-zero once a bounded wait gave up (read
 
 enum Form { ROWS_K, ROWS_MN, WEIGHTS };  // rows with W contiguous along the contraction; along the features
 
-constexpr int kCopyWarps = 4, kCopyDepth = 4;  // warps that fetch single rows; stages that each has in flight
+constexpr int kCopyWarps = 4;              // warps that fetch single rows
+constexpr int kCopyRows = 4 * kCopyWarps;  // rows that they fetch 128 bytes of at a time
 constexpr uint32_t kHalfTile = 64 * 128;  // 64 rows of 128 bytes
 constexpr int kMaxGroups = 1024;
 
 struct GroupArgs {
   const int* offsets;
-  const int *arows, *brows;  // row numbers of the M and N operands (null: in order)
-  int Ma, Mb;                // rows of those operands
+  const int* rows;  // rows form: row numbers (null: in order)
+  int M;            // and the rows that there are
   int R, E, N, K;
   void* out;
   long long ldo;
   int type, out_type;  // FS_TYPE_*
   int out_vec;         // values of a store: 8, 2 or 1
   int nstage;
-  // operands as plain memory, for rows that are fetched one by one
-  const void *aptr, *bptr;
-  long long lda, ldb;
+  const void* x;  // the rows as plain memory, for fetching them one by one
+  long long ldx;
 };
 
 // ------------------------------------------------------------------ PTX of CTA pairs and gathered loads
@@ -96,11 +97,13 @@ __device__ __forceinline__ void expect_cluster(uint32_t bar, uint32_t bytes) {
 }
 // 16 bytes, of which those past the first `valid` become zeros (the source is not read for them).
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int valid) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid) : "memory");
+  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid) : "memory");
 }
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// Arrives at a barrier of this CTA when all copies that the thread has started so far are there.
+__device__ __forceinline__ void copy_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void copy_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 template <int CG>
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   if (CG == 2)
@@ -301,30 +304,27 @@ __device__ __forceinline__ void write_block(uint16_t* out, long long ld, int row
   }
 }
 
-// One lane's part of an operand block that comes row by row: 16-byte chunk `chunk` of row i of the operand (through `rows`, if
-// given; zeros where i is not below hi or the number is not that of a row), its first value being column c of `width`.
-__device__ __forceinline__ void copy_chunk(uint32_t dst, const void* base, long long ld, const int* rows, int M, int i, int hi, int c,
-                                           int width) {
-  int r = i < hi ? (rows ? __ldg(rows + i) : i) : -1;
-  int valid = r >= 0 && r < M ? (width - c) * 2 : 0;
-  valid = min(max(valid, 0), 16);
-  copy16(dst, static_cast<const uint16_t*>(base) + (valid ? r * ld + c : 0), valid);
+// A row number that nothing waits for before it is used.
+__device__ __forceinline__ int load_early(const int* p) {
+  int v;
+  asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
 }
 
-// COPY: rows of the N operand come one by one (rows form); the weights form always has warps for that.
+// COPY (rows form): the rows come one by one.
 template <int FORM, int CG, int BN, bool COPY>
-__global__ void __launch_bounds__(COPY ? 192 + 32 * kCopyWarps : 192, 1)
+__global__ void __launch_bounds__(224 + (COPY ? 32 * kCopyWarps : 0), 1)
 group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB) {
   constexpr int BNC = BN / CG;                         // columns whose operand this CTA fetches
   constexpr uint32_t kA = 2 * kHalfTile, kB = BNC * 128, kStage = kA + kB;
   constexpr bool A_MN = FORM != ROWS_K, B_MN = FORM == WEIGHTS;
   constexpr uint32_t kColumns = 2 * BN;
-  static_assert(kColumns >= 32 && kColumns <= 512 && kStage % 1024 == 0 && (COPY || FORM != WEIGHTS), "tile");
+  static_assert(kColumns >= 32 && kColumns <= 512 && kStage % 1024 == 0 && !(COPY && FORM == WEIGHTS), "tile");
   extern __shared__ uint8_t raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   uint8_t* staging = ring + (size_t)a.nstage * kStage;  // 2 KB for each of warps 0 to 3
   uint64_t* bars = reinterpret_cast<uint64_t*>(staging + 8192);
-  const int FULL = 0, EMPTY = a.nstage, ACC_FULL = 2 * a.nstage, ACC_EMPTY = ACC_FULL + 2, DRAIN = ACC_EMPTY + 2;
+  const int FULL = 0, EMPTY = a.nstage, PARTS = 2 * a.nstage, ACC_FULL = 3 * a.nstage, ACC_EMPTY = ACC_FULL + 2, DRAIN = ACC_EMPTY + 2;
   uint32_t* slot = reinterpret_cast<uint32_t*>(bars + DRAIN + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(slot + 1);
   int *gs = reinterpret_cast<int*>(slot + 2), *ts = gs + a.E + 2;
@@ -338,8 +338,9 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
     read_groups<FORM != WEIGHTS>(a, gs, ts, (a.N + 128 * CG - 1) / (128 * CG), BN);
   } else if (warp == 4 && lane == 0) {
     for (int s = 0; s < a.nstage; ++s) {
-      mbar_init(bar(FULL + s), CG * (COPY ? 1 + kCopyWarps : 1));  // in CTA 0: every fetching warp of the pair
+      mbar_init(bar(FULL + s), CG * (COPY ? 2 : 1));  // in CTA 0: warp 4 and, with COPY, warp 6 of either CTA
       mbar_init(bar(EMPTY + s), 1);
+      mbar_init(bar(PARTS + s), COPY ? 32 * kCopyWarps : 1);  // what warp 6 waits for
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar(ACC_FULL + i), 1);
@@ -372,31 +373,30 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
         const int npc = (t.cols + 16 * CG - 1) / (16 * CG) * 16;  // columns of the product that this CTA fetches
         const int m0 = t.m0 + rank * 128;
         for (int kb = 0; kb < t.blocks; ++kb) {
-          if (!mbar_wait(bar(EMPTY + s), ph ^ 1, abort_flag, 2000)) {
+          if (!mbar_wait(bar(EMPTY + s), ph ^ 1, abort_flag)) {
             ok = false;
             break;
           }
           const uint32_t full = full_bar(s), dst = smem_u32(ring + (size_t)s * kStage);
-          const int i0 = t.lo + kb * 64;
-          const bool part = FORM == WEIGHTS && i0 + 64 > t.hi;  // rows of another group follow
-          const bool load_a = !(FORM == WEIGHTS && (a.arows || part)), load_b = !(COPY && (FORM != WEIGHTS || a.brows || part));
-          expect_cluster(full, (load_a ? kA : 0u) + (load_b ? kB : 0u));
-          if (FORM == ROWS_K) {
-            load_3d<CG>(dst, &mapA, kb * 64, m0, t.e, full);
-          } else if (FORM == ROWS_MN) {
-            load_3d<CG>(dst, &mapA, m0, kb * 64, t.e, full);
-            load_3d<CG>(dst + kHalfTile, &mapA, m0 + 64, kb * 64, t.e, full);
-          } else if (load_a) {
-            load_2d<CG>(dst, &mapA, m0, i0, full);
-            load_2d<CG>(dst + kHalfTile, &mapA, m0 + 64, i0, full);
-          }
-          if (load_b) {
-            if (FORM == WEIGHTS) {
+          if (FORM == WEIGHTS) {  // a block that ends inside of a step goes through warp 6
+            const int i0 = t.lo + kb * 64;
+            const bool open = kb == t.blocks - 1 && (t.hi - t.lo) % 16 != 0;
+            const uint32_t to = open ? bar(PARTS + s) : full;
+            if (open) mbar_expect_tx(to, kStage);
+            else expect_cluster(to, kStage);
 #pragma unroll
-              for (int c = 0; c < BNC / 64; ++c) load_2d<CG>(dst + kA + c * kHalfTile, &mapB, t.n0 + rank * npc + c * 64, i0, full);
+            for (int c = 0; c < 2; ++c) load_2d<CG>(dst + c * kHalfTile, &mapA, m0 + c * 64, i0, to);
+#pragma unroll
+            for (int c = 0; c < BNC / 64; ++c) load_2d<CG>(dst + kA + c * kHalfTile, &mapB, t.n0 + rank * npc + c * 64, i0, to);
+          } else {
+            expect_cluster(full, kA + (COPY ? 0u : kB));
+            if (FORM == ROWS_K) {
+              load_3d<CG>(dst, &mapA, kb * 64, m0, t.e, full);
             } else {
-              load_2d<CG>(dst + kA, &mapB, kb * 64, t.lo + rank * npc, full);
+              load_3d<CG>(dst, &mapA, m0, kb * 64, t.e, full);
+              load_3d<CG>(dst + kHalfTile, &mapA, m0 + 64, kb * 64, t.e, full);
             }
+            if (!COPY) load_2d<CG>(dst + kA, &mapB, kb * 64, t.lo + rank * npc, full);
           }
           ++issued;
           if (++s == a.nstage) {
@@ -425,12 +425,12 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
         const int np = (t.cols + 16 * CG - 1) / (16 * CG) * (16 * CG);
         const uint32_t idesc = idesc0 | ((uint32_t)(np >> 3) << 17);
         const int buf = n & 1;
-        if (!__all_sync(0xffffffffu, mbar_wait(bar(ACC_EMPTY + buf), ((n >> 1) & 1) ^ 1, abort_flag, 2000))) break;
+        if (!__all_sync(0xffffffffu, mbar_wait(bar(ACC_EMPTY + buf), ((n >> 1) & 1) ^ 1, abort_flag))) break;
         ++n;
         tc_fence_after();
         const uint32_t d = tmem + buf * BN;
         for (int kb = 0; kb < t.blocks; ++kb) {
-          if (!__all_sync(0xffffffffu, mbar_wait(bar(FULL + s), ph, abort_flag, 2000))) {
+          if (!__all_sync(0xffffffffu, mbar_wait(bar(FULL + s), ph, abort_flag))) {
             ok = false;
             break;
           }
@@ -509,78 +509,98 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
         }
       }
     }
-  } else if (COPY) {
+  } else if (COPY && warp > 6) {
     // ===================== single rows =====================
-    // Chunk ch of rows r, r + 16, ... of every half tile (64 rows of 128 bytes, chunk exchanged with its row as the 128-byte
-    // swizzle has it). A stage is reported full when the copies of kCopyDepth - 1 stages later are under way; at once if
-    // nothing of it is copied here.
-    const int id = threadIdx.x - 192, r = id >> 3, ch = id & 7;
-    const uint32_t at = r * 128 + ((ch ^ (r & 7)) << 4);  // 16 rows on: 2048 bytes
-    int s = 0;
-    uint32_t ph = 0, copied = 0;  // bit i: the stage i before the last one has copies that are not reported
+    // Chunk ch of rows r, r + kCopyRows, ... of a stage, the chunk exchanged with its row as the 128-byte swizzle has it.
+    // These warps only start copies; that a stage's copies are there is seen by warp 6. Row numbers are read a tile ahead:
+    // what is read behind the copies comes back after them.
+    constexpr int kSteps = (BNC + kCopyRows - 1) / kCopyRows;
+    const int id = threadIdx.x - 224, r = id >> 3, ch = id & 7;
+    const uint32_t at = kA + r * 128 + ((ch ^ (r & 7)) << 4);
+    int s = 0, ahead[kSteps];
+    uint32_t ph = 0;
     bool ok = true;
-    auto report = [&](int stage, bool copies) {
-      if (copies) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) arrive_cluster(full_bar(stage));
+    Tiles<FORM, CG, BN> ahead_tiles = tiles;
+    auto read_ahead = [&](int it) {
+      if (it >= total) return;
+      const Tile t = ahead_tiles.at(it);
+      const int npc = (t.cols + 16 * CG - 1) / (16 * CG) * 16;
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) {
+        const int i = t.lo + rank * npc + r + kCopyRows * j;
+        ahead[j] = t.blocks && r + kCopyRows * j < npc && i < t.hi ? load_early(a.rows + i) : -1;
+      }
     };
-    auto stage_before = [&](int n) { return s >= n ? s - n : s - n + a.nstage; };
+    read_ahead(first);
     for (int it = first; ok && it < total; it += stride) {
       const Tile t = tiles.at(it);
-      const int npc = (t.cols + 16 * CG - 1) / (16 * CG) * 16, m0 = t.m0 + rank * 128;
-      const uint16_t* src[8];
-      if (FORM != WEIGHTS && t.blocks) {
+      const uint16_t* src[kSteps];
 #pragma unroll
-        for (int j = 0; j < BNC / 16; ++j) {
-          const int i = t.lo + rank * npc + r + 16 * j, v = i < t.hi && r + 16 * j < npc ? __ldg(a.brows + i) : -1;
-          src[j] = v >= 0 && v < a.Mb ? static_cast<const uint16_t*>(a.bptr) + v * a.ldb + ch * 8 : nullptr;
-        }
-      }
+      for (int j = 0; j < kSteps; ++j)
+        src[j] = (unsigned)ahead[j] < (unsigned)a.M ? static_cast<const uint16_t*>(a.x) + ahead[j] * a.ldx + ch * 8 : nullptr;
+      read_ahead(it + stride);
       for (int kb = 0; kb < t.blocks; ++kb) {
         if (!__all_sync(0xffffffffu, mbar_wait(bar(EMPTY + s), ph ^ 1, abort_flag, 2000))) {
           ok = false;
           break;
         }
         const uint32_t dst = smem_u32(ring + (size_t)s * kStage) + at;
-        bool copies = true;
-        if (FORM == WEIGHTS) {
-          const int i0 = t.lo + kb * 64;
-          const bool part = i0 + 64 > t.hi;
-          copies = part || a.arows || a.brows;
-          if (a.arows || part) {
+        const int valid = min(max((a.K - kb * 64 - ch * 8) * 2, 0), 16);
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              copy_chunk(dst + j * 2048, a.aptr, a.lda, a.arows, a.Ma, i0 + r + 16 * (j & 3), t.hi, m0 + (j >> 2) * 64 + ch * 8, a.N);
-          }
-          if (a.brows || part) {
-#pragma unroll
-            for (int j = 0; j < BNC / 16; ++j)
-              copy_chunk(dst + kA + j * 2048, a.bptr, a.ldb, a.brows, a.Mb, i0 + r + 16 * (j & 3), t.hi,
-                         t.n0 + rank * npc + (j >> 2) * 64 + ch * 8, a.K);
-          }
-        } else {
-          const int valid = min(max((a.K - kb * 64 - ch * 8) * 2, 0), 16);
-#pragma unroll
-          for (int j = 0; j < BNC / 16; ++j)
-            copy16(dst + kA + j * 2048, src[j] && valid ? src[j] + kb * 64 : a.bptr, src[j] ? valid : 0);
-        }
-        copy_commit();
-        copied = copied << 1 | (copies ? 1u : 0u);
-        if (!copies) report(s, false);
-        if (copied >> (kCopyDepth - 1) & 1u) {
-          copy_wait<kCopyDepth - 1>();
-          report(stage_before(kCopyDepth - 1), true);
-        }
+        for (int j = 0; j < kSteps; ++j)
+          copy16(dst + j * kCopyRows * 128, src[j] && valid ? src[j] + kb * 64 : a.x, src[j] ? valid : 0);
+        copy_arrive(bar(PARTS + s));
         if (++s == a.nstage) {
           s = 0;
           ph ^= 1;
         }
       }
     }
-    copy_wait<0>();
-    if (ok)
-      for (int i = kCopyDepth - 2; i >= 0; --i)
-        if (copied >> i & 1u) report(stage_before(i + 1), true);  // s is one past the last stage here
+    copy_wait_all();
+  } else if (COPY) {
+    // ===================== warp 6: reports of copied stages =====================
+    // Copies are ordinary writes: their completion, seen here, is made visible to the tensor core, which reads by the
+    // asynchronous proxy, and reported to CTA 0 by a thread that has no copies of its own to wait for.
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = lane == 0;
+    for (int it = first; ok && it < total; it += stride) {
+      const Tile t = tiles.at(it);
+      for (int kb = 0; kb < t.blocks; ++kb) {
+        if (!mbar_wait(bar(PARTS + s), ph, abort_flag)) {
+          ok = false;
+          break;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        arrive_cluster(full_bar(s));
+        if (++s == a.nstage) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+    }
+  } else if (FORM == WEIGHTS) {
+    // ===================== warp 6: ends of groups =====================
+    int s = 0;         // first stage of the tile
+    uint32_t uses = 0;  // bit s: parity of the uses of stage s here
+    for (int it = first; it < total; it += stride) {
+      const Tile t = tiles.at(it);
+      const int rows = t.hi - t.lo, stage = (s + t.blocks - 1) % a.nstage;
+      s = (s + t.blocks) % a.nstage;
+      if (rows % 16 == 0) continue;
+      if (!__all_sync(0xffffffffu, mbar_wait(bar(PARTS + stage), uses >> stage & 1, abort_flag, 2000))) break;
+      uses ^= 1u << stage;
+      uint8_t* block = ring + (size_t)stage * kStage;
+      const int from = rows & 63, chunks = ((rows + 15) / 16 * 16 - rows) * 8;  // 16-byte chunks of a half tile
+      for (int c = lane; c < chunks; c += 32)
+#pragma unroll
+        for (int h = 0; h < 2 + BNC / 64; ++h)
+          *reinterpret_cast<uint4*>(block + h * kHalfTile + from * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) arrive_cluster(full_bar(stage));
+      __syncwarp();
+    }
   }
   __syncwarp();
   tc_fence_before();
@@ -625,9 +645,9 @@ int no_map() { return report_error(FS_ERR_CUDA, "cuTensorMapEncodeTiled failed")
 template <int FORM, int CG, int BN, bool COPY>
 int launch_group(GroupArgs a, const CUtensorMap& mapA, const CUtensorMap& mapB, long long most_tiles, cudaStream_t st) {
   constexpr size_t kStage = 2 * kHalfTile + BN / CG * 128;
-  const size_t fixed = 1024 + 8192 + 8 * (2 * 12 + 5) + 8 + 8 * ((size_t)a.E + 2);
+  const size_t fixed = 1024 + 8192 + 8 * (3 * 12 + 5) + 8 + 8 * ((size_t)a.E + 2);
   a.nstage = (int)((kSmemMax - fixed) / kStage);
-  static_assert((kSmemMax - 1024 - 8192 - 248 - 8 * (kMaxGroups + 2)) / kStage > kCopyDepth, "stages");
+  static_assert((kSmemMax - 1024 - 8192 - 344 - 8 * (kMaxGroups + 2)) / kStage >= 4, "stages");
   if (a.nstage > 12) a.nstage = 12;
   size_t smem = fixed + a.nstage * kStage;
   if (smem < (size_t)kSmemMin) smem = kSmemMin;
@@ -640,7 +660,7 @@ int launch_group(GroupArgs a, const CUtensorMap& mapA, const CUtensorMap& mapB, 
   if (grid < 1) grid = 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)grid * CG);
-  cfg.blockDim = dim3(COPY ? 192 + 32 * kCopyWarps : 192);
+  cfg.blockDim = dim3(224 + (COPY ? 32 * kCopyWarps : 0));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr{};
@@ -658,9 +678,9 @@ int launch_group(GroupArgs a, const CUtensorMap& mapA, const CUtensorMap& mapB, 
 template <int CG, int BN>
 int launch_rows(const GroupArgs& a, bool k_major, const CUtensorMap& mapA, cudaStream_t st) {
   CUtensorMap mapB = {};
-  if (!a.brows && !encode_rows(&mapB, a.type, a.bptr, a.K, a.Mb, a.ldb, BN / CG)) return no_map();
+  if (!a.rows && !encode_rows(&mapB, a.type, a.x, a.K, a.M, a.ldx, BN / CG)) return no_map();
   const long long tiles = ((a.R + BN - 1ll) / BN + a.E + 1) * ((a.N + 128 * CG - 1) / (128 * CG));
-  if (a.brows)
+  if (a.rows)
     return k_major ? launch_group<ROWS_K, CG, BN, true>(a, mapA, mapB, tiles, st) : launch_group<ROWS_MN, CG, BN, true>(a, mapA, mapB, tiles, st);
   return k_major ? launch_group<ROWS_K, CG, BN, false>(a, mapA, mapB, tiles, st) : launch_group<ROWS_MN, CG, BN, false>(a, mapA, mapB, tiles, st);
 }
@@ -723,8 +743,8 @@ int fs_grouped_mm(const void* x, long long ldx, int M, const int* rows, int R, c
     return report_error(FS_ERR_BAD_ARG, "rows or experts of w overlap");
   if (!loadable(x, ldx) || !loadable(w, w_ld) || w_expert % 8) return not_loadable();
   GroupArgs a{};
-  a.offsets = offsets; a.brows = rows; a.Mb = M; a.R = R; a.E = E; a.N = N; a.K = K;
-  a.out = out; a.ldo = ldo; a.type = type; a.out_type = out_type; a.bptr = x; a.ldb = ldx;
+  a.offsets = offsets; a.rows = rows; a.M = M; a.R = R; a.E = E; a.N = N; a.K = K;
+  a.out = out; a.ldo = ldo; a.type = type; a.out_type = out_type; a.x = x; a.ldx = ldx;
   a.out_vec = store_values(out, ldo, N);
   CUtensorMap mapA = {};
   if (!encode(&mapA, type, w, 3, {k_major ? K : N, k_major ? N : K, E}, {w_ld, w_expert ? w_expert : w_ld}, k_major ? 128 : 64))
@@ -736,13 +756,11 @@ int fs_grouped_mm(const void* x, long long ldx, int M, const int* rows, int R, c
   return launch_rows<1, 32>(a, k_major, mapA, st);
 }
 
-int fs_grouped_mm_wgrad(const void* dy, long long lddy, int M_dy, const int* dy_rows, const void* x, long long ldx, int M_x,
-                        const int* x_rows, int R, int E, int N, int K, const int* offsets, void* dw, int type,
-                        void* stream) {
+int fs_grouped_mm_wgrad(const void* dy, long long lddy, const void* x, long long ldx, int R, int E, int N, int K,
+                        const int* offsets, void* dw, int type, void* stream) {
   int s = check_group(type, R, E, N, K, offsets);
   if (s != FS_OK) return s;
-  if (!dw || (R > 0 && (!dy || !x || M_dy < 1 || M_x < 1)) || lddy < N || ldx < K || (!dy_rows && M_dy < R) || (!x_rows && M_x < R))
-    return report_error(FS_ERR_BAD_ARG, "null argument, or too few rows or columns");
+  if (!dw || (R > 0 && (!dy || !x)) || lddy < N || ldx < K) return report_error(FS_ERR_BAD_ARG, "null argument, or too few columns");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (R == 0) {
     const cudaError_t e = cudaMemsetAsync(dw, 0, (size_t)E * N * K * 2, st);
@@ -750,13 +768,12 @@ int fs_grouped_mm_wgrad(const void* dy, long long lddy, int M_dy, const int* dy_
   }
   if (!loadable(dy, lddy) || !loadable(x, ldx)) return not_loadable();
   GroupArgs a{};
-  a.offsets = offsets; a.arows = dy_rows; a.Ma = M_dy; a.brows = x_rows; a.Mb = M_x; a.R = R; a.E = E; a.N = N; a.K = K;
+  a.offsets = offsets; a.R = R; a.E = E; a.N = N; a.K = K;
   a.out = dw; a.type = a.out_type = type; a.out_vec = store_values(dw, K, K);
-  a.aptr = dy; a.lda = lddy; a.bptr = x; a.ldb = ldx;
   CUtensorMap mapA = {}, mapB = {};
-  if (!encode_rows(&mapA, type, dy, N, M_dy, lddy, 64) || !encode_rows(&mapB, type, x, K, M_x, ldx, 64)) return no_map();
-  if (N > 128 && K > 128) return launch_group<WEIGHTS, 2, 256, true>(a, mapA, mapB, (long long)E * ((N + 255) / 256) * ((K + 255) / 256), st);
-  return launch_group<WEIGHTS, 1, 128, true>(a, mapA, mapB, (long long)E * ((N + 127) / 128) * ((K + 127) / 128), st);
+  if (!encode_rows(&mapA, type, dy, N, R, lddy, 64) || !encode_rows(&mapB, type, x, K, R, ldx, 64)) return no_map();
+  if (N > 128 && K > 128) return launch_group<WEIGHTS, 2, 256, false>(a, mapA, mapB, (long long)E * ((N + 255) / 256) * ((K + 255) / 256), st);
+  return launch_group<WEIGHTS, 1, 128, false>(a, mapA, mapB, (long long)E * ((N + 127) / 128) * ((K + 127) / 128), st);
 }
 
 }  // extern "C"

@@ -197,14 +197,19 @@ def _mm(x, rows, count, w, offsets, transposed=False, dtype=None):
     return out
 
 
-def _wgrad(dy, dy_rows, x, x_rows, count, offsets):
-    dev, e = x.device, offsets.shape[0] - 1
+def _wgrad(dy, x, offsets):
+    """``[E, N, K]``: per expert the sum over its rows of ``dy [R, N]`` times ``x [R, K]``."""
+    dev, e, r = x.device, offsets.shape[0] - 1, x.shape[0]
     dy, x = _loadable_rows(dy), _loadable_rows(x)
     out = torch.empty((e, dy.shape[1], x.shape[1]), dtype=x.dtype, device=dev)
-    _lib.call("fs_grouped_mm_wgrad", dev, _lib.ptr(dy), _ld(dy), dy.shape[0], _lib.ptr(dy_rows), _lib.ptr(x), _ld(x),
-              x.shape[0], _lib.ptr(x_rows), count, e, dy.shape[1], x.shape[1], _lib.ptr(offsets), _lib.ptr(out),
-              _TYPES[x.dtype], _lib.stream_ptr(dev))
+    _lib.call("fs_grouped_mm_wgrad", dev, _lib.ptr(dy), _ld(dy), _lib.ptr(x), _ld(x), r, e, dy.shape[1], x.shape[1],
+              _lib.ptr(offsets), _lib.ptr(out), _TYPES[x.dtype], _lib.stream_ptr(dev))
     return out
+
+
+def _gather(x, rows):
+    """``x[rows]``, zeros for the rows of no pair."""
+    return _combine(x, None, rows.view(-1, 1))
 
 
 class _GroupedMmFunction(torch.autograd.Function):
@@ -227,7 +232,8 @@ class _GroupedMmFunction(torch.autograd.Function):
                 dx = _mm(dy, None, ctx.count, w, offsets, transposed=True, dtype=torch.float32)
                 dx = _combine(dx, None, position, x.dtype)
         if ctx.needs_input_grad[1]:
-            dw = _wgrad(dy, None, x, rows, ctx.count, offsets)
+            # a copy of the rows in order costs less than fetching them one by one for every tile of the product
+            dw = _wgrad(dy, x if rows is None else _gather(x, rows), offsets)
         return dx, dw, None, None, None, None
 
 
@@ -349,7 +355,7 @@ def gated_act(u: torch.Tensor, routing: Optional[Routing] = None, *, checkpoint:
 def _combine(o, gates, position, dtype=None):
     dev, (t, k), d = o.device, position.shape, o.shape[1]
     y = torch.empty((t, d), dtype=dtype or o.dtype, device=dev)
-    _lib.call("fs_combine", dev, _lib.ptr(o), _TYPES[o.dtype], _ld(o), t, k, d, _lib.ptr(gates), _lib.ptr(position),
+    _lib.call("fs_combine", dev, _lib.ptr(o), _TYPES[o.dtype], _ld(o), o.shape[0], t, k, d, _lib.ptr(gates), _lib.ptr(position),
               _lib.ptr(y), _TYPES[y.dtype], _lib.stream_ptr(dev))
     return y
 
@@ -403,7 +409,7 @@ def combine_rows(o: torch.Tensor, routing: Routing, *, weighted: bool = True) ->
 
 class _ExpertMlpFunction(torch.autograd.Function):
     """Keeps x, the routing and u (in 8 bits) from the forward pass. The gates are in the activation, so the backward pass
-    needs neither the experts' outputs nor their gradients as rows: both products with dy read it through the routing."""
+    needs neither the experts' outputs nor their gradients: both of its products with the outer weights read dy."""
 
     @staticmethod
     def forward(ctx, x, w_in, w_out, gates, offsets, pairs, rows, position, checkpoint):
@@ -418,11 +424,12 @@ class _ExpertMlpFunction(torch.autograd.Function):
         x, w_in, w_out, gates, offsets, pairs, rows, position, u, codes, scales = ctx.saved_tensors
         need_x, need_in, need_out, need_gates = ctx.needs_input_grad[:4]
         dy, count = _loadable_rows(dy), pairs.shape[0]
-        dh = _mm(dy, rows, count, w_out, offsets, transposed=True)
+        dy = _gather(dy, rows)  # for two products
+        dh = _mm(dy, None, count, w_out, offsets, transposed=True)
         du, dgates, h = _act_grad(u, codes, scales, gates, pairs, position, dh, need_gates, need_out)
         dx = _combine(_mm(du, None, count, w_in, offsets, transposed=True), None, position) if need_x else None
-        dw_in = _wgrad(du, None, x, rows, count, offsets) if need_in else None
-        dw_out = _wgrad(dy, rows, h, None, count, offsets) if need_out else None
+        dw_in = _wgrad(du, _gather(x, rows), offsets) if need_in else None
+        dw_out = _wgrad(dy, h, offsets) if need_out else None
         return dx, dw_in, dw_out, dgates, None, None, None, None, None
 
 

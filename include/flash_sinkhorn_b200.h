@@ -509,11 +509,10 @@ int fs_grouped_mm(const void* x, long long ldx, int M, const int* rows, int R, c
                   long long w_row, long long w_col, int E, int N, int K, const int* offsets, void* out, int out_type,
                   long long ldo, int type, void* stream);
 
-/* Its gradient to the weights: dw[e, n, k] = sum over the rows i of expert e of dy[dy_row(i), n] x[x_row(i), k], zeros for
- * an expert without rows; dw is E x N x K, densely packed. dy and x are aligned and strided as x above. */
-int fs_grouped_mm_wgrad(const void* dy, long long lddy, int M_dy, const int* dy_rows, const void* x, long long ldx, int M_x,
-                        const int* x_rows, int R, int E, int N, int K, const int* offsets, void* dw, int type,
-                        void* stream);
+/* Its gradient to the weights: dw[e, n, k] = sum over the rows i of expert e of dy[i, n] x[i, k], zeros for an expert
+ * without rows; dy and x have R rows and are aligned and strided as x above, dw is E x N x K, densely packed. */
+int fs_grouped_mm_wgrad(const void* dy, long long lddy, const void* x, long long ldx, int R, int E, int N, int K,
+                        const int* offsets, void* dw, int type, void* stream);
 
 /* Gated activation of R rows u = [g | v] of 2 F values: h = p g sigmoid(g) v, p = gates[pairs[i]] (1 without pairs; rows
  * of no pair give zeros). codes [R, 2 F] and scales [R, 2 ceil(F / 32)] (or null) receive u in 8 bits: blocks of 32 along
@@ -528,12 +527,12 @@ int fs_gated_act_grad(const void* u, long long ldu, const int8_t* codes, const u
                       float* dgates, void* h, void* stream);
 
 /* Rows back into tokens: y[t, :] = sum over the slots s with a row of gates[t, s] o[position[t, s], :] (gates null:
- * weights of 1). o has T * k rows of D values, y is T x D, densely packed, of the type of o or, where that is FS_TYPE_F32,
- * of any. */
-int fs_combine(const void* o, int type, long long ldo, int T, int k, int D, const float* gates, const int* position, void* y,
-               int y_type, void* stream);
+ * weights of 1; positions outside [0, M): no row). o has M rows of D values; y is T x D, densely packed, of the type of o
+ * or, where that is FS_TYPE_F32, of any. With k = 1 and no gates it gathers rows. */
+int fs_combine(const void* o, int type, long long ldo, int M, int T, int k, int D, const float* gates, const int* position,
+               void* y, int y_type, void* stream);
 
-/* Its gradients: d_o [T * k, D] densely packed, and dgates [T, k] (or null; then o may be null too). */
+/* Its gradients, for M = T * k: d_o [T * k, D] densely packed, and dgates [T, k] (or null; then o may be null too). */
 int fs_combine_grad(const void* o, int type, long long ldo, int T, int k, int D, const float* gates, const int* position,
                     const int* pairs, const void* dy, long long lddy, void* d_o, float* dgates, void* stream);
 

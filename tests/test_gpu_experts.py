@@ -235,11 +235,10 @@ def check_mm(ex, x, w, offsets, rows=None):
     return got
 
 
-def check_wgrad(ex, dy, dy_rows, x, x_rows, r, offsets):
-    e, n, k, dtype = offsets.shape[0] - 1, dy.shape[1], x.shape[1], x.dtype
-    got = ex._wgrad(dy, dy_rows, x, x_rows, r, offsets)
-    ys = dy.double() if dy_rows is None else dy.double()[dy_rows.long().clamp_min(0)]
-    xs = x.double() if x_rows is None else x.double()[x_rows.long().clamp_min(0)]
+def check_wgrad(ex, dy, x, offsets):
+    e, n, k, r, dtype = offsets.shape[0] - 1, dy.shape[1], x.shape[1], x.shape[0], x.dtype
+    got = ex._wgrad(dy, x, offsets)
+    ys, xs = dy.double(), x.double()
     want, size = torch.zeros(e, n, k, dtype=torch.float64, device="cuda"), torch.zeros(e, n, k, dtype=torch.float64, device="cuda")
     most = 1
     for j, (lo, hi) in enumerate(group_rows(offsets, r)):
@@ -274,7 +273,7 @@ def test_grouped_mm(ex, counts, n, k):
     dy = normal(g, r, n, dtype=dtype)
     assert (check_mm(ex, x, w, off)[sum(counts):] == 0).all()
     check_mm(ex, dy, w.transpose(1, 2), off)
-    check_wgrad(ex, dy, None, x, None, r, off)
+    check_wgrad(ex, dy, x, off)
 
 
 @pytest.mark.parametrize("k,n,tokens,slots,e", [(64, 96, 1, 2, 16), (256, 192, 5, 1, 3), (136, 72, 33, 4, 64), (300, 501, 200, 2, 7),
@@ -289,17 +288,19 @@ def test_grouped_mm_of_gathered_rows(ex, k, n, tokens, slots, e, dtype):
     r = tokens * slots
     check_mm(ex, x, w, routing.offsets, routing.rows)
     dy = normal(g, r, n, dtype=dtype)
-    check_wgrad(ex, dy, None, x, routing.rows, r, routing.offsets)
+    xs = ex._gather(x, routing.rows)
+    live = routing.rows >= 0
+    assert torch.equal(xs[live], x[routing.rows[live].long()]) and not xs[~live].any()
+    check_wgrad(ex, dy, xs, routing.offsets)
     dyt = normal(g, tokens, n, dtype=dtype)
     check_mm(ex, dyt, w.transpose(1, 2), routing.offsets, routing.rows)
-    check_wgrad(ex, dyt, routing.rows, normal(g, r, k, dtype=dtype), None, r, routing.offsets)
 
     # through the public call: the gradient of a token is the sum over its rows in fp32, rounded once
     xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
     y = ex.grouped_mm(xl, wl, routing, gather=True)
     dx, dw = torch.autograd.grad(y, (xl, wl), dy)
     assert torch.equal(y, ex._mm(x, routing.rows, r, w, routing.offsets))
-    assert torch.equal(dw, ex._wgrad(dy, None, x, routing.rows, r, routing.offsets))
+    assert torch.equal(dw, ex._wgrad(dy, xs, routing.offsets))
     pos = routing.position.long()
     part = ex._mm(dy, None, r, w, routing.offsets, transposed=True, dtype=FP32).double()[pos.clamp_min(0)] * (pos >= 0)[..., None]
     within(dx, part.sum(1), ULP[dtype] * part.sum(1).abs() + ACC * part.abs().sum(1) + TINY[dtype])
@@ -313,7 +314,7 @@ def test_grouped_mm_larger(ex, counts, n, k):
     x, w, dy = normal(g, r, k, dtype=BF16), normal(g, len(counts), n, k, scale=k**-0.5, dtype=BF16), normal(g, r, n, dtype=BF16)
     check_mm(ex, x, w, off)
     check_mm(ex, dy, w.transpose(1, 2), off)
-    check_wgrad(ex, dy, None, x, None, r, off)
+    check_wgrad(ex, dy, x, off)
 
 
 def test_grouped_mm_strides_and_alignment(ex):
@@ -328,7 +329,7 @@ def test_grouped_mm_strides_and_alignment(ex):
         for w in (weights[:, :n, shift:shift + k], weights[:, shift:shift + k, :n].transpose(1, 2),
                   weights[:, 3:3 + n, :k].contiguous(), weights[:1, :n, :k].expand(4, n, k)):
             check_mm(ex, x, w, off)
-        check_wgrad(ex, wide[:, shift + k:shift + k + n], None, x, None, r, off)
+        check_wgrad(ex, wide[:, shift + k:shift + k + n], x, off)
     # neither dimension of the weights is contiguous, rows of x overlap: copied, not refused
     assert torch.equal(ex.grouped_mm(wide[:, :k], weights[:, :2 * n:2, :2 * k:2], off),
                        ex.grouped_mm(wide[:, :k], weights[:, :2 * n:2, :2 * k:2].contiguous(), off))
@@ -345,7 +346,7 @@ def test_grouped_mm_keeps_groups_apart(ex, bad, n, k):
     r = sum(counts) + 30
     off = offsets_of(counts)
     x, w, dy = normal(g, r, k, dtype=BF16), normal(g, 5, n, k, scale=0.1, dtype=BF16), normal(g, r, n, dtype=BF16)
-    clean = ex._mm(x, None, r, w, off), ex._mm(dy, None, r, w, off, transposed=True), ex._wgrad(dy, None, x, None, r, off)
+    clean = ex._mm(x, None, r, w, off), ex._mm(dy, None, r, w, off, transposed=True), ex._wgrad(dy, x, off)
     x2, dy2 = x.clone(), dy.clone()
     lo, hi = 37, 57
     for t in (x2, dy2):
@@ -353,7 +354,7 @@ def test_grouped_mm_keeps_groups_apart(ex, bad, n, k):
         t[sum(counts):] = bad
     w2 = w.clone()
     w2[1] = bad
-    out, dx, dw = ex._mm(x2, None, r, w2, off), ex._mm(dy2, None, r, w2, off, transposed=True), ex._wgrad(dy2, None, x2, None, r, off)
+    out, dx, dw = ex._mm(x2, None, r, w2, off), ex._mm(dy2, None, r, w2, off, transposed=True), ex._wgrad(dy2, x2, off)
     keep = torch.ones(r, dtype=torch.bool, device="cuda")
     keep[lo:hi] = False
     assert torch.equal(out[keep], clean[0][keep]) and torch.equal(dx[keep], clean[1][keep])
@@ -369,7 +370,7 @@ def test_grouped_mm_offsets_outside_the_rows(ex):
     for odd, even in (([0, 40, 30, 1 << 30, 5], [0, 40, 40, 100, 100]), ([0, -5, 20, 20, 2147483647], [0, 0, 20, 20, 100])):
         a, b = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in (odd, even))
         assert torch.equal(ex._mm(x, None, 100, w, a), ex._mm(x, None, 100, w, b))
-        assert torch.equal(ex._wgrad(x, None, x, None, 100, a), ex._wgrad(x, None, x, None, 100, b))
+        assert torch.equal(ex._wgrad(x, x, a), ex._wgrad(x, x, b))
 
 
 def test_grouped_mm_row_numbers_outside_the_tokens(ex):
@@ -383,8 +384,7 @@ def test_grouped_mm_row_numbers_outside_the_tokens(ex):
     zeros = torch.cat([x, x.new_zeros(1, 64)])
     good = torch.where((rows >= 0) & (rows < 50), rows, 50).to(torch.int32)
     assert torch.equal(out, ex._mm(zeros, good, 300, w, off))
-    dy = normal(g, 300, 96, dtype=BF16)
-    assert torch.equal(ex._wgrad(dy, None, x, rows, 300, off), ex._wgrad(dy, None, zeros, good, 300, off))
+    assert torch.equal(ex._gather(x, rows), zeros[good.long()])
 
 
 def test_grouped_mm_weights_past_32_bits(ex):
@@ -399,7 +399,7 @@ def test_grouped_mm_weights_past_32_bits(ex):
         x = normal(g, r, k, dtype=BF16)
         want, size = x.double() @ w[-1].double().T, x.double().abs() @ w[-1].double().abs().T
         within(ex._mm(x, None, r, w, off), want, ULP[BF16] * want.abs() + ACC * 64 * size)
-        dw = ex._wgrad(x, None, x, None, r, off)
+        dw = ex._wgrad(x, x, off)
         assert not dw[:-1].any()
         want, size = x.double().T @ x.double(), x.double().abs().T @ x.double().abs()
         within(dw[-1], want, ULP[BF16] * want.abs() + ACC * 64 * size)
