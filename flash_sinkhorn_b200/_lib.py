@@ -334,7 +334,8 @@ class GradItem(ctypes.Structure):
 
 
 def stream_ptr(device: torch.device) -> int:
-    return int(torch.cuda.current_stream(device).cuda_stream)
+    # the handle itself: a Stream object around it costs 2 us
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
 
 
 def raise_if_device_timeout(device: torch.device) -> None:
@@ -354,9 +355,12 @@ def raise_if_device_timeout(device: torch.device) -> None:
 
 def call(name: str, device: torch.device, *args) -> None:
     """Invoke a compute entry point with `device` current; raise on failure."""
-    lib = load()
-    with torch.cuda.device(device):
+    lib = _lib or load()
+    if device.index == torch.cuda.current_device():
         status = getattr(lib, name)(*args)
+    else:
+        with torch.cuda.device(device):
+            status = getattr(lib, name)(*args)
     if status != 0:
         msg = lib.fs_last_error().decode("utf-8", "replace")
         raise FlashSinkhornError(f"{name} failed with {_STATUS_NAMES.get(status, status)}: {msg}")

@@ -42,34 +42,47 @@ class Routing(NamedTuple):
     position: torch.Tensor  #: ``[T, k]`` int32 row of each pair, -1 for a slot without an expert
 
 
-def _check_type(name: str, t: torch.Tensor, types=tuple(_TYPES)) -> int:
+def _check_type(name: str, t: torch.Tensor, types=tuple(_TYPES)) -> None:
     if t.dtype not in types:
         raise ValueError(f"{name} must be of type {', '.join(str(d).split('.')[-1] for d in types)}, got {t.dtype}")
-    return _TYPES[t.dtype]
+
+
+def _device_of(name: str, t: torch.Tensor, **others: torch.Tensor) -> torch.device:
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor.")
+    dev = t.device
+    for other, v in others.items():
+        if v.device != dev:
+            raise ValueError(f"{other} must be on the same CUDA device as {name} ({dev}), got {v.device}")
+    return dev
 
 
 def _rows_of(t: torch.Tensor) -> torch.Tensor:
     """``t`` itself where its rows are contiguous and do not overlap, else a copy."""
-    if t.stride(1) == 1 and t.stride(0) >= t.shape[1]:
-        return t
-    return t.contiguous()
+    ld, one = t.stride()
+    return t if one == 1 and ld >= t.shape[1] else t.contiguous()
 
 
 def _ld(t: torch.Tensor) -> int:
-    return max(t.stride(0), t.shape[1])
+    ld, width = t.stride(0), t.shape[1]
+    return ld if ld > width else width  # the stride of a single row says nothing
 
 
-def _check_routing(r: Routing, device: torch.device) -> None:
+def _check_routing(r: Routing, device: torch.device, *used: str) -> None:
+    """The fields ``used`` have the types, shapes and places that the kernels count on."""
     if not isinstance(r, Routing):
         raise ValueError(f"routing must be a Routing, got {type(r).__name__}")
-    t, k = r.position.shape if r.position.ndim == 2 else (-1, -1)
-    shapes = {"gates": (t, k), "experts": (t, k), "pairs": (t * k,), "rows": (t * k,), "position": (t, k)}
-    for name, shape in shapes.items():
+    shape = r.position.shape
+    if len(shape) != 2 or shape[1] < 1:
+        raise ValueError(f"routing.position must be of shape (T, k), got {tuple(shape)}")
+    for name in used:
         v = getattr(r, name)
         want = torch.float32 if name == "gates" else torch.int32
-        if t < 0 or tuple(v.shape) != shape or v.dtype != want or not v.is_contiguous() or v.device != device:
-            raise ValueError(f"routing.{name} must be a contiguous {want} tensor of shape {shape} on {device}")
-    _check_offsets(r.offsets, device)
+        fits = v.shape == shape if name in ("gates", "experts", "position") else (
+            v.ndim == 1 and (v.shape[0] == shape[0] * shape[1] if name != "offsets" else v.shape[0] > 1))
+        if not fits or v.dtype != want or v.device != device or not v.is_contiguous():
+            raise ValueError(f"routing.{name} must be a contiguous {want} tensor on {device} that fits {tuple(shape)} "
+                             f"(tokens, slots), got {v.dtype} {tuple(v.shape)} on {v.device}")
 
 
 def _check_offsets(offsets: torch.Tensor, device: torch.device) -> None:
@@ -85,15 +98,18 @@ def _check_offsets(offsets: torch.Tensor, device: torch.device) -> None:
 
 def _route(logits, k, bias, mask, over_all):
     dev, (t, e) = logits.device, logits.shape
+    n = t * k
     gates = torch.empty((t, k), dtype=torch.float32, device=dev)
-    whole = torch.empty(4 * t * k + e + 1, dtype=torch.int32, device=dev)
-    experts, pairs, rows, position, offsets = whole.split([t * k] * 4 + [e + 1])
-    nbytes = int(_lib.load().fs_route_bytes(t, e, k))
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _lib.call("fs_route", dev, _lib.ptr(logits), _TYPES[logits.dtype], _ld(logits), t, e, k, _lib.ptr(bias), _lib.ptr(mask),
-              int(over_all), _lib.ptr(gates), _lib.ptr(experts), _lib.ptr(offsets), _lib.ptr(pairs), _lib.ptr(rows),
-              _lib.ptr(position), _lib.ptr(ws), nbytes, _lib.stream_ptr(dev))
-    return gates, experts.view(t, k), offsets, pairs, rows, position.view(t, k)
+    nbytes = _lib.load().fs_route_bytes(t, e, k)
+    whole = torch.empty(4 * n + e + 1 + nbytes // 4, dtype=torch.int32, device=dev)  # with the scratch at its end
+    experts, position = whole[:2 * n].view(2, t, k).unbind()
+    pairs, rows = whole[2 * n:4 * n].view(2, n).unbind()
+    offsets = whole[4 * n:4 * n + e + 1]
+    at = whole.data_ptr()
+    _lib.call("fs_route", dev, logits.data_ptr(), _TYPES[logits.dtype], _ld(logits), t, e, k, _lib.ptr(bias), _lib.ptr(mask),
+              over_all, gates.data_ptr(), at, at + 16 * n, at + 8 * n, at + 12 * n, at + 4 * n, at + 16 * n + 4 * (e + 1), nbytes,
+              _lib.stream_ptr(dev))
+    return gates, experts, offsets, pairs, rows, position
 
 
 class _RouteFunction(torch.autograd.Function):
@@ -138,20 +154,23 @@ def route_tokens(logits: torch.Tensor, k: int, *, bias: Optional[torch.Tensor] =
         raise ValueError(f"k must be between 1 and {min(e, MAX_K)}, got {k}")
     if normalize not in ("selected", "all"):
         raise ValueError(f"normalize must be 'selected' or 'all', got {normalize!r}")
-    dev = _lib.require_cuda(logits=logits, bias=bias, mask=mask)
+    _device_of("logits", logits)
     if bias is not None:
+        _device_of("logits", logits, bias=bias)
         if bias.shape != (e,):
             raise ValueError(f"bias must have shape ({e},), got {tuple(bias.shape)}")
         if bias.requires_grad:
             raise ValueError("bias must not require grad (it only takes part in the choice)")
         bias = _lib.f32c(bias)
     if mask is not None:
+        _device_of("logits", logits, mask=mask)
         if mask.shape != (t,) or mask.dtype != torch.bool:
             raise ValueError(f"mask must be a bool tensor of shape ({t},), got {mask.dtype} {tuple(mask.shape)}")
         mask = mask.contiguous()
     if t * int(k) >= 1 << 31:
         raise ValueError("T * k must be below 2^31")
-    logits = _rows_of(logits)
+    if t and e:
+        logits = _rows_of(logits)
     if torch.is_grad_enabled() and logits.requires_grad:
         return Routing(*_RouteFunction.apply(logits, int(k), bias, mask, normalize == "all"))
     return Routing(*_route(logits, int(k), bias, mask, normalize == "all"))
@@ -165,9 +184,9 @@ def route_tokens(logits: torch.Tensor, k: int, *, bias: Optional[torch.Tensor] =
 def _loadable_rows(t: torch.Tensor) -> torch.Tensor:
     """``t [R, C]`` as the tensor loads of the products take it: rows a multiple of 16 bytes apart, the first one aligned to
     16 bytes; ``t`` itself, or a copy with padded rows."""
-    if t.stride(1) == 1 and t.stride(0) >= t.shape[1] and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0:
+    (ld, one), (r, c) = t.stride(), t.shape
+    if one == 1 and ld >= c and ld % 8 == 0 and t.data_ptr() % 16 == 0:
         return t
-    r, c = t.shape
     out = torch.empty((r, -(-c // 8) * 8), dtype=t.dtype, device=t.device)[:, :c]
     return out.copy_(t)
 
@@ -186,14 +205,14 @@ def _loadable_weights(w: torch.Tensor) -> torch.Tensor:
 
 def _mm(x, rows, count, w, offsets, transposed=False, dtype=None):
     """``[count, N]``: rows of x (through ``rows``, if given) times their expert's matrix, or its transpose."""
-    dev, (e, n, k) = x.device, w.shape
+    dev, (e, n, k), kind = x.device, w.shape, x.dtype
     x, w = _loadable_rows(x), _loadable_weights(w)
-    strides = w.stride()
+    se, sn, sk = w.stride()
     if transposed:
-        n, k, strides = k, n, (strides[0], strides[2], strides[1])
-    out = torch.empty((count, n), dtype=dtype or x.dtype, device=dev)
-    _lib.call("fs_grouped_mm", dev, _lib.ptr(x), _ld(x), x.shape[0], _lib.ptr(rows), count, _lib.ptr(w), *strides, e, n, k,
-              _lib.ptr(offsets), _lib.ptr(out), _TYPES[out.dtype], n, _TYPES[x.dtype], _lib.stream_ptr(dev))
+        n, k, sn, sk = k, n, sk, sn
+    out = torch.empty((count, n), dtype=dtype or kind, device=dev)
+    _lib.call("fs_grouped_mm", dev, x.data_ptr(), _ld(x), x.shape[0], _lib.ptr(rows), count, w.data_ptr(), se, sn, sk, e, n, k,
+              offsets.data_ptr(), out.data_ptr(), _TYPES[dtype or kind], n, _TYPES[kind], _lib.stream_ptr(dev))
     return out
 
 
@@ -253,14 +272,15 @@ def grouped_mm(x: torch.Tensor, weight: torch.Tensor, groups: Union[Routing, tor
     _check_type("x", x, (torch.float16, torch.bfloat16))
     if weight.dtype != x.dtype:
         raise ValueError(f"weight must be of the type of x ({x.dtype}), got {weight.dtype}")
-    dev = _lib.require_cuda(x=x, weight=weight)
+    dev = _device_of("x", x, weight=weight)
     e, n, k = weight.shape
     if x.shape[1] != k or k == 0 or n == 0:
         raise ValueError(f"x must have as many columns as weight ({k} > 0), got {x.shape[1]}; N must be > 0, got {n}")
     rows = position = None
     if isinstance(groups, Routing):
-        _check_routing(groups, dev)
-        offsets, count = groups.offsets, groups.pairs.shape[0]
+        _check_routing(groups, dev, "offsets", *(("rows", "position") if gather else ()))
+        offsets, (tokens, slots) = groups.offsets, groups.position.shape
+        count = tokens * slots
         if gather:
             rows, position = groups.rows, groups.position
     else:
@@ -268,9 +288,8 @@ def grouped_mm(x: torch.Tensor, weight: torch.Tensor, groups: Union[Routing, tor
             raise ValueError("gather needs a Routing")
         _check_offsets(groups, dev)
         offsets, count = groups, x.shape[0]
-    want = position.shape[0] if gather else count
-    if x.shape[0] != want:
-        raise ValueError(f"x must have {want} rows, got {x.shape[0]}")
+    if x.shape[0] != (tokens if gather else count):
+        raise ValueError(f"x must have {tokens if gather else count} rows, got {x.shape[0]}")
     if offsets.shape[0] != e + 1 or e > MAX_EXPERTS:
         raise ValueError(f"groups must have as many experts as weight ({e}, at most {MAX_EXPERTS}), got {offsets.shape[0] - 1}")
     x, weight = _loadable_rows(x), _loadable_weights(weight)
@@ -285,40 +304,41 @@ def grouped_mm(x: torch.Tensor, weight: torch.Tensor, groups: Union[Routing, tor
 
 
 def _act(u, gates, pairs, checkpoint):
-    dev, r, f = u.device, u.shape[0], u.shape[1] // 2
-    h = torch.empty((r, f), dtype=u.dtype, device=dev)
-    codes = scales = None
-    if checkpoint:
-        codes = torch.empty((r, 2 * f), dtype=torch.int8, device=dev)
-        scales = torch.empty((r, 2 * (-(-f // _BLOCK))), dtype=torch.uint8, device=dev)
-    _lib.call("fs_gated_act", dev, _lib.ptr(u), _TYPES[u.dtype], _ld(u), r, f, _lib.ptr(gates), _lib.ptr(pairs),
-              _lib.ptr(h), _lib.ptr(codes), _lib.ptr(scales), _lib.stream_ptr(dev))
-    return h, codes, scales
+    """The result, and with ``checkpoint`` one buffer with the codes ``[R, 2 F]`` and, behind them, their scales."""
+    dev, (r, f2), kind = u.device, u.shape, u.dtype
+    f = f2 // 2
+    h = torch.empty((r, f), dtype=kind, device=dev)
+    held = torch.empty(r * (f2 + 2 * (-(-f // _BLOCK))), dtype=torch.uint8, device=dev) if checkpoint else None
+    codes = _lib.ptr(held)
+    _lib.call("fs_gated_act", dev, u.data_ptr(), _TYPES[kind], _ld(u), r, f, _lib.ptr(gates), _lib.ptr(pairs), h.data_ptr(),
+              codes, codes and codes + r * f2, _lib.stream_ptr(dev))
+    return h, held
 
 
-def _act_grad(u, codes, scales, gates, pairs, position, dh, want_gates, want_h):
-    dev, (r, f) = dh.device, dh.shape
-    du = torch.empty((r, 2 * f), dtype=dh.dtype, device=dev)
+def _act_grad(u, held, gates, pairs, position, dh, want_gates, want_h):
+    dev, (r, f), kind = dh.device, dh.shape, dh.dtype
+    du = torch.empty((r, 2 * f), dtype=kind, device=dev)
     dgates = torch.empty_like(gates) if want_gates else None
-    h = torch.empty((r, f), dtype=dh.dtype, device=dev) if want_h else None
-    _lib.call("fs_gated_act_grad", dev, _lib.ptr(u), 0 if u is None else _ld(u), _lib.ptr(codes), _lib.ptr(scales),
-              _TYPES[dh.dtype], r, f, _lib.ptr(gates), _lib.ptr(pairs), _lib.ptr(position), _lib.ptr(dh), _ld(dh),
-              _lib.ptr(du), _lib.ptr(dgates), _lib.ptr(h), _lib.stream_ptr(dev))
+    h = torch.empty((r, f), dtype=kind, device=dev) if want_h else None
+    codes = _lib.ptr(held)
+    _lib.call("fs_gated_act_grad", dev, _lib.ptr(u), 0 if u is None else _ld(u), codes, codes and codes + 2 * r * f, _TYPES[kind], r, f,
+              _lib.ptr(gates), _lib.ptr(pairs), _lib.ptr(position), dh.data_ptr(), _ld(dh), du.data_ptr(), _lib.ptr(dgates),
+              _lib.ptr(h), _lib.stream_ptr(dev))
     return du, dgates, h
 
 
 class _GatedActFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, u, gates, pairs, position, checkpoint):
-        h, codes, scales = _act(u, gates, pairs, checkpoint)
-        ctx.save_for_backward(None if checkpoint else u, codes, scales, gates, pairs, position)
+        h, held = _act(u, gates, pairs, checkpoint)
+        ctx.save_for_backward(None if checkpoint else u, held, gates, pairs, position)
         return h
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dh):
-        u, codes, scales, gates, pairs, position = ctx.saved_tensors
-        du, dgates, _ = _act_grad(u, codes, scales, gates, pairs, position, _rows_of(dh), ctx.needs_input_grad[1], False)
+        u, held, gates, pairs, position = ctx.saved_tensors
+        du, dgates, _ = _act_grad(u, held, gates, pairs, position, _rows_of(dh), ctx.needs_input_grad[1], False)
         return du if ctx.needs_input_grad[0] else None, dgates, None, None, None
 
 
@@ -334,10 +354,10 @@ def gated_act(u: torch.Tensor, routing: Optional[Routing] = None, *, checkpoint:
     if u.ndim != 2 or u.shape[1] == 0 or u.shape[1] % 2:
         raise ValueError(f"u must be 2D [R, 2 F] with F > 0, got shape {tuple(u.shape)}")
     _check_type("u", u)
-    dev = _lib.require_cuda(u=u)
+    dev = _device_of("u", u)
     gates = pairs = position = None
     if routing is not None:
-        _check_routing(routing, dev)
+        _check_routing(routing, dev, "gates", "pairs", "position")
         gates, pairs, position = routing.gates, routing.pairs, routing.position
         if u.shape[0] != pairs.shape[0]:
             raise ValueError(f"u must have {pairs.shape[0]} rows, got {u.shape[0]}")
@@ -353,10 +373,10 @@ def gated_act(u: torch.Tensor, routing: Optional[Routing] = None, *, checkpoint:
 
 
 def _combine(o, gates, position, dtype=None):
-    dev, (t, k), d = o.device, position.shape, o.shape[1]
-    y = torch.empty((t, d), dtype=dtype or o.dtype, device=dev)
-    _lib.call("fs_combine", dev, _lib.ptr(o), _TYPES[o.dtype], _ld(o), o.shape[0], t, k, d, _lib.ptr(gates), _lib.ptr(position),
-              _lib.ptr(y), _TYPES[y.dtype], _lib.stream_ptr(dev))
+    dev, (t, k), (m, d), kind = o.device, position.shape, o.shape, o.dtype
+    y = torch.empty((t, d), dtype=dtype or kind, device=dev)
+    _lib.call("fs_combine", dev, o.data_ptr(), _TYPES[kind], _ld(o), m, t, k, d, _lib.ptr(gates), position.data_ptr(),
+              y.data_ptr(), _TYPES[dtype or kind], _lib.stream_ptr(dev))
     return y
 
 
@@ -391,7 +411,7 @@ def combine_rows(o: torch.Tensor, routing: Routing, *, weighted: bool = True) ->
     if o.ndim != 2 or o.shape[1] == 0:
         raise ValueError(f"o must be 2D [T * k, D] with D > 0, got shape {tuple(o.shape)}")
     _check_type("o", o)
-    _check_routing(routing, _lib.require_cuda(o=o))
+    _check_routing(routing, _device_of("o", o), "gates", "pairs", "position")
     if o.shape[0] != routing.pairs.shape[0]:
         raise ValueError(f"o must have {routing.pairs.shape[0]} rows, got {o.shape[0]}")
     if routing.position.shape[1] > MAX_K:
@@ -414,19 +434,19 @@ class _ExpertMlpFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_in, w_out, gates, offsets, pairs, rows, position, checkpoint):
         u = _mm(x, rows, pairs.shape[0], w_in, offsets)
-        h, codes, scales = _act(u, gates, pairs, checkpoint)
-        ctx.save_for_backward(x, w_in, w_out, gates, offsets, pairs, rows, position, None if checkpoint else u, codes, scales)
+        h, held = _act(u, gates, pairs, checkpoint)
+        ctx.save_for_backward(x, w_in, w_out, gates, offsets, pairs, rows, position, None if checkpoint else u, held)
         return _combine(_mm(h, None, pairs.shape[0], w_out, offsets), None, position)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, w_in, w_out, gates, offsets, pairs, rows, position, u, codes, scales = ctx.saved_tensors
+        x, w_in, w_out, gates, offsets, pairs, rows, position, u, held = ctx.saved_tensors
         need_x, need_in, need_out, need_gates = ctx.needs_input_grad[:4]
         dy, count = _loadable_rows(dy), pairs.shape[0]
         dy = _gather(dy, rows)  # for two products
         dh = _mm(dy, None, count, w_out, offsets, transposed=True)
-        du, dgates, h = _act_grad(u, codes, scales, gates, pairs, position, dh, need_gates, need_out)
+        du, dgates, h = _act_grad(u, held, gates, pairs, position, dh, need_gates, need_out)
         dx = _combine(_mm(du, None, count, w_in, offsets, transposed=True), None, position) if need_x else None
         dw_in = _wgrad(du, _gather(x, rows), offsets) if need_in else None
         dw_out = _wgrad(dy, h, offsets) if need_out else None
@@ -447,8 +467,7 @@ def expert_mlp(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, routing
     _check_type("x", x, (torch.float16, torch.bfloat16))
     if w_in.dtype != x.dtype or w_out.dtype != x.dtype:
         raise ValueError(f"w_in and w_out must be of the type of x ({x.dtype}), got {w_in.dtype} and {w_out.dtype}")
-    dev = _lib.require_cuda(x=x, w_in=w_in, w_out=w_out)
-    _check_routing(routing, dev)
+    _check_routing(routing, _device_of("x", x, w_in=w_in, w_out=w_out), "gates", "offsets", "pairs", "rows", "position")
     (t, d), e, f = x.shape, w_in.shape[0], w_out.shape[2]
     if w_in.shape != (e, 2 * f, d) or w_out.shape != (e, d, f) or d == 0 or f == 0:
         raise ValueError(f"w_in must be [E, 2 F, {d}] and w_out [E, {d}, F], got {tuple(w_in.shape)} and {tuple(w_out.shape)}")
