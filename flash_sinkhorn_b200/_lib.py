@@ -8,6 +8,8 @@ library is missing, or a call returns a non-zero status, an exception is raised.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 from ctypes import c_char_p, c_double, c_float, c_int, c_size_t, c_void_p
 from typing import Optional
@@ -187,6 +189,25 @@ def load() -> ctypes.CDLL:
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+_binding = None
+
+
+def torch_binding():
+    """The torch binding of the routed-experts operators (``lib/fs_torch.so``), attached to the loaded library."""
+    global _binding
+    if _binding is None:
+        path = os.path.join(os.path.dirname(_LIB_PATH), "fs_torch.so")
+        lib = load()
+        if not os.path.exists(path):
+            raise ImportError(f"fs_torch.so not found at {path}. Build it with `python -m flash_sinkhorn_b200.build_ext`.")
+        loader = importlib.machinery.ExtensionFileLoader("fs_torch", path)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("fs_torch", loader))
+        loader.exec_module(module)
+        module.attach({name: ctypes.cast(getattr(lib, name), c_void_p).value for name in module.entries()}, FlashSinkhornError)
+        _binding = module
+    return _binding
 
 
 def precision_id(allow_tf32: bool) -> int:

@@ -18,10 +18,21 @@ ACC = 2.0**-22
 FUN = 2.0**-19  # relative error of sigmoid and of the few products around it in fp32
 
 
+class Kernels:
+    """The public operators, and the kernels by themselves (leading underscore)."""
+
+    def __init__(self):
+        from flash_sinkhorn_b200 import _lib, experts
+        self.__dict__.update({name: getattr(experts, name) for name in experts.__all__})
+        raw = _lib.torch_binding()
+        self._mm = lambda x, rows, count, w, offsets, transposed=False, dtype=None: raw.mm(x, rows, count, w, offsets, transposed,
+                                                                                          dtype == FP32)
+        self._wgrad, self._gather, self._act, self._act_grad = raw.wgrad, raw.gather, raw.act, raw.act_grad
+
+
 @pytest.fixture(scope="module")
 def ex():
-    from flash_sinkhorn_b200 import experts
-    return experts
+    return Kernels()
 
 
 def gen(seed):
@@ -774,9 +785,28 @@ def test_refusals(ex):
         lambda: ex.combine_rows(x.double(), r), lambda: ex.combine_rows(cpu, r),
         lambda: ex.expert_mlp(x, w_in, w_out.half(), r), lambda: ex.expert_mlp(x[:5], w_in, w_out, r),
         lambda: ex.expert_mlp(x, w_in[:, :-2], w_out, r), lambda: ex.expert_mlp(x.float(), w_in.float(), w_out.float(), r),
+        lambda: ex.route_tokens(logits, 2, bias=torch.zeros(4)), lambda: ex.grouped_mm(x, w_in.cpu(), r, gather=True),
         lambda: ex.transport_bias(x, logits), lambda: ex.transport_bias(x[:0], w_in[0]),
     ]
     for i, call in enumerate(bad):
         with pytest.raises(ValueError):
             call()
             pytest.fail(f"call {i} was not refused")
+
+
+def test_gradients_are_not_differentiable_again(ex):
+    g = gen(76)
+    x, w_in, w_out, logits = layer(ex, g, 6, 64, 32, 4, 2)
+    x.requires_grad_(True)
+    y = ex.expert_mlp(x, w_in, w_out, ex.route_tokens(logits, 2))
+    (dx,) = torch.autograd.grad(y, (x,), torch.ones_like(y), create_graph=True)
+    assert torch.isfinite(dx).all()
+    with pytest.raises(RuntimeError, match="cannot be differentiated again"):
+        dx.float().sum().backward()
+
+
+def test_a_failed_call_raises_the_library_s_error(ex):
+    from flash_sinkhorn_b200 import _lib
+    x, w = torch.zeros(4, 8, dtype=BF16, device="cuda"), torch.zeros(2000, 8, 8, dtype=BF16, device="cuda")
+    with pytest.raises(_lib.FlashSinkhornError, match="FS_ERR_BAD_ARG"):
+        ex._mm(x, None, 4, w, torch.zeros(2001, dtype=torch.int32, device="cuda"))
