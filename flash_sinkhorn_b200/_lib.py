@@ -156,7 +156,7 @@ SIGNATURES = {
         c_int, [_P, _L, _P, _L, c_int, c_int, c_int, c_int, _P, _P, c_int, _P]),
     "fs_gated_act": (c_int, [_P, c_int, _L, c_int, c_int, _P, _P, _P, _P, _P, _P]),
     "fs_gated_act_grad": (c_int, [_P, _L, _P, _P, c_int, c_int, c_int, _P, _P, _P, _P, _L, _P, _P, _P, _P]),
-    "fs_combine": (c_int, [_P, c_int, _L, c_int, c_int, c_int, c_int, _P, _P, _P, c_int, _P]),
+    "fs_combine": (c_int, [_P, c_int, _L, c_int, c_int, c_int, c_int, _P, _P, _P, c_int, _L, _P]),
     "fs_combine_grad": (c_int, [_P, c_int, _L, c_int, c_int, c_int, _P, _P, _P, _P, _L, _P, _P, _P]),
 }
 

@@ -583,6 +583,7 @@ struct CombineArgs {
   const float* gates;  // null: weights of 1
   const int *position, *pairs;
   void* y;
+  long long ldy;
   const void* dy;
   long long lddy;
   void* d_o;
@@ -615,7 +616,7 @@ __global__ void __launch_bounds__(kActWarps * 32) combine_kernel(const CombineAr
           for (int i = 0; i < VEC; ++i) y[i] += wj * o[i];
         }
       }
-      if (c < a.D) store_f32<Y, VEC>(static_cast<Y*>(a.y) + (long long)t * a.D + c, y);
+      if (c < a.D) store_f32<Y, VEC>(static_cast<Y*>(a.y) + (long long)t * a.ldy + c, y);
     }
   }
 }
@@ -765,15 +766,15 @@ int fs_gated_act_grad(const void* u, long long ldu, const int8_t* codes, const u
 }
 
 int fs_combine(const void* o, int type, long long ldo, int M, int T, int k, int D, const float* gates, const int* position,
-               void* y, int y_type, void* stream) {
+               void* y, int y_type, long long ldy, void* stream) {
   int s = check_rows(type, T, D);
   if (s != FS_OK || T == 0) return s;
   if (k < 1 || k > kMaxK || (long long)T * k > 0x7fffffffll) return report_error(FS_ERR_BAD_ARG, "k must be in [1, 32], T * k below 2^31");
-  if (!o || M < 0 || !position || !y || ldo < D || y_type < 0 || y_type > 2 || (y_type != type && type != FS_TYPE_F32))
+  if (!o || M < 0 || !position || !y || ldo < D || ldy < D || y_type < 0 || y_type > 2 || (y_type != type && type != FS_TYPE_F32))
     return report_error(FS_ERR_BAD_ARG, "null argument, rows shorter than D, or a wrong type of the result");
   CombineArgs a{};
-  a.o = o; a.ldo = ldo; a.M = M; a.T = T; a.k = k; a.D = D; a.gates = gates; a.position = position; a.y = y;
-  return launch_combine(a, type, y_type, false, lane_values(D, type_bytes(type), ldo, 0, o, y), static_cast<cudaStream_t>(stream));
+  a.o = o; a.ldo = ldo; a.M = M; a.T = T; a.k = k; a.D = D; a.gates = gates; a.position = position; a.y = y; a.ldy = ldy;
+  return launch_combine(a, type, y_type, false, lane_values(D, type_bytes(type), ldo, ldy, o, y), static_cast<cudaStream_t>(stream));
 }
 
 int fs_combine_grad(const void* o, int type, long long ldo, int T, int k, int D, const float* gates, const int* position,

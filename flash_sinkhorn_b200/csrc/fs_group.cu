@@ -13,7 +13,9 @@
 //
 // One persistent CTA per SM, or a pair of CTAs on neighbouring SMs that share a 256 x 256 tile (each holds 128 features and
 // fetches half of the rows: two thirds of the bytes per product of 128 x 256 tiles). Warp 4 fetches whole tiles (TMA into a
-// ring of stages of 64 contraction values), warp 5 issues the products into one of two TMEM accumulators, warps 0 to 3
+// ring of stages of 64 contraction values), warp 5 issues the products into one of two TMEM accumulators (either by one
+// thread from beginning to end: choosing it anew for every instruction cost 500 clocks a stage, as much as the products of a
+// 256 x 256 tile), warps 0 to 3
 // write the other one out. Rows in another order are fetched by warps 7 to 10, 16 bytes a lane (cp.async): TMA's loads of
 // four rows each took 75 clocks apiece, 2.6 times the time of the whole product. Group boundaries are read by the kernel
 // itself; every CTA takes every n-th tile, features fastest, so that the CTAs working at one time share a group's weights
@@ -92,8 +94,10 @@ __device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, in
         "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
         ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
 }
-__device__ __forceinline__ void expect_cluster(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+template <int CG>
+__device__ __forceinline__ void expect_at(uint32_t bar, uint32_t bytes) {  // bar: in CTA 0 of the pair
+  if (CG == 2) asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+  else mbar_expect_tx(bar, bytes);
 }
 // 16 bytes, of which those past the first `valid` become zeros (the source is not read for them).
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int valid) {
@@ -181,7 +185,11 @@ struct Tiles {
       t.hi = gs[t.e + 1];
       t.blocks = (t.hi - t.lo + 63) / 64;
     } else {
-      while (tile >= ts[e + 1]) ++e;
+      for (int end = a.E; e < end;) {  // the first group from e on that ends behind the tile
+        const int mid = (e + end) / 2;
+        if (tile >= ts[mid + 1]) e = mid + 1;
+        else end = mid;
+      }
       const int rest = tile - ts[e], n = rest / mt;
       t.e = e;
       t.m0 = (rest - n * mt) * 128 * CG;
@@ -330,7 +338,8 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
   int *gs = reinterpret_cast<int*>(slot + 2), *ts = gs + a.E + 2;
   auto bar = [&](int i) { return smem_u32(bars + i); };
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // from a shuffle, so that the compiler knows the roles' branches to be uniform and keeps operands in uniform registers
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = CG == 2 ? (int)cta_rank() : 0;
   const int first = blockIdx.x / CG, stride = gridDim.x / CG;
 
@@ -367,7 +376,7 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
     int s = 0, issued = 0;
     uint32_t ph = 0;
     bool ok = true;
-    if (lane == 0) {
+    if (elect_one()) {
       for (int it = first; ok && it < total; it += stride) {
         const Tile t = tiles.at(it);
         const int npc = (t.cols + 16 * CG - 1) / (16 * CG) * 16;  // columns of the product that this CTA fetches
@@ -383,13 +392,13 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
             const bool open = kb == t.blocks - 1 && (t.hi - t.lo) % 16 != 0;
             const uint32_t to = open ? bar(PARTS + s) : full;
             if (open) mbar_expect_tx(to, kStage);
-            else expect_cluster(to, kStage);
+            else expect_at<CG>(to, kStage);
 #pragma unroll
             for (int c = 0; c < 2; ++c) load_2d<CG>(dst + c * kHalfTile, &mapA, m0 + c * 64, i0, to);
 #pragma unroll
             for (int c = 0; c < BNC / 64; ++c) load_2d<CG>(dst + kA + c * kHalfTile, &mapB, t.n0 + rank * npc + c * 64, i0, to);
           } else {
-            expect_cluster(full, kA + (COPY ? 0u : kB));
+            expect_at<CG>(full, kA + (COPY ? 0u : kB));
             if (FORM == ROWS_K) {
               load_3d<CG>(dst, &mapA, kb * 64, m0, t.e, full);
             } else {
@@ -412,7 +421,7 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
     }
   } else if (warp == 5) {
     // ===================== products =====================
-    if (rank == 0) {
+    if (rank == 0 && elect_one()) {
       const uint32_t type = a.type == FS_TYPE_BF16 ? 1u : 0u;
       const uint32_t idesc0 = (1u << 4) | (type << 7) | (type << 10) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) |
                               ((uint32_t)(128 * CG >> 4) << 24);
@@ -425,12 +434,12 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
         const int np = (t.cols + 16 * CG - 1) / (16 * CG) * (16 * CG);
         const uint32_t idesc = idesc0 | ((uint32_t)(np >> 3) << 17);
         const int buf = n & 1;
-        if (!__all_sync(0xffffffffu, mbar_wait(bar(ACC_EMPTY + buf), ((n >> 1) & 1) ^ 1, abort_flag))) break;
+        if (!mbar_wait(bar(ACC_EMPTY + buf), ((n >> 1) & 1) ^ 1, abort_flag)) break;
         ++n;
         tc_fence_after();
         const uint32_t d = tmem + buf * BN;
         for (int kb = 0; kb < t.blocks; ++kb) {
-          if (!__all_sync(0xffffffffu, mbar_wait(bar(FULL + s), ph, abort_flag))) {
+          if (!mbar_wait(bar(FULL + s), ph, abort_flag)) {
             ok = false;
             break;
           }
@@ -440,21 +449,18 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
           const int left = FORM == WEIGHTS ? t.hi - t.lo - kb * 64 : a.K - kb * 64;  // contraction values from here on
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks)
-            if (ks * 16 < left && elect_one())
-              mma_f16<CG>(d, pack_desc(al + ks * step_of(A_MN), kDescHi128), pack_desc(bl + ks * step_of(B_MN), kDescHi128), idesc,
-                          kb | ks);
-          if (elect_one()) commit<CG>(bar(EMPTY + s));
-          __syncwarp();
+            if (ks * 16 < left)
+              mma_f16<CG>(d, pack_desc(al + ks * step_of(A_MN), kDescHi128), pack_desc(bl + ks * step_of(B_MN), kDescHi128), idesc, kb | ks);
+          commit<CG>(bar(EMPTY + s));
           if (++s == a.nstage) {
             s = 0;
             ph ^= 1;
           }
         }
         if (!ok) break;
-        if (elect_one()) commit<CG>(bar(ACC_FULL + buf));
-        __syncwarp();
+        commit<CG>(bar(ACC_FULL + buf));
       }
-      if (*abort_flag && elect_one()) {  // every product issued here ends before TMEM is freed
+      if (*abort_flag) {  // every product issued here ends before TMEM is freed
         commit<CG>(bar(DRAIN));
         mbar_wait_quiet(bar(DRAIN), 0);
       }

@@ -154,15 +154,17 @@ std::vector<Tensor> route_raw(const Tensor& logits, int64_t k, const Tensor& bia
   return {gates, experts, offsets, pairs, rows, position};
 }
 
-Tensor combine_raw(const Tensor& o, const Tensor& gates, const Tensor& position, at::ScalarType type) {
+// pad: rows of the result a multiple of 8 values apart.
+Tensor combine_raw(const Tensor& o, const Tensor& gates, const Tensor& position, at::ScalarType type, bool pad = false) {
   const Place at(o);
-  const int64_t t = position.size(0), d = o.size(1);
-  Tensor y = at::empty({t, d}, o.options().dtype(type));
+  const int64_t t = position.size(0), d = o.size(1), ldy = pad ? (d + 7) / 8 * 8 : d;
+  Tensor y = at::empty({t, ldy}, o.options().dtype(type));
   FS_CALL(fs_combine, o.data_ptr(), type_of(o), ld(o), (int)o.size(0), (int)t, (int)position.size(1), (int)d, floats(gates), ints(position),
-          y.data_ptr(), type_of(y), at.stream);
-  return y;
+          y.data_ptr(), type_of(y), ldy, at.stream);
+  return pad ? y.narrow(1, 0, d) : y;
 }
-Tensor gather_raw(const Tensor& x, const Tensor& rows) { return combine_raw(rows_of(x), Tensor(), rows.view({-1, 1}), x.scalar_type()); }
+// x[rows] as the products take it, zeros for the rows of no pair.
+Tensor gather_raw(const Tensor& x, const Tensor& rows) { return combine_raw(rows_of(x), Tensor(), rows.view({-1, 1}), x.scalar_type(), true); }
 
 Tensor mm_raw(const Tensor& x0, const Tensor& rows, int64_t count, const Tensor& w0, const Tensor& offsets, bool transposed, bool fp32) {
   const Place at(x0);
@@ -216,13 +218,14 @@ std::tuple<Tensor, Tensor, Tensor> act_grad_raw(const Tensor& u, const Tensor& h
 
 // ------------------------------------------------------------------ autograd
 struct Route : torch::autograd::Function<Route> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& logits, int64_t k, const optional<Tensor>& bias0, const optional<Tensor>& mask0,
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits0, int64_t k, const optional<Tensor>& bias0, const optional<Tensor>& mask0,
                                bool over_all) {
-    const Tensor bias = none(bias0), mask = none(mask0);
+    const Tensor bias = none(bias0), mask = none(mask0), logits = rows_of(logits0);
     auto out = route_raw(logits, k, bias, mask, over_all);
     ctx->save_for_backward({logits, bias, mask, out[0], out[1]});
     ctx->saved_data["all"] = over_all;
     ctx->mark_non_differentiable({out[1], out[2], out[3], out[4], out[5]});
+    ctx->set_materialize_grads(false);  // five zero gradients of whole numbers
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -242,9 +245,9 @@ struct Route : torch::autograd::Function<Route> {
 };
 
 struct GroupedMm : torch::autograd::Function<GroupedMm> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& offsets, const optional<Tensor>& rows0,
+  static Tensor forward(AutogradContext* ctx, const Tensor& x0, const Tensor& w0, const Tensor& offsets, const optional<Tensor>& rows0,
                         const optional<Tensor>& position, int64_t count) {
-    const Tensor rows = none(rows0);
+    const Tensor x = loadable_rows(x0), w = loadable_weights(w0), rows = none(rows0);
     ctx->save_for_backward({x, w, offsets, rows, none(position)});
     return mm_raw(x, rows, count, w, offsets, false, false);
   }
@@ -268,9 +271,9 @@ struct GroupedMm : torch::autograd::Function<GroupedMm> {
 };
 
 struct GatedAct : torch::autograd::Function<GatedAct> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& u, const optional<Tensor>& gates0, const optional<Tensor>& pairs0,
+  static Tensor forward(AutogradContext* ctx, const Tensor& u0, const optional<Tensor>& gates0, const optional<Tensor>& pairs0,
                         const optional<Tensor>& position, bool checkpoint) {
-    const Tensor gates = none(gates0), pairs = none(pairs0);
+    const Tensor u = rows_of(u0), gates = none(gates0), pairs = none(pairs0);
     auto [h, held] = act_raw(u, gates, pairs, checkpoint);
     ctx->save_for_backward({checkpoint ? Tensor() : u, held, gates, pairs, none(position)});
     return h;
@@ -285,8 +288,8 @@ struct GatedAct : torch::autograd::Function<GatedAct> {
 };
 
 struct Combine : torch::autograd::Function<Combine> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& o, const optional<Tensor>& gates0, const Tensor& position, const Tensor& pairs) {
-    const Tensor gates = none(gates0);
+  static Tensor forward(AutogradContext* ctx, const Tensor& o0, const optional<Tensor>& gates0, const Tensor& position, const Tensor& pairs) {
+    const Tensor o = rows_of(o0), gates = none(gates0);
     const bool keep = gates.defined() && gates.requires_grad();
     ctx->save_for_backward({keep ? o : Tensor(), gates, position, pairs});
     return combine_raw(o, gates, position, o.scalar_type());
@@ -311,8 +314,9 @@ struct Combine : torch::autograd::Function<Combine> {
 // Keeps x, the routing and u (in 8 bits) from the forward pass. The gates are in the activation, so the backward pass needs
 // neither the experts' outputs nor their gradients: both of its products with the outer weights read dy.
 struct Mlp : torch::autograd::Function<Mlp> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w_in, const Tensor& w_out, const Tensor& gates, const Tensor& offsets,
+  static Tensor forward(AutogradContext* ctx, const Tensor& x0, const Tensor& w_in0, const Tensor& w_out0, const Tensor& gates, const Tensor& offsets,
                         const Tensor& pairs, const Tensor& rows, const Tensor& position, bool checkpoint) {
+    const Tensor x = loadable_rows(x0), w_in = loadable_weights(w_in0), w_out = loadable_weights(w_out0);
     const int64_t count = pairs.size(0);
     const Tensor u = mm_raw(x, rows, count, w_in, offsets, false, false);
     auto [h, held] = act_raw(u, gates, pairs, checkpoint);
@@ -360,8 +364,8 @@ std::vector<Tensor> route_tokens(const Tensor& logits0, int64_t k, const optiona
                       type_name(mask), " ", shape_of(mask));
     mask = mask.contiguous();
   }
-  const Tensor logits = rows_of(logits0);
-  return wants_grad({&logits}) ? Route::apply(logits, k, maybe(bias), maybe(mask), over_all) : route_raw(logits, k, bias, mask, over_all);
+  if (wants_grad({&logits0})) return Route::apply(logits0, k, maybe(bias), maybe(mask), over_all);
+  return route_raw(rows_of(logits0), k, bias, mask, over_all);
 }
 
 Tensor grouped_mm(const Tensor& x0, const Tensor& w0, const Tensor& offsets, const optional<Tensor>& rows0, const optional<Tensor>& position0,
@@ -394,7 +398,7 @@ Tensor grouped_mm(const Tensor& x0, const Tensor& w0, const Tensor& offsets, con
                     "), got ", offsets.size(0) - 1);
   require(count < (int64_t(1) << 31) && x0.size(0) < (int64_t(1) << 31), "rows must be fewer than 2^31");
   if (!wants_grad({&x0, &w0})) return mm_raw(x0, rows, count, w0, offsets, false, false);
-  return GroupedMm::apply(loadable_rows(x0), loadable_weights(w0), offsets, maybe(rows), maybe(position), count);
+  return GroupedMm::apply(x0, w0, offsets, maybe(rows), maybe(position), count);
 }
 
 Tensor gated_act(const Tensor& u0, const optional<Tensor>& gates0, const optional<Tensor>& pairs0, const optional<Tensor>& position0, bool checkpoint) {
@@ -409,9 +413,8 @@ Tensor gated_act(const Tensor& u0, const optional<Tensor>& gates0, const optiona
     require(u0.size(0) == pairs.size(0), "u must have ", pairs.size(0), " rows, got ", u0.size(0));
   }
   require(u0.size(0) < (int64_t(1) << 31), "rows must be fewer than 2^31");
-  const Tensor u = rows_of(u0);
-  if (!wants_grad({&u, &gates})) return act_raw(u, gates, pairs, false).first;
-  return GatedAct::apply(u, maybe(gates), maybe(pairs), maybe(position), checkpoint);
+  if (!wants_grad({&u0, &gates})) return act_raw(rows_of(u0), gates, pairs, false).first;
+  return GatedAct::apply(u0, maybe(gates), maybe(pairs), maybe(position), checkpoint);
 }
 
 Tensor combine_rows(const Tensor& o0, const Tensor& gates0, const Tensor& pairs, const Tensor& position, bool weighted) {
@@ -424,8 +427,9 @@ Tensor combine_rows(const Tensor& o0, const Tensor& gates0, const Tensor& pairs,
   require(o0.size(0) == pairs.size(0), "o must have ", pairs.size(0), " rows, got ", o0.size(0));
   require(position.size(1) <= kMaxK, "k must be at most ", kMaxK, ", got ", position.size(1));
   require(o0.size(0) < (int64_t(1) << 31), "rows must be fewer than 2^31");
-  const Tensor o = rows_of(o0), gates = weighted ? gates0 : Tensor();
-  return wants_grad({&o, &gates}) ? Combine::apply(o, maybe(gates), position, pairs) : combine_raw(o, gates, position, o.scalar_type());
+  const Tensor gates = weighted ? gates0 : Tensor();
+  if (wants_grad({&o0, &gates})) return Combine::apply(o0, maybe(gates), position, pairs);
+  return combine_raw(rows_of(o0), gates, position, o0.scalar_type());
 }
 
 Tensor expert_mlp(const Tensor& x0, const Tensor& w_in0, const Tensor& w_out0, const Tensor& gates, const Tensor& offsets, const Tensor& pairs,
@@ -447,11 +451,10 @@ Tensor expert_mlp(const Tensor& x0, const Tensor& w_in0, const Tensor& w_out0, c
                     "w_in must be [E, 2 F, ", d, "] and w_out [E, ", d, ", F], got ", shape_of(w_in0), " and ", shape_of(w_out0));
   require(position.size(0) == t && offsets.size(0) == e + 1 && position.size(1) <= kMaxK && e <= kMaxExperts && position.numel() < (int64_t(1) << 31),
                     "routing must be of ", t, " tokens and ", e, " experts (at most ", kMaxExperts, "), at most ", kMaxK, " for a token");
-  const Tensor x = loadable_rows(x0), w_in = loadable_weights(w_in0), w_out = loadable_weights(w_out0);
-  if (wants_grad({&x, &w_in, &w_out, &gates})) return Mlp::apply(x, w_in, w_out, gates, offsets, pairs, rows, position, checkpoint);
+  if (wants_grad({&x0, &w_in0, &w_out0, &gates})) return Mlp::apply(x0, w_in0, w_out0, gates, offsets, pairs, rows, position, checkpoint);
   const int64_t count = pairs.size(0);
-  const Tensor h = act_raw(mm_raw(x, rows, count, w_in, offsets, false, false), gates, pairs, false).first;
-  return combine_raw(mm_raw(h, Tensor(), count, w_out, offsets, false, false), Tensor(), position, x.scalar_type());
+  const Tensor h = act_raw(mm_raw(x0, rows, count, w_in0, offsets, false, false), gates, pairs, false).first;
+  return combine_raw(mm_raw(h, Tensor(), count, w_out0, offsets, false, false), Tensor(), position, x0.scalar_type());
 }
 
 }  // namespace

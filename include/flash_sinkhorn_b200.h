@@ -527,10 +527,10 @@ int fs_gated_act_grad(const void* u, long long ldu, const int8_t* codes, const u
                       float* dgates, void* h, void* stream);
 
 /* Rows back into tokens: y[t, :] = sum over the slots s with a row of gates[t, s] o[position[t, s], :] (gates null:
- * weights of 1; positions outside [0, M): no row). o has M rows of D values; y is T x D, densely packed, of the type of o
- * or, where that is FS_TYPE_F32, of any. With k = 1 and no gates it gathers rows. */
+ * weights of 1; positions outside [0, M): no row). o has M rows of D values; y is T x D, of the type of o or, where that
+ * is FS_TYPE_F32, of any. With k = 1 and no gates it gathers rows. */
 int fs_combine(const void* o, int type, long long ldo, int M, int T, int k, int D, const float* gates, const int* position,
-               void* y, int y_type, void* stream);
+               void* y, int y_type, long long ldy, void* stream);
 
 /* Its gradients, for M = T * k: d_o [T * k, D] densely packed, and dgates [T, k] (or null; then o may be null too). */
 int fs_combine_grad(const void* o, int type, long long ldo, int T, int k, int D, const float* gates, const int* position,
