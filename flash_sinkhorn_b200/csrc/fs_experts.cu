@@ -16,10 +16,11 @@ constexpr unsigned kAll = 0xffffffffu;
 // are on: logit and bias above -inf, token not masked. Its gates are the soft-max of the LOGITS over the chosen experts or
 // over all that are on. The (token, slot) pairs of an expert keep their order, so the result is the same in every run.
 //
-// One warp per token, expert j in lane j % 32. Two kernels of at most kMaxBlocks CTAs, CTA b with tokens [b c, (b + 1) c):
-// the first selects and counts the CTA's pairs per expert, the second adds up the counts of the CTAs before it (every CTA
-// for itself: E x kMaxBlocks words from L2, cheaper than a third launch or CTAs that wait for one another) and numbers
-// its own pairs. Batches of one CTA do both in one launch.
+// One warp per token, lane l with experts [l PER, (l + 1) PER): the k-fold choice is a maximum over each lane's own experts and
+// one over the lanes (redux), and the lowest of several lanes with the same score has the lowest expert. Two kernels of at
+// most kMaxBlocks CTAs, CTA b with tokens [b c, (b + 1) c): the first selects and counts the CTA's pairs per expert, the
+// second adds up the counts of the CTAs before it (every CTA for itself: E x kMaxBlocks words from L2, cheaper than a third
+// launch or CTAs that wait for one another) and numbers its own pairs. Batches of one CTA do both in one launch.
 
 constexpr int kRouteWarps = 16;
 constexpr int kMaxBlocks = 296;    // two CTAs on each of 148 SMs
@@ -33,6 +34,7 @@ struct RouteArgs {
   const float* bias;
   const uint8_t* mask;
   int over_all;
+  bool vec;
   float* gates;
   int *experts, *offsets, *pairs, *rows, *position;
   int* counts;  // [E, blocks]
@@ -55,86 +57,155 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 __device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kAll, v, o));
-  return v;
+  float m;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
 }
 
+// PER neighbouring values of a row of E; `fill` past its end. vec: they are aligned, and PER divides E.
 template <typename T, int PER>
-__device__ __forceinline__ void load_logits(const RouteArgs& a, int t, int lane, float (&l)[PER], bool (&on)[PER]) {
-  const T* row = static_cast<const T*>(a.logits) + (long long)t * a.ld;
-  const bool token_on = !a.mask || a.mask[t];
+__device__ __forceinline__ void load_part(const T* row, int lane, int E, bool vec, float fill, float (&v)[PER]) {
+  if (vec) {
+    if (lane * PER < E) {
+      load_f32<T, PER>(row + lane * PER, v);
+    } else {
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int j = i * 32 + lane;
-    l[i] = j < a.E ? to_f32(row[j]) : -INFINITY;
-    on[i] = token_on && l[i] != -INFINITY && (!a.bias || j >= a.E || a.bias[j] != -INFINITY);
+      for (int i = 0; i < PER; ++i) v[i] = fill;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) v[i] = lane * PER + i < E ? to_f32(row[lane * PER + i]) : fill;
   }
 }
-// Largest logit of the experts that are on, and the sum of exp(logit - largest) over them.
-template <int PER>
-__device__ __forceinline__ void soft_max_over(const float (&l)[PER], const bool (&on)[PER], float& top, float& sum) {
-  top = -INFINITY;
+// Logits of a token, -inf for the experts that are off.
+template <typename T, int PER>
+__device__ __forceinline__ void load_logits(const RouteArgs& a, int t, int lane, const float (&bias)[PER], float (&l)[PER]) {
+  load_part<T, PER>(static_cast<const T*>(a.logits) + (long long)t * a.ld, lane, a.E, a.vec, -INFINITY, l);
+  const bool on = !a.mask || a.mask[t];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) top = on[i] ? fmaxf(top, l[i]) : top;
-  top = warp_max(top);
-  sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) sum += on[i] ? expf(l[i] - top) : 0.f;
-  sum = warp_sum(sum);
+  for (int i = 0; i < PER; ++i) l[i] = on && bias[i] != -INFINITY ? l[i] : -INFINITY;
 }
+template <int PER>
+__device__ __forceinline__ void load_bias(const RouteArgs& a, int lane, float (&bias)[PER]) {
+#pragma unroll
+  for (int i = 0; i < PER; ++i) bias[i] = a.bias && lane * PER + i < a.E ? a.bias[lane * PER + i] : 0.f;
+}
+// Largest of the logits (-inf: none is on), and 1 / the sum of exp(logit - largest).
+template <int PER>
+__device__ __forceinline__ void soft_max_over(const float (&l)[PER], float& top, float& inv) {
+  top = l[0];
+#pragma unroll
+  for (int i = 1; i < PER; ++i) top = fmaxf(top, l[i]);
+  top = warp_max(top);
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) sum += expf(l[i] - top);
+  inv = 1.f / warp_sum(sum);
+}
+
+// The experts of a lane that are still to be had, best first on demand. Up to 8 are sorted once (Batcher's odd-even merge
+// network; equal keys by number), and taking the best is a shift; more are looked through anew after each one taken, which
+// costs less than a network of 16 inputs.
+template <int PER>
+struct Candidates {
+  static constexpr bool kSorted = PER <= 8;
+  unsigned key[PER];
+  int number[PER];  // sorted: expert of each key within the lane; else number[0] is that of the best
+  unsigned best;
+  __device__ __forceinline__ void look() {
+    best = 0u;
+    number[0] = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (key[i] > best) {
+        best = key[i];
+        number[0] = i;
+      }
+  }
+  __device__ __forceinline__ void prepare() {
+    if (!kSorted) {
+      look();
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) number[i] = i;
+#pragma unroll
+    for (int p = 1; p < PER; p *= 2)
+#pragma unroll
+      for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+        for (int j = k % p; j + k < PER; j += 2 * k)
+#pragma unroll
+          for (int i = j; i < j + k && i + k < PER; ++i)
+            if (i / (2 * p) == (i + k) / (2 * p)) {
+              const unsigned x = key[i], y = key[i + k];
+              const int nx = number[i], ny = number[i + k];
+              const bool swap = y > x || (y == x && ny < nx);
+              key[i] = swap ? y : x;
+              key[i + k] = swap ? x : y;
+              number[i] = swap ? ny : nx;
+              number[i + k] = swap ? nx : ny;
+            }
+    best = key[0];
+  }
+  __device__ __forceinline__ void take(bool mine) {
+    if (kSorted) {
+#pragma unroll
+      for (int i = 0; i + 1 < PER; ++i) {
+        key[i] = mine ? key[i + 1] : key[i];
+        number[i] = mine ? number[i + 1] : number[i];
+      }
+      key[PER - 1] = mine ? 0u : key[PER - 1];
+      best = key[0];
+    } else {
+      if (mine) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) key[i] = i == number[0] ? 0u : key[i];
+        look();
+      }
+      __syncwarp();
+    }
+  }
+};
 
 template <typename T, int PER>
 __device__ __forceinline__ void select_tokens(const RouteArgs& a, int* count) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int t0 = blockIdx.x * a.chunk, t1 = min(t0 + a.chunk, a.T);
+  float bias[PER], next[PER];
+  load_bias<PER>(a, lane, bias);
+  constexpr bool kEarly = PER <= 8;  // the next token's logits are on their way while this one's experts are chosen
+  if (kEarly && t0 + warp < t1) load_logits<T, PER>(a, t0 + warp, lane, bias, next);
   for (int t = t0 + warp; t < t1; t += kRouteWarps) {
-    float l[PER];
-    bool on[PER];
-    load_logits<T, PER>(a, t, lane, l, on);
-    unsigned key[PER];
+    float l[PER], top, inv;
+    if (kEarly) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int j = i * 32 + lane;
-      key[i] = on[i] ? score_key(a.bias ? l[i] + a.bias[j] : l[i]) : 0u;
-    }
-    int expert = -1;       // of slot `lane`
-    float chosen = 0.f;    // its logit
-    for (int s = 0; s < a.k; ++s) {
-      unsigned best = key[0];
-#pragma unroll
-      for (int i = 1; i < PER; ++i) best = max(best, key[i]);
-      best = __reduce_max_sync(kAll, best);
-      if (best == 0u) break;
-      int at = 0x7fffffff;
-#pragma unroll
-      for (int i = PER - 1; i >= 0; --i) at = key[i] == best ? i * 32 + lane : at;
-      at = __reduce_min_sync(kAll, at);
-      float mine = 0.f;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        if (i == at >> 5) {
-          mine = l[i];
-          if (lane == (at & 31)) key[i] = 0u;
-        }
-      }
-      mine = __shfl_sync(kAll, mine, at & 31);
-      if (lane == s) {
-        expert = at;
-        chosen = mine;
-      }
-    }
-    float top, sum;
-    if (a.over_all) {
-      soft_max_over<PER>(l, on, top, sum);
+      for (int i = 0; i < PER; ++i) l[i] = next[i];
+      if (t + kRouteWarps < t1) load_logits<T, PER>(a, t + kRouteWarps, lane, bias, next);
     } else {
+      load_logits<T, PER>(a, t, lane, bias, l);
+    }
+    Candidates<PER> left;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) left.key[i] = l[i] != -INFINITY ? score_key(l[i] + bias[i]) : 0u;
+    left.prepare();
+    if (a.over_all) soft_max_over<PER>(l, top, inv);
+    int expert = -1;  // of slot `lane`
+    for (int s = 0; s < a.k; ++s) {
+      const unsigned best = __reduce_max_sync(kAll, left.best);
+      if (best == 0u) break;
+      const int owner = __ffs(__ballot_sync(kAll, left.best == best)) - 1, j = owner * PER + __shfl_sync(kAll, left.number[0], owner);
+      expert = lane == s ? j : expert;
+      left.take(lane == owner);
+    }
+    const float chosen = expert >= 0 ? to_f32(static_cast<const T*>(a.logits)[(long long)t * a.ld + expert]) : -INFINITY;
+    if (!a.over_all) {
       const float one[1] = {chosen};
-      const bool has[1] = {expert >= 0};
-      soft_max_over<1>(one, has, top, sum);
+      soft_max_over<1>(one, top, inv);
     }
     if (lane < a.k) {
       const long long p = (long long)t * a.k + lane;
-      a.gates[p] = expert >= 0 ? expf(chosen - top) / sum : 0.f;
+      a.gates[p] = expert >= 0 ? expf(chosen - top) * inv : 0.f;
       a.experts[p] = expert;
       if (expert >= 0) atomicAdd(count + expert, 1);
     }
@@ -168,48 +239,77 @@ __device__ __forceinline__ int scan_in_place(int* v, int n, int* scratch) {
   return base;
 }
 
+// The pairs of a warp, in order; the experts of the first kEarlyPairs x 32 of them are read ahead.
+constexpr int kEarlyPairs = 4;
+struct WarpPairs {
+  long long begin, end;
+  int early[kEarlyPairs];
+  __device__ __forceinline__ WarpPairs(const RouteArgs& a) {
+    const int warp = threadIdx.x >> 5;
+    const long long p0 = (long long)blockIdx.x * a.chunk * a.k, p1 = min((long long)a.T, (long long)(blockIdx.x + 1) * a.chunk) * a.k;
+    const long long share = ((p1 - p0 + kRouteWarps - 1) / kRouteWarps + 31) / 32 * 32;
+    begin = p0 + warp * share;
+    end = min(p1, begin + share);
+  }
+  __device__ __forceinline__ void read(const RouteArgs& a, long long from) {
+#pragma unroll
+    for (int i = 0; i < kEarlyPairs; ++i) {
+      const long long p = from + i * 32 + (threadIdx.x & 31);
+      early[i] = p < end ? a.experts[p] : -1;
+    }
+  }
+};
+
 // Rows of this CTA's pairs. first[e]: row of its first pair of expert e. hist: [kRouteWarps, E].
-__device__ __forceinline__ void number_pairs(const RouteArgs& a, int* first, int* hist, int total) {
+__device__ __forceinline__ void number_pairs(const RouteArgs& a, WarpPairs& w, int* first, int* hist, int total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int j = threadIdx.x; j < kRouteWarps * a.E; j += kRouteWarps * 32) hist[j] = 0;
   __syncthreads();
-  const long long p0 = (long long)blockIdx.x * a.chunk * a.k;
-  const long long p1 = min((long long)a.T, (long long)(blockIdx.x + 1) * a.chunk) * a.k;
-  const long long share = ((p1 - p0 + kRouteWarps - 1) / kRouteWarps + 31) / 32 * 32;  // pairs of a warp, in order
-  const long long w0 = p0 + warp * share, w1 = min(p1, w0 + share);
   int* mine = hist + warp * a.E;
-  for (long long p = w0 + lane; p - lane < w1; p += 32) {
-    const int e = p < w1 ? a.experts[p] : -1;
-    const unsigned same = __match_any_sync(kAll, e);
-    if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
-    __syncwarp();
-  }
-  __syncthreads();
-  for (int e = threadIdx.x; e < a.E; e += kRouteWarps * 32) {
-    int at = first[e];
+  constexpr int kRound = kEarlyPairs * 32;
+  for (long long from = w.begin; from < w.end; from += kRound) {
+    if (from > w.begin) w.read(a, from);
 #pragma unroll
-    for (int w = 0; w < kRouteWarps; ++w) {
-      const int c = hist[w * a.E + e];
-      hist[w * a.E + e] = at;
-      at += c;
+    for (int i = 0; i < kEarlyPairs; ++i) {
+      const int e = w.early[i];
+      const unsigned same = __match_any_sync(kAll, e);
+      if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
+      __syncwarp();
     }
   }
   __syncthreads();
-  for (long long p = w0 + lane; p - lane < w1; p += 32) {
-    const int e = p < w1 ? a.experts[p] : -1;
-    const unsigned same = __match_any_sync(kAll, e);
-    const int rank = __popc(same & ((1u << lane) - 1u));
-    const int at = e >= 0 ? mine[e] + rank : -1;
-    __syncwarp();
-    if (e >= 0 && rank == 0) mine[e] += __popc(same);
-    __syncwarp();
-    if (p < w1) {
-      a.position[p] = at;
-      if (at >= 0) {
-        a.pairs[at] = (int)p;
-        a.rows[at] = (int)(p / a.k);
+  for (int e = threadIdx.x; e < a.E; e += kRouteWarps * 32) {
+    int at = first[e], c[kRouteWarps];
+#pragma unroll
+    for (int j = 0; j < kRouteWarps; ++j) c[j] = hist[j * a.E + e];
+#pragma unroll
+    for (int j = 0; j < kRouteWarps; ++j) {
+      hist[j * a.E + e] = at;
+      at += c[j];
+    }
+  }
+  __syncthreads();
+  const bool again = w.end - w.begin > kRound;
+  for (long long from = w.begin; from < w.end; from += kRound) {
+    if (again) w.read(a, from);
+#pragma unroll
+    for (int i = 0; i < kEarlyPairs; ++i) {
+      const int e = w.early[i];
+      const long long p = from + i * 32 + lane;
+      const unsigned same = __match_any_sync(kAll, e);
+      const int rank = __popc(same & ((1u << lane) - 1u));
+      const int at = e >= 0 ? mine[e] + rank : -1;
+      __syncwarp();
+      if (e >= 0 && rank == 0) mine[e] += __popc(same);
+      __syncwarp();
+      if (p < w.end) {
+        a.position[p] = at;
+        if (at >= 0) {
+          a.pairs[at] = (int)p;
+          a.rows[at] = (int)((unsigned)p / (unsigned)a.k);
+        }
+        if (p >= total) a.pairs[p] = a.rows[p] = -1;  // rows after the last one that is routed
       }
-      if (p >= total) a.pairs[p] = a.rows[p] = -1;  // rows after the last one that is routed
     }
   }
 }
@@ -231,27 +331,37 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_select_kernel(const Ro
   __syncthreads();
   for (int e = threadIdx.x; e < a.E; e += kRouteWarps * 32) a.offsets[e] = count[e];
   if (threadIdx.x == 0) a.offsets[a.E] = total;
-  number_pairs(a, count, sm + a.E, total);
+  WarpPairs pairs(a);
+  pairs.read(a, pairs.begin);
+  number_pairs(a, pairs, count, sm + a.E, total);
 }
 
 __global__ void __launch_bounds__(kRouteWarps * 32) route_order_kernel(const RouteArgs a) {
   extern __shared__ int sm[];
   __shared__ int scratch[kRouteWarps];
   int *all = sm, *before = sm + a.E;  // pairs of expert e in all CTAs, in the CTAs before this one
+  WarpPairs pairs(a);
+  pairs.read(a, pairs.begin);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int e = warp; e < a.E; e += kRouteWarps) {
-    int n = 0, b = 0;
+  constexpr int kSide = 4;  // experts that a warp adds up side by side, so that its loads are in flight together
+  for (int e0 = warp * kSide; e0 < a.E; e0 += kRouteWarps * kSide) {
+    int n[kSide] = {}, b[kSide] = {};
 #pragma unroll 4
-    for (int c = lane; c < a.blocks; c += 32) {
-      const int v = a.counts[e * a.blocks + c];
-      n += v;
-      b += c < (int)blockIdx.x ? v : 0;
-    }
-    n = __reduce_add_sync(kAll, n);
-    b = __reduce_add_sync(kAll, b);
-    if (lane == 0) {
-      all[e] = n;
-      before[e] = b;
+    for (int c = lane; c < a.blocks; c += 32)
+#pragma unroll
+      for (int i = 0; i < kSide; ++i) {
+        const int v = e0 + i < a.E ? a.counts[(e0 + i) * a.blocks + c] : 0;
+        n[i] += v;
+        b[i] += c < (int)blockIdx.x ? v : 0;
+      }
+#pragma unroll
+    for (int i = 0; i < kSide; ++i) {
+      n[i] = __reduce_add_sync(kAll, n[i]);
+      b[i] = __reduce_add_sync(kAll, b[i]);
+      if (lane == 0 && e0 + i < a.E) {
+        all[e0 + i] = n[i];
+        before[e0 + i] = b[i];
+      }
     }
   }
   __syncthreads();
@@ -262,13 +372,18 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_order_kernel(const Rou
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) a.offsets[a.E] = total;
   __syncthreads();
-  number_pairs(a, before, sm + 2 * a.E, total);
+  number_pairs(a, pairs, before, sm + 2 * a.E, total);
 }
 
-// d logit_j = [j chosen as slot s] g_s dg_s - p_j sum_s g_s dg_s, p = the soft-max that the gates were taken from.
+// d logit_j = [j chosen as slot s] g_s dg_s - p_j sum_s g_s dg_s, p = the soft-max that the gates were taken from. The chosen
+// experts' terms are added in a row of shared memory (E floats of every warp).
 template <typename T, int PER>
 __global__ void __launch_bounds__(kRouteWarps * 32) route_grad_kernel(const RouteArgs a) {
+  extern __shared__ float rows[];
   const int lane = threadIdx.x & 31;
+  float* row = rows + (threadIdx.x >> 5) * (32 * PER);
+  float bias[PER];
+  load_bias<PER>(a, lane, bias);
   for (long long t = (long long)blockIdx.x * kRouteWarps + (threadIdx.x >> 5); t < a.T; t += (long long)gridDim.x * kRouteWarps) {
     const long long p = t * a.k + lane;
     const int expert = lane < a.k ? a.experts_in[p] : -1;
@@ -276,27 +391,29 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_grad_kernel(const Rout
     const float own = expert >= 0 ? gate * a.grad[p] : 0.f, inner = warp_sum(own);
     float v[PER];
     if (a.over_all) {
-      float l[PER], top, sum;
-      bool on[PER];
-      load_logits<T, PER>(a, (int)t, lane, l, on);
-      soft_max_over<PER>(l, on, top, sum);
+      float l[PER], top, inv;
+      load_logits<T, PER>(a, (int)t, lane, bias, l);
+      soft_max_over<PER>(l, top, inv);
 #pragma unroll
-      for (int i = 0; i < PER; ++i) v[i] = on[i] ? -inner * (expf(l[i] - top) / sum) : 0.f;
+      for (int i = 0; i < PER; ++i) v[i] = l[i] != -INFINITY ? -inner * (expf(l[i] - top) * inv) : 0.f;
     } else {
 #pragma unroll
       for (int i = 0; i < PER; ++i) v[i] = 0.f;
     }
-    const float add = a.over_all ? own : own - gate * inner;
-    for (int s = 0; s < a.k; ++s) {
-      const int e = __shfl_sync(kAll, expert, s);
-      const float g = __shfl_sync(kAll, add, s);
+    __syncwarp();
+    store_f32<float, PER>(row + lane * PER, v);
+    __syncwarp();
+    if (expert >= 0 && expert < a.E) row[expert] += a.over_all ? own : own - gate * inner;
+    __syncwarp();
+    load_f32<float, PER>(row + lane * PER, v);
+    T* out = static_cast<T*>(a.out) + t * a.E + lane * PER;
+    if (a.vec) {
+      if (lane * PER < a.E) store_f32<T, PER>(out, v);
+    } else {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) v[i] += e == i * 32 + lane ? g : 0.f;
+      for (int i = 0; i < PER; ++i)
+        if (lane * PER + i < a.E) out[i] = from_f32<T>(v[i]);
     }
-    T* row = static_cast<T*>(a.out) + t * a.E;
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (i * 32 + lane < a.E) row[i * 32 + lane] = from_f32<T>(v[i]);
   }
 }
 
@@ -317,10 +434,15 @@ int allow_smem(K kernel, size_t bytes) {
 }
 
 template <typename T, int PER>
-int launch_route(const RouteArgs& a, bool grad, cudaStream_t st) {
+int launch_route(RouteArgs a, bool grad, cudaStream_t st) {
+  const size_t part = sizeof(T) * PER < 16 ? sizeof(T) * PER : 16;
+  a.vec = a.E % PER == 0 && a.ld % PER == 0 && aligned(a.logits, part) && aligned(a.out, part);
   if (grad) {
     const long long want = ((long long)a.T + kRouteWarps - 1) / kRouteWarps;
-    route_grad_kernel<T, PER><<<(int)(want < 592 ? want : 592), kRouteWarps * 32, 0, st>>>(a);
+    const size_t bytes = (size_t)kRouteWarps * 32 * PER * 4;
+    const int s = allow_smem(route_grad_kernel<T, PER>, bytes);
+    if (s != FS_OK) return s;
+    route_grad_kernel<T, PER><<<(int)(want < 592 ? want : 592), kRouteWarps * 32, bytes, st>>>(a);
     return launched(1);
   }
   const size_t one = (size_t)(a.blocks > 1 ? 1 : 1 + kRouteWarps) * a.E * 4, two = (size_t)(2 + kRouteWarps) * a.E * 4;
@@ -397,6 +519,14 @@ __device__ __forceinline__ unsigned block_exponent(unsigned amax_bits) {
 __device__ __forceinline__ float block_scale(unsigned code) {
   return code == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(code << 23);
 }
+// Integers of at most 2^22 in magnitude and floats by way of an addition: 1.5 * 2^23 + x holds the nearest integer (ties to
+// even) in its low bits, and a byte under the exponent of 2^23 is 2^23 plus its value. The conversion instructions have a
+// sixteenth of the rate, which exp and the reciprocal of the sigmoid already take up.
+constexpr float kToInt = 12582912.f;       // 1.5 * 2^23
+constexpr float kFromByte = 8388608.f;     // 2^23
+__device__ __forceinline__ uint32_t four_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {  // the lowest byte of each
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
 // Codes of this lane's values (whole warps; 32 / VEC lanes hold a block); the exponent code of the block comes back.
 template <int VEC>
 __device__ __forceinline__ unsigned encode(const float (&x)[VEC], int8_t (&q)[VEC]) {
@@ -406,10 +536,42 @@ __device__ __forceinline__ unsigned encode(const float (&x)[VEC], int8_t (&q)[VE
 #pragma unroll
   for (int o = 16 / VEC; o; o >>= 1) top = max(top, __shfl_xor_sync(kAll, top, o));
   const unsigned code = block_exponent(top);
-  const float inv = code == 255u ? 0.f : __uint_as_float((254u - code) << 23);
+  const float inv = code == 255u ? 0.f : __uint_as_float((254u - code) << 23);  // infinities and NaN times 0: not looked at
+  uint32_t n[VEC];
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) q[i] = code == 255u ? (int8_t)0 : (int8_t)__float2int_rn(x[i] * inv);
+  for (int i = 0; i < VEC; ++i) n[i] = __float_as_uint(fmaf(x[i], inv, kToInt));
+  if (VEC % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i + 3 < VEC; i += 4) {
+      const uint32_t w = four_bytes(n[i], n[i + 1], n[i + 2], n[i + 3]);
+      q[i] = (int8_t)w;
+      q[i + 1] = (int8_t)(w >> 8);
+      q[i + 2] = (int8_t)(w >> 16);
+      q[i + 3] = (int8_t)(w >> 24);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) q[i] = (int8_t)n[i];
+  }
   return code;
+}
+// The values that codes stand for: code * scale, as (2^23 + 128 + code) * scale - (2^23 + 128) * scale with one exact rounding.
+template <int VEC>
+__device__ __forceinline__ void decode(const int8_t* codes, float scale, float (&x)[VEC]) {
+  const float off = -(kFromByte + 128.f) * scale;
+  uint32_t w[VEC / 4 ? VEC / 4 : 1];
+  if (VEC == 8) {
+    const uint2 v = *reinterpret_cast<const uint2*>(codes);
+    w[0] = v.x;
+    w[VEC / 8] = v.y;
+  } else if (VEC == 4) {
+    w[0] = *reinterpret_cast<const uint32_t*>(codes);
+  } else {
+    w[0] = (uint8_t)*codes;
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i)
+    x[i] = fmaf(__uint_as_float(__byte_perm(w[i / 4] ^ 0x80808080u, 0x4b000000u, 0x7440u + (unsigned)(i % 4))), scale, off);
 }
 
 __device__ __forceinline__ float row_gate(const ActArgs& a, int r, bool& routed) {
@@ -488,14 +650,8 @@ __global__ void __launch_bounds__(kActWarps * 32) act_grad_kernel(const ActArgs 
         if (CODES) {
           const int8_t* codes = a.codes + (long long)r * 2 * a.F + c;
           const uint8_t* sc = a.scales + (long long)r * 2 * nb + c / 32;
-          const Pack<int8_t, VEC> qg = *reinterpret_cast<const Pack<int8_t, VEC>*>(codes);
-          const Pack<int8_t, VEC> qv = *reinterpret_cast<const Pack<int8_t, VEC>*>(codes + a.F);
-          const float sg = block_scale(sc[0]), sv = block_scale(sc[nb]);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            g[i] = sg * (float)qg.v[i];
-            v[i] = sv * (float)qv.v[i];
-          }
+          decode<VEC>(codes, block_scale(sc[0]), g);
+          decode<VEC>(codes + a.F, block_scale(sc[nb]), v);
         } else {
           const T* row = static_cast<const T*>(a.u) + (long long)r * a.ldu + c;
           load_f32<T, VEC>(row, g);
