@@ -2,6 +2,10 @@
 // with its 8-bit checkpoint, and the sum of the experts' rows back into tokens. All of it is bound by memory traffic (the
 // routing of a large batch by instruction issue); every value is read once and nothing is kept between calls.
 #include "fs_experts.cuh"
+#include "fs_tc.cuh"
+
+#include <algorithm>
+#include <cstring>
 
 namespace fs {
 namespace ex {
@@ -488,8 +492,7 @@ int check_route(const void* logits, int type, long long ld, int T, int E, int k)
 // scaling by a power of two is exact the codes do not depend on how the quotient is rounded. A block with an infinity or
 // a NaN has exponent code 255 and stands for NaN throughout.
 //
-// A warp per row (or per part of a row, where there are few), VEC values of each half per lane and step: 16-byte loads for
-// 16-bit types. 32 / VEC neighbouring lanes share a block.
+// VEC values of each half per lane: 16-byte loads for 16-bit types. 32 / VEC neighbouring lanes share a block.
 
 constexpr int kActWarps = 8;
 
@@ -527,48 +530,57 @@ constexpr float kFromByte = 8388608.f;     // 2^23
 __device__ __forceinline__ uint32_t four_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {  // the lowest byte of each
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
-// Codes of this lane's values (whole warps; 32 / VEC lanes hold a block); the exponent code of the block comes back.
-template <int VEC>
-__device__ __forceinline__ unsigned encode(const float (&x)[VEC], int8_t (&q)[VEC]) {
+// fp32 bits of the largest magnitude of the lane's values and those of its neighbours in the block (whole warps; 32 / VEC
+// lanes hold a block). 16-bit types compare pairs of bit patterns.
+template <typename T, int VEC>
+__device__ __forceinline__ unsigned block_maximum(const Pack<T, VEC>& q) {
   unsigned top = 0u;
+  if constexpr (sizeof(T) == 2 && VEC % 2 == 0) {
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+    for (int i = 0; i < VEC / 2; ++i) top = __vmaxu2(top, q.w[i] & 0x7fff7fffu);
 #pragma unroll
-  for (int o = 16 / VEC; o; o >>= 1) top = max(top, __shfl_xor_sync(kAll, top, o));
-  const unsigned code = block_exponent(top);
+    for (int o = 16 / VEC; o; o >>= 1) top = __vmaxu2(top, __shfl_xor_sync(kAll, top, o));
+    const unsigned short bits = (unsigned short)max(top & 0xffffu, top >> 16);
+    T value;
+    memcpy(&value, &bits, 2);
+    return __float_as_uint(to_f32(value));
+  } else {
+    float x[VEC];
+    unpack<T, VEC>(q, x);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = 16 / VEC; o; o >>= 1) top = max(top, __shfl_xor_sync(kAll, top, o));
+    return top;
+  }
+}
+// Codes of VEC values under an exponent code, as bytes.
+template <int VEC>
+struct alignas(VEC) Codes {
+  uint8_t b[VEC];
+};
+template <int VEC>
+__device__ __forceinline__ Codes<VEC> encode(const float (&x)[VEC], unsigned code) {
   const float inv = code == 255u ? 0.f : __uint_as_float((254u - code) << 23);  // infinities and NaN times 0: not looked at
-  uint32_t n[VEC];
+  uint32_t n[VEC], w[(VEC + 3) / 4];
 #pragma unroll
   for (int i = 0; i < VEC; ++i) n[i] = __float_as_uint(fmaf(x[i], inv, kToInt));
-  if (VEC % 4 == 0) {
+  if constexpr (VEC % 4 == 0) {
 #pragma unroll
-    for (int i = 0; i + 3 < VEC; i += 4) {
-      const uint32_t w = four_bytes(n[i], n[i + 1], n[i + 2], n[i + 3]);
-      q[i] = (int8_t)w;
-      q[i + 1] = (int8_t)(w >> 8);
-      q[i + 2] = (int8_t)(w >> 16);
-      q[i + 3] = (int8_t)(w >> 24);
-    }
+    for (int i = 0; i < VEC; i += 4) w[i / 4] = four_bytes(n[i], n[i + 1], n[i + 2], n[i + 3]);
   } else {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) q[i] = (int8_t)n[i];
+    w[0] = n[0];
   }
-  return code;
+  Codes<VEC> q;
+  memcpy(&q, w, VEC);
+  return q;
 }
 // The values that codes stand for: code * scale, as (2^23 + 128 + code) * scale - (2^23 + 128) * scale with one exact rounding.
 template <int VEC>
-__device__ __forceinline__ void decode(const int8_t* codes, float scale, float (&x)[VEC]) {
+__device__ __forceinline__ void decode(const Codes<VEC>& codes, float scale, float (&x)[VEC]) {
   const float off = -(kFromByte + 128.f) * scale;
-  uint32_t w[VEC / 4 ? VEC / 4 : 1];
-  if (VEC == 8) {
-    const uint2 v = *reinterpret_cast<const uint2*>(codes);
-    w[0] = v.x;
-    w[VEC / 8] = v.y;
-  } else if (VEC == 4) {
-    w[0] = *reinterpret_cast<const uint32_t*>(codes);
-  } else {
-    w[0] = (uint8_t)*codes;
-  }
+  uint32_t w[(VEC + 3) / 4] = {};
+  memcpy(w, &codes, VEC);
 #pragma unroll
   for (int i = 0; i < VEC; ++i)
     x[i] = fmaf(__uint_as_float(__byte_perm(w[i / 4] ^ 0x80808080u, 0x4b000000u, 0x7440u + (unsigned)(i % 4))), scale, off);
@@ -581,51 +593,55 @@ __device__ __forceinline__ float row_gate(const ActArgs& a, int r, bool& routed)
   routed = p >= 0 && p < a.R;  // as many pairs as rows
   return routed ? a.gates[p] : 0.f;
 }
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
-
+// 1 / (1 + 2^(-x log2 e)), to about 2^-21; 0 where the power overflows. The instructions by themselves, with results below
+// the normal range flushed: the intrinsics spend as much again on those.
+__device__ __forceinline__ float sigmoid(float x) {
+  float e, s;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
+  return s;
+}
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kActWarps * 32) act_kernel(const ActArgs a) {
+__device__ __forceinline__ Pack<T, VEC> read_pack(const T* p, bool in) {
+  if (in) return *reinterpret_cast<const Pack<T, VEC>*>(p);
+  Pack<T, VEC> q;
+  memset(&q, 0, sizeof(q));
+  return q;
+}
+// A warp per row, or per part of a row where there are few.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kActWarps * 32, 4) act_kernel(const ActArgs a) {
   const int lane = threadIdx.x & 31;
-  constexpr int kLanes = 32 / VEC;  // of a block
-  const int steps = (a.F + 32 * VEC - 1) / (32 * VEC), share = (steps + a.parts - 1) / a.parts;
-  const int nb = (a.F + 31) / 32;
-  const long long items = (long long)a.R * a.parts;
-  for (long long it = (long long)blockIdx.x * kActWarps + (threadIdx.x >> 5); it < items; it += (long long)gridDim.x * kActWarps) {
-    const int r = (int)(it / a.parts), s0 = (int)(it - (long long)r * a.parts) * share, s1 = min(s0 + share, steps);
-    bool routed;
-    const float p = row_gate(a, r, routed);
-    const T* row = static_cast<const T*>(a.u) + (long long)r * a.ldu;
-    T* out = static_cast<T*>(a.h) + (long long)r * a.F;
-#pragma unroll 2
-    for (int s = s0; s < s1; ++s) {
-      const int c = (s * 32 + lane) * VEC;
-      const bool in = c < a.F;
-      float g[VEC], v[VEC], h[VEC];
+  constexpr int kLanes = 32 / VEC;  // of a block of the checkpoint
+  const int steps = (a.F + 32 * VEC - 1) / (32 * VEC), share = (steps + a.parts - 1) / a.parts, nb = (a.F + 31) / 32;
+  const long long it = (long long)blockIdx.x * kActWarps + (threadIdx.x >> 5), r = a.parts == 1 ? it : it / a.parts;
+  if (r >= a.R) return;
+  const int s0 = a.parts == 1 ? 0 : (int)(it - r * a.parts) * share, end = min(a.F, (s0 + share) * 32 * VEC);
+  bool routed;
+  const float p = row_gate(a, (int)r, routed);
+  const T* row = static_cast<const T*>(a.u) + r * a.ldu;
+  T* out = static_cast<T*>(a.h) + r * a.F;
+  uint8_t* codes = a.codes && routed ? reinterpret_cast<uint8_t*>(a.codes) + r * 2 * a.F : nullptr;
+  uint8_t* scales = a.scales + r * 2 * nb;
+  for (int c = (s0 * 32 + lane) * VEC; c - lane * VEC < end; c += 32 * VEC) {
+    const bool in = c < a.F;
+    const Pack<T, VEC> qg = read_pack<T, VEC>(row + c, in), qv = read_pack<T, VEC>(row + a.F + c, in);
+    float g[VEC], v[VEC], h[VEC];
+    unpack<T, VEC>(qg, g);
+    unpack<T, VEC>(qv, v);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) g[i] = v[i] = h[i] = 0.f;
-      if (routed) {
-        if (in) {
-          load_f32<T, VEC>(row + c, g);
-          load_f32<T, VEC>(row + a.F + c, v);
-        }
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) h[i] = p * (g[i] * sigmoid(g[i])) * v[i];
-        if (a.codes) {
-          Pack<int8_t, VEC> q[2];
-          const unsigned eg = encode<VEC>(g, q[0].v), ev = encode<VEC>(v, q[1].v);
-          if (in) {
-            int8_t* codes = a.codes + (long long)r * 2 * a.F + c;
-            *reinterpret_cast<Pack<int8_t, VEC>*>(codes) = q[0];
-            *reinterpret_cast<Pack<int8_t, VEC>*>(codes + a.F) = q[1];
-            if (lane % kLanes == 0) {
-              uint8_t* sc = a.scales + (long long)r * 2 * nb + c / 32;
-              sc[0] = (uint8_t)eg;
-              sc[nb] = (uint8_t)ev;
-            }
-          }
+    for (int i = 0; i < VEC; ++i) h[i] = routed ? p * (g[i] * sigmoid(g[i])) * v[i] : 0.f;
+    if (in) store_f32<T, VEC>(out + c, h);
+    if (codes) {
+      const unsigned eg = block_exponent(block_maximum<T, VEC>(qg)), ev = block_exponent(block_maximum<T, VEC>(qv));
+      if (in) {
+        *reinterpret_cast<Codes<VEC>*>(codes + c) = encode<VEC>(g, eg);
+        *reinterpret_cast<Codes<VEC>*>(codes + a.F + c) = encode<VEC>(v, ev);
+        if (lane % kLanes == 0) {
+          scales[c / 32] = (uint8_t)eg;
+          scales[nb + c / 32] = (uint8_t)ev;
         }
       }
-      if (in) store_f32<T, VEC>(out + c, h);
     }
   }
 }
@@ -633,50 +649,45 @@ __global__ void __launch_bounds__(kActWarps * 32) act_kernel(const ActArgs a) {
 // du = [p dh v s (1 + g (1 - s)) | p dh g s] with s = sigmoid(g), and d p = sum dh g s v, from the checkpoint (CODES) or
 // from u as it was. One warp per row: the sum over the row stays in the warp.
 template <typename T, int VEC, bool CODES>
-__global__ void __launch_bounds__(kActWarps * 32) act_grad_kernel(const ActArgs a) {
+__global__ void __launch_bounds__(kActWarps * 32, 4) act_grad_kernel(const ActArgs a) {
   const int lane = threadIdx.x & 31, nb = (a.F + 31) / 32;
-  for (int r = blockIdx.x * kActWarps + (threadIdx.x >> 5); r < a.R; r += gridDim.x * kActWarps) {
-    bool routed;
-    const float p = row_gate(a, r, routed);
-    T *du = static_cast<T*>(a.du) + (long long)r * 2 * a.F, *hr = a.h ? static_cast<T*>(a.h) + (long long)r * a.F : nullptr;
-    float dp = 0.f;
-#pragma unroll 2
-    for (int c = lane * VEC; c < a.F; c += 32 * VEC) {
-      float dg[VEC], dv[VEC], h[VEC];
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) dg[i] = dv[i] = h[i] = 0.f;
-      if (routed) {
-        float g[VEC], v[VEC], d[VEC];
-        if (CODES) {
-          const int8_t* codes = a.codes + (long long)r * 2 * a.F + c;
-          const uint8_t* sc = a.scales + (long long)r * 2 * nb + c / 32;
-          decode<VEC>(codes, block_scale(sc[0]), g);
-          decode<VEC>(codes + a.F, block_scale(sc[nb]), v);
-        } else {
-          const T* row = static_cast<const T*>(a.u) + (long long)r * a.ldu + c;
-          load_f32<T, VEC>(row, g);
-          load_f32<T, VEC>(row + a.F, v);
-        }
-        load_f32<T, VEC>(static_cast<const T*>(a.dh) + (long long)r * a.lddh + c, d);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float s = sigmoid(g[i]), gs = g[i] * s, pd = p * d[i];
-          dv[i] = pd * gs;
-          dg[i] = pd * v[i] * (s + gs * (1.f - s));
-          dp += d[i] * gs * v[i];
-          h[i] = p * gs * v[i];
-        }
-      }
-      store_f32<T, VEC>(du + c, dg);
-      store_f32<T, VEC>(du + a.F + c, dv);
-      if (hr) store_f32<T, VEC>(hr + c, h);
+  const long long r = (long long)blockIdx.x * kActWarps + (threadIdx.x >> 5);
+  if (r >= a.R) return;
+  bool routed;
+  const float p = row_gate(a, (int)r, routed);
+  const uint8_t *codes = reinterpret_cast<const uint8_t*>(a.codes) + r * 2 * a.F, *scales = a.scales + r * 2 * nb;
+  const T *row = static_cast<const T*>(a.u) + r * a.ldu, *dh = static_cast<const T*>(a.dh) + r * a.lddh;
+  T *du = static_cast<T*>(a.du) + r * 2 * a.F, *hr = a.h ? static_cast<T*>(a.h) + r * a.F : nullptr;
+  float dp = 0.f;
+  for (int c = lane * VEC; c < a.F; c += 32 * VEC) {
+    float g[VEC], v[VEC], d[VEC], dg[VEC], dv[VEC], h[VEC];
+    load_f32<T, VEC>(dh + c, d);
+    if (CODES) {
+      const Codes<VEC> cg = *reinterpret_cast<const Codes<VEC>*>(codes + c), cv = *reinterpret_cast<const Codes<VEC>*>(codes + a.F + c);
+      const unsigned eg = scales[c / 32], ev = scales[nb + c / 32];
+      decode<VEC>(cg, block_scale(eg), g);
+      decode<VEC>(cv, block_scale(ev), v);
+    } else {
+      load_f32<T, VEC>(row + c, g);
+      load_f32<T, VEC>(row + a.F + c, v);
     }
-    if (a.dgates) {
-      dp = warp_sum(dp);
-      if (lane == 0) {
-        if (routed) a.dgates[a.pairs[r]] = dp;
-        if (a.position[r] < 0) a.dgates[r] = 0.f;  // r as a pair: one that has no row
-      }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const float s = sigmoid(g[i]), gs = g[i] * s, dgs = d[i] * gs;
+      dv[i] = routed ? p * dgs : 0.f;
+      dg[i] = routed ? p * d[i] * v[i] * fmaf(gs, 1.f - s, s) : 0.f;
+      h[i] = routed ? p * gs * v[i] : 0.f;
+      dp = fmaf(dgs, v[i], dp);
+    }
+    store_f32<T, VEC>(du + c, dg);
+    store_f32<T, VEC>(du + a.F + c, dv);
+    if (hr) store_f32<T, VEC>(hr + c, h);
+  }
+  if (a.dgates) {
+    dp = warp_sum(dp);
+    if (lane == 0) {
+      if (routed) a.dgates[a.pairs[r]] = dp;
+      if (a.position[r] < 0) a.dgates[r] = 0.f;  // r as a pair: one that has no row
     }
   }
 }
@@ -704,14 +715,12 @@ int row_blocks(long long items) {
 
 template <typename T, int VEC>
 int launch_act(ActArgs a, bool grad, cudaStream_t st) {
-  if (!grad) {
-    a.parts = row_parts(a.R, a.F, VEC);
-    act_kernel<T, VEC><<<row_blocks((long long)a.R * a.parts), kActWarps * 32, 0, st>>>(a);
-  } else if (a.codes) {
-    act_grad_kernel<T, VEC, true><<<row_blocks(a.R), kActWarps * 32, 0, st>>>(a);
-  } else {
-    act_grad_kernel<T, VEC, false><<<row_blocks(a.R), kActWarps * 32, 0, st>>>(a);
-  }
+  a.parts = grad ? 1 : row_parts(a.R, a.F, VEC);
+  const long long warps = (long long)a.R * a.parts;
+  const int blocks = (int)((warps + kActWarps - 1) / kActWarps);
+  if (!grad) act_kernel<T, VEC><<<blocks, kActWarps * 32, 0, st>>>(a);
+  else if (a.codes) act_grad_kernel<T, VEC, true><<<blocks, kActWarps * 32, 0, st>>>(a);
+  else act_grad_kernel<T, VEC, false><<<blocks, kActWarps * 32, 0, st>>>(a);
   return launched(1);
 }
 template <typename T>

@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/flash_sinkhorn_b200.h"
 
 namespace fs {
@@ -28,21 +30,60 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 // N consecutive values as one load or store of up to 16 bytes each; the pointer is aligned to N values (at most 16 bytes).
+// Held as 32-bit words (two 16-bit values each): as an array of values each would take a register.
 template <typename T, int N>
 struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Pack {
-  T v[N];
+  static constexpr bool kWords = N * sizeof(T) % 4 == 0;
+  static constexpr int kCount = kWords ? (int)(N * sizeof(T) / 4) : N;
+  typename std::conditional<kWords, uint32_t, T>::type w[kCount];
 };
+__device__ __forceinline__ void two_f32(uint32_t w, float& lo, float& hi, __nv_bfloat16) {
+  lo = __uint_as_float(w << 16);
+  hi = __uint_as_float(w & 0xffff0000u);
+}
+__device__ __forceinline__ void two_f32(uint32_t w, float& lo, float& hi, __half) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  lo = f.x;
+  hi = f.y;
+}
+__device__ __forceinline__ uint32_t from_two(float lo, float hi, __nv_bfloat16) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+__device__ __forceinline__ uint32_t from_two(float lo, float hi, __half) {
+  const __half2 p = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+template <typename T, int N>
+__device__ __forceinline__ void unpack(const Pack<T, N>& q, float (&out)[N]) {
+  if constexpr (!Pack<T, N>::kWords) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = to_f32(q.w[i]);
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = __uint_as_float(q.w[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) two_f32(q.w[i], out[2 * i], out[2 * i + 1], T());
+  }
+}
 template <typename T, int N>
 __device__ __forceinline__ void load_f32(const T* p, float (&out)[N]) {
-  const Pack<T, N> q = *reinterpret_cast<const Pack<T, N>*>(p);
-#pragma unroll
-  for (int i = 0; i < N; ++i) out[i] = to_f32(q.v[i]);
+  unpack<T, N>(*reinterpret_cast<const Pack<T, N>*>(p), out);
 }
 template <typename T, int N>
 __device__ __forceinline__ void store_f32(T* p, const float (&in)[N]) {
   Pack<T, N> q;
+  if constexpr (!Pack<T, N>::kWords) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) q.v[i] = from_f32<T>(in[i]);
+    for (int i = 0; i < N; ++i) q.w[i] = from_f32<T>(in[i]);
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) q.w[i] = __float_as_uint(in[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) q.w[i] = from_two(in[2 * i], in[2 * i + 1], T());
+  }
   *reinterpret_cast<Pack<T, N>*>(p) = q;
 }
 

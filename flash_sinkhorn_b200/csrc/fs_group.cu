@@ -237,12 +237,7 @@ __device__ void read_groups(const GroupArgs& a, int* gs, int* ts, int per_column
 }
 
 __device__ __forceinline__ uint32_t pack_two(float lo, float hi, int type) {
-  if (type == FS_TYPE_BF16) {
-    const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&p);
-  }
-  const __half2 p = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&p);
+  return type == FS_TYPE_BF16 ? from_two(lo, hi, __nv_bfloat16()) : from_two(lo, hi, __half());
 }
 
 // 32 lanes x 32 columns of an accumulator as 16-bit values into a warp's staging tile of 32 rows of 64 bytes, whose 16-byte
@@ -617,6 +612,109 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
   if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_group_error, 1);
 }
 
+// ------------------------------------------------------------------ few rows
+// A single token: the products of one or two rows are bound by reading their experts' weights, and tiles of 128 features put
+// a token's two experts of 2048 features on 32 of 148 SMs. Here a warp takes one feature of one expert, its lanes 16 bytes of
+// it at a time and four of these at once; the sums are fp32 in a fixed order. Two rows of two experts, 2048 x 2048: 4.7 us
+// against 10.4 us with tiles (1.2 us of either are the launch); four rows of four experts 14.8 us against 11.3 us, so
+// these go the other way.
+constexpr int kFewRows = 2;  // rows of a call that go this way
+constexpr int kFewWarps = 8;
+
+// sums[r] of the rows x[r] (null: none) with the feature w.
+template <typename T, int ROWS>
+__device__ __forceinline__ void few_rows_dot(const T* w, const T* const (&x)[ROWS], int K, int lane, float (&sums)[ROWS]) {
+  constexpr int kDeep = 4;
+  const int chunks = K / 8;
+#pragma unroll 1
+  for (int c0 = lane; c0 < chunks; c0 += 32 * kDeep) {
+    Pack<T, 8> q[kDeep], p[kDeep][ROWS];
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d) {
+      const int c = c0 + 32 * d;
+      if (c < chunks) q[d] = *reinterpret_cast<const Pack<T, 8>*>(w + c * 8);
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r)
+        if (c < chunks && x[r]) p[d][r] = *reinterpret_cast<const Pack<T, 8>*>(x[r] + c * 8);
+    }
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d) {
+      float a[8], b[8];
+      unpack<T, 8>(q[d], a);
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        unpack<T, 8>(p[d][r], b);
+        if (c0 + 32 * d < chunks && x[r])
+#pragma unroll
+          for (int j = 0; j < 8; ++j) sums[r] = fmaf(a[j], b[j], sums[r]);
+      }
+    }
+  }
+  if (lane < K % 8)  // values after the last 16 bytes
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+      if (x[r]) sums[r] = fmaf(to_f32(w[chunks * 8 + lane]), to_f32(x[r][chunks * 8 + lane]), sums[r]);
+}
+
+template <typename T, int ROWS>  // rows of the call, 1 or 2
+__global__ void __launch_bounds__(32 * kFewWarps, 4) few_rows_kernel(const GroupArgs a, const T* w, long long w_expert, long long w_row) {
+  __shared__ int first_after[2];
+  const int lane = threadIdx.x & 31, i = blockIdx.y;
+  // The expert of row i is the one before the first offset above i (offsets as their running maximum); a row whose
+  // predecessor has the same one is left to the CTA of the expert's first row.
+  if (threadIdx.x < 2) first_after[threadIdx.x] = a.E + 1;
+  __syncthreads();
+  int above = a.E + 1, reached = a.E + 1;  // first offset above row i, above row i - 1
+  for (int j = 1 + threadIdx.x; j <= a.E; j += 32 * kFewWarps) {
+    const int v = a.offsets[j];
+    if (v > i) above = min(above, j);
+    if (v >= i) reached = min(reached, j);
+  }
+  above = __reduce_min_sync(0xffffffffu, above);
+  reached = __reduce_min_sync(0xffffffffu, reached);
+  if (lane == 0) {
+    atomicMin(&first_after[0], above);
+    atomicMin(&first_after[1], reached);
+  }
+  __syncthreads();
+  const int e = first_after[0] - 1;
+  const int f = blockIdx.x * kFewWarps + (threadIdx.x >> 5);
+  if (f >= a.N) return;
+  auto store = [&](int row, float v) {
+    const long long at = (long long)row * a.ldo + f;
+    if (a.out_type == FS_TYPE_F32) static_cast<float*>(a.out)[at] = v;
+    else static_cast<T*>(a.out)[at] = from_f32<T>(v);
+  };
+  if (e == a.E) {  // a row of no expert
+    if (lane == 0) store(i, 0.f);
+    return;
+  }
+  if (i > 0 && first_after[1] == first_after[0]) return;
+  const int end = min(a.offsets[e + 1], a.R);
+  const T* x[ROWS];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const int n = i + r < end ? (a.rows ? a.rows[i + r] : i + r) : -1;
+    x[r] = (unsigned)n < (unsigned)a.M ? static_cast<const T*>(a.x) + n * a.ldx : nullptr;
+  }
+  float sums[ROWS] = {};
+  few_rows_dot<T, ROWS>(w + e * w_expert + f * w_row, x, a.K, lane, sums);
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sums[r] += __shfl_xor_sync(0xffffffffu, sums[r], o);
+    if (lane == r && i + r < end) store(i + r, sums[r]);
+  }
+}
+template <typename T>
+int launch_few(const GroupArgs& a, const void* w, long long w_expert, long long w_row, cudaStream_t st) {
+  const dim3 grid((a.N + kFewWarps - 1) / kFewWarps, a.R);
+  const T* wt = static_cast<const T*>(w);
+  if (a.R == 1) few_rows_kernel<T, 1><<<grid, 32 * kFewWarps, 0, st>>>(a, wt, w_expert, w_row);
+  else few_rows_kernel<T, 2><<<grid, 32 * kFewWarps, 0, st>>>(a, wt, w_expert, w_row);
+  return launched(1);
+}
+
 // ------------------------------------------------------------------ host side
 PFN_cuTensorMapEncodeTiled_v12000 encoder() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
@@ -752,10 +850,13 @@ int fs_grouped_mm(const void* x, long long ldx, int M, const int* rows, int R, c
   a.offsets = offsets; a.rows = rows; a.M = M; a.R = R; a.E = E; a.N = N; a.K = K;
   a.out = out; a.ldo = ldo; a.type = type; a.out_type = out_type; a.x = x; a.ldx = ldx;
   a.out_vec = store_values(out, ldo, N);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (R <= kFewRows && k_major) {
+    return type == FS_TYPE_F16 ? launch_few<__half>(a, w, w_expert, w_row, st) : launch_few<__nv_bfloat16>(a, w, w_expert, w_row, st);
+  }
   CUtensorMap mapA = {};
   if (!encode(&mapA, type, w, 3, {k_major ? K : N, k_major ? N : K, E}, {w_ld, w_expert ? w_expert : w_ld}, k_major ? 128 : 64))
     return no_map();
-  const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int mean = R / E;
   if (mean >= 96 && N > 128) return launch_rows<2, 256>(a, k_major, mapA, st);
   if (mean >= 48) return launch_rows<1, 128>(a, k_major, mapA, st);
