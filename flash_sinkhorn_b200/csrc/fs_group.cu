@@ -12,14 +12,13 @@
 // meets a zero.
 //
 // One persistent CTA per SM, or a pair of CTAs on neighbouring SMs that share a 256 x 256 tile (each holds 128 features and
-// fetches half of the rows: two thirds of the bytes per product of 128 x 256 tiles). Warp 4 fetches whole tiles (TMA into a
-// ring of stages of 64 contraction values), warp 5 issues the products into one of two TMEM accumulators (either by one
+// fetches half of the rows: two thirds of the bytes per product of 128 x 256 tiles). One warp fetches whole tiles (TMA into a
+// ring of stages of 64 contraction values), one issues the products into one of two TMEM accumulators (either by one
 // thread from beginning to end: choosing it anew for every instruction cost 500 clocks a stage, as much as the products of a
-// 256 x 256 tile), warps 0 to 3
-// write the other one out. Rows in another order are fetched by warps 7 to 10, 16 bytes a lane (cp.async): TMA's loads of
-// four rows each took 75 clocks apiece, 2.6 times the time of the whole product. Group boundaries are read by the kernel
-// itself; every CTA takes every n-th tile, features fastest, so that the CTAs working at one time share a group's weights
-// and rows in L2.
+// 256 x 256 tile), and eight write the other one out, through shared memory in pieces of 64 bytes. Rows in another order are
+// fetched by four more, 16 bytes a lane (cp.async): TMA's loads of four rows each took 75 clocks apiece, 2.6 times the time
+// of the whole product. Group boundaries are read by the kernel itself; every CTA takes every n-th tile, features fastest,
+// so that the CTAs working at one time share a group's weights and rows in L2.
 #include "fs_experts.cuh"
 #include "fs_ptx.cuh"
 #include "fs_tc.cuh"
@@ -38,6 +37,10 @@ __device__ int g_group_error = 0;  // non-zero once a bounded wait gave up (read
 
 enum Form { ROWS_K, ROWS_MN, WEIGHTS };  // rows with W contiguous along the contraction; along the features
 
+// Warps: 0 to kOutWarps - 1 write results, then one each for whole tiles, products and reports, then the copying ones.
+constexpr int kOutWarps = 8, kLoadWarp = kOutWarps, kMmaWarp = kOutWarps + 1, kReportWarp = kOutWarps + 2;
+constexpr int kThreads = 32 * (kOutWarps + 3);
+constexpr int kStaging = 2048 * kOutWarps;
 constexpr int kCopyWarps = 4;              // warps that fetch single rows
 constexpr int kCopyRows = 4 * kCopyWarps;  // rows that they fetch 128 bytes of at a time
 constexpr uint32_t kHalfTile = 64 * 128;  // 64 rows of 128 bytes
@@ -245,29 +248,29 @@ __device__ __forceinline__ uint32_t pack_two(float lo, float hi, int type) {
 __device__ __forceinline__ uint32_t staged(uint32_t base, int row, int chunk) {
   return base + row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
 }
-template <bool FLIP>
-__device__ __forceinline__ void stage_block(uint32_t tmem, uint32_t base, int lane, int type) {
+// The accumulator's values as the tensor core's fragments: of 16 TMEM lanes (h) and 8 columns (i), a lane holds columns
+// 2 (lane % 4) and the next one of rows lane / 4 (g = 0) and lane / 4 + 8 (g = 1), in r[16 h + 4 i + 2 g].
+__device__ __forceinline__ void read_block(uint32_t tmem, uint32_t (&r)[32]) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {  // 16 lanes of TMEM at a time
-    uint32_t r[16];
+  for (int h = 0; h < 2; ++h)
     asm volatile(
         "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "=r"(r[16 * h]), "=r"(r[16 * h + 1]), "=r"(r[16 * h + 2]), "=r"(r[16 * h + 3]), "=r"(r[16 * h + 4]), "=r"(r[16 * h + 5]),
+          "=r"(r[16 * h + 6]), "=r"(r[16 * h + 7]), "=r"(r[16 * h + 8]), "=r"(r[16 * h + 9]), "=r"(r[16 * h + 10]),
+          "=r"(r[16 * h + 11]), "=r"(r[16 * h + 12]), "=r"(r[16 * h + 13]), "=r"(r[16 * h + 14]), "=r"(r[16 * h + 15])
         : "r"(tmem + ((uint32_t)(16 * h) << 16))
         : "memory");
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
-                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-                 :
-                 : "memory");
-    // a lane holds columns 8 i + 2 (lane % 4) and the next one of rows lane / 4 (g = 0) and lane / 4 + 8 (g = 1)
+}
+template <bool FLIP>
+__device__ __forceinline__ void stage_block(const uint32_t (&r)[32], uint32_t base, int lane, int type) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       uint32_t m[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        m[i] = pack_two(__uint_as_float(r[4 * i + 2 * g]), __uint_as_float(r[4 * i + 2 * g + 1]), type);
+        m[i] = pack_two(__uint_as_float(r[16 * h + 4 * i + 2 * g]), __uint_as_float(r[16 * h + 4 * i + 2 * g + 1]), type);
       if (FLIP)
         asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(staged(base, lane, 2 * h + g)),
                      "r"(m[0]), "r"(m[1]), "r"(m[2]), "r"(m[3])
@@ -277,7 +280,6 @@ __device__ __forceinline__ void stage_block(uint32_t tmem, uint32_t base, int la
                      ::"r"(staged(base, 16 * h + 8 * g + (lane & 7), lane >> 3)), "r"(m[0]), "r"(m[1]), "r"(m[2]), "r"(m[3])
                      : "memory");
     }
-  }
 }
 // rows x cols values (at most 32 x 32) of the staging tile, or zeros, to out, rows ld values apart.
 __device__ __forceinline__ void write_block(uint16_t* out, long long ld, int rows, int cols, int vec, bool zero, uint32_t base, int lane) {
@@ -316,7 +318,7 @@ __device__ __forceinline__ int load_early(const int* p) {
 
 // COPY (rows form): the rows come one by one.
 template <int FORM, int CG, int BN, bool COPY>
-__global__ void __launch_bounds__(224 + (COPY ? 32 * kCopyWarps : 0), 1)
+__global__ void __launch_bounds__(kThreads + (COPY ? 32 * kCopyWarps : 0), 1)
 group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB) {
   constexpr int BNC = BN / CG;                         // columns whose operand this CTA fetches
   constexpr uint32_t kA = 2 * kHalfTile, kB = BNC * 128, kStage = kA + kB;
@@ -325,8 +327,8 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
   static_assert(kColumns >= 32 && kColumns <= 512 && kStage % 1024 == 0 && !(COPY && FORM == WEIGHTS), "tile");
   extern __shared__ uint8_t raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* staging = ring + (size_t)a.nstage * kStage;  // 2 KB for each of warps 0 to 3
-  uint64_t* bars = reinterpret_cast<uint64_t*>(staging + 8192);
+  uint8_t* staging = ring + (size_t)a.nstage * kStage;  // 2 KB for each warp that writes results
+  uint64_t* bars = reinterpret_cast<uint64_t*>(staging + kStaging);
   const int FULL = 0, EMPTY = a.nstage, PARTS = 2 * a.nstage, ACC_FULL = 3 * a.nstage, ACC_EMPTY = ACC_FULL + 2, DRAIN = ACC_EMPTY + 2;
   uint32_t* slot = reinterpret_cast<uint32_t*>(bars + DRAIN + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(slot + 1);
@@ -340,21 +342,21 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
 
   if (warp == 0) {
     read_groups<FORM != WEIGHTS>(a, gs, ts, (a.N + 128 * CG - 1) / (128 * CG), BN);
-  } else if (warp == 4 && lane == 0) {
+  } else if (warp == kLoadWarp && lane == 0) {
     for (int s = 0; s < a.nstage; ++s) {
-      mbar_init(bar(FULL + s), CG * (COPY ? 2 : 1));  // in CTA 0: warp 4 and, with COPY, warp 6 of either CTA
+      mbar_init(bar(FULL + s), CG * (COPY ? 2 : 1));  // in CTA 0: both CTAs' loads and, with COPY, reports
       mbar_init(bar(EMPTY + s), 1);
-      mbar_init(bar(PARTS + s), COPY ? 32 * kCopyWarps : 1);  // what warp 6 waits for
+      mbar_init(bar(PARTS + s), COPY ? 32 * kCopyWarps : 1);  // what the reporting warp waits for
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar(ACC_FULL + i), 1);
-      mbar_init(bar(ACC_EMPTY + i), 4 * CG);  // in CTA 0: every warp of the pair that writes results
+      mbar_init(bar(ACC_EMPTY + i), kOutWarps * CG);  // in CTA 0: every warp of the pair that writes results
     }
     mbar_init(bar(DRAIN), 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  } else if (warp == 5) {
+  } else if (warp == kMmaWarp) {
     alloc_columns<CG>(smem_u32(slot), kColumns);
   }
   tc_fence_before();
@@ -366,7 +368,7 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
   const int total = tiles.total();
   auto full_bar = [&](int s) { return CG == 2 ? in_leader(bar(FULL + s)) : bar(FULL + s); };
 
-  if (warp == 4) {
+  if (warp == kLoadWarp) {
     // ===================== whole tiles =====================
     int s = 0, issued = 0;
     uint32_t ph = 0;
@@ -382,7 +384,7 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
             break;
           }
           const uint32_t full = full_bar(s), dst = smem_u32(ring + (size_t)s * kStage);
-          if (FORM == WEIGHTS) {  // a block that ends inside of a step goes through warp 6
+          if (FORM == WEIGHTS) {  // a block that ends inside of a step goes by way of warp kReportWarp
             const int i0 = t.lo + kb * 64;
             const bool open = kb == t.blocks - 1 && (t.hi - t.lo) % 16 != 0;
             const uint32_t to = open ? bar(PARTS + s) : full;
@@ -414,7 +416,7 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
         for (int j = issued > a.nstage ? issued - a.nstage : 0; j < issued; ++j)
           mbar_wait_quiet(bar(FULL + j % a.nstage), (j / a.nstage) & 1);
     }
-  } else if (warp == 5) {
+  } else if (warp == kMmaWarp) {
     // ===================== products =====================
     if (rank == 0 && elect_one()) {
       const uint32_t type = a.type == FS_TYPE_BF16 ? 1u : 0u;
@@ -460,10 +462,12 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
         mbar_wait_quiet(bar(DRAIN), 0);
       }
     }
-  } else if (warp < 4) {
+  } else if (warp < kOutWarps) {
     // ===================== results =====================
-    const int q = warp;  // quarter of the TMEM lanes that this warp may read
-    const uint32_t stage = smem_u32(staging + 2048 * q);
+    // Two warps to a quarter of the TMEM lanes, with every other 32 columns each.
+    const int q = warp & 3, side = warp >> 2;
+    const uint32_t stage = smem_u32(staging + 2048 * warp);
+    constexpr int kStep = 32 * kOutWarps / 4;
     int n = 0;
     for (int it = first; it < total; it += stride) {
       const Tile t = tiles.at(it);
@@ -477,8 +481,8 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
       }
       const uint32_t acc = tmem + buf * BN + ((uint32_t)(q * 32) << 16);
       if (f < a.N) {
-        for (int c = 0; c < t.cols; c += 32) {
-          if (FORM != WEIGHTS && a.out_type == FS_TYPE_F32) {
+        if (FORM != WEIGHTS && a.out_type == FS_TYPE_F32) {
+          for (int c = 32 * side; c < t.cols; c += kStep) {
             float v[32];
             if (!zero) tmem_ld32(acc + c, v);
             float* p = static_cast<float*>(a.out) + (long long)(t.lo + c) * a.ldo + f + lane;
@@ -487,18 +491,24 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
               for (int j = 0; j < 32; ++j)
                 if (c + j < t.cols) p[j * a.ldo] = zero ? 0.f : v[j];
             }
-            continue;
           }
-          if (!zero) {
-            stage_block<FORM != WEIGHTS>(acc + c, stage, lane, a.out_type);
+        } else {
+          uint32_t r[32];
+          if (!zero && 32 * side < t.cols) read_block(acc + 32 * side, r);
+          for (int c = 32 * side; c < t.cols; c += kStep) {
+            if (!zero) {
+              tmem_ld_wait(r);
+              stage_block<FORM != WEIGHTS>(r, stage, lane, a.out_type);
+              if (c + kStep < t.cols) read_block(acc + c + kStep, r);  // on its way while this one is written
+              __syncwarp();
+            }
+            uint16_t* out = static_cast<uint16_t*>(a.out);
+            if (FORM == WEIGHTS)
+              write_block(out + ((long long)t.e * a.N + f) * a.K + t.n0 + c, a.K, a.N - f, t.cols - c, a.out_vec, zero, stage, lane);
+            else
+              write_block(out + (long long)(t.lo + c) * a.ldo + f, a.ldo, t.cols - c, a.N - f, a.out_vec, zero, stage, lane);
             __syncwarp();
           }
-          uint16_t* out = static_cast<uint16_t*>(a.out);
-          if (FORM == WEIGHTS)
-            write_block(out + ((long long)t.e * a.N + f) * a.K + t.n0 + c, a.K, a.N - f, t.cols - c, a.out_vec, zero, stage, lane);
-          else
-            write_block(out + (long long)(t.lo + c) * a.ldo + f, a.ldo, t.cols - c, a.N - f, a.out_vec, zero, stage, lane);
-          __syncwarp();
         }
       }
       if (!zero) {
@@ -510,13 +520,13 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
         }
       }
     }
-  } else if (COPY && warp > 6) {
+  } else if (COPY && warp > kReportWarp) {
     // ===================== single rows =====================
     // Chunk ch of rows r, r + kCopyRows, ... of a stage, the chunk exchanged with its row as the 128-byte swizzle has it.
-    // These warps only start copies; that a stage's copies are there is seen by warp 6. Row numbers are read a tile ahead:
+    // These warps only start copies; that a stage's copies are there is seen by warp kReportWarp. Row numbers are read a tile ahead:
     // what is read behind the copies comes back after them.
     constexpr int kSteps = (BNC + kCopyRows - 1) / kCopyRows;
-    const int id = threadIdx.x - 224, r = id >> 3, ch = id & 7;
+    const int id = threadIdx.x - kThreads, r = id >> 3, ch = id & 7;
     const uint32_t at = kA + r * 128 + ((ch ^ (r & 7)) << 4);
     int s = 0, ahead[kSteps];
     uint32_t ph = 0;
@@ -559,7 +569,7 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
     }
     copy_wait_all();
   } else if (COPY) {
-    // ===================== warp 6: reports of copied stages =====================
+    // ===================== reports of copied stages =====================
     // Copies are ordinary writes: their completion, seen here, is made visible to the tensor core, which reads by the
     // asynchronous proxy, and reported to CTA 0 by a thread that has no copies of its own to wait for.
     int s = 0;
@@ -581,7 +591,7 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
       }
     }
   } else if (FORM == WEIGHTS) {
-    // ===================== warp 6: ends of groups =====================
+    // ===================== ends of groups =====================
     int s = 0;         // first stage of the tile
     uint32_t uses = 0;  // bit s: parity of the uses of stage s here
     for (int it = first; it < total; it += stride) {
@@ -608,7 +618,7 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
   __syncthreads();
   if (CG == 2) cluster_sync_all();
   tc_fence_after();
-  if (warp == 5) free_columns<CG>(tmem, kColumns);
+  if (warp == kMmaWarp) free_columns<CG>(tmem, kColumns);
   if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_group_error, 1);
 }
 
@@ -749,9 +759,9 @@ int no_map() { return report_error(FS_ERR_CUDA, "cuTensorMapEncodeTiled failed")
 template <int FORM, int CG, int BN, bool COPY>
 int launch_group(GroupArgs a, const CUtensorMap& mapA, const CUtensorMap& mapB, long long most_tiles, cudaStream_t st) {
   constexpr size_t kStage = 2 * kHalfTile + BN / CG * 128;
-  const size_t fixed = 1024 + 8192 + 8 * (3 * 12 + 5) + 8 + 8 * ((size_t)a.E + 2);
+  const size_t fixed = 1024 + kStaging + 8 * (3 * 12 + 5) + 8 + 8 * ((size_t)a.E + 2);
   a.nstage = (int)((kSmemMax - fixed) / kStage);
-  static_assert((kSmemMax - 1024 - 8192 - 344 - 8 * (kMaxGroups + 2)) / kStage >= 4, "stages");
+  static_assert((kSmemMax - 1024 - kStaging - 344 - 8 * (kMaxGroups + 2)) / kStage >= 4, "stages");
   if (a.nstage > 12) a.nstage = 12;
   size_t smem = fixed + a.nstage * kStage;
   if (smem < (size_t)kSmemMin) smem = kSmemMin;
@@ -764,7 +774,7 @@ int launch_group(GroupArgs a, const CUtensorMap& mapA, const CUtensorMap& mapB, 
   if (grid < 1) grid = 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)grid * CG);
-  cfg.blockDim = dim3(224 + (COPY ? 32 * kCopyWarps : 0));
+  cfg.blockDim = dim3(kThreads + (COPY ? 32 * kCopyWarps : 0));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr{};
