@@ -603,7 +603,7 @@ __device__ __forceinline__ float sigmoid(float x) {
 }
 template <typename T, int VEC>
 __device__ __forceinline__ Pack<T, VEC> read_pack(const T* p, bool in) {
-  if (in) return *reinterpret_cast<const Pack<T, VEC>*>(p);
+  if (in) return read_only<T, VEC>(p);
   Pack<T, VEC> q;
   memset(&q, 0, sizeof(q));
   return q;
@@ -661,15 +661,15 @@ __global__ void __launch_bounds__(kActWarps * 32, 4) act_grad_kernel(const ActAr
   float dp = 0.f;
   for (int c = lane * VEC; c < a.F; c += 32 * VEC) {
     float g[VEC], v[VEC], d[VEC], dg[VEC], dv[VEC], h[VEC];
-    load_f32<T, VEC>(dh + c, d);
+    unpack<T, VEC>(read_only<T, VEC>(dh + c), d);
     if (CODES) {
       const Codes<VEC> cg = *reinterpret_cast<const Codes<VEC>*>(codes + c), cv = *reinterpret_cast<const Codes<VEC>*>(codes + a.F + c);
       const unsigned eg = scales[c / 32], ev = scales[nb + c / 32];
       decode<VEC>(cg, block_scale(eg), g);
       decode<VEC>(cv, block_scale(ev), v);
     } else {
-      load_f32<T, VEC>(row + c, g);
-      load_f32<T, VEC>(row + a.F + c, v);
+      unpack<T, VEC>(read_only<T, VEC>(row + c), g);
+      unpack<T, VEC>(read_only<T, VEC>(row + a.F + c), v);
     }
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {

@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <cstring>
 #include <type_traits>
 
 #include "../../include/flash_sinkhorn_b200.h"
@@ -66,6 +67,32 @@ __device__ __forceinline__ void unpack(const Pack<T, N>& q, float (&out)[N]) {
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) two_f32(q.w[i], out[2 * i], out[2 * i + 1], T());
   }
+}
+// From global memory that nothing writes meanwhile: such loads may move ahead of stores to other arrays.
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> read_only(const T* p) {
+  Pack<T, N> q;
+  constexpr int kBytes = N * sizeof(T);
+  if constexpr (kBytes % 16 == 0) {
+#pragma unroll
+    for (int i = 0; i < kBytes / 16; ++i) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i);
+      q.w[4 * i] = v.x;
+      q.w[4 * i + 1] = v.y;
+      q.w[4 * i + 2] = v.z;
+      q.w[4 * i + 3] = v.w;
+    }
+  } else if constexpr (kBytes == 8) {
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+    q.w[0] = v.x;
+    q.w[1] = v.y;
+  } else if constexpr (kBytes == 4) {
+    q.w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+  } else {
+    const unsigned short v = __ldg(reinterpret_cast<const unsigned short*>(p));
+    memcpy(&q.w[0], &v, 2);
+  }
+  return q;
 }
 template <typename T, int N>
 __device__ __forceinline__ void load_f32(const T* p, float (&out)[N]) {
