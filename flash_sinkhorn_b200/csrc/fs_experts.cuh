@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <cstring>
 #include <type_traits>
 
@@ -118,9 +119,15 @@ inline bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintp
 inline int type_bytes(int type) { return type == FS_TYPE_F32 ? 4 : 2; }
 
 inline int check_device() {
+  static std::atomic<uint64_t> fits{0};  // devices that have been looked at
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess) return report_error(FS_ERR_CUDA, "cannot query the current CUDA device");
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (fits.load(std::memory_order_relaxed) & bit) return FS_OK;
   const int arch = fs_device_arch();
   if (arch < 0) return report_error(FS_ERR_CUDA, "cannot query the current CUDA device");
   if (arch / 10 != 10) return report_error(FS_ERR_UNSUPPORTED, "this library is built for sm_100a only");
+  fits.fetch_or(bit, std::memory_order_relaxed);
   return FS_OK;
 }
 inline int launched(int kernels) {

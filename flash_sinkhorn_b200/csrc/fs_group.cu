@@ -25,6 +25,7 @@
 
 #include <cudaTypedefs.h>
 
+#include <atomic>
 #include <mutex>
 
 namespace fs {
@@ -766,7 +767,14 @@ int launch_group(GroupArgs a, const CUtensorMap& mapA, const CUtensorMap& mapB, 
   size_t smem = fixed + a.nstage * kStage;
   if (smem < (size_t)kSmemMin) smem = kSmemMin;
   const auto kernel = group_kernel<FORM, CG, BN, COPY>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<uint64_t> allowed{0};  // devices on which the kernel may take all shared memory
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (e == cudaSuccess && !(allowed.load(std::memory_order_relaxed) & bit)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
+    if (e == cudaSuccess) allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
   if (e != cudaSuccess) return report_error(FS_ERR_CUDA, cudaGetErrorString(e));
   if (most_tiles > 0x3fffffffll) return report_error(FS_ERR_UNSUPPORTED, "more than 2^30 tiles");
   long long grid = detail::free_ctas() / CG;
@@ -797,6 +805,23 @@ int launch_rows(const GroupArgs& a, bool k_major, const CUtensorMap& mapA, cudaS
   if (a.rows)
     return k_major ? launch_group<ROWS_K, CG, BN, true>(a, mapA, mapB, tiles, st) : launch_group<ROWS_MN, CG, BN, true>(a, mapA, mapB, tiles, st);
   return k_major ? launch_group<ROWS_K, CG, BN, false>(a, mapA, mapB, tiles, st) : launch_group<ROWS_MN, CG, BN, false>(a, mapA, mapB, tiles, st);
+}
+
+// Tile of the rows form: 32, 64 or 128 rows for one CTA (0, 1, 2), 128 or 256 for a pair (3, 4). The smallest with which all
+// tiles are under way at once (half a tile of every group partly filled): 1024 rows of 8 groups, 512 x 512, take 6.2 us with
+// 32 rows a tile and 10.0 us with 256. Where none does, by the rows of a mean group: a group of 40 rows or less is read with
+// its weights anyhow, and larger tiles read the weights less often from L2. 64 groups, 2048 -> 1024, us with tiles 0 to 4:
+// mean 24: 53 49 53 50 53, mean 64: 70 59 54 51 56, mean 192: 182 111 93 77 75, mean 512: 454 266 219 191 149.
+int pick_rows(int R, int E, int N) {
+  const int kRows[5] = {32, 64, 128, 128, 256}, ctas = detail::free_ctas();
+  const int most = N > 128 ? 5 : 3;  // a pair takes 256 features
+  for (int i = 0; i < most; ++i) {
+    const int pair = i < 3 ? 1 : 2;
+    const double tiles = ((double)R / kRows[i] + 0.5 * (E < R ? E : R)) * ((N + 128 * pair - 1) / (128 * pair));
+    if (tiles * pair <= ctas) return i;
+  }
+  const int mean = R / E, by_mean = mean < 24 ? 0 : mean < 40 ? 1 : mean < 160 ? 3 : 4;
+  return by_mean < most ? by_mean : most - 1;
 }
 
 // Values of a 16-bit store: all rows start at multiples of it, and it divides the width.
@@ -867,10 +892,13 @@ int fs_grouped_mm(const void* x, long long ldx, int M, const int* rows, int R, c
   CUtensorMap mapA = {};
   if (!encode(&mapA, type, w, 3, {k_major ? K : N, k_major ? N : K, E}, {w_ld, w_expert ? w_expert : w_ld}, k_major ? 128 : 64))
     return no_map();
-  const int mean = R / E;
-  if (mean >= 96 && N > 128) return launch_rows<2, 256>(a, k_major, mapA, st);
-  if (mean >= 48) return launch_rows<1, 128>(a, k_major, mapA, st);
-  return launch_rows<1, 32>(a, k_major, mapA, st);
+  switch (pick_rows(R, E, N)) {
+    case 0: return launch_rows<1, 32>(a, k_major, mapA, st);
+    case 1: return launch_rows<1, 64>(a, k_major, mapA, st);
+    case 2: return launch_rows<1, 128>(a, k_major, mapA, st);
+    case 3: return launch_rows<2, 128>(a, k_major, mapA, st);
+    default: return launch_rows<2, 256>(a, k_major, mapA, st);
+  }
 }
 
 int fs_grouped_mm_wgrad(const void* dy, long long lddy, const void* x, long long ldx, int R, int E, int N, int K,
@@ -889,8 +917,13 @@ int fs_grouped_mm_wgrad(const void* dy, long long lddy, const void* x, long long
   a.out = dw; a.type = a.out_type = type; a.out_vec = store_values(dw, K, K);
   CUtensorMap mapA = {}, mapB = {};
   if (!encode_rows(&mapA, type, dy, N, R, lddy, 64) || !encode_rows(&mapB, type, x, K, R, ldx, 64)) return no_map();
-  if (N > 128 && K > 128) return launch_group<WEIGHTS, 2, 256, false>(a, mapA, mapB, (long long)E * ((N + 255) / 256) * ((K + 255) / 256), st);
-  return launch_group<WEIGHTS, 1, 128, false>(a, mapA, mapB, (long long)E * ((N + 127) / 128) * ((K + 127) / 128), st);
+  // The largest tile, unless smaller ones are all under way at once: 7 x 501 x 300 outputs of 6000 rows take 20.4 us with
+  // 128 x 64, 24.2 us with 256 x 256.
+  auto tiles = [&](int m, int n) { return (long long)E * ((N + m - 1) / m) * ((K + n - 1) / n); };
+  const int ctas = detail::free_ctas();
+  if (tiles(128, 64) <= ctas) return launch_group<WEIGHTS, 1, 64, false>(a, mapA, mapB, tiles(128, 64), st);
+  if (tiles(128, 128) <= ctas || N <= 128 || K <= 128) return launch_group<WEIGHTS, 1, 128, false>(a, mapA, mapB, tiles(128, 128), st);
+  return launch_group<WEIGHTS, 2, 256, false>(a, mapA, mapB, tiles(256, 256), st);
 }
 
 }  // extern "C"
