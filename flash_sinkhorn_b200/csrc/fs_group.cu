@@ -16,7 +16,7 @@
 // ring of stages of 64 contraction values), one issues the products into one of two TMEM accumulators (either by one
 // thread from beginning to end: choosing it anew for every instruction cost 500 clocks a stage, as much as the products of a
 // 256 x 256 tile), and eight write the other one out, through shared memory in pieces of 64 bytes. Rows in another order are
-// fetched by four more, 16 bytes a lane (cp.async): TMA's loads of four rows each took 75 clocks apiece, 2.6 times the time
+// fetched by eight more, 16 bytes a lane (cp.async): TMA's loads of four rows each took 75 clocks apiece, 2.6 times the time
 // of the whole product. Group boundaries are read by the kernel itself; every CTA takes every n-th tile, features fastest,
 // so that the CTAs working at one time share a group's weights and rows in L2.
 #include "fs_experts.cuh"
@@ -42,8 +42,10 @@ enum Form { ROWS_K, ROWS_MN, WEIGHTS };  // rows with W contiguous along the con
 constexpr int kOutWarps = 8, kLoadWarp = kOutWarps, kMmaWarp = kOutWarps + 1, kReportWarp = kOutWarps + 2;
 constexpr int kThreads = 32 * (kOutWarps + 3);
 constexpr int kStaging = 2048 * kOutWarps;
-constexpr int kCopyWarps = 4;              // warps that fetch single rows
-constexpr int kCopyRows = 4 * kCopyWarps;  // rows that they fetch 128 bytes of at a time
+// Eight warps fetch single rows, four of them every other stage each: one iteration of a warp (a wait, up to eight copies) takes
+// about as long as the products of a stage.
+constexpr int kCopyWarps = 8, kCopyGroup = 128;  // threads that fetch a stage
+constexpr int kCopyRows = kCopyGroup / 8;        // rows that they fetch 128 bytes of at a time
 constexpr uint32_t kHalfTile = 64 * 128;  // 64 rows of 128 bytes
 constexpr int kMaxGroups = 1024;
 
@@ -347,7 +349,7 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
     for (int s = 0; s < a.nstage; ++s) {
       mbar_init(bar(FULL + s), CG * (COPY ? 2 : 1));  // in CTA 0: both CTAs' loads and, with COPY, reports
       mbar_init(bar(EMPTY + s), 1);
-      mbar_init(bar(PARTS + s), COPY ? 32 * kCopyWarps : 1);  // what the reporting warp waits for
+      mbar_init(bar(PARTS + s), COPY ? kCopyGroup : 1);  // what the reporting warp waits for
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar(ACC_FULL + i), 1);
@@ -527,9 +529,9 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
     // These warps only start copies; that a stage's copies are there is seen by warp kReportWarp. Row numbers are read a tile ahead:
     // what is read behind the copies comes back after them.
     constexpr int kSteps = (BNC + kCopyRows - 1) / kCopyRows;
-    const int id = threadIdx.x - kThreads, r = id >> 3, ch = id & 7;
+    const int side = (threadIdx.x - kThreads) / kCopyGroup, id = (threadIdx.x - kThreads) % kCopyGroup, r = id >> 3, ch = id & 7;
     const uint32_t at = kA + r * 128 + ((ch ^ (r & 7)) << 4);
-    int s = 0, ahead[kSteps];
+    int s = side, ahead[kSteps], turn = 0;
     uint32_t ph = 0;
     bool ok = true;
     Tiles<FORM, CG, BN> ahead_tiles = tiles;
@@ -551,7 +553,8 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
       for (int j = 0; j < kSteps; ++j)
         src[j] = (unsigned)ahead[j] < (unsigned)a.M ? static_cast<const uint16_t*>(a.x) + ahead[j] * a.ldx + ch * 8 : nullptr;
       read_ahead(it + stride);
-      for (int kb = 0; kb < t.blocks; ++kb) {
+      for (int kb = 0; kb < t.blocks; ++kb, turn ^= 1) {
+        if (turn != side) continue;
         if (!__all_sync(0xffffffffu, mbar_wait(bar(EMPTY + s), ph ^ 1, abort_flag, 2000))) {
           ok = false;
           break;
@@ -562,8 +565,9 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
         for (int j = 0; j < kSteps; ++j)
           copy16(dst + j * kCopyRows * 128, src[j] && valid ? src[j] + kb * 64 : a.x, src[j] ? valid : 0);
         copy_arrive(bar(PARTS + s));
-        if (++s == a.nstage) {
-          s = 0;
+        s += 2;
+        if (s >= a.nstage) {
+          s -= a.nstage;
           ph ^= 1;
         }
       }
