@@ -26,8 +26,8 @@ constexpr unsigned kAll = 0xffffffffu;
 // second adds up the counts of the CTAs before it (every CTA for itself: E x kMaxBlocks words from L2, cheaper than a third
 // launch or CTAs that wait for one another) and numbers its own pairs. Batches of one CTA do both in one launch.
 
-constexpr int kRouteWarps = 16;
-constexpr int kMaxBlocks = 296;    // two CTAs on each of 148 SMs
+constexpr int kMaxBlocks = 148;    // one for each SM: what the second kernel reads of the counts grows with the square of it
+constexpr int kOrderWarps = 32, kGradWarps = 16;
 constexpr int kMaxExperts = 1024;  // 32 per lane
 constexpr int kMaxK = 32;          // one slot per lane
 
@@ -127,10 +127,13 @@ struct Candidates {
       }
   }
   __device__ __forceinline__ void prepare() {
-    if (!kSorted) {
+    if constexpr (!kSorted) {
       look();
-      return;
+    } else {
+      sort();
     }
+  }
+  __device__ __forceinline__ void sort() {
 #pragma unroll
     for (int i = 0; i < PER; ++i) number[i] = i;
 #pragma unroll
@@ -153,7 +156,7 @@ struct Candidates {
     best = key[0];
   }
   __device__ __forceinline__ void take(bool mine) {
-    if (kSorted) {
+    if constexpr (kSorted) {
 #pragma unroll
       for (int i = 0; i + 1 < PER; ++i) {
         key[i] = mine ? key[i + 1] : key[i];
@@ -172,7 +175,7 @@ struct Candidates {
   }
 };
 
-template <typename T, int PER>
+template <typename T, int PER, int WARPS>
 __device__ __forceinline__ void select_tokens(const RouteArgs& a, int* count) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int t0 = blockIdx.x * a.chunk, t1 = min(t0 + a.chunk, a.T);
@@ -180,12 +183,12 @@ __device__ __forceinline__ void select_tokens(const RouteArgs& a, int* count) {
   load_bias<PER>(a, lane, bias);
   constexpr bool kEarly = PER <= 8;  // the next token's logits are on their way while this one's experts are chosen
   if (kEarly && t0 + warp < t1) load_logits<T, PER>(a, t0 + warp, lane, bias, next);
-  for (int t = t0 + warp; t < t1; t += kRouteWarps) {
+  for (int t = t0 + warp; t < t1; t += WARPS) {
     float l[PER], top, inv;
     if (kEarly) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) l[i] = next[i];
-      if (t + kRouteWarps < t1) load_logits<T, PER>(a, t + kRouteWarps, lane, bias, next);
+      if (t + WARPS < t1) load_logits<T, PER>(a, t + WARPS, lane, bias, next);
     } else {
       load_logits<T, PER>(a, t, lane, bias, l);
     }
@@ -217,10 +220,11 @@ __device__ __forceinline__ void select_tokens(const RouteArgs& a, int* count) {
 }
 
 // Exclusive prefix over v[0 .. n) in shared memory, by all threads of the CTA; the total comes back.
+template <int WARPS>
 __device__ __forceinline__ int scan_in_place(int* v, int n, int* scratch) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int base = 0;
-  for (int c = 0; c < n; c += kRouteWarps * 32) {
+  for (int c = 0; c < n; c += WARPS * 32) {
     const int j = c + threadIdx.x, x = j < n ? v[j] : 0;
     int inc = x;
 #pragma unroll
@@ -232,7 +236,7 @@ __device__ __forceinline__ int scan_in_place(int* v, int n, int* scratch) {
     __syncthreads();
     int before = 0, total = 0;
 #pragma unroll
-    for (int w = 0; w < kRouteWarps; ++w) {
+    for (int w = 0; w < WARPS; ++w) {
       before += w < warp ? scratch[w] : 0;
       total += scratch[w];
     }
@@ -245,13 +249,14 @@ __device__ __forceinline__ int scan_in_place(int* v, int n, int* scratch) {
 
 // The pairs of a warp, in order; the experts of the first kEarlyPairs x 32 of them are read ahead.
 constexpr int kEarlyPairs = 4;
+template <int WARPS>
 struct WarpPairs {
   long long begin, end;
   int early[kEarlyPairs];
   __device__ __forceinline__ WarpPairs(const RouteArgs& a) {
     const int warp = threadIdx.x >> 5;
     const long long p0 = (long long)blockIdx.x * a.chunk * a.k, p1 = min((long long)a.T, (long long)(blockIdx.x + 1) * a.chunk) * a.k;
-    const long long share = ((p1 - p0 + kRouteWarps - 1) / kRouteWarps + 31) / 32 * 32;
+    const long long share = ((p1 - p0 + WARPS - 1) / WARPS + 31) / 32 * 32;
     begin = p0 + warp * share;
     end = min(p1, begin + share);
   }
@@ -264,47 +269,56 @@ struct WarpPairs {
   }
 };
 
-// Rows of this CTA's pairs. first[e]: row of its first pair of expert e. hist: [kRouteWarps, E].
-__device__ __forceinline__ void number_pairs(const RouteArgs& a, WarpPairs& w, int* first, int* hist, int total) {
+// Rows of this CTA's pairs. first[e]: row of its first pair of expert e. hist: [WARPS, E].
+template <int WARPS>
+__device__ __forceinline__ void number_pairs(const RouteArgs& a, WarpPairs<WARPS>& w, int* first, int* hist, int total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int j = threadIdx.x; j < kRouteWarps * a.E; j += kRouteWarps * 32) hist[j] = 0;
+  for (int j = threadIdx.x; j < WARPS * a.E; j += WARPS * 32) hist[j] = 0;
   __syncthreads();
   int* mine = hist + warp * a.E;
   constexpr int kRound = kEarlyPairs * 32;
+  unsigned same[kEarlyPairs];  // lanes with the same expert
   for (long long from = w.begin; from < w.end; from += kRound) {
     if (from > w.begin) w.read(a, from);
 #pragma unroll
+    for (int i = 0; i < kEarlyPairs; ++i) same[i] = __match_any_sync(kAll, w.early[i]);
+#pragma unroll
     for (int i = 0; i < kEarlyPairs; ++i) {
       const int e = w.early[i];
-      const unsigned same = __match_any_sync(kAll, e);
-      if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
+      if (e >= 0 && lane == __ffs(same[i]) - 1) mine[e] += __popc(same[i]);
       __syncwarp();
     }
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < a.E; e += kRouteWarps * 32) {
-    int at = first[e], c[kRouteWarps];
+  for (int e = threadIdx.x; e < a.E; e += WARPS * 32) {
+    int at = first[e], c[16];
 #pragma unroll
-    for (int j = 0; j < kRouteWarps; ++j) c[j] = hist[j * a.E + e];
+    for (int j0 = 0; j0 < WARPS; j0 += 16) {
 #pragma unroll
-    for (int j = 0; j < kRouteWarps; ++j) {
-      hist[j * a.E + e] = at;
-      at += c[j];
+      for (int j = 0; j < 16; ++j) c[j] = hist[(j0 + j) * a.E + e];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        hist[(j0 + j) * a.E + e] = at;
+        at += c[j];
+      }
     }
   }
   __syncthreads();
   const bool again = w.end - w.begin > kRound;
   for (long long from = w.begin; from < w.end; from += kRound) {
-    if (again) w.read(a, from);
+    if (again) {
+      w.read(a, from);
+#pragma unroll
+      for (int i = 0; i < kEarlyPairs; ++i) same[i] = __match_any_sync(kAll, w.early[i]);
+    }
 #pragma unroll
     for (int i = 0; i < kEarlyPairs; ++i) {
       const int e = w.early[i];
       const long long p = from + i * 32 + lane;
-      const unsigned same = __match_any_sync(kAll, e);
-      const int rank = __popc(same & ((1u << lane) - 1u));
+      const int rank = __popc(same[i] & ((1u << lane) - 1u));
       const int at = e >= 0 ? mine[e] + rank : -1;
       __syncwarp();
-      if (e >= 0 && rank == 0) mine[e] += __popc(same);
+      if (e >= 0 && rank == 0) mine[e] += __popc(same[i]);
       __syncwarp();
       if (p < w.end) {
         a.position[p] = at;
@@ -318,39 +332,44 @@ __device__ __forceinline__ void number_pairs(const RouteArgs& a, WarpPairs& w, i
   }
 }
 
+// Warps of a CTA that chooses: as many as the registers of 16 or more experts a lane allow.
+template <int PER>
+constexpr int kSelectWarps = PER <= 8 ? 32 : 16;
+
 template <typename T, int PER>
-__global__ void __launch_bounds__(kRouteWarps * 32) route_select_kernel(const RouteArgs a) {
+__global__ void __launch_bounds__(kSelectWarps<PER> * 32) route_select_kernel(const RouteArgs a) {
+  constexpr int WARPS = kSelectWarps<PER>;
   extern __shared__ int sm[];
-  __shared__ int scratch[kRouteWarps];
+  __shared__ int scratch[WARPS];
   int* count = sm;  // [E], then the histograms of the warps
-  for (int e = threadIdx.x; e < a.E; e += kRouteWarps * 32) count[e] = 0;
+  for (int e = threadIdx.x; e < a.E; e += WARPS * 32) count[e] = 0;
   __syncthreads();
-  select_tokens<T, PER>(a, count);
+  select_tokens<T, PER, WARPS>(a, count);
   __syncthreads();
   if (a.blocks > 1) {
-    for (int e = threadIdx.x; e < a.E; e += kRouteWarps * 32) a.counts[e * a.blocks + blockIdx.x] = count[e];
+    for (int e = threadIdx.x; e < a.E; e += WARPS * 32) a.counts[e * a.blocks + blockIdx.x] = count[e];
     return;
   }
-  const int total = scan_in_place(count, a.E, scratch);
+  const int total = scan_in_place<WARPS>(count, a.E, scratch);
   __syncthreads();
-  for (int e = threadIdx.x; e < a.E; e += kRouteWarps * 32) a.offsets[e] = count[e];
+  for (int e = threadIdx.x; e < a.E; e += WARPS * 32) a.offsets[e] = count[e];
   if (threadIdx.x == 0) a.offsets[a.E] = total;
-  WarpPairs pairs(a);
+  WarpPairs<WARPS> pairs(a);
   pairs.read(a, pairs.begin);
   number_pairs(a, pairs, count, sm + a.E, total);
 }
 
-__global__ void __launch_bounds__(kRouteWarps * 32) route_order_kernel(const RouteArgs a) {
+__global__ void __launch_bounds__(kOrderWarps * 32) route_order_kernel(const RouteArgs a) {
   extern __shared__ int sm[];
-  __shared__ int scratch[kRouteWarps];
+  __shared__ int scratch[kOrderWarps];
   int *all = sm, *before = sm + a.E;  // pairs of expert e in all CTAs, in the CTAs before this one
-  WarpPairs pairs(a);
+  WarpPairs<kOrderWarps> pairs(a);
   pairs.read(a, pairs.begin);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   constexpr int kSide = 4;  // experts that a warp adds up side by side, so that its loads are in flight together
-  for (int e0 = warp * kSide; e0 < a.E; e0 += kRouteWarps * kSide) {
+  for (int e0 = warp * kSide; e0 < a.E; e0 += kOrderWarps * kSide) {
     int n[kSide] = {}, b[kSide] = {};
-#pragma unroll 4
+#pragma unroll 5
     for (int c = lane; c < a.blocks; c += 32)
 #pragma unroll
       for (int i = 0; i < kSide; ++i) {
@@ -369,8 +388,8 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_order_kernel(const Rou
     }
   }
   __syncthreads();
-  const int total = scan_in_place(all, a.E, scratch);
-  for (int e = threadIdx.x; e < a.E; e += kRouteWarps * 32) {
+  const int total = scan_in_place<kOrderWarps>(all, a.E, scratch);
+  for (int e = threadIdx.x; e < a.E; e += kOrderWarps * 32) {
     if (blockIdx.x == 0) a.offsets[e] = all[e];
     before[e] += all[e];
   }
@@ -382,13 +401,13 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_order_kernel(const Rou
 // d logit_j = [j chosen as slot s] g_s dg_s - p_j sum_s g_s dg_s, p = the soft-max that the gates were taken from. The chosen
 // experts' terms are added in a row of shared memory (E floats of every warp).
 template <typename T, int PER>
-__global__ void __launch_bounds__(kRouteWarps * 32) route_grad_kernel(const RouteArgs a) {
+__global__ void __launch_bounds__(kGradWarps * 32) route_grad_kernel(const RouteArgs a) {
   extern __shared__ float rows[];
   const int lane = threadIdx.x & 31;
   float* row = rows + (threadIdx.x >> 5) * (32 * PER);
   float bias[PER];
   load_bias<PER>(a, lane, bias);
-  for (long long t = (long long)blockIdx.x * kRouteWarps + (threadIdx.x >> 5); t < a.T; t += (long long)gridDim.x * kRouteWarps) {
+  for (long long t = (long long)blockIdx.x * kGradWarps + (threadIdx.x >> 5); t < a.T; t += (long long)gridDim.x * kGradWarps) {
     const long long p = t * a.k + lane;
     const int expert = lane < a.k ? a.experts_in[p] : -1;
     const float gate = expert >= 0 ? a.gates_in[p] : 0.f;
@@ -421,12 +440,12 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_grad_kernel(const Rout
   }
 }
 
-// Tokens per CTA: a whole number of rounds of its warps, and at most kMaxBlocks CTAs. Small batches (16 tokens a warp)
-// stay in one CTA and one launch: 256 tokens of 64 experts take less time there than a second launch does.
+// Tokens per CTA: whole rounds of 32 warps, at most kMaxBlocks CTAs. Batches of up to 256 tokens stay in one CTA and one
+// launch: 256 tokens of 64 experts take less time there than a second launch does.
 void plan_route(int T, int& chunk, int& blocks) {
   chunk = (T + kMaxBlocks - 1) / kMaxBlocks;
-  chunk = (chunk + kRouteWarps - 1) / kRouteWarps * kRouteWarps;
-  if (T <= 16 * kRouteWarps) chunk = 16 * kRouteWarps;
+  chunk = (chunk + 31) / 32 * 32;
+  if (T <= 256) chunk = 256;
   blocks = T > 0 ? (T + chunk - 1) / chunk : 1;
 }
 
@@ -442,19 +461,20 @@ int launch_route(RouteArgs a, bool grad, cudaStream_t st) {
   const size_t part = sizeof(T) * PER < 16 ? sizeof(T) * PER : 16;
   a.vec = a.E % PER == 0 && a.ld % PER == 0 && aligned(a.logits, part) && aligned(a.out, part);
   if (grad) {
-    const long long want = ((long long)a.T + kRouteWarps - 1) / kRouteWarps;
-    const size_t bytes = (size_t)kRouteWarps * 32 * PER * 4;
+    const long long want = ((long long)a.T + kGradWarps - 1) / kGradWarps;
+    const size_t bytes = (size_t)kGradWarps * 32 * PER * 4;
     const int s = allow_smem(route_grad_kernel<T, PER>, bytes);
     if (s != FS_OK) return s;
-    route_grad_kernel<T, PER><<<(int)(want < 592 ? want : 592), kRouteWarps * 32, bytes, st>>>(a);
+    route_grad_kernel<T, PER><<<(int)(want < 592 ? want : 592), kGradWarps * 32, bytes, st>>>(a);
     return launched(1);
   }
-  const size_t one = (size_t)(a.blocks > 1 ? 1 : 1 + kRouteWarps) * a.E * 4, two = (size_t)(2 + kRouteWarps) * a.E * 4;
+  constexpr int kWarps = kSelectWarps<PER>;
+  const size_t one = (size_t)(a.blocks > 1 ? 1 : 1 + kWarps) * a.E * 4, two = (size_t)(2 + kOrderWarps) * a.E * 4;
   int s = allow_smem(route_select_kernel<T, PER>, one);
   if (s != FS_OK) return s;
   if (a.blocks > 1 && (s = allow_smem(route_order_kernel, two)) != FS_OK) return s;
-  route_select_kernel<T, PER><<<a.blocks, kRouteWarps * 32, one, st>>>(a);
-  if (a.blocks > 1) route_order_kernel<<<a.blocks, kRouteWarps * 32, two, st>>>(a);
+  route_select_kernel<T, PER><<<a.blocks, kWarps * 32, one, st>>>(a);
+  if (a.blocks > 1) route_order_kernel<<<a.blocks, kOrderWarps * 32, two, st>>>(a);
   return launched(a.blocks > 1 ? 2 : 1);
 }
 template <typename T>
@@ -786,42 +806,63 @@ __global__ void __launch_bounds__(kActWarps * 32) combine_kernel(const CombineAr
   }
 }
 
-// do_i = w dy_t and d w = <dy_t, o_i> for the row i of a pair; rows of no pair get zeros, pairs of no row a zero gradient.
+// do_i = w dy_t and d w = <dy_t, o_i> for the row i of a pair, zeros for a pair of no row and a row of no pair. A warp takes four
+// slots of a token, so that dy is read once for them: by rows it comes back from DRAM for every slot, 45 % more bytes at
+// four slots (112 us against 93 us for 65536 rows of 2048).
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kActWarps * 32) combine_grad_kernel(const CombineArgs a) {
-  const int lane = threadIdx.x & 31, n = a.T * a.k;
-  for (int r = blockIdx.x * kActWarps + (threadIdx.x >> 5); r < n; r += gridDim.x * kActWarps) {
-    const int pair = a.pairs[r];
-    const bool routed = pair >= 0 && pair < n;
-    const float w = routed ? (a.gates ? a.gates[pair] : 1.f) : 0.f;
-    const T* dy = static_cast<const T*>(a.dy) + (long long)(routed ? pair / a.k : 0) * a.lddy;
-    const T* o = static_cast<const T*>(a.o) + (long long)r * a.ldo;
-    T* out = static_cast<T*>(a.d_o) + (long long)r * a.D;
-    float dw = 0.f;
-#pragma unroll 2
+  constexpr int kSlots = 4;
+  const int lane = threadIdx.x & 31, n = a.T * a.k, groups = (a.k + kSlots - 1) / kSlots;
+  const long long it = (long long)blockIdx.x * kActWarps + (threadIdx.x >> 5);
+  const int t = (int)(it / groups), s0 = (int)(it - (long long)t * groups) * kSlots, slots = min(kSlots, a.k - s0);
+  if (t >= a.T) return;
+  const int first = t * a.k + s0;
+  const int at = lane < slots ? a.position[first + lane] : -1, other = lane < slots ? a.pairs[first + lane] : 0;
+  const float weight = lane < slots && a.gates ? a.gates[first + lane] : 1.f;
+  const T* dy = static_cast<const T*>(a.dy) + (long long)t * a.lddy;
+  int row[kSlots];
+  float w[kSlots], dw[kSlots] = {};
+  bool any = false, empty[kSlots];  // empty: row first + j belongs to no pair
+#pragma unroll
+  for (int j = 0; j < kSlots; ++j) {
+    const int r = __shfl_sync(kAll, at, j), p = __shfl_sync(kAll, other, j);
+    w[j] = __shfl_sync(kAll, weight, j);
+    row[j] = r < n ? r : -1;
+    empty[j] = j < slots && (p < 0 || p >= n);
+    any = any || row[j] >= 0;
+  }
+  if (any) {
     for (int c = lane * VEC; c < a.D; c += 32 * VEC) {
-      float g[VEC];
+      const Pack<T, VEC> qg = read_only<T, VEC>(dy + c);
+      Pack<T, VEC> qo[kSlots];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) g[i] = 0.f;
-      if (routed) {
-        load_f32<T, VEC>(dy + c, g);
+      for (int j = 0; j < kSlots; ++j)
+        if (row[j] >= 0 && a.dgates) qo[j] = read_only<T, VEC>(static_cast<const T*>(a.o) + (long long)row[j] * a.ldo + c);
+      float g[VEC], x[VEC];
+      unpack<T, VEC>(qg, g);
+#pragma unroll
+      for (int j = 0; j < kSlots; ++j) {
+        if (row[j] < 0) continue;
         if (a.dgates) {
-          float x[VEC];
-          load_f32<T, VEC>(o + c, x);
+          unpack<T, VEC>(qo[j], x);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) dw += g[i] * x[i];
+          for (int i = 0; i < VEC; ++i) dw[j] = fmaf(g[i], x[i], dw[j]);
         }
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) g[i] *= w;
+        for (int i = 0; i < VEC; ++i) x[i] = g[i] * w[j];
+        store_f32<T, VEC>(static_cast<T*>(a.d_o) + (long long)row[j] * a.D + c, x);
       }
-      store_f32<T, VEC>(out + c, g);
     }
-    if (a.dgates) {
-      dw = warp_sum(dw);
-      if (lane == 0) {
-        if (routed) a.dgates[pair] = dw;
-        if (a.position[r] < 0) a.dgates[r] = 0.f;  // r as a pair: one that has no row
-      }
+  }
+#pragma unroll
+  for (int j = 0; j < kSlots; ++j) {
+    if (empty[j]) {
+      const float zero[VEC] = {};
+      for (int c = lane * VEC; c < a.D; c += 32 * VEC) store_f32<T, VEC>(static_cast<T*>(a.d_o) + (long long)(first + j) * a.D + c, zero);
+    }
+    if (a.dgates && j < slots) {
+      const float d = warp_sum(dw[j]);
+      if (lane == 0) a.dgates[first + j] = d;
     }
   }
 }
@@ -830,7 +871,7 @@ template <typename T, typename Y, int VEC>
 int launch_combine(CombineArgs a, bool grad, cudaStream_t st) {
   a.parts = row_parts(a.T, a.D, VEC);
   if (!grad) combine_kernel<T, Y, VEC><<<row_blocks((long long)a.T * a.parts), kActWarps * 32, 0, st>>>(a);
-  else combine_grad_kernel<T, VEC><<<row_blocks((long long)a.T * a.k), kActWarps * 32, 0, st>>>(a);
+  else combine_grad_kernel<T, VEC><<<(int)(((long long)a.T * ((a.k + 3) / 4) + kActWarps - 1) / kActWarps), kActWarps * 32, 0, st>>>(a);
   return launched(1);
 }
 template <typename T, typename Y>
