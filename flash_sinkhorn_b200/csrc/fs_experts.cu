@@ -722,10 +722,10 @@ int lane_values(int F, int bytes, long long ld0, long long ld1, P... ptrs) {
   return 1;
 }
 
-// Parts of a row, where the rows alone do not give every SM some warps.
+// Parts of a row, where the rows alone do not give every SM 16 warps (more of those that take few values at a time).
 int row_parts(long long rows, int width, int vec) {
   const int steps = (width + 32 * vec - 1) / (32 * vec);
-  const long long want = rows > 0 ? (148 * 16 + rows - 1) / rows : 1;
+  const long long want = rows > 0 ? (148 * 16 * (8 / vec) + rows - 1) / rows : 1;
   return (int)(want < 1 ? 1 : want > steps ? steps : want);
 }
 int row_blocks(long long items) {
@@ -783,7 +783,7 @@ __global__ void __launch_bounds__(kActWarps * 32) combine_kernel(const CombineAr
   for (long long it = (long long)blockIdx.x * kActWarps + (threadIdx.x >> 5); it < items; it += (long long)gridDim.x * kActWarps) {
     const int t = (int)(it / a.parts), s0 = (int)(it - (long long)t * a.parts) * share, s1 = min(s0 + share, steps);
     const long long pair = (long long)t * a.k + lane;
-    const int at = lane < a.k ? a.position[pair] : -1;
+    const int at = lane < a.k ? (a.position ? a.position[pair] : t) : -1;
     const float w = lane < a.k && a.gates ? a.gates[pair] : 1.f;
     for (int s = s0; s < s1; ++s) {
       const int c = (s * 32 + lane) * VEC;
@@ -976,7 +976,7 @@ int fs_combine(const void* o, int type, long long ldo, int M, int T, int k, int 
   int s = check_rows(type, T, D);
   if (s != FS_OK || T == 0) return s;
   if (k < 1 || k > kMaxK || (long long)T * k > 0x7fffffffll) return report_error(FS_ERR_BAD_ARG, "k must be in [1, 32], T * k below 2^31");
-  if (!o || M < 0 || !position || !y || ldo < D || ldy < D || y_type < 0 || y_type > 2 || (y_type != type && type != FS_TYPE_F32))
+  if (!o || M < 0 || (!position && k != 1) || !y || ldo < D || ldy < D || y_type < 0 || y_type > 2 || (y_type != type && type != FS_TYPE_F32))
     return report_error(FS_ERR_BAD_ARG, "null argument, rows shorter than D, or a wrong type of the result");
   CombineArgs a{};
   a.o = o; a.ldo = ldo; a.M = M; a.T = T; a.k = k; a.D = D; a.gates = gates; a.position = position; a.y = y; a.ldy = ldy;

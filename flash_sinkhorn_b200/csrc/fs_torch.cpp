@@ -109,19 +109,31 @@ optional<Tensor> maybe(const Tensor& t) { return t.defined() ? optional<Tensor>(
 
 // `t` itself where its rows are contiguous and do not overlap, else a copy.
 Tensor rows_of(const Tensor& t) { return t.stride(1) == 1 && t.stride(0) >= t.size(1) ? t : t.contiguous(); }
+bool aligned16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+// Rows [R, C] of `t`, `from` values apart, copied 8 ceil(C / 8) values apart.
+Tensor padded(const Tensor& t, int64_t r, int64_t c, int64_t from) {
+  const Place at(t);
+  const int64_t to = (c + 7) / 8 * 8;
+  Tensor out = at::empty({r, to}, t.options());
+  FS_CALL(fs_combine, t.data_ptr(), type_of(t), from, (int)r, (int)r, 1, (int)c, nullptr, nullptr, out.data_ptr(), type_of(t), to, at.stream);
+  return out;
+}
 // `t [R, C]` as tensor loads take it: rows a multiple of 16 bytes apart, the first one aligned to 16 bytes; `t` itself, or a
 // copy with padded rows.
-bool aligned16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
-Tensor loadable_rows(const Tensor& t) {
-  const int64_t r = t.size(0), c = t.size(1);
-  if (t.stride(1) == 1 && t.stride(0) >= c && t.stride(0) % 8 == 0 && aligned16(t)) return t;
-  return at::empty({r, (c + 7) / 8 * 8}, t.options()).narrow(1, 0, c).copy_(t);
+Tensor loadable_rows(const Tensor& t0) {
+  const int64_t r = t0.size(0), c = t0.size(1);
+  if (t0.stride(1) == 1 && t0.stride(0) >= c && t0.stride(0) % 8 == 0 && aligned16(t0)) return t0;
+  const Tensor t = rows_of(t0);
+  return padded(t, r, c, ld(t)).narrow(1, 0, c);
 }
 // `w [E, N, K]` where one of its two matrix dimensions is contiguous and the other strides are multiples of 16 bytes.
-Tensor loadable_weights(const Tensor& w) {
-  const int64_t e = w.size(0), n = w.size(1), k = w.size(2), se = w.stride(0), sn = w.stride(1), sk = w.stride(2);
-  if (aligned16(w) && se % 8 == 0 && (se > 0 || e == 1) && ((sk == 1 && sn >= k && sn % 8 == 0) || (sn == 1 && sk >= n && sk % 8 == 0))) return w;
-  return at::empty({e, n, (k + 7) / 8 * 8}, w.options()).narrow(2, 0, k).copy_(w);
+Tensor loadable_weights(const Tensor& w0) {
+  const int64_t e = w0.size(0), n = w0.size(1), k = w0.size(2), se = w0.stride(0), sn = w0.stride(1), sk = w0.stride(2);
+  if (aligned16(w0) && se % 8 == 0 && (se > 0 || e == 1) && ((sk == 1 && sn >= k && sn % 8 == 0) || (sn == 1 && sk >= n && sk % 8 == 0))) return w0;
+  const Tensor w = w0.contiguous();
+  if (k % 8 == 0 && aligned16(w)) return w;
+  require(e * n < (int64_t(1) << 31), "weight of ", k, " columns has too many rows to be padded");
+  return padded(w, e * n, k, k).view({e, n, (k + 7) / 8 * 8}).narrow(2, 0, k);
 }
 
 bool wants_grad(std::initializer_list<const Tensor*> ts) {

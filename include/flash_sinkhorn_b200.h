@@ -528,7 +528,8 @@ int fs_gated_act_grad(const void* u, long long ldu, const int8_t* codes, const u
 
 /* Rows back into tokens: y[t, :] = sum over the slots s with a row of gates[t, s] o[position[t, s], :] (gates null:
  * weights of 1; positions outside [0, M): no row). o has M rows of D values; y is T x D, of the type of o or, where that
- * is FS_TYPE_F32, of any. With k = 1 and no gates it gathers rows. */
+ * is FS_TYPE_F32, of any. With k = 1 and no gates it gathers rows; position null (k = 1): row
+ * t of o, a copy with other distances between the rows. */
 int fs_combine(const void* o, int type, long long ldo, int M, int T, int k, int D, const float* gates, const int* position,
                void* y, int y_type, long long ldy, void* stream);
 
