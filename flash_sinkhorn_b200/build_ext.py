@@ -13,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -23,7 +24,7 @@ SOURCES = ["fs_api.cu", "fs_simt.cu", "fs_tc.cu", "fs_tck.cu", "fs_sym.cu", "fs_
            "fs_experts.cu", "fs_group.cu"]
 FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC",
 ]
 
 
@@ -70,12 +71,21 @@ def build_binding(force: bool = False, verbose: bool = False) -> str:
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
+    """Compiles the sources side by side and links them; the binding at the same time."""
+    from concurrent.futures import ThreadPoolExecutor
+
     sources = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f != BINDING_SOURCE]
-    if force or _stale(OUT, sources):
-        os.makedirs(os.path.dirname(OUT), exist_ok=True)
-        cmd = [os.environ.get("NVCC", "nvcc")] + FLAGS + (["-Xptxas", "-v"] if verbose else []) + [os.path.join(CSRC, s) for s in SOURCES]
-        _run(cmd, OUT, verbose)
-    build_binding(force, verbose)
+    os.makedirs(os.path.dirname(OUT), exist_ok=True)
+    with ThreadPoolExecutor(os.cpu_count() or 4) as pool:
+        binding = pool.submit(build_binding, force, verbose)
+        if force or _stale(OUT, sources):
+            nvcc = [os.environ.get("NVCC", "nvcc")] + FLAGS
+            with tempfile.TemporaryDirectory() as folder:
+                objects = [os.path.join(folder, s[:-3] + ".o") for s in SOURCES]
+                options = ["-Xptxas", "-v"] if verbose else []
+                list(pool.map(lambda s, o: _run(nvcc + options + ["-c", os.path.join(CSRC, s)], o, verbose), SOURCES, objects))
+                _run(nvcc + ["-shared"] + objects, OUT, verbose)
+        binding.result()
     return OUT
 
 
