@@ -640,6 +640,21 @@ def test_combine_strides_and_positions_outside(ex):
     assert torch.equal(ex.combine_rows(o, routing._replace(position=position)), ex.combine_rows(o, routing._replace(gates=gates)))
 
 
+def test_combine_gradients_against_differences(ex):
+    """The sum is linear in the rows and in the gates: a difference of any length gives the directional derivative."""
+    g = gen(62)
+    routing = ex.route_tokens(normal(g, 70, 9), 3, mask=torch.arange(70, device="cuda") % 8 != 1)
+    gates = routing.gates.clone().requires_grad_(True)
+    o, dy = normal(g, 210, 130).requires_grad_(True), normal(g, 70, 130)
+    do, dg = torch.autograd.grad(ex.combine_rows(o, routing._replace(gates=gates)), (o, gates), dy)
+    eo, eg = normal(g, 210, 130), normal(g, 70, 3) * (routing.position >= 0)
+    with torch.no_grad():
+        for grad, step, moved in ((do, eo, ex.combine_rows(eo, routing)), (dg, eg, ex.combine_rows(o, routing._replace(gates=eg)))):
+            a, b = (grad.double() * step.double()).sum(), (dy.double() * moved.double()).sum()
+            size = (grad.double() * step.double()).abs().sum() + (dy.double() * moved.double()).abs().sum()
+            assert (a - b).abs() <= 2.0**-20 * size
+
+
 # ---------------------------------------------------------------------------------------------------------------
 # The layer, and how all of it behaves as a part of a program
 # ---------------------------------------------------------------------------------------------------------------
@@ -696,6 +711,30 @@ def test_expert_mlp(ex, t, d, f, e, k, dtype, checkpoint):
     assert torch.equal(y, y2)
     dx, dlog = torch.autograd.grad(y2, (x, logits), dy)
     assert norm(dx, got[0].double()) < 8 * 2 * ULP[dtype] and norm(dlog, got[3].double()) < 8 * 2 * ULP[dtype]
+
+
+def test_expert_mlp_gradient_against_differences(ex):
+    """Differences of the layer in 64 bits along one direction of all its inputs, against the fp16 layer's gradients."""
+    g = gen(70)
+    t, d, f, e, k = 120, 96, 80, 6, 2
+    x, w_in, w_out, logits = layer(ex, g, t, d, f, e, k, FP16)
+    leaves = [v.requires_grad_(True) for v in (x, w_in, w_out, logits)]
+    routing = ex.route_tokens(logits, k)
+    dy = normal(g, t, d, dtype=FP16)
+    grads = torch.autograd.grad(ex.expert_mlp(x, w_in, w_out, routing, checkpoint=False), leaves, dy)
+    steps = [normal(g, *v.shape).double() * v.detach().double().std() for v in leaves]
+    chosen = routing.experts.long()
+
+    def value(h):
+        a, b, c, l = (v.detach().double() + h * s for v, s in zip(leaves, steps))
+        return (plain_layer(a, b, c, torch.softmax(l.gather(1, chosen), 1), routing.experts) * dy.double()).sum()
+
+    diff = (value(1e-4) - value(-1e-4)) / 2e-4
+    got = sum((a.double() * s).sum() for a, s in zip(grads, steps))
+    # six tensors rounded to fp16 between input and gradient, none of them along the direction in particular; the sums of
+    # thousands of such terms are compared by their magnitudes' root sum of squares
+    size = math.sqrt(sum(((a.double() * s) ** 2).sum().item() for a, s in zip(grads, steps)))
+    assert (got - diff).abs().item() <= 40 * 6 * ULP[FP16] * size
 
 
 def test_same_bits_in_every_run_and_on_another_stream(ex):
