@@ -9,9 +9,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/utils/pybind.h>
 
-#include <ATen/ops/empty.h>
-#include <ATen/ops/empty_like.h>
-#include <ATen/ops/zeros.h>
+#include <ATen/cuda/EmptyTensor.h>
 
 #include "../../include/flash_sinkhorn_b200.h"
 
@@ -52,9 +50,13 @@ std::string text(const std::string& s) { return s; }
 std::string text(int64_t v) { return std::to_string(v); }
 std::string text(const c10::Device& d) { return d.str(); }
 template <typename... Parts>
-void require(bool holds, const Parts&... parts) {
-  if (!holds) throw Refused((text(parts) + ...));
+[[noreturn]] void refuse(const Parts&... parts) {
+  throw Refused((text(parts) + ...));
 }
+#define REQUIRE(holds, ...) /* the message is put together only where it is needed */ \
+  do {                                                                                \
+    if (!(holds)) refuse(__VA_ARGS__);                                                \
+  } while (0)
 #define FS_CALL(name, ...) check_status(#name, lib.name(__VA_ARGS__))
 
 // The device of a call's tensors, current while it lives, and the stream of the caller there.
@@ -63,6 +65,10 @@ struct Place {
   void* stream;
   explicit Place(const Tensor& t) : guard(t.device()), stream(at::cuda::getCurrentCUDAStream(t.device().index()).stream()) {}
 };
+
+// Without a way through the dispatcher, which takes longer than the allocation.
+Tensor fresh(at::IntArrayRef size, at::ScalarType type, const Tensor& like) { return at::detail::empty_cuda(size, type, like.device(), c10::nullopt); }
+Tensor fresh(at::IntArrayRef size, const Tensor& like) { return fresh(size, like.scalar_type(), like); }
 
 int type_of(const Tensor& t) {
   return t.scalar_type() == at::kFloat ? FS_TYPE_F32 : t.scalar_type() == at::kHalf ? FS_TYPE_F16 : FS_TYPE_BF16;
@@ -75,26 +81,26 @@ std::string shape_of(const Tensor& t) {
 const char* type_name(const Tensor& t) { return c10::toString(t.scalar_type()); }
 void check_type(const char* name, const Tensor& t, bool fp32) {
   const auto k = t.scalar_type();
-  require(k == at::kHalf || k == at::kBFloat16 || (fp32 && k == at::kFloat), name, " must be of type ",
+  REQUIRE(k == at::kHalf || k == at::kBFloat16 || (fp32 && k == at::kFloat), name, " must be of type ",
                     fp32 ? "float32, float16 or bfloat16" : "float16 or bfloat16", ", got ", type_name(t));
 }
-void check_cuda(const char* name, const Tensor& t) { require(t.is_cuda(), name, " must be a CUDA tensor."); }
+void check_cuda(const char* name, const Tensor& t) { REQUIRE(t.is_cuda(), name, " must be a CUDA tensor."); }
 void check_place(const char* name, const Tensor& t, const char* first, const Tensor& f) {
-  require(t.device() == f.device(), name, " must be on the same CUDA device as ", first, " (", f.device(), "), got ", t.device());
+  REQUIRE(t.device() == f.device(), name, " must be on the same CUDA device as ", first, " (", f.device(), "), got ", t.device());
 }
 // A field of a routing of `position`'s tokens and slots.
 void check_field(const char* name, const Tensor& t, const Tensor& position, bool per_row, at::ScalarType type, const Tensor& on) {
   const bool fits = per_row ? t.dim() == 1 && t.size(0) == position.size(0) * position.size(1) : t.sizes() == position.sizes();
-  require(fits && t.scalar_type() == type && t.device() == on.device() && t.is_contiguous(), "routing.", name,
+  REQUIRE(fits && t.scalar_type() == type && t.device() == on.device() && t.is_contiguous(), "routing.", name,
                     " must be a contiguous ", c10::toString(type), " tensor on ", on.device(), " that fits ", shape_of(position),
                     " (tokens, slots), got ", type_name(t), " ", shape_of(t), " on ", t.device());
 }
 void check_position(const Tensor& position, const Tensor& on) {
-  require(position.dim() == 2 && position.size(1) >= 1, "routing.position must be of shape (T, k), got ", shape_of(position));
+  REQUIRE(position.dim() == 2 && position.size(1) >= 1, "routing.position must be of shape (T, k), got ", shape_of(position));
   check_field("position", position, position, false, at::kInt, on);
 }
 void check_offsets(const Tensor& offsets, const Tensor& on) {
-  require(offsets.dim() == 1 && offsets.scalar_type() == at::kInt && offsets.is_contiguous() && offsets.device() == on.device() &&
+  REQUIRE(offsets.dim() == 1 && offsets.scalar_type() == at::kInt && offsets.is_contiguous() && offsets.device() == on.device() &&
                         offsets.size(0) > 1,
                     "offsets must be a contiguous int32 tensor of shape (E + 1,) on ", on.device());
 }
@@ -114,7 +120,7 @@ bool aligned16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr(
 Tensor padded(const Tensor& t, int64_t r, int64_t c, int64_t from) {
   const Place at(t);
   const int64_t to = (c + 7) / 8 * 8;
-  Tensor out = at::empty({r, to}, t.options());
+  Tensor out = fresh({r, to}, t);
   FS_CALL(fs_combine, t.data_ptr(), type_of(t), from, (int)r, (int)r, 1, (int)c, nullptr, nullptr, out.data_ptr(), type_of(t), to, at.stream);
   return out;
 }
@@ -132,7 +138,7 @@ Tensor loadable_weights(const Tensor& w0) {
   if (aligned16(w0) && se % 8 == 0 && (se > 0 || e == 1) && ((sk == 1 && sn >= k && sn % 8 == 0) || (sn == 1 && sk >= n && sk % 8 == 0))) return w0;
   const Tensor w = w0.contiguous();
   if (k % 8 == 0 && aligned16(w)) return w;
-  require(e * n < (int64_t(1) << 31), "weight of ", k, " columns has too many rows to be padded");
+  REQUIRE(e * n < (int64_t(1) << 31), "weight of ", k, " columns has too many rows to be padded");
   return padded(w, e * n, k, k).view({e, n, (k + 7) / 8 * 8}).narrow(2, 0, k);
 }
 
@@ -155,11 +161,9 @@ std::vector<Tensor> route_raw(const Tensor& logits, int64_t k, const Tensor& bia
   const Place at(logits);
   const int64_t t = logits.size(0), e = logits.size(1), n = t * k;
   const size_t bytes = lib.fs_route_bytes((int)t, (int)e, (int)k);
-  const auto whole_numbers = logits.options().dtype(at::kInt);
-  Tensor gates = at::empty({t, k}, logits.options().dtype(at::kFloat)), experts = at::empty({t, k}, whole_numbers);
-  Tensor offsets = at::empty({e + 1}, whole_numbers), pairs = at::empty({n}, whole_numbers), rows = at::empty({n}, whole_numbers);
-  Tensor position = at::empty({t, k}, whole_numbers), ws;
-  if (bytes) ws = at::empty({(int64_t)bytes}, logits.options().dtype(at::kByte));
+  Tensor gates = fresh({t, k}, at::kFloat, logits), experts = fresh({t, k}, at::kInt, logits), offsets = fresh({e + 1}, at::kInt, logits);
+  Tensor pairs = fresh({n}, at::kInt, logits), rows = fresh({n}, at::kInt, logits), position = fresh({t, k}, at::kInt, logits), ws;
+  if (bytes) ws = fresh({(int64_t)bytes}, at::kByte, logits);
   FS_CALL(fs_route, logits.data_ptr(), type_of(logits), ld(logits), (int)t, (int)e, (int)k, floats(bias), static_cast<const uint8_t*>(data(mask)),
           over_all, floats(gates), experts.data_ptr<int>(), offsets.data_ptr<int>(), pairs.data_ptr<int>(), rows.data_ptr<int>(),
           position.data_ptr<int>(), data(ws), bytes, at.stream);
@@ -170,7 +174,7 @@ std::vector<Tensor> route_raw(const Tensor& logits, int64_t k, const Tensor& bia
 Tensor combine_raw(const Tensor& o, const Tensor& gates, const Tensor& position, at::ScalarType type, bool pad = false) {
   const Place at(o);
   const int64_t t = position.size(0), d = o.size(1), ldy = pad ? (d + 7) / 8 * 8 : d;
-  Tensor y = at::empty({t, ldy}, o.options().dtype(type));
+  Tensor y = fresh({t, ldy}, type, o);
   FS_CALL(fs_combine, o.data_ptr(), type_of(o), ld(o), (int)o.size(0), (int)t, (int)position.size(1), (int)d, floats(gates), ints(position),
           y.data_ptr(), type_of(y), ldy, at.stream);
   return pad ? y.narrow(1, 0, d) : y;
@@ -186,7 +190,7 @@ Tensor mm_raw(const Tensor& x0, const Tensor& rows, int64_t count, const Tensor&
     std::swap(n, k);
     std::swap(sn, sk);
   }
-  Tensor out = at::empty({count, n}, fp32 ? x.options().dtype(at::kFloat) : x.options());
+  Tensor out = fresh({count, n}, fp32 ? at::kFloat : x.scalar_type(), x);
   FS_CALL(fs_grouped_mm, x.data_ptr(), ld(x), (int)x.size(0), ints(rows), (int)count, w.data_ptr(), w.stride(0), sn, sk, (int)w.size(0), (int)n,
           (int)k, ints(offsets), out.data_ptr(), type_of(out), n, type_of(x), at.stream);
   return out;
@@ -195,7 +199,7 @@ Tensor wgrad_raw(const Tensor& dy0, const Tensor& x0, const Tensor& offsets) {
   const Place at(x0);
   const Tensor dy = loadable_rows(dy0), x = loadable_rows(x0);
   const int64_t e = offsets.size(0) - 1, n = dy.size(1), k = x.size(1);
-  Tensor out = at::empty({e, n, k}, x.options());
+  Tensor out = fresh({e, n, k}, x);
   FS_CALL(fs_grouped_mm_wgrad, dy.data_ptr(), ld(dy), x.data_ptr(), ld(x), (int)x.size(0), (int)e, (int)n, (int)k, ints(offsets), out.data_ptr(),
           type_of(x), at.stream);
   return out;
@@ -205,10 +209,10 @@ Tensor wgrad_raw(const Tensor& dy0, const Tensor& x0, const Tensor& offsets) {
 std::pair<Tensor, Tensor> act_raw(const Tensor& u, const Tensor& gates, const Tensor& pairs, bool checkpoint) {
   const Place at(u);
   const int64_t r = u.size(0), f = u.size(1) / 2;
-  Tensor h = at::empty({r, f}, u.options()), held;
+  Tensor h = fresh({r, f}, u), held;
   int8_t* codes = nullptr;
   if (checkpoint) {
-    held = at::empty({r * (2 * f + 2 * ((f + kBlock - 1) / kBlock))}, u.options().dtype(at::kByte));
+    held = fresh({r * (2 * f + 2 * ((f + kBlock - 1) / kBlock))}, at::kByte, u);
     codes = static_cast<int8_t*>(held.data_ptr());
   }
   FS_CALL(fs_gated_act, u.data_ptr(), type_of(u), ld(u), (int)r, (int)f, floats(gates), ints(pairs), h.data_ptr(), codes,
@@ -219,9 +223,9 @@ std::tuple<Tensor, Tensor, Tensor> act_grad_raw(const Tensor& u, const Tensor& h
                                                 const Tensor& dh, bool want_gates, bool want_h) {
   const Place at(dh);
   const int64_t r = dh.size(0), f = dh.size(1);
-  Tensor du = at::empty({r, 2 * f}, dh.options()), dgates, h;
-  if (want_gates) dgates = at::empty_like(gates);
-  if (want_h) h = at::empty({r, f}, dh.options());
+  Tensor du = fresh({r, 2 * f}, dh), dgates, h;
+  if (want_gates) dgates = fresh(gates.sizes(), gates);
+  if (want_h) h = fresh({r, f}, dh);
   const auto codes = static_cast<const int8_t*>(data(held));
   FS_CALL(fs_gated_act_grad, data(u), ld(u), codes, codes ? reinterpret_cast<const uint8_t*>(codes) + r * 2 * f : nullptr, type_of(dh), (int)r, (int)f,
           floats(gates), ints(pairs), ints(position), dh.data_ptr(), ld(dh), du.data_ptr(), floats(dgates), data(h), at.stream);
@@ -248,7 +252,7 @@ struct Route : torch::autograd::Function<Route> {
     Tensor out;
     if (grads[0].defined()) {
       const Tensor grad = grads[0].contiguous();
-      out = at::empty(logits.sizes(), logits.options());
+      out = fresh(logits.sizes(), logits);
       FS_CALL(fs_route_grad, logits.data_ptr(), type_of(logits), ld(logits), (int)logits.size(0), (int)logits.size(1), (int)gates.size(1),
               floats(s[1]), static_cast<const uint8_t*>(data(s[2])), over_all, floats(gates), ints(s[4]), floats(grad), out.data_ptr(), at.stream);
     }
@@ -314,8 +318,8 @@ struct Combine : torch::autograd::Function<Combine> {
       const Place at(position);
       const Tensor dy = rows_of(grads[0]);
       const int64_t t = position.size(0), k = position.size(1), d = dy.size(1);
-      d_o = at::empty({t * k, d}, dy.options());
-      if (o.defined()) dgates = at::empty_like(gates);
+      d_o = fresh({t * k, d}, dy);
+      if (o.defined()) dgates = fresh(gates.sizes(), gates);
       FS_CALL(fs_combine_grad, data(o), type_of(dy), ld(o), (int)t, (int)k, (int)d, floats(gates), ints(position), ints(s[3]), dy.data_ptr(), ld(dy),
               d_o.data_ptr(), floats(dgates), at.stream);
     }
@@ -356,23 +360,23 @@ struct Mlp : torch::autograd::Function<Mlp> {
 
 // ------------------------------------------------------------------ public calls
 std::vector<Tensor> route_tokens(const Tensor& logits0, int64_t k, const optional<Tensor>& bias0, const optional<Tensor>& mask0, bool over_all) {
-  require(logits0.dim() == 2, "logits must be 2D [T, E], got shape ", shape_of(logits0));
+  REQUIRE(logits0.dim() == 2, "logits must be 2D [T, E], got shape ", shape_of(logits0));
   check_type("logits", logits0, true);
   check_cuda("logits", logits0);
   const int64_t t = logits0.size(0), e = logits0.size(1);
-  require(e >= 1 && e <= kMaxExperts, "the number of experts must be between 1 and ", kMaxExperts, ", got ", e);
-  require(k >= 1 && k <= std::min(e, kMaxK), "k must be between 1 and ", std::min(e, kMaxK), ", got ", k);
-  require(t * k < (int64_t(1) << 31), "T * k must be below 2^31");
+  REQUIRE(e >= 1 && e <= kMaxExperts, "the number of experts must be between 1 and ", kMaxExperts, ", got ", e);
+  REQUIRE(k >= 1 && k <= std::min(e, kMaxK), "k must be between 1 and ", std::min(e, kMaxK), ", got ", k);
+  REQUIRE(t * k < (int64_t(1) << 31), "T * k must be below 2^31");
   Tensor bias = none(bias0), mask = none(mask0);
   if (bias.defined()) {
     check_place("bias", bias, "logits", logits0);
-    require(bias.dim() == 1 && bias.size(0) == e, "bias must have shape (", e, ",), got ", shape_of(bias));
-    require(!bias.requires_grad(), "bias must not require grad (it only takes part in the choice)");
+    REQUIRE(bias.dim() == 1 && bias.size(0) == e, "bias must have shape (", e, ",), got ", shape_of(bias));
+    REQUIRE(!bias.requires_grad(), "bias must not require grad (it only takes part in the choice)");
     bias = bias.to(at::kFloat).contiguous();
   }
   if (mask.defined()) {
     check_place("mask", mask, "logits", logits0);
-    require(mask.dim() == 1 && mask.size(0) == t && mask.scalar_type() == at::kBool, "mask must be a bool tensor of shape (", t, ",), got ",
+    REQUIRE(mask.dim() == 1 && mask.size(0) == t && mask.scalar_type() == at::kBool, "mask must be a bool tensor of shape (", t, ",), got ",
                       type_name(mask), " ", shape_of(mask));
     mask = mask.contiguous();
   }
@@ -382,13 +386,13 @@ std::vector<Tensor> route_tokens(const Tensor& logits0, int64_t k, const optiona
 
 Tensor grouped_mm(const Tensor& x0, const Tensor& w0, const Tensor& offsets, const optional<Tensor>& rows0, const optional<Tensor>& position0,
                   bool gather) {
-  require(x0.dim() == 2 && w0.dim() == 3, "x must be 2D and weight 3D [E, N, K], got shapes ", shape_of(x0), " and ", shape_of(w0));
+  REQUIRE(x0.dim() == 2 && w0.dim() == 3, "x must be 2D and weight 3D [E, N, K], got shapes ", shape_of(x0), " and ", shape_of(w0));
   check_type("x", x0, false);
-  require(w0.scalar_type() == x0.scalar_type(), "weight must be of the type of x (", type_name(x0), "), got ", type_name(w0));
+  REQUIRE(w0.scalar_type() == x0.scalar_type(), "weight must be of the type of x (", type_name(x0), "), got ", type_name(w0));
   check_cuda("x", x0);
   check_place("weight", w0, "x", x0);
   const int64_t e = w0.size(0), n = w0.size(1), k = w0.size(2);
-  require(x0.size(1) == k && k > 0 && n > 0, "x must have as many columns as weight (", k, " > 0), got ", x0.size(1),
+  REQUIRE(x0.size(1) == k && k > 0 && n > 0, "x must have as many columns as weight (", k, " > 0), got ", x0.size(1),
                     "; N must be > 0, got ", n);
   check_offsets(offsets, x0);
   int64_t count = x0.size(0);
@@ -403,18 +407,18 @@ Tensor grouped_mm(const Tensor& x0, const Tensor& w0, const Tensor& offsets, con
       position = Tensor();
     }
     const int64_t want = gather ? position.size(0) : count;
-    require(x0.size(0) == want, "x must have ", want, " rows, got ", x0.size(0));
+    REQUIRE(x0.size(0) == want, "x must have ", want, " rows, got ", x0.size(0));
   }
-  require(!gather || position.size(1) <= kMaxK, "k must be at most ", kMaxK);
-  require(offsets.size(0) == e + 1 && e <= kMaxExperts, "groups must have as many experts as weight (", e, ", at most ", kMaxExperts,
+  REQUIRE(!gather || position.size(1) <= kMaxK, "k must be at most ", kMaxK);
+  REQUIRE(offsets.size(0) == e + 1 && e <= kMaxExperts, "groups must have as many experts as weight (", e, ", at most ", kMaxExperts,
                     "), got ", offsets.size(0) - 1);
-  require(count < (int64_t(1) << 31) && x0.size(0) < (int64_t(1) << 31), "rows must be fewer than 2^31");
+  REQUIRE(count < (int64_t(1) << 31) && x0.size(0) < (int64_t(1) << 31), "rows must be fewer than 2^31");
   if (!wants_grad({&x0, &w0})) return mm_raw(x0, rows, count, w0, offsets, false, false);
   return GroupedMm::apply(x0, w0, offsets, maybe(rows), maybe(position), count);
 }
 
 Tensor gated_act(const Tensor& u0, const optional<Tensor>& gates0, const optional<Tensor>& pairs0, const optional<Tensor>& position0, bool checkpoint) {
-  require(u0.dim() == 2 && u0.size(1) > 0 && u0.size(1) % 2 == 0, "u must be 2D [R, 2 F] with F > 0, got shape ", shape_of(u0));
+  REQUIRE(u0.dim() == 2 && u0.size(1) > 0 && u0.size(1) % 2 == 0, "u must be 2D [R, 2 F] with F > 0, got shape ", shape_of(u0));
   check_type("u", u0, true);
   check_cuda("u", u0);
   const Tensor gates = none(gates0), pairs = none(pairs0), position = none(position0);
@@ -422,23 +426,23 @@ Tensor gated_act(const Tensor& u0, const optional<Tensor>& gates0, const optiona
     check_position(position, u0);
     check_field("gates", gates, position, false, at::kFloat, u0);
     check_field("pairs", pairs, position, true, at::kInt, u0);
-    require(u0.size(0) == pairs.size(0), "u must have ", pairs.size(0), " rows, got ", u0.size(0));
+    REQUIRE(u0.size(0) == pairs.size(0), "u must have ", pairs.size(0), " rows, got ", u0.size(0));
   }
-  require(u0.size(0) < (int64_t(1) << 31), "rows must be fewer than 2^31");
+  REQUIRE(u0.size(0) < (int64_t(1) << 31), "rows must be fewer than 2^31");
   if (!wants_grad({&u0, &gates})) return act_raw(rows_of(u0), gates, pairs, false).first;
   return GatedAct::apply(u0, maybe(gates), maybe(pairs), maybe(position), checkpoint);
 }
 
 Tensor combine_rows(const Tensor& o0, const Tensor& gates0, const Tensor& pairs, const Tensor& position, bool weighted) {
-  require(o0.dim() == 2 && o0.size(1) > 0, "o must be 2D [T * k, D] with D > 0, got shape ", shape_of(o0));
+  REQUIRE(o0.dim() == 2 && o0.size(1) > 0, "o must be 2D [T * k, D] with D > 0, got shape ", shape_of(o0));
   check_type("o", o0, true);
   check_cuda("o", o0);
   check_position(position, o0);
   check_field("gates", gates0, position, false, at::kFloat, o0);
   check_field("pairs", pairs, position, true, at::kInt, o0);
-  require(o0.size(0) == pairs.size(0), "o must have ", pairs.size(0), " rows, got ", o0.size(0));
-  require(position.size(1) <= kMaxK, "k must be at most ", kMaxK, ", got ", position.size(1));
-  require(o0.size(0) < (int64_t(1) << 31), "rows must be fewer than 2^31");
+  REQUIRE(o0.size(0) == pairs.size(0), "o must have ", pairs.size(0), " rows, got ", o0.size(0));
+  REQUIRE(position.size(1) <= kMaxK, "k must be at most ", kMaxK, ", got ", position.size(1));
+  REQUIRE(o0.size(0) < (int64_t(1) << 31), "rows must be fewer than 2^31");
   const Tensor gates = weighted ? gates0 : Tensor();
   if (wants_grad({&o0, &gates})) return Combine::apply(o0, maybe(gates), position, pairs);
   return combine_raw(rows_of(o0), gates, position, o0.scalar_type());
@@ -446,9 +450,9 @@ Tensor combine_rows(const Tensor& o0, const Tensor& gates0, const Tensor& pairs,
 
 Tensor expert_mlp(const Tensor& x0, const Tensor& w_in0, const Tensor& w_out0, const Tensor& gates, const Tensor& offsets, const Tensor& pairs,
                   const Tensor& rows, const Tensor& position, bool checkpoint) {
-  require(x0.dim() == 2 && w_in0.dim() == 3 && w_out0.dim() == 3, "x must be 2D, w_in and w_out 3D");
+  REQUIRE(x0.dim() == 2 && w_in0.dim() == 3 && w_out0.dim() == 3, "x must be 2D, w_in and w_out 3D");
   check_type("x", x0, false);
-  require(w_in0.scalar_type() == x0.scalar_type() && w_out0.scalar_type() == x0.scalar_type(), "w_in and w_out must be of the type of x (",
+  REQUIRE(w_in0.scalar_type() == x0.scalar_type() && w_out0.scalar_type() == x0.scalar_type(), "w_in and w_out must be of the type of x (",
                     type_name(x0), "), got ", type_name(w_in0), " and ", type_name(w_out0));
   check_cuda("x", x0);
   check_place("w_in", w_in0, "x", x0);
@@ -459,9 +463,9 @@ Tensor expert_mlp(const Tensor& x0, const Tensor& w_in0, const Tensor& w_out0, c
   check_field("rows", rows, position, true, at::kInt, x0);
   check_offsets(offsets, x0);
   const int64_t t = x0.size(0), d = x0.size(1), e = w_in0.size(0), f = w_out0.size(2);
-  require(w_in0.size(1) == 2 * f && w_in0.size(2) == d && w_out0.size(0) == e && w_out0.size(1) == d && d > 0 && f > 0,
+  REQUIRE(w_in0.size(1) == 2 * f && w_in0.size(2) == d && w_out0.size(0) == e && w_out0.size(1) == d && d > 0 && f > 0,
                     "w_in must be [E, 2 F, ", d, "] and w_out [E, ", d, ", F], got ", shape_of(w_in0), " and ", shape_of(w_out0));
-  require(position.size(0) == t && offsets.size(0) == e + 1 && position.size(1) <= kMaxK && e <= kMaxExperts && position.numel() < (int64_t(1) << 31),
+  REQUIRE(position.size(0) == t && offsets.size(0) == e + 1 && position.size(1) <= kMaxK && e <= kMaxExperts && position.numel() < (int64_t(1) << 31),
                     "routing must be of ", t, " tokens and ", e, " experts (at most ", kMaxExperts, "), at most ", kMaxK, " for a token");
   if (wants_grad({&x0, &w_in0, &w_out0, &gates})) return Mlp::apply(x0, w_in0, w_out0, gates, offsets, pairs, rows, position, checkpoint);
   const int64_t count = pairs.size(0);
