@@ -136,7 +136,8 @@ Tensor loadable_rows(const Tensor& t0) {
 Tensor loadable_weights(const Tensor& w0) {
   const int64_t e = w0.size(0), n = w0.size(1), k = w0.size(2), se = w0.stride(0), sn = w0.stride(1), sk = w0.stride(2);
   if (aligned16(w0) && se % 8 == 0 && (se > 0 || e == 1) && ((sk == 1 && sn >= k && sn % 8 == 0) || (sn == 1 && sk >= n && sk % 8 == 0))) return w0;
-  const Tensor w = w0.contiguous();
+  Tensor w = w0.contiguous();
+  if (w.stride(0) != n * k || w.stride(1) != k || w.stride(2) != 1) w = w.as_strided({e, n, k}, {n * k, k, 1});  // of dimensions of size 1
   if (k % 8 == 0 && aligned16(w)) return w;
   REQUIRE(e * n < (int64_t(1) << 31), "weight of ", k, " columns has too many rows to be padded");
   return padded(w, e * n, k, k).view({e, n, (k + 7) / 8 * 8}).narrow(2, 0, k);

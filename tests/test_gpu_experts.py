@@ -348,6 +348,23 @@ def test_grouped_mm_strides_and_alignment(ex):
                        ex.grouped_mm(wide[:1, :k].repeat(r, 1), weights[:, :n, :k], off))
 
 
+@pytest.mark.parametrize("r", [1, 2, 40])
+@pytest.mark.parametrize("n,k,strides", [(64, 72, (64 * 72 + 1, 72, 1)), (64, 72, (0, 72, 1)), (1, 64, (3, 5, 1)), (64, 1, (7, 1, 3)),
+                                         (1, 1, (2, 3, 5)), (72, 64, (5, 1, 72))])
+def test_grouped_mm_strides_of_single_experts_and_features(ex, r, n, k, strides):
+    """A dimension of size 1 may have any stride."""
+    g = gen(22)
+    w = normal(g, 8000, dtype=BF16).as_strided((1, n, k), strides)
+    x = normal(g, r, k, dtype=BF16)
+    off = offsets_of([r])
+    check_mm(ex, x, w, off)
+    check_mm(ex, normal(g, r, n, dtype=BF16), w.transpose(1, 2), off)
+    leaf = w.detach().requires_grad_(True)
+    (dw,) = torch.autograd.grad(ex.grouped_mm(x, leaf, off).sum(), leaf)
+    size = x.double().abs().sum(0)
+    assert ((dw.double() - x.double().sum(0)).abs() <= ULP[BF16] * x.double().sum(0).abs() + ACC * size * min(r, 64)).all()
+
+
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
 @pytest.mark.parametrize("n,k", [(64, 128), (256, 256), (200, 320)])
 def test_grouped_mm_keeps_groups_apart(ex, bad, n, k):
