@@ -632,15 +632,15 @@ __device__ __forceinline__ Codes<VEC> encode(const float (&x)[VEC], unsigned cod
   memcpy(&q, w, VEC);
   return q;
 }
-// The values that codes stand for: code * scale, as (2^23 + 128 + code) * scale - (2^23 + 128) * scale with one exact rounding.
+// The values that codes stand for: ((2^23 + 128 + code) - (2^23 + 128)) * scale, exact in both steps. (2^23 times the scale is beyond
+// fp32 for blocks from 2^111 on, so the difference comes first.)
 template <int VEC>
 __device__ __forceinline__ void decode(const Codes<VEC>& codes, float scale, float (&x)[VEC]) {
-  const float off = -(kFromByte + 128.f) * scale;
   uint32_t w[(VEC + 3) / 4] = {};
   memcpy(w, &codes, VEC);
 #pragma unroll
   for (int i = 0; i < VEC; ++i)
-    x[i] = fmaf(__uint_as_float(__byte_perm(w[i / 4] ^ 0x80808080u, 0x4b000000u, 0x7440u + (unsigned)(i % 4))), scale, off);
+    x[i] = (__uint_as_float(__byte_perm(w[i / 4] ^ 0x80808080u, 0x4b000000u, 0x7440u + (unsigned)(i % 4))) - (kFromByte + 128.f)) * scale;
 }
 
 __device__ __forceinline__ float row_gate(const ActArgs& a, int r, bool& routed) {

@@ -1,0 +1,41 @@
+"""Routed experts at the ends of their ranges: magnitudes, sizes, threads, derivatives that are not theirs to give.
+
+Bounds are those of the operators' other tests: half a unit in the last place for each rounding to the type, ``FUN`` for
+the sigmoid and the products around it, ``ACC`` per term of a sum in fp32.
+"""
+import pytest
+import torch
+
+from test_gpu_experts import BF16, FP32, FUN, TINY, ULP, act_reference, ex, gen, held_in_8_bits, normal, within  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def large_blocks(dtype, top, seed):
+    """Rows [g | v] of one block each: a large g beside an ordinary v, and the other way round; zeros and ones in the large one."""
+    g = gen(seed)
+    rows = []
+    for big_first in (True, False):
+        for power in (104, 105, 110, 111, 112, 119, 120, 126, 127):
+            big = (torch.rand(32, generator=g, device="cuda") * 2 - 1) * (top * 2.0**power)
+            big[0], big[1], big[2], big[3] = top * 2.0**power, -top * 2.0**power, 0.0, 1.0
+            small = torch.rand(32, generator=g, device="cuda") * 0.9 - 0.45
+            rows.append(torch.cat([big, small] if big_first else [small, big]))
+    return torch.stack(rows).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+def test_gated_act_checkpoint_of_large_values(ex, dtype):  # noqa: F811
+    """Blocks up to the end of the type's range come back as their codes say, and their gradients with them."""
+    u = large_blocks(dtype, 1.984375, 1)  # 127 / 64: the largest of a block is its 127th step
+    dh = normal(gen(2), u.shape[0], 32, scale=2.0**-40, dtype=dtype)
+    h, held = ex._act(u, None, None, True)
+    du, _, again = ex._act_grad(None, held, None, None, None, dh, False, True)
+    want, dwant, size, _ = act_reference(u, 1.0, dh, True)
+    within(h, want, (ULP[dtype] + FUN) * want.abs() + TINY[dtype])
+    within(du, dwant, ULP[dtype] * dwant.abs() + FUN * size + TINY[dtype])
+    held_u = torch.cat([held_in_8_bits(u[:, :32]), held_in_8_bits(u[:, 32:])], 1)
+    want = act_reference(held_u, 1.0, dh, False)[0]
+    within(again, want, (ULP[dtype] + FUN) * want.abs() + TINY[dtype])
+    leaf = u.clone().requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(ex.gated_act(leaf), leaf, dh)[0], du)
