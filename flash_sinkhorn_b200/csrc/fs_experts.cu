@@ -633,14 +633,15 @@ __device__ __forceinline__ Codes<VEC> encode(const float (&x)[VEC], unsigned cod
   return q;
 }
 // The values that codes stand for: ((2^23 + 128 + code) - (2^23 + 128)) * scale, exact in both steps. (2^23 times the scale is beyond
-// fp32 for blocks from 2^111 on, so the difference comes first.)
+// fp32 for blocks from 2^111 on, so the difference comes first. A block's largest of 1.992 * 2^127 or more is held as 64 * 2^122 =
+// 2^128: rounded towards zero, the product is the largest finite value, off by a quarter of a step at most.)
 template <int VEC>
 __device__ __forceinline__ void decode(const Codes<VEC>& codes, float scale, float (&x)[VEC]) {
   uint32_t w[(VEC + 3) / 4] = {};
   memcpy(w, &codes, VEC);
 #pragma unroll
   for (int i = 0; i < VEC; ++i)
-    x[i] = (__uint_as_float(__byte_perm(w[i / 4] ^ 0x80808080u, 0x4b000000u, 0x7440u + (unsigned)(i % 4))) - (kFromByte + 128.f)) * scale;
+    x[i] = __fmul_rz(__uint_as_float(__byte_perm(w[i / 4] ^ 0x80808080u, 0x4b000000u, 0x7440u + (unsigned)(i % 4))) - (kFromByte + 128.f), scale);
 }
 
 __device__ __forceinline__ float row_gate(const ActArgs& a, int r, bool& routed) {

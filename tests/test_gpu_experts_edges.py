@@ -39,3 +39,23 @@ def test_gated_act_checkpoint_of_large_values(ex, dtype):  # noqa: F811
     within(again, want, (ULP[dtype] + FUN) * want.abs() + TINY[dtype])
     leaf = u.clone().requires_grad_(True)
     assert torch.equal(torch.autograd.grad(ex.gated_act(leaf), leaf, dh)[0], du)
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+def test_gated_act_checkpoint_of_the_largest_values(ex, dtype):  # noqa: F811
+    """A largest magnitude that rounds up to 2^128 stands for the largest of fp32: within 1/128 of itself, not an infinity."""
+    top = torch.finfo(dtype).max
+    u = torch.ones(4, 64, device="cuda", dtype=dtype)
+    u[0, 0], u[1, 0], u[2, 32], u[3, 40] = top, -top, top, -top
+    u[:2, 1], u[2:, 33] = 0.5 * top, -0.25 * top  # 32 and 16 steps of 2^122
+    u[:2, 32:] *= 0.25
+    dh = torch.full((4, 32), 2.0**-40, device="cuda", dtype=dtype)
+    h, held = ex._act(u, None, None, True)
+    du, _, again = ex._act_grad(None, held, None, None, None, dh, False, True)
+    held_u = torch.cat([held_in_8_bits(u[:, :32]), held_in_8_bits(u[:, 32:])], 1).clamp(-torch.finfo(FP32).max, torch.finfo(FP32).max)
+    assert ((held_u - u.double()).abs() <= u.double().abs().reshape(4, 2, 32).amax(2).repeat_interleave(32, 1) / 128).all()
+    want, dwant, size, _ = act_reference(held_u, 1.0, dh, False)
+    within(du, dwant, ULP[dtype] * dwant.abs() + FUN * size + TINY[dtype])
+    fits = want.abs() < top * (1 - 2 * ULP[dtype])  # 0.73 and 0.25 times the largest
+    within(again[fits], want[fits], (ULP[dtype] + FUN) * want[fits].abs() + TINY[dtype])
+    assert fits.all() and torch.isfinite(h).all()
