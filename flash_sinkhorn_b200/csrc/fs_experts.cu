@@ -484,12 +484,23 @@ void plan_route(int T, int& chunk, int& blocks) {
   blocks = T > 0 ? (T + chunk - 1) / chunk : 1;
 }
 
+// Lets `kernel` take `most` bytes of dynamic shared memory, once for each device. The limit belongs to the kernel and all host
+// threads, so it is the most that any call takes and never the size of the present one. `allowed`: the kernel's own, devices
+// on which it is set.
 template <typename K>
-int allow_smem(K kernel, size_t bytes) {
-  if (bytes <= 48 * 1024) return FS_OK;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+int allow_smem(K kernel, size_t most, std::atomic<uint64_t>& allowed) {
+  if (most <= 48 * 1024) return FS_OK;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (e == cudaSuccess && !(allowed.load(std::memory_order_relaxed) & bit)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+    if (e == cudaSuccess) allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
   return e == cudaSuccess ? FS_OK : report_error(FS_ERR_CUDA, cudaGetErrorString(e));
 }
+
+std::atomic<uint64_t> g_order_allowed{0};  // of route_order_kernel, which all instances of launch_route share
 
 template <typename T, int PER>
 int launch_route(RouteArgs a, bool grad, cudaStream_t st) {
@@ -499,7 +510,8 @@ int launch_route(RouteArgs a, bool grad, cudaStream_t st) {
   if (grad) {
     const long long want = ((long long)a.T + kGradWarps - 1) / kGradWarps;
     const size_t bytes = (size_t)kGradWarps * 32 * PER * 4;
-    const int s = allow_smem(route_grad_kernel<T, PER>, bytes);
+    static std::atomic<uint64_t> grad_allowed{0};
+    const int s = allow_smem(route_grad_kernel<T, PER>, bytes, grad_allowed);
     if (s != FS_OK) return s;
     const long long most = 148 * kGradCtas<PER>;
     route_grad_kernel<T, PER><<<(int)(want < most ? want : most), kGradWarps * 32, bytes, st>>>(a);
@@ -507,9 +519,10 @@ int launch_route(RouteArgs a, bool grad, cudaStream_t st) {
   }
   constexpr int kWarps = kSelectWarps<PER>;
   const size_t one = (size_t)(a.blocks > 1 ? 1 : 1 + kWarps) * a.E * 4, two = (size_t)(2 + kOrderWarps) * a.E * 4;
-  int s = allow_smem(route_select_kernel<T, PER>, one);
+  static std::atomic<uint64_t> select_allowed{0};
+  int s = allow_smem(route_select_kernel<T, PER>, (size_t)(1 + kWarps) * 32 * PER * 4, select_allowed);
   if (s != FS_OK) return s;
-  if (a.blocks > 1 && (s = allow_smem(route_order_kernel, two)) != FS_OK) return s;
+  if (a.blocks > 1 && (s = allow_smem(route_order_kernel, (size_t)(2 + kOrderWarps) * kMaxExperts * 4, g_order_allowed)) != FS_OK) return s;
   route_select_kernel<T, PER><<<a.blocks, kWarps * 32, one, st>>>(a);
   if (a.blocks > 1) route_order_kernel<<<a.blocks, kOrderWarps * 32, two, st>>>(a);
   return launched(a.blocks > 1 ? 2 : 1);

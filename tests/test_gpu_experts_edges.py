@@ -3,6 +3,8 @@
 Bounds are those of the operators' other tests: half a unit in the last place for each rounding to the type, ``FUN`` for
 the sigmoid and the products around it, ``ACC`` per term of a sum in fp32.
 """
+import threading
+
 import pytest
 import torch
 
@@ -59,3 +61,29 @@ def test_gated_act_checkpoint_of_the_largest_values(ex, dtype):  # noqa: F811
     fits = want.abs() < top * (1 - 2 * ULP[dtype])  # 0.73 and 0.25 times the largest
     within(again[fits], want[fits], (ULP[dtype] + FUN) * want[fits].abs() + TINY[dtype])
     assert fits.all() and torch.isfinite(h).all()
+
+
+def test_routing_from_several_threads(ex):  # noqa: F811
+    """Threads whose routings need different amounts of shared memory do not take it from one another."""
+    failed, outputs = [], {}
+
+    def work(name, e, k, tokens, times):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                logits = normal(gen(e), tokens, e).requires_grad_(True)
+                for i in range(times):
+                    r = ex.route_tokens(logits, k, normalize="all")
+                    (d,) = torch.autograd.grad(r.gates, (logits,), torch.ones_like(r.gates))
+                    if i in (0, times - 1):
+                        outputs[name, i > 0] = [v.detach().clone() for v in (*r, d)]
+            torch.cuda.synchronize()
+        except Exception as error:
+            failed.append((name, str(error)))
+
+    sizes = [(1024, 2, 500), (512, 2, 500), (400, 3, 300), (1024, 4, 40), (700, 1, 64), (370, 2, 200)]
+    threads = [threading.Thread(target=work, args=(i, *size, 1000)) for i, size in enumerate(sizes)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not failed, failed[:3]
+    for i in range(len(sizes)):
+        assert all(torch.equal(a, b) for a, b in zip(outputs[i, False], outputs[i, True]))
