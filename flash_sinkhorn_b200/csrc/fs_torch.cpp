@@ -143,7 +143,11 @@ Tensor loadable_weights(const Tensor& w0) {
   return padded(w, e * n, k, k).view({e, n, (k + 7) / 8 * 8}).narrow(2, 0, k);
 }
 
+// Whether a call goes by way of autograd: for a gradient, and for tensors with a forward-mode tangent (whatever the gradient
+// mode), which these operators have no rule for: autograd's refusal is better than a result whose tangent counts as zero.
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    if (t->defined() && t->_fw_grad(0).defined()) return true;
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : ts)
     if (t->defined() && t->requires_grad()) return true;

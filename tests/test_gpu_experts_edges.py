@@ -87,3 +87,28 @@ def test_routing_from_several_threads(ex):  # noqa: F811
     assert not failed, failed[:3]
     for i in range(len(sizes)):
         assert all(torch.equal(a, b) for a, b in zip(outputs[i, False], outputs[i, True]))
+
+
+@pytest.mark.parametrize("mode", ["gradients", "no_grad"])
+def test_forward_mode_derivatives_are_refused(ex, mode):  # noqa: F811
+    """A tangent is not dropped, which would count as a derivative of zero."""
+    g = gen(5)
+    logits, u, o, gates = normal(g, 6, 8), normal(g, 12, 64), normal(g, 12, 32), torch.rand(6, 2, device="cuda")
+    x, w, w_in, w_out = (normal(g, *s, dtype=BF16) for s in ((12, 64), (8, 16, 64), (8, 32, 32), (8, 32, 16)))
+    y = normal(g, 6, 32, dtype=BF16)
+    r = ex.route_tokens(logits, 2)
+    off = r.offsets
+    calls = [
+        (lambda t: ex.route_tokens(t, 2), logits), (lambda t: ex.grouped_mm(t, w, off), x), (lambda t: ex.grouped_mm(x, t, off), w),
+        (lambda t: ex.gated_act(t), u), (lambda t: ex.gated_act(u, r._replace(gates=t), checkpoint=False), gates),
+        (lambda t: ex.combine_rows(t, r, weighted=False), o), (lambda t: ex.combine_rows(o, r._replace(gates=t)), gates),
+        (lambda t: ex.expert_mlp(t, w_in, w_out, r), y), (lambda t: ex.expert_mlp(y, t, w_out, r), w_in),
+        (lambda t: ex.expert_mlp(y, w_in, t, r), w_out), (lambda t: ex.expert_mlp(y, w_in, w_out, r._replace(gates=t)), gates),
+    ]
+    with torch.autograd.forward_ad.dual_level(), torch.set_grad_enabled(mode == "gradients"):
+        for i, (call, t) in enumerate(calls):
+            with pytest.raises(RuntimeError, match="jvp"):
+                call(torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)))
+                pytest.fail(f"call {i} was not refused")
+    for call, t in calls:  # without a tangent they go through
+        call(t)
