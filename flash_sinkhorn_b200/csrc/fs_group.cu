@@ -17,7 +17,10 @@
 // thread from beginning to end: choosing it anew for every instruction cost 500 clocks a stage, as much as the products of a
 // 256 x 256 tile), and eight write the other one out, through shared memory in pieces of 64 bytes. Rows in another order are
 // fetched by eight more, 16 bytes a lane (cp.async): TMA's loads of four rows each took 75 clocks apiece, 2.6 times the time
-// of the whole product. Group boundaries are read by the kernel itself; every CTA takes every n-th tile, features fastest,
+// of the whole product. That is for single CTAs: in a pair, rows that one CTA has written have to reach the thread of the other
+// one that issues the products by a release and an acquire at the cluster's scope, about a microsecond for each stage of
+// 0.27 (541 -> 941 us for 65536 rows of 64 groups, 2048 x 2048), so products that want pairs take their rows in order, and
+// whoever has them in another one copies them first (fs_grouped_mm_in_order). Group boundaries are read by the kernel itself; every CTA takes every n-th tile, features fastest,
 // so that the CTAs working at one time share a group's weights and rows in L2.
 #include "fs_experts.cuh"
 #include "fs_ptx.cuh"
@@ -77,8 +80,33 @@ __device__ __forceinline__ uint32_t in_leader(uint32_t addr) {  // the same shar
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// Frees something of the leader's: only execution is ordered, for which the default scope will do.
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// Shared memory that this CTA has written goes to the thread of the leader that issues the products reading it: released and
+// acquired at the cluster's scope. For the end of a group only, once in a tile.
+__device__ __forceinline__ void arrive_release_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool wait_acquire_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  const long long t0 = clock64();
+  for (;;) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if (*abort_flag) return false;
+    if (clock64() - t0 > kSpinLimit) {
+      *abort_flag = 1;
+      return false;
+    }
+  }
 }
 template <int CG>
 __device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
@@ -319,7 +347,7 @@ __device__ __forceinline__ int load_early(const int* p) {
   return v;
 }
 
-// COPY (rows form): the rows come one by one.
+// COPY (rows form, single CTAs): the rows come one by one.
 template <int FORM, int CG, int BN, bool COPY>
 __global__ void __launch_bounds__(kThreads + (COPY ? 32 * kCopyWarps : 0), 1)
 group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB) {
@@ -327,7 +355,7 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
   constexpr uint32_t kA = 2 * kHalfTile, kB = BNC * 128, kStage = kA + kB;
   constexpr bool A_MN = FORM != ROWS_K, B_MN = FORM == WEIGHTS;
   constexpr uint32_t kColumns = 2 * BN;
-  static_assert(kColumns >= 32 && kColumns <= 512 && kStage % 1024 == 0 && !(COPY && FORM == WEIGHTS), "tile");
+  static_assert(kColumns >= 32 && kColumns <= 512 && kStage % 1024 == 0 && !(COPY && (FORM == WEIGHTS || CG == 2)), "tile");
   extern __shared__ uint8_t raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   uint8_t* staging = ring + (size_t)a.nstage * kStage;  // 2 KB for each warp that writes results
@@ -347,7 +375,7 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
     read_groups<FORM != WEIGHTS>(a, gs, ts, (a.N + 128 * CG - 1) / (128 * CG), BN);
   } else if (warp == kLoadWarp && lane == 0) {
     for (int s = 0; s < a.nstage; ++s) {
-      mbar_init(bar(FULL + s), CG * (COPY ? 2 : 1));  // in CTA 0: both CTAs' loads and, with COPY, reports
+      mbar_init(bar(FULL + s), CG + (COPY ? 1 : 0));  // in CTA 0: both CTAs' loads; with COPY, the load and the report
       mbar_init(bar(EMPTY + s), 1);
       mbar_init(bar(PARTS + s), COPY ? kCopyGroup : 1);  // what the reporting warp waits for
     }
@@ -439,7 +467,8 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
         tc_fence_after();
         const uint32_t d = tmem + buf * BN;
         for (int kb = 0; kb < t.blocks; ++kb) {
-          if (!mbar_wait(bar(FULL + s), ph, abort_flag)) {
+          const bool end = CG == 2 && FORM == WEIGHTS && kb == t.blocks - 1 && (t.hi - t.lo) % 16 != 0;  // by way of warp kReportWarp
+          if (!(end ? wait_acquire_cluster(bar(FULL + s), ph, abort_flag) : mbar_wait(bar(FULL + s), ph, abort_flag))) {
             ok = false;
             break;
           }
@@ -576,7 +605,7 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
   } else if (COPY) {
     // ===================== reports of copied stages =====================
     // Copies are ordinary writes: their completion, seen here, is made visible to the tensor core, which reads by the
-    // asynchronous proxy, and reported to CTA 0 by a thread that has no copies of its own to wait for.
+    // asynchronous proxy, and reported by a thread that has no copies of its own to wait for.
     int s = 0;
     uint32_t ph = 0;
     bool ok = lane == 0;
@@ -588,7 +617,7 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
           break;
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        arrive_cluster(full_bar(s));
+        mbar_arrive(bar(FULL + s));
         if (++s == a.nstage) {
           s = 0;
           ph ^= 1;
@@ -614,7 +643,10 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
           *reinterpret_cast<uint4*>(block + h * kHalfTile + from * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) arrive_cluster(full_bar(stage));
+      if (lane == 0) {
+        if (CG == 2) arrive_release_cluster(full_bar(stage));
+        else mbar_arrive(bar(FULL + stage));
+      }
       __syncwarp();
     }
   }
@@ -804,10 +836,11 @@ int launch_group(GroupArgs a, const CUtensorMap& mapA, const CUtensorMap& mapB, 
 template <int CG, int BN>
 int launch_rows(const GroupArgs& a, bool k_major, const CUtensorMap& mapA, cudaStream_t st) {
   CUtensorMap mapB = {};
-  if (!a.rows && !encode_rows(&mapB, a.type, a.x, a.K, a.M, a.ldx, BN / CG)) return no_map();
   const long long tiles = ((a.R + BN - 1ll) / BN + a.E + 1) * ((a.N + 128 * CG - 1) / (128 * CG));
-  if (a.rows)
-    return k_major ? launch_group<ROWS_K, CG, BN, true>(a, mapA, mapB, tiles, st) : launch_group<ROWS_MN, CG, BN, true>(a, mapA, mapB, tiles, st);
+  if constexpr (CG == 1)
+    if (a.rows)
+      return k_major ? launch_group<ROWS_K, CG, BN, true>(a, mapA, mapB, tiles, st) : launch_group<ROWS_MN, CG, BN, true>(a, mapA, mapB, tiles, st);
+  if (!encode_rows(&mapB, a.type, a.x, a.K, a.M, a.ldx, BN / CG)) return no_map();
   return k_major ? launch_group<ROWS_K, CG, BN, false>(a, mapA, mapB, tiles, st) : launch_group<ROWS_MN, CG, BN, false>(a, mapA, mapB, tiles, st);
 }
 
@@ -816,9 +849,14 @@ int launch_rows(const GroupArgs& a, bool k_major, const CUtensorMap& mapA, cudaS
 // 32 rows a tile and 10.0 us with 256. Where none does, by the rows of a mean group: a group of 40 rows or less is read with
 // its weights anyhow, and larger tiles read the weights less often from L2. 64 groups, 2048 -> 1024, us with tiles 0 to 4:
 // mean 24: 53 49 53 50 53, mean 64: 70 59 54 51 56, mean 192: 182 111 93 77 75, mean 512: 454 266 219 191 149.
-int pick_rows(int R, int E, int N) {
+// Rows that come one by one go to single CTAs, unless a copy into order and pairs take less: us one by one and by copy and
+// product, 4 slots a token; 64 experts, 2048 -> 2048: 4096 rows 92 and 101, 8192: 130 and 123, 65536: 676 and 487; 64 experts,
+// 512 -> 1024: 2048 rows 19.1 and 18.5, 65536: 121 and 93; 8 experts, 512 -> 512: 8192 rows 12.6 and 14.7, 16384: 20.2 and 20.1;
+// 16 experts, 1024 -> 256: 16384 rows 17.7 and 23.4, 65536: 53 and 81, so up to 256 features they stay one by one.
+constexpr int kOneByOneFeatures = 256;
+int pick_rows(int R, int E, int N, bool one_by_one) {
   const int kRows[5] = {32, 64, 128, 128, 256}, ctas = detail::free_ctas();
-  const int most = N > 128 ? 5 : 3;  // a pair takes 256 features
+  const int most = N > 128 && !one_by_one ? 5 : 3;  // a pair takes 256 features
   for (int i = 0; i < most; ++i) {
     const int pair = i < 3 ? 1 : 2;
     const double tiles = ((double)R / kRows[i] + 0.5 * (E < R ? E : R)) * ((N + 128 * pair - 1) / (128 * pair));
@@ -872,6 +910,11 @@ using namespace fs::ex;
 
 extern "C" {
 
+int fs_grouped_mm_in_order(int R, int E, int N) {
+  if (R < 1 || E < 1 || N < 1) return 0;
+  return R > kFewRows && N > kOneByOneFeatures && pick_rows(R, E, N, false) >= 3;
+}
+
 int fs_grouped_mm(const void* x, long long ldx, int M, const int* rows, int R, const void* w, long long w_expert,
                   long long w_row, long long w_col, int E, int N, int K, const int* offsets, void* out, int out_type,
                   long long ldo, int type, void* stream) {
@@ -896,7 +939,7 @@ int fs_grouped_mm(const void* x, long long ldx, int M, const int* rows, int R, c
   CUtensorMap mapA = {};
   if (!encode(&mapA, type, w, 3, {k_major ? K : N, k_major ? N : K, E}, {w_ld, w_expert ? w_expert : w_ld}, k_major ? 128 : 64))
     return no_map();
-  switch (pick_rows(R, E, N)) {
+  switch (pick_rows(R, E, N, rows != nullptr)) {
     case 0: return launch_rows<1, 32>(a, k_major, mapA, st);
     case 1: return launch_rows<1, 64>(a, k_major, mapA, st);
     case 2: return launch_rows<1, 128>(a, k_major, mapA, st);

@@ -24,7 +24,7 @@ constexpr int64_t kMaxExperts = 1024, kMaxK = 32, kBlock = 32;
 
 // Entry points of the library that is loaded.
 #define FS_ENTRIES(F)                                                                                                     \
-  F(fs_last_error) F(fs_route_bytes) F(fs_route) F(fs_route_grad) F(fs_grouped_mm) F(fs_grouped_mm_wgrad) F(fs_gated_act) \
+  F(fs_last_error) F(fs_route_bytes) F(fs_route) F(fs_route_grad) F(fs_grouped_mm) F(fs_grouped_mm_in_order) F(fs_grouped_mm_wgrad) F(fs_gated_act) \
   F(fs_gated_act_grad) F(fs_combine) F(fs_combine_grad)
 struct Library {
 #define FS_MEMBER(name) decltype(&::name) name = nullptr;
@@ -187,9 +187,10 @@ Tensor combine_raw(const Tensor& o, const Tensor& gates, const Tensor& position,
 // x[rows] as the products take it, zeros for the rows of no pair.
 Tensor gather_raw(const Tensor& x, const Tensor& rows) { return combine_raw(rows_of(x), Tensor(), rows.view({-1, 1}), x.scalar_type(), true); }
 
-Tensor mm_raw(const Tensor& x0, const Tensor& rows, int64_t count, const Tensor& w0, const Tensor& offsets, bool transposed, bool fp32) {
+Tensor mm_raw(const Tensor& x0, const Tensor& rows0, int64_t count, const Tensor& w0, const Tensor& offsets, bool transposed, bool fp32) {
   const Place at(x0);
-  const Tensor x = loadable_rows(x0), w = loadable_weights(w0);
+  const bool order = rows0.defined() && lib.fs_grouped_mm_in_order((int)count, (int)w0.size(0), (int)w0.size(transposed ? 2 : 1));
+  const Tensor x = order ? gather_raw(x0, rows0) : loadable_rows(x0), rows = order ? Tensor() : rows0, w = loadable_weights(w0);
   int64_t n = w.size(1), k = w.size(2), sn = w.stride(1), sk = w.stride(2);
   if (transposed) {
     std::swap(n, k);
@@ -268,7 +269,8 @@ struct Route : torch::autograd::Function<Route> {
 struct GroupedMm : torch::autograd::Function<GroupedMm> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x0, const Tensor& w0, const Tensor& offsets, const optional<Tensor>& rows0,
                         const optional<Tensor>& position, int64_t count) {
-    const Tensor x = loadable_rows(x0), w = loadable_weights(w0), rows = none(rows0);
+    const Tensor rows = none(rows0), w = loadable_weights(w0);
+    const Tensor x = rows.defined() ? rows_of(x0) : loadable_rows(x0);  // whatever reads gathered rows again copies them into order
     ctx->save_for_backward({x, w, offsets, rows, none(position)});
     return mm_raw(x, rows, count, w, offsets, false, false);
   }
@@ -337,7 +339,7 @@ struct Combine : torch::autograd::Function<Combine> {
 struct Mlp : torch::autograd::Function<Mlp> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x0, const Tensor& w_in0, const Tensor& w_out0, const Tensor& gates, const Tensor& offsets,
                         const Tensor& pairs, const Tensor& rows, const Tensor& position, bool checkpoint) {
-    const Tensor x = loadable_rows(x0), w_in = loadable_weights(w_in0), w_out = loadable_weights(w_out0);
+    const Tensor x = rows_of(x0), w_in = loadable_weights(w_in0), w_out = loadable_weights(w_out0);
     const int64_t count = pairs.size(0);
     const Tensor u = mm_raw(x, rows, count, w_in, offsets, false, false);
     auto [h, held] = act_raw(u, gates, pairs, checkpoint);

@@ -63,8 +63,8 @@ def grouped_mm(x: torch.Tensor, weight: torch.Tensor, groups: Union[Routing, tor
     ``groups``: a :class:`Routing`, or int32 offsets ``[E + 1]`` from 0 (group e has rows ``offsets[e]`` to
     ``offsets[e + 1]``; any sizes, zero among them). ``weight [E, N, K]`` as a linear layer holds it, or the transposed
     view of ``[E, K, N]``. ``x [R, K]`` in the order of the groups; with ``gather`` (and a routing) ``x [T, K]`` is in the
-    order of the tokens and row ``i`` reads token ``routing.rows[i]``, without a copy. fp16 or bf16, both the same; sums in
-    fp32, one rounding. Differentiable in both. Operands that tensor loads do not take (16 bytes of alignment, rows and
+    order of the tokens and row ``i`` reads token ``routing.rows[i]``; batches of thousands of rows are copied into order
+    first, ``R * K`` values that live for the call. fp16 or bf16, both the same; sums in fp32, one rounding. Differentiable in both. Operands that tensor loads do not take (16 bytes of alignment, rows and
     experts a multiple of 8 values apart) are copied in every call: keep weights padded to a multiple of 8.
     """
     if isinstance(groups, Routing):

@@ -509,6 +509,10 @@ int fs_grouped_mm(const void* x, long long ldx, int M, const int* rows, int R, c
                   long long w_row, long long w_col, int E, int N, int K, const int* offsets, void* out, int out_type,
                   long long ldo, int type, void* stream);
 
+/* 1 where a product of R rows, E experts and N features that has its rows in another order (`rows` not null) takes longer than
+ * copying them into order first (fs_combine with k = 1) and multiplying them so, else 0. Host arithmetic only. */
+int fs_grouped_mm_in_order(int R, int E, int N);
+
 /* Its gradient to the weights: dw[e, n, k] = sum over the rows i of expert e of dy[i, n] x[i, k], zeros for an expert
  * without rows; dy and x have R rows and are aligned and strided as x above, dw is E x N x K, densely packed. */
 int fs_grouped_mm_wgrad(const void* dy, long long lddy, const void* x, long long ldx, int R, int E, int N, int K,

@@ -8,7 +8,8 @@ import threading
 import pytest
 import torch
 
-from test_gpu_experts import BF16, FP32, FUN, TINY, ULP, act_reference, ex, gen, held_in_8_bits, normal, within  # noqa: F401
+from test_gpu_experts import (ACC, BF16, FP32, FUN, TINY, ULP, act_reference, check_mm, check_wgrad, ex, gen, held_in_8_bits, normal,  # noqa: F401
+                              offsets_of, within)
 
 pytestmark = pytest.mark.gpu
 
@@ -112,3 +113,30 @@ def test_forward_mode_derivatives_are_refused(ex, mode):  # noqa: F811
                 pytest.fail(f"call {i} was not refused")
     for call, t in calls:  # without a tangent they go through
         call(t)
+
+
+# copied: tiles of 128 rows and 128 features are more than 148 (6,000 rows: 147), and there are more than 256 features
+@pytest.mark.parametrize("tokens,slots,e,n,k,copied", [(3000, 2, 4, 320, 200, 0), (4000, 2, 4, 320, 200, 1), (3000, 2, 4, 256, 200, 0),
+                                                       (16384, 4, 64, 512, 256, 1), (16384, 4, 64, 256, 256, 0)])
+def test_gathered_rows_go_to_single_ctas_or_are_copied(ex, tokens, slots, e, n, k, copied):  # noqa: F811
+    """Rows in another order: products that want pairs of CTAs copy them first, and both ways give what the rows say."""
+    from flash_sinkhorn_b200 import _lib
+    lib, r = _lib.load(), tokens * slots
+    assert lib.fs_grouped_mm_in_order(r, e, n) == copied
+    g = gen(n + e)
+    routing = ex.route_tokens(normal(g, tokens, e), slots, mask=torch.arange(tokens, device="cuda") % 7 != 3)
+    x, w = normal(g, tokens, k, dtype=BF16), normal(g, e, n, k, scale=k**-0.5, dtype=BF16)
+    by_binding = check_mm(ex, x, w, routing.offsets, routing.rows)
+    out = torch.empty_like(by_binding)
+    _lib.call("fs_grouped_mm", x.device, x.data_ptr(), k, tokens, routing.rows.data_ptr(), r, w.data_ptr(), n * k, k, 1, e, n, k,
+              routing.offsets.data_ptr(), out.data_ptr(), 2, n, 2, _lib.stream_ptr(x.device))
+    xs, ends, want = x.double()[routing.rows.long().clamp_min(0)], routing.offsets.tolist(), torch.zeros(r, n, dtype=torch.float64, device="cuda")
+    size = torch.zeros_like(want)
+    for j in range(e):
+        want[ends[j]:ends[j + 1]] = xs[ends[j]:ends[j + 1]] @ w[j].double().T
+        size[ends[j]:ends[j + 1]] = xs[ends[j]:ends[j + 1]].abs() @ w[j].double().abs().T
+    within(out, want, ULP[BF16] * want.abs() + ACC * 64 * size + TINY[BF16])
+    dy = normal(g, r, n, dtype=BF16)
+    for _ in range(20):  # ends of groups in shared memory of both CTAs of a pair
+        again = ex._wgrad(dy, ex._gather(x, routing.rows), routing.offsets)
+    assert torch.equal(again, check_wgrad(ex, dy, ex._gather(x, routing.rows), routing.offsets))
