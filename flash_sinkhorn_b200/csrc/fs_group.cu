@@ -108,6 +108,20 @@ __device__ __forceinline__ bool wait_acquire_cluster(uint32_t bar, uint32_t pari
     }
   }
 }
+// For a barrier behind the products of many blocks of 64 contraction values, which take some 540 clocks each and are given
+// 4096: the limit of a single wait would run out within a group of 32 million rows, whose products are one tile.
+__device__ __forceinline__ bool wait_blocks(uint32_t bar, uint32_t parity, volatile int* abort_flag, long long blocks) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64(), limit = kSpinLimit + 4096 * blocks;
+  while (!mbar_try_wait_hint(bar, parity, 2000)) {
+    if (*abort_flag) return false;
+    if (clock64() - t0 > limit) {
+      *abort_flag = 1;
+      return false;
+    }
+  }
+  return true;
+}
 template <int CG>
 __device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
   if (CG == 2)
@@ -507,7 +521,7 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
       const int buf = n & 1;
       const bool zero = t.blocks == 0;
       if (!zero) {
-        if (!__all_sync(0xffffffffu, mbar_wait(bar(ACC_FULL + buf), (n >> 1) & 1, abort_flag, 2000))) break;
+        if (!__all_sync(0xffffffffu, wait_blocks(bar(ACC_FULL + buf), (n >> 1) & 1, abort_flag, t.blocks))) break;
         ++n;
         tc_fence_after();
       }
@@ -626,14 +640,17 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
     }
   } else if (FORM == WEIGHTS) {
     // ===================== ends of groups =====================
-    int s = 0;         // first stage of the tile
-    uint32_t uses = 0;  // bit s: parity of the uses of stage s here
+    int s = 0;             // first stage of the tile
+    uint32_t uses = 0;     // bit s: parity of the uses of stage s here
+    long long blocks = 0;  // since the last wait, which may be tiles ago
     for (int it = first; it < total; it += stride) {
       const Tile t = tiles.at(it);
       const int rows = t.hi - t.lo, stage = (s + t.blocks - 1) % a.nstage;
       s = (s + t.blocks) % a.nstage;
+      blocks += t.blocks;
       if (rows % 16 == 0) continue;
-      if (!__all_sync(0xffffffffu, mbar_wait(bar(PARTS + stage), uses >> stage & 1, abort_flag, 2000))) break;
+      if (!__all_sync(0xffffffffu, wait_blocks(bar(PARTS + stage), uses >> stage & 1, abort_flag, blocks))) break;
+      blocks = 0;
       uses ^= 1u << stage;
       uint8_t* block = ring + (size_t)stage * kStage;
       const int from = rows & 63, chunks = ((rows + 15) / 16 * 16 - rows) * 8;  // 16-byte chunks of a half tile

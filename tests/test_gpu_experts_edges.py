@@ -14,6 +14,13 @@ from test_gpu_experts import (ACC, BF16, FP32, FUN, TINY, ULP, act_reference, ch
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(scope="module", autouse=True)
+def no_wait_gave_up():
+    from flash_sinkhorn_b200 import _lib
+    yield
+    assert _lib.load().fs_device_error() == 0
+
+
 def large_blocks(dtype, top, seed):
     """Rows [g | v] of one block each: a large g beside an ordinary v, and the other way round; zeros and ones in the large one."""
     g = gen(seed)
@@ -140,3 +147,27 @@ def test_gathered_rows_go_to_single_ctas_or_are_copied(ex, tokens, slots, e, n, 
     for _ in range(20):  # ends of groups in shared memory of both CTAs of a pair
         again = ex._wgrad(dy, ex._gather(x, routing.rows), routing.offsets)
     assert torch.equal(again, check_wgrad(ex, dy, ex._gather(x, routing.rows), routing.offsets))
+
+
+@pytest.mark.parametrize("ctas,counts", [(0, [100_000_019]), (1, [99_999_984, 37])])
+def test_weight_gradient_of_a_very_long_group(ex, ctas, counts):  # noqa: F811
+    """One tile's products take longer than a single wait lasts (2^28 clocks): the warps behind them wait in proportion. In the
+    second case the end that is zeroed comes a long tile after the warp that does so has started to wait."""
+    from flash_sinkhorn_b200 import _lib
+    lib, r = _lib.load(), sum(counts)
+    g = gen(91)
+    x = torch.zeros(r, 64, dtype=BF16, device="cuda")
+    at = torch.cat([torch.randint(0, r, (100_000,), generator=g, device="cuda"), torch.arange(r - 60, r, device="cuda"),
+                    torch.arange(60, device="cuda")]).unique()
+    x[at] = torch.randint(-1, 2, (at.numel(), 64), generator=g, device="cuda").to(BF16)  # sums are exact in fp32 in any order
+    want, ends = [], offsets_of(counts).tolist()
+    for lo, hi in zip(ends[:-1], ends[1:]):
+        rows = x[at[(at >= lo) & (at < hi)]].double()
+        want.append((rows.T @ rows).to(BF16))
+    before = lib.fs_set_cta_limit(ctas)
+    try:
+        got = ex._wgrad(x, x, offsets_of(counts))
+        torch.cuda.synchronize()
+    finally:
+        lib.fs_set_cta_limit(before)
+    assert lib.fs_device_error() == 0 and torch.equal(got, torch.stack(want))
