@@ -152,6 +152,7 @@ SIGNATURES = {
     "fs_route_grad": (c_int, [_P, c_int, _L, c_int, c_int, c_int, _P, _P, c_int, _P, _P, _P, _P, _P]),
     "fs_grouped_mm": (
         c_int, [_P, _L, c_int, _P, c_int, _P, _L, _L, _L, c_int, c_int, c_int, _P, _P, c_int, _L, c_int, _P]),
+    "fs_set_product_limit": (_L, [_L]),
     "fs_grouped_mm_in_order": (c_int, [c_int, c_int, c_int]),
     "fs_grouped_mm_wgrad": (
         c_int, [_P, _L, _P, _L, c_int, c_int, c_int, c_int, _P, _P, c_int, _P]),

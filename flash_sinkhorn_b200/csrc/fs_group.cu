@@ -38,6 +38,7 @@ namespace {
 using namespace fs::tc;
 
 __device__ int g_group_error = 0;  // non-zero once a bounded wait gave up (read by fs_device_error)
+thread_local long long t_product_limit = kSpinLimit;  // clocks, fs_set_product_limit
 
 enum Form { ROWS_K, ROWS_MN, WEIGHTS };  // rows with W contiguous along the contraction; along the features
 
@@ -64,6 +65,7 @@ struct GroupArgs {
   int nstage;
   const void* x;  // the rows as plain memory, for fetching them one by one
   long long ldx;
+  long long limit;  // clocks that the warps which write results wait, besides what the products take; 0: none at all
 };
 
 // ------------------------------------------------------------------ PTX of CTA pairs and gathered loads
@@ -110,9 +112,12 @@ __device__ __forceinline__ bool wait_acquire_cluster(uint32_t bar, uint32_t pari
 }
 // For a barrier behind the products of many blocks of 64 contraction values, which take some 540 clocks each and are given
 // 4096: the limit of a single wait would run out within a group of 32 million rows, whose products are one tile.
-__device__ __forceinline__ bool wait_blocks(uint32_t bar, uint32_t parity, volatile int* abort_flag, long long blocks) {
+__device__ __forceinline__ bool wait_blocks(uint32_t bar, uint32_t parity, volatile int* abort_flag, long long blocks, long long limit) {
+  if (limit == 0) *abort_flag = 1;  // without a look, for tests
+  if (limit == 0) return false;
   if (mbar_try_wait(bar, parity)) return true;
-  const long long t0 = clock64(), limit = kSpinLimit + 4096 * blocks;
+  const long long t0 = clock64();
+  limit += 4096 * blocks;
   while (!mbar_try_wait_hint(bar, parity, 2000)) {
     if (*abort_flag) return false;
     if (clock64() - t0 > limit) {
@@ -146,6 +151,11 @@ template <int CG>
 __device__ __forceinline__ void expect_at(uint32_t bar, uint32_t bytes) {  // bar: in CTA 0 of the pair
   if (CG == 2) asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
   else mbar_expect_tx(bar, bytes);
+}
+// After a wait that gave up: for the copies in flight to land, until about 0.14 s after `t0` at most.
+__device__ __forceinline__ void wait_landed(uint32_t bar, uint32_t parity, long long t0) {
+  while (!mbar_try_wait(bar, parity))
+    if (clock64() - t0 > kSpinLimit) return;
 }
 // 16 bytes, of which those past the first `valid` become zeros (the source is not read for them).
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int valid) {
@@ -326,29 +336,30 @@ __device__ __forceinline__ void stage_block(const uint32_t (&r)[32], uint32_t ba
                      : "memory");
     }
 }
-// rows x cols values (at most 32 x 32) of the staging tile, or zeros, to out, rows ld values apart.
-__device__ __forceinline__ void write_block(uint16_t* out, long long ld, int rows, int cols, int vec, bool zero, uint32_t base, int lane) {
+// rows x cols values (at most 32 x 32) of the staging tile, or `fill` (two values) throughout, to out, rows ld values apart.
+__device__ __forceinline__ void write_block(uint16_t* out, long long ld, int rows, int cols, int vec, bool filled, uint32_t fill, uint32_t base,
+                                            int lane) {
   if (vec == 8) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = 8 * i + (lane >> 2), c = lane & 3;
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (!zero) asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(staged(base, r, c)));
+      uint4 v = make_uint4(fill, fill, fill, fill);
+      if (!filled) asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(staged(base, r, c)));
       if (r < rows && 8 * c < cols) *reinterpret_cast<uint4*>(out + r * ld + 8 * c) = v;
     }
   } else if (vec == 2) {
 #pragma unroll 4
     for (int i = 0; i < 16; ++i) {
       const int r = 2 * i + (lane >> 4), c = 2 * (lane & 15);
-      uint32_t v = 0u;
-      if (!zero) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(staged(base, r, c >> 3) + (c & 7) * 2));
+      uint32_t v = fill;
+      if (!filled) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(staged(base, r, c >> 3) + (c & 7) * 2));
       if (r < rows && c < cols) *reinterpret_cast<uint32_t*>(out + r * ld + c) = v;
     }
   } else {
 #pragma unroll 4
     for (int r = 0; r < 32; ++r) {
-      uint16_t v = 0;
-      if (!zero) asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(staged(base, r, lane >> 3) + (lane & 7) * 2));
+      uint16_t v = (uint16_t)fill;
+      if (!filled) asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(staged(base, r, lane >> 3) + (lane & 7) * 2));
       if (r < rows && lane < cols) out[r * ld + lane] = v;
     }
   }
@@ -411,11 +422,12 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
   const uint32_t tmem = *slot;
   Tiles<FORM, CG, BN> tiles(a, gs, ts);
   const int total = tiles.total();
+  int issued = 0;  // stages that this CTA's loading thread has started
   auto full_bar = [&](int s) { return CG == 2 ? in_leader(bar(FULL + s)) : bar(FULL + s); };
 
   if (warp == kLoadWarp) {
     // ===================== whole tiles =====================
-    int s = 0, issued = 0;
+    int s = 0;
     uint32_t ph = 0;
     bool ok = true;
     if (elect_one()) {
@@ -456,10 +468,6 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
           }
         }
       }
-      // let the copies in flight land (in CTA 0 also the other one's; it stays until the pair has met)
-      if (*abort_flag && rank == 0)
-        for (int j = issued > a.nstage ? issued - a.nstage : 0; j < issued; ++j)
-          mbar_wait_quiet(bar(FULL + j % a.nstage), (j / a.nstage) & 1);
     }
   } else if (warp == kMmaWarp) {
     // ===================== products =====================
@@ -503,10 +511,6 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
         if (!ok) break;
         commit<CG>(bar(ACC_FULL + buf));
       }
-      if (*abort_flag) {  // every product issued here ends before TMEM is freed
-        commit<CG>(bar(DRAIN));
-        mbar_wait_quiet(bar(DRAIN), 0);
-      }
     }
   } else if (warp < kOutWarps) {
     // ===================== results =====================
@@ -515,34 +519,37 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
     const uint32_t stage = smem_u32(staging + 2048 * warp);
     constexpr int kStep = 32 * kOutWarps / 4;
     int n = 0;
+    bool lost = false;  // a wait of this CTA gave up: NaN from here on
     for (int it = first; it < total; it += stride) {
       const Tile t = tiles.at(it);
       const int f = t.m0 + rank * 128 + q * 32;  // first of this warp's features
       const int buf = n & 1;
-      const bool zero = t.blocks == 0;
-      if (!zero) {
-        if (!__all_sync(0xffffffffu, wait_blocks(bar(ACC_FULL + buf), (n >> 1) & 1, abort_flag, t.blocks))) break;
+      const bool none = t.blocks == 0;  // no products: zeros
+      if (!none && !lost) {
+        lost = !__all_sync(0xffffffffu, wait_blocks(bar(ACC_FULL + buf), (n >> 1) & 1, abort_flag, t.blocks, a.limit));
         ++n;
         tc_fence_after();
       }
+      const bool filled = none || lost;
+      const uint32_t fill = none ? 0u : 0x7fff7fffu;  // NaN in any of the types
       const uint32_t acc = tmem + buf * BN + ((uint32_t)(q * 32) << 16);
       if (f < a.N) {
         if (FORM != WEIGHTS && a.out_type == FS_TYPE_F32) {
           for (int c = 32 * side; c < t.cols; c += kStep) {
             float v[32];
-            if (!zero) tmem_ld32(acc + c, v);
+            if (!filled) tmem_ld32(acc + c, v);
             float* p = static_cast<float*>(a.out) + (long long)(t.lo + c) * a.ldo + f + lane;
             if (f + lane < a.N) {
 #pragma unroll
               for (int j = 0; j < 32; ++j)
-                if (c + j < t.cols) p[j * a.ldo] = zero ? 0.f : v[j];
+                if (c + j < t.cols) p[j * a.ldo] = filled ? __uint_as_float(fill) : v[j];
             }
           }
         } else {
           uint32_t r[32];
-          if (!zero && 32 * side < t.cols) read_block(acc + 32 * side, r);
+          if (!filled && 32 * side < t.cols) read_block(acc + 32 * side, r);
           for (int c = 32 * side; c < t.cols; c += kStep) {
-            if (!zero) {
+            if (!filled) {
               tmem_ld_wait(r);
               stage_block<FORM != WEIGHTS>(r, stage, lane, a.out_type);
               if (c + kStep < t.cols) read_block(acc + c + kStep, r);  // on its way while this one is written
@@ -550,14 +557,14 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
             }
             uint16_t* out = static_cast<uint16_t*>(a.out);
             if (FORM == WEIGHTS)
-              write_block(out + ((long long)t.e * a.N + f) * a.K + t.n0 + c, a.K, a.N - f, t.cols - c, a.out_vec, zero, stage, lane);
+              write_block(out + ((long long)t.e * a.N + f) * a.K + t.n0 + c, a.K, a.N - f, t.cols - c, a.out_vec, filled, fill, stage, lane);
             else
-              write_block(out + (long long)(t.lo + c) * a.ldo + f, a.ldo, t.cols - c, a.N - f, a.out_vec, zero, stage, lane);
+              write_block(out + (long long)(t.lo + c) * a.ldo + f, a.ldo, t.cols - c, a.N - f, a.out_vec, filled, fill, stage, lane);
             __syncwarp();
           }
         }
       }
-      if (!zero) {
+      if (!filled) {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
@@ -649,7 +656,7 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
       s = (s + t.blocks) % a.nstage;
       blocks += t.blocks;
       if (rows % 16 == 0) continue;
-      if (!__all_sync(0xffffffffu, wait_blocks(bar(PARTS + stage), uses >> stage & 1, abort_flag, blocks))) break;
+      if (!__all_sync(0xffffffffu, wait_blocks(bar(PARTS + stage), uses >> stage & 1, abort_flag, blocks, kSpinLimit))) break;
       blocks = 0;
       uses ^= 1u << stage;
       uint8_t* block = ring + (size_t)stage * kStage;
@@ -670,6 +677,27 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
   __syncwarp();
   tc_fence_before();
   __syncthreads();
+  if (*abort_flag) {  // nobody waits any more, and the flag does not change
+    if (warp == kMmaWarp && rank == 0) {  // every product issued here ends before TMEM is freed
+      if (elect_one()) {
+        commit<CG>(bar(DRAIN));
+        mbar_wait_quiet(bar(DRAIN), 0);
+      }
+      __syncwarp();
+    } else if (warp == kLoadWarp) {
+      // The copies in flight land before the CTA ends. Those of the second CTA of a pair are counted in the first one, which
+      // does not know of stages that it has not started itself: the second one stays for a millisecond, hundreds of times what
+      // a copy takes.
+      if (elect_one()) {
+        const long long t0 = clock64();
+        if (rank == 0)
+          for (int j = issued > a.nstage ? issued - a.nstage : 0; j < issued; ++j) wait_landed(bar(FULL + j % a.nstage), (j / a.nstage) & 1, t0);
+        else
+          while (clock64() - t0 < (1ll << 21)) {}
+      }
+      __syncwarp();
+    }
+  }
   if (CG == 2) cluster_sync_all();
   tc_fence_after();
   if (warp == kMmaWarp) free_columns<CG>(tmem, kColumns);
@@ -927,6 +955,12 @@ using namespace fs::ex;
 
 extern "C" {
 
+long long fs_set_product_limit(long long clocks) {
+  const long long before = t_product_limit;
+  t_product_limit = clocks < 0 ? kSpinLimit : clocks;
+  return before;
+}
+
 int fs_grouped_mm_in_order(int R, int E, int N) {
   if (R < 1 || E < 1 || N < 1) return 0;
   return R > kFewRows && N > kOneByOneFeatures && pick_rows(R, E, N, false) >= 3;
@@ -949,6 +983,7 @@ int fs_grouped_mm(const void* x, long long ldx, int M, const int* rows, int R, c
   a.offsets = offsets; a.rows = rows; a.M = M; a.R = R; a.E = E; a.N = N; a.K = K;
   a.out = out; a.ldo = ldo; a.type = type; a.out_type = out_type; a.x = x; a.ldx = ldx;
   a.out_vec = store_values(out, ldo, N);
+  a.limit = t_product_limit;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (R <= kFewRows && k_major) {
     return type == FS_TYPE_F16 ? launch_few<__half>(a, w, w_expert, w_row, st) : launch_few<__nv_bfloat16>(a, w, w_expert, w_row, st);
@@ -979,6 +1014,7 @@ int fs_grouped_mm_wgrad(const void* dy, long long lddy, const void* x, long long
   GroupArgs a{};
   a.offsets = offsets; a.R = R; a.E = E; a.N = N; a.K = K;
   a.out = dw; a.type = a.out_type = type; a.out_vec = store_values(dw, K, K);
+  a.limit = t_product_limit;
   CUtensorMap mapA = {}, mapB = {};
   if (!encode_rows(&mapA, type, dy, N, R, lddy, 64) || !encode_rows(&mapB, type, x, K, R, ldx, 64)) return no_map();
   // The largest tile, unless smaller ones are all under way at once: 7 x 501 x 300 outputs of 6000 rows take 20.4 us with

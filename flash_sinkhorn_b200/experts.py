@@ -11,7 +11,9 @@ largest where ``x.w_e + bias_e`` is, with one price per expert: :func:`transport
 * :func:`expert_mlp` - the three in a row, as one layer with one backward pass.
 
 All of it runs on the current stream of the tensors' device, never waits for the host (group sizes stay on the device, so
-a call can be captured in a CUDA graph), and gives the same bits in every run. Sums are held in fp32. Extension without a
+a call can be captured in a CUDA graph), and gives the same bits in every run. Sums are held in fp32. Waits inside the
+products are bounded: should one ever give up, the results it leaves are NaN and the library's health word is set
+(``fs_device_error()``, which waits for the device). Extension without a
 counterpart in the reference.
 """
 from __future__ import annotations

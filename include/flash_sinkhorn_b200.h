@@ -504,10 +504,16 @@ int fs_route_grad(const void* logits, int type, long long ld, int T, int E, int 
  * W_e is N x K with element (n, k) at w[e * w_expert + n * w_row + k * w_col]; w_row or w_col is 1. out is R x N, of the type
  * of x and w (FS_TYPE_F16 or FS_TYPE_BF16) or FS_TYPE_F32. x and w are aligned to 16 bytes, ldx, w_expert and the other
  * stride of w multiples of 8. offsets[0] is taken as 0; offsets that decrease or leave [0, R] are taken as their running
- * maximum within it. E <= 1024. */
+ * maximum within it. E <= 1024. Waits inside the kernel are bounded: should one give up, fs_device_error() is set and what the
+ * thread block had still to write is NaN. */
 int fs_grouped_mm(const void* x, long long ldx, int M, const int* rows, int R, const void* w, long long w_expert,
                   long long w_row, long long w_col, int E, int N, int K, const int* offsets, void* out, int out_type,
                   long long ldo, int type, void* stream);
+
+/* SM clocks that the writers of a product's results wait for it, besides 4096 for each 64 values of its contraction, before the
+ * thread block gives up. Negative: the default, 2^28. Holds for the products that the calling thread launches (in a backward
+ * pass that is the thread of autograd). Returns the previous value. For tests of that path: with 0 all blocks give up at once. */
+long long fs_set_product_limit(long long clocks);
 
 /* 1 where a product of R rows, E experts and N features that has its rows in another order (`rows` not null) takes longer than
  * copying them into order first (fs_combine with k = 1) and multiplying them so, else 0. Host arithmetic only. */

@@ -171,3 +171,31 @@ def test_weight_gradient_of_a_very_long_group(ex, ctas, counts):  # noqa: F811
     finally:
         lib.fs_set_cta_limit(before)
     assert lib.fs_device_error() == 0 and torch.equal(got, torch.stack(want))
+
+
+# tiles of single CTAs (rows in order and one by one, weights of either layout), of pairs; sizes that end inside tiles
+@pytest.mark.parametrize("tokens,e,n,k,gather", [(40, 3, 100, 72, False), (40, 3, 100, 72, True), (600, 3, 200, 328, False), (5000, 2, 700, 520, False),
+                                                 (3000, 2, 1200, 1100, False), (9000, 2, 250, 136, True)])
+def test_products_that_give_up(ex, tokens, e, n, k, gather):  # noqa: F811
+    """Where a wait gives up, nothing passes for a result: NaN in what was not written, and the health word is set."""
+    from flash_sinkhorn_b200 import _lib
+    lib = _lib.load()
+    g = gen(n)
+    routing = ex.route_tokens(normal(g, tokens, e), 1, mask=torch.arange(tokens, device="cuda") % 8 != 5)
+    off, routed = routing.offsets, int(routing.offsets[-1])
+    x, w, dy = normal(g, tokens, k, dtype=BF16), normal(g, e, n, k, scale=k**-0.5, dtype=BF16), normal(g, tokens, n, dtype=BF16)
+    rows = routing.rows if gather else None
+    calls = [lambda: ex._mm(x, rows, tokens, w, off), lambda: ex._mm(dy, rows, tokens, w, off, transposed=True),
+             lambda: ex._mm(dy, None, tokens, w, off, transposed=True, dtype=FP32), lambda: ex._wgrad(dy, x, off)]
+    good = [call() for call in calls]
+    for i, call in enumerate(calls):
+        usual = lib.fs_set_product_limit(0)
+        try:
+            out = call()
+            assert lib.fs_device_error() == 1
+        finally:
+            lib.fs_set_product_limit(usual)
+            torch.cuda.synchronize()
+            assert lib.fs_clear_device_error() == 0
+        assert torch.isnan(out if i == 3 else out[:routed]).all() and (i == 3 or not out[routed:].any())
+    assert lib.fs_device_error() == 0 and all(torch.equal(call(), want) for call, want in zip(calls, good))
