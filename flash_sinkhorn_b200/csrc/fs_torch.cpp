@@ -356,8 +356,8 @@ struct Mlp : torch::autograd::Function<Mlp> {
       const Tensor dh = mm_raw(dy, Tensor(), count, w_out, offsets, true, false);
       Tensor du, h;
       std::tie(du, dgates, h) = act_grad_raw(s[8], s[9], gates, pairs, position, dh, ctx->needs_input_grad(3), ctx->needs_input_grad(2));
-      if (ctx->needs_input_grad(0))
-        dx = combine_raw(mm_raw(du, Tensor(), count, w_in, offsets, true, false), Tensor(), position, x.scalar_type());
+      if (ctx->needs_input_grad(0))  // rows in fp32, so that the sum over a token's rows is rounded once
+        dx = combine_raw(mm_raw(du, Tensor(), count, w_in, offsets, true, true), Tensor(), position, x.scalar_type());
       if (ctx->needs_input_grad(1)) dw_in = wgrad_raw(du, gather_raw(x, rows), offsets);
       if (ctx->needs_input_grad(2)) dw_out = wgrad_raw(dy, h, offsets);
     }

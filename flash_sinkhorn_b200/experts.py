@@ -109,7 +109,9 @@ def expert_mlp(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, routing
     ``x [T, D]``, ``w_in [E, 2 F, D]``, ``w_out [E, D, F]``, all fp16 or all bf16; differentiable in ``x``, the weights and
     ``routing.gates``. ``checkpoint`` as in :func:`gated_act`: of everything between x and y only the inner activations
     stay for the backward pass, in 8 bits, and the outer product's weight gradient uses the activation recomputed from
-    them.
+    them. The operators' results between x and y are of the type of x (a token's rows of the second product are rounded,
+    then summed in fp32 and rounded again), as are the gradients between dy and dx, but for the rows that are summed to
+    dx, which are fp32.
     """
     _check_routing(routing)
     r = routing

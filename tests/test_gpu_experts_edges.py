@@ -8,7 +8,7 @@ import threading
 import pytest
 import torch
 
-from test_gpu_experts import (ACC, BF16, FP32, FUN, TINY, ULP, act_reference, check_mm, check_wgrad, ex, gen, held_in_8_bits, normal,  # noqa: F401
+from test_gpu_experts import (ACC, BF16, FP16, FP32, FUN, TINY, ULP, act_reference, check_mm, check_wgrad, ex, gen, held_in_8_bits, normal,  # noqa: F401
                               offsets_of, within)
 
 pytestmark = pytest.mark.gpu
@@ -199,3 +199,26 @@ def test_products_that_give_up(ex, tokens, e, n, k, gather):  # noqa: F811
             assert lib.fs_clear_device_error() == 0
         assert torch.isnan(out if i == 3 else out[:routed]).all() and (i == 3 or not out[routed:].any())
     assert lib.fs_device_error() == 0 and all(torch.equal(call(), want) for call, want in zip(calls, good))
+
+
+@pytest.mark.parametrize("t,d,f,e,k", [(90, 136, 72, 6, 3), (257, 264, 128, 12, 8)])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_layer_sums_a_token_s_gradient_before_it_rounds(ex, t, d, f, e, k, dtype):  # noqa: F811
+    """dx of the layer is that of its parts, element by element: the rows of a token are summed in fp32 and rounded once."""
+    g = gen(t)
+    x = normal(g, t, d, dtype=dtype).requires_grad_(True)
+    w_in, w_out = normal(g, e, 2 * f, d, scale=d**-0.5, dtype=dtype), normal(g, e, d, f, scale=f**-0.5, dtype=dtype)
+    routing, dy = ex.route_tokens(normal(g, t, e), k, mask=torch.arange(t, device="cuda") % 9 != 4), normal(g, t, d, dtype=dtype)
+    (got,) = torch.autograd.grad(ex.expert_mlp(x, w_in, w_out, routing, checkpoint=False), x, dy)
+    # the gradient of u as the layer has it, from the kernels by themselves; from there on in 64 bits
+    r = t * k
+    u = ex._mm(x.detach(), routing.rows, r, w_in, routing.offsets)
+    dh = ex._mm(ex._gather(dy, routing.rows), None, r, w_out, routing.offsets, transposed=True)
+    du = ex._act_grad(u, None, routing.gates, routing.pairs, routing.position, dh, False, False)[0].double()
+    want, size = torch.zeros(t, d, dtype=torch.float64, device="cuda"), torch.zeros(t, d, dtype=torch.float64, device="cuda")
+    ends = routing.offsets.tolist()
+    for j, (lo, hi) in enumerate(zip(ends[:-1], ends[1:])):
+        to = routing.rows[lo:hi].long()
+        want.index_add_(0, to, du[lo:hi] @ w_in[j].double())
+        size.index_add_(0, to, du[lo:hi].abs() @ w_in[j].double().abs())
+    within(got, want, ULP[dtype] * want.abs() + ACC * 64 * size + TINY[dtype])
