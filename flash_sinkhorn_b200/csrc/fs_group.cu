@@ -52,6 +52,7 @@ constexpr int kCopyWarps = 8, kCopyGroup = 128;  // threads that fetch a stage
 constexpr int kCopyRows = kCopyGroup / 8;        // rows that they fetch 128 bytes of at a time
 constexpr uint32_t kHalfTile = 64 * 128;  // 64 rows of 128 bytes
 constexpr int kMaxGroups = 1024;
+constexpr int kMaxRows = 0x7fffffff - 511;  // no tile reaches past 2^31 rows: neither the indices nor the boxes of tensor loads overflow
 
 struct GroupArgs {
   const int* offsets;
@@ -919,8 +920,8 @@ int store_values(const void* out, long long ld, int width) {
 
 int check_group(int type, int R, int E, int N, int K, const int* offsets) {
   if (type != FS_TYPE_F16 && type != FS_TYPE_BF16) return report_error(FS_ERR_BAD_ARG, "type must be FS_TYPE_F16 or FS_TYPE_BF16");
-  if (R < 0 || E < 1 || E > kMaxGroups || N < 1 || K < 1 || N > (1 << 22) || K > (1 << 22))
-    return report_error(FS_ERR_BAD_ARG, "R must be >= 0, E in [1, 1024], N and K in [1, 2^22]");
+  if (R < 0 || R > kMaxRows || E < 1 || E > kMaxGroups || N < 1 || K < 1 || N > (1 << 22) || K > (1 << 22))
+    return report_error(FS_ERR_BAD_ARG, "R must be in [0, 2^31 - 512], E in [1, 1024], N and K in [1, 2^22]");
   if (!offsets) return report_error(FS_ERR_BAD_ARG, "null argument");
   // A thread that has launched nothing yet (autograd's) has no current context, which the encoding of tensor maps needs;
   // setting the device that is current binds it.
@@ -971,8 +972,8 @@ int fs_grouped_mm(const void* x, long long ldx, int M, const int* rows, int R, c
                   long long ldo, int type, void* stream) {
   int s = check_group(type, R, E, N, K, offsets);
   if (s != FS_OK || R == 0) return s;
-  if (!x || !w || !out || ldx < K || ldo < N || M < 1 || (!rows && M < R) || (out_type != type && out_type != FS_TYPE_F32))
-    return report_error(FS_ERR_BAD_ARG, "null argument, too few rows or columns, or a wrong type of the result");
+  if (!x || !w || !out || ldx < K || ldo < N || M < 1 || M > kMaxRows || (!rows && M < R) || (out_type != type && out_type != FS_TYPE_F32))
+    return report_error(FS_ERR_BAD_ARG, "null argument, too few or too many rows or columns, or a wrong type of the result");
   const bool k_major = w_col == 1;
   const long long w_ld = k_major ? w_row : w_col;
   if (!k_major && w_row != 1) return report_error(FS_ERR_BAD_ARG, "w_row or w_col must be 1");

@@ -20,7 +20,7 @@ using c10::optional;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-constexpr int64_t kMaxExperts = 1024, kMaxK = 32, kBlock = 32;
+constexpr int64_t kMaxExperts = 1024, kMaxK = 32, kBlock = 32, kMaxRows = (int64_t(1) << 31) - 512;  // rows: of products
 
 // Entry points of the library that is loaded.
 #define FS_ENTRIES(F)                                                                                                     \
@@ -419,7 +419,7 @@ Tensor grouped_mm(const Tensor& x0, const Tensor& w0, const Tensor& offsets, con
   REQUIRE(!gather || position.size(1) <= kMaxK, "k must be at most ", kMaxK);
   REQUIRE(offsets.size(0) == e + 1 && e <= kMaxExperts, "groups must have as many experts as weight (", e, ", at most ", kMaxExperts,
                     "), got ", offsets.size(0) - 1);
-  REQUIRE(count < (int64_t(1) << 31) && x0.size(0) < (int64_t(1) << 31), "rows must be fewer than 2^31");
+  REQUIRE(count <= kMaxRows && x0.size(0) <= kMaxRows, "rows must be at most 2^31 - 512");
   if (!wants_grad({&x0, &w0})) return mm_raw(x0, rows, count, w0, offsets, false, false);
   return GroupedMm::apply(x0, w0, offsets, maybe(rows), maybe(position), count);
 }
@@ -472,8 +472,8 @@ Tensor expert_mlp(const Tensor& x0, const Tensor& w_in0, const Tensor& w_out0, c
   const int64_t t = x0.size(0), d = x0.size(1), e = w_in0.size(0), f = w_out0.size(2);
   REQUIRE(w_in0.size(1) == 2 * f && w_in0.size(2) == d && w_out0.size(0) == e && w_out0.size(1) == d && d > 0 && f > 0,
                     "w_in must be [E, 2 F, ", d, "] and w_out [E, ", d, ", F], got ", shape_of(w_in0), " and ", shape_of(w_out0));
-  REQUIRE(position.size(0) == t && offsets.size(0) == e + 1 && position.size(1) <= kMaxK && e <= kMaxExperts && position.numel() < (int64_t(1) << 31),
-                    "routing must be of ", t, " tokens and ", e, " experts (at most ", kMaxExperts, "), at most ", kMaxK, " for a token");
+  REQUIRE(position.size(0) == t && offsets.size(0) == e + 1 && position.size(1) <= kMaxK && e <= kMaxExperts && position.numel() <= kMaxRows,
+                    "routing must be of ", t, " tokens and ", e, " experts (at most ", kMaxExperts, "), at most ", kMaxK, " for a token and 2^31 - 512 in all");
   if (wants_grad({&x0, &w_in0, &w_out0, &gates})) return Mlp::apply(x0, w_in0, w_out0, gates, offsets, pairs, rows, position, checkpoint);
   const int64_t count = pairs.size(0);
   const Tensor h = act_raw(mm_raw(x0, rows, count, w_in0, offsets, false, false), gates, pairs, false).first;

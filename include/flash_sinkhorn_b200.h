@@ -504,7 +504,7 @@ int fs_route_grad(const void* logits, int type, long long ld, int T, int E, int 
  * W_e is N x K with element (n, k) at w[e * w_expert + n * w_row + k * w_col]; w_row or w_col is 1. out is R x N, of the type
  * of x and w (FS_TYPE_F16 or FS_TYPE_BF16) or FS_TYPE_F32. x and w are aligned to 16 bytes, ldx, w_expert and the other
  * stride of w multiples of 8. offsets[0] is taken as 0; offsets that decrease or leave [0, R] are taken as their running
- * maximum within it. E <= 1024. Waits inside the kernel are bounded: should one give up, fs_device_error() is set and what the
+ * maximum within it. E <= 1024; R and M at most 2^31 - 512. Waits inside the kernel are bounded: should one give up, fs_device_error() is set and what the
  * thread block had still to write is NaN. */
 int fs_grouped_mm(const void* x, long long ldx, int M, const int* rows, int R, const void* w, long long w_expert,
                   long long w_row, long long w_col, int E, int N, int K, const int* offsets, void* out, int out_type,
@@ -520,7 +520,7 @@ long long fs_set_product_limit(long long clocks);
 int fs_grouped_mm_in_order(int R, int E, int N);
 
 /* Its gradient to the weights: dw[e, n, k] = sum over the rows i of expert e of dy[i, n] x[i, k], zeros for an expert
- * without rows; dy and x have R rows and are aligned and strided as x above, dw is E x N x K, densely packed. */
+ * without rows; dy and x have R <= 2^31 - 512 rows and are aligned and strided as x above, dw is E x N x K, densely packed. */
 int fs_grouped_mm_wgrad(const void* dy, long long lddy, const void* x, long long ldx, int R, int E, int N, int K,
                         const int* offsets, void* dw, int type, void* stream);
 

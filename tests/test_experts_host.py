@@ -30,6 +30,16 @@ def test_scratch_of_a_routing():
     assert lib.fs_route_bytes(10, 1025, 2) == 0
 
 
+@pytest.mark.parametrize("r", [(1 << 31) - 1, (1 << 31) - 511])
+def test_products_of_too_many_rows_are_refused(r):
+    """Before anything else is looked at: a tile of the last rows would reach past 2^31."""
+    lib = _lib.load()
+    at = 256  # never read
+    for call in (lambda: lib.fs_grouped_mm(at, 8, 8, at, r, at, 64, 8, 1, 2, 8, 8, at, at, 2, 8, 2, None),
+                 lambda: lib.fs_grouped_mm_wgrad(at, 8, at, 8, r, 2, 8, 8, at, at, 2, None)):
+        assert call() == 1 and b"2^31 - 512" in lib.fs_last_error()  # FS_ERR_BAD_ARG
+
+
 def test_refusals_on_the_host(ex):
     x, w = torch.zeros(6, 8, dtype=torch.bfloat16), torch.zeros(2, 8, 8, dtype=torch.bfloat16)
     r = ex.Routing(torch.zeros(3, 2), *[torch.zeros(3, 2, dtype=torch.int32)] * 5)

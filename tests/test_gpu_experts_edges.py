@@ -222,3 +222,29 @@ def test_layer_sums_a_token_s_gradient_before_it_rounds(ex, t, d, f, e, k, dtype
         want.index_add_(0, to, du[lo:hi] @ w_in[j].double())
         size.index_add_(0, to, du[lo:hi].abs() @ w_in[j].double().abs())
     within(got, want, ULP[dtype] * want.abs() + ACC * 64 * size + TINY[dtype])
+
+
+def nonzero_rows(t):
+    """Rows of eight 16-bit values that hold anything but zeros of either sign."""
+    words = t.view(torch.int64)
+    return torch.cat([((words[c:c + (1 << 28), 0] | words[c:c + (1 << 28), 1]) & 0x7FFF7FFF7FFF7FFF).nonzero()[:, 0] + c
+                      for c in range(0, t.shape[0], 1 << 28)])
+
+
+def test_products_of_the_most_rows(ex):  # noqa: F811
+    g, most = gen(4), (1 << 31) - 512
+    off, w = offsets_of([most - 77, 50]), normal(g, 2, 8, 8, dtype=BF16)  # 27 rows of no expert
+    at = torch.tensor([0, 1, 1 << 30, most - 300, most - 129, most - 128, most - 78, most - 77, most - 40, most - 28], device="cuda")
+    x, few = torch.zeros(most, 8, dtype=BF16, device="cuda"), normal(g, 10, 8, dtype=BF16)
+    x[at] = few
+    out = ex.grouped_mm(x, w, off)
+    assert torch.equal(nonzero_rows(out), at)
+    we = w.double()[(at >= most - 77).long()]
+    want, size = torch.einsum("rnk,rk->rn", we, few.double()), torch.einsum("rnk,rk->rn", we.abs(), few.double().abs())
+    within(out[at], want, ULP[BF16] * want.abs() + ACC * 8 * size)
+    del out
+    x[most - 1] = 1  # of no expert
+    dw = ex._wgrad(x, x, off)
+    for j, mine in enumerate((at < most - 77, at >= most - 77)):
+        v = few[mine].double()
+        within(dw[j], v.T @ v, ULP[BF16] * (v.T @ v).abs() + ACC * 16 * (v.abs().T @ v.abs()))
