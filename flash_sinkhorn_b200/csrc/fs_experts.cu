@@ -193,17 +193,18 @@ struct Candidates {
 template <typename T, int PER, int WARPS>
 __device__ __forceinline__ void select_tokens(const RouteArgs& a, int* count) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int t0 = blockIdx.x * a.chunk, t1 = min(t0 + a.chunk, a.T);
+  const int t0 = blockIdx.x * a.chunk, tokens = min(a.chunk, a.T - t0);
   float bias[PER], next[PER];
   load_bias<PER>(a, lane, bias);
   constexpr bool kEarly = PER <= 8;  // the next token's logits are on their way while this one's experts are chosen
-  if (kEarly && t0 + warp < t1) load_logits<T, PER>(a, t0 + warp, lane, bias, next);
-  for (int t = t0 + warp; t < t1; t += WARPS) {
+  if (kEarly && warp < tokens) load_logits<T, PER>(a, t0 + warp, lane, bias, next);
+  for (int i = warp; i < tokens; i += WARPS) {
+    const int t = t0 + i;
     float l[PER], top, inv;
     if (kEarly) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) l[i] = next[i];
-      if (t + WARPS < t1) load_logits<T, PER>(a, t + WARPS, lane, bias, next);
+      if (i + WARPS < tokens) load_logits<T, PER>(a, t + WARPS, lane, bias, next);
     } else {
       load_logits<T, PER>(a, t, lane, bias, l);
     }
@@ -478,10 +479,10 @@ __global__ void __launch_bounds__(kGradWarps * 32, kGradCtas<PER>) route_grad_ke
 // 64 tokens of 16 experts take 6.8 us there and 7.5 us in two launches (of 64 experts 8.1 and 10.5), 128 tokens 9.0 and
 // 7.8 us (11.3 and 10.4).
 void plan_route(int T, int& chunk, int& blocks) {
-  chunk = (T + kMaxBlocks - 1) / kMaxBlocks;
+  chunk = (int)(((long long)T + kMaxBlocks - 1) / kMaxBlocks);
   chunk = (chunk + 31) / 32 * 32;
   if (T <= 64) chunk = 64;
-  blocks = T > 0 ? (T + chunk - 1) / chunk : 1;
+  blocks = T > 0 ? (T - 1) / chunk + 1 : 1;
 }
 
 // Lets `kernel` take `most` bytes of dynamic shared memory, once for each device. The limit belongs to the kernel and all host

@@ -30,6 +30,12 @@ def test_scratch_of_a_routing():
     assert lib.fs_route_bytes(10, 1025, 2) == 0
 
 
+@pytest.mark.parametrize("t", [(1 << 31) - 1, (1 << 31) - 200, (1 << 31) - 14_000_000])
+def test_scratch_of_the_longest_batches(t):
+    """Up to 2^31 - 1 pairs, as the arguments are checked: one count for each expert and block, at most 148 blocks."""
+    assert _lib.load().fs_route_bytes(t, 4, 1) == 4 * 4 * 148
+
+
 @pytest.mark.parametrize("r", [(1 << 31) - 1, (1 << 31) - 511])
 def test_products_of_too_many_rows_are_refused(r):
     """Before anything else is looked at: a tile of the last rows would reach past 2^31."""

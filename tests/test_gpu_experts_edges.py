@@ -248,3 +248,22 @@ def test_products_of_the_most_rows(ex):  # noqa: F811
     for j, mine in enumerate((at < most - 77, at >= most - 77)):
         v = few[mine].double()
         within(dw[j], v.T @ v, ULP[BF16] * (v.T @ v).abs() + ACC * 16 * (v.abs().T @ v.abs()))
+
+
+MOST = (1 << 31) - 1  # pairs
+
+
+def test_routing_of_the_longest_batch(ex):  # noqa: F811
+    logits = torch.zeros(MOST, 2, dtype=BF16, device="cuda")
+    logits[:, 1] = -1
+    other = torch.cat([torch.tensor([0, 5, MOST - 14_000_001, MOST - 40, MOST - 1]), torch.randint(10, MOST - 50, (2000,), generator=torch.Generator().manual_seed(1))])
+    other = other.unique().cuda()
+    logits[other, 1] = 1
+    r = ex.route_tokens(logits, 1)
+    m = other.numel()
+    assert r.offsets.tolist() == [0, MOST - m, MOST]
+    assert torch.equal(r.pairs[MOST - m:].long(), other) and torch.equal(r.rows[MOST - m:], r.pairs[MOST - m:])
+    assert (r.experts[other] == 1).all() and int(torch.count_nonzero(r.experts)) == m
+    assert torch.equal(r.position[other, 0].long(), torch.arange(MOST - m, MOST, device="cuda"))
+    some = torch.randint(0, MOST - m, (5000,), generator=gen(3), device="cuda")
+    assert torch.equal(r.position[r.pairs[some].long(), 0].long(), some) and (r.gates[some] == 1).all()
