@@ -38,6 +38,7 @@ namespace {
 using namespace fs::tc;
 
 __device__ int g_group_error = 0;  // non-zero once a bounded wait gave up (read by fs_device_error)
+std::atomic<bool> g_launched{false};   // whether this process has launched a product: if not, the word is not looked at
 thread_local long long t_product_limit = kSpinLimit;  // clocks, fs_set_product_limit
 
 enum Form { ROWS_K, ROWS_MN, WEIGHTS };  // rows with W contiguous along the contraction; along the features
@@ -873,6 +874,7 @@ int launch_group(GroupArgs a, const CUtensorMap& mapA, const CUtensorMap& mapB, 
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
+  g_launched.store(true, std::memory_order_relaxed);
   e = cudaLaunchKernelEx(&cfg, kernel, a, mapA, mapB);
   if (e != cudaSuccess) return report_error(FS_ERR_CUDA, cudaGetErrorString(e));
   count_launches(1);
@@ -938,12 +940,16 @@ int not_loadable() {
 
 }  // namespace
 
+// Solvers read the health word where the host waits anyway. A copy of this part takes 12 us, and 10 ms the first time, for the
+// kernels' module to be loaded: not for programs without products.
 int group_error_flag() {
+  if (!g_launched.load(std::memory_order_relaxed)) return 0;
   int v = 0;
   if (cudaMemcpyFromSymbol(&v, g_group_error, sizeof(int)) != cudaSuccess) return -1;
   return v ? 1 : 0;
 }
 int clear_group_error_flag() {
+  if (!g_launched.load(std::memory_order_relaxed)) return 0;
   const int zero = 0;
   return cudaMemcpyToSymbol(g_group_error, &zero, sizeof(int)) == cudaSuccess ? 0 : -1;
 }

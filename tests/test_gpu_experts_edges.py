@@ -3,6 +3,9 @@
 Bounds are those of the operators' other tests: half a unit in the last place for each rounding to the type, ``FUN`` for
 the sigmoid and the products around it, ``ACC`` per term of a sum in fp32.
 """
+import os
+import subprocess
+import sys
 import threading
 
 import pytest
@@ -267,3 +270,25 @@ def test_routing_of_the_longest_batch(ex):  # noqa: F811
     assert torch.equal(r.position[other, 0].long(), torch.arange(MOST - m, MOST, device="cuda"))
     some = torch.randint(0, MOST - m, (5000,), generator=gen(3), device="cuda")
     assert torch.equal(r.position[r.pairs[some].long(), 0].long(), some) and (r.gates[some] == 1).all()
+
+
+def test_health_word_before_and_after_the_first_product():
+    """A process that has launched no product does not look at the products' part of the word; one that has does."""
+    script = """
+import torch
+from flash_sinkhorn_b200 import _lib, experts
+lib = _lib.load()
+torch.zeros(1, device="cuda")
+assert lib.fs_device_error() == 0 and lib.fs_clear_device_error() == 0
+x, w = torch.ones(40, 64, dtype=torch.bfloat16, device="cuda"), torch.ones(2, 64, 64, dtype=torch.bfloat16, device="cuda")
+off = torch.tensor([0, 20, 40], dtype=torch.int32, device="cuda")
+usual = lib.fs_set_product_limit(0)
+out = experts.grouped_mm(x, w, off)
+lib.fs_set_product_limit(usual)
+assert lib.fs_device_error() == 1 and bool(torch.isnan(out).all())
+assert lib.fs_clear_device_error() == 0 and lib.fs_device_error() == 0
+assert bool((experts.grouped_mm(x, w, off) == 64).all()) and lib.fs_device_error() == 0
+"""
+    done = subprocess.run([sys.executable, "-c", script], capture_output=True, text=True, timeout=300,
+                          cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert done.returncode == 0, done.stderr[-2000:]
