@@ -558,8 +558,9 @@ int check_route(const void* logits, int type, long long ld, int T, int E, int k)
 // ---------------------------------------------------------------------------------------------------------------
 // h = p silu(g) v of rows u = [g | v], p = the gate of the row's pair (1 without a routing). The backward pass needs g and
 // v; the checkpoint holds them in blocks of 32 along the row as integers in [-127, 127] times 2^e, e the smallest exponent
-// at which the block's largest magnitude rounds to 127 at most: 8.25 bits instead of 16, an error of at most half a step
-// = 2^-7 of the block's maximum (a quarter of that of an 8-bit float with 3 bits of fraction at the same size), and since
+// at which the block's largest magnitude rounds to 127 at most: 8.25 bits instead of 16, an error of at most half a step. The
+// maximum is 63.75 to 127.5 steps, so that is 1/127.5 of it at most (an eighth of the error of an 8-bit float with 3 bits of
+// fraction at 64 to 128 steps, whose own steps are 8 there), and since
 // scaling by a power of two is exact the codes do not depend on how the quotient is rounded. A block with an infinity or
 // a NaN has exponent code 255 and stands for NaN throughout.
 //
@@ -665,8 +666,9 @@ __device__ __forceinline__ float row_gate(const ActArgs& a, int r, bool& routed)
   routed = p >= 0 && p < a.R;  // as many pairs as rows
   return routed ? a.gates[p] : 0.f;
 }
-// 1 / (1 + 2^(-x log2 e)), to about 2^-21; 0 where the power overflows. The instructions by themselves, with results below
-// the normal range flushed: the intrinsics spend as much again on those.
+// 1 / (1 + 2^(-x log2 e)), to a relative 2^-21 and, below 0, |x| 2^-23 more: the power's argument is rounded to fp32, at -80 to
+// 2^-18. 0 from about -87.3 down, where the sigmoid leaves the normal range of fp32. The instructions by themselves, with results
+// below the normal range flushed: the intrinsics spend as much again on those.
 __device__ __forceinline__ float sigmoid(float x) {
   float e, s;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.4426950408889634f));

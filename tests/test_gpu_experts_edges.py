@@ -292,3 +292,21 @@ assert bool((experts.grouped_mm(x, w, off) == 64).all()) and lib.fs_device_error
     done = subprocess.run([sys.executable, "-c", script], capture_output=True, text=True, timeout=300,
                           cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+def test_gated_act_of_large_negative_values(ex):  # noqa: F811
+    """The sigmoid's relative error grows with |g| as stated, down to where it leaves the normal range and becomes 0.
+
+    Beside it: two products and a rounding for h, three for dv; dg is s + g s (1 - s), whose terms share the error of s and differ
+    by a factor of 19 or more."""
+    n = 4096
+    g, v, d = torch.linspace(-87.2, -20, n, device="cuda"), normal(gen(6), n, scale=3.0), normal(gen(7), n)
+    g[-64:] = torch.linspace(-1000.0, -87.5, 64, device="cuda")
+    u = torch.cat([g, v])[None].requires_grad_(True)
+    h = ex.gated_act(u, checkpoint=False)
+    (du,) = torch.autograd.grad(h, u, d[None])
+    z, s = g.double(), torch.sigmoid(g.double())
+    bound = 2.0**-21 + z.abs() * 2.0**-23 + 4 * 2.0**-24
+    for got, want in ((h[0], z * s * v.double()), (du[0, n:], d.double() * z * s), (du[0, :n], d.double() * v.double() * s * (1 + z * (1 - s)))):
+        assert ((got.double() - want).abs() <= bound * 20 / 18 * want.abs())[:-64].all()
+        assert not got[-64:].any()
