@@ -1,6 +1,7 @@
 // Routed experts around their matrix products: the choice of experts and the order of the rows, the gated activation
 // with its 8-bit checkpoint, and the sum of the experts' rows back into tokens. All of it is bound by memory traffic (the
-// routing of a large batch by instruction issue); every value is read once and nothing is kept between calls.
+// routing of a large batch by instruction issue); values are read once (the routing reads the chosen logits again) and nothing
+// is kept between calls.
 #include "fs_experts.cuh"
 #include "fs_tc.cuh"
 

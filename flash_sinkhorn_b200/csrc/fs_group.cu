@@ -18,10 +18,11 @@
 // 256 x 256 tile), and eight write the other one out, through shared memory in pieces of 64 bytes. Rows in another order are
 // fetched by eight more, 16 bytes a lane (cp.async): TMA's loads of four rows each took 75 clocks apiece, 2.6 times the time
 // of the whole product. That is for single CTAs: in a pair, rows that one CTA has written have to reach the thread of the other
-// one that issues the products by a release and an acquire at the cluster's scope, about a microsecond for each stage of
-// 0.27 (541 -> 941 us for 65536 rows of 64 groups, 2048 x 2048), so products that want pairs take their rows in order, and
-// whoever has them in another one copies them first (fs_grouped_mm_in_order). Group boundaries are read by the kernel itself; every CTA takes every n-th tile, features fastest,
-// so that the CTAs working at one time share a group's weights and rows in L2.
+// one that issues the products by a release and an acquire at the cluster's scope, about a microsecond for each stage of 0.27
+// (541 -> 941 us for 65536 rows of 64 groups, 2048 x 2048; 582 with a copy first), so products that want pairs take their rows
+// in order, and whoever has them in another one copies them first (fs_grouped_mm_in_order). Group boundaries are read by the
+// kernel itself; every CTA takes every n-th tile, features fastest, so that the CTAs working at one time share a group's weights
+// and rows in L2.
 #include "fs_experts.cuh"
 #include "fs_ptx.cuh"
 #include "fs_tc.cuh"
