@@ -160,6 +160,18 @@ SIGNATURES = {
     "fs_gated_act_grad": (c_int, [_P, _L, _P, _P, c_int, c_int, c_int, _P, _P, _P, _P, _L, _P, _P, _P, _P]),
     "fs_combine": (c_int, [_P, c_int, _L, c_int, c_int, c_int, c_int, _P, _P, _P, c_int, _L, _P]),
     "fs_combine_grad": (c_int, [_P, c_int, _L, c_int, c_int, c_int, _P, _P, _P, _P, _L, _P, _P, _P]),
+    "fs_layer_norm": (c_int, [_P, c_int, _L, c_int, c_int, _P, _P, c_int, c_float, _P, _P, _P, _P]),
+    "fs_layer_norm_grad_bytes": (c_size_t, [c_int, c_int]),
+    "fs_layer_norm_grad": (
+        c_int, [_P, c_int, _L, c_int, c_int, _P, c_int, _P, _P, _P, _L, _P, _P, _P, _P, c_size_t, _P]),
+    "fs_weights8": (c_int, [_P, c_int, _L, _L, c_int, c_int, c_int, _P, _L, _L, _P, _P]),
+    "fs_grouped_mm8_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "fs_grouped_mm8": (
+        c_int, [_P, c_int, _L, c_int, _P, c_int, _P, _L, _L, _P, c_int, c_int, c_int, c_int, _P, _P, c_int, _L, _P,
+                c_size_t, _P]),
+    "fs_orthogonalize_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "fs_orthogonalize": (
+        c_int, [_P, c_int, _L, _L, c_int, c_int, c_int, c_int, c_float, c_float, c_float, c_float, _P, c_int, _P, c_size_t, _P]),
 }
 
 _lib: Optional[ctypes.CDLL] = None

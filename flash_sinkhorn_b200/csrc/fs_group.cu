@@ -24,13 +24,11 @@
 // kernel itself; every CTA takes every n-th tile, features fastest, so that the CTAs working at one time share a group's weights
 // and rows in L2.
 #include "fs_experts.cuh"
+#include "fs_pair.cuh"
 #include "fs_ptx.cuh"
 #include "fs_tc.cuh"
 
-#include <cudaTypedefs.h>
-
 #include <atomic>
-#include <mutex>
 
 namespace fs {
 namespace ex {
@@ -71,95 +69,7 @@ struct GroupArgs {
   long long limit;  // clocks that the warps which write results wait, besides what the products take; 0: none at all
 };
 
-// ------------------------------------------------------------------ PTX of CTA pairs and gathered loads
-__device__ __forceinline__ uint32_t cta_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t in_leader(uint32_t addr) {  // the same shared-memory address in CTA 0 of the cluster
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// Frees something of the leader's: only execution is ordered, for which the default scope will do.
-__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-// Shared memory that this CTA has written goes to the thread of the leader that issues the products reading it: released and
-// acquired at the cluster's scope. For the end of a group only, once in a tile.
-__device__ __forceinline__ void arrive_release_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ bool wait_acquire_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-  const long long t0 = clock64();
-  for (;;) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    if (ok) return true;
-    if (*abort_flag) return false;
-    if (clock64() - t0 > kSpinLimit) {
-      *abort_flag = 1;
-      return false;
-    }
-  }
-}
-// For a barrier behind the products of many blocks of 64 contraction values, which take some 540 clocks each and are given
-// 4096: the limit of a single wait would run out within a group of 32 million rows, whose products are one tile.
-__device__ __forceinline__ bool wait_blocks(uint32_t bar, uint32_t parity, volatile int* abort_flag, long long blocks, long long limit) {
-  if (limit == 0) *abort_flag = 1;  // without a look, for tests
-  if (limit == 0) return false;
-  if (mbar_try_wait(bar, parity)) return true;
-  const long long t0 = clock64();
-  limit += 4096 * blocks;
-  while (!mbar_try_wait_hint(bar, parity, 2000)) {
-    if (*abort_flag) return false;
-    if (clock64() - t0 > limit) {
-      *abort_flag = 1;
-      return false;
-    }
-  }
-  return true;
-}
-template <int CG>
-__device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
-  if (CG == 2)
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];"
-        ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
-  else
-    tma_load_2d(dst, map, c0, c1, bar);
-}
-template <int CG>
-__device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
-  if (CG == 2)
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5}], [%2];"
-        ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
-  else
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-        ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
-}
-template <int CG>
-__device__ __forceinline__ void expect_at(uint32_t bar, uint32_t bytes) {  // bar: in CTA 0 of the pair
-  if (CG == 2) asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-  else mbar_expect_tx(bar, bytes);
-}
-// After a wait that gave up: for the copies in flight to land, until about 0.14 s after `t0` at most.
-__device__ __forceinline__ void wait_landed(uint32_t bar, uint32_t parity, long long t0) {
-  while (!mbar_try_wait(bar, parity))
-    if (clock64() - t0 > kSpinLimit) return;
-}
+// ------------------------------------------------------------------ PTX of gathered loads
 // 16 bytes, of which those past the first `valid` become zeros (the source is not read for them).
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int valid) {
   asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid) : "memory");
@@ -169,44 +79,6 @@ __device__ __forceinline__ void copy_arrive(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void copy_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-template <int CG>
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  if (CG == 2)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
-  else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
-}
-template <int CG>
-__device__ __forceinline__ void commit(uint32_t bar) {  // arrives at this barrier of every CTA of the pair
-  if (CG == 2)
-    asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-        ::"r"(bar), "h"((uint16_t)3) : "memory");
-  else
-    umma_commit(bar);
-}
-template <int CG>
-__device__ __forceinline__ void alloc_columns(uint32_t slot, uint32_t n) {
-  if (CG == 2) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(n) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-  } else {
-    tmem_alloc(slot, n);
-    tmem_relinquish();
-  }
-}
-template <int CG>
-__device__ __forceinline__ void free_columns(uint32_t addr, uint32_t n) {
-  if (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(n) : "memory");
-  else tmem_dealloc(addr, n);
-}
-
 // Shared-memory operands, 128-byte swizzle. K-major: rows of 64 contraction values, groups of 8 rows 1024 bytes apart; a step
 // of 16 values is 32 bytes on. MN-major: 64 rows (contraction) of 64 features, the next 64 features one half tile on (the
 // leading offset), groups of 8 contraction rows 1024 bytes apart; a step of 16 contraction rows is 2048 bytes on.
@@ -263,39 +135,6 @@ struct Tiles {
     return t;
   }
 };
-
-// First rows of the groups (running maximum of the offsets within [0, R]), of the rows of no expert (gs[E]) and the end
-// (gs[E + 1]); with TILES the number of tiles before each of them. One warp.
-template <bool TILES>
-__device__ void read_groups(const GroupArgs& a, int* gs, int* ts, int per_column, int bn) {
-  const int lane = threadIdx.x & 31;
-  int top = 0, sum = 0;
-  if (lane == 0) gs[0] = 0;
-  for (int c = 0; c <= a.E; c += 32) {
-    const int j = c + lane;
-    int end = j < a.E ? min(max(a.offsets[j + 1], 0), a.R) : a.R;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, end, o);
-      end = lane >= o ? max(end, v) : end;
-    }
-    end = max(end, top);
-    const int before = __shfl_up_sync(0xffffffffu, end, 1), begin = lane ? before : top;
-    if (j <= a.E) gs[j + 1] = end;
-    top = __shfl_sync(0xffffffffu, end, 31);
-    if (TILES) {
-      int n = j <= a.E ? (end - begin + bn - 1) / bn * per_column : 0;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, n, o);
-        n += lane >= o ? v : 0;
-      }
-      if (j <= a.E) ts[j + 1] = sum + n;
-      sum += __shfl_sync(0xffffffffu, n, 31);
-    }
-  }
-  if (TILES && lane == 0) ts[0] = 0;
-}
 
 __device__ __forceinline__ uint32_t pack_two(float lo, float hi, int type) {
   return type == FS_TYPE_BF16 ? from_two(lo, hi, __nv_bfloat16()) : from_two(lo, hi, __half());
@@ -400,7 +239,7 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
   const int first = blockIdx.x / CG, stride = gridDim.x / CG;
 
   if (warp == 0) {
-    read_groups<FORM != WEIGHTS>(a, gs, ts, (a.N + 128 * CG - 1) / (128 * CG), BN);
+    read_groups<FORM != WEIGHTS>(a.offsets, a.E, a.R, gs, ts, (a.N + 128 * CG - 1) / (128 * CG), BN);
   } else if (warp == kLoadWarp && lane == 0) {
     for (int s = 0; s < a.nstage; ++s) {
       mbar_init(bar(FULL + s), CG + (COPY ? 1 : 0));  // in CTA 0: both CTAs' loads; with COPY, the load and the report
@@ -811,19 +650,6 @@ int launch_few(const GroupArgs& a, const void* w, long long w_expert, long long 
 }
 
 // ------------------------------------------------------------------ host side
-PFN_cuTensorMapEncodeTiled_v12000 encoder() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* sym = nullptr;
-    cudaDriverEntryPointQueryResult found;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &found) == cudaSuccess &&
-        found == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(sym);
-  });
-  return fn;
-}
-
 // 16-bit tensor of 2 or 3 dimensions, contiguous along the first; boxes of 64 x box_rows.
 bool encode(CUtensorMap* map, int type, const void* base, int dims, const long long (&size)[3], const long long (&stride)[2],
             int box_rows) {
@@ -940,6 +766,8 @@ int not_loadable() {
 }
 
 }  // namespace
+
+long long product_limit() { return t_product_limit; }
 
 // Solvers read the health word where the host waits anyway. A copy of this part takes 12 us, and 10 ms the first time, for the
 // kernels' module to be loaded: not for programs without products.

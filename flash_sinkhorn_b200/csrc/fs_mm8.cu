@@ -1,0 +1,733 @@
+// Matrix products grouped by expert in 8-bit floating point (4 bits of exponent, 3 of mantissa), with a scale for each block of 128:
+//
+//   x[i, k] = sx[i, k / 128] qx[i, k],   w_e[n, k] = sw_e[n / 128, k / 128] qw_e[n, k]
+//   out[i, n] = sum over blocks c of sx[i, c] sw_e[n / 128, c] (sum over k in c of qx[i, k] qw_e[n, k])
+//
+// and the same with w_e transposed, the gradient to x. Scales are the smallest powers of two with which a block's largest magnitude
+// is at most 448, so a division by one is exact, the codes are the same wherever they are computed, and the type's exponent makes up for
+// the half of its range that a power of two may leave (a value is off by half a step of its own either way).
+//
+// Rows go into 8 bits and into the order of the experts in one pass. In the product the ROWS of a group are the M side of the
+// tensor-core instruction, so that a thread's 32 or more accumulators share the row's scale. The tensor core sums one block of 128 in
+// TMEM (fp32); eight warps read that while the next block is summed beside it, and add it, scaled, to sums in registers.
+// Per block and 128 x 256 tile the products take 512 clocks of the tensor core, reading 256 of TMEM and adding 256 of the fp32 units.
+#include "fs_experts.cuh"
+#include "fs_pair.cuh"
+#include "fs_tc.cuh"
+
+#include <cuda_fp8.h>
+
+#include <atomic>
+
+namespace fs {
+namespace ex {
+long long product_limit();  // fs_group.cu: of the calling thread
+
+namespace {
+
+__device__ int g_mm8_error = 0;  // non-zero once a bounded wait gave up (read by fs_device_error)
+std::atomic<bool> g_mm8_launched{false};
+
+constexpr int kBlock8 = 128;  // values that share a scale
+constexpr float kTop8 = 448.f;
+
+// ------------------------------------------------------------------ into 8 bits
+// Bits of the scale for a largest magnitude (float bits), and of its reciprocal; NaN and 0 for an infinity or a NaN.
+__device__ __forceinline__ void scale_of(uint32_t top, float& scale, float& inverse) {
+  // 448 = 1.75 * 2^8: 1.f * 2^e needs 2^(e - 8), or one more where 1.f is above 1.75
+  int j = (int)(top >> 23) - 135 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+  j = max(j, -126);
+  const bool finite = top < 0x7f800000u;
+  scale = __uint_as_float(finite ? (uint32_t)(j + 127) << 23 : 0x7fc00000u);
+  inverse = __uint_as_float(finite ? (uint32_t)(127 - j) << 23 : 0u);
+}
+__device__ __forceinline__ uint32_t four_codes(float a, float b, float c, float d) {
+  const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return (uint32_t)lo | (uint32_t)hi << 16;
+}
+// Eight values from column c on of a row of K, zeros past its end; vec: aligned to 16 bytes and K a multiple of 8.
+template <typename T>
+__device__ __forceinline__ void eight(const T* row, int c, int K, bool vec, float (&v)[8]) {
+  if (vec && c < K) {
+    unpack<T, 8>(read_only<T, 8>(row + c), v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = c + j < K ? to_f32(row[c + j]) : 0.f;
+  }
+}
+__device__ __forceinline__ uint32_t top_of(const float (&v)[8]) {
+  uint32_t m = 0u;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+  return m;
+}
+// `finite` false: zeros (the scale is NaN).
+__device__ __forceinline__ uint2 codes_of(const float (&v)[8], float inverse) {
+  if (inverse == 0.f) return make_uint2(0u, 0u);
+  return make_uint2(four_codes(v[0] * inverse, v[1] * inverse, v[2] * inverse, v[3] * inverse),
+                    four_codes(v[4] * inverse, v[5] * inverse, v[6] * inverse, v[7] * inverse));
+}
+
+// Rows x[rows[i]] of M rows of K values (zeros for numbers outside; rows null: row i) to codes [R, ldc] and scales [ceil(K / 128)][R]. Sixteen
+// lanes take a block of 128 values of a row. ldc is a multiple of 16; codes past K are zeros.
+template <typename T>
+__global__ void __launch_bounds__(256) rows8_kernel(const T* x, long long ldx, int M, const int* rows, int R, int K, uint8_t* codes, long long ldc,
+                                                    float* scales, bool vec) {
+  const int lane = threadIdx.x & 15, per_row = (K + kBlock8 - 1) / kBlock8;
+  const long long unit = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 4;
+  const long long i = unit / per_row;
+  const bool in = i < R;
+  const int b = (int)(unit - i * per_row), c = b * kBlock8 + lane * 8, t = !in ? -1 : rows ? __ldg(rows + i) : (int)i;
+  float v[8];
+  eight(x + (long long)t * ldx, (unsigned)t < (unsigned)M ? c : K, K, vec, v);
+  uint32_t top = top_of(v);
+#pragma unroll
+  for (int o = 8; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (!in) return;
+  float scale, inverse;
+  scale_of(top, scale, inverse);
+  if (c < ldc) *reinterpret_cast<uint2*>(codes + i * ldc + c) = codes_of(v, inverse);
+  if (lane == 0) scales[(long long)b * R + i] = scale;
+}
+
+// Weights w [E, N, K] to codes (rows c_row, matrices c_expert apart) and scales [E][ceil(N / 128)][ceil(K / 128)]: a CTA to a block of
+// 128 x 128, which it holds in registers between the search for the largest magnitude and the codes.
+template <typename T>
+__global__ void __launch_bounds__(256) weights8_kernel(const T* w, long long w_expert, long long w_row, int N, int K, uint8_t* codes, long long c_expert,
+                                                       long long c_row, float* scales, bool vec) {
+  __shared__ uint32_t part[8];
+  const int kb = (K + kBlock8 - 1) / kBlock8, nb = (N + kBlock8 - 1) / kBlock8;
+  const int e = blockIdx.x / (kb * nb), rest = blockIdx.x - e * kb * nb, n0 = rest / kb * kBlock8, k0 = rest % kb * kBlock8;
+  const int lane = threadIdx.x & 15, r0 = threadIdx.x >> 4, c = k0 + lane * 8;
+  Pack<T, 8> held[8];
+  uint32_t top = 0u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int n = n0 + r0 + 16 * i;
+    float v[8] = {};
+    if (n < N) eight(w + e * w_expert + n * w_row, c, K, vec, v);
+    store_f32<T, 8>(reinterpret_cast<T*>(&held[i]), v);  // back to the type they had: exact
+    top = max(top, top_of(v));
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, part[i]);
+  float scale, inverse;
+  scale_of(top, scale, inverse);
+  if (threadIdx.x == 0) scales[blockIdx.x] = scale;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int n = n0 + r0 + 16 * i;
+    if (n >= N || c >= (K + 15) / 16 * 16) continue;
+    float v[8];
+    unpack<T, 8>(held[i], v);
+    *reinterpret_cast<uint2*>(codes + e * c_expert + n * c_row + c) = codes_of(v, inverse);
+  }
+}
+
+// ------------------------------------------------------------------ products
+constexpr int kSumWarps = 8, kFetchWarp = 8, kIssueWarp = 9, kThreads8 = 32 * 10;
+constexpr uint32_t kTileA = 128 * 128;
+constexpr int kStage8 = 2048 * kSumWarps;  // staging of results
+
+struct Mm8Args {
+  const int* offsets;
+  int R, E, N, K;  // K: contraction
+  const float* sx;  // [ceil(K / 128)][R]
+  const float* sw;
+  long long sw_expert;
+  int sw_n, sw_k;  // distances of scales along N and K
+  void* out;
+  long long ldo;
+  int out_type, out_bytes;  // bytes of a store: 16, 4 or 2
+  int nstage;
+  long long limit;
+};
+
+template <int CG>
+__device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if (CG == 2)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+struct Tile8 {
+  int e, n0, lo, hi, blocks;  // expert, first feature, rows of the tile, blocks of 128 contraction values (0: rows of no expert)
+};
+template <int CG, int BN>
+struct Tiles8 {
+  const Mm8Args& a;
+  const int *gs, *ts;
+  int nt, e = 0;
+  __device__ Tiles8(const Mm8Args& args, const int* rows, const int* tiles) : a(args), gs(rows), ts(tiles) { nt = (a.N + BN - 1) / BN; }
+  __device__ int total() const { return ts[a.E + 1]; }
+  __device__ Tile8 at(int tile) {  // in increasing order
+    for (int end = a.E; e < end;) {
+      const int mid = (e + end) / 2;
+      if (tile >= ts[mid + 1]) e = mid + 1;
+      else end = mid;
+    }
+    const int rest = tile - ts[e], m = rest / nt;
+    Tile8 t;
+    t.e = e;
+    t.n0 = (rest - m * nt) * BN;
+    t.lo = gs[e] + m * 128 * CG;
+    t.hi = min(t.lo + 128 * CG, gs[e + 1]);
+    t.blocks = e < a.E ? (a.K + kBlock8 - 1) / kBlock8 : 0;
+    return t;
+  }
+};
+
+__device__ __forceinline__ uint32_t two16(u64 v, int type) {
+  float lo, hi;
+  upk(v, lo, hi);
+  return type == FS_TYPE_BF16 ? from_two(lo, hi, __nv_bfloat16()) : from_two(lo, hi, __half());
+}
+
+// MN: w contiguous along N (the transposed product). Single CTAs fetch rows in boxes of 32, as many as the tile has.
+template <bool MN, int CG, int BN>
+__global__ void __launch_bounds__(kThreads8, 1)
+mm8_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB) {
+  constexpr int BNC = BN / CG, kBufs = BN == 256 ? 2 : 4;
+  constexpr uint32_t kTileB = BNC * 128, kStage = kTileA + kTileB, kColumns = BN * kBufs;
+  constexpr int kBoxA = CG == 2 ? 128 : 32;
+  static_assert(kColumns <= 512 && kStage % 1024 == 0 && !(MN && BNC < 128), "tile");
+  extern __shared__ uint8_t raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* staging = ring + (size_t)a.nstage * kStage;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(staging + kStage8);
+  const int FULL = 0, EMPTY = a.nstage, ACC_FULL = 2 * a.nstage, ACC_EMPTY = ACC_FULL + kBufs, DRAIN = ACC_EMPTY + kBufs;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(bars + DRAIN + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(slot + 1);
+  int *gs = reinterpret_cast<int*>(slot + 2), *ts = gs + a.E + 2;
+  auto bar = [&](int i) { return smem_u32(bars + i); };
+
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int rank = CG == 2 ? (int)cta_rank() : 0;
+  const int first = blockIdx.x / CG, stride = gridDim.x / CG;
+
+  if (warp == 0) {
+    read_groups<true>(a.offsets, a.E, a.R, gs, ts, (a.N + BN - 1) / BN, 128 * CG);
+  } else if (warp == kFetchWarp && lane == 0) {
+    for (int s = 0; s < a.nstage; ++s) {
+      mbar_init(bar(FULL + s), CG);  // in CTA 0: both CTAs' loads
+      mbar_init(bar(EMPTY + s), 1);
+    }
+    for (int i = 0; i < kBufs; ++i) {
+      mbar_init(bar(ACC_FULL + i), 1);
+      mbar_init(bar(ACC_EMPTY + i), kSumWarps * CG);  // in CTA 0: all warps of the pair that sum
+    }
+    mbar_init(bar(DRAIN), 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  } else if (warp == kIssueWarp) {
+    alloc_columns<CG>(smem_u32(slot), kColumns);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (CG == 2) cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem = *slot;
+  Tiles8<CG, BN> tiles(a, gs, ts);
+  const int total = tiles.total();
+  int issued = 0;  // stages that this CTA's loading thread has started
+
+  if (warp == kFetchWarp) {
+    // ===================== loads =====================
+    if (elect_one()) {
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int it = first; ok && it < total; it += stride) {
+        const Tile8 t = tiles.at(it);
+        const int boxes = CG == 2 ? 1 : (t.hi - t.lo + kBoxA - 1) / kBoxA;
+        for (int kb = 0; kb < t.blocks; ++kb) {
+          if (!mbar_wait(bar(EMPTY + s), ph ^ 1, abort_flag)) {
+            ok = false;
+            break;
+          }
+          const uint32_t full = CG == 2 ? in_leader(bar(FULL + s)) : bar(FULL + s), dst = smem_u32(ring + (size_t)s * kStage);
+          expect_at<CG>(full, boxes * kBoxA * 128 + kTileB);
+          for (int i = 0; i < boxes; ++i) load_2d<CG>(dst + i * kBoxA * 128, &mapA, kb * 128, t.lo + rank * 128 + i * kBoxA, full);
+          if (MN) {
+#pragma unroll
+            for (int c = 0; c < BNC / 128; ++c)
+              load_3d<CG>(dst + kTileA + c * kTileA, &mapB, t.n0 + rank * BNC + c * 128, kb * 128, t.e, full);
+          } else {
+            load_3d<CG>(dst + kTileA, &mapB, kb * 128, t.n0 + rank * BNC, t.e, full);
+          }
+          ++issued;
+          if (++s == a.nstage) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+      }
+    }
+  } else if (warp == kIssueWarp) {
+    // ===================== products =====================
+    if (rank == 0 && elect_one()) {
+      // fp32 sums, both operands e4m3 (0)
+      constexpr uint32_t idesc = (1u << 4) | ((MN ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(128 * CG >> 4) << 24);
+      // a step of 32 contraction values: 32 bytes on, or 32 rows of 128 bytes; MN: the next 128 features one tile on
+      constexpr uint32_t kStepB = (MN ? 32u * 128u : 32u) >> 4, kLeadB = MN ? kTileA >> 4 : 1u;
+      int s = 0, buf = 0;
+      uint32_t ph = 0, acc_ph = 0;
+      bool ok = true;
+      for (int it = first; ok && it < total; it += stride) {
+        const Tile8 t = tiles.at(it);
+        for (int kb = 0; kb < t.blocks; ++kb) {
+          if (!mbar_wait(bar(ACC_EMPTY + buf), acc_ph ^ 1, abort_flag) || !mbar_wait(bar(FULL + s), ph, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t base = smem_u32(ring + (size_t)s * kStage);
+          const uint32_t al = desc_lo(base), bl = (((base + kTileA) & 0x3FFFFu) >> 4) | (kLeadB << 16);
+          const int left = a.K - kb * kBlock8;
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+            if (ks * 32 < left)
+              mma_f8<CG>(tmem + buf * BN, pack_desc(al + ks * 2, kDescHi128), pack_desc(bl + ks * kStepB, kDescHi128), idesc, ks);
+          commit<CG>(bar(EMPTY + s));
+          commit<CG>(bar(ACC_FULL + buf));
+          if (++s == a.nstage) {
+            s = 0;
+            ph ^= 1;
+          }
+          if (++buf == kBufs) {
+            buf = 0;
+            acc_ph ^= 1;
+          }
+        }
+      }
+    }
+  } else {
+    // ===================== sums and results =====================
+    // Two warps to a quarter of the TMEM lanes (rows), with one half of the features each.
+    constexpr int kMine = BN / 2;
+    const int q = warp & 3, side = warp >> 2;
+    const uint32_t stage = smem_u32(staging + 2048 * warp);
+    int buf = 0;
+    uint32_t acc_ph = 0;
+    bool lost = false;  // a wait of this CTA gave up: NaN from here on
+    for (int it = first; it < total; it += stride) {
+      const Tile8 t = tiles.at(it);
+      const int row0 = t.lo + rank * 128 + q * 32, n0 = t.n0 + side * kMine;
+      u64 sum[kMine / 2];
+#pragma unroll
+      for (int i = 0; i < kMine / 2; ++i) sum[i] = 0ull;
+      const float* sx = a.sx + min(row0 + lane, a.R - 1);
+      const float* sw = a.sw + t.e * a.sw_expert + (long long)min(n0, a.N - 1) / kBlock8 * a.sw_n;
+      float x_next = 0.f, w_next = 0.f;
+      if (t.blocks) {
+        x_next = __ldg(sx);
+        w_next = __ldg(sw);
+      }
+      for (int kb = 0; kb < t.blocks && !lost; ++kb) {
+        const float f = x_next * w_next;
+        if (kb + 1 < t.blocks) {
+          x_next = __ldg(sx + (long long)(kb + 1) * a.R);
+          w_next = __ldg(sw + (long long)(kb + 1) * a.sw_k);
+        }
+        lost = !__all_sync(0xffffffffu, wait_blocks(bar(ACC_FULL + buf), acc_ph, abort_flag, 4, a.limit));
+        if (lost) break;
+        tc_fence_after();
+        const u64 f2 = pk(f, f);
+#pragma unroll
+        for (int j = 0; j < kMine / 32; ++j) {
+          uint32_t r[32];
+          tmem_ld32_nowait(tmem + buf * BN + side * kMine + 32 * j + ((uint32_t)(q * 32) << 16), r);
+          tmem_ld_wait(r);
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            sum[16 * j + i] = fma2(pk(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), f2, sum[16 * j + i]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (CG == 2) arrive_cluster(in_leader(bar(ACC_EMPTY + buf)));
+          else mbar_arrive(bar(ACC_EMPTY + buf));
+        }
+        if (++buf == kBufs) {
+          buf = 0;
+          acc_ph ^= 1;
+        }
+      }
+      if (lost && t.blocks) {
+        const float nan = __uint_as_float(0x7fc00000u);
+#pragma unroll
+        for (int i = 0; i < kMine / 2; ++i) sum[i] = pk(nan, nan);
+      }
+      const int rows = t.hi - row0;
+      if (rows <= 0) continue;
+      const int width = a.out_type == FS_TYPE_F32 ? 4 : 2;
+      char* out = static_cast<char*>(a.out) + (long long)row0 * a.ldo * width;
+#pragma unroll
+      for (int j = 0; j < kMine / 32; ++j) {
+        const int n = n0 + 32 * j;
+        if (n >= a.N) break;
+        if (a.out_type != FS_TYPE_F32) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            stage16(staged_row(stage, lane, c), two16(sum[16 * j + 4 * c], a.out_type), two16(sum[16 * j + 4 * c + 1], a.out_type),
+                    two16(sum[16 * j + 4 * c + 2], a.out_type), two16(sum[16 * j + 4 * c + 3], a.out_type));
+          __syncwarp();
+          write_rows(out + 2ll * n, a.ldo * 2, rows, 2 * (a.N - n), a.out_bytes, stage, lane);
+          __syncwarp();
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              float v[4];
+              upk(sum[16 * j + 8 * h + 2 * c], v[0], v[1]);
+              upk(sum[16 * j + 8 * h + 2 * c + 1], v[2], v[3]);
+              stage16(staged_row(stage, lane, c), __float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+            }
+            __syncwarp();
+            write_rows(out + 4ll * (n + 16 * h), a.ldo * 4, rows, 4 * (a.N - n - 16 * h), a.out_bytes, stage, lane);
+            __syncwarp();
+          }
+        }
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {  // nobody waits any more, and the flag does not change
+    if (warp == kIssueWarp && rank == 0) {  // every product issued here ends before TMEM is freed
+      if (elect_one()) {
+        commit<CG>(bar(DRAIN));
+        mbar_wait_quiet(bar(DRAIN), 0);
+      }
+      __syncwarp();
+    } else if (warp == kFetchWarp) {
+      // The copies in flight land before the CTA ends; those of the second CTA of a pair, which the first one counts, are
+      // given a millisecond, hundreds of times what a copy takes.
+      if (elect_one()) {
+        const long long t0 = clock64();
+        if (rank == 0)
+          for (int j = issued > a.nstage ? issued - a.nstage : 0; j < issued; ++j) wait_landed(bar(FULL + j % a.nstage), (j / a.nstage) & 1, t0);
+        else
+          while (clock64() - t0 < (1ll << 21)) {}
+      }
+      __syncwarp();
+    }
+  }
+  if (CG == 2) cluster_sync_all();
+  tc_fence_after();
+  if (warp == kIssueWarp) free_columns<CG>(tmem, kColumns);
+  if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_mm8_error, 1);
+}
+
+// ------------------------------------------------------------------ few rows
+// A single token: bound by reading its experts' weights, so a warp takes one feature of one expert, 16 codes a lane and load, as the
+// 16-bit products do. Each CTA puts the rows into 8 bits itself (a few microseconds less than a launch that does it once).
+constexpr int kFewRows8 = 2, kFewWarps8 = 8, kFewMost8 = 8192;  // rows; contraction values that shared memory takes
+
+// Shared memory of a row: its codes, padded to 128, and their scales.
+__host__ __device__ constexpr size_t few8_row_bytes(int blocks) { return ((size_t)blocks * (kBlock8 + 4) + 15) / 16 * 16; }
+__device__ __forceinline__ float2 two_of_codes(uint32_t pair) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(pair & 0xffffu), __NV_E4M3);
+  return __half22float2(__half2(h));
+}
+template <typename T, int ROWS>
+__global__ void __launch_bounds__(32 * kFewWarps8, 4)
+few8_kernel(const Mm8Args a, const T* x0, long long ldx, int M, const int* rows, const uint8_t* w, long long w_expert, long long w_row, bool vec) {
+  __shared__ int first_after[2];
+  extern __shared__ __align__(16) uint8_t held[];
+  const int lane = threadIdx.x & 31, i = blockIdx.y, blocks = (a.K + kBlock8 - 1) / kBlock8;
+  // The expert of row i is the one before the first offset above i (offsets as their running maximum); a row whose
+  // predecessor has the same one is left to the CTA of the expert's first row.
+  if (threadIdx.x < 2) first_after[threadIdx.x] = a.E + 1;
+  __syncthreads();
+  int above = a.E + 1, reached = a.E + 1;  // first offset above row i, above row i - 1
+  for (int j = 1 + threadIdx.x; j <= a.E; j += 32 * kFewWarps8) {
+    const int v = a.offsets[j];
+    if (v > i) above = min(above, j);
+    if (v >= i) reached = min(reached, j);
+  }
+  above = __reduce_min_sync(0xffffffffu, above);
+  reached = __reduce_min_sync(0xffffffffu, reached);
+  if (lane == 0) {
+    atomicMin(&first_after[0], above);
+    atomicMin(&first_after[1], reached);
+  }
+  __syncthreads();
+  const int e = first_after[0] - 1, f = blockIdx.x * kFewWarps8 + (threadIdx.x >> 5);
+  auto store = [&](int row, float v) {
+    const long long at = (long long)row * a.ldo + f;
+    if (a.out_type == FS_TYPE_F32) static_cast<float*>(a.out)[at] = v;
+    else static_cast<T*>(a.out)[at] = from_f32<T>(v);
+  };
+  if (e == a.E) {  // a row of no expert
+    if (lane == 0 && f < a.N) store(i, 0.f);
+    return;
+  }
+  if (i > 0 && first_after[1] == first_after[0]) return;
+  const int end = min(a.offsets[e + 1], a.R);
+  const size_t row_bytes = few8_row_bytes(blocks);
+  for (int u = threadIdx.x >> 4; u < ROWS * blocks; u += 2 * kFewWarps8) {
+    const int r = u / blocks, b = u - r * blocks, l = threadIdx.x & 15;
+    const int n = i + r < end ? (rows ? rows[i + r] : i + r) : -1;
+    float v[8] = {};
+    if ((unsigned)n < (unsigned)M) eight(x0 + n * ldx, b * kBlock8 + l * 8, a.K, vec, v);
+    uint32_t top = top_of(v);
+#pragma unroll
+    for (int o = 8; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffu << (threadIdx.x & 16), top, o));
+    float scale, inverse;
+    scale_of(top, scale, inverse);
+    *reinterpret_cast<uint2*>(held + r * row_bytes + b * kBlock8 + l * 8) = codes_of(v, inverse);
+    if (l == 0) *reinterpret_cast<float*>(held + r * row_bytes + blocks * kBlock8 + 4 * b) = scale;
+  }
+  __syncthreads();
+  if (f >= a.N) return;
+  const uint8_t* wf = w + e * w_expert + f * w_row;
+  const float* sw = a.sw + e * a.sw_expert + (long long)(f / kBlock8) * a.sw_n;
+  float sums[ROWS] = {};
+  constexpr int kDeep = 4;
+  const int chunks = (a.K + 15) / 16;
+#pragma unroll 1
+  for (int c0 = lane; c0 < chunks; c0 += 32 * kDeep) {
+    uint4 q[kDeep];
+    float s[kDeep];
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d) {
+      const int c = c0 + 32 * d;
+      if (c >= chunks) continue;
+      if (16 * c + 16 <= a.K) {
+        q[d] = __ldg(reinterpret_cast<const uint4*>(wf + 16 * c));
+      } else {  // what lies past the row's end is not read
+        uint32_t part[4] = {};
+        for (int k = 16 * c; k < a.K; ++k) part[(k >> 2) & 3] |= (uint32_t)wf[k] << (8 * (k & 3));
+        q[d] = make_uint4(part[0], part[1], part[2], part[3]);
+      }
+      s[d] = __ldg(sw + (long long)(c >> 3) * a.sw_k);
+    }
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d) {
+      const int c = c0 + 32 * d;
+      if (c >= chunks) continue;
+      const uint32_t wq[4] = {q[d].x, q[d].y, q[d].z, q[d].w};
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        const uint4 p = *reinterpret_cast<const uint4*>(held + r * row_bytes + 16 * c);
+        const uint32_t xq[4] = {p.x, p.y, p.z, p.w};
+        float t = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float2 wv = two_of_codes(wq[j] >> (16 * h)), xv = two_of_codes(xq[j] >> (16 * h));
+            t = fmaf(wv.y, xv.y, fmaf(wv.x, xv.x, t));
+          }
+        sums[r] = fmaf(t, s[d] * *reinterpret_cast<const float*>(held + r * row_bytes + blocks * kBlock8 + 4 * (c >> 3)), sums[r]);
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sums[r] += __shfl_xor_sync(0xffffffffu, sums[r], o);
+    if (lane == r && i + r < end) store(i + r, sums[r]);
+  }
+}
+
+// ------------------------------------------------------------------ host side
+// 8-bit tensor of 2 or 3 dimensions, contiguous along the first; boxes of 128 x box_rows.
+bool encode8(CUtensorMap* map, const void* base, int dims, const long long (&size)[3], const long long (&stride)[2], int box_rows) {
+  const cuuint64_t sizes[3] = {(cuuint64_t)size[0], (cuuint64_t)size[1], (cuuint64_t)size[2]};
+  const cuuint64_t strides[2] = {(cuuint64_t)stride[0], (cuuint64_t)stride[1]};
+  const cuuint32_t box[3] = {128, (cuuint32_t)box_rows, 1}, ones[3] = {1, 1, 1};
+  const auto fn = encoder();
+  return fn && fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, dims, const_cast<void*>(base), sizes, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool MN, int CG, int BN>
+int launch_mm8(Mm8Args a, const uint8_t* x, long long ldx, const uint8_t* w, long long w_expert, long long w_row, cudaStream_t st) {
+  CUtensorMap mapA = {}, mapB = {};
+  // w's own rows and columns: K and N change places in the transposed product
+  const long long w_cols = MN ? a.N : a.K, w_rows = MN ? a.K : a.N;
+  if (!encode8(&mapA, x, 2, {a.K, a.R, 1}, {ldx, 0}, CG == 2 ? 128 : 32) ||
+      !encode8(&mapB, w, 3, {w_cols, w_rows, a.E}, {w_row, w_expert ? w_expert : w_row}, MN ? 128 : BN / CG))
+    return report_error(FS_ERR_CUDA, "cuTensorMapEncodeTiled failed");
+  constexpr size_t kStage = kTileA + BN / CG * 128;
+  const size_t fixed = 1024 + kStage8 + 8 * (2 * 12 + 9) + 8 + 8 * ((size_t)a.E + 2);
+  a.nstage = (int)((kSmemMax - fixed) / kStage);
+  if (a.nstage > 12) a.nstage = 12;
+  size_t smem = fixed + a.nstage * kStage;
+  if (smem < (size_t)kSmemMin) smem = kSmemMin;
+  const auto kernel = mm8_kernel<MN, CG, BN>;
+  static std::atomic<uint64_t> allowed{0};  // devices on which the kernel may take all shared memory
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (e == cudaSuccess && !(allowed.load(std::memory_order_relaxed) & bit)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
+    if (e == cudaSuccess) allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
+  if (e != cudaSuccess) return report_error(FS_ERR_CUDA, cudaGetErrorString(e));
+  const long long most = ((a.R + 128ll * CG - 1) / (128 * CG) + a.E + 1) * ((a.N + BN - 1) / BN);
+  if (most > 0x3fffffffll) return report_error(FS_ERR_UNSUPPORTED, "more than 2^30 tiles");
+  long long grid = detail::free_ctas() / CG;
+  if (grid > most) grid = most;
+  if (grid < 1) grid = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)grid * CG);
+  cfg.blockDim = dim3(kThreads8);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = CG;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  g_mm8_launched.store(true, std::memory_order_relaxed);
+  e = cudaLaunchKernelEx(&cfg, kernel, a, mapA, mapB);
+  if (e != cudaSuccess) return report_error(FS_ERR_CUDA, cudaGetErrorString(e));
+  count_launches(1);
+  return FS_OK;
+}
+
+template <typename T>
+int launch_rows8(const void* x, long long ldx, int M, const int* rows, int R, int K, uint8_t* codes, long long ldc, float* scales, cudaStream_t st) {
+  const long long units = (long long)R * ((K + kBlock8 - 1) / kBlock8), grid = (units + 15) / 16;
+  if (grid > 0x7fffffffll) return report_error(FS_ERR_UNSUPPORTED, "too many blocks of 128 values");
+  const bool vec = aligned(x, 16) && ldx % 8 == 0 && K % 8 == 0;
+  rows8_kernel<T><<<(unsigned)grid, 256, 0, st>>>(static_cast<const T*>(x), ldx, M, rows, R, K, codes, ldc, scales, vec);
+  return launched(1);
+}
+template <typename T>
+int launch_few8(const Mm8Args& a, const void* x, long long ldx, int M, const int* rows, const uint8_t* w, long long w_expert, long long w_row, cudaStream_t st) {
+  const dim3 grid((a.N + kFewWarps8 - 1) / kFewWarps8, a.R);
+  const size_t smem = a.R * few8_row_bytes((a.K + kBlock8 - 1) / kBlock8);
+  const bool vec = aligned(x, 16) && ldx % 8 == 0 && a.K % 8 == 0;
+  const T* xt = static_cast<const T*>(x);
+  if (a.R == 1) few8_kernel<T, 1><<<grid, 32 * kFewWarps8, smem, st>>>(a, xt, ldx, M, rows, w, w_expert, w_row, vec);
+  else few8_kernel<T, 2><<<grid, 32 * kFewWarps8, smem, st>>>(a, xt, ldx, M, rows, w, w_expert, w_row, vec);
+  return launched(1);
+}
+
+bool few8(int R, int K, bool transposed) { return R <= kFewRows8 && K <= kFewMost8 && !transposed; }
+long long ldc_of(int K) { return ((long long)K + 15) / 16 * 16; }
+size_t codes_bytes(int R, int K) { return ((size_t)R * ldc_of(K) + 255) / 256 * 256; }
+
+int check8(int R, int E, int N, int K) {
+  if (R < 0 || R > 0x7fffffff - 511 || E < 1 || E > 1024 || N < 1 || K < 1 || N > (1 << 22) || K > (1 << 22))
+    return report_error(FS_ERR_BAD_ARG, "R must be in [0, 2^31 - 512], E in [1, 1024], N and K in [1, 2^22]");
+  // A thread that has launched nothing yet (autograd's) has no current context, which the encoding of tensor maps needs;
+  // setting the device that is current binds it.
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess)
+    return report_error(FS_ERR_CUDA, "cannot make the current CUDA device's context current");
+  return check_device();
+}
+bool is16(int type) { return type == FS_TYPE_F16 || type == FS_TYPE_BF16; }
+
+}  // namespace
+
+int mm8_error_flag() {
+  if (!g_mm8_launched.load(std::memory_order_relaxed)) return 0;
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_mm8_error, sizeof(int)) != cudaSuccess) return -1;
+  return v ? 1 : 0;
+}
+int clear_mm8_error_flag() {
+  if (!g_mm8_launched.load(std::memory_order_relaxed)) return 0;
+  const int zero = 0;
+  return cudaMemcpyToSymbol(g_mm8_error, &zero, sizeof(int)) == cudaSuccess ? 0 : -1;
+}
+
+}  // namespace ex
+}  // namespace fs
+
+using namespace fs;
+using namespace fs::ex;
+
+extern "C" {
+
+int fs_weights8(const void* w, int type, long long w_expert, long long w_row, int E, int N, int K, uint8_t* codes, long long c_expert, long long c_row,
+                float* scales, void* stream) {
+  const int s = check8(0, E, N, K);
+  if (s != FS_OK) return s;
+  if (!is16(type)) return report_error(FS_ERR_BAD_ARG, "type must be FS_TYPE_F16 or FS_TYPE_BF16");
+  if (!w || !codes || !scales || w_row < K || w_expert < 0 || c_row < K || c_row % 16 || c_expert % 16 || c_expert < 0 || (E > 1 && c_expert < c_row * N) || !aligned(codes, 16))
+    return report_error(FS_ERR_BAD_ARG, "null argument, or rows or experts that overlap or are not a multiple of 16 codes apart");
+  const long long grid = (long long)E * ((N + kBlock8 - 1) / kBlock8) * ((K + kBlock8 - 1) / kBlock8);
+  if (grid > 0x7fffffffll) return report_error(FS_ERR_UNSUPPORTED, "too many blocks of 128 x 128 values");
+  const bool vec = aligned(w, 16) && w_row % 8 == 0 && w_expert % 8 == 0 && K % 8 == 0;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (type == FS_TYPE_F16)
+    weights8_kernel<<<(unsigned)grid, 256, 0, st>>>(static_cast<const __half*>(w), w_expert, w_row, N, K, codes, c_expert, c_row, scales, vec);
+  else
+    weights8_kernel<<<(unsigned)grid, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(w), w_expert, w_row, N, K, codes, c_expert, c_row, scales, vec);
+  return launched(1);
+}
+
+size_t fs_grouped_mm8_bytes(int R, int K, int transposed) {
+  if (R < 1 || K < 1 || few8(R, K, transposed != 0)) return 0;
+  return codes_bytes(R, K) + (size_t)R * ((K + kBlock8 - 1) / kBlock8) * sizeof(float);
+}
+
+int fs_grouped_mm8(const void* x, int type, long long ldx, int M, const int* rows, int R, const uint8_t* w, long long w_expert,
+                   long long w_row, const float* scales, int E, int N, int K, int transposed, const int* offsets, void* out,
+                   int out_type, long long ldo, void* ws, size_t ws_bytes, void* stream) {
+  int s = check8(R, E, N, K);
+  if (s != FS_OK || R == 0) return s;
+  if (!is16(type) || (out_type != type && out_type != FS_TYPE_F32))
+    return report_error(FS_ERR_BAD_ARG, "type must be FS_TYPE_F16 or FS_TYPE_BF16, the result's the same or FS_TYPE_F32");
+  if (!x || !w || !scales || !offsets || !out || ldx < K || ldo < N || M < 1 || M > 0x7fffffff - 511 || (!rows && M < R))
+    return report_error(FS_ERR_BAD_ARG, "null argument, or too few or too many rows or columns");
+  const int w_cols = transposed ? N : K, w_rows = transposed ? K : N;
+  if (w_row < w_cols || w_row % 16 || w_expert % 16 || w_expert < 0 || (E > 1 && w_expert == 0) || !aligned(w, 16))
+    return report_error(FS_ERR_BAD_ARG, "rows and experts of w must be a multiple of 16 codes apart and not overlap, the first one aligned to 16 bytes");
+  Mm8Args a{};
+  a.offsets = offsets; a.R = R; a.E = E; a.N = N; a.K = K; a.out = out; a.ldo = ldo; a.out_type = out_type;
+  a.sw = scales;
+  const long long across = (w_cols + kBlock8 - 1) / kBlock8, down = (w_rows + kBlock8 - 1) / kBlock8;
+  if (across * down > 0x7fffffffll) return report_error(FS_ERR_UNSUPPORTED, "too many blocks of 128 x 128 values");
+  a.sw_expert = across * down; a.sw_n = transposed ? 1 : (int)across; a.sw_k = transposed ? (int)across : 1;
+  a.limit = product_limit();
+  const int width = type_bytes(out_type);
+  a.out_bytes = aligned(out, 16) && ldo * width % 16 == 0 && (long long)N * width % 16 == 0 ? 16
+                : aligned(out, 4) && ldo * width % 4 == 0 && (long long)N * width % 4 == 0  ? 4 : 2;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (few8(R, K, transposed != 0))
+    return type == FS_TYPE_F16 ? launch_few8<__half>(a, x, ldx, M, rows, w, w_expert, w_row, st)
+                               : launch_few8<__nv_bfloat16>(a, x, ldx, M, rows, w, w_expert, w_row, st);
+  if (!ws || ws_bytes < fs_grouped_mm8_bytes(R, K, transposed)) return report_error(FS_ERR_WORKSPACE, "workspace too small");
+  if (!aligned(ws, 256)) return report_error(FS_ERR_BAD_ARG, "workspace must be aligned to 256 bytes");
+  uint8_t* codes = static_cast<uint8_t*>(ws);
+  float* sx = reinterpret_cast<float*>(codes + codes_bytes(R, K));
+  a.sx = sx;
+  const long long ldc = ldc_of(K);
+  s = type == FS_TYPE_F16 ? launch_rows8<__half>(x, ldx, M, rows, R, K, codes, ldc, sx, st)
+                          : launch_rows8<__nv_bfloat16>(x, ldx, M, rows, R, K, codes, ldc, sx, st);
+  if (s != FS_OK) return s;
+  const long long tiles = ((R + 255ll) / 256 + (E < R ? E : R) / 2) * ((N + 255) / 256);
+  if (transposed) {
+    if (tiles * 2 > detail::free_ctas() && N > 128) return launch_mm8<true, 2, 256>(a, codes, ldc, w, w_expert, w_row, st);
+    return launch_mm8<true, 1, 128>(a, codes, ldc, w, w_expert, w_row, st);
+  }
+  if (tiles * 2 > detail::free_ctas() && N > 128 && R / E > 64) return launch_mm8<false, 2, 256>(a, codes, ldc, w, w_expert, w_row, st);
+  const long long mid = ((R + 127ll) / 128 + (E < R ? E : R) / 2) * ((N + 127) / 128);
+  if (mid > detail::free_ctas() && R / E > 64) return launch_mm8<false, 1, 128>(a, codes, ldc, w, w_expert, w_row, st);
+  return launch_mm8<false, 1, 64>(a, codes, ldc, w, w_expert, w_row, st);
+}
+
+}  // extern "C"

@@ -1,0 +1,587 @@
+// Orthogonal updates: for each matrix G of a stack, with n = its smaller dimension as rows (a tall matrix is worked on transposed),
+//
+//   X = G / (|G| + eps)  (|.|: Frobenius),   then in every step   A = X X^T,  P = b A + c A A,  X <- a X + P X
+//
+// which maps each singular value s to a s + b s^3 + c s^5 and leaves the singular vectors: a chain of matrix products.
+//
+// Operands are fp16, sums fp32 (TMEM). A step multiplies the parts along small singular values by a = 3.4 or so, 485 over five steps, and
+// with them whatever roundings left there: with bf16 operands a matrix with decaying singular values comes out 7 % off,
+// with fp16 ones 1 %. So X is held as a sum of two fp16 values: the products take the upper one, and a X, which is what
+// carries the small parts on, is of both (22 bits); the roundings of the products come in with b s^2 and c s^4 only, 0.02 to
+// 0.2 % for those matrices, below the rounding of a bf16 result. X is held times 2^8, A and P times 2^10, so that small entries
+// keep their bits: entries of X up to 255 and of P up to 63 in magnitude fit.
+//
+// A and P are symmetric: only tiles on and below the diagonal are computed, and written twice. The products are batched over the
+// stack; tiles of 256 x 256 by pairs of CTAs, or 128 x 128 or 128 x 64 by single ones where there are too few.
+#include "fs_experts.cuh"
+#include "fs_pair.cuh"
+#include "fs_tc.cuh"
+
+#include <atomic>
+
+namespace fs {
+namespace ex {
+long long product_limit();  // fs_group.cu: of the calling thread
+
+namespace {
+
+__device__ int g_ortho_error = 0;  // non-zero once a bounded wait gave up (read by fs_device_error)
+std::atomic<bool> g_ortho_launched{false};
+
+constexpr float kXScale = 256.f, kAScale = 1024.f;  // X and A are held times these
+constexpr int kNormParts = 64;                      // CTAs that sum the squares of a matrix
+
+// ------------------------------------------------------------------ X = G / |G|
+// Sums of squares in 64 bits: those of 32-bit values would overflow from 2^64 on.
+template <typename T>
+__global__ void __launch_bounds__(256) squares_kernel(const T* g, long long g_matrix, long long g_row, int rows, int cols, double* parts) {
+  __shared__ double warp_sums[8];
+  const T* m = g + blockIdx.y * g_matrix;
+  double s = 0.0;
+  for (int r = blockIdx.x; r < rows; r += gridDim.x)
+    for (int c = threadIdx.x; c < cols; c += 256) {
+      const double v = (double)to_f32(m[(long long)r * g_row + c]);
+      s = fma(v, v, s);
+    }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if ((threadIdx.x & 31) == 0) warp_sums[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 8; ++w) s += warp_sums[w];
+    parts[blockIdx.y * gridDim.x + blockIdx.x] = s;
+  }
+}
+// Tiles of 32 x 32 of G to both parts of X, transposed for a tall G; X [n, k], rows ldx apart.
+template <typename T>
+__global__ void __launch_bounds__(256) begin_kernel(const T* g, long long g_matrix, long long g_row, int rows, int cols, const double* parts, int count,
+                                                    float eps, bool tall, __half* hi, __half* lo, long long ldx) {
+  __shared__ float tile[32][33];
+  __shared__ float factor;
+  const int b = blockIdx.z, r0 = blockIdx.y * 32, c0 = blockIdx.x * 32, x = threadIdx.x & 31, y = threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    double s = 0.0;
+    for (int i = 0; i < count; ++i) s += parts[b * count + i];
+    factor = (float)((double)kXScale / (sqrt(s) + (double)eps));
+  }
+  __syncthreads();
+  const float f = factor;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = r0 + y + 8 * i, c = c0 + x;
+    tile[y + 8 * i][x] = r < rows && c < cols ? to_f32(g[b * g_matrix + (long long)r * g_row + c]) * f : 0.f;
+  }
+  __syncthreads();
+  const int n = tall ? cols : rows, k = tall ? rows : cols, n0 = tall ? c0 : r0, k0 = tall ? r0 : c0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = n0 + y + 8 * i, col = k0 + x;
+    if (row >= n || col >= k) continue;
+    const float v = tall ? tile[x][y + 8 * i] : tile[y + 8 * i][x];
+    const __half h = __float2half_rn(v);
+    const long long at = ((long long)b * n + row) * ldx + col;
+    hi[at] = h;
+    lo[at] = __float2half_rn(v - __half2float(h));
+  }
+}
+
+// ------------------------------------------------------------------ products
+enum Product { GRAM, SQUARE, APPLY, LAST };  // LAST: APPLY to the result
+
+constexpr int kWriteWarps = 8, kGetWarp = 8, kMulWarp = 9, kThreadsO = 32 * 10;
+constexpr int kStageO = 2048 * kWriteWarps;
+
+struct OrthoArgs {
+  int batch, n, k;          // X is n x k, A and P are n x n
+  long long ldx, lda;
+  const __half *hi, *lo;    // X as it is (APPLY, LAST)
+  __half *hi_out, *lo_out;  // lo_out may be lo
+  const __half* a;          // A (SQUARE)
+  __half* sym;              // A (GRAM) or P (SQUARE)
+  float ca, cb, cc;
+  void* out;  // LAST: [n, k] or, tall, [k, n]
+  int out_type, out_bytes;
+  bool tall;
+  int nstage;
+  long long limit;
+};
+
+template <int FORM, int CG, int BN>
+struct TilesO {
+  const OrthoArgs& a;
+  int mt, nt, per;
+  __device__ explicit TilesO(const OrthoArgs& args) : a(args) {
+    constexpr int BM = 128 * CG, R = BM / BN > 0 ? BM / BN : 1;
+    mt = (a.n + BM - 1) / BM;
+    if (FORM >= APPLY) {
+      nt = (a.k + BN - 1) / BN;
+      per = mt * nt;
+    } else {  // tiles (i, j) with j < (i + 1) R, as far as there are columns
+      nt = (a.n + BN - 1) / BN;
+      per = R * mt * (mt - 1) / 2 + nt;
+      if (per < 0) per = 0;
+    }
+  }
+  __device__ long long total() const { return (long long)per * a.batch; }
+  __device__ void at(long long tile, int& b, int& m0, int& n0) const {
+    constexpr int BM = 128 * CG, R = BM / BN > 0 ? BM / BN : 1;
+    b = (int)(tile / per);
+    int rest = (int)(tile - (long long)b * per);
+    if (FORM >= APPLY) {
+      const int j = rest / mt;
+      m0 = (rest - j * mt) * BM;
+      n0 = j * BN;
+    } else {
+      int i = 0;
+      while (i + 1 < mt && rest >= (i + 1) * R) rest -= (++i) * R;
+      m0 = i * BM;
+      n0 = rest * BN;
+    }
+  }
+};
+
+// 32 values of a row, of which there are `left`, padded to a multiple of 8.
+__device__ __forceinline__ void load_row32(const __half* p, long long left, float (&v)[32]) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const uint4 q = 8 * c < left ? *(reinterpret_cast<const uint4*>(p) + c) : make_uint4(0u, 0u, 0u, 0u);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) two_f32(w[j], v[8 * c + 2 * j], v[8 * c + 2 * j + 1], __half());
+  }
+}
+
+template <int FORM, int CG, int BN>
+__global__ void __launch_bounds__(kThreadsO, 1)
+ortho_kernel(const OrthoArgs a, const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB) {
+  constexpr bool B_MN = FORM >= APPLY;
+  constexpr int BNC = BN / CG;  // columns whose operand this CTA fetches
+  constexpr uint32_t kA = 128 * 128, kB = BNC * 128, kStage = kA + kB, kHalf = 64 * 128, kColumns = 2 * BN;
+  static_assert(kColumns <= 512 && kStage % 1024 == 0 && BNC >= 64, "tile");
+  extern __shared__ uint8_t raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* staging = ring + (size_t)a.nstage * kStage;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(staging + kStageO);
+  const int FULL = 0, EMPTY = a.nstage, ACC_FULL = 2 * a.nstage, ACC_EMPTY = ACC_FULL + 2, DRAIN = ACC_EMPTY + 2;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(bars + DRAIN + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(slot + 1);
+  auto bar = [&](int i) { return smem_u32(bars + i); };
+
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int rank = CG == 2 ? (int)cta_rank() : 0;
+  const int first = blockIdx.x / CG, stride = gridDim.x / CG;
+  const int contraction = FORM == GRAM ? a.k : a.n, blocks = (contraction + 63) / 64;
+
+  if (warp == kGetWarp && lane == 0) {
+    for (int s = 0; s < a.nstage; ++s) {
+      mbar_init(bar(FULL + s), CG);  // in CTA 0: both CTAs' loads
+      mbar_init(bar(EMPTY + s), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(ACC_FULL + i), 1);
+      mbar_init(bar(ACC_EMPTY + i), kWriteWarps * CG);  // in CTA 0: all warps of the pair that write
+    }
+    mbar_init(bar(DRAIN), 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  } else if (warp == kMulWarp) {
+    alloc_columns<CG>(smem_u32(slot), kColumns);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (CG == 2) cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem = *slot;
+  const TilesO<FORM, CG, BN> tiles(a);
+  const long long total = tiles.total();
+  int issued = 0;
+
+  if (warp == kGetWarp) {
+    // ===================== loads =====================
+    if (elect_one()) {
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (long long it = first; ok && it < total; it += stride) {
+        int b, m0, n0;
+        tiles.at(it, b, m0, n0);
+        for (int kb = 0; kb < blocks; ++kb) {
+          if (!mbar_wait(bar(EMPTY + s), ph ^ 1, abort_flag)) {
+            ok = false;
+            break;
+          }
+          const uint32_t full = CG == 2 ? in_leader(bar(FULL + s)) : bar(FULL + s), dst = smem_u32(ring + (size_t)s * kStage);
+          expect_at<CG>(full, kStage);
+          load_3d<CG>(dst, &mapA, kb * 64, m0 + rank * 128, b, full);
+          if (B_MN) {
+#pragma unroll
+            for (int c = 0; c < BNC / 64; ++c) load_3d<CG>(dst + kA + c * kHalf, &mapB, n0 + rank * BNC + c * 64, kb * 64, b, full);
+          } else {
+            load_3d<CG>(dst + kA, &mapB, kb * 64, n0 + rank * BNC, b, full);
+          }
+          ++issued;
+          if (++s == a.nstage) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+      }
+    }
+  } else if (warp == kMulWarp) {
+    // ===================== products =====================
+    if (rank == 0 && elect_one()) {
+      // fp32 sums of fp16 operands
+      constexpr uint32_t idesc = (1u << 4) | ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(128 * CG >> 4) << 24);
+      // a step of 16 contraction values: 32 bytes on, or 16 rows of 128 bytes; MN: the next 64 columns one half tile on
+      constexpr uint32_t kStepB = (B_MN ? 16u * 128u : 32u) >> 4, kLeadB = B_MN ? kHalf >> 4 : 1u;
+      int s = 0, n = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (long long it = first; ok && it < total; it += stride, ++n) {
+        const int buf = n & 1;
+        if (!mbar_wait(bar(ACC_EMPTY + buf), ((n >> 1) & 1) ^ 1, abort_flag)) break;
+        tc_fence_after();
+        for (int kb = 0; kb < blocks; ++kb) {
+          if (!mbar_wait(bar(FULL + s), ph, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t base = smem_u32(ring + (size_t)s * kStage);
+          const uint32_t al = desc_lo(base), bl = (((base + kA) & 0x3FFFFu) >> 4) | (kLeadB << 16);
+          const int left = contraction - kb * 64;
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+            if (ks * 16 < left)
+              mma_f16<CG>(tmem + buf * BN, pack_desc(al + ks * 2, kDescHi128), pack_desc(bl + ks * kStepB, kDescHi128), idesc, kb | ks);
+          commit<CG>(bar(EMPTY + s));
+          if (++s == a.nstage) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+        if (!ok) break;
+        commit<CG>(bar(ACC_FULL + buf));
+      }
+    }
+  } else {
+    // ===================== results =====================
+    // Two warps to a quarter of the TMEM lanes (rows), with every other 32 columns each.
+    const int q = warp & 3, side = warp >> 2;
+    const uint32_t stage = smem_u32(staging + 2048 * warp);
+    int t = 0;
+    bool lost = false;  // a wait of this CTA gave up: NaN from here on
+    for (long long it = first; it < total; it += stride, ++t) {
+      int b, m0, n0;
+      tiles.at(it, b, m0, n0);
+      const int buf = t & 1, row0 = m0 + rank * 128 + q * 32, row = row0 + lane;
+      if (!lost) {
+        lost = !__all_sync(0xffffffffu, wait_blocks(bar(ACC_FULL + buf), (t >> 1) & 1, abort_flag, blocks, a.limit));
+        tc_fence_after();
+      }
+      const int width = FORM >= APPLY ? a.k : a.n;  // columns of the product
+#pragma unroll 1
+      for (int c = 32 * side; c < BN; c += 64) {
+        const int col = n0 + c;
+        if (col >= width || row0 >= a.n) break;
+        float v[32];
+        if (lost) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(0x7fc00000u);
+        } else {
+          tmem_ld32(tmem + buf * BN + c + ((uint32_t)(q * 32) << 16), v);
+        }
+        const bool in = row < a.n;
+        if (FORM == GRAM) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] *= kAScale / (kXScale * kXScale);
+        } else if (FORM == SQUARE) {
+          float old[32];
+          if (in) load_row32(a.a + ((long long)b * a.n + row) * a.lda + col, a.lda - col, old);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = fmaf(v[j], a.cc / kAScale, a.cb * old[j]);
+        } else {
+          float old[32], low[32];
+          const long long at = ((long long)b * a.n + row) * a.ldx + col;
+          if (in) {
+            load_row32(a.hi + at, a.ldx - col, old);
+            load_row32(a.lo + at, a.ldx - col, low);
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = fmaf(v[j], 1.f / kAScale, a.ca * (old[j] + low[j]));
+        }
+        const int rows = a.n - row0;
+        if (FORM == LAST) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] *= 1.f / kXScale;
+          uint16_t* out = static_cast<uint16_t*>(a.out) + (long long)b * a.n * a.k;
+          if (a.tall) {  // 32 lanes write 64 bytes of a row of the result
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const uint32_t w = a.out_type == FS_TYPE_BF16 ? from_two(v[j], 0.f, __nv_bfloat16()) : from_two(v[j], 0.f, __half());
+              if (in && col + j < a.k) out[(long long)(col + j) * a.n + row] = (uint16_t)w;
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t w[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                w[j] = a.out_type == FS_TYPE_BF16 ? from_two(v[8 * i + 2 * j], v[8 * i + 2 * j + 1], __nv_bfloat16())
+                                                  : from_two(v[8 * i + 2 * j], v[8 * i + 2 * j + 1], __half());
+              stage16(staged_row(stage, lane, i), w[0], w[1], w[2], w[3]);
+            }
+            __syncwarp();
+            write_rows(reinterpret_cast<char*>(out + (long long)row0 * a.k + col), 2ll * a.k, rows, 2 * (a.k - col), a.out_bytes, stage, lane);
+            __syncwarp();
+          }
+        } else {
+          uint32_t h[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) h[j] = from_two(v[2 * j], v[2 * j + 1], __half());
+          const long long ld = FORM == APPLY ? a.ldx : a.lda;
+          __half* out = (FORM == APPLY ? a.hi_out : a.sym) + ((long long)b * a.n + row0) * ld + col;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) stage16(staged_row(stage, lane, i), h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+          __syncwarp();
+          write_rows(reinterpret_cast<char*>(out), 2 * ld, rows, 2 * (width - col), 16, stage, lane);  // rows are padded to 16 bytes
+          __syncwarp();
+          if (FORM == APPLY) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              float x, y;
+              two_f32(h[j], x, y, __half());
+              h[j] = from_two(v[2 * j] - x, v[2 * j + 1] - y, __half());
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) stage16(staged_row(stage, lane, i), h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+            __syncwarp();
+            write_rows(reinterpret_cast<char*>(a.lo_out + ((long long)b * a.n + row0) * ld + col), 2 * ld, rows, 2 * (width - col), 16, stage, lane);
+            __syncwarp();
+          } else if (n0 + BN <= m0 && in) {  // and the same above the diagonal
+            uint16_t* mirror = reinterpret_cast<uint16_t*>(a.sym) + ((long long)b * a.n + col) * ld + row;
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (col + j < a.n) mirror[j * ld] = (uint16_t)(j & 1 ? h[j / 2] >> 16 : h[j / 2]);
+          }
+        }
+      }
+      if (!lost) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (CG == 2) arrive_cluster(in_leader(bar(ACC_EMPTY + buf)));
+          else mbar_arrive(bar(ACC_EMPTY + buf));
+        }
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {  // nobody waits any more, and the flag does not change
+    if (warp == kMulWarp && rank == 0) {  // every product issued here ends before TMEM is freed
+      if (elect_one()) {
+        commit<CG>(bar(DRAIN));
+        mbar_wait_quiet(bar(DRAIN), 0);
+      }
+      __syncwarp();
+    } else if (warp == kGetWarp) {
+      // The copies in flight land before the CTA ends; those of the second CTA of a pair, which the first one counts, are
+      // given a millisecond, hundreds of times what a copy takes.
+      if (elect_one()) {
+        const long long t0 = clock64();
+        if (rank == 0)
+          for (int j = issued > a.nstage ? issued - a.nstage : 0; j < issued; ++j) wait_landed(bar(FULL + j % a.nstage), (j / a.nstage) & 1, t0);
+        else
+          while (clock64() - t0 < (1ll << 21)) {}
+      }
+      __syncwarp();
+    }
+  }
+  if (CG == 2) cluster_sync_all();
+  tc_fence_after();
+  if (warp == kMulWarp) free_columns<CG>(tmem, kColumns);
+  if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_ortho_error, 1);
+}
+
+// ------------------------------------------------------------------ host side
+// fp16 stack [batch][rows][cols], rows ld apart; boxes of 64 x box_rows.
+bool encode_stack(CUtensorMap* map, const __half* base, long long cols, long long rows, long long batch, long long ld, int box_rows) {
+  const cuuint64_t sizes[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)batch};
+  const cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)(ld * rows) * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1}, ones[3] = {1, 1, 1};
+  const auto fn = encoder();
+  return fn && fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<__half*>(base), sizes, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int FORM, int CG, int BN>
+int launch_ortho(OrthoArgs a, cudaStream_t st) {
+  CUtensorMap mapA = {}, mapB = {};
+  const __half* left = FORM == GRAM ? a.hi : FORM == SQUARE ? a.a : a.sym;
+  const bool good =
+      FORM == GRAM ? encode_stack(&mapA, left, a.k, a.n, a.batch, a.ldx, 128) && encode_stack(&mapB, left, a.k, a.n, a.batch, a.ldx, BN / CG)
+      : FORM == SQUARE ? encode_stack(&mapA, left, a.n, a.n, a.batch, a.lda, 128) && encode_stack(&mapB, left, a.n, a.n, a.batch, a.lda, BN / CG)
+                       : encode_stack(&mapA, left, a.n, a.n, a.batch, a.lda, 128) && encode_stack(&mapB, a.hi, a.k, a.n, a.batch, a.ldx, 64);
+  if (!good) return report_error(FS_ERR_CUDA, "cuTensorMapEncodeTiled failed");
+  constexpr size_t kStage = 128 * 128 + BN / CG * 128;
+  constexpr size_t fixed = 1024 + kStageO + 8 * (2 * 12 + 5) + 8;
+  a.nstage = (int)((kSmemMax - fixed) / kStage);
+  if (a.nstage > 12) a.nstage = 12;
+  size_t smem = fixed + a.nstage * kStage;
+  if (smem < (size_t)kSmemMin) smem = kSmemMin;
+  const auto kernel = ortho_kernel<FORM, CG, BN>;
+  static std::atomic<uint64_t> allowed{0};  // devices on which the kernel may take all shared memory
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (e == cudaSuccess && !(allowed.load(std::memory_order_relaxed) & bit)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
+    if (e == cudaSuccess) allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
+  if (e != cudaSuccess) return report_error(FS_ERR_CUDA, cudaGetErrorString(e));
+  const long long mt = (a.n + 128 * CG - 1) / (128 * CG), most = mt * (((FORM >= APPLY ? a.k : a.n) + BN - 1) / BN) * a.batch;
+  long long grid = detail::free_ctas() / CG;
+  if (grid > most) grid = most;
+  if (grid < 1) grid = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)grid * CG);
+  cfg.blockDim = dim3(kThreadsO);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = CG;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  g_ortho_launched.store(true, std::memory_order_relaxed);
+  e = cudaLaunchKernelEx(&cfg, kernel, a, mapA, mapB);
+  if (e != cudaSuccess) return report_error(FS_ERR_CUDA, cudaGetErrorString(e));
+  count_launches(1);
+  return FS_OK;
+}
+template <int FORM>
+int launch_form(const OrthoArgs& a, cudaStream_t st) {
+  const int ctas = detail::free_ctas();
+  auto tiles = [&](int bm, int bn) {
+    const long long m = (a.n + bm - 1) / bm, n = ((FORM >= APPLY ? a.k : a.n) + bn - 1) / bn;
+    return (FORM >= APPLY ? m * n : m * n / 2 + 1) * a.batch;
+  };
+  if (tiles(256, 256) * 2 > ctas) return launch_ortho<FORM, 2, 256>(a, st);
+  if (tiles(128, 128) > ctas) return launch_ortho<FORM, 1, 128>(a, st);
+  return launch_ortho<FORM, 1, 64>(a, st);
+}
+
+template <typename T>
+int begin(const void* g, long long g_matrix, long long g_row, int batch, int rows, int cols, double* parts, float eps, bool tall, __half* hi, __half* lo,
+          long long ldx, cudaStream_t st) {
+  const T* gt = static_cast<const T*>(g);
+  const int count = rows < kNormParts ? rows : kNormParts;
+  for (int b0 = 0; b0 < batch; b0 += 65535) {  // the limit of a grid's second and third dimension
+    const int nb = batch - b0 < 65535 ? batch - b0 : 65535;
+    squares_kernel<T><<<dim3(count, nb), 256, 0, st>>>(gt + b0 * g_matrix, g_matrix, g_row, rows, cols, parts + (size_t)b0 * count);
+    const long long at = (long long)b0 * (tall ? cols : rows) * ldx;
+    begin_kernel<T><<<dim3((cols + 31) / 32, (rows + 31) / 32, nb), 256, 0, st>>>(gt + b0 * g_matrix, g_matrix, g_row, rows, cols,
+                                                                                  parts + (size_t)b0 * count, count, eps, tall, hi + at, lo + at, ldx);
+  }
+  return launched(2);
+}
+
+struct OrthoSpace {
+  size_t x, a, parts, all;  // bytes of one part of X, of A, of the sums of squares
+};
+OrthoSpace ortho_space(int batch, int rows, int cols) {
+  const size_t n = rows < cols ? rows : cols, k = rows < cols ? cols : rows;
+  auto round = [](size_t v, size_t to) { return (v + to - 1) / to * to; };
+  OrthoSpace s;
+  s.x = round((size_t)batch * n * round(k, 8) * 2, 256);
+  s.a = round((size_t)batch * n * round(n, 8) * 2, 256);
+  s.parts = round((size_t)batch * kNormParts * sizeof(double), 256);
+  s.all = 3 * s.x + 2 * s.a + s.parts;
+  return s;
+}
+
+}  // namespace
+
+int ortho_error_flag() {
+  if (!g_ortho_launched.load(std::memory_order_relaxed)) return 0;
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_ortho_error, sizeof(int)) != cudaSuccess) return -1;
+  return v ? 1 : 0;
+}
+int clear_ortho_error_flag() {
+  if (!g_ortho_launched.load(std::memory_order_relaxed)) return 0;
+  const int zero = 0;
+  return cudaMemcpyToSymbol(g_ortho_error, &zero, sizeof(int)) == cudaSuccess ? 0 : -1;
+}
+
+}  // namespace ex
+}  // namespace fs
+
+using namespace fs;
+using namespace fs::ex;
+
+extern "C" {
+
+size_t fs_orthogonalize_bytes(int batch, int rows, int cols) {
+  if (batch < 1 || rows < 1 || cols < 1) return 0;
+  return ortho_space(batch, rows, cols).all;
+}
+
+int fs_orthogonalize(const void* g, int type, long long g_matrix, long long g_row, int batch, int rows, int cols, int steps, float a, float b,
+                     float c, float eps, void* out, int out_type, void* ws, size_t ws_bytes, void* stream) {
+  if (type < FS_TYPE_F32 || type > FS_TYPE_BF16 || (out_type != FS_TYPE_F16 && out_type != FS_TYPE_BF16))
+    return report_error(FS_ERR_BAD_ARG, "type must be one of FS_TYPE_*, that of the result FS_TYPE_F16 or FS_TYPE_BF16");
+  if (batch < 0 || rows < 1 || cols < 1 || rows > 65536 || cols > 65536 || g_row < cols || steps < 1 || steps > 64 || !(eps > 0.f))
+    return report_error(FS_ERR_BAD_ARG, "batch must not be negative, rows and cols in [1, 65536], rows not overlap, steps in [1, 64] and eps be positive");
+  const int s = check_device();
+  if (s != FS_OK || batch == 0) return s;
+  if (!g || !out || g_matrix < 0) return report_error(FS_ERR_BAD_ARG, "null argument");
+  const OrthoSpace space = ortho_space(batch, rows, cols);
+  if (!ws || ws_bytes < space.all) return report_error(FS_ERR_WORKSPACE, "workspace too small");
+  if (!aligned(ws, 256)) return report_error(FS_ERR_BAD_ARG, "workspace must be aligned to 256 bytes");
+  int dev = 0;  // binds the device's context to a thread that has launched nothing yet: the encoding of tensor maps needs one
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess)
+    return report_error(FS_ERR_CUDA, "cannot make the current CUDA device's context current");
+  const bool tall = rows > cols;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  uint8_t* p = static_cast<uint8_t*>(ws);
+  __half *hi = reinterpret_cast<__half*>(p), *other = reinterpret_cast<__half*>(p + space.x), *lo = reinterpret_cast<__half*>(p + 2 * space.x);
+  __half *sym = reinterpret_cast<__half*>(p + 3 * space.x), *poly = reinterpret_cast<__half*>(p + 3 * space.x + space.a);
+  double* parts = reinterpret_cast<double*>(p + 3 * space.x + 2 * space.a);
+  OrthoArgs o{};
+  o.batch = batch;
+  o.n = tall ? cols : rows;
+  o.k = tall ? rows : cols;
+  o.ldx = (o.k + 7) / 8 * 8;
+  o.lda = (o.n + 7) / 8 * 8;
+  o.ca = a; o.cb = b; o.cc = c;
+  o.lo = o.lo_out = lo;
+  o.out = out; o.out_type = out_type; o.tall = tall;
+  o.out_bytes = aligned(out, 16) && o.k % 8 == 0 ? 16 : aligned(out, 4) && o.k % 2 == 0 ? 4 : 2;
+  o.limit = product_limit();
+  int r = type == FS_TYPE_F32  ? begin<float>(g, g_matrix, g_row, batch, rows, cols, parts, eps, tall, hi, lo, o.ldx, st)
+          : type == FS_TYPE_F16 ? begin<__half>(g, g_matrix, g_row, batch, rows, cols, parts, eps, tall, hi, lo, o.ldx, st)
+                                : begin<__nv_bfloat16>(g, g_matrix, g_row, batch, rows, cols, parts, eps, tall, hi, lo, o.ldx, st);
+  for (int i = 0; i < steps && r == FS_OK; ++i) {
+    o.hi = hi;
+    o.hi_out = other;
+    o.sym = sym;
+    r = launch_form<GRAM>(o, st);
+    if (r != FS_OK) return r;
+    o.a = sym;
+    o.sym = poly;
+    r = launch_form<SQUARE>(o, st);
+    if (r != FS_OK) return r;
+    r = i + 1 < steps ? launch_form<APPLY>(o, st) : launch_form<LAST>(o, st);
+    __half* t = hi;
+    hi = other;
+    other = t;
+  }
+  return r;
+}
+
+}  // extern "C"

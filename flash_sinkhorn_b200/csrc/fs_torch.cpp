@@ -25,7 +25,8 @@ constexpr int64_t kMaxExperts = 1024, kMaxK = 32, kBlock = 32, kMaxRows = (int64
 // Entry points of the library that is loaded.
 #define FS_ENTRIES(F)                                                                                                     \
   F(fs_last_error) F(fs_route_bytes) F(fs_route) F(fs_route_grad) F(fs_grouped_mm) F(fs_grouped_mm_in_order) F(fs_grouped_mm_wgrad) F(fs_gated_act) \
-  F(fs_gated_act_grad) F(fs_combine) F(fs_combine_grad)
+  F(fs_gated_act_grad) F(fs_combine) F(fs_combine_grad) F(fs_layer_norm) F(fs_layer_norm_grad_bytes) F(fs_layer_norm_grad) F(fs_weights8)             \
+  F(fs_grouped_mm8_bytes) F(fs_grouped_mm8) F(fs_orthogonalize_bytes) F(fs_orthogonalize)
 struct Library {
 #define FS_MEMBER(name) decltype(&::name) name = nullptr;
   FS_ENTRIES(FS_MEMBER)
@@ -238,6 +239,63 @@ std::tuple<Tensor, Tensor, Tensor> act_grad_raw(const Tensor& u, const Tensor& h
   return {du, dgates, h};
 }
 
+// Rows [R, F] of a tensor of any number of dimensions, and the call on them.
+Tensor as_rows(const Tensor& t) {
+  const int64_t f = t.size(-1);
+  return rows_of(t.dim() == 2 ? t : t.reshape({t.numel() / f, f}));
+}
+struct Norm {
+  Tensor y, mean, rstd;
+};
+Norm norm_raw(const Tensor& x, const Tensor& w, const Tensor& b, double eps, bool keep) {
+  const Place at(x);
+  Norm n;
+  n.y = fresh(x.sizes(), x);
+  if (keep) {  // one buffer
+    const Tensor both = fresh({2, x.size(0)}, at::kFloat, x);
+    n.mean = both.select(0, 0);
+    n.rstd = both.select(0, 1);
+  }
+  FS_CALL(fs_layer_norm, data(x), type_of(x), ld(x), (int)x.size(0), (int)x.size(1), data(w), data(b), type_of(w.defined() ? w : b.defined() ? b : x),
+          (float)eps, data(n.y), floats(n.mean), floats(n.rstd), at.stream);
+  return n;
+}
+
+// Codes [E, N, K], rows and experts a multiple of 16 apart, and scales.
+std::pair<Tensor, Tensor> weights8_raw(const Tensor& w0) {
+  const Place at(w0);
+  const Tensor w = w0.stride(2) == 1 && w0.stride(1) >= w0.size(2) && w0.stride(0) >= 0 ? w0 : w0.contiguous();
+  const int64_t e = w.size(0), n = w.size(1), k = w.size(2), to = (k + 15) / 16 * 16;
+  const Tensor codes = fresh({e, n, to}, at::kFloat8_e4m3fn, w), scales = fresh({e, (n + 127) / 128, (k + 127) / 128}, at::kFloat, w);
+  // strides of dimensions of size 1 say nothing
+  FS_CALL(fs_weights8, w.data_ptr(), type_of(w), w.stride(0), std::max(w.stride(1), k), (int)e, (int)n, (int)k, static_cast<uint8_t*>(codes.data_ptr()), n * to,
+          to, floats(scales), at.stream);
+  return {codes.narrow(2, 0, k), scales};
+}
+// `codes [E, N, K]` as tensor loads take them; themselves, or a copy with padded rows.
+Tensor loadable_codes(const Tensor& c) {
+  const int64_t e = c.size(0), n = c.size(1), k = c.size(2), to = (k + 15) / 16 * 16;
+  if (aligned16(c) && c.stride(2) == 1 && c.stride(1) % 16 == 0 && c.stride(1) >= k && c.stride(0) % 16 == 0 && (c.stride(0) > 0 || e == 1)) return c;
+  const Place at(c);
+  const Tensor out = fresh({e, n, to}, c).narrow(2, 0, k);
+  out.copy_(c);
+  return out;
+}
+// x in order (rows undefined) or x[rows], times the weights or their transposes.
+Tensor mm8_raw(const Tensor& x, const Tensor& rows, int64_t count, const Tensor& codes0, const Tensor& scales, const Tensor& offsets, bool transposed,
+               bool fp32) {
+  const Place at(x);
+  const Tensor codes = loadable_codes(codes0);
+  const int64_t n = codes.size(transposed ? 2 : 1), k = codes.size(transposed ? 1 : 2);
+  const size_t bytes = lib.fs_grouped_mm8_bytes((int)count, (int)k, transposed);
+  Tensor out = fresh({count, n}, fp32 ? at::kFloat : x.scalar_type(), x), ws;
+  if (bytes) ws = fresh({(int64_t)bytes}, at::kByte, x);
+  FS_CALL(fs_grouped_mm8, data(x), type_of(x), ld(x), (int)x.size(0), ints(rows), (int)count,
+          static_cast<const uint8_t*>(codes.data_ptr()), codes.stride(0), codes.stride(1), floats(scales), (int)codes.size(0), (int)n, (int)k, transposed,
+          ints(offsets), data(out), type_of(out), n, data(ws), bytes, at.stream);
+  return out;
+}
+
 // ------------------------------------------------------------------ autograd
 struct Route : torch::autograd::Function<Route> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits0, int64_t k, const optional<Tensor>& bias0, const optional<Tensor>& mask0,
@@ -365,6 +423,67 @@ struct Mlp : torch::autograd::Function<Mlp> {
   }
 };
 
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x0, const optional<Tensor>& w0, const optional<Tensor>& b0, double eps) {
+    const Tensor x = as_rows(x0), w = none(w0), b = none(b0);
+    const Norm n = norm_raw(x, w, b, eps, true);
+    ctx->save_for_backward({x, w, n.mean, n.rstd});
+    ctx->saved_data["type"] = type_of(w.defined() ? w : b.defined() ? b : x);
+    ctx->saved_data["bias"] = b.defined();
+    return n.y.view(x0.sizes());
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const Tensor &x = s[0], &w = s[1];
+    Tensor dx, dw, db;
+    if (grads[0].defined()) {
+      const Place at(x);
+      const Tensor dy = as_rows(grads[0]);
+      const int64_t r = x.size(0), f = x.size(1), w_type = ctx->saved_data["type"].toInt();
+      const auto like = w_type == FS_TYPE_F32 ? at::kFloat : w_type == FS_TYPE_F16 ? at::kHalf : at::kBFloat16;
+      if (ctx->needs_input_grad(0)) dx = fresh(x.sizes(), x);
+      size_t input = 1;  // of those that are there
+      if (w.defined() && ctx->needs_input_grad(input++)) dw = fresh({f}, like, x);
+      if (ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(input)) db = fresh({f}, like, x);
+      Tensor ws;
+      const size_t bytes = dw.defined() || db.defined() ? lib.fs_layer_norm_grad_bytes((int)r, (int)f) : 0;
+      if (bytes) ws = fresh({(int64_t)bytes}, at::kByte, x);
+      FS_CALL(fs_layer_norm_grad, data(x), type_of(x), ld(x), (int)r, (int)f, data(w), (int)w_type, floats(s[2]), floats(s[3]), data(dy), ld(dy), data(dx),
+              data(dw), data(db), data(ws), bytes, at.stream);
+      if (dx.defined()) dx = dx.view(grads[0].sizes());
+    }
+    return once({dx, dw, db, Tensor()});
+  }
+};
+
+// The gradient to x goes through the same codes of the weights, that to 16-bit weights is of the rows as they were.
+struct GroupedMm8 : torch::autograd::Function<GroupedMm8> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x0, const optional<Tensor>& w, const optional<Tensor>& codes0, const optional<Tensor>& scales0,
+                        const Tensor& offsets, const optional<Tensor>& rows0, const optional<Tensor>& position0, int64_t count) {
+    const Tensor x = rows_of(x0), rows = none(rows0), position = none(position0);
+    Tensor codes = none(codes0), scales = none(scales0);
+    if (w.has_value()) std::tie(codes, scales) = weights8_raw(*w);
+    const bool grad_x = x0.requires_grad(), grad_w = w.has_value() && w->requires_grad();
+    ctx->save_for_backward({grad_w ? x : Tensor(), grad_x ? codes : Tensor(), grad_x ? scales : Tensor(), offsets, rows, position});
+    return mm8_raw(x, rows, count, codes, scales, offsets, false, false);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const Tensor &x = s[0], &codes = s[1], &offsets = s[3], &rows = s[4], &position = s[5];
+    Tensor dx, dw;
+    if (grads[0].defined()) {
+      const Tensor dy = rows_of(grads[0]);
+      if (ctx->needs_input_grad(0)) {
+        // of gathered rows in fp32, so that the sum over a token's rows is rounded once
+        dx = mm8_raw(dy, Tensor(), dy.size(0), codes, s[2], offsets, true, rows.defined());
+        if (rows.defined()) dx = combine_raw(dx, Tensor(), position, dy.scalar_type());
+      }
+      if (ctx->needs_input_grad(1)) dw = wgrad_raw(dy, rows.defined() ? gather_raw(x, rows) : x, offsets);
+    }
+    return once({dx, dw, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
+  }
+};
+
 // ------------------------------------------------------------------ public calls
 std::vector<Tensor> route_tokens(const Tensor& logits0, int64_t k, const optional<Tensor>& bias0, const optional<Tensor>& mask0, bool over_all) {
   REQUIRE(logits0.dim() == 2, "logits must be 2D [T, E], got shape ", shape_of(logits0));
@@ -480,6 +599,104 @@ Tensor expert_mlp(const Tensor& x0, const Tensor& w_in0, const Tensor& w_out0, c
   return combine_raw(mm_raw(h, Tensor(), count, w_out0, offsets, false, false), Tensor(), position, x0.scalar_type());
 }
 
+Tensor layer_norm(const Tensor& x, const optional<Tensor>& w0, const optional<Tensor>& b0, double eps) {
+  REQUIRE(x.dim() >= 1 && x.size(-1) > 0, "x must be [..., F] with F > 0, got shape ", shape_of(x));
+  check_type("x", x, true);
+  check_cuda("x", x);
+  const Tensor w = none(w0), b = none(b0);
+  const int64_t f = x.size(-1);
+  for (const auto& [name, t] : {std::pair<const char*, const Tensor&>{"weight", w}, {"bias", b}}) {
+    if (!t.defined()) continue;
+    check_place(name, t, "x", x);
+    REQUIRE(t.dim() == 1 && t.size(0) == f, name, " must have shape (", f, ",), got ", shape_of(t));
+    REQUIRE(t.scalar_type() == x.scalar_type() || t.scalar_type() == at::kFloat, name, " must be float32 or of the type of x (", type_name(x), "), got ",
+            type_name(t));
+  }
+  REQUIRE(!w.defined() || !b.defined() || w.scalar_type() == b.scalar_type(), "weight and bias must be of one type");
+  REQUIRE(eps >= 0 && eps < 3e38, "eps must not be negative");
+  REQUIRE(f <= (1 << 24) && x.numel() / f < (int64_t(1) << 31), "F must be at most 2^24, rows fewer than 2^31");
+  const Tensor wc = w.defined() ? w.contiguous() : w, bc = b.defined() ? b.contiguous() : b;
+  if (wants_grad({&x, &w, &b})) return LayerNorm::apply(x, maybe(wc), maybe(bc), eps);
+  return norm_raw(as_rows(x), wc, bc, eps, false).y.view(x.sizes());
+}
+
+std::pair<Tensor, Tensor> to_blocks8(const Tensor& w) {
+  REQUIRE(w.dim() == 3 && w.size(0) > 0 && w.size(1) > 0 && w.size(2) > 0, "weight must be 3D [E, N, K] and not empty, got shape ", shape_of(w));
+  check_type("weight", w, false);
+  check_cuda("weight", w);
+  REQUIRE(w.size(0) <= kMaxExperts && w.size(1) <= (1 << 22) && w.size(2) <= (1 << 22), "weight must have at most ", kMaxExperts,
+          " experts, N and K be at most 2^22");
+  return weights8_raw(w);
+}
+
+Tensor grouped_mm8(const Tensor& x0, const optional<Tensor>& w0, const optional<Tensor>& codes0, const optional<Tensor>& scales0, const Tensor& offsets,
+                   const optional<Tensor>& rows0, const optional<Tensor>& position0, bool gather) {
+  const Tensor w16 = none(w0), codes = none(codes0), scales = none(scales0);
+  const Tensor& w = w16.defined() ? w16 : codes;
+  REQUIRE(x0.dim() == 2 && w.dim() == 3, "x must be 2D and weight 3D [E, N, K], got shapes ", shape_of(x0), " and ", shape_of(w));
+  check_type("x", x0, false);
+  const int64_t e = w.size(0), n = w.size(1), k = w.size(2);
+  if (w16.defined()) {
+    REQUIRE(w.scalar_type() == x0.scalar_type(), "weight must be of the type of x (", type_name(x0), ") or a Blocks8, got ", type_name(w));
+  } else {
+    REQUIRE(w.scalar_type() == at::kFloat8_e4m3fn, "codes must be of type float8_e4m3fn, got ", type_name(w));
+    REQUIRE(scales.scalar_type() == at::kFloat && scales.is_contiguous() && scales.dim() == 3 && scales.size(0) == e && scales.size(1) == (n + 127) / 128 &&
+                scales.size(2) == (k + 127) / 128,
+            "scales must be a contiguous float32 tensor of shape (E, ceil(N / 128), ceil(K / 128)) for codes ", shape_of(w), ", got ", type_name(scales), " ",
+            shape_of(scales));
+    REQUIRE(!scales.requires_grad(), "scales must not require grad");
+  }
+  check_cuda("x", x0);
+  check_place("weight", w, "x", x0);
+  if (scales.defined()) check_place("scales", scales, "x", x0);
+  REQUIRE(x0.size(1) == k && k > 0 && n > 0, "x must have as many columns as weight (", k, " > 0), got ", x0.size(1), "; N must be > 0, got ", n);
+  REQUIRE(n <= (1 << 22) && k <= (1 << 22), "N and K must be at most 2^22");
+  check_offsets(offsets, x0);
+  int64_t count = x0.size(0);
+  Tensor rows, position = none(position0);
+  if (position.defined()) {  // of a routing
+    check_position(position, x0);
+    count = position.numel();
+    if (gather) {
+      rows = none(rows0);
+      check_field("rows", rows, position, true, at::kInt, x0);
+    } else {
+      position = Tensor();
+    }
+    const int64_t want = gather ? position.size(0) : count;
+    REQUIRE(x0.size(0) == want, "x must have ", want, " rows, got ", x0.size(0));
+  }
+  REQUIRE(!gather || position.size(1) <= kMaxK, "k must be at most ", kMaxK);
+  REQUIRE(offsets.size(0) == e + 1 && e <= kMaxExperts, "groups must have as many experts as weight (", e, ", at most ", kMaxExperts, "), got ",
+          offsets.size(0) - 1);
+  REQUIRE(count <= kMaxRows && x0.size(0) <= kMaxRows, "rows must be at most 2^31 - 512");
+  if (wants_grad({&x0, &w16})) return GroupedMm8::apply(x0, maybe(w16), maybe(codes), maybe(scales), offsets, maybe(rows), maybe(position), count);
+  if (!w16.defined()) return mm8_raw(rows_of(x0), rows, count, codes, scales, offsets, false, false);
+  const auto [c, s] = weights8_raw(w16);
+  return mm8_raw(rows_of(x0), rows, count, c, s, offsets, false, false);
+}
+
+Tensor orthogonalize(const Tensor& g0, int64_t steps, double a, double b, double c, double eps, bool bf16) {
+  REQUIRE(g0.dim() >= 2 && g0.size(-1) > 0 && g0.size(-2) > 0, "g must be [..., N, K] with N, K > 0, got shape ", shape_of(g0));
+  check_type("g", g0, true);
+  check_cuda("g", g0);
+  const int64_t n = g0.size(-2), k = g0.size(-1), batch = g0.numel() / (n * k);
+  REQUIRE(n <= 65536 && k <= 65536, "N and K must be at most 65536, got ", n, " and ", k);
+  REQUIRE(batch < (1 << 20), "a stack must have fewer than 2^20 matrices");
+  REQUIRE(steps >= 1 && steps <= 64, "steps must be between 1 and 64, got ", steps);
+  REQUIRE(std::abs(a) <= 16 && std::abs(b) + std::abs(c) <= 32, "coefficients must be at most 16, and the last two together at most 32, in magnitude");
+  REQUIRE(eps >= 1e-30 && eps < 3e38, "eps must be positive (1e-30 at least)");
+  Tensor g = g0.dim() == 3 ? g0 : g0.reshape({batch, n, k});
+  if (g.stride(2) != 1 || g.stride(1) < k || g.stride(0) < 0) g = g.contiguous();
+  const Place at(g);
+  const Tensor out = fresh(g0.sizes(), bf16 ? at::kBFloat16 : at::kHalf, g);
+  const size_t bytes = lib.fs_orthogonalize_bytes((int)batch, (int)n, (int)k);
+  const Tensor ws = fresh({(int64_t)bytes}, at::kByte, g);
+  FS_CALL(fs_orthogonalize, data(g), type_of(g), g.stride(0), std::max(g.stride(1), k), (int)batch, (int)n, (int)k, (int)steps, (float)a, (float)b, (float)c,
+          (float)eps, data(out), type_of(out), data(ws), bytes, at.stream);
+  return out;
+}
+
 }  // namespace
 
 namespace py = pybind11;
@@ -517,6 +734,10 @@ PYBIND11_MODULE(fs_torch, m) {
   m.def("gated_act", &gated_act, no_gil);
   m.def("combine_rows", &combine_rows, no_gil);
   m.def("expert_mlp", &expert_mlp, no_gil);
+  m.def("layer_norm", &layer_norm, no_gil);
+  m.def("to_blocks8", &to_blocks8, no_gil);
+  m.def("grouped_mm8", &grouped_mm8, no_gil);
+  m.def("orthogonalize", &orthogonalize, no_gil);
   // the kernels by themselves, without autograd
   m.def("mm", [](const Tensor& x, const optional<Tensor>& rows, int64_t count, const Tensor& w, const Tensor& offsets, bool transposed, bool fp32) {
     return mm_raw(x, none(rows), count, w, offsets, transposed, fp32);

@@ -10,6 +10,13 @@ largest where ``x.w_e + bias_e`` is, with one price per expert: :func:`transport
 * :func:`combine_rows` - the experts' rows summed back into tokens;
 * :func:`expert_mlp` - the three in a row, as one layer with one backward pass.
 
+And what stands around such a layer:
+
+* :func:`layer_norm` - the norm in front of the router and the experts;
+* :func:`grouped_mm8` - the experts' products in 8-bit floating point, with weights held so (:class:`Blocks8`,
+  :func:`to_blocks8`) or put into 8 bits in every step; :func:`expert_mlp` takes held weights too;
+* :func:`orthogonalize` - the update of the experts' matrices with all singular values brought to about 1.
+
 All of it runs on the current stream of the tensors' device, never waits for the host (group sizes stay on the device, so
 a call can be captured in a CUDA graph), and gives the same bits in every run. Sums are held in fp32. Waits inside the
 products are bounded: should one ever give up, the results it leaves are NaN and the library's health word is set
@@ -18,13 +25,14 @@ counterpart in the reference.
 """
 from __future__ import annotations
 
-from typing import NamedTuple, Optional, Union
+from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
 
 from flash_sinkhorn_b200 import _lib
 
-__all__ = ["Routing", "route_tokens", "grouped_mm", "gated_act", "combine_rows", "expert_mlp", "transport_bias"]
+__all__ = ["Routing", "Blocks8", "route_tokens", "grouped_mm", "grouped_mm8", "to_blocks8", "gated_act", "combine_rows", "expert_mlp",
+           "layer_norm", "orthogonalize", "transport_bias"]
 
 
 class Routing(NamedTuple):
@@ -36,6 +44,16 @@ class Routing(NamedTuple):
     pairs: torch.Tensor  #: ``[T * k]`` int32 pair (``token * k + slot``) of each row, -1 after the last routed one
     rows: torch.Tensor  #: ``[T * k]`` int32 token of each row, -1 after the last routed one
     position: torch.Tensor  #: ``[T, k]`` int32 row of each pair, -1 for a slot without an expert
+
+
+class Blocks8(NamedTuple):
+    """Weights ``[E, N, K]`` in 8-bit floating point, a scale for each block of 128 x 128: ``codes * scales`` stands for them.
+
+    What :func:`to_blocks8` gives, or codes and scales from elsewhere: scales may have any finite value, not powers of two only.
+    """
+
+    codes: torch.Tensor  #: ``[E, N, K]`` float8_e4m3fn; rows a multiple of 16 values apart, or every call copies them
+    scales: torch.Tensor  #: ``[E, ceil(N / 128), ceil(K / 128)]`` float32
 
 
 def _check_routing(routing) -> None:
@@ -76,6 +94,37 @@ def grouped_mm(x: torch.Tensor, weight: torch.Tensor, groups: Union[Routing, tor
     return _lib.torch_binding().grouped_mm(x, weight, groups, None, None, False)
 
 
+def to_blocks8(weight: torch.Tensor) -> Blocks8:
+    """``weight [E, N, K]`` (fp16 or bf16) in 8 bits, for :func:`grouped_mm8` and :func:`expert_mlp`. Carries no gradient.
+
+    The scale of 128 x 128 values is the smallest power of two (from ``2**-126`` on) at which their largest magnitude is at most 448,
+    and each value is rounded to the nearest code, ties to even: off by at most 1/16 of itself, or ``2**-10`` of the scale if
+    that is more. A block with an infinity or a NaN has the scale NaN, and the products that read it are NaN.
+    """
+    return Blocks8(*_lib.torch_binding().to_blocks8(weight))
+
+
+def grouped_mm8(x: torch.Tensor, weight: Union[Blocks8, torch.Tensor], groups: Union[Routing, torch.Tensor], *,
+                gather: bool = False) -> torch.Tensor:
+    """:func:`grouped_mm` in 8-bit floating point: ``out[i] = q(weight[e]) @ q(x[i])``, in the type of x (fp16 or bf16).
+
+    ``x`` is put into 8 bits in every call, blocks of 128 values along its rows with a scale each, as :func:`to_blocks8` does
+    blocks of 128 x 128; so is ``weight`` given as a tensor ``[E, N, K]`` of the type of x (training). A :class:`Blocks8` is taken as it
+    is (serving). ``groups`` and ``gather`` as in :func:`grouped_mm`. Sums are fp32, within blocks of 128 by the tensor core; one rounding.
+
+    Differentiable in x and in a ``weight`` given as a tensor: the roundings to 8 bits count as the identity. The gradient to x is
+    ``q(dy) @ q(weight[e])``, with blocks of 128 along the rows of ``dy`` and the same codes of the weights; that to ``weight`` is
+    the 16-bit product of ``dy`` and ``x`` as they are.
+    """
+    held = isinstance(weight, Blocks8)
+    w, codes, scales = (None, *weight) if held else (weight, None, None)
+    if isinstance(groups, Routing):
+        return _lib.torch_binding().grouped_mm8(x, w, codes, scales, groups.offsets, groups.rows, groups.position, bool(gather))
+    if gather:
+        raise ValueError("gather needs a Routing")
+    return _lib.torch_binding().grouped_mm8(x, w, codes, scales, groups, None, None, False)
+
+
 def gated_act(u: torch.Tensor, routing: Optional[Routing] = None, *, checkpoint: bool = True) -> torch.Tensor:
     """``silu(g) * v`` of ``u = [g | v]`` (``[R, 2 F]`` to ``[R, F]``), times the gate of each row's pair if a routing is given.
 
@@ -104,7 +153,7 @@ def combine_rows(o: torch.Tensor, routing: Routing, *, weighted: bool = True) ->
     return _lib.torch_binding().combine_rows(o, routing.gates, routing.pairs, routing.position, bool(weighted))
 
 
-def expert_mlp(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, routing: Routing, *,
+def expert_mlp(x: torch.Tensor, w_in: Union[torch.Tensor, Blocks8], w_out: Union[torch.Tensor, Blocks8], routing: Routing, *,
                checkpoint: bool = True) -> torch.Tensor:
     """A layer of gated experts: ``y[t] = sum_s gates[t, s] * w_out[e] @ (silu(g) * v)``, ``[g | v] = w_in[e] @ x[t]``.
 
@@ -114,10 +163,44 @@ def expert_mlp(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, routing
     them. The operators' results between x and y are of the type of x (a token's rows of the second product are rounded,
     then summed in fp32 and rounded again), as are the gradients between dy and dx, but for the rows that are summed to
     dx, which are fp32.
+
+    With both weights given as :class:`Blocks8` the products are those of :func:`grouped_mm8`; differentiable in ``x`` and
+    ``routing.gates`` then.
     """
     _check_routing(routing)
+    if isinstance(w_in, Blocks8) or isinstance(w_out, Blocks8):
+        if not (isinstance(w_in, Blocks8) and isinstance(w_out, Blocks8)):
+            raise ValueError("w_in and w_out must both be Blocks8, or neither")
+        h = gated_act(grouped_mm8(x, w_in, routing, gather=True), routing, checkpoint=checkpoint)
+        return combine_rows(grouped_mm8(h, w_out, routing), routing, weighted=False)
     r = routing
     return _lib.torch_binding().expert_mlp(x, w_in, w_out, r.gates, r.offsets, r.pairs, r.rows, r.position, bool(checkpoint))
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, *,
+               eps: float = 1e-5) -> torch.Tensor:
+    """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension of ``x [..., F]`` (fp32, fp16 or bf16), in its type.
+
+    ``weight`` and ``bias`` ``[F]``: float32 or the type of x, both the same; either may be left out. Differentiable in all three;
+    mean and deviation stay for the backward pass, and the sums over the rows for ``weight`` and ``bias`` are fp32 in a fixed order.
+    """
+    return _lib.torch_binding().layer_norm(x, weight, bias, float(eps))
+
+
+def orthogonalize(g: torch.Tensor, *, steps: int = 5, coefficients: Tuple[float, float, float] = (3.4445, -4.7750, 2.0315),
+                  eps: float = 1e-7, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """Brings the singular values of each matrix of ``g [..., N, K]`` to about 1 and leaves its singular vectors, for updates.
+
+    ``X = g / (|g| + eps)`` with the Frobenius norm, then ``steps`` times ``X <- a X + b (X X^T) X + c (X X^T)^2 X`` with
+    ``coefficients = (a, b, c)``; the default ones bring values from 0.003 on to between 0.7 and 1.2 in five steps. ``g`` is fp32, fp16 or
+    bf16, the result of ``dtype`` (fp16 or bf16) and carries no gradient. Products are of fp16 operands with fp32 sums, the part
+    ``a X`` is of 22 bits: the result is off by 0.1 to 0.3 % of its norm (a single row: up to 2 %) besides its rounding. Coefficients have to keep the
+    singular values at 2 or less. A matrix with an infinity or a NaN gives NaN, zeros give zeros.
+    """
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"dtype must be torch.float16 or torch.bfloat16, got {dtype}")
+    a, b, c = (float(v) for v in coefficients)
+    return _lib.torch_binding().orthogonalize(g.detach(), int(steps), a, b, c, float(eps), dtype == torch.bfloat16)
 
 
 def transport_bias(x: torch.Tensor, router: torch.Tensor, *, eps: float = 0.1, n_iters: int = 20,

@@ -547,6 +547,52 @@ int fs_combine(const void* o, int type, long long ldo, int M, int T, int k, int 
 int fs_combine_grad(const void* o, int type, long long ldo, int T, int k, int D, const float* gates, const int* position,
                     const int* pairs, const void* dy, long long lddy, void* d_o, float* dgates, void* stream);
 
+/* What stands around routed experts; matrices, types and sums as above.
+ *
+ * Layer norm of `rows` rows of F values: y = (x - mean) rstd w + b, rstd = 1 / sqrt(var + eps). w and b (either may be null: 1 and
+ * 0) are of the type of x or FS_TYPE_F32, densely packed. y is densely packed; mean and rstd [rows] (both or neither) are what
+ * the gradient takes. */
+int fs_layer_norm(const void* x, int type, long long ldx, int rows, int F, const void* w, const void* b, int w_type, float eps,
+                  void* y, float* mean, float* rstd, void* stream);
+
+/* Scratch of fs_layer_norm_grad (needed for dw or db). */
+size_t fs_layer_norm_grad_bytes(int rows, int F);
+
+/* Its gradients dx [rows, F], densely packed, dw and db [F] of w_type; any of them may be null. */
+int fs_layer_norm_grad(const void* x, int type, long long ldx, int rows, int F, const void* w, int w_type, const float* mean,
+                       const float* rstd, const void* dy, long long lddy, void* dx, void* dw, void* db, void* ws, size_t ws_bytes,
+                       void* stream);
+
+/* Weights [E, N, K] in 8-bit floating point (4 bits of exponent, 3 of mantissa): w[e, n, k] becomes
+ * codes[e * c_expert + n * c_row + k] times scales[e][n / 128][k / 128], rounded to nearest, ties to even. A scale is the smallest
+ * power of two (from 2^-126 on) at which the largest magnitude of its 128 x 128 values becomes at most 448; NaN for a block
+ * with an infinity or a NaN. Codes past K up to a multiple of 16 are zeros. c_row and c_expert are multiples of 16, codes aligned to 16 bytes.
+ * scales: densely packed, E x ceil(N / 128) x ceil(K / 128). */
+int fs_weights8(const void* w, int type, long long w_expert, long long w_row, int E, int N, int K, uint8_t* codes,
+                long long c_expert, long long c_row, float* scales, void* stream);
+
+/* Scratch of fs_grouped_mm8 (0: none), aligned to 256 bytes. */
+size_t fs_grouped_mm8_bytes(int R, int K, int transposed);
+
+/* Products grouped by expert in 8 bits: out[i, :] = W_e q(x[row(i), :]) for the rows i of expert e, zeros for the rows of none; q puts
+ * blocks of 128 values along a row into 8 bits as fs_weights8 does blocks of 128 x 128. W_e is given by codes w, N x K (transposed: K x N,
+ * and its transpose is multiplied) with rows w_row and experts w_expert apart (multiples of 16, w aligned to 16 bytes) and
+ * scales as fs_weights8 leaves them, of any finite value. Each block of 128 products is summed by the tensor core, then scaled and added in fp32.
+ * rows, M, offsets, out and waits as in fs_grouped_mm. */
+int fs_grouped_mm8(const void* x, int type, long long ldx, int M, const int* rows, int R, const uint8_t* w, long long w_expert,
+                   long long w_row, const float* scales, int E, int N, int K, int transposed, const int* offsets, void* out,
+                   int out_type, long long ldo, void* ws, size_t ws_bytes, void* stream);
+
+/* Scratch of fs_orthogonalize, aligned to 256 bytes. */
+size_t fs_orthogonalize_bytes(int batch, int rows, int cols);
+
+/* For each matrix G of a stack (rows g_row, matrices g_matrix values apart; at most 65536 x 65536): X = G / (|G| + eps), then `steps` times
+ * X <- a X + (b A + c A A) X with A = X X^T (a tall G: of its transpose). out: densely packed, FS_TYPE_F16 or FS_TYPE_BF16. Operands are
+ * fp16, X a sum of two of them. Values of X stay below 255 and those of b A + c A A below 63 in magnitude, or become infinite. Waits as in
+ * fs_grouped_mm. */
+int fs_orthogonalize(const void* g, int type, long long g_matrix, long long g_row, int batch, int rows, int cols, int steps,
+                     float a, float b, float c, float eps, void* out, int out_type, void* ws, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
