@@ -70,25 +70,44 @@ __device__ __forceinline__ uint2 codes_of(const float (&v)[8], float inverse) {
 }
 
 // Rows x[rows[i]] of M rows of K values (zeros for numbers outside; rows null: row i) to codes [R, ldc] and scales [ceil(K / 128)][R]. Sixteen
-// lanes take a block of 128 values of a row. ldc is a multiple of 16; codes past K are zeros.
+// lanes take a block of 128 values of a row, a CTA 32 rows of `span` blocks, so that 32 rows' scales are written side by side. ldc is a
+// multiple of 16; codes past K are zeros. Bound by memory: four blocks of every sixteen lanes are under way at once.
+constexpr int kRows8 = 32, kSpan8 = 64;
 template <typename T>
-__global__ void __launch_bounds__(256) rows8_kernel(const T* x, long long ldx, int M, const int* rows, int R, int K, uint8_t* codes, long long ldc,
+__global__ void __launch_bounds__(256) rows8_kernel(const T* x, long long ldx, int M, const int* rows, int R, int K, int span, uint8_t* codes, long long ldc,
                                                     float* scales, bool vec) {
-  const int lane = threadIdx.x & 15, per_row = (K + kBlock8 - 1) / kBlock8;
-  const long long unit = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 4;
-  const long long i = unit / per_row;
-  const bool in = i < R;
-  const int b = (int)(unit - i * per_row), c = b * kBlock8 + lane * 8, t = !in ? -1 : rows ? __ldg(rows + i) : (int)i;
-  float v[8];
-  eight(x + (long long)t * ldx, (unsigned)t < (unsigned)M ? c : K, K, vec, v);
-  uint32_t top = top_of(v);
+  __shared__ int from[kRows8];
+  __shared__ float found[kSpan8][kRows8];
+  constexpr int kDeep = 4;
+  const int lane = threadIdx.x & 15, group = threadIdx.x >> 4, b0 = blockIdx.y * span;
+  const int blocks = min(span, (K + kBlock8 - 1) / kBlock8 - b0);
+  const long long i0 = (long long)blockIdx.x * kRows8;
+  const int count = (int)min((long long)kRows8, R - i0);
+  if (threadIdx.x < kRows8) from[threadIdx.x] = threadIdx.x >= count ? -1 : rows ? __ldg(rows + i0 + threadIdx.x) : (int)(i0 + threadIdx.x);
+  __syncthreads();
+  for (int u0 = group; u0 < blocks * kRows8; u0 += 16 * kDeep) {
+    float v[kDeep][8];
 #pragma unroll
-  for (int o = 8; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (!in) return;
-  float scale, inverse;
-  scale_of(top, scale, inverse);
-  if (c < ldc) *reinterpret_cast<uint2*>(codes + i * ldc + c) = codes_of(v, inverse);
-  if (lane == 0) scales[(long long)b * R + i] = scale;
+    for (int d = 0; d < kDeep; ++d) {
+      const int u = u0 + 16 * d, r = u & (kRows8 - 1), t = from[r], c = (b0 + (u / kRows8)) * kBlock8 + lane * 8;
+      eight(x + (long long)t * ldx, u < blocks * kRows8 && (unsigned)t < (unsigned)M ? c : K, K, vec, v[d]);
+    }
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d) {
+      const int u = u0 + 16 * d, r = u & (kRows8 - 1), b = u / kRows8, c = (b0 + b) * kBlock8 + lane * 8;
+      uint32_t top = top_of(v[d]);
+#pragma unroll
+      for (int o = 8; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffu << (threadIdx.x & 16), top, o));
+      if (b >= blocks || r >= count) continue;
+      float scale, inverse;
+      scale_of(top, scale, inverse);
+      if (c < ldc) *reinterpret_cast<uint2*>(codes + (i0 + r) * ldc + c) = codes_of(v[d], inverse);
+      if (lane == 0) found[b][r] = scale;
+    }
+  }
+  __syncthreads();
+  for (int u = threadIdx.x; u < blocks * kRows8; u += 256)
+    if ((u & (kRows8 - 1)) < count) scales[(long long)(b0 + u / kRows8) * R + i0 + (u & (kRows8 - 1))] = found[u / kRows8][u & (kRows8 - 1)];
 }
 
 // Weights w [E, N, K] to codes (rows c_row, matrices c_expert apart) and scales [E][ceil(N / 128)][ceil(K / 128)]: a CTA to a block of
@@ -129,9 +148,11 @@ __global__ void __launch_bounds__(256) weights8_kernel(const T* w, long long w_e
 }
 
 // ------------------------------------------------------------------ products
-constexpr int kSumWarps = 8, kFetchWarp = 8, kIssueWarp = 9, kThreads8 = 32 * 10;
+// Warps: a warpgroup for loads and products (two of its warps idle), then two that sum. With 256 columns the sums take
+// more than the 168 registers that 384 threads have each: 40 for the first group, 232 for the others (128 x 40 + 256 x 232 = 384 x 168).
+constexpr int kSumWarps = 8, kFetchWarp = 0, kIssueWarp = 1, kGroupWarp = 2, kFirstSum = 4, kThreads8 = 32 * (kFirstSum + kSumWarps);
 constexpr uint32_t kTileA = 128 * 128;
-constexpr int kStage8 = 2048 * kSumWarps;  // staging of results
+constexpr int kStage8 = 4096 * kSumWarps;  // staging of results
 
 struct Mm8Args {
   const int* offsets;
@@ -143,6 +164,7 @@ struct Mm8Args {
   void* out;
   long long ldo;
   int out_type, out_bytes;  // bytes of a store: 16, 4 or 2
+  bool boxes;               // whole blocks of 32 rows are written by TMA
   int nstage;
   long long limit;
 };
@@ -197,7 +219,7 @@ __device__ __forceinline__ uint32_t two16(u64 v, int type) {
 // MN: w contiguous along N (the transposed product). Single CTAs fetch rows in boxes of 32, as many as the tile has.
 template <bool MN, int CG, int BN>
 __global__ void __launch_bounds__(kThreads8, 1)
-mm8_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB) {
+mm8_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB, const __grid_constant__ CUtensorMap mapC) {
   constexpr int BNC = BN / CG, kBufs = BN == 256 ? 2 : 4;
   constexpr uint32_t kTileB = BNC * 128, kStage = kTileA + kTileB, kColumns = BN * kBufs;
   constexpr int kBoxA = CG == 2 ? 128 : 32;
@@ -216,7 +238,7 @@ mm8_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapA, const __gr
   const int rank = CG == 2 ? (int)cta_rank() : 0;
   const int first = blockIdx.x / CG, stride = gridDim.x / CG;
 
-  if (warp == 0) {
+  if (warp == kGroupWarp) {
     read_groups<true>(a.offsets, a.E, a.R, gs, ts, (a.N + BN - 1) / BN, 128 * CG);
   } else if (warp == kFetchWarp && lane == 0) {
     for (int s = 0; s < a.nstage; ++s) {
@@ -243,9 +265,10 @@ mm8_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapA, const __gr
   const int total = tiles.total();
   int issued = 0;  // stages that this CTA's loading thread has started
 
-  if (warp == kFetchWarp) {
+  if (warp < kFirstSum) {
+    if (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     // ===================== loads =====================
-    if (elect_one()) {
+    if (warp == kFetchWarp && elect_one()) {
       int s = 0;
       uint32_t ph = 0;
       bool ok = true;
@@ -275,9 +298,8 @@ mm8_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapA, const __gr
         }
       }
     }
-  } else if (warp == kIssueWarp) {
     // ===================== products =====================
-    if (rank == 0 && elect_one()) {
+    if (warp == kIssueWarp && rank == 0 && elect_one()) {
       // fp32 sums, both operands e4m3 (0)
       constexpr uint32_t idesc = (1u << 4) | ((MN ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(128 * CG >> 4) << 24);
       // a step of 32 contraction values: 32 bytes on, or 32 rows of 128 bytes; MN: the next 128 features one tile on
@@ -315,13 +337,25 @@ mm8_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapA, const __gr
     }
   } else {
     // ===================== sums and results =====================
+    if (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     // Two warps to a quarter of the TMEM lanes (rows), with one half of the features each.
     constexpr int kMine = BN / 2;
-    const int q = warp & 3, side = warp >> 2;
-    const uint32_t stage = smem_u32(staging + 2048 * warp);
+    const int q = warp & 3, side = (warp - kFirstSum) >> 2;
+    const uint32_t stage = smem_u32(staging + 4096 * (warp - kFirstSum));
     int buf = 0;
     uint32_t acc_ph = 0;
     bool lost = false;  // a wait of this CTA gave up: NaN from here on
+    auto release = [&]() {  // the staging tile, by the copy that reads it
+      if (a.boxes) {
+        if (lane == 0) bulk_read();
+        __syncwarp();
+      }
+    };
+    auto send = [&](int n, int row) {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) store_box(&mapC, n, row, stage);
+    };
     for (int it = first; it < total; it += stride) {
       const Tile8 t = tiles.at(it);
       const int row0 = t.lo + rank * 128 + q * 32, n0 = t.n0 + side * kMine;
@@ -341,24 +375,29 @@ mm8_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapA, const __gr
           x_next = __ldg(sx + (long long)(kb + 1) * a.R);
           w_next = __ldg(sw + (long long)(kb + 1) * a.sw_k);
         }
-        lost = !__all_sync(0xffffffffu, wait_blocks(bar(ACC_FULL + buf), acc_ph, abort_flag, 4, a.limit));
+        lost = !__all_sync(0xffffffffu, wait_close(bar(ACC_FULL + buf), acc_ph, abort_flag, a.limit));
         if (lost) break;
         tc_fence_after();
         const u64 f2 = pk(f, f);
+        const uint32_t acc = tmem + buf * BN + side * kMine + ((uint32_t)(q * 32) << 16);
+        uint32_t r[2][32];  // 32 columns are on their way while the ones before them are added
+        tmem_ld32_nowait(acc, r[0]);
 #pragma unroll
         for (int j = 0; j < kMine / 32; ++j) {
-          uint32_t r[32];
-          tmem_ld32_nowait(tmem + buf * BN + side * kMine + 32 * j + ((uint32_t)(q * 32) << 16), r);
-          tmem_ld_wait(r);
+          tmem_ld_wait(r[j & 1]);
+          if (j + 1 < kMine / 32) {
+            tmem_ld32_nowait(acc + 32 * (j + 1), r[(j + 1) & 1]);
+          } else {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              if (CG == 2) arrive_cluster(in_leader(bar(ACC_EMPTY + buf)));
+              else mbar_arrive(bar(ACC_EMPTY + buf));
+            }
+          }
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            sum[16 * j + i] = fma2(pk(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), f2, sum[16 * j + i]);
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          if (CG == 2) arrive_cluster(in_leader(bar(ACC_EMPTY + buf)));
-          else mbar_arrive(bar(ACC_EMPTY + buf));
+            sum[16 * j + i] = fma2(pk(__uint_as_float(r[j & 1][2 * i]), __uint_as_float(r[j & 1][2 * i + 1])), f2, sum[16 * j + i]);
         }
         if (++buf == kBufs) {
           buf = 0;
@@ -374,35 +413,49 @@ mm8_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapA, const __gr
       if (rows <= 0) continue;
       const int width = a.out_type == FS_TYPE_F32 ? 4 : 2;
       char* out = static_cast<char*>(a.out) + (long long)row0 * a.ldo * width;
+      const bool whole = a.boxes && rows >= 32;  // the rows behind the last one are another tile's
+      // 128 bytes of each row at a time
+      const int at16 = kMine < 64 ? kMine : 64;
+      if (a.out_type != FS_TYPE_F32) {
 #pragma unroll
-      for (int j = 0; j < kMine / 32; ++j) {
-        const int n = n0 + 32 * j;
-        if (n >= a.N) break;
-        if (a.out_type != FS_TYPE_F32) {
+        for (int j = 0; j < kMine; j += at16) {
+          if (n0 + j >= a.N) break;
+          release();
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            stage16(staged_row(stage, lane, c), two16(sum[16 * j + 4 * c], a.out_type), two16(sum[16 * j + 4 * c + 1], a.out_type),
-                    two16(sum[16 * j + 4 * c + 2], a.out_type), two16(sum[16 * j + 4 * c + 3], a.out_type));
-          __syncwarp();
-          write_rows(out + 2ll * n, a.ldo * 2, rows, 2 * (a.N - n), a.out_bytes, stage, lane);
-          __syncwarp();
-        } else {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              float v[4];
-              upk(sum[16 * j + 8 * h + 2 * c], v[0], v[1]);
-              upk(sum[16 * j + 8 * h + 2 * c + 1], v[2], v[3]);
-              stage16(staged_row(stage, lane, c), __float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-            }
+          for (int c = 0; c < at16 / 8; ++c)
+            stage16(staged_row(stage, lane, c), two16(sum[j / 2 + 4 * c], a.out_type), two16(sum[j / 2 + 4 * c + 1], a.out_type),
+                    two16(sum[j / 2 + 4 * c + 2], a.out_type), two16(sum[j / 2 + 4 * c + 3], a.out_type));
+          if (whole) {
+            send(n0 + j, row0);
+          } else {
             __syncwarp();
-            write_rows(out + 4ll * (n + 16 * h), a.ldo * 4, rows, 4 * (a.N - n - 16 * h), a.out_bytes, stage, lane);
+            write_rows(out + 2ll * (n0 + j), a.ldo * 2, rows, 2 * min(a.N - n0 - j, at16), a.out_bytes, stage, lane);
+            __syncwarp();
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < kMine; j += 32) {
+          if (n0 + j >= a.N) break;
+          release();
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            float v[4];
+            upk(sum[j / 2 + 2 * c], v[0], v[1]);
+            upk(sum[j / 2 + 2 * c + 1], v[2], v[3]);
+            stage16(staged_row(stage, lane, c), __float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+          }
+          if (whole) {
+            send(n0 + j, row0);
+          } else {
+            __syncwarp();
+            write_rows(out + 4ll * (n0 + j), a.ldo * 4, rows, 4 * min(a.N - n0 - j, 32), a.out_bytes, stage, lane);
             __syncwarp();
           }
         }
       }
     }
+    if (a.boxes && lane == 0) bulk_done();
   }
   __syncwarp();
   tc_fence_before();
@@ -557,13 +610,27 @@ bool encode8(CUtensorMap* map, const void* base, int dims, const long long (&siz
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Results of R rows; boxes of 32 rows of 128 bytes.
+bool encode_out(CUtensorMap* map, int type, void* base, long long cols, long long rows, long long ld) {
+  const int width = type_bytes(type);
+  const cuuint64_t sizes[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)(ld * width)};
+  const cuuint32_t box[2] = {(cuuint32_t)(128 / width), 32}, ones[2] = {1, 1};
+  const auto fn = encoder();
+  return fn && fn(map, type == FS_TYPE_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == FS_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                  2, base, sizes, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <bool MN, int CG, int BN>
 int launch_mm8(Mm8Args a, const uint8_t* x, long long ldx, const uint8_t* w, long long w_expert, long long w_row, cudaStream_t st) {
-  CUtensorMap mapA = {}, mapB = {};
+  CUtensorMap mapA = {}, mapB = {}, mapC = {};
+  const int width = type_bytes(a.out_type);
+  a.boxes = BN >= 128 && aligned(a.out, 16) && a.ldo * width % 16 == 0;  // a warp has 128 bytes of a row
   // w's own rows and columns: K and N change places in the transposed product
   const long long w_cols = MN ? a.N : a.K, w_rows = MN ? a.K : a.N;
   if (!encode8(&mapA, x, 2, {a.K, a.R, 1}, {ldx, 0}, CG == 2 ? 128 : 32) ||
-      !encode8(&mapB, w, 3, {w_cols, w_rows, a.E}, {w_row, w_expert ? w_expert : w_row}, MN ? 128 : BN / CG))
+      !encode8(&mapB, w, 3, {w_cols, w_rows, a.E}, {w_row, w_expert ? w_expert : w_row}, MN ? 128 : BN / CG) ||
+      (a.boxes && !encode_out(&mapC, a.out_type, a.out, a.N, a.R, a.ldo)))
     return report_error(FS_ERR_CUDA, "cuTensorMapEncodeTiled failed");
   constexpr size_t kStage = kTileA + BN / CG * 128;
   const size_t fixed = 1024 + kStage8 + 8 * (2 * 12 + 9) + 8 + 8 * ((size_t)a.E + 2);
@@ -598,7 +665,7 @@ int launch_mm8(Mm8Args a, const uint8_t* x, long long ldx, const uint8_t* w, lon
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   g_mm8_launched.store(true, std::memory_order_relaxed);
-  e = cudaLaunchKernelEx(&cfg, kernel, a, mapA, mapB);
+  e = cudaLaunchKernelEx(&cfg, kernel, a, mapA, mapB, mapC);
   if (e != cudaSuccess) return report_error(FS_ERR_CUDA, cudaGetErrorString(e));
   count_launches(1);
   return FS_OK;
@@ -606,10 +673,11 @@ int launch_mm8(Mm8Args a, const uint8_t* x, long long ldx, const uint8_t* w, lon
 
 template <typename T>
 int launch_rows8(const void* x, long long ldx, int M, const int* rows, int R, int K, uint8_t* codes, long long ldc, float* scales, cudaStream_t st) {
-  const long long units = (long long)R * ((K + kBlock8 - 1) / kBlock8), grid = (units + 15) / 16;
-  if (grid > 0x7fffffffll) return report_error(FS_ERR_UNSUPPORTED, "too many blocks of 128 values");
+  const int blocks = (K + kBlock8 - 1) / kBlock8, over = (R + kRows8 - 1) / kRows8;
+  int span = kSpan8;
+  while (span > 1 && (long long)over * ((blocks + span - 1) / span) < 4 * 148) span /= 2;
   const bool vec = aligned(x, 16) && ldx % 8 == 0 && K % 8 == 0;
-  rows8_kernel<T><<<(unsigned)grid, 256, 0, st>>>(static_cast<const T*>(x), ldx, M, rows, R, K, codes, ldc, scales, vec);
+  rows8_kernel<T><<<dim3(over, (blocks + span - 1) / span), 256, 0, st>>>(static_cast<const T*>(x), ldx, M, rows, R, K, span, codes, ldc, scales, vec);
   return launched(1);
 }
 template <typename T>

@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(256) begin_kernel(const T* g, long long g_matr
 enum Product { GRAM, SQUARE, APPLY, LAST };  // LAST: APPLY to the result
 
 constexpr int kWriteWarps = 8, kGetWarp = 8, kMulWarp = 9, kThreadsO = 32 * 10;
-constexpr int kStageO = 2048 * kWriteWarps;
+constexpr int kStageO = 4096 * kWriteWarps;
 
 struct OrthoArgs {
   int batch, n, k;          // X is n x k, A and P are n x n
@@ -269,7 +269,7 @@ ortho_kernel(const OrthoArgs a, const __grid_constant__ CUtensorMap mapA, const 
     // ===================== results =====================
     // Two warps to a quarter of the TMEM lanes (rows), with every other 32 columns each.
     const int q = warp & 3, side = warp >> 2;
-    const uint32_t stage = smem_u32(staging + 2048 * warp);
+    const uint32_t stage = smem_u32(staging + 4096 * warp);
     int t = 0;
     bool lost = false;  // a wait of this CTA gave up: NaN from here on
     for (long long it = first; it < total; it += stride, ++t) {
@@ -333,7 +333,7 @@ ortho_kernel(const OrthoArgs a, const __grid_constant__ CUtensorMap mapA, const 
               stage16(staged_row(stage, lane, i), w[0], w[1], w[2], w[3]);
             }
             __syncwarp();
-            write_rows(reinterpret_cast<char*>(out + (long long)row0 * a.k + col), 2ll * a.k, rows, 2 * (a.k - col), a.out_bytes, stage, lane);
+            write_rows(reinterpret_cast<char*>(out + (long long)row0 * a.k + col), 2ll * a.k, rows, min(2 * (a.k - col), 64), a.out_bytes, stage, lane);
             __syncwarp();
           }
         } else {
@@ -345,7 +345,7 @@ ortho_kernel(const OrthoArgs a, const __grid_constant__ CUtensorMap mapA, const 
 #pragma unroll
           for (int i = 0; i < 4; ++i) stage16(staged_row(stage, lane, i), h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
           __syncwarp();
-          write_rows(reinterpret_cast<char*>(out), 2 * ld, rows, 2 * (width - col), 16, stage, lane);  // rows are padded to 16 bytes
+          write_rows(reinterpret_cast<char*>(out), 2 * ld, rows, min(2 * (width - col), 64), 16, stage, lane);  // rows are padded to 16 bytes
           __syncwarp();
           if (FORM == APPLY) {
 #pragma unroll
@@ -357,7 +357,7 @@ ortho_kernel(const OrthoArgs a, const __grid_constant__ CUtensorMap mapA, const 
 #pragma unroll
             for (int i = 0; i < 4; ++i) stage16(staged_row(stage, lane, i), h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
             __syncwarp();
-            write_rows(reinterpret_cast<char*>(a.lo_out + ((long long)b * a.n + row0) * ld + col), 2 * ld, rows, 2 * (width - col), 16, stage, lane);
+            write_rows(reinterpret_cast<char*>(a.lo_out + ((long long)b * a.n + row0) * ld + col), 2 * ld, rows, min(2 * (width - col), 64), 16, stage, lane);
             __syncwarp();
           } else if (n0 + BN <= m0 && in) {  // and the same above the diagonal
             uint16_t* mirror = reinterpret_cast<uint16_t*>(a.sym) + ((long long)b * a.n + col) * ld + row;

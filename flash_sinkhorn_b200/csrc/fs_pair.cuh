@@ -71,6 +71,21 @@ __device__ __forceinline__ bool wait_blocks(uint32_t bar, uint32_t parity, volat
   }
   return true;
 }
+// For a wait that ends within a microsecond, many times in a tile: without parking the thread.
+__device__ __forceinline__ bool wait_close(uint32_t bar, uint32_t parity, volatile int* abort_flag, long long limit) {
+  if (limit == 0) *abort_flag = 1;  // without a look, for tests
+  if (limit == 0) return false;
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity)) {
+    if (*abort_flag) return false;
+    if (clock64() - t0 > limit) {
+      *abort_flag = 1;
+      return false;
+    }
+  }
+  return true;
+}
 template <int CG>
 __device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
   if (CG == 2)
@@ -172,38 +187,47 @@ __device__ void read_groups(const int* offsets, int E, int R, int* gs, int* ts, 
   if (TILES && lane == 0) ts[0] = 0;
 }
 
-// 16-byte chunk `chunk` of row `row` of a warp's staging tile of 32 rows of 64 bytes.
-__device__ __forceinline__ uint32_t staged_row(uint32_t base, int row, int chunk) { return base + row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4); }
-// rows x bytes (at most 32 x 64) of the staging tile to out, rows ld bytes apart, by stores of `vec` bytes.
+// 16-byte chunk `chunk` of row `row` of a warp's staging tile of 32 rows of 128 bytes: neither side meets bank conflicts.
+__device__ __forceinline__ uint32_t staged_row(uint32_t base, int row, int chunk) { return base + row * 128 + ((chunk ^ (row & 7)) << 4); }
+// rows x bytes (at most 32 x 128) of the staging tile to out, rows ld bytes apart, by stores of `vec` bytes.
 __device__ __forceinline__ void write_rows(char* out, long long ld, int rows, int bytes, int vec, uint32_t base, int lane) {
   if (vec == 16) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = 8 * i + (lane >> 2), c = lane & 3;
+    for (int i = 0; i < 8; ++i) {
+      const int r = 4 * i + (lane >> 3), c = lane & 7;
       uint4 v;
       asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(staged_row(base, r, c)));
       if (r < rows && 16 * c < bytes) *reinterpret_cast<uint4*>(out + r * ld + 16 * c) = v;
     }
   } else if (vec == 4) {
 #pragma unroll 4
-    for (int i = 0; i < 16; ++i) {
-      const int r = 2 * i + (lane >> 4), c = 4 * (lane & 15);
+    for (int r = 0; r < 32; ++r) {
       uint32_t v;
-      asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(staged_row(base, r, c >> 4) + (c & 15)));
-      if (r < rows && c < bytes) *reinterpret_cast<uint32_t*>(out + r * ld + c) = v;
+      asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(staged_row(base, r, lane >> 2) + (lane & 3) * 4));
+      if (r < rows && 4 * lane < bytes) *reinterpret_cast<uint32_t*>(out + r * ld + 4 * lane) = v;
     }
   } else {
 #pragma unroll 4
-    for (int r = 0; r < 32; ++r) {
+    for (int i = 0; i < 64; ++i) {
+      const int r = i >> 1, c = 2 * lane + 64 * (i & 1);
       uint16_t v;
-      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(staged_row(base, r, lane >> 3) + (lane & 7) * 2));
-      if (r < rows && 2 * lane < bytes) *reinterpret_cast<uint16_t*>(out + r * ld + 2 * lane) = v;
+      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(staged_row(base, r, c >> 4) + (c & 15)));
+      if (r < rows && c < bytes) *reinterpret_cast<uint16_t*>(out + r * ld + c) = v;
     }
   }
 }
 __device__ __forceinline__ void stage16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+
+// A warp's staging tile to the box of an output at (c0, c1), by TMA (the tile is laid out as its 128-byte swizzle has it). One lane; the tile
+// is free again after bulk_read(), everything is written after bulk_done().
+__device__ __forceinline__ void store_box(const CUtensorMap* map, int c0, int c1, uint32_t tile) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(tile), "r"(c0), "r"(c1) : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void bulk_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 PFN_cuTensorMapEncodeTiled_v12000 encoder() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
