@@ -69,82 +69,114 @@ __device__ __forceinline__ uint2 codes_of(const float (&v)[8], float inverse) {
                     four_codes(v[4] * inverse, v[5] * inverse, v[6] * inverse, v[7] * inverse));
 }
 
-// Rows x[rows[i]] of M rows of K values (zeros for numbers outside; rows null: row i) to codes [R, ldc] and scales [ceil(K / 128)][R]. Sixteen
-// lanes take a block of 128 values of a row, a CTA 32 rows of `span` blocks, so that 32 rows' scales are written side by side. ldc is a
-// multiple of 16; codes past K are zeros. Bound by memory: four blocks of every sixteen lanes are under way at once.
-constexpr int kRows8 = 32, kSpan8 = 64;
+// Sixteen values from column c on of a row of K as they are in memory, zeros past its end. VEC: rows aligned to 16 bytes, K a multiple of 8.
+template <bool VEC, typename T>
+__device__ __forceinline__ void sixteen(const T* row, int c, int K, uint32_t (&w)[8]) {
+  if (VEC) {
+    const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+    const uint4 p = c < K ? __ldg(reinterpret_cast<const uint4*>(row + c)) : none, q = c + 8 < K ? __ldg(reinterpret_cast<const uint4*>(row + c) + 1) : none;
+    w[0] = p.x; w[1] = p.y; w[2] = p.z; w[3] = p.w;
+    w[4] = q.x; w[5] = q.y; w[6] = q.z; w[7] = q.w;
+  } else {
+    const uint16_t* v = reinterpret_cast<const uint16_t*>(row);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t lo = c + 2 * j < K ? __ldg(v + c + 2 * j) : 0u, hi = c + 2 * j + 1 < K ? __ldg(v + c + 2 * j + 1) : 0u;
+      w[j] = lo | hi << 16;
+    }
+  }
+}
+// Magnitudes of 16-bit floating-point values are ordered as whole numbers: largest ones of both halves.
+__device__ __forceinline__ uint32_t top_pair(const uint32_t (&w)[8]) {
+  uint32_t m = 0u;
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) m = __vimax3_u16x2(m, w[j] & 0x7fff7fffu, w[j + 1] & 0x7fff7fffu);
+  return m;
+}
+// The larger half of a pair as float bits.
+__device__ __forceinline__ uint32_t top_bits(uint32_t m, __nv_bfloat16) { return max(m << 16, m & 0xffff0000u); }
+__device__ __forceinline__ uint32_t top_bits(uint32_t m, __half) {
+  return __float_as_uint(__half2float(__ushort_as_half((unsigned short)max(m & 0xffffu, m >> 16))));
+}
 template <typename T>
+__device__ __forceinline__ uint4 sixteen_codes(const uint32_t (&w)[8], float inverse) {
+  uint32_t q[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float a, b, c, d;
+    two_f32(w[2 * j], a, b, T());
+    two_f32(w[2 * j + 1], c, d, T());
+    q[j] = four_codes(a * inverse, b * inverse, c * inverse, d * inverse);
+  }
+  return inverse == 0.f ? make_uint4(0u, 0u, 0u, 0u) : make_uint4(q[0], q[1], q[2], q[3]);
+}
+
+// Rows x[rows[i]] of M rows of K values (zeros for numbers outside; rows null: row i) to codes [R, ldc] and scales [ceil(K / 128)][R]. Eight lanes
+// take a row, sixteen values of a block each, a CTA 32 rows of `span` blocks, so that 32 rows' scales are written side by side. ldc is a
+// multiple of 16; codes past K are zeros. Instructions count as much as bytes: magnitudes are compared in pairs, as whole numbers.
+constexpr int kRows8 = 32, kSpan8 = 64;
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) rows8_kernel(const T* x, long long ldx, int M, const int* rows, int R, int K, int span, uint8_t* codes, long long ldc,
-                                                    float* scales, bool vec) {
-  __shared__ int from[kRows8];
+                                                    float* scales) {
   __shared__ float found[kSpan8][kRows8];
   constexpr int kDeep = 4;
-  const int lane = threadIdx.x & 15, group = threadIdx.x >> 4, b0 = blockIdx.y * span;
+  const int lane = threadIdx.x & 7, r = threadIdx.x >> 3, b0 = blockIdx.y * span;
   const int blocks = min(span, (K + kBlock8 - 1) / kBlock8 - b0);
-  const long long i0 = (long long)blockIdx.x * kRows8;
-  const int count = (int)min((long long)kRows8, R - i0);
-  if (threadIdx.x < kRows8) from[threadIdx.x] = threadIdx.x >= count ? -1 : rows ? __ldg(rows + i0 + threadIdx.x) : (int)(i0 + threadIdx.x);
-  __syncthreads();
-  for (int u0 = group; u0 < blocks * kRows8; u0 += 16 * kDeep) {
-    float v[kDeep][8];
+  const long long i0 = (long long)blockIdx.x * kRows8, i = i0 + r;
+  const int t = i >= R ? -1 : rows ? __ldg(rows + i) : (int)i;
+  const T* row = x + (long long)t * ldx;
+  const int end = (unsigned)t < (unsigned)M ? K : 0;
+  uint8_t* out = codes + i * ldc;
+  for (int j = 0; j < blocks; j += kDeep) {
+    uint32_t w[kDeep][8];
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d) sixteen<VEC>(row, (b0 + j + d) * kBlock8 + lane * 16, j + d < blocks ? end : 0, w[d]);
 #pragma unroll
     for (int d = 0; d < kDeep; ++d) {
-      const int u = u0 + 16 * d, r = u & (kRows8 - 1), t = from[r], c = (b0 + (u / kRows8)) * kBlock8 + lane * 8;
-      eight(x + (long long)t * ldx, u < blocks * kRows8 && (unsigned)t < (unsigned)M ? c : K, K, vec, v[d]);
-    }
+      uint32_t m = top_pair(w[d]);
 #pragma unroll
-    for (int d = 0; d < kDeep; ++d) {
-      const int u = u0 + 16 * d, r = u & (kRows8 - 1), b = u / kRows8, c = (b0 + b) * kBlock8 + lane * 8;
-      uint32_t top = top_of(v[d]);
-#pragma unroll
-      for (int o = 8; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffu << (threadIdx.x & 16), top, o));
-      if (b >= blocks || r >= count) continue;
+      for (int o = 4; o; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
       float scale, inverse;
-      scale_of(top, scale, inverse);
-      if (c < ldc) *reinterpret_cast<uint2*>(codes + (i0 + r) * ldc + c) = codes_of(v[d], inverse);
-      if (lane == 0) found[b][r] = scale;
+      scale_of(top_bits(m, T()), scale, inverse);
+      const int c = (b0 + j + d) * kBlock8 + lane * 16;
+      if (j + d < blocks && i < R && c < ldc) *reinterpret_cast<uint4*>(out + c) = sixteen_codes<T>(w[d], inverse);
+      if (j + d < blocks && lane == 0) found[j + d][r] = scale;
     }
   }
   __syncthreads();
-  for (int u = threadIdx.x; u < blocks * kRows8; u += 256)
-    if ((u & (kRows8 - 1)) < count) scales[(long long)(b0 + u / kRows8) * R + i0 + (u & (kRows8 - 1))] = found[u / kRows8][u & (kRows8 - 1)];
+  for (int u = threadIdx.x; u < blocks * kRows8; u += 256) {
+    const int k = u & (kRows8 - 1);
+    if (i0 + k < R) scales[(long long)(b0 + u / kRows8) * R + i0 + k] = found[u / kRows8][k];
+  }
 }
 
 // Weights w [E, N, K] to codes (rows c_row, matrices c_expert apart) and scales [E][ceil(N / 128)][ceil(K / 128)]: a CTA to a block of
 // 128 x 128, which it holds in registers between the search for the largest magnitude and the codes.
-template <typename T>
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) weights8_kernel(const T* w, long long w_expert, long long w_row, int N, int K, uint8_t* codes, long long c_expert,
-                                                       long long c_row, float* scales, bool vec) {
+                                                       long long c_row, float* scales) {
   __shared__ uint32_t part[8];
   const int kb = (K + kBlock8 - 1) / kBlock8, nb = (N + kBlock8 - 1) / kBlock8;
   const int e = blockIdx.x / (kb * nb), rest = blockIdx.x - e * kb * nb, n0 = rest / kb * kBlock8, k0 = rest % kb * kBlock8;
-  const int lane = threadIdx.x & 15, r0 = threadIdx.x >> 4, c = k0 + lane * 8;
-  Pack<T, 8> held[8];
-  uint32_t top = 0u;
+  const int c = k0 + (threadIdx.x & 7) * 16, r = n0 + (threadIdx.x >> 3);
+  uint32_t held[4][8], m = 0u;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int n = n0 + r0 + 16 * i;
-    float v[8] = {};
-    if (n < N) eight(w + e * w_expert + n * w_row, c, K, vec, v);
-    store_f32<T, 8>(reinterpret_cast<T*>(&held[i]), v);  // back to the type they had: exact
-    top = max(top, top_of(v));
-  }
-  top = __reduce_max_sync(0xffffffffu, top);
+  for (int i = 0; i < 4; ++i) sixteen<VEC>(w + e * w_expert + (long long)(r + 32 * i) * w_row, c, r + 32 * i < N ? K : 0, held[i]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = __vmaxu2(m, top_pair(held[i]));
+  const uint32_t top = __reduce_max_sync(0xffffffffu, top_bits(m, T()));
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
   __syncthreads();
+  uint32_t all = part[0];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, part[i]);
+  for (int i = 1; i < 8; ++i) all = max(all, part[i]);
   float scale, inverse;
-  scale_of(top, scale, inverse);
+  scale_of(all, scale, inverse);
   if (threadIdx.x == 0) scales[blockIdx.x] = scale;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int n = n0 + r0 + 16 * i;
-    if (n >= N || c >= (K + 15) / 16 * 16) continue;
-    float v[8];
-    unpack<T, 8>(held[i], v);
-    *reinterpret_cast<uint2*>(codes + e * c_expert + n * c_row + c) = codes_of(v, inverse);
-  }
+  for (int i = 0; i < 4; ++i)
+    if (r + 32 * i < N && c < (K + 15) / 16 * 16)
+      *reinterpret_cast<uint4*>(codes + e * c_expert + (long long)(r + 32 * i) * c_row + c) = sixteen_codes<T>(held[i], inverse);
 }
 
 // ------------------------------------------------------------------ products
@@ -677,7 +709,10 @@ int launch_rows8(const void* x, long long ldx, int M, const int* rows, int R, in
   int span = kSpan8;
   while (span > 1 && (long long)over * ((blocks + span - 1) / span) < 4 * 148) span /= 2;
   const bool vec = aligned(x, 16) && ldx % 8 == 0 && K % 8 == 0;
-  rows8_kernel<T><<<dim3(over, (blocks + span - 1) / span), 256, 0, st>>>(static_cast<const T*>(x), ldx, M, rows, R, K, span, codes, ldc, scales, vec);
+  const dim3 grid(over, (blocks + span - 1) / span);
+  const T* xt = static_cast<const T*>(x);
+  if (vec) rows8_kernel<T, true><<<grid, 256, 0, st>>>(xt, ldx, M, rows, R, K, span, codes, ldc, scales);
+  else rows8_kernel<T, false><<<grid, 256, 0, st>>>(xt, ldx, M, rows, R, K, span, codes, ldc, scales);
   return launched(1);
 }
 template <typename T>
@@ -740,10 +775,12 @@ int fs_weights8(const void* w, int type, long long w_expert, long long w_row, in
   if (grid > 0x7fffffffll) return report_error(FS_ERR_UNSUPPORTED, "too many blocks of 128 x 128 values");
   const bool vec = aligned(w, 16) && w_row % 8 == 0 && w_expert % 8 == 0 && K % 8 == 0;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (type == FS_TYPE_F16)
-    weights8_kernel<<<(unsigned)grid, 256, 0, st>>>(static_cast<const __half*>(w), w_expert, w_row, N, K, codes, c_expert, c_row, scales, vec);
-  else
-    weights8_kernel<<<(unsigned)grid, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(w), w_expert, w_row, N, K, codes, c_expert, c_row, scales, vec);
+  auto go = [&](auto* p) {
+    if (vec) weights8_kernel<std::remove_const_t<std::remove_pointer_t<decltype(p)>>, true><<<(unsigned)grid, 256, 0, st>>>(p, w_expert, w_row, N, K, codes, c_expert, c_row, scales);
+    else weights8_kernel<std::remove_const_t<std::remove_pointer_t<decltype(p)>>, false><<<(unsigned)grid, 256, 0, st>>>(p, w_expert, w_row, N, K, codes, c_expert, c_row, scales);
+  };
+  if (type == FS_TYPE_F16) go(static_cast<const __half*>(w));
+  else go(static_cast<const __nv_bfloat16*>(w));
   return launched(1);
 }
 
