@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(256) weights8_kernel(const T* w, long long w_e
 // more than the 168 registers that 384 threads have each: 40 for the first group, 232 for the others (128 x 40 + 256 x 232 = 384 x 168).
 constexpr int kSumWarps = 8, kFetchWarp = 0, kIssueWarp = 1, kGroupWarp = 2, kFirstSum = 4, kThreads8 = 32 * (kFirstSum + kSumWarps);
 constexpr uint32_t kTileA = 128 * 128;
-constexpr int kStage8 = 4096 * kSumWarps;  // staging of results
+constexpr int kStage8 = 2 * 4096 * kSumWarps;  // staging of results, two tiles of 32 x 128 bytes for each warp
 
 struct Mm8Args {
   const int* offsets;
@@ -213,6 +213,21 @@ __device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint3
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
         ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+// Sixteen columns of the accumulators; the values are there after the wait.
+__device__ __forceinline__ void read16(uint32_t at, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+                 "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(at));
+}
+__device__ __forceinline__ void wait16(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                 "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
 }
 
 struct Tile8 {
@@ -373,13 +388,15 @@ mm8_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapA, const __gr
     // Two warps to a quarter of the TMEM lanes (rows), with one half of the features each.
     constexpr int kMine = BN / 2;
     const int q = warp & 3, side = (warp - kFirstSum) >> 2;
-    const uint32_t stage = smem_u32(staging + 4096 * (warp - kFirstSum));
+    const uint32_t stages = smem_u32(staging + 8192 * (warp - kFirstSum));
     int buf = 0;
     uint32_t acc_ph = 0;
     bool lost = false;  // a wait of this CTA gave up: NaN from here on
-    auto release = [&]() {  // the staging tile, by the copy that reads it
+    uint32_t stage = stages;
+    auto release = [&]() {  // the next staging tile, by the copy before last
       if (a.boxes) {
-        if (lane == 0) bulk_read();
+        stage = stages + (stage == stages ? 4096 : 0);
+        if (lane == 0) bulk_read<1>();
         __syncwarp();
       }
     };
@@ -388,19 +405,27 @@ mm8_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapA, const __gr
       __syncwarp();
       if (lane == 0) store_box(&mapC, n, row, stage);
     };
+    // The tile after this one and its first factors are looked up before this one's results are written.
+    const float *sx = a.sx, *sw = a.sw;
+    float x_next = 0.f, w_next = 0.f;
+    Tile8 next = {};
+    auto look = [&](int it) {
+      if (it >= total) return;
+      next = tiles.at(it);
+      sx = a.sx + min(next.lo + rank * 128 + q * 32 + lane, a.R - 1);
+      sw = a.sw + next.e * a.sw_expert + (long long)min(next.n0 + side * kMine, a.N - 1) / kBlock8 * a.sw_n;
+      if (next.blocks) {
+        x_next = __ldg(sx);
+        w_next = __ldg(sw);
+      }
+    };
+    look(first);
     for (int it = first; it < total; it += stride) {
-      const Tile8 t = tiles.at(it);
+      const Tile8 t = next;
       const int row0 = t.lo + rank * 128 + q * 32, n0 = t.n0 + side * kMine;
       u64 sum[kMine / 2];
 #pragma unroll
       for (int i = 0; i < kMine / 2; ++i) sum[i] = 0ull;
-      const float* sx = a.sx + min(row0 + lane, a.R - 1);
-      const float* sw = a.sw + t.e * a.sw_expert + (long long)min(n0, a.N - 1) / kBlock8 * a.sw_n;
-      float x_next = 0.f, w_next = 0.f;
-      if (t.blocks) {
-        x_next = __ldg(sx);
-        w_next = __ldg(sw);
-      }
       for (int kb = 0; kb < t.blocks && !lost; ++kb) {
         const float f = x_next * w_next;
         if (kb + 1 < t.blocks) {
@@ -412,13 +437,13 @@ mm8_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapA, const __gr
         tc_fence_after();
         const u64 f2 = pk(f, f);
         const uint32_t acc = tmem + buf * BN + side * kMine + ((uint32_t)(q * 32) << 16);
-        uint32_t r[2][32];  // 32 columns are on their way while the ones before them are added
-        tmem_ld32_nowait(acc, r[0]);
+        uint32_t r[2][16];  // 16 columns are on their way while the ones before them are added
+        read16(acc, r[0]);
 #pragma unroll
-        for (int j = 0; j < kMine / 32; ++j) {
-          tmem_ld_wait(r[j & 1]);
-          if (j + 1 < kMine / 32) {
-            tmem_ld32_nowait(acc + 32 * (j + 1), r[(j + 1) & 1]);
+        for (int j = 0; j < kMine / 16; ++j) {
+          wait16(r[j & 1]);
+          if (j + 1 < kMine / 16) {
+            read16(acc + 16 * (j + 1), r[(j + 1) & 1]);
           } else {
             tc_fence_before();
             __syncwarp();
@@ -428,14 +453,15 @@ mm8_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapA, const __gr
             }
           }
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            sum[16 * j + i] = fma2(pk(__uint_as_float(r[j & 1][2 * i]), __uint_as_float(r[j & 1][2 * i + 1])), f2, sum[16 * j + i]);
+          for (int i = 0; i < 8; ++i)
+            sum[8 * j + i] = fma2(pk(__uint_as_float(r[j & 1][2 * i]), __uint_as_float(r[j & 1][2 * i + 1])), f2, sum[8 * j + i]);
         }
         if (++buf == kBufs) {
           buf = 0;
           acc_ph ^= 1;
         }
       }
+      look(it + stride);
       if (lost && t.blocks) {
         const float nan = __uint_as_float(0x7fc00000u);
 #pragma unroll

@@ -71,13 +71,24 @@ __device__ __forceinline__ bool wait_blocks(uint32_t bar, uint32_t parity, volat
   }
   return true;
 }
-// For a wait that ends within a microsecond, many times in a tile: without parking the thread.
+// For a wait that ends within a microsecond, many times in a tile: without putting the thread to sleep.
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 __device__ __forceinline__ bool wait_close(uint32_t bar, uint32_t parity, volatile int* abort_flag, long long limit) {
   if (limit == 0) *abort_flag = 1;  // without a look, for tests
   if (limit == 0) return false;
-  if (mbar_try_wait(bar, parity)) return true;
+  if (mbar_test(bar, parity)) return true;
   const long long t0 = clock64();
-  while (!mbar_try_wait(bar, parity)) {
+  while (!mbar_test(bar, parity)) {
     if (*abort_flag) return false;
     if (clock64() - t0 > limit) {
       *abort_flag = 1;
@@ -226,7 +237,8 @@ __device__ __forceinline__ void store_box(const CUtensorMap* map, int c0, int c1
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(tile), "r"(c0), "r"(c1) : "memory");
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
-__device__ __forceinline__ void bulk_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+template <int LEFT>  // but the last LEFT ones
+__device__ __forceinline__ void bulk_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(LEFT) : "memory"); }
 __device__ __forceinline__ void bulk_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 PFN_cuTensorMapEncodeTiled_v12000 encoder() {
