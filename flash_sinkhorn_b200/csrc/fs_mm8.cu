@@ -233,7 +233,7 @@ __device__ __forceinline__ void wait16(uint32_t (&r)[16]) {
 struct Tile8 {
   int e, n0, lo, hi, blocks;  // expert, first feature, rows of the tile, blocks of 128 contraction values (0: rows of no expert)
 };
-template <int CG, int BN>
+template <int BM, int BN>  // rows and features of a tile
 struct Tiles8 {
   const Mm8Args& a;
   const int *gs, *ts;
@@ -250,8 +250,8 @@ struct Tiles8 {
     Tile8 t;
     t.e = e;
     t.n0 = (rest - m * nt) * BN;
-    t.lo = gs[e] + m * 128 * CG;
-    t.hi = min(t.lo + 128 * CG, gs[e + 1]);
+    t.lo = gs[e] + m * BM;
+    t.hi = min(t.lo + BM, gs[e + 1]);
     t.blocks = e < a.E ? (a.K + kBlock8 - 1) / kBlock8 : 0;
     return t;
   }
@@ -308,7 +308,7 @@ mm8_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapA, const __gr
   if (CG == 2) cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem = *slot;
-  Tiles8<CG, BN> tiles(a, gs, ts);
+  Tiles8<128 * CG, BN> tiles(a, gs, ts);
   const int total = tiles.total();
   int issued = 0;  // stages that this CTA's loading thread has started
 
@@ -544,6 +544,207 @@ mm8_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapA, const __gr
   if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_mm8_error, 1);
 }
 
+// ------------------------------------------------------------------ short groups
+// Groups of up to a few dozen rows are bound by reading their weights. Here the FEATURES are the M side and the rows N, as in the
+// 16-bit products: a stage is 16 KB of weights and 4 KB of rows, an accumulator kShortRows columns, of which 256 / kShortRows are in use in turn, so that the
+// tensor core does not wait for the sums. Two CTAs to an SM: one's first loads of a tile hide behind the other one's products.
+constexpr int kShortRows = 32;                                       // of a tile: a lane's factor is that of one
+constexpr int kShortThreads = 192, kShortFetch = 4, kShortIssue = 5;  // four warps that sum
+constexpr size_t kShortSmem = 112 * 1024;                            // two fit an SM, and no kernel of this library beside one: they take 120 KB
+
+__global__ void __launch_bounds__(kShortThreads, 2)
+mm8_short_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUtensorMap mapX) {
+  constexpr uint32_t kStage = kTileA + kShortRows * 128, kColumns = 256;
+  constexpr int kBufs = kColumns / kShortRows, kAhead = 4;
+  extern __shared__ uint8_t raw[];
+  __shared__ __align__(16) float factors[4][2][kShortRows];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + (size_t)a.nstage * kStage);
+  const int FULL = 0, EMPTY = a.nstage, ACC_FULL = 2 * a.nstage, ACC_EMPTY = ACC_FULL + kBufs, DRAIN = ACC_EMPTY + kBufs;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(bars + DRAIN + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(slot + 1);
+  int *gs = reinterpret_cast<int*>(slot + 2), *ts = gs + a.E + 2;
+  auto bar = [&](int i) { return smem_u32(bars + i); };
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int first = blockIdx.x, stride = gridDim.x;
+
+  if (warp == 0) {
+    read_groups<true>(a.offsets, a.E, a.R, gs, ts, (a.N + 127) / 128, kShortRows);
+  } else if (warp == kShortFetch && lane == 0) {
+    for (int s = 0; s < 2 * a.nstage + 2 * kBufs + 1; ++s) mbar_init(bar(s), s >= ACC_EMPTY && s < DRAIN ? 4 : 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  } else if (warp == kShortIssue) {
+    alloc_columns<1>(smem_u32(slot), kColumns);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *slot;
+  Tiles8<kShortRows, 128> tiles(a, gs, ts);
+  const int total = tiles.total();
+  int issued = 0;
+
+  if (warp == kShortFetch) {
+    // ===================== loads =====================
+    if (elect_one()) {
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int it = first; ok && it < total; it += stride) {
+        const Tile8 t = tiles.at(it);
+        for (int kb = 0; kb < t.blocks; ++kb) {
+          if (!mbar_wait(bar(EMPTY + s), ph ^ 1, abort_flag)) {
+            ok = false;
+            break;
+          }
+          const uint32_t full = bar(FULL + s), dst = smem_u32(ring + (size_t)s * kStage);
+          mbar_expect_tx(full, kStage);
+          load_3d<1>(dst, &mapW, kb * 128, t.n0, t.e, full);
+          tma_load_2d(dst + kTileA, &mapX, kb * 128, t.lo, full);
+          ++issued;
+          if (++s == a.nstage) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+      }
+    }
+  } else if (warp == kShortIssue) {
+    // ===================== products =====================
+    if (elect_one()) {
+      int s = 0, buf = 0;
+      uint32_t ph = 0, acc_ph = 0;
+      bool ok = true;
+      for (int it = first; ok && it < total; it += stride) {
+        const Tile8 t = tiles.at(it);
+        const uint32_t idesc = (1u << 4) | ((uint32_t)((t.hi - t.lo + 15) / 16 * 2) << 17) | ((uint32_t)(128 >> 4) << 24);
+        for (int kb = 0; kb < t.blocks; ++kb) {
+          if (!mbar_wait(bar(ACC_EMPTY + buf), acc_ph ^ 1, abort_flag) || !mbar_wait(bar(FULL + s), ph, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t base = smem_u32(ring + (size_t)s * kStage), al = desc_lo(base), bl = desc_lo(base + kTileA);
+          const int left = a.K - kb * kBlock8;
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+            if (ks * 32 < left) mma_f8<1>(tmem + buf * kShortRows, pack_desc(al + ks * 2, kDescHi128), pack_desc(bl + ks * 2, kDescHi128), idesc, ks);
+          commit<1>(bar(EMPTY + s));
+          commit<1>(bar(ACC_FULL + buf));
+          if (++s == a.nstage) {
+            s = 0;
+            ph ^= 1;
+          }
+          if (++buf == kBufs) {
+            buf = 0;
+            acc_ph ^= 1;
+          }
+        }
+      }
+    }
+  } else {
+    // ===================== sums and results =====================
+    // A lane has a feature; the rows' factors, a lane's for its row, are read four blocks ahead and handed round in shared memory.
+    int buf = 0;
+    uint32_t acc_ph = 0;
+    bool lost = false;  // a wait of this CTA gave up: NaN from here on
+    float xs[kAhead], ws[kAhead];
+    const float *sx = a.sx, *sw = a.sw;
+    Tile8 next = {};
+    auto ask = [&](int kb, int d) {
+      if (kb >= next.blocks) return;
+      xs[d] = next.lo + lane < next.hi ? __ldg(sx + (long long)kb * a.R) : 0.f;
+      ws[d] = __ldg(sw + (long long)kb * a.sw_k);
+    };
+    auto look = [&](int it) {
+      if (it >= total) return;
+      next = tiles.at(it);
+      sx = a.sx + next.lo + lane;
+      sw = a.sw + next.e * a.sw_expert + (long long)(next.n0 / kBlock8) * a.sw_n;
+#pragma unroll
+      for (int d = 0; d < kAhead; ++d) ask(d, d);
+    };
+    look(first);
+    for (int it = first; it < total; it += stride) {
+      const Tile8 t = next;
+      u64 sum[kShortRows / 2];
+#pragma unroll
+      for (int i = 0; i < kShortRows / 2; ++i) sum[i] = 0ull;
+      for (int k0 = 0; k0 < t.blocks; k0 += kAhead)
+#pragma unroll
+        for (int d = 0; d < kAhead; ++d) {
+          if (k0 + d >= t.blocks || lost) continue;
+          float* mine = factors[warp][d & 1];
+          mine[lane] = xs[d] * ws[d];
+          ask(k0 + d + kAhead, d);
+          __syncwarp();
+          lost = !__all_sync(0xffffffffu, wait_close(bar(ACC_FULL + buf), acc_ph, abort_flag, a.limit));
+          if (lost) continue;
+          tc_fence_after();
+#pragma unroll
+          for (int j = 0; j < kShortRows / 16; ++j) {
+            uint32_t r[16];
+            read16(tmem + buf * kShortRows + 16 * j + ((uint32_t)(warp * 32) << 16), r);
+            wait16(r);
+            if (j + 1 == kShortRows / 16) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(bar(ACC_EMPTY + buf));
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float4 f = *reinterpret_cast<const float4*>(mine + 16 * j + 4 * i);
+              sum[8 * j + 2 * i] = fma2(pk(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1])), pk(f.x, f.y), sum[8 * j + 2 * i]);
+              sum[8 * j + 2 * i + 1] = fma2(pk(__uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3])), pk(f.z, f.w), sum[8 * j + 2 * i + 1]);
+            }
+          }
+          if (++buf == kBufs) {
+            buf = 0;
+            acc_ph ^= 1;
+          }
+        }
+      look(it + stride);
+      const int f = t.n0 + warp * 32 + lane, rows = t.hi - t.lo;
+      if (f >= a.N) continue;
+#pragma unroll
+      for (int j = 0; j < kShortRows; ++j) {
+        float lo, hi;
+        upk(sum[j / 2], lo, hi);
+        const float v = lost && t.blocks ? __uint_as_float(0x7fc00000u) : j & 1 ? hi : lo;
+        if (j < rows) {
+          const long long at = (long long)(t.lo + j) * a.ldo + f;
+          if (a.out_type == FS_TYPE_F32) static_cast<float*>(a.out)[at] = v;
+          else if (a.out_type == FS_TYPE_BF16) static_cast<__nv_bfloat16*>(a.out)[at] = from_f32<__nv_bfloat16>(v);
+          else static_cast<__half*>(a.out)[at] = from_f32<__half>(v);
+        }
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {  // nobody waits any more, and the flag does not change: products and copies in flight end first
+    if (warp == kShortIssue) {
+      if (elect_one()) {
+        commit<1>(bar(DRAIN));
+        mbar_wait_quiet(bar(DRAIN), 0);
+      }
+      __syncwarp();
+    } else if (warp == kShortFetch) {
+      if (elect_one()) {
+        const long long t0 = clock64();
+        for (int j = issued > a.nstage ? issued - a.nstage : 0; j < issued; ++j) wait_landed(bar(FULL + j % a.nstage), (j / a.nstage) & 1, t0);
+      }
+      __syncwarp();
+    }
+  }
+  tc_fence_after();
+  if (warp == kShortIssue) free_columns<1>(tmem, kColumns);
+  if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_mm8_error, 1);
+}
+
 // ------------------------------------------------------------------ few rows
 // A single token: bound by reading its experts' weights, so a warp takes one feature of one expert, 16 codes a lane and load, as the
 // 16-bit products do. Each CTA puts the rows into 8 bits itself (a few microseconds less than a launch that does it once).
@@ -729,6 +930,34 @@ int launch_mm8(Mm8Args a, const uint8_t* x, long long ldx, const uint8_t* w, lon
   return FS_OK;
 }
 
+int launch_short8(Mm8Args a, const uint8_t* x, long long ldx, const uint8_t* w, long long w_expert, long long w_row, cudaStream_t st) {
+  CUtensorMap mapW = {}, mapX = {};
+  if (!encode8(&mapW, w, 3, {a.K, a.N, a.E}, {w_row, w_expert ? w_expert : w_row}, 128) || !encode8(&mapX, x, 2, {a.K, a.R, 1}, {ldx, 0}, kShortRows))
+    return report_error(FS_ERR_CUDA, "cuTensorMapEncodeTiled failed");
+  constexpr size_t kStage = kTileA + kShortRows * 128, kStatic = 4 * 2 * kShortRows * sizeof(float);
+  const size_t fixed = 1024 + 8 * (2 * 8 + 2 * (256 / kShortRows) + 1) + 8 + 8 * ((size_t)a.E + 2);
+  a.nstage = (int)((kShortSmem - kStatic - fixed) / kStage);
+  static_assert((kShortSmem - kStatic - 1024 - 8 * 33 - 8 - 8 * 1026) / kStage >= 4 && (kShortSmem / kStage) <= 8, "stages");
+  const auto kernel = mm8_short_kernel;
+  static std::atomic<uint64_t> allowed{0};  // devices on which the kernel may take that much shared memory
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (e == cudaSuccess && !(allowed.load(std::memory_order_relaxed) & bit)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kShortSmem - kStatic));
+    if (e == cudaSuccess) allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
+  if (e != cudaSuccess) return report_error(FS_ERR_CUDA, cudaGetErrorString(e));
+  const long long most = ((a.R + kShortRows - 1ll) / kShortRows + a.E + 1) * ((a.N + 127) / 128);
+  if (most > 0x3fffffffll) return report_error(FS_ERR_UNSUPPORTED, "more than 2^30 tiles");
+  long long grid = 2 * detail::free_ctas();
+  if (grid > most) grid = most;
+  if (grid < 1) grid = 1;
+  g_mm8_launched.store(true, std::memory_order_relaxed);
+  kernel<<<(unsigned)grid, kShortThreads, kShortSmem - kStatic, st>>>(a, mapW, mapX);
+  return launched(1);
+}
+
 template <typename T>
 int launch_rows8(const void* x, long long ldx, int M, const int* rows, int R, int K, uint8_t* codes, long long ldc, float* scales, cudaStream_t st) {
   const int blocks = (K + kBlock8 - 1) / kBlock8, over = (R + kRows8 - 1) / kRows8;
@@ -851,14 +1080,14 @@ int fs_grouped_mm8(const void* x, int type, long long ldx, int M, const int* row
                           : launch_rows8<__nv_bfloat16>(x, ldx, M, rows, R, K, codes, ldc, sx, st);
   if (s != FS_OK) return s;
   const long long tiles = ((R + 255ll) / 256 + (E < R ? E : R) / 2) * ((N + 255) / 256);
+  const bool pairs = tiles * 2 > detail::free_ctas() && N > 128;
   if (transposed) {
-    if (tiles * 2 > detail::free_ctas() && N > 128) return launch_mm8<true, 2, 256>(a, codes, ldc, w, w_expert, w_row, st);
+    if (pairs) return launch_mm8<true, 2, 256>(a, codes, ldc, w, w_expert, w_row, st);
     return launch_mm8<true, 1, 128>(a, codes, ldc, w, w_expert, w_row, st);
   }
-  if (tiles * 2 > detail::free_ctas() && N > 128 && R / E > 64) return launch_mm8<false, 2, 256>(a, codes, ldc, w, w_expert, w_row, st);
-  const long long mid = ((R + 127ll) / 128 + (E < R ? E : R) / 2) * ((N + 127) / 128);
-  if (mid > detail::free_ctas() && R / E > 64) return launch_mm8<false, 1, 128>(a, codes, ldc, w, w_expert, w_row, st);
-  return launch_mm8<false, 1, 64>(a, codes, ldc, w, w_expert, w_row, st);
+  if (R / E <= 40) return launch_short8(a, codes, ldc, w, w_expert, w_row, st);
+  if (pairs && R / E >= 160) return launch_mm8<false, 2, 256>(a, codes, ldc, w, w_expert, w_row, st);
+  return launch_mm8<false, 1, 128>(a, codes, ldc, w, w_expert, w_row, st);
 }
 
 }  // extern "C"
