@@ -32,56 +32,81 @@ constexpr float kXScale = 256.f, kAScale = 1024.f;  // X and A are held times th
 constexpr int kNormParts = 64;                      // CTAs that sum the squares of a matrix
 
 // ------------------------------------------------------------------ X = G / |G|
-// Sums of squares in 64 bits: those of 32-bit values would overflow from 2^64 on.
-template <typename T>
+// Sums of squares in 64 bits: those of 32-bit values would overflow from 2^64 on. V values to a load.
+template <typename T, int V>
 __global__ void __launch_bounds__(256) squares_kernel(const T* g, long long g_matrix, long long g_row, int rows, int cols, double* parts) {
   __shared__ double warp_sums[8];
   const T* m = g + blockIdx.y * g_matrix;
+  const int lane = threadIdx.x & 31;
   double s = 0.0;
-  for (int r = blockIdx.x; r < rows; r += gridDim.x)
-    for (int c = threadIdx.x; c < cols; c += 256) {
-      const double v = (double)to_f32(m[(long long)r * g_row + c]);
-      s = fma(v, v, s);
+  for (int r = blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.x * 8) {  // a warp to a row
+    const T* row = m + (long long)r * g_row;
+    constexpr int kDeep = 4;
+    for (int c0 = lane * V; c0 < cols; c0 += 32 * V * kDeep) {
+      Pack<T, V> p[kDeep];
+#pragma unroll
+      for (int d = 0; d < kDeep; ++d)
+        if (c0 + 32 * V * d < cols) p[d] = read_only<T, V>(row + c0 + 32 * V * d);
+#pragma unroll
+      for (int d = 0; d < kDeep; ++d) {
+        float v[V];
+        unpack<T, V>(p[d], v);
+        if (c0 + 32 * V * d < cols)
+#pragma unroll
+          for (int j = 0; j < V; ++j) s = fma((double)v[j], (double)v[j], s);
+      }
     }
+  }
 #pragma unroll
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if ((threadIdx.x & 31) == 0) warp_sums[threadIdx.x >> 5] = s;
+  if (lane == 0) warp_sums[threadIdx.x >> 5] = s;
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 1; w < 8; ++w) s += warp_sums[w];
     parts[blockIdx.y * gridDim.x + blockIdx.x] = s;
   }
 }
-// Tiles of 32 x 32 of G to both parts of X, transposed for a tall G; X [n, k], rows ldx apart.
-template <typename T>
+// Tiles of 64 x 64 of G to both parts of X, transposed for a tall G; X [n, k], rows ldx apart. V values to a load of G.
+template <typename T, int V>
 __global__ void __launch_bounds__(256) begin_kernel(const T* g, long long g_matrix, long long g_row, int rows, int cols, const double* parts, int count,
                                                     float eps, bool tall, __half* hi, __half* lo, long long ldx) {
-  __shared__ float tile[32][33];
-  __shared__ float factor;
-  const int b = blockIdx.z, r0 = blockIdx.y * 32, c0 = blockIdx.x * 32, x = threadIdx.x & 31, y = threadIdx.x >> 5;
-  if (threadIdx.x == 0) {
-    double s = 0.0;
-    for (int i = 0; i < count; ++i) s += parts[b * count + i];
-    factor = (float)((double)kXScale / (sqrt(s) + (double)eps));
-  }
-  __syncthreads();
-  const float f = factor;
+  __shared__ float tile[64][65];
+  const int b = blockIdx.z, r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
+  constexpr int kLanes = 64 / V;  // to a row of the tile
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = r0 + y + 8 * i, c = c0 + x;
-    tile[y + 8 * i][x] = r < rows && c < cols ? to_f32(g[b * g_matrix + (long long)r * g_row + c]) * f : 0.f;
+  for (int y = threadIdx.x / kLanes; y < 64; y += 256 / kLanes) {
+    const int r = r0 + y, x = threadIdx.x % kLanes * V;
+    float v[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = 0.f;
+    if (r < rows && c0 + x < cols) unpack<T, V>(read_only<T, V>(g + b * g_matrix + (long long)r * g_row + c0 + x), v);
+#pragma unroll
+    for (int j = 0; j < V; ++j) tile[y][x + j] = v[j];
   }
+  // every warp adds the sums of squares in the same order
+  double s = 0.0;
+  for (int i = threadIdx.x & 31; i < count; i += 32) s += parts[b * count + i];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  const float f = (float)((double)kXScale / (sqrt(s) + (double)eps));
   __syncthreads();
   const int n = tall ? cols : rows, k = tall ? rows : cols, n0 = tall ? c0 : r0, k0 = tall ? r0 : c0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = n0 + y + 8 * i, col = k0 + x;
+  for (int y = threadIdx.x >> 3; y < 64; y += 32) {
+    const int row = n0 + y, x = (threadIdx.x & 7) * 8, col = k0 + x;
     if (row >= n || col >= k) continue;
-    const float v = tall ? tile[x][y + 8 * i] : tile[y + 8 * i][x];
-    const __half h = __float2half_rn(v);
-    const long long at = ((long long)b * n + row) * ldx + col;
-    hi[at] = h;
-    lo[at] = __float2half_rn(v - __half2float(h));
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float v0 = (tall ? tile[x + 2 * j][y] : tile[y][x + 2 * j]) * f, v1 = (tall ? tile[x + 2 * j + 1][y] : tile[y][x + 2 * j + 1]) * f;
+      float u0, u1;
+      h[j] = from_two(v0, v1, __half());
+      two_f32(h[j], u0, u1, __half());
+      l[j] = from_two(v0 - u0, v1 - u1, __half());
+    }
+    const long long at = ((long long)b * n + row) * ldx + col;  // rows are padded to 16 bytes
+    *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
+    *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
   }
 }
 
@@ -89,7 +114,7 @@ __global__ void __launch_bounds__(256) begin_kernel(const T* g, long long g_matr
 enum Product { GRAM, SQUARE, APPLY, LAST };  // LAST: APPLY to the result
 
 constexpr int kWriteWarps = 8, kGetWarp = 8, kMulWarp = 9, kThreadsO = 32 * 10;
-constexpr int kStageO = 4096 * kWriteWarps;
+constexpr int kStageO = 8192 * kWriteWarps;  // two tiles of 32 rows of 128 bytes for each warp that writes
 
 struct OrthoArgs {
   int batch, n, k;          // X is n x k, A and P are n x n
@@ -140,15 +165,10 @@ struct TilesO {
   }
 };
 
-// 32 values of a row, of which there are `left`, padded to a multiple of 8.
-__device__ __forceinline__ void load_row32(const __half* p, long long left, float (&v)[32]) {
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const uint4 q = 8 * c < left ? *(reinterpret_cast<const uint4*>(p) + c) : make_uint4(0u, 0u, 0u, 0u);
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) two_f32(w[j], v[8 * c + 2 * j], v[8 * c + 2 * j + 1], __half());
-  }
+__device__ __forceinline__ uint4 load_chunk(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
 }
 
 template <int FORM, int CG, int BN>
@@ -267,105 +287,143 @@ ortho_kernel(const OrthoArgs a, const __grid_constant__ CUtensorMap mapA, const 
     }
   } else {
     // ===================== results =====================
-    // Two warps to a quarter of the TMEM lanes (rows), with every other 32 columns each.
+    // Two warps to a quarter of the TMEM lanes (rows), with every other block of kCols columns each. What a block adds to its
+    // product (A, or both parts of X) comes by whole rows of 16-byte loads, is under way in registers while the block before it is
+    // worked on, and goes through shared memory to the lanes that have its rows; results go back the same way.
+    constexpr int kCols = BN >= 128 ? 64 : 32, kPer = kCols / 8, kFrom = FORM == GRAM ? 0 : FORM == SQUARE ? 1 : 2;
     const int q = warp & 3, side = warp >> 2;
-    const uint32_t stage = smem_u32(staging + 4096 * warp);
-    int t = 0;
+    const uint32_t stage = smem_u32(staging + 8192 * warp);
+    const int width = FORM >= APPLY ? a.k : a.n;  // columns of the product
+    const long long ld = FORM >= APPLY ? a.ldx : a.lda;
+    uint4 ahead[kFrom ? kFrom : 1][kPer];
+    auto ask = [&](int b, int row0, int col) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int r = row0 + i * (32 / kPer) + lane / kPer, c = col + 8 * (lane % kPer);
+        const long long at = ((long long)b * a.n + r) * ld + c;
+        const bool in = r < a.n && c < width;  // rows are padded to 16 bytes
+#pragma unroll
+        for (int k = 0; k < kFrom; ++k)
+          ahead[k][i] = in ? *reinterpret_cast<const uint4*>((FORM == SQUARE ? a.a : k ? a.lo : a.hi) + at) : make_uint4(0u, 0u, 0u, 0u);
+      }
+    };
+    int t = 0, b = 0, m0 = 0, n0 = 0;
     bool lost = false;  // a wait of this CTA gave up: NaN from here on
+    if (first < total) {
+      tiles.at(first, b, m0, n0);
+      if (kFrom) ask(b, m0 + rank * 128 + q * 32, n0 + kCols * side);
+    }
     for (long long it = first; it < total; it += stride, ++t) {
-      int b, m0, n0;
-      tiles.at(it, b, m0, n0);
       const int buf = t & 1, row0 = m0 + rank * 128 + q * 32, row = row0 + lane;
+      int next_b = 0, next_m = 0, next_n = 0;
+      if (it + stride < total) tiles.at(it + stride, next_b, next_m, next_n);
       if (!lost) {
         lost = !__all_sync(0xffffffffu, wait_blocks(bar(ACC_FULL + buf), (t >> 1) & 1, abort_flag, blocks, a.limit));
         tc_fence_after();
       }
-      const int width = FORM >= APPLY ? a.k : a.n;  // columns of the product
 #pragma unroll 1
-      for (int c = 32 * side; c < BN; c += 64) {
+      for (int c = kCols * side; c < BN; c += 2 * kCols) {
         const int col = n0 + c;
-        if (col >= width || row0 >= a.n) break;
-        float v[32];
-        if (lost) {
+        if (kFrom) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(0x7fc00000u);
-        } else {
-          tmem_ld32(tmem + buf * BN + c + ((uint32_t)(q * 32) << 16), v);
+          for (int i = 0; i < kPer; ++i)
+#pragma unroll
+            for (int k = 0; k < kFrom; ++k)
+              stage16(staged_row(stage + 4096 * k, i * (32 / kPer) + lane / kPer, lane % kPer), ahead[k][i].x, ahead[k][i].y, ahead[k][i].z, ahead[k][i].w);
+          __syncwarp();
+          if (c + 2 * kCols < BN) ask(b, row0, col + 2 * kCols);
+          else if (it + stride < total) ask(next_b, next_m + rank * 128 + q * 32, next_n + kCols * side);
         }
-        const bool in = row < a.n;
-        if (FORM == GRAM) {
+        if (col < width && row0 < a.n) {
+          const bool across = FORM == LAST ? a.tall : FORM <= SQUARE && n0 + BN <= m0;  // also, or only, written transposed
+          uint32_t w[kCols / 2];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] *= kAScale / (kXScale * kXScale);
-        } else if (FORM == SQUARE) {
-          float old[32];
-          if (in) load_row32(a.a + ((long long)b * a.n + row) * a.lda + col, a.lda - col, old);
+          for (int h = 0; h < kCols; h += 32) {
+            float v[32];
+            if (lost) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = fmaf(v[j], a.cc / kAScale, a.cb * old[j]);
-        } else {
-          float old[32], low[32];
-          const long long at = ((long long)b * a.n + row) * a.ldx + col;
-          if (in) {
-            load_row32(a.hi + at, a.ldx - col, old);
-            load_row32(a.lo + at, a.ldx - col, low);
-          }
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = fmaf(v[j], 1.f / kAScale, a.ca * (old[j] + low[j]));
-        }
-        const int rows = a.n - row0;
-        if (FORM == LAST) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] *= 1.f / kXScale;
-          uint16_t* out = static_cast<uint16_t*>(a.out) + (long long)b * a.n * a.k;
-          if (a.tall) {  // 32 lanes write 64 bytes of a row of the result
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const uint32_t w = a.out_type == FS_TYPE_BF16 ? from_two(v[j], 0.f, __nv_bfloat16()) : from_two(v[j], 0.f, __half());
-              if (in && col + j < a.k) out[(long long)(col + j) * a.n + row] = (uint16_t)w;
+              for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(0x7fc00000u);
+            } else {
+              tmem_ld32(tmem + buf * BN + c + h + ((uint32_t)(q * 32) << 16), v);
             }
-          } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              uint32_t w[4];
+              const uint32_t at = staged_row(stage, lane, h / 8 + i);
+              float* x = v + 8 * i;
+              if (FORM == GRAM) {
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
-                w[j] = a.out_type == FS_TYPE_BF16 ? from_two(v[8 * i + 2 * j], v[8 * i + 2 * j + 1], __nv_bfloat16())
-                                                  : from_two(v[8 * i + 2 * j], v[8 * i + 2 * j + 1], __half());
-              stage16(staged_row(stage, lane, i), w[0], w[1], w[2], w[3]);
+                for (int j = 0; j < 8; ++j) x[j] *= kAScale / (kXScale * kXScale);
+              } else {
+                const uint4 p = load_chunk(at), l = kFrom == 2 ? load_chunk(at + 4096) : make_uint4(0u, 0u, 0u, 0u);
+                const uint32_t pw[4] = {p.x, p.y, p.z, p.w}, lw[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  float p0, p1, l0 = 0.f, l1 = 0.f;
+                  two_f32(pw[j], p0, p1, __half());
+                  if (kFrom == 2) two_f32(lw[j], l0, l1, __half());
+                  const float own = FORM == SQUARE ? a.cb : FORM == LAST ? a.ca / kXScale : a.ca;
+                  const float product = FORM == SQUARE ? a.cc / kAScale : FORM == LAST ? 1.f / (kAScale * kXScale) : 1.f / kAScale;
+                  x[2 * j] = fmaf(x[2 * j], product, own * (p0 + l0));
+                  x[2 * j + 1] = fmaf(x[2 * j + 1], product, own * (p1 + l1));
+                }
+              }
+              uint32_t* u = w + h / 2 + 4 * i;
+              uint32_t lower[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                u[j] = FORM == LAST && a.out_type == FS_TYPE_BF16 ? from_two(x[2 * j], x[2 * j + 1], __nv_bfloat16()) : from_two(x[2 * j], x[2 * j + 1], __half());
+                if (FORM == APPLY) {
+                  float u0, u1;
+                  two_f32(u[j], u0, u1, __half());
+                  lower[j] = from_two(x[2 * j] - u0, x[2 * j + 1] - u1, __half());
+                }
+              }
+              if (FORM != LAST || !across) stage16(at, u[0], u[1], u[2], u[3]);
+              if (FORM == APPLY) stage16(at + 4096, lower[0], lower[1], lower[2], lower[3]);
             }
-            __syncwarp();
-            write_rows(reinterpret_cast<char*>(out + (long long)row0 * a.k + col), 2ll * a.k, rows, min(2 * (a.k - col), 64), a.out_bytes, stage, lane);
-            __syncwarp();
           }
-        } else {
-          uint32_t h[16];
+          if (FORM != APPLY && across) {
+            // Pairs of lanes exchange halves, so that each has two rows of a column; a column's 32 rows are 64 bytes side by side.
+            __syncwarp();
 #pragma unroll
-          for (int j = 0; j < 16; ++j) h[j] = from_two(v[2 * j], v[2 * j + 1], __half());
-          const long long ld = FORM == APPLY ? a.ldx : a.lda;
-          __half* out = (FORM == APPLY ? a.hi_out : a.sym) + ((long long)b * a.n + row0) * ld + col;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) stage16(staged_row(stage, lane, i), h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
-          __syncwarp();
-          write_rows(reinterpret_cast<char*>(out), 2 * ld, rows, min(2 * (width - col), 64), 16, stage, lane);  // rows are padded to 16 bytes
-          __syncwarp();
-          if (FORM == APPLY) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              float x, y;
-              two_f32(h[j], x, y, __half());
-              h[j] = from_two(v[2 * j] - x, v[2 * j + 1] - y, __half());
+            for (int j = 0; j < kCols / 2; ++j) {
+              const uint32_t other = __shfl_xor_sync(0xffffffffu, w[j], 1);
+              const uint32_t two = lane & 1 ? __byte_perm(other, w[j], 0x7632) : __byte_perm(w[j], other, 0x5410);
+              asm volatile("st.shared.u32 [%0], %1;" ::"r"(stage + 4096 + (2 * j + (lane & 1)) * 64 + (lane >> 1) * 4), "r"(two) : "memory");
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) stage16(staged_row(stage, lane, i), h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
             __syncwarp();
-            write_rows(reinterpret_cast<char*>(a.lo_out + ((long long)b * a.n + row0) * ld + col), 2 * ld, rows, min(2 * (width - col), 64), 16, stage, lane);
-            __syncwarp();
-          } else if (n0 + BN <= m0 && in) {  // and the same above the diagonal
-            uint16_t* mirror = reinterpret_cast<uint16_t*>(a.sym) + ((long long)b * a.n + col) * ld + row;
+            const long long pitch = FORM == LAST ? a.n : ld;
+            uint16_t* out = FORM == LAST ? static_cast<uint16_t*>(a.out) + ((long long)b * a.k + col) * a.n + row0
+                                         : reinterpret_cast<uint16_t*>(a.sym) + ((long long)b * a.n + col) * ld + row0;
+            if (FORM != LAST || a.out_bytes == 16) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (col + j < a.n) mirror[j * ld] = (uint16_t)(j & 1 ? h[j / 2] >> 16 : h[j / 2]);
+              for (int i = 0; i < kCols / 8; ++i) {
+                const int r = 8 * i + (lane >> 2), ch = lane & 3;
+                const uint4 x = load_chunk(stage + 4096 + r * 64 + ch * 16);
+                if (col + r < width && row0 + 8 * ch < a.n) *reinterpret_cast<uint4*>(out + r * pitch + 8 * ch) = x;
+              }
+            } else {
+#pragma unroll 4
+              for (int r = 0; r < kCols; ++r) {
+                uint16_t x;
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(stage + 4096 + r * 64 + lane * 2) : "memory");
+                if (col + r < width && row < a.n) out[r * pitch + lane] = x;
+              }
+            }
+          }
+          __syncwarp();
+          const int rows = a.n - row0, bytes = min(2 * (width - col), 2 * kCols);
+          const long long at = ((long long)b * a.n + row0) * ld + col;
+          if (FORM == LAST) {
+            if (!across)
+              write_rows(reinterpret_cast<char*>(static_cast<uint16_t*>(a.out) + ((long long)b * a.n + row0) * a.k + col), 2ll * a.k, rows, bytes, a.out_bytes,
+                         stage, lane);
+          } else {
+            write_rows(reinterpret_cast<char*>((FORM == APPLY ? a.hi_out : a.sym) + at), 2 * ld, rows, bytes, 16, stage, lane);
+            if (FORM == APPLY) write_rows(reinterpret_cast<char*>(a.lo_out + at), 2 * ld, rows, bytes, 16, stage + 4096, lane);
           }
         }
+        __syncwarp();
       }
       if (!lost) {
         tc_fence_before();
@@ -375,6 +433,9 @@ ortho_kernel(const OrthoArgs a, const __grid_constant__ CUtensorMap mapA, const 
           else mbar_arrive(bar(ACC_EMPTY + buf));
         }
       }
+      b = next_b;
+      m0 = next_m;
+      n0 = next_n;
     }
   }
   __syncwarp();
@@ -478,14 +539,22 @@ int launch_form(const OrthoArgs& a, cudaStream_t st) {
 template <typename T>
 int begin(const void* g, long long g_matrix, long long g_row, int batch, int rows, int cols, double* parts, float eps, bool tall, __half* hi, __half* lo,
           long long ldx, cudaStream_t st) {
-  const T* gt = static_cast<const T*>(g);
-  const int count = rows < kNormParts ? rows : kNormParts;
+  constexpr int kWide = 16 / sizeof(T);
+  const bool wide = aligned(g, 16) && g_matrix % kWide == 0 && g_row % kWide == 0 && cols % kWide == 0;
+  const int want = (rows + 7) / 8, count = want < kNormParts ? want : kNormParts;
   for (int b0 = 0; b0 < batch; b0 += 65535) {  // the limit of a grid's second and third dimension
     const int nb = batch - b0 < 65535 ? batch - b0 : 65535;
-    squares_kernel<T><<<dim3(count, nb), 256, 0, st>>>(gt + b0 * g_matrix, g_matrix, g_row, rows, cols, parts + (size_t)b0 * count);
+    const T* from = static_cast<const T*>(g) + b0 * g_matrix;
+    double* sums = parts + (size_t)b0 * count;
     const long long at = (long long)b0 * (tall ? cols : rows) * ldx;
-    begin_kernel<T><<<dim3((cols + 31) / 32, (rows + 31) / 32, nb), 256, 0, st>>>(gt + b0 * g_matrix, g_matrix, g_row, rows, cols,
-                                                                                  parts + (size_t)b0 * count, count, eps, tall, hi + at, lo + at, ldx);
+    const dim3 over(count, nb), tiles((cols + 63) / 64, (rows + 63) / 64, nb);
+    if (wide) {
+      squares_kernel<T, kWide><<<over, 256, 0, st>>>(from, g_matrix, g_row, rows, cols, sums);
+      begin_kernel<T, kWide><<<tiles, 256, 0, st>>>(from, g_matrix, g_row, rows, cols, sums, count, eps, tall, hi + at, lo + at, ldx);
+    } else {
+      squares_kernel<T, 1><<<over, 256, 0, st>>>(from, g_matrix, g_row, rows, cols, sums);
+      begin_kernel<T, 1><<<tiles, 256, 0, st>>>(from, g_matrix, g_row, rows, cols, sums, count, eps, tall, hi + at, lo + at, ldx);
+    }
   }
   return launched(2);
 }
@@ -561,7 +630,8 @@ int fs_orthogonalize(const void* g, int type, long long g_matrix, long long g_ro
   o.ca = a; o.cb = b; o.cc = c;
   o.lo = o.lo_out = lo;
   o.out = out; o.out_type = out_type; o.tall = tall;
-  o.out_bytes = aligned(out, 16) && o.k % 8 == 0 ? 16 : aligned(out, 4) && o.k % 2 == 0 ? 4 : 2;
+  const int inner = tall ? o.n : o.k;  // values of a row of the result
+  o.out_bytes = aligned(out, 16) && inner % 8 == 0 ? 16 : aligned(out, 4) && inner % 2 == 0 ? 4 : 2;
   o.limit = product_limit();
   int r = type == FS_TYPE_F32  ? begin<float>(g, g_matrix, g_row, batch, rows, cols, parts, eps, tall, hi, lo, o.ldx, st)
           : type == FS_TYPE_F16 ? begin<__half>(g, g_matrix, g_row, batch, rows, cols, parts, eps, tall, hi, lo, o.ldx, st)
