@@ -29,6 +29,7 @@ __device__ int g_ortho_error = 0;  // non-zero once a bounded wait gave up (read
 std::atomic<bool> g_ortho_launched{false};
 
 constexpr float kXScale = 256.f, kAScale = 1024.f;  // X and A are held times these
+constexpr float kFewTimes = 16.f;  // X goes without its lower part once a rounding grows to no more than this, 16 * 2^-12 / sqrt(3) = 0.2 %
 constexpr int kNormParts = 64;                      // CTAs that sum the squares of a matrix
 
 // ------------------------------------------------------------------ X = G / |G|
@@ -119,14 +120,15 @@ constexpr int kStageO = 8192 * kWriteWarps;  // two tiles of 32 rows of 128 byte
 struct OrthoArgs {
   int batch, n, k;          // X is n x k, A and P are n x n
   long long ldx, lda;
-  const __half *hi, *lo;    // X as it is (APPLY, LAST)
-  __half *hi_out, *lo_out;  // lo_out may be lo
+  const __half *hi, *lo;    // X as it is (APPLY, LAST); lo null: zeros
+  __half *hi_out, *lo_out;  // lo_out may be lo, or null: not wanted
   const __half* a;          // A (SQUARE)
   __half* sym;              // A (GRAM) or P (SQUARE)
   float ca, cb, cc;
   void* out;  // LAST: [n, k] or, tall, [k, n]
   int out_type, out_bytes;
   bool tall;
+  bool backwards;  // the last matrix first: it is what the product before left in L2
   int nstage;
   long long limit;
 };
@@ -152,6 +154,7 @@ struct TilesO {
     constexpr int BM = 128 * CG, R = BM / BN > 0 ? BM / BN : 1;
     b = (int)(tile / per);
     int rest = (int)(tile - (long long)b * per);
+    if (a.backwards) b = a.batch - 1 - b;
     if (FORM >= APPLY) {
       const int j = rest / mt;
       m0 = (rest - j * mt) * BM;
@@ -304,7 +307,7 @@ ortho_kernel(const OrthoArgs a, const __grid_constant__ CUtensorMap mapA, const 
         const bool in = r < a.n && c < width;  // rows are padded to 16 bytes
 #pragma unroll
         for (int k = 0; k < kFrom; ++k)
-          ahead[k][i] = in ? *reinterpret_cast<const uint4*>((FORM == SQUARE ? a.a : k ? a.lo : a.hi) + at) : make_uint4(0u, 0u, 0u, 0u);
+          ahead[k][i] = in && (k == 0 || a.lo) ? *reinterpret_cast<const uint4*>((FORM == SQUARE ? a.a : k ? a.lo : a.hi) + at) : make_uint4(0u, 0u, 0u, 0u);
       }
     };
     int t = 0, b = 0, m0 = 0, n0 = 0;
@@ -420,7 +423,7 @@ ortho_kernel(const OrthoArgs a, const __grid_constant__ CUtensorMap mapA, const 
                          stage, lane);
           } else {
             write_rows(reinterpret_cast<char*>((FORM == APPLY ? a.hi_out : a.sym) + at), 2 * ld, rows, bytes, 16, stage, lane);
-            if (FORM == APPLY) write_rows(reinterpret_cast<char*>(a.lo_out + at), 2 * ld, rows, bytes, 16, stage + 4096, lane);
+            if (FORM == APPLY && a.lo_out) write_rows(reinterpret_cast<char*>(a.lo_out + at), 2 * ld, rows, bytes, 16, stage + 4096, lane);
           }
         }
         __syncwarp();
@@ -636,16 +639,27 @@ int fs_orthogonalize(const void* g, int type, long long g_matrix, long long g_ro
   int r = type == FS_TYPE_F32  ? begin<float>(g, g_matrix, g_row, batch, rows, cols, parts, eps, tall, hi, lo, o.ldx, st)
           : type == FS_TYPE_F16 ? begin<__half>(g, g_matrix, g_row, batch, rows, cols, parts, eps, tall, hi, lo, o.ldx, st)
                                 : begin<__nv_bfloat16>(g, g_matrix, g_row, batch, rows, cols, parts, eps, tall, hi, lo, o.ldx, st);
+  float grown = 1.f;  // what the steps from the last one on make of a rounding along small singular values
+  int lower_until = steps;
+  while (lower_until > 1 && grown * fabsf(a) <= kFewTimes) {
+    grown *= fabsf(a);
+    --lower_until;
+  }
   for (int i = 0; i < steps && r == FS_OK; ++i) {
     o.hi = hi;
+    o.lo = i < lower_until ? lo : nullptr;
     o.hi_out = other;
+    o.lo_out = i + 1 < lower_until ? lo : nullptr;
     o.sym = sym;
+    o.backwards = !o.backwards;
     r = launch_form<GRAM>(o, st);
     if (r != FS_OK) return r;
     o.a = sym;
     o.sym = poly;
+    o.backwards = !o.backwards;
     r = launch_form<SQUARE>(o, st);
     if (r != FS_OK) return r;
+    o.backwards = !o.backwards;
     r = i + 1 < steps ? launch_form<APPLY>(o, st) : launch_form<LAST>(o, st);
     __half* t = hi;
     hi = other;
