@@ -5,14 +5,22 @@
 //
 // Both passes are bound by memory: x is read and y written, then x and dy read and dx written. A row lies in the registers of
 // a group of warps (the mean first, then the squares of the differences from it: one read, and no cancellation), groups walk
-// over the rows with the next row's loads under way, and in the backward pass each thread adds what its columns contribute
+// over the rows with several rows' loads under way, and in the backward pass each thread adds what its columns contribute
 // to dw and db over all its rows. A CTA leaves one row of sums, which a second launch adds in a fixed order, so every run gives
 // the same bits. Sums are fp32; y, dx, dw and db are rounded once.
 #include "fs_experts.cuh"
+#include "fs_ptx.cuh"
 
 namespace fs {
 namespace ex {
 namespace {
+
+using tc::add2;
+using tc::fma2;
+using tc::mul2;
+using tc::pk;
+using tc::u64;
+using tc::upk;
 
 constexpr int kMaxNormThreads = 512;
 constexpr int kLongThreads = 512;  // of rows that registers do not hold
@@ -35,8 +43,8 @@ __device__ __forceinline__ float warp_sum(float v) {
 }
 __device__ __forceinline__ void group_barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
-// The sum over a group's warps of one or two values, the same bits in every thread; slot: 2 x 16 floats of this group that the
-// call before this one did not use.
+// The sum over a group's warps of one or two values, the same bits in every thread; slot: N x 16 floats of this group, zeros where there
+// is no warp, that the call before this one did not use.
 template <int N>
 __device__ __forceinline__ void group_sum(float (&v)[N], float* slot, int warps, int barrier) {
   const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % warps;
@@ -48,202 +56,313 @@ __device__ __forceinline__ void group_sum(float (&v)[N], float* slot, int warps,
     for (int i = 0; i < N; ++i) slot[16 * i + warp] = v[i];
   group_barrier(barrier, warps * 32);
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = warp_sum(lane < warps ? slot[16 * i + lane] : 0.f);
+  for (int i = 0; i < N; ++i) {
+    const float4 p = *reinterpret_cast<const float4*>(slot + 16 * i);
+    v[i] = (p.x + p.y) + (p.z + p.w);
+    if (warps > 4) {
+      const float4 q = *reinterpret_cast<const float4*>(slot + 16 * i + 4);
+      v[i] += (q.x + q.y) + (q.z + q.w);
+    }
+    if (warps > 8) {
+      const float4 q = *reinterpret_cast<const float4*>(slot + 16 * i + 8), u = *reinterpret_cast<const float4*>(slot + 16 * i + 12);
+      v[i] += ((q.x + q.y) + (q.z + q.w)) + ((u.x + u.y) + (u.z + u.w));
+    }
+  }
+}
+// Pairs of a pack's values (V = 1: the value and 0).
+template <typename T, int V>
+__device__ __forceinline__ void pairs(const Pack<T, V>& q, u64 (&p)[(V + 1) / 2]) {
+  if constexpr (V == 1) {
+    p[0] = pk(to_f32(*reinterpret_cast<const T*>(&q.w[0])), 0.f);
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) p[i] = pk(__uint_as_float(q.w[2 * i]), __uint_as_float(q.w[2 * i + 1]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      float lo, hi;
+      two_f32(q.w[i], lo, hi, T());
+      p[i] = pk(lo, hi);
+    }
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_pairs(T* to, const u64 (&p)[(V + 1) / 2]) {
+  float v[V + 1];
+#pragma unroll
+  for (int i = 0; i < (V + 1) / 2; ++i) upk(p[i], v[2 * i], v[2 * i + 1]);
+  float out[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) out[i] = v[i];
+  store_f32<T, V>(to, out);
+}
+__device__ __forceinline__ float both(u64 v) {
+  float lo, hi;
+  upk(v, lo, hi);
+  return lo + hi;
 }
 
-// N values of w or b (null: `other`) from column c on, of which those past F count as 0.
+// V values of w or b (null: `other`) from column c on, inside of F.
 template <typename W, int V>
-__device__ __forceinline__ void columns(const void* p, int c, int F, float other, float (&v)[V]) {
-  if (c >= F) {
+__device__ __forceinline__ void columns(const void* p, int c, float other, u64 (&v)[(V + 1) / 2]) {
+  if (!p) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = 0.f;
-  } else if (!p) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = other;
+    for (int i = 0; i < (V + 1) / 2; ++i) v[i] = pk(other, other);
   } else {
-    unpack<W, V>(read_only<W, V>(static_cast<const W*>(p) + c), v);
+    pairs<W, V>(read_only<W, V>(static_cast<const W*>(p) + c), v);
   }
 }
 
-// One row per group of a.group threads, V values to a load, NV loads a thread. V > 1: rows, weights and F are aligned to it.
+// Values of rows to come, in shared memory that only the thread itself reads: S - 1 rows are under way without a register, and
+// no thread waits for another one. Loads of V values; those of two bytes are not to be had asynchronously and are waited for.
+template <typename T, int V>
+__device__ __forceinline__ void fetch(Pack<T, V>* to, const T* from) {
+  constexpr int kBytes = V * sizeof(T);
+  const uint32_t at = (uint32_t)__cvta_generic_to_shared(to);
+  if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
+  else if constexpr (kBytes == 4) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at), "l"(from) : "memory");
+  else *to = read_only<T, V>(from);
+}
+__device__ __forceinline__ void fetch_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>  // all but the last LEFT rows
+__device__ __forceinline__ void fetch_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+
+constexpr int kForwardStages = 6;  // rows under way of the forward pass, with the one that is worked on
+
+// One row per group of a.group threads, V values to a load, NV loads a thread. V > 1: rows, weights and F are aligned to it. Up to 16 values
+// of a thread, w and b stay in registers (from L1 for every row of 2048, they took as long as the row itself) and several rows are under way;
+// above that a row's loads are under way all at once.
 template <typename T, typename W, int V, int NV>
-__global__ void __launch_bounds__(kMaxNormThreads) norm_kernel(const NormArgs a) {
-  constexpr bool kHold = V * NV <= 16;  // w and b stay in registers
-  __shared__ float slots[2][16][32];
-  const int groups = blockDim.x / a.group, g = threadIdx.x / a.group, t = threadIdx.x % a.group, warps = a.group / 32;
-  float w[kHold ? NV : 1][V], b[kHold ? NV : 1][V];
+__global__ void __launch_bounds__(V * NV <= (V > 1 ? 16 : 8) ? 256 : kMaxNormThreads, V * NV <= (V > 1 ? 16 : 8) ? 3 : 1) norm_kernel(const NormArgs a) {
+  constexpr bool kHold = V * NV <= (V > 1 ? 16 : 8);
+  constexpr int P = (V + 1) / 2, S = kHold ? kForwardStages : 1;
+  __shared__ __align__(16) float slots[2][16][16];
+  extern __shared__ __align__(16) uint8_t raw[];
+  Pack<T, V>* ring = reinterpret_cast<Pack<T, V>*>(raw) + threadIdx.x;  // kHold: [S][NV][threads]
+  const int group = a.group, groups = blockDim.x / group, g = threadIdx.x / group, t = threadIdx.x % group, warps = group / 32;
+  u64 w[kHold ? NV : 1][P], b[kHold ? NV : 1][P];
   if (kHold)
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      columns<W, V>(a.w, (i * a.group + t) * V, a.F, 1.f, w[i]);
-      columns<W, V>(a.b, (i * a.group + t) * V, a.F, 0.f, b[i]);
-    }
-  const float per = 1.f / a.F;
-  Pack<T, V> next[NV];
-  auto load = [&](long long row) {
-    const T* x = static_cast<const T*>(a.x) + row * a.ldx;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * a.group + t) * V;
-      if (c < a.F) next[i] = read_only<T, V>(x + c);
-    }
-  };
-  const long long stride = (long long)gridDim.x * groups;
-  long long row = (long long)blockIdx.x * groups + g;
-  if (row < a.rows) load(row);
-  for (; row < a.rows; row += stride) {
-    float x[NV][V], s[1] = {0.f};
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      unpack<T, V>(next[i], x[i]);
-      const bool in = (i * a.group + t) * V < a.F;
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        x[i][j] = in ? x[i][j] : 0.f;
-        s[0] += x[i][j];
+    for (int i = 0; i < NV; ++i)
+      if ((i * group + t) * V < a.F) {
+        columns<W, V>(a.w, (i * group + t) * V, 1.f, w[i]);
+        columns<W, V>(a.b, (i * group + t) * V, 0.f, b[i]);
       }
+  if (warps > 1) {
+    for (int i = threadIdx.x; i < 512; i += blockDim.x) (&slots[0][0][0])[i] = 0.f;
+    __syncthreads();
+  }
+  const float per = 1.f / a.F;
+  const long long stride = (long long)gridDim.x * groups;
+  long long row = (long long)blockIdx.x * groups + g, ahead = row;
+  auto ask = [&](int s) {
+    if (ahead < a.rows) {
+      const T* x = static_cast<const T*>(a.x) + ahead * a.ldx + t * V;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if ((i * group + t) * V < a.F) fetch<T, V>(ring + (s * NV + i) * blockDim.x, x + i * group * V);
     }
-    if (row + stride < a.rows) load(row + stride);
+    ahead += stride;
+    fetch_commit();
+  };
+  if (kHold)
+    for (int s = 0; s < S - 1; ++s) ask(s);
+  for (int stage = 0; row < a.rows; row += stride, stage = stage + 1 == S ? 0 : stage + 1) {
+    Pack<T, V> q[NV];
+    if (kHold) {
+      ask(stage ? stage - 1 : S - 1);
+      fetch_wait<S - 1>();
+    }
+    const T* x = static_cast<const T*>(a.x) + row * a.ldx + t * V;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if ((i * group + t) * V < a.F) q[i] = kHold ? ring[(stage * NV + i) * blockDim.x] : read_only<T, V>(x + i * group * V);
+    u64 sum = 0ull;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      u64 p[P];
+      pairs<T, V>(q[i], p);
+      if ((i * group + t) * V < a.F)
+#pragma unroll
+        for (int j = 0; j < P; ++j) sum = add2(sum, p[j]);
+    }
+    float s[1] = {both(sum)};
     group_sum(s, slots[0][g], warps, 1 + g);
     const float mean = s[0] * per;
-    s[0] = 0.f;
+    const u64 less = pk(-mean, V == 1 ? 0.f : -mean);
+    sum = 0ull;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const bool in = (i * a.group + t) * V < a.F;
+      u64 p[P];
+      pairs<T, V>(q[i], p);
+      if ((i * group + t) * V < a.F)
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        x[i][j] -= mean;
-        s[0] = in ? fmaf(x[i][j], x[i][j], s[0]) : s[0];
-      }
+        for (int j = 0; j < P; ++j) {
+          const u64 d = add2(p[j], less);
+          sum = fma2(d, d, sum);
+        }
     }
+    s[0] = both(sum);
     group_sum(s, slots[1][g], warps, 1 + g);
     const float r = 1.f / sqrtf(fmaf(s[0], per, a.eps));
     if (a.mean && t == 0) {
       a.mean[row] = mean;
       a.rstd[row] = r;
     }
+    const u64 r2 = pk(r, r);
     T* out = static_cast<T*>(a.out) + row * a.F;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * a.group + t) * V;
+      const int c = (i * group + t) * V;
+      if (c >= a.F) continue;
+      constexpr int kOne = kHold ? 1 : 0;
+      const int k = i * kOne;
+      u64 p[P];
+      pairs<T, V>(q[i], p);
       if (!kHold) {
-        columns<W, V>(a.w, c, a.F, 1.f, w[0]);
-        columns<W, V>(a.b, c, a.F, 0.f, b[0]);
+        columns<W, V>(a.w, c, 1.f, w[0]);
+        columns<W, V>(a.b, c, 0.f, b[0]);
       }
 #pragma unroll
-      for (int j = 0; j < V; ++j) x[i][j] = fmaf(x[i][j] * r, w[kHold ? i : 0][j], b[kHold ? i : 0][j]);
-      if (c < a.F) store_f32<T, V>(out + c, x[i]);
+      for (int j = 0; j < P; ++j) p[j] = fma2(mul2(add2(p[j], less), r2), w[k][j], b[k][j]);
+      store_pairs<T, V>(out + c, p);
     }
   }
 }
 
-// The gradients, from mean and rstd as the forward pass left them.
-template <typename T, typename W, int V, int NV>
-__global__ void __launch_bounds__(kMaxNormThreads) norm_grad_kernel(const NormArgs a) {
-  constexpr bool kHold = V * NV <= 16;
-  __shared__ float slots[2][16][32];
-  extern __shared__ float merge[];  // [groups - 1][2][F]
+// Rows under way, with the one that is worked on, by a thread's bytes of a row and its gradient: two CTAs of 96 KB to an SM, or one of 192 KB.
+__host__ __device__ constexpr int norm_stages(int bytes) { return bytes <= 64 ? 6 : bytes <= 128 ? 3 : bytes <= 256 ? 3 : 1; }
+
+// The gradients, from mean and rstd as the forward pass left them. SUMS: those to w and b as well; up to 16 values of a thread, of which w and what
+// both passes over them need stay in registers (read and unpacked again, they took a third of all instructions).
+template <typename T, typename W, int V, int NV, bool SUMS>
+__global__ void __launch_bounds__(256, SUMS ? 2 : 1) norm_grad_kernel(const NormArgs a) {
+  constexpr int P = (V + 1) / 2, S = norm_stages(2 * NV * (int)sizeof(Pack<T, V>));
+  __shared__ __align__(16) float slots[2][8][32];
+  extern __shared__ __align__(16) uint8_t raw[];
+  Pack<T, V>* ring = reinterpret_cast<Pack<T, V>*>(raw) + threadIdx.x;  // [S][2][NV][threads]; in the end the groups' sums
   const int groups = blockDim.x / a.group, g = threadIdx.x / a.group, t = threadIdx.x % a.group, warps = a.group / 32;
-  float w[kHold ? NV : 1][V], dw[NV][V], db[NV][V];
+  u64 dw[SUMS ? NV : 1][P], db[SUMS ? NV : 1][P];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    if (kHold) columns<W, V>(a.w, (i * a.group + t) * V, a.F, 1.f, w[i]);
+  for (int i = 0; i < (SUMS ? NV : 1); ++i)
 #pragma unroll
-    for (int j = 0; j < V; ++j) dw[i][j] = db[i][j] = 0.f;
+    for (int j = 0; j < P; ++j) dw[i][j] = db[i][j] = 0ull;
+  u64 w[SUMS ? NV : 1][P];
+  if (SUMS)
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if ((i * a.group + t) * V < a.F) columns<W, V>(a.w, (i * a.group + t) * V, 1.f, w[i]);
+  if (warps > 1) {
+    for (int i = threadIdx.x; i < 512; i += blockDim.x) (&slots[0][0][0])[i] = 0.f;
+    __syncthreads();
   }
   const float per = 1.f / a.F;
-  Pack<T, V> nx[NV], ng[NV];
-  float nmean = 0.f, nr = 0.f;
-  auto load = [&](long long row) {
-    const T *x = static_cast<const T*>(a.x) + row * a.ldx, *dy = static_cast<const T*>(a.dy) + row * a.lddy;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * a.group + t) * V;
-      if (c < a.F) {
-        nx[i] = read_only<T, V>(x + c);
-        ng[i] = read_only<T, V>(dy + c);
-      }
-    }
-    nmean = __ldg(a.mean + row);
-    nr = __ldg(a.rstd + row);
-  };
   const long long stride = (long long)gridDim.x * groups;
-  long long row = (long long)blockIdx.x * groups + g;
-  if (row < a.rows) load(row);
-  for (int turn = 0; row < a.rows; row += stride, turn ^= 1) {
-    Pack<T, V> qx[NV], qg[NV];
-    const float mean = nmean, r = nr;
-    float s[2] = {0.f, 0.f};
+  long long row = (long long)blockIdx.x * groups + g, ahead = row;
+  auto ask = [&](int s) {
+    if (ahead < a.rows) {
+      const T *x = static_cast<const T*>(a.x) + ahead * a.ldx + t * V, *dy = static_cast<const T*>(a.dy) + ahead * a.lddy + t * V;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      qx[i] = nx[i];
-      qg[i] = ng[i];
-    }
-    if (row + stride < a.rows) load(row + stride);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * a.group + t) * V;
-      float x[V], dy[V];
-      unpack<T, V>(qx[i], x);
-      unpack<T, V>(qg[i], dy);
-      if (!kHold) columns<W, V>(a.w, c, a.F, 1.f, w[0]);
-      if (c < a.F)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float n = (x[j] - mean) * r, u = dy[j] * w[kHold ? i : 0][j];
-          s[0] += u;
-          s[1] = fmaf(u, n, s[1]);
-          dw[i][j] = fmaf(dy[j], n, dw[i][j]);
-          db[i][j] += dy[j];
+      for (int i = 0; i < NV; ++i)
+        if ((i * a.group + t) * V < a.F) {
+          fetch<T, V>(ring + (s * 2 * NV + i) * blockDim.x, x + i * a.group * V);
+          fetch<T, V>(ring + ((s * 2 + 1) * NV + i) * blockDim.x, dy + i * a.group * V);
         }
     }
-    group_sum(s, slots[turn][g], warps, 1 + g);
-    const float m1 = s[0] * per, m2 = s[1] * per;
+    ahead += stride;
+    fetch_commit();
+  };
+  for (int s = 0; s < S - 1; ++s) ask(s);
+  float next_mean = 0.f, next_r = 0.f;
+  if (row < a.rows) {
+    next_mean = __ldg(a.mean + row);
+    next_r = __ldg(a.rstd + row);
+  }
+  for (int s = 0, turn = 0; row < a.rows; row += stride, s = s + 1 == S ? 0 : s + 1, turn ^= 1) {
+    ask(s ? s - 1 : S - 1);
+    const float r = next_r;
+    const u64 r2 = pk(r, r), shift = pk(-next_mean * r, V == 1 ? 0.f : -next_mean * r);  // n = x r + shift
+    if (row + stride < a.rows) {
+      next_mean = __ldg(a.mean + row + stride);
+      next_r = __ldg(a.rstd + row + stride);
+    }
+    fetch_wait<S - 1>();
+    const Pack<T, V>*px = ring + s * 2 * NV * blockDim.x, *pg = px + NV * blockDim.x;
+    u64 su = 0ull, sn = 0ull, n[SUMS ? NV : 1][P], u[SUMS ? NV : 1][P];
+    auto read = [&](int i, int k) {  // n, and dy into u
+      pairs<T, V>(px[i * blockDim.x], n[k]);
+      pairs<T, V>(pg[i * blockDim.x], u[k]);
+      if (!SUMS) columns<W, V>(a.w, (i * a.group + t) * V, 1.f, w[0]);
+#pragma unroll
+      for (int j = 0; j < P; ++j) n[k][j] = fma2(n[k][j], r2, shift);
+    };
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      constexpr int kOne = SUMS ? 1 : 0;
+      const int k = i * kOne;
+      if ((i * a.group + t) * V >= a.F) continue;
+      read(i, k);
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        if (SUMS) {
+          dw[k][j] = fma2(u[k][j], n[k][j], dw[k][j]);
+          db[k][j] = add2(db[k][j], u[k][j]);
+        }
+        const u64 v = mul2(u[k][j], w[k][j]);
+        su = add2(su, v);
+        sn = fma2(v, n[k][j], sn);
+      }
+    }
+    if (!a.out) continue;
+    float sum[2] = {both(su), both(sn)};
+    group_sum(sum, slots[turn][g], warps, 1 + g);
+    const u64 m1 = pk(-sum[0] * per, -sum[0] * per), m2 = pk(-sum[1] * per, -sum[1] * per);
     T* out = static_cast<T*>(a.out) + row * a.F;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * a.group + t) * V;
-      float x[V], dy[V];
-      unpack<T, V>(qx[i], x);
-      unpack<T, V>(qg[i], dy);
-      if (!kHold) columns<W, V>(a.w, c, a.F, 1.f, w[0]);
+      constexpr int kOne = SUMS ? 1 : 0;
+      const int c = (i * a.group + t) * V, k = i * kOne;
+      if (c >= a.F) continue;
+      if (!SUMS) read(i, 0);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float n = (x[j] - mean) * r;
-        x[j] = r * (fmaf(dy[j], w[kHold ? i : 0][j], -m1) - n * m2);
-      }
-      if (c < a.F && a.out) store_f32<T, V>(out + c, x);
+      for (int j = 0; j < P; ++j) n[k][j] = mul2(r2, fma2(m2, n[k][j], fma2(u[k][j], w[k][j], m1)));
+      store_pairs<T, V>(out + c, n[k]);
     }
   }
-  if (!a.sums) return;
+  if (!SUMS) return;
+  fetch_wait<0>();
+  float* merge = reinterpret_cast<float*>(raw);  // [groups - 1][2][F]
   __syncthreads();
+  auto each = [&](auto&& f) {  // f(column, its dw, its db)
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int c = (i * a.group + t) * V + j;
-      if (g > 0 && c < a.F) {
-        merge[(size_t)(g - 1) * 2 * a.F + c] = dw[i][j];
-        merge[(size_t)(g - 1) * 2 * a.F + a.F + c] = db[i][j];
+      for (int j = 0; j < P; ++j) {
+        const int c = (i * a.group + t) * V + 2 * j;
+        float w0, w1, b0, b1;
+        upk(dw[i][j], w0, w1);
+        upk(db[i][j], b0, b1);
+        if (c < a.F) f(c, w0, b0);
+        if (V > 1 && c < a.F) f(c + 1, w1, b1);
       }
+  };
+  each([&](int c, float w, float b) {
+    if (g > 0) {
+      merge[(size_t)(g - 1) * 2 * a.F + c] = w;
+      merge[(size_t)(g - 1) * 2 * a.F + a.F + c] = b;
     }
+  });
   __syncthreads();
   if (g > 0) return;
   float* sums = a.sums + (size_t)blockIdx.x * 2 * a.F;
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int c = (i * a.group + t) * V + j;
-      if (c < a.F) {
-        for (int k = 0; k < groups - 1; ++k) {
-          dw[i][j] += merge[(size_t)k * 2 * a.F + c];
-          db[i][j] += merge[(size_t)k * 2 * a.F + a.F + c];
-        }
-        sums[c] = dw[i][j];
-        sums[a.F + c] = db[i][j];
-      }
+  each([&](int c, float w, float b) {
+    for (int k = 0; k < groups - 1; ++k) {
+      w += merge[(size_t)k * 2 * a.F + c];
+      b += merge[(size_t)k * 2 * a.F + a.F + c];
     }
+    sums[c] = w;
+    sums[a.F + c] = b;
+  });
 }
 
 // dw and db from the CTAs' sums: 32 columns of [2][F] to a block, its eight warps an eighth of the CTAs each.
@@ -314,96 +433,186 @@ __global__ void __launch_bounds__(kLongThreads) norm_long_grad_kernel(const Norm
     }
   }
 }
-// Column sums of long rows: a CTA takes 256 columns and every gridDim.y-th row.
-template <typename T>
+// Column sums by themselves, where a row is too long for its threads to keep them: a warp takes 32 V columns, a CTA's eight warps every
+// 8 gridDim.y-th row each.
+template <typename T, int V>
 __global__ void __launch_bounds__(256) norm_columns_kernel(const NormArgs a) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= a.F) return;
-  float dw = 0.f, db = 0.f;
-#pragma unroll 4
-  for (long long row = blockIdx.y; row < a.rows; row += gridDim.y) {
-    const float dy = to_f32(static_cast<const T*>(a.dy)[row * a.lddy + c]);
-    dw = fmaf(dy, (to_f32(static_cast<const T*>(a.x)[row * a.ldx + c]) - a.mean[row]) * a.rstd[row], dw);
-    db += dy;
+  __shared__ float part[8][2][32 * V];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = (blockIdx.x * 32 + lane) * V;
+  float dw[V], db[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) dw[j] = db[j] = 0.f;
+  if (c < a.F) {
+    constexpr int kDeep = 4;
+    const long long stride = 8ll * gridDim.y;
+    for (long long row = blockIdx.y * 8 + warp; row < a.rows; row += stride * kDeep) {
+      Pack<T, V> px[kDeep], pg[kDeep];
+      float r[kDeep], shift[kDeep];
+#pragma unroll
+      for (int d = 0; d < kDeep; ++d) {
+        const long long at = row + d * stride;
+        if (at >= a.rows) continue;
+        px[d] = read_only<T, V>(static_cast<const T*>(a.x) + at * a.ldx + c);
+        pg[d] = read_only<T, V>(static_cast<const T*>(a.dy) + at * a.lddy + c);
+        r[d] = __ldg(a.rstd + at);
+        shift[d] = -__ldg(a.mean + at) * r[d];
+      }
+#pragma unroll
+      for (int d = 0; d < kDeep; ++d) {
+        if (row + d * stride >= a.rows) continue;
+        float x[V], dy[V];
+        unpack<T, V>(px[d], x);
+        unpack<T, V>(pg[d], dy);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          dw[j] = fmaf(dy[j], fmaf(x[j], r[d], shift[d]), dw[j]);
+          db[j] += dy[j];
+        }
+      }
+    }
   }
-  float* sums = a.sums + (size_t)blockIdx.y * 2 * a.F;
-  sums[c] = dw;
-  sums[a.F + c] = db;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    part[warp][0][lane * V + j] = dw[j];
+    part[warp][1][lane * V + j] = db[j];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 64 * V; i += 256) {
+    const int which = i / (32 * V), k = i - which * 32 * V, column = blockIdx.x * 32 * V + k;
+    if (column >= a.F) continue;
+    float s = part[0][which][k];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) s += part[j][which][k];
+    a.sums[(size_t)blockIdx.y * 2 * a.F + (size_t)which * a.F + column] = s;
+  }
 }
 
 // ------------------------------------------------------------------ host side
 struct NormPlan {
-  int vec, loads;    // values to a load, loads of a thread; 0: rows too long
+  int vec, values;  // values to a load and of a thread; 0 values: rows too long
   int group, block;  // threads of a row and of a CTA
-  int ctas;          // of the backward pass, each leaving sums
+  int ctas;          // of the backward pass's sums
 };
 
-constexpr int kCtasOfSums = 296;
+constexpr int kMostSums = 592;  // rows of sums
 
-// 16-byte loads where all rows and the weights allow it, else single values.
-NormPlan plan_norm(int rows, int F, int type, int w_type, bool aligned16) {
+// 16-byte loads where all rows and the weights allow it, else single values. Forward: 16 values of a thread, 8 for short or few rows, 64
+// (single values: 16) where a row is too long for 256 threads.
+NormPlan plan_forward(int rows, int F, int type, bool aligned16) {
   NormPlan p{};
-  const int wide = type == FS_TYPE_F32 ? 4 : 8;
-  p.vec = aligned16 && F % wide == 0 ? wide : 1;
-  const int per = p.vec > 1 ? 8 / p.vec * p.vec : 4;  // values of a thread, as few as one row in 512 threads allows
-  int values = per;
-  while (values <= (p.vec > 1 ? 32 : 16) && (long long)values * kMaxNormThreads < F) values *= 2;
-  if (values > (p.vec > 1 ? 32 : 16)) {
-    p.loads = 0;
-    p.vec = 1;
+  p.vec = aligned16 && F % (type == FS_TYPE_F32 ? 4 : 8) == 0 ? (type == FS_TYPE_F32 ? 4 : 8) : 1;
+  const int few = p.vec > 1 ? 8 : 4;
+  int values = 2 * few;
+  if (F <= few * 32 || (rows < 148 * 4 && F <= few * 256)) values = few;
+  else if (values * 256 < F) values = p.vec > 1 ? 64 : 16;
+  if ((long long)values * kMaxNormThreads < F) {
     p.group = p.block = kLongThreads;
-    p.ctas = rows < kCtasOfSums ? rows : kCtasOfSums;
     return p;
   }
-  p.loads = values / p.vec;
+  p.values = values;
   p.group = (F + values * 32 - 1) / (values * 32) * 32;
-  const int groups = kMaxNormThreads / p.group;
-  p.block = p.group * (groups > 8 ? 8 : groups);
-  const long long want = ((long long)rows + p.block / p.group - 1) / (p.block / p.group);
-  p.ctas = want < kCtasOfSums ? (int)want : kCtasOfSums;
-  (void)w_type;
+  p.block = p.group < 256 ? 256 / p.group * p.group : p.group;
+  return p;
+}
+// Backward: 16 values of a thread with the sums of their columns, or 8 for short rows; from 4096 values (single values: 2048) on 32 without sums.
+NormPlan plan_backward(int rows, int F, int type, bool aligned16) {
+  NormPlan p{};
+  p.vec = aligned16 && F % (type == FS_TYPE_F32 ? 4 : 8) == 0 ? (type == FS_TYPE_F32 ? 4 : 8) : 1;
+  const int most = p.vec > 1 ? 16 : 8;
+  int values = p.vec > 1 ? 8 : 4;
+  while (values < most && values * 32 < F) values *= 2;
+  const bool keeps = values * 256 >= F;
+  if (keeps) {
+    p.values = values;
+    p.group = (F + values * 32 - 1) / (values * 32) * 32;
+    p.block = 256 / p.group * p.group;
+    const long long want = ((long long)rows + p.block / p.group - 1) / (p.block / p.group), most_ctas = 2 * 148;
+    p.ctas = (int)(want < most_ctas ? want : most_ctas);
+    return p;
+  }
+  values = p.vec > 1 ? 64 : 16;
+  if (values * 256 >= F) {
+    p.values = values;
+    p.group = p.block = (F + values * 32 - 1) / (values * 32) * 32;
+  } else {
+    p.group = p.block = kLongThreads;
+  }
+  const int across = (F + 32 * p.vec - 1) / (32 * p.vec);
+  int down = (4 * 148 + across - 1) / across;
+  if (down > (rows + 7) / 8) down = (rows + 7) / 8;
+  p.ctas = down;
   return p;
 }
 
-template <typename T, typename W, int V, int NV>
-int launch_norm(const NormPlan& p, const NormArgs& a, bool grad, cudaStream_t st) {
-  const int groups = p.block / p.group;
-  if (!grad) {
-    long long grid = ((long long)a.rows + groups - 1) / groups;
-    if (grid > 148 * 4) grid = 148 * 4;
-    norm_kernel<T, W, V, NV><<<(unsigned)grid, p.block, 0, st>>>(a);
-  } else {
-    const size_t smem = a.sums ? (size_t)(groups - 1) * 2 * a.F * 4 : 0;
-    norm_grad_kernel<T, W, V, NV><<<p.ctas, p.block, smem, st>>>(a);
+template <typename K>
+int allow_smem(K kernel, size_t bytes, std::atomic<uint64_t>& allowed) {
+  if (bytes <= 40 * 1024) return FS_OK;  // with the static part below what needs no leave
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (e == cudaSuccess && !(allowed.load(std::memory_order_relaxed) & bit)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+    if (e == cudaSuccess) allowed.fetch_or(bit, std::memory_order_relaxed);
   }
+  return e == cudaSuccess ? FS_OK : report_error(FS_ERR_CUDA, cudaGetErrorString(e));
+}
+template <typename T, typename W, int V, int NV, bool SUMS>
+int launch_norm_grad(const NormPlan& p, const NormArgs& a, cudaStream_t st) {
+  static std::atomic<uint64_t> allowed{0};
+  const auto kernel = norm_grad_kernel<T, W, V, NV, SUMS>;
+  const int groups = p.block / p.group, most = 148 * 2;
+  const long long rows = ((long long)a.rows + groups - 1) / groups;
+  size_t smem = (size_t)norm_stages(2 * NV * (int)sizeof(Pack<T, V>)) * 2 * NV * p.block * sizeof(Pack<T, V>);
+  const size_t merge = (size_t)(groups - 1) * 2 * a.F * sizeof(float);
+  if (SUMS && merge > smem) smem = merge;
+  const int s = allow_smem(kernel, smem, allowed);
+  if (s != FS_OK) return s;
+  kernel<<<(unsigned)(SUMS ? p.ctas : rows < most ? rows : most), p.block, smem, st>>>(a);
   return launched(1);
+}
+template <typename T, typename W, int V, int NV>
+int launch_forward(const NormPlan& p, const NormArgs& a, cudaStream_t st) {
+  static std::atomic<uint64_t> allowed{0};
+  constexpr bool kHold = V * NV <= (V > 1 ? 16 : 8);
+  const int groups = p.block / p.group, most = kHold ? 3 * 148 : 8 * 148;
+  const long long grid = ((long long)a.rows + groups - 1) / groups;
+  const size_t smem = kHold ? (size_t)kForwardStages * NV * sizeof(Pack<T, V>) * p.block : 0;
+  const int s = allow_smem(norm_kernel<T, W, V, NV>, smem, allowed);
+  if (s != FS_OK) return s;
+  norm_kernel<T, W, V, NV><<<(unsigned)(grid < most ? grid : most), p.block, smem, st>>>(a);
+  return launched(1);
+}
+template <typename T, typename W, int V>
+int launch_backward(const NormPlan& p, const NormArgs& a, cudaStream_t st) {
+  constexpr int kShort = V > 1 ? 8 : 4, kLong = V > 1 ? 64 : 16;
+  if (p.values == kLong) return a.out ? launch_norm_grad<T, W, V, kLong / V, false>(p, a, st) : FS_OK;
+  if (p.values == kShort) return a.sums ? launch_norm_grad<T, W, V, kShort / V, true>(p, a, st) : launch_norm_grad<T, W, V, kShort / V, false>(p, a, st);
+  return a.sums ? launch_norm_grad<T, W, V, 2 * kShort / V, true>(p, a, st) : launch_norm_grad<T, W, V, 2 * kShort / V, false>(p, a, st);
 }
 template <typename T, typename W>
 int launch_typed(const NormPlan& p, const NormArgs& a, bool grad, cudaStream_t st) {
   constexpr int kWide = sizeof(T) == 4 ? 4 : 8;
-  if (p.loads == 0) {
+  if (p.values == 0) {
     const int grid = a.rows < 148 * 4 ? a.rows : 148 * 4;
-    if (!grad) {
-      norm_long_kernel<T, W><<<grid, kLongThreads, 0, st>>>(a);
-      return launched(1);
-    }
-    if (a.out) norm_long_grad_kernel<T, W><<<grid, kLongThreads, 0, st>>>(a);
-    int s = a.out ? launched(1) : FS_OK;
-    if (s == FS_OK && a.sums) {
-      norm_columns_kernel<T><<<dim3((a.F + 255) / 256, p.ctas), 256, 0, st>>>(a);
-      s = launched(1);
-    }
-    return s;
+    if (!grad) norm_long_kernel<T, W><<<grid, kLongThreads, 0, st>>>(a);
+    else if (a.out) norm_long_grad_kernel<T, W><<<grid, kLongThreads, 0, st>>>(a);
+    const int s = launched(!grad || a.out ? 1 : 0);
+    if (s != FS_OK || !grad) return s;
+  } else if (!grad) {
+    if (p.vec == 1)
+      return p.values == 4 ? launch_forward<T, W, 1, 4>(p, a, st) : p.values == 8 ? launch_forward<T, W, 1, 8>(p, a, st) : launch_forward<T, W, 1, 16>(p, a, st);
+    return p.values == 8    ? launch_forward<T, W, kWide, 8 / kWide>(p, a, st)
+           : p.values == 16 ? launch_forward<T, W, kWide, 16 / kWide>(p, a, st)
+                            : launch_forward<T, W, kWide, 64 / kWide>(p, a, st);
+  } else {
+    const int s = p.vec > 1 ? launch_backward<T, W, kWide>(p, a, st) : launch_backward<T, W, 1>(p, a, st);
+    if (s != FS_OK || p.values < (p.vec > 1 ? 64 : 16)) return s;
   }
-  const int values = p.vec * p.loads;
-  if (p.vec == 1) {
-    if (values == 4) return launch_norm<T, W, 1, 4>(p, a, grad, st);
-    if (values == 8) return launch_norm<T, W, 1, 8>(p, a, grad, st);
-    return launch_norm<T, W, 1, 16>(p, a, grad, st);
-  }
-  if (values == 8) return launch_norm<T, W, kWide, 8 / kWide>(p, a, grad, st);
-  if (values == 16) return launch_norm<T, W, kWide, 16 / kWide>(p, a, grad, st);
-  return launch_norm<T, W, kWide, 32 / kWide>(p, a, grad, st);
+  if (!a.sums) return FS_OK;
+  const dim3 grid((a.F + 32 * p.vec - 1) / (32 * p.vec), p.ctas);
+  if (p.vec > 1) norm_columns_kernel<T, kWide><<<grid, 256, 0, st>>>(a);
+  else norm_columns_kernel<T, 1><<<grid, 256, 0, st>>>(a);
+  return launched(1);
 }
 int launch_any(const NormPlan& p, const NormArgs& a, int type, int w_type, bool grad, cudaStream_t st) {
   if (type == FS_TYPE_F32) return launch_typed<float, float>(p, a, grad, st);
@@ -435,7 +644,7 @@ extern "C" {
 
 size_t fs_layer_norm_grad_bytes(int rows, int F) {
   if (rows < 1 || F < 1) return 0;
-  return (size_t)(rows < kCtasOfSums ? rows : kCtasOfSums) * 2 * F * sizeof(float);
+  return (size_t)(rows < kMostSums ? rows : kMostSums) * 2 * F * sizeof(float);
 }
 
 int fs_layer_norm(const void* x, int type, long long ldx, int rows, int F, const void* w, const void* b, int w_type, float eps,
@@ -446,7 +655,7 @@ int fs_layer_norm(const void* x, int type, long long ldx, int rows, int F, const
   const int bytes = type_bytes(type);
   NormArgs a{};
   a.x = x; a.ldx = ldx; a.w = w; a.b = b; a.out = y; a.mean = mean; a.rstd = rstd; a.rows = rows; a.F = F; a.eps = eps;
-  const NormPlan p = plan_norm(rows, F, type, w_type, wide_rows(x, ldx, bytes) && aligned(y, 16) && wide_weights(w) && wide_weights(b));
+  const NormPlan p = plan_forward(rows, F, type, wide_rows(x, ldx, bytes) && aligned(y, 16) && wide_weights(w) && wide_weights(b));
   a.group = p.group;
   return launch_any(p, a, type, w_type, false, static_cast<cudaStream_t>(stream));
 }
@@ -473,7 +682,7 @@ int fs_layer_norm_grad(const void* x, int type, long long ldx, int rows, int F, 
   NormArgs a{};
   a.x = x; a.ldx = ldx; a.w = w; a.dy = dy; a.lddy = lddy; a.out = dx; a.rows = rows; a.F = F;
   a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd); a.sums = sums ? static_cast<float*>(ws) : nullptr;
-  const NormPlan p = plan_norm(rows, F, type, w_type, wide_rows(x, ldx, bytes) && wide_rows(dy, lddy, bytes) && aligned(dx, 16) && wide_weights(w));
+  const NormPlan p = plan_backward(rows, F, type, wide_rows(x, ldx, bytes) && wide_rows(dy, lddy, bytes) && aligned(dx, 16) && wide_weights(w));
   a.group = p.group;
   const int r = launch_any(p, a, type, w_type, true, st);
   if (r != FS_OK || !sums) return r;
