@@ -70,8 +70,9 @@ __global__ void __launch_bounds__(256) squares_kernel(const T* g, long long g_ma
 // Tiles of 64 x 64 of G to both parts of X, transposed for a tall G; X [n, k], rows ldx apart. V values to a load of G.
 template <typename T, int V>
 __global__ void __launch_bounds__(256) begin_kernel(const T* g, long long g_matrix, long long g_row, int rows, int cols, const double* parts, int count,
-                                                    float eps, bool tall, __half* hi, __half* lo, long long ldx) {
+                                                    float eps, bool tall, __half* hi, __half* lo, long long ldx, unsigned* meeting) {
   __shared__ float tile[64][65];
+  if (blockIdx.x + blockIdx.y + blockIdx.z + threadIdx.x == 0) *meeting = 0u;
   const int b = blockIdx.z, r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
   constexpr int kLanes = 64 / V;  // to a row of the tile
 #pragma unroll
@@ -174,58 +175,87 @@ __device__ __forceinline__ uint4 load_chunk(uint32_t at) {
   return v;
 }
 
-template <int FORM, int CG, int BN>
-__global__ void __launch_bounds__(kThreadsO, 1)
-ortho_kernel(const OrthoArgs a, const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB) {
-  constexpr bool B_MN = FORM >= APPLY;
-  constexpr int BNC = BN / CG;  // columns whose operand this CTA fetches
-  constexpr uint32_t kA = 128 * 128, kB = BNC * 128, kStage = kA + kB, kHalf = 64 * 128, kColumns = 2 * BN;
-  static_assert(kColumns <= 512 && kStage % 1024 == 0 && BNC >= 64, "tile");
-  extern __shared__ uint8_t raw[];
-  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* staging = ring + (size_t)a.nstage * kStage;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(staging + kStageO);
-  const int FULL = 0, EMPTY = a.nstage, ACC_FULL = 2 * a.nstage, ACC_EMPTY = ACC_FULL + 2, DRAIN = ACC_EMPTY + 2;
-  uint32_t* slot = reinterpret_cast<uint32_t*>(bars + DRAIN + 1);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(slot + 1);
-  auto bar = [&](int i) { return smem_u32(bars + i); };
+// What the threads of a CTA share over the products of a launch, and how far they are: the same in every lane of a warp.
+struct OrthoPipe {
+  uint8_t *ring, *staging;
+  uint64_t* bars;
+  volatile int* abort_flag;
+  uint32_t tmem;
+  int nstage, warp, lane, rank;
+  int s;        // next stage
+  uint32_t ph;  // its phase
+  int tiles;    // that this CTA has done
+  int issued;   // stages that this CTA's loading thread has started
+  __device__ uint32_t bar(int i) const { return smem_u32(bars + i); }
+  __device__ int full() const { return 0; }
+  __device__ int empty() const { return nstage; }
+  __device__ int acc_full() const { return 2 * nstage; }
+  __device__ int acc_empty() const { return 2 * nstage + 2; }
+  __device__ int drain() const { return 2 * nstage + 4; }
+};
 
-  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int rank = CG == 2 ? (int)cta_rank() : 0;
-  const int first = blockIdx.x / CG, stride = gridDim.x / CG;
-  const int contraction = FORM == GRAM ? a.k : a.n, blocks = (contraction + 63) / 64;
-
-  if (warp == kGetWarp && lane == 0) {
-    for (int s = 0; s < a.nstage; ++s) {
-      mbar_init(bar(FULL + s), CG);  // in CTA 0: both CTAs' loads
-      mbar_init(bar(EMPTY + s), 1);
+template <int CG, int BN>
+__device__ __forceinline__ OrthoPipe ortho_begin(uint8_t* raw, int nstage) {
+  constexpr uint32_t kStage = 128 * 128 + BN / CG * 128, kColumns = 2 * BN;
+  static_assert(kColumns <= 512 && kStage % 1024 == 0 && BN / CG >= 64, "tile");
+  OrthoPipe p;
+  p.ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  p.staging = p.ring + (size_t)nstage * kStage;
+  p.bars = reinterpret_cast<uint64_t*>(p.staging + kStageO);
+  p.nstage = nstage;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(p.bars + p.drain() + 1);
+  p.abort_flag = reinterpret_cast<volatile int*>(slot + 1);
+  p.warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);
+  p.lane = threadIdx.x & 31;
+  p.rank = CG == 2 ? (int)cta_rank() : 0;
+  p.s = p.tiles = p.issued = 0;
+  p.ph = 0;
+  if (p.warp == kGetWarp && p.lane == 0) {
+    for (int s = 0; s < nstage; ++s) {
+      mbar_init(p.bar(p.full() + s), CG);  // in CTA 0: both CTAs' loads
+      mbar_init(p.bar(p.empty() + s), 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(bar(ACC_FULL + i), 1);
-      mbar_init(bar(ACC_EMPTY + i), kWriteWarps * CG);  // in CTA 0: all warps of the pair that write
+      mbar_init(p.bar(p.acc_full() + i), 1);
+      mbar_init(p.bar(p.acc_empty() + i), kWriteWarps * CG);  // in CTA 0: all warps of the pair that write
     }
-    mbar_init(bar(DRAIN), 1);
-    *abort_flag = 0;
+    mbar_init(p.bar(p.drain()), 1);
+    *p.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  } else if (warp == kMulWarp) {
+  } else if (p.warp == kMulWarp) {
     alloc_columns<CG>(smem_u32(slot), kColumns);
   }
   tc_fence_before();
   __syncthreads();
   if (CG == 2) cluster_sync_all();
   tc_fence_after();
-  const uint32_t tmem = *slot;
+  p.tmem = *slot;
+  return p;
+}
+
+// This CTA's tiles of one product.
+template <int FORM, int CG, int BN>
+__device__ __forceinline__ void ortho_product(const OrthoArgs& a, const CUtensorMap* mapA, const CUtensorMap* mapB, OrthoPipe& p) {
+  constexpr bool B_MN = FORM >= APPLY;
+  constexpr int BNC = BN / CG;  // columns whose operand this CTA fetches
+  constexpr uint32_t kA = 128 * 128, kB = BNC * 128, kStage = kA + kB, kHalf = 64 * 128;
+  uint8_t *const ring = p.ring, *const staging = p.staging;
+  volatile int* const abort_flag = p.abort_flag;
+  const uint32_t tmem = p.tmem;
+  const int warp = p.warp, lane = p.lane, rank = p.rank, FULL = p.full(), EMPTY = p.empty(), ACC_FULL = p.acc_full(), ACC_EMPTY = p.acc_empty();
+  auto bar = [&](int i) { return p.bar(i); };
+  const int first = blockIdx.x / CG, stride = gridDim.x / CG;
+  const int contraction = FORM == GRAM ? a.k : a.n, blocks = (contraction + 63) / 64;
   const TilesO<FORM, CG, BN> tiles(a);
   const long long total = tiles.total();
-  int issued = 0;
 
   if (warp == kGetWarp) {
     // ===================== loads =====================
     if (elect_one()) {
-      int s = 0;
-      uint32_t ph = 0;
-      bool ok = true;
+      int s = p.s;
+      uint32_t ph = p.ph;
+      bool ok = *abort_flag == 0;  // a CTA that has given up starts nothing more
       for (long long it = first; ok && it < total; it += stride) {
         int b, m0, n0;
         tiles.at(it, b, m0, n0);
@@ -236,15 +266,15 @@ ortho_kernel(const OrthoArgs a, const __grid_constant__ CUtensorMap mapA, const 
           }
           const uint32_t full = CG == 2 ? in_leader(bar(FULL + s)) : bar(FULL + s), dst = smem_u32(ring + (size_t)s * kStage);
           expect_at<CG>(full, kStage);
-          load_3d<CG>(dst, &mapA, kb * 64, m0 + rank * 128, b, full);
+          load_3d<CG>(dst, mapA, kb * 64, m0 + rank * 128, b, full);
           if (B_MN) {
 #pragma unroll
-            for (int c = 0; c < BNC / 64; ++c) load_3d<CG>(dst + kA + c * kHalf, &mapB, n0 + rank * BNC + c * 64, kb * 64, b, full);
+            for (int c = 0; c < BNC / 64; ++c) load_3d<CG>(dst + kA + c * kHalf, mapB, n0 + rank * BNC + c * 64, kb * 64, b, full);
           } else {
-            load_3d<CG>(dst + kA, &mapB, kb * 64, n0 + rank * BNC, b, full);
+            load_3d<CG>(dst + kA, mapB, kb * 64, n0 + rank * BNC, b, full);
           }
-          ++issued;
-          if (++s == a.nstage) {
+          ++p.issued;
+          if (++s == p.nstage) {
             s = 0;
             ph ^= 1;
           }
@@ -258,9 +288,9 @@ ortho_kernel(const OrthoArgs a, const __grid_constant__ CUtensorMap mapA, const 
       constexpr uint32_t idesc = (1u << 4) | ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(128 * CG >> 4) << 24);
       // a step of 16 contraction values: 32 bytes on, or 16 rows of 128 bytes; MN: the next 64 columns one half tile on
       constexpr uint32_t kStepB = (B_MN ? 16u * 128u : 32u) >> 4, kLeadB = B_MN ? kHalf >> 4 : 1u;
-      int s = 0, n = 0;
-      uint32_t ph = 0;
-      bool ok = true;
+      int s = p.s, n = p.tiles;
+      uint32_t ph = p.ph;
+      bool ok = *abort_flag == 0;  // a CTA that has given up starts nothing more
       for (long long it = first; ok && it < total; it += stride, ++n) {
         const int buf = n & 1;
         if (!mbar_wait(bar(ACC_EMPTY + buf), ((n >> 1) & 1) ^ 1, abort_flag)) break;
@@ -279,7 +309,7 @@ ortho_kernel(const OrthoArgs a, const __grid_constant__ CUtensorMap mapA, const 
             if (ks * 16 < left)
               mma_f16<CG>(tmem + buf * BN, pack_desc(al + ks * 2, kDescHi128), pack_desc(bl + ks * kStepB, kDescHi128), idesc, kb | ks);
           commit<CG>(bar(EMPTY + s));
-          if (++s == a.nstage) {
+          if (++s == p.nstage) {
             s = 0;
             ph ^= 1;
           }
@@ -307,11 +337,11 @@ ortho_kernel(const OrthoArgs a, const __grid_constant__ CUtensorMap mapA, const 
         const bool in = r < a.n && c < width;  // rows are padded to 16 bytes
 #pragma unroll
         for (int k = 0; k < kFrom; ++k)
-          ahead[k][i] = in && (k == 0 || a.lo) ? *reinterpret_cast<const uint4*>((FORM == SQUARE ? a.a : k ? a.lo : a.hi) + at) : make_uint4(0u, 0u, 0u, 0u);
+          ahead[k][i] = in && (k == 0 || a.lo) ? __ldcg(reinterpret_cast<const uint4*>((FORM == SQUARE ? a.a : k ? a.lo : a.hi) + at)) : make_uint4(0u, 0u, 0u, 0u);
       }
     };
-    int t = 0, b = 0, m0 = 0, n0 = 0;
-    bool lost = false;  // a wait of this CTA gave up: NaN from here on
+    int t = p.tiles, b = 0, m0 = 0, n0 = 0;
+    bool lost = *abort_flag != 0;  // a wait of this CTA gave up: NaN from here on
     if (first < total) {
       tiles.at(first, b, m0, n0);
       if (kFrom) ask(b, m0 + rank * 128 + q * 32, n0 + kCols * side);
@@ -321,7 +351,7 @@ ortho_kernel(const OrthoArgs a, const __grid_constant__ CUtensorMap mapA, const 
       int next_b = 0, next_m = 0, next_n = 0;
       if (it + stride < total) tiles.at(it + stride, next_b, next_m, next_n);
       if (!lost) {
-        lost = !__all_sync(0xffffffffu, wait_blocks(bar(ACC_FULL + buf), (t >> 1) & 1, abort_flag, blocks, a.limit));
+        lost = !__all_sync(0xffffffffu, wait_close(bar(ACC_FULL + buf), (t >> 1) & 1, abort_flag, a.limit ? a.limit + 4096ll * blocks : 0));
         tc_fence_after();
       }
 #pragma unroll 1
@@ -441,23 +471,34 @@ ortho_kernel(const OrthoArgs a, const __grid_constant__ CUtensorMap mapA, const 
       n0 = next_n;
     }
   }
+  // every lane goes on from here, whichever one did the work
+  const int done = first < total ? (int)((total - first + stride - 1) / stride) : 0;
+  const long long past = p.s + (long long)done * blocks;
+  p.ph ^= (uint32_t)(past / p.nstage) & 1u;
+  p.s = (int)(past % p.nstage);
+  p.tiles += done;
+}
+
+template <int CG, int BN>
+__device__ __forceinline__ void ortho_end(const OrthoPipe& p) {
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (*abort_flag) {  // nobody waits any more, and the flag does not change
-    if (warp == kMulWarp && rank == 0) {  // every product issued here ends before TMEM is freed
+  if (*p.abort_flag) {  // nobody waits any more, and the flag does not change
+    if (p.warp == kMulWarp && p.rank == 0) {  // every product issued here ends before TMEM is freed
       if (elect_one()) {
-        commit<CG>(bar(DRAIN));
-        mbar_wait_quiet(bar(DRAIN), 0);
+        commit<CG>(p.bar(p.drain()));
+        mbar_wait_quiet(p.bar(p.drain()), 0);
       }
       __syncwarp();
-    } else if (warp == kGetWarp) {
+    } else if (p.warp == kGetWarp) {
       // The copies in flight land before the CTA ends; those of the second CTA of a pair, which the first one counts, are
       // given a millisecond, hundreds of times what a copy takes.
       if (elect_one()) {
         const long long t0 = clock64();
-        if (rank == 0)
-          for (int j = issued > a.nstage ? issued - a.nstage : 0; j < issued; ++j) wait_landed(bar(FULL + j % a.nstage), (j / a.nstage) & 1, t0);
+        if (p.rank == 0)
+          for (int j = p.issued > p.nstage ? p.issued - p.nstage : 0; j < p.issued; ++j)
+            wait_landed(p.bar(p.full() + j % p.nstage), (j / p.nstage) & 1, t0);
         else
           while (clock64() - t0 < (1ll << 21)) {}
       }
@@ -466,8 +507,78 @@ ortho_kernel(const OrthoArgs a, const __grid_constant__ CUtensorMap mapA, const 
   }
   if (CG == 2) cluster_sync_all();
   tc_fence_after();
-  if (warp == kMulWarp) free_columns<CG>(tmem, kColumns);
-  if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_ortho_error, 1);
+  if (p.warp == kMulWarp) free_columns<CG>(p.tmem, 2 * BN);
+  if (threadIdx.x == 0 && *p.abort_flag) atomicExch(&g_ortho_error, 1);
+}
+
+template <int FORM, int CG, int BN>
+__global__ void __launch_bounds__(kThreadsO, 1)
+ortho_kernel(const OrthoArgs a, const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB) {
+  extern __shared__ uint8_t raw[];
+  OrthoPipe p = ortho_begin<CG, BN>(raw, a.nstage);
+  ortho_product<FORM, CG, BN>(a, &mapA, &mapB, p);
+  ortho_end<CG, BN>(p);
+}
+
+// All products of all steps in one launch, for small matrices, whose products take less than a launch: every CTA does its tiles of
+// one, then waits for the others (bounded; a cooperative launch, so that they are all there).
+struct OrthoChain {
+  int steps, lower_until;
+  __half *x[2], *lo, *sym, *poly;
+  unsigned* meeting;  // zero at the start
+};
+struct OrthoMaps {
+  CUtensorMap x128[2], x64[2], a128, a64, p128;  // boxes of 128 or 64 rows
+};
+constexpr int kChainBN = 64, kChainTiles = 2;  // columns of a tile, and tiles of a CTA
+
+// What this CTA has written is there for the loads of all others behind it: the CTA's barrier and one thread's release order all of its
+// writes, and a fence of the thread that releases and of the one that loads orders them before tensor loads (which go another way to
+// memory). The same fences by all threads took 3 us.
+__device__ __forceinline__ void ortho_meet(const OrthoPipe& p, unsigned* meeting, unsigned target) {
+  __syncthreads();
+  if (threadIdx.x == 0 && !*p.abort_flag) {
+    unsigned seen;
+    asm volatile("fence.proxy.async.global;" ::: "memory");
+    asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(meeting) : "memory");
+    const long long t0 = clock64();
+    do {
+      asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(meeting) : "memory");
+      if (seen < target && clock64() - t0 > kSpinLimit) *p.abort_flag = 1;
+    } while (seen < target && !*p.abort_flag);
+  }
+  __syncthreads();
+  if (p.warp == kGetWarp) asm volatile("fence.proxy.async.global;" ::: "memory");
+}
+
+__global__ void __launch_bounds__(kThreadsO, 1) ortho_chain_kernel(OrthoArgs a, const OrthoChain c, const __grid_constant__ OrthoMaps maps) {
+  extern __shared__ uint8_t raw[];
+  if (threadIdx.x < sizeof(OrthoMaps) / sizeof(CUtensorMap))
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<const CUtensorMap*>(&maps) + threadIdx.x) : "memory");
+  OrthoPipe p = ortho_begin<1, kChainBN>(raw, a.nstage);
+  unsigned target = 0;
+#pragma unroll 1
+  for (int i = 0; i < c.steps; ++i) {
+    const int from = i & 1;
+    a.hi = c.x[from];
+    a.lo = i < c.lower_until ? c.lo : nullptr;
+    a.hi_out = c.x[from ^ 1];
+    a.lo_out = i + 1 < c.lower_until ? c.lo : nullptr;
+    a.sym = c.sym;
+    ortho_product<GRAM, 1, kChainBN>(a, &maps.x128[from], &maps.x64[from], p);
+    ortho_meet(p, c.meeting, target += gridDim.x);
+    a.a = c.sym;
+    a.sym = c.poly;
+    ortho_product<SQUARE, 1, kChainBN>(a, &maps.a128, &maps.a64, p);
+    ortho_meet(p, c.meeting, target += gridDim.x);
+    if (i + 1 < c.steps) {
+      ortho_product<APPLY, 1, kChainBN>(a, &maps.p128, &maps.x64[from], p);
+      ortho_meet(p, c.meeting, target += gridDim.x);
+    } else {
+      ortho_product<LAST, 1, kChainBN>(a, &maps.p128, &maps.x64[from], p);
+    }
+  }
+  ortho_end<1, kChainBN>(p);
 }
 
 // ------------------------------------------------------------------ host side
@@ -527,6 +638,49 @@ int launch_ortho(OrthoArgs a, cudaStream_t st) {
   count_launches(1);
   return FS_OK;
 }
+// Whether all of it is one launch: tiles of 128 x 64, of which a CTA has few.
+bool chained(const OrthoArgs& a) {
+  const long long m = (a.n + 127) / 128, n = (a.k + kChainBN - 1) / kChainBN;
+  return m * n * a.batch <= kChainTiles * (long long)detail::free_ctas();
+}
+int launch_chain(OrthoArgs a, const OrthoChain& c, cudaStream_t st) {
+  OrthoMaps maps = {};
+  for (int i = 0; i < 2; ++i)
+    if (!encode_stack(&maps.x128[i], c.x[i], a.k, a.n, a.batch, a.ldx, 128) || !encode_stack(&maps.x64[i], c.x[i], a.k, a.n, a.batch, a.ldx, 64))
+      return report_error(FS_ERR_CUDA, "cuTensorMapEncodeTiled failed");
+  if (!encode_stack(&maps.a128, c.sym, a.n, a.n, a.batch, a.lda, 128) || !encode_stack(&maps.a64, c.sym, a.n, a.n, a.batch, a.lda, 64) ||
+      !encode_stack(&maps.p128, c.poly, a.n, a.n, a.batch, a.lda, 128))
+    return report_error(FS_ERR_CUDA, "cuTensorMapEncodeTiled failed");
+  constexpr size_t kStage = 128 * 128 + kChainBN * 128, fixed = 1024 + kStageO + 8 * (2 * 12 + 5) + 8;
+  a.nstage = (int)((kSmemMax - fixed) / kStage);
+  static_assert(fixed + 6 * kStage >= (size_t)kSmemMin && (kSmemMax - fixed) / kStage <= 12 && (kSmemMax - fixed) / kStage >= 6, "shared memory");
+  static std::atomic<uint64_t> allowed{0};  // devices on which the kernel may take all shared memory
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (e == cudaSuccess && !(allowed.load(std::memory_order_relaxed) & bit)) {
+    e = cudaFuncSetAttribute(ortho_chain_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
+    if (e == cudaSuccess) allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
+  if (e != cudaSuccess) return report_error(FS_ERR_CUDA, cudaGetErrorString(e));
+  const long long most = (a.n + 127) / 128 * ((a.k + kChainBN - 1) / kChainBN) * a.batch;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(most < detail::free_ctas() ? most : detail::free_ctas()));
+  cfg.blockDim = dim3(kThreadsO);
+  cfg.dynamicSmemBytes = fixed + a.nstage * kStage;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeCooperative;
+  attr.val.cooperative = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  g_ortho_launched.store(true, std::memory_order_relaxed);
+  e = cudaLaunchKernelEx(&cfg, ortho_chain_kernel, a, c, maps);
+  if (e != cudaSuccess) return report_error(FS_ERR_CUDA, cudaGetErrorString(e));
+  count_launches(1);
+  return FS_OK;
+}
+
 template <int FORM>
 int launch_form(const OrthoArgs& a, cudaStream_t st) {
   const int ctas = detail::free_ctas();
@@ -541,7 +695,7 @@ int launch_form(const OrthoArgs& a, cudaStream_t st) {
 
 template <typename T>
 int begin(const void* g, long long g_matrix, long long g_row, int batch, int rows, int cols, double* parts, float eps, bool tall, __half* hi, __half* lo,
-          long long ldx, cudaStream_t st) {
+          long long ldx, unsigned* meeting, cudaStream_t st) {
   constexpr int kWide = 16 / sizeof(T);
   const bool wide = aligned(g, 16) && g_matrix % kWide == 0 && g_row % kWide == 0 && cols % kWide == 0;
   const int want = (rows + 7) / 8, count = want < kNormParts ? want : kNormParts;
@@ -553,10 +707,10 @@ int begin(const void* g, long long g_matrix, long long g_row, int batch, int row
     const dim3 over(count, nb), tiles((cols + 63) / 64, (rows + 63) / 64, nb);
     if (wide) {
       squares_kernel<T, kWide><<<over, 256, 0, st>>>(from, g_matrix, g_row, rows, cols, sums);
-      begin_kernel<T, kWide><<<tiles, 256, 0, st>>>(from, g_matrix, g_row, rows, cols, sums, count, eps, tall, hi + at, lo + at, ldx);
+      begin_kernel<T, kWide><<<tiles, 256, 0, st>>>(from, g_matrix, g_row, rows, cols, sums, count, eps, tall, hi + at, lo + at, ldx, meeting);
     } else {
       squares_kernel<T, 1><<<over, 256, 0, st>>>(from, g_matrix, g_row, rows, cols, sums);
-      begin_kernel<T, 1><<<tiles, 256, 0, st>>>(from, g_matrix, g_row, rows, cols, sums, count, eps, tall, hi + at, lo + at, ldx);
+      begin_kernel<T, 1><<<tiles, 256, 0, st>>>(from, g_matrix, g_row, rows, cols, sums, count, eps, tall, hi + at, lo + at, ldx, meeting);
     }
   }
   return launched(2);
@@ -572,7 +726,7 @@ OrthoSpace ortho_space(int batch, int rows, int cols) {
   s.x = round((size_t)batch * n * round(k, 8) * 2, 256);
   s.a = round((size_t)batch * n * round(n, 8) * 2, 256);
   s.parts = round((size_t)batch * kNormParts * sizeof(double), 256);
-  s.all = 3 * s.x + 2 * s.a + s.parts;
+  s.all = 3 * s.x + 2 * s.a + s.parts + 256;  // and the word of meetings
   return s;
 }
 
@@ -624,6 +778,7 @@ int fs_orthogonalize(const void* g, int type, long long g_matrix, long long g_ro
   __half *hi = reinterpret_cast<__half*>(p), *other = reinterpret_cast<__half*>(p + space.x), *lo = reinterpret_cast<__half*>(p + 2 * space.x);
   __half *sym = reinterpret_cast<__half*>(p + 3 * space.x), *poly = reinterpret_cast<__half*>(p + 3 * space.x + space.a);
   double* parts = reinterpret_cast<double*>(p + 3 * space.x + 2 * space.a);
+  unsigned* meeting = reinterpret_cast<unsigned*>(p + 3 * space.x + 2 * space.a + space.parts);
   OrthoArgs o{};
   o.batch = batch;
   o.n = tall ? cols : rows;
@@ -636,14 +791,18 @@ int fs_orthogonalize(const void* g, int type, long long g_matrix, long long g_ro
   const int inner = tall ? o.n : o.k;  // values of a row of the result
   o.out_bytes = aligned(out, 16) && inner % 8 == 0 ? 16 : aligned(out, 4) && inner % 2 == 0 ? 4 : 2;
   o.limit = product_limit();
-  int r = type == FS_TYPE_F32  ? begin<float>(g, g_matrix, g_row, batch, rows, cols, parts, eps, tall, hi, lo, o.ldx, st)
-          : type == FS_TYPE_F16 ? begin<__half>(g, g_matrix, g_row, batch, rows, cols, parts, eps, tall, hi, lo, o.ldx, st)
-                                : begin<__nv_bfloat16>(g, g_matrix, g_row, batch, rows, cols, parts, eps, tall, hi, lo, o.ldx, st);
+  int r = type == FS_TYPE_F32  ? begin<float>(g, g_matrix, g_row, batch, rows, cols, parts, eps, tall, hi, lo, o.ldx, meeting, st)
+          : type == FS_TYPE_F16 ? begin<__half>(g, g_matrix, g_row, batch, rows, cols, parts, eps, tall, hi, lo, o.ldx, meeting, st)
+                                : begin<__nv_bfloat16>(g, g_matrix, g_row, batch, rows, cols, parts, eps, tall, hi, lo, o.ldx, meeting, st);
   float grown = 1.f;  // what the steps from the last one on make of a rounding along small singular values
   int lower_until = steps;
   while (lower_until > 1 && grown * fabsf(a) <= kFewTimes) {
     grown *= fabsf(a);
     --lower_until;
+  }
+  if (r == FS_OK && chained(o)) {
+    const OrthoChain chain{steps, lower_until, {hi, other}, lo, sym, poly, meeting};
+    return launch_chain(o, chain, st);
   }
   for (int i = 0; i < steps && r == FS_OK; ++i) {
     o.hi = hi;
