@@ -750,11 +750,11 @@ mm8_short_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapW, cons
 // 16-bit products do. Each CTA puts the rows into 8 bits itself (a few microseconds less than a launch that does it once).
 constexpr int kFewRows8 = 2, kFewWarps8 = 8, kFewMost8 = 8192;  // rows; contraction values that shared memory takes
 
-// Shared memory of a row: its codes, padded to 128, and their scales.
-__host__ __device__ constexpr size_t few8_row_bytes(int blocks) { return ((size_t)blocks * (kBlock8 + 4) + 15) / 16 * 16; }
-__device__ __forceinline__ float2 two_of_codes(uint32_t pair) {
+// Shared memory of a row: what its codes stand for as fp16 (exact), padded to 128, and their scales.
+__host__ __device__ constexpr size_t few8_row_bytes(int blocks) { return ((size_t)blocks * (2 * kBlock8 + 4) + 15) / 16 * 16; }
+__device__ __forceinline__ uint32_t two_of_codes(uint32_t pair) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(pair & 0xffffu), __NV_E4M3);
-  return __half22float2(__half2(h));
+  return (uint32_t)h.x | (uint32_t)h.y << 16;
 }
 template <typename T, int ROWS>
 __global__ void __launch_bounds__(32 * kFewWarps8, 4)
@@ -762,6 +762,20 @@ few8_kernel(const Mm8Args a, const T* x0, long long ldx, int M, const int* rows,
   __shared__ int first_after[2];
   extern __shared__ __align__(16) uint8_t held[];
   const int lane = threadIdx.x & 31, i = blockIdx.y, blocks = (a.K + kBlock8 - 1) / kBlock8;
+  // The rows' first blocks are on their way while the expert is looked for, its weights while the rows are put into 8 bits.
+  constexpr int kEarly = 2;
+  const size_t row_bytes = few8_row_bytes(blocks);
+  float early[kEarly][8];
+  int from[ROWS];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) from[r] = i + r < a.R ? (rows ? __ldg(rows + i + r) : i + r) : -1;
+  auto fetch = [&](int u, float (&v)[8]) {
+    const int r = u / blocks, b = u - r * blocks, n = ROWS > 1 && r ? from[ROWS - 1] : from[0];
+    const bool in = u < ROWS * blocks && (unsigned)n < (unsigned)M;
+    eight(x0 + (in ? n : 0) * ldx, in ? b * kBlock8 + (threadIdx.x & 15) * 8 : a.K, a.K, vec, v);
+  };
+#pragma unroll
+  for (int k = 0; k < kEarly; ++k) fetch((threadIdx.x >> 4) + 2 * kFewWarps8 * k, early[k]);
   // The expert of row i is the one before the first offset above i (offsets as their running maximum); a row whose
   // predecessor has the same one is left to the CTA of the expert's first row.
   if (threadIdx.x < 2) first_after[threadIdx.x] = a.E + 1;
@@ -791,31 +805,13 @@ few8_kernel(const Mm8Args a, const T* x0, long long ldx, int M, const int* rows,
   }
   if (i > 0 && first_after[1] == first_after[0]) return;
   const int end = min(a.offsets[e + 1], a.R);
-  const size_t row_bytes = few8_row_bytes(blocks);
-  for (int u = threadIdx.x >> 4; u < ROWS * blocks; u += 2 * kFewWarps8) {
-    const int r = u / blocks, b = u - r * blocks, l = threadIdx.x & 15;
-    const int n = i + r < end ? (rows ? rows[i + r] : i + r) : -1;
-    float v[8] = {};
-    if ((unsigned)n < (unsigned)M) eight(x0 + n * ldx, b * kBlock8 + l * 8, a.K, vec, v);
-    uint32_t top = top_of(v);
-#pragma unroll
-    for (int o = 8; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffu << (threadIdx.x & 16), top, o));
-    float scale, inverse;
-    scale_of(top, scale, inverse);
-    *reinterpret_cast<uint2*>(held + r * row_bytes + b * kBlock8 + l * 8) = codes_of(v, inverse);
-    if (l == 0) *reinterpret_cast<float*>(held + r * row_bytes + blocks * kBlock8 + 4 * b) = scale;
-  }
-  __syncthreads();
-  if (f >= a.N) return;
-  const uint8_t* wf = w + e * w_expert + f * w_row;
-  const float* sw = a.sw + e * a.sw_expert + (long long)(f / kBlock8) * a.sw_n;
-  float sums[ROWS] = {};
+  const uint8_t* wf = w + e * w_expert + min(f, a.N - 1) * w_row;
+  const float* sw = a.sw + e * a.sw_expert + (long long)(min(f, a.N - 1) / kBlock8) * a.sw_n;
   constexpr int kDeep = 4;
   const int chunks = (a.K + 15) / 16;
-#pragma unroll 1
-  for (int c0 = lane; c0 < chunks; c0 += 32 * kDeep) {
-    uint4 q[kDeep];
-    float s[kDeep];
+  uint4 q[kDeep];
+  float s[kDeep];
+  auto ask = [&](int c0) {
 #pragma unroll
     for (int d = 0; d < kDeep; ++d) {
       const int c = c0 + 32 * d;
@@ -829,6 +825,36 @@ few8_kernel(const Mm8Args a, const T* x0, long long ldx, int M, const int* rows,
       }
       s[d] = __ldg(sw + (long long)(c >> 3) * a.sw_k);
     }
+  };
+  ask(lane);
+  const int units = min(ROWS, end - i) * blocks;  // of rows of this expert
+  auto hold = [&](int u, const float (&v)[8]) {
+    const int r = u / blocks, b = u - r * blocks, l = threadIdx.x & 15;
+    uint32_t top = top_of(v);
+#pragma unroll
+    for (int o = 8; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffu << (threadIdx.x & 16), top, o));
+    float scale, inverse;
+    scale_of(top, scale, inverse);
+    if (u >= units) return;
+    const uint2 c = codes_of(v, inverse);
+    *reinterpret_cast<uint4*>(held + r * row_bytes + 2 * (b * kBlock8 + l * 8)) =
+        make_uint4(two_of_codes(c.x), two_of_codes(c.x >> 16), two_of_codes(c.y), two_of_codes(c.y >> 16));
+    if (l == 0) *reinterpret_cast<float*>(held + r * row_bytes + 2 * blocks * kBlock8 + 4 * b) = scale;
+  };
+#pragma unroll
+  for (int k = 0; k < kEarly; ++k)
+    if ((threadIdx.x >> 4 & ~1) + 2 * kFewWarps8 * k < units) hold((threadIdx.x >> 4) + 2 * kFewWarps8 * k, early[k]);
+  for (int u = (threadIdx.x >> 4) + 2 * kFewWarps8 * kEarly; u < units; u += 2 * kFewWarps8) {
+    float v[8];
+    fetch(u, v);
+    hold(u, v);
+  }
+  __syncthreads();
+  if (f >= a.N) return;
+  float sums[ROWS] = {};
+#pragma unroll 1
+  for (int c0 = lane; c0 < chunks; c0 += 32 * kDeep) {
+    if (c0 != lane) ask(c0);
 #pragma unroll
     for (int d = 0; d < kDeep; ++d) {
       const int c = c0 + 32 * d;
@@ -836,17 +862,18 @@ few8_kernel(const Mm8Args a, const T* x0, long long ldx, int M, const int* rows,
       const uint32_t wq[4] = {q[d].x, q[d].y, q[d].z, q[d].w};
 #pragma unroll
       for (int r = 0; r < ROWS; ++r) {
-        const uint4 p = *reinterpret_cast<const uint4*>(held + r * row_bytes + 16 * c);
-        const uint32_t xq[4] = {p.x, p.y, p.z, p.w};
+        if (r > 0 && i + r >= end) continue;
+        const uint4 p0 = *reinterpret_cast<const uint4*>(held + r * row_bytes + 32 * c), p1 = *reinterpret_cast<const uint4*>(held + r * row_bytes + 32 * c + 16);
+        const uint32_t xh[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
         float t = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float2 wv = two_of_codes(wq[j] >> (16 * h)), xv = two_of_codes(xq[j] >> (16 * h));
-            t = fmaf(wv.y, xv.y, fmaf(wv.x, xv.x, t));
-          }
-        sums[r] = fmaf(t, s[d] * *reinterpret_cast<const float*>(held + r * row_bytes + blocks * kBlock8 + 4 * (c >> 3)), sums[r]);
+        for (int j = 0; j < 8; ++j) {
+          float w0, w1, x0, x1;
+          two_f32(two_of_codes(wq[j / 2] >> (16 * (j & 1))), w0, w1, __half());
+          two_f32(xh[j], x0, x1, __half());
+          t = fmaf(w1, x1, fmaf(w0, x0, t));
+        }
+        sums[r] = fmaf(t, s[d] * *reinterpret_cast<const float*>(held + r * row_bytes + 2 * blocks * kBlock8 + 4 * (c >> 3)), sums[r]);
       }
     }
   }
