@@ -154,6 +154,10 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
     if (t->defined() && t->requires_grad()) return true;
   return false;
 }
+// For calls whose results carry no gradient: a forward-mode tangent would be dropped without a word.
+void check_tangent(const char* name, const Tensor& t) {
+  REQUIRE(!t._fw_grad(0).defined(), name, " must not have a forward-mode tangent");
+}
 // Gradients of a backward pass that cannot be differentiated itself: an error where that is tried.
 variable_list once(variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -624,6 +628,7 @@ std::pair<Tensor, Tensor> to_blocks8(const Tensor& w) {
   REQUIRE(w.dim() == 3 && w.size(0) > 0 && w.size(1) > 0 && w.size(2) > 0, "weight must be 3D [E, N, K] and not empty, got shape ", shape_of(w));
   check_type("weight", w, false);
   check_cuda("weight", w);
+  check_tangent("weight", w);
   REQUIRE(w.size(0) <= kMaxExperts && w.size(1) <= (1 << 22) && w.size(2) <= (1 << 22), "weight must have at most ", kMaxExperts,
           " experts, N and K be at most 2^22");
   return weights8_raw(w);
@@ -644,7 +649,7 @@ Tensor grouped_mm8(const Tensor& x0, const optional<Tensor>& w0, const optional<
                 scales.size(2) == (k + 127) / 128,
             "scales must be a contiguous float32 tensor of shape (E, ceil(N / 128), ceil(K / 128)) for codes ", shape_of(w), ", got ", type_name(scales), " ",
             shape_of(scales));
-    REQUIRE(!scales.requires_grad(), "scales must not require grad");
+    REQUIRE(!scales.requires_grad() && !w.requires_grad(), "codes and scales must not require grad");
   }
   check_cuda("x", x0);
   check_place("weight", w, "x", x0);
@@ -681,6 +686,7 @@ Tensor orthogonalize(const Tensor& g0, int64_t steps, double a, double b, double
   check_type("g", g0, true);
   check_cuda("g", g0);
   const int64_t n = g0.size(-2), k = g0.size(-1), batch = g0.numel() / (n * k);
+  check_tangent("g", g0);
   REQUIRE(n <= 65536 && k <= 65536, "N and K must be at most 65536, got ", n, " and ", k);
   REQUIRE(batch < (1 << 20), "a stack must have fewer than 2^20 matrices");
   REQUIRE(steps >= 1 && steps <= 64, "steps must be between 1 and 64, got ", steps);

@@ -200,7 +200,7 @@ def orthogonalize(g: torch.Tensor, *, steps: int = 5, coefficients: Tuple[float,
     if dtype not in (torch.float16, torch.bfloat16):
         raise ValueError(f"dtype must be torch.float16 or torch.bfloat16, got {dtype}")
     a, b, c = (float(v) for v in coefficients)
-    return _lib.torch_binding().orthogonalize(g.detach(), int(steps), a, b, c, float(eps), dtype == torch.bfloat16)
+    return _lib.torch_binding().orthogonalize(g, int(steps), a, b, c, float(eps), dtype == torch.bfloat16)
 
 
 def transport_bias(x: torch.Tensor, router: torch.Tensor, *, eps: float = 0.1, n_iters: int = 20,
