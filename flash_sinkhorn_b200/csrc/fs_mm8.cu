@@ -393,10 +393,13 @@ mm8_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapA, const __gr
     uint32_t acc_ph = 0;
     bool lost = false;  // a wait of this CTA gave up: NaN from here on
     uint32_t stage = stages;
-    auto release = [&]() {  // the next staging tile, by the copy before last
+    auto release = [&](bool whole) {  // the next staging tile: by the copy before last, or by all if no copy follows from this one
       if (a.boxes) {
         stage = stages + (stage == stages ? 4096 : 0);
-        if (lane == 0) bulk_read<1>();
+        if (lane == 0) {
+          if (whole) bulk_read<1>();
+          else bulk_read<0>();
+        }
         __syncwarp();
       }
     };
@@ -478,7 +481,7 @@ mm8_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapA, const __gr
 #pragma unroll
         for (int j = 0; j < kMine; j += at16) {
           if (n0 + j >= a.N) break;
-          release();
+          release(whole);
 #pragma unroll
           for (int c = 0; c < at16 / 8; ++c)
             stage16(staged_row(stage, lane, c), two16(sum[j / 2 + 4 * c], a.out_type), two16(sum[j / 2 + 4 * c + 1], a.out_type),
@@ -495,7 +498,7 @@ mm8_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapA, const __gr
 #pragma unroll
         for (int j = 0; j < kMine; j += 32) {
           if (n0 + j >= a.N) break;
-          release();
+          release(whole);
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
             float v[4];

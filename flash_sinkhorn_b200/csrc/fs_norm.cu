@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(256) norm_sums_kernel(const float* sums, int c
 // Rows too long for registers: a CTA per row, which reads it three times (the second and third time from L2).
 template <typename T, typename W>
 __global__ void __launch_bounds__(kLongThreads) norm_long_kernel(const NormArgs a) {
-  __shared__ float slots[2][32];
+  __shared__ __align__(16) float slots[2][32];
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
     float s[1] = {0.f};
@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(kLongThreads) norm_long_kernel(const NormArgs 
 }
 template <typename T, typename W>
 __global__ void __launch_bounds__(kLongThreads) norm_long_grad_kernel(const NormArgs a) {
-  __shared__ float slots[2][32];
+  __shared__ __align__(16) float slots[2][32];
   int turn = 0;
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
     const T *x = static_cast<const T*>(a.x) + row * a.ldx, *dy = static_cast<const T*>(a.dy) + row * a.lddy;
