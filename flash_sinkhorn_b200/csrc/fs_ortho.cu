@@ -116,7 +116,9 @@ __global__ void __launch_bounds__(256) begin_kernel(const T* g, long long g_matr
 enum Product { GRAM, SQUARE, APPLY, LAST };  // LAST: APPLY to the result
 
 constexpr int kWriteWarps = 8, kGetWarp = 8, kMulWarp = 9, kThreadsO = 32 * 10;
-constexpr int kStageO = 8192 * kWriteWarps;  // two tiles of 32 rows of 128 bytes for each warp that writes
+// Shared memory for results: two tiles of 32 rows of 64 columns, or 32 of narrow tiles, for each warp that writes.
+__host__ __device__ constexpr int ortho_part(int bn) { return bn >= 128 ? 4096 : 2048; }
+__host__ __device__ constexpr int ortho_staging(int bn) { return 2 * ortho_part(bn) * kWriteWarps; }
 
 struct OrthoArgs {
   int batch, n, k;          // X is n x k, A and P are n x n
@@ -201,7 +203,7 @@ __device__ __forceinline__ OrthoPipe ortho_begin(uint8_t* raw, int nstage) {
   OrthoPipe p;
   p.ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   p.staging = p.ring + (size_t)nstage * kStage;
-  p.bars = reinterpret_cast<uint64_t*>(p.staging + kStageO);
+  p.bars = reinterpret_cast<uint64_t*>(p.staging + ortho_staging(BN));
   p.nstage = nstage;
   uint32_t* slot = reinterpret_cast<uint32_t*>(p.bars + p.drain() + 1);
   p.abort_flag = reinterpret_cast<volatile int*>(slot + 1);
@@ -323,9 +325,9 @@ __device__ __forceinline__ void ortho_product(const OrthoArgs& a, const CUtensor
     // Two warps to a quarter of the TMEM lanes (rows), with every other block of kCols columns each. What a block adds to its
     // product (A, or both parts of X) comes by whole rows of 16-byte loads, is under way in registers while the block before it is
     // worked on, and goes through shared memory to the lanes that have its rows; results go back the same way.
-    constexpr int kCols = BN >= 128 ? 64 : 32, kPer = kCols / 8, kFrom = FORM == GRAM ? 0 : FORM == SQUARE ? 1 : 2;
+    constexpr int kCols = BN >= 128 ? 64 : 32, kPart = ortho_part(BN), kPitch = 2 * kCols, kPer = kCols / 8, kFrom = FORM == GRAM ? 0 : FORM == SQUARE ? 1 : 2;
     const int q = warp & 3, side = warp >> 2;
-    const uint32_t stage = smem_u32(staging + 8192 * warp);
+    const uint32_t stage = smem_u32(staging + 2 * kPart * warp);
     const int width = FORM >= APPLY ? a.k : a.n;  // columns of the product
     const long long ld = FORM >= APPLY ? a.ldx : a.lda;
     uint4 ahead[kFrom ? kFrom : 1][kPer];
@@ -337,7 +339,12 @@ __device__ __forceinline__ void ortho_product(const OrthoArgs& a, const CUtensor
         const bool in = r < a.n && c < width;  // rows are padded to 16 bytes
 #pragma unroll
         for (int k = 0; k < kFrom; ++k)
-          ahead[k][i] = in && (k == 0 || a.lo) ? __ldcg(reinterpret_cast<const uint4*>((FORM == SQUARE ? a.a : k ? a.lo : a.hi) + at)) : make_uint4(0u, 0u, 0u, 0u);
+          if (in && (k == 0 || a.lo)) {  // in a chain of products, what other SMs have written in the same launch: past L1
+            const uint4* from = reinterpret_cast<const uint4*>((FORM == SQUARE ? a.a : k ? a.lo : a.hi) + at);
+            ahead[k][i] = CG == 2 ? *from : __ldcg(from);
+          } else {
+            ahead[k][i] = make_uint4(0u, 0u, 0u, 0u);
+          }
       }
     };
     int t = p.tiles, b = 0, m0 = 0, n0 = 0;
@@ -351,7 +358,8 @@ __device__ __forceinline__ void ortho_product(const OrthoArgs& a, const CUtensor
       int next_b = 0, next_m = 0, next_n = 0;
       if (it + stride < total) tiles.at(it + stride, next_b, next_m, next_n);
       if (!lost) {
-        lost = !__all_sync(0xffffffffu, wait_close(bar(ACC_FULL + buf), (t >> 1) & 1, abort_flag, a.limit ? a.limit + 4096ll * blocks : 0));
+        lost = !__all_sync(0xffffffffu, CG == 2 ? wait_blocks(bar(ACC_FULL + buf), (t >> 1) & 1, abort_flag, blocks, a.limit)
+                                                : wait_close(bar(ACC_FULL + buf), (t >> 1) & 1, abort_flag, a.limit ? a.limit + 4096ll * blocks : 0));
         tc_fence_after();
       }
 #pragma unroll 1
@@ -362,7 +370,7 @@ __device__ __forceinline__ void ortho_product(const OrthoArgs& a, const CUtensor
           for (int i = 0; i < kPer; ++i)
 #pragma unroll
             for (int k = 0; k < kFrom; ++k)
-              stage16(staged_row(stage + 4096 * k, i * (32 / kPer) + lane / kPer, lane % kPer), ahead[k][i].x, ahead[k][i].y, ahead[k][i].z, ahead[k][i].w);
+              stage16(staged_row<kPitch>(stage + kPart * k, i * (32 / kPer) + lane / kPer, lane % kPer), ahead[k][i].x, ahead[k][i].y, ahead[k][i].z, ahead[k][i].w);
           __syncwarp();
           if (c + 2 * kCols < BN) ask(b, row0, col + 2 * kCols);
           else if (it + stride < total) ask(next_b, next_m + rank * 128 + q * 32, next_n + kCols * side);
@@ -381,13 +389,13 @@ __device__ __forceinline__ void ortho_product(const OrthoArgs& a, const CUtensor
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const uint32_t at = staged_row(stage, lane, h / 8 + i);
+              const uint32_t at = staged_row<kPitch>(stage, lane, h / 8 + i);
               float* x = v + 8 * i;
               if (FORM == GRAM) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[j] *= kAScale / (kXScale * kXScale);
               } else {
-                const uint4 p = load_chunk(at), l = kFrom == 2 ? load_chunk(at + 4096) : make_uint4(0u, 0u, 0u, 0u);
+                const uint4 p = load_chunk(at), l = kFrom == 2 ? load_chunk(at + kPart) : make_uint4(0u, 0u, 0u, 0u);
                 const uint32_t pw[4] = {p.x, p.y, p.z, p.w}, lw[4] = {l.x, l.y, l.z, l.w};
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -412,7 +420,7 @@ __device__ __forceinline__ void ortho_product(const OrthoArgs& a, const CUtensor
                 }
               }
               if (FORM != LAST || !across) stage16(at, u[0], u[1], u[2], u[3]);
-              if (FORM == APPLY) stage16(at + 4096, lower[0], lower[1], lower[2], lower[3]);
+              if (FORM == APPLY) stage16(at + kPart, lower[0], lower[1], lower[2], lower[3]);
             }
           }
           if (FORM != APPLY && across) {
@@ -422,7 +430,7 @@ __device__ __forceinline__ void ortho_product(const OrthoArgs& a, const CUtensor
             for (int j = 0; j < kCols / 2; ++j) {
               const uint32_t other = __shfl_xor_sync(0xffffffffu, w[j], 1);
               const uint32_t two = lane & 1 ? __byte_perm(other, w[j], 0x7632) : __byte_perm(w[j], other, 0x5410);
-              asm volatile("st.shared.u32 [%0], %1;" ::"r"(stage + 4096 + (2 * j + (lane & 1)) * 64 + (lane >> 1) * 4), "r"(two) : "memory");
+              asm volatile("st.shared.u32 [%0], %1;" ::"r"(stage + kPart + (2 * j + (lane & 1)) * 64 + (lane >> 1) * 4), "r"(two) : "memory");
             }
             __syncwarp();
             const long long pitch = FORM == LAST ? a.n : ld;
@@ -432,14 +440,14 @@ __device__ __forceinline__ void ortho_product(const OrthoArgs& a, const CUtensor
 #pragma unroll
               for (int i = 0; i < kCols / 8; ++i) {
                 const int r = 8 * i + (lane >> 2), ch = lane & 3;
-                const uint4 x = load_chunk(stage + 4096 + r * 64 + ch * 16);
+                const uint4 x = load_chunk(stage + kPart + r * 64 + ch * 16);
                 if (col + r < width && row0 + 8 * ch < a.n) *reinterpret_cast<uint4*>(out + r * pitch + 8 * ch) = x;
               }
             } else {
 #pragma unroll 4
               for (int r = 0; r < kCols; ++r) {
                 uint16_t x;
-                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(stage + 4096 + r * 64 + lane * 2) : "memory");
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(stage + kPart + r * 64 + lane * 2) : "memory");
                 if (col + r < width && row < a.n) out[r * pitch + lane] = x;
               }
             }
@@ -449,11 +457,11 @@ __device__ __forceinline__ void ortho_product(const OrthoArgs& a, const CUtensor
           const long long at = ((long long)b * a.n + row0) * ld + col;
           if (FORM == LAST) {
             if (!across)
-              write_rows(reinterpret_cast<char*>(static_cast<uint16_t*>(a.out) + ((long long)b * a.n + row0) * a.k + col), 2ll * a.k, rows, bytes, a.out_bytes,
+              write_rows<kPitch>(reinterpret_cast<char*>(static_cast<uint16_t*>(a.out) + ((long long)b * a.n + row0) * a.k + col), 2ll * a.k, rows, bytes, a.out_bytes,
                          stage, lane);
           } else {
-            write_rows(reinterpret_cast<char*>((FORM == APPLY ? a.hi_out : a.sym) + at), 2 * ld, rows, bytes, 16, stage, lane);
-            if (FORM == APPLY && a.lo_out) write_rows(reinterpret_cast<char*>(a.lo_out + at), 2 * ld, rows, bytes, 16, stage + 4096, lane);
+            write_rows<kPitch>(reinterpret_cast<char*>((FORM == APPLY ? a.hi_out : a.sym) + at), 2 * ld, rows, bytes, 16, stage, lane);
+            if (FORM == APPLY && a.lo_out) write_rows<kPitch>(reinterpret_cast<char*>(a.lo_out + at), 2 * ld, rows, bytes, 16, stage + kPart, lane);
           }
         }
         __syncwarp();
@@ -602,7 +610,7 @@ int launch_ortho(OrthoArgs a, cudaStream_t st) {
                        : encode_stack(&mapA, left, a.n, a.n, a.batch, a.lda, 128) && encode_stack(&mapB, a.hi, a.k, a.n, a.batch, a.ldx, 64);
   if (!good) return report_error(FS_ERR_CUDA, "cuTensorMapEncodeTiled failed");
   constexpr size_t kStage = 128 * 128 + BN / CG * 128;
-  constexpr size_t fixed = 1024 + kStageO + 8 * (2 * 12 + 5) + 8;
+  constexpr size_t fixed = 1024 + ortho_staging(BN) + 8 * (2 * 12 + 5) + 8;
   a.nstage = (int)((kSmemMax - fixed) / kStage);
   if (a.nstage > 12) a.nstage = 12;
   size_t smem = fixed + a.nstage * kStage;
@@ -651,9 +659,9 @@ int launch_chain(OrthoArgs a, const OrthoChain& c, cudaStream_t st) {
   if (!encode_stack(&maps.a128, c.sym, a.n, a.n, a.batch, a.lda, 128) || !encode_stack(&maps.a64, c.sym, a.n, a.n, a.batch, a.lda, 64) ||
       !encode_stack(&maps.p128, c.poly, a.n, a.n, a.batch, a.lda, 128))
     return report_error(FS_ERR_CUDA, "cuTensorMapEncodeTiled failed");
-  constexpr size_t kStage = 128 * 128 + kChainBN * 128, fixed = 1024 + kStageO + 8 * (2 * 12 + 5) + 8;
+  constexpr size_t kStage = 128 * 128 + kChainBN * 128, fixed = 1024 + ortho_staging(kChainBN) + 8 * (2 * 12 + 5) + 8;
   a.nstage = (int)((kSmemMax - fixed) / kStage);
-  static_assert(fixed + 6 * kStage >= (size_t)kSmemMin && (kSmemMax - fixed) / kStage <= 12 && (kSmemMax - fixed) / kStage >= 6, "shared memory");
+  static_assert(fixed + 8 * kStage >= (size_t)kSmemMin && (kSmemMax - fixed) / kStage == 8, "shared memory");
   static std::atomic<uint64_t> allowed{0};  // devices on which the kernel may take all shared memory
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);

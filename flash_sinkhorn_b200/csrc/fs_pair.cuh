@@ -198,31 +198,39 @@ __device__ void read_groups(const int* offsets, int E, int R, int* gs, int* ts, 
   if (TILES && lane == 0) ts[0] = 0;
 }
 
-// 16-byte chunk `chunk` of row `row` of a warp's staging tile of 32 rows of 128 bytes: neither side meets bank conflicts.
-__device__ __forceinline__ uint32_t staged_row(uint32_t base, int row, int chunk) { return base + row * 128 + ((chunk ^ (row & 7)) << 4); }
-// rows x bytes (at most 32 x 128) of the staging tile to out, rows ld bytes apart, by stores of `vec` bytes.
+// 16-byte chunk `chunk` of row `row` of a warp's staging tile of 32 rows of PITCH bytes (128 or 64): neither side meets bank conflicts.
+template <int PITCH = 128>
+__device__ __forceinline__ uint32_t staged_row(uint32_t base, int row, int chunk) {
+  return base + row * PITCH + ((chunk ^ (PITCH == 128 ? row & 7 : (row >> 1) & 3)) << 4);
+}
+// rows x bytes (at most 32 x PITCH) of the staging tile to out, rows ld bytes apart, by stores of `vec` bytes.
+template <int PITCH = 128>
 __device__ __forceinline__ void write_rows(char* out, long long ld, int rows, int bytes, int vec, uint32_t base, int lane) {
   if (vec == 16) {
+    constexpr int kLanes = PITCH / 16;  // to a row
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = 4 * i + (lane >> 3), c = lane & 7;
+    for (int i = 0; i < kLanes; ++i) {
+      const int r = 32 / kLanes * i + lane / kLanes, c = lane % kLanes;
       uint4 v;
-      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(staged_row(base, r, c)));
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(staged_row<PITCH>(base, r, c)));
       if (r < rows && 16 * c < bytes) *reinterpret_cast<uint4*>(out + r * ld + 16 * c) = v;
     }
   } else if (vec == 4) {
+    constexpr int kLanes = PITCH / 4;
 #pragma unroll 4
-    for (int r = 0; r < 32; ++r) {
+    for (int i = 0; i < kLanes; ++i) {
+      const int r = 32 / kLanes * i + lane / kLanes, c = 4 * (lane % kLanes);
       uint32_t v;
-      asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(staged_row(base, r, lane >> 2) + (lane & 3) * 4));
-      if (r < rows && 4 * lane < bytes) *reinterpret_cast<uint32_t*>(out + r * ld + 4 * lane) = v;
+      asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(staged_row<PITCH>(base, r, c >> 4) + (c & 15)));
+      if (r < rows && c < bytes) *reinterpret_cast<uint32_t*>(out + r * ld + c) = v;
     }
   } else {
+    constexpr int kParts = PITCH / 64;
 #pragma unroll 4
-    for (int i = 0; i < 64; ++i) {
-      const int r = i >> 1, c = 2 * lane + 64 * (i & 1);
+    for (int i = 0; i < 32 * kParts; ++i) {
+      const int r = i / kParts, c = 2 * lane + 64 * (i % kParts);
       uint16_t v;
-      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(staged_row(base, r, c >> 4) + (c & 15)));
+      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(staged_row<PITCH>(base, r, c >> 4) + (c & 15)));
       if (r < rows && c < bytes) *reinterpret_cast<uint16_t*>(out + r * ld + c) = v;
     }
   }
