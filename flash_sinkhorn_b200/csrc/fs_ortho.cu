@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(256) begin_kernel(const T* g, long long g_matr
 // ------------------------------------------------------------------ products
 enum Product { GRAM, SQUARE, APPLY, LAST };  // LAST: APPLY to the result
 
-constexpr int kWriteWarps = 8, kGetWarp = 8, kMulWarp = 9, kThreadsO = 32 * 10;
+constexpr int kWriteWarps = 8, kGetWarp = 8, kMulWarp = 9, kGetWarpB = 10, kThreadsO = 32 * 11;
 // Shared memory for results: two tiles of 32 rows of 64 columns, or 32 of narrow tiles, for each warp that writes.
 __host__ __device__ constexpr int ortho_part(int bn) { return bn >= 128 ? 4096 : 2048; }
 __host__ __device__ constexpr int ortho_staging(int bn) { return 2 * ortho_part(bn) * kWriteWarps; }
@@ -187,7 +187,6 @@ struct OrthoPipe {
   int s;        // next stage
   uint32_t ph;  // its phase
   int tiles;    // that this CTA has done
-  int issued;   // stages that this CTA's loading thread has started
   __device__ uint32_t bar(int i) const { return smem_u32(bars + i); }
   __device__ int full() const { return 0; }
   __device__ int empty() const { return nstage; }
@@ -210,11 +209,11 @@ __device__ __forceinline__ OrthoPipe ortho_begin(uint8_t* raw, int nstage) {
   p.warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);
   p.lane = threadIdx.x & 31;
   p.rank = CG == 2 ? (int)cta_rank() : 0;
-  p.s = p.tiles = p.issued = 0;
+  p.s = p.tiles = 0;
   p.ph = 0;
   if (p.warp == kGetWarp && p.lane == 0) {
     for (int s = 0; s < nstage; ++s) {
-      mbar_init(p.bar(p.full() + s), CG);  // in CTA 0: both CTAs' loads
+      mbar_init(p.bar(p.full() + s), 2 * CG);  // in CTA 0: both CTAs' loads of either operand
       mbar_init(p.bar(p.empty() + s), 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -252,8 +251,10 @@ __device__ __forceinline__ void ortho_product(const OrthoArgs& a, const CUtensor
   const TilesO<FORM, CG, BN> tiles(a);
   const long long total = tiles.total();
 
-  if (warp == kGetWarp) {
+  if (warp == kGetWarp || warp == kGetWarpB) {
     // ===================== loads =====================
+    // A warp for each operand: one thread takes 150 to 200 clocks for a tensor load, and a stage of P X has three of them for products of 512
+    // (32 matrices of 2048 x 1024: 1405 -> 1346 us).
     if (elect_one()) {
       int s = p.s;
       uint32_t ph = p.ph;
@@ -267,15 +268,18 @@ __device__ __forceinline__ void ortho_product(const OrthoArgs& a, const CUtensor
             break;
           }
           const uint32_t full = CG == 2 ? in_leader(bar(FULL + s)) : bar(FULL + s), dst = smem_u32(ring + (size_t)s * kStage);
-          expect_at<CG>(full, kStage);
-          load_3d<CG>(dst, mapA, kb * 64, m0 + rank * 128, b, full);
-          if (B_MN) {
-#pragma unroll
-            for (int c = 0; c < BNC / 64; ++c) load_3d<CG>(dst + kA + c * kHalf, mapB, n0 + rank * BNC + c * 64, kb * 64, b, full);
+          if (warp == kGetWarp) {
+            expect_at<CG>(full, kA);
+            load_3d<CG>(dst, mapA, kb * 64, m0 + rank * 128, b, full);
           } else {
-            load_3d<CG>(dst + kA, mapB, kb * 64, n0 + rank * BNC, b, full);
+            expect_at<CG>(full, kB);
+            if (B_MN) {
+#pragma unroll
+              for (int c = 0; c < BNC / 64; ++c) load_3d<CG>(dst + kA + c * kHalf, mapB, n0 + rank * BNC + c * 64, kb * 64, b, full);
+            } else {
+              load_3d<CG>(dst + kA, mapB, kb * 64, n0 + rank * BNC, b, full);
+            }
           }
-          ++p.issued;
           if (++s == p.nstage) {
             s = 0;
             ph ^= 1;
@@ -500,15 +504,10 @@ __device__ __forceinline__ void ortho_end(const OrthoPipe& p) {
       }
       __syncwarp();
     } else if (p.warp == kGetWarp) {
-      // The copies in flight land before the CTA ends; those of the second CTA of a pair, which the first one counts, are
-      // given a millisecond, hundreds of times what a copy takes.
+      // The copies in flight land before the CTA ends: they are given a millisecond, hundreds of times what a copy takes.
       if (elect_one()) {
         const long long t0 = clock64();
-        if (p.rank == 0)
-          for (int j = p.issued > p.nstage ? p.issued - p.nstage : 0; j < p.issued; ++j)
-            wait_landed(p.bar(p.full() + j % p.nstage), (j / p.nstage) & 1, t0);
-        else
-          while (clock64() - t0 < (1ll << 21)) {}
+        while (clock64() - t0 < (1ll << 21)) {}
       }
       __syncwarp();
     }
@@ -556,7 +555,7 @@ __device__ __forceinline__ void ortho_meet(const OrthoPipe& p, unsigned* meeting
     } while (seen < target && !*p.abort_flag);
   }
   __syncthreads();
-  if (p.warp == kGetWarp) asm volatile("fence.proxy.async.global;" ::: "memory");
+  if (p.warp == kGetWarp || p.warp == kGetWarpB) asm volatile("fence.proxy.async.global;" ::: "memory");
 }
 
 __global__ void __launch_bounds__(kThreadsO, 1) ortho_chain_kernel(OrthoArgs a, const OrthoChain c, const __grid_constant__ OrthoMaps maps) {
