@@ -152,39 +152,51 @@ __global__ void __launch_bounds__(V * NV <= (V > 1 ? 16 : 8) ? 256 : kMaxNormThr
     for (int i = threadIdx.x; i < 512; i += blockDim.x) (&slots[0][0][0])[i] = 0.f;
     __syncthreads();
   }
+  bool in[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) in[i] = (i * group + t) * V < a.F;
   const float per = 1.f / a.F;
   const long long stride = (long long)gridDim.x * groups;
-  long long row = (long long)blockIdx.x * groups + g, ahead = row;
+  long long row = (long long)blockIdx.x * groups + g;
+  long long left = row < a.rows ? (a.rows - row + stride - 1) / stride : 0, coming = left;  // rows of this group, and those not yet asked for
+  const T* x = static_cast<const T*>(a.x) + row * a.ldx + t * V;
+  T* out = static_cast<T*>(a.out) + row * a.F + t * V;
+  const long long x_step = stride * a.ldx, out_step = stride * a.F;
   auto ask = [&](int s) {
-    if (ahead < a.rows) {
-      const T* x = static_cast<const T*>(a.x) + ahead * a.ldx + t * V;
+    if (coming > 0) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if ((i * group + t) * V < a.F) fetch<T, V>(ring + (s * NV + i) * blockDim.x, x + i * group * V);
+        if (in[i]) fetch<T, V>(ring + (s * NV + i) * blockDim.x, x + i * group * V);
+      x += x_step;
+      --coming;
     }
-    ahead += stride;
     fetch_commit();
   };
   if (kHold)
     for (int s = 0; s < S - 1; ++s) ask(s);
-  for (int stage = 0; row < a.rows; row += stride, stage = stage + 1 == S ? 0 : stage + 1) {
+  for (int stage = 0; left > 0; --left, row += stride, out += out_step, stage = stage + 1 == S ? 0 : stage + 1) {
     Pack<T, V> q[NV];
     if (kHold) {
       ask(stage ? stage - 1 : S - 1);
       fetch_wait<S - 1>();
-    }
-    const T* x = static_cast<const T*>(a.x) + row * a.ldx + t * V;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if ((i * group + t) * V < a.F) q[i] = kHold ? ring[(stage * NV + i) * blockDim.x] : read_only<T, V>(x + i * group * V);
-    u64 sum = 0ull;
+      for (int i = 0; i < NV; ++i)
+        if (in[i]) q[i] = ring[(stage * NV + i) * blockDim.x];
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (in[i]) q[i] = read_only<T, V>(x + i * group * V);
+      x += x_step;
+    }
+    // unpacked once where registers hold that, else in each of the three passes
+    u64 v[kHold ? NV : 1][P], sum = 0ull;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      u64 p[P];
-      pairs<T, V>(q[i], p);
-      if ((i * group + t) * V < a.F)
+      const int k = kHold ? i : 0;
+      pairs<T, V>(q[i], v[k]);
+      if (in[i])
 #pragma unroll
-        for (int j = 0; j < P; ++j) sum = add2(sum, p[j]);
+        for (int j = 0; j < P; ++j) sum = add2(sum, v[k][j]);
     }
     float s[1] = {both(sum)};
     group_sum(s, slots[0][g], warps, 1 + g);
@@ -193,39 +205,37 @@ __global__ void __launch_bounds__(V * NV <= (V > 1 ? 16 : 8) ? 256 : kMaxNormThr
     sum = 0ull;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      u64 p[P];
-      pairs<T, V>(q[i], p);
-      if ((i * group + t) * V < a.F)
+      const int k = kHold ? i : 0;
+      if (!kHold) pairs<T, V>(q[i], v[0]);
+      if (in[i])
 #pragma unroll
         for (int j = 0; j < P; ++j) {
-          const u64 d = add2(p[j], less);
-          sum = fma2(d, d, sum);
+          v[k][j] = add2(v[k][j], less);
+          sum = fma2(v[k][j], v[k][j], sum);
         }
     }
     s[0] = both(sum);
     group_sum(s, slots[1][g], warps, 1 + g);
-    const float r = 1.f / sqrtf(fmaf(s[0], per, a.eps));
+    const float r = __frsqrt_rn(fmaf(s[0], per, a.eps));
     if (a.mean && t == 0) {
       a.mean[row] = mean;
       a.rstd[row] = r;
     }
     const u64 r2 = pk(r, r);
-    T* out = static_cast<T*>(a.out) + row * a.F;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * group + t) * V;
-      if (c >= a.F) continue;
-      constexpr int kOne = kHold ? 1 : 0;
-      const int k = i * kOne;
-      u64 p[P];
-      pairs<T, V>(q[i], p);
+      const int k = kHold ? i : 0;
+      if (!in[i]) continue;
       if (!kHold) {
-        columns<W, V>(a.w, c, 1.f, w[0]);
-        columns<W, V>(a.b, c, 0.f, b[0]);
+        pairs<T, V>(q[i], v[0]);
+#pragma unroll
+        for (int j = 0; j < P; ++j) v[0][j] = add2(v[0][j], less);
+        columns<W, V>(a.w, (i * group + t) * V, 1.f, w[0]);
+        columns<W, V>(a.b, (i * group + t) * V, 0.f, b[0]);
       }
 #pragma unroll
-      for (int j = 0; j < P; ++j) p[j] = fma2(mul2(add2(p[j], less), r2), w[k][j], b[k][j]);
-      store_pairs<T, V>(out + c, p);
+      for (int j = 0; j < P; ++j) v[k][j] = fma2(mul2(v[k][j], r2), w[k][j], b[k][j]);
+      store_pairs<T, V>(out + i * group * V, v[k]);
     }
   }
 }
@@ -256,35 +266,45 @@ __global__ void __launch_bounds__(256, SUMS ? 2 : 1) norm_grad_kernel(const Norm
     for (int i = threadIdx.x; i < 512; i += blockDim.x) (&slots[0][0][0])[i] = 0.f;
     __syncthreads();
   }
+  bool in[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) in[i] = (i * a.group + t) * V < a.F;
   const float per = 1.f / a.F;
-  const long long stride = (long long)gridDim.x * groups;
-  long long row = (long long)blockIdx.x * groups + g, ahead = row;
+  const long long stride = (long long)gridDim.x * groups, row = (long long)blockIdx.x * groups + g;
+  long long left = row < a.rows ? (a.rows - row + stride - 1) / stride : 0, coming = left;  // rows of this group, and those not yet asked for
+  const T *x = static_cast<const T*>(a.x) + row * a.ldx + t * V, *dy = static_cast<const T*>(a.dy) + row * a.lddy + t * V;
+  T* out = a.out ? static_cast<T*>(a.out) + row * a.F + t * V : nullptr;
+  const float *mean = a.mean + row, *rstd = a.rstd + row;
+  const long long x_step = stride * a.ldx, dy_step = stride * a.lddy, out_step = stride * a.F;
   auto ask = [&](int s) {
-    if (ahead < a.rows) {
-      const T *x = static_cast<const T*>(a.x) + ahead * a.ldx + t * V, *dy = static_cast<const T*>(a.dy) + ahead * a.lddy + t * V;
+    if (coming > 0) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if ((i * a.group + t) * V < a.F) {
+        if (in[i]) {
           fetch<T, V>(ring + (s * 2 * NV + i) * blockDim.x, x + i * a.group * V);
           fetch<T, V>(ring + ((s * 2 + 1) * NV + i) * blockDim.x, dy + i * a.group * V);
         }
+      x += x_step;
+      dy += dy_step;
+      --coming;
     }
-    ahead += stride;
     fetch_commit();
   };
   for (int s = 0; s < S - 1; ++s) ask(s);
   float next_mean = 0.f, next_r = 0.f;
-  if (row < a.rows) {
-    next_mean = __ldg(a.mean + row);
-    next_r = __ldg(a.rstd + row);
+  if (left > 0) {
+    next_mean = __ldg(mean);
+    next_r = __ldg(rstd);
   }
-  for (int s = 0, turn = 0; row < a.rows; row += stride, s = s + 1 == S ? 0 : s + 1, turn ^= 1) {
+  for (int s = 0, turn = 0; left > 0; --left, s = s + 1 == S ? 0 : s + 1, turn ^= 1) {
     ask(s ? s - 1 : S - 1);
     const float r = next_r;
     const u64 r2 = pk(r, r), shift = pk(-next_mean * r, V == 1 ? 0.f : -next_mean * r);  // n = x r + shift
-    if (row + stride < a.rows) {
-      next_mean = __ldg(a.mean + row + stride);
-      next_r = __ldg(a.rstd + row + stride);
+    if (left > 1) {
+      mean += stride;
+      rstd += stride;
+      next_mean = __ldg(mean);
+      next_r = __ldg(rstd);
     }
     fetch_wait<S - 1>();
     const Pack<T, V>*px = ring + s * 2 * NV * blockDim.x, *pg = px + NV * blockDim.x;
@@ -300,7 +320,7 @@ __global__ void __launch_bounds__(256, SUMS ? 2 : 1) norm_grad_kernel(const Norm
     for (int i = 0; i < NV; ++i) {
       constexpr int kOne = SUMS ? 1 : 0;
       const int k = i * kOne;
-      if ((i * a.group + t) * V >= a.F) continue;
+      if (!in[i]) continue;
       read(i, k);
 #pragma unroll
       for (int j = 0; j < P; ++j) {
@@ -313,21 +333,21 @@ __global__ void __launch_bounds__(256, SUMS ? 2 : 1) norm_grad_kernel(const Norm
         sn = fma2(v, n[k][j], sn);
       }
     }
-    if (!a.out) continue;
+    if (!out) continue;
     float sum[2] = {both(su), both(sn)};
     group_sum(sum, slots[turn][g], warps, 1 + g);
     const u64 m1 = pk(-sum[0] * per, -sum[0] * per), m2 = pk(-sum[1] * per, -sum[1] * per);
-    T* out = static_cast<T*>(a.out) + row * a.F;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       constexpr int kOne = SUMS ? 1 : 0;
-      const int c = (i * a.group + t) * V, k = i * kOne;
-      if (c >= a.F) continue;
+      const int k = i * kOne;
+      if (!in[i]) continue;
       if (!SUMS) read(i, 0);
 #pragma unroll
       for (int j = 0; j < P; ++j) n[k][j] = mul2(r2, fma2(m2, n[k][j], fma2(u[k][j], w[k][j], m1)));
-      store_pairs<T, V>(out + c, n[k]);
+      store_pairs<T, V>(out + i * a.group * V, n[k]);
     }
+    out += out_step;
   }
   if (!SUMS) return;
   fetch_wait<0>();
@@ -402,7 +422,7 @@ __global__ void __launch_bounds__(kLongThreads) norm_long_kernel(const NormArgs 
       s[0] = fmaf(d, d, s[0]);
     }
     group_sum(s, slots[1], kLongThreads / 32, 1);
-    const float r = 1.f / sqrtf(s[0] / a.F + a.eps);
+    const float r = __frsqrt_rn(s[0] / a.F + a.eps);
     if (a.mean && threadIdx.x == 0) {
       a.mean[row] = mean;
       a.rstd[row] = r;
