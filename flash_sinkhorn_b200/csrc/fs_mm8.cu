@@ -8,9 +8,14 @@
 // the half of its range that a power of two may leave (a value is off by half a step of its own either way).
 //
 // Rows go into 8 bits and into the order of the experts in one pass. In the product the ROWS of a group are the M side of the
-// tensor-core instruction, so that a thread's 32 or more accumulators share the row's scale. The tensor core sums one block of 128 in
+// tensor-core instruction, so that a thread's accumulators share the row's scale. The tensor core sums one block of 128 in
 // TMEM (fp32); eight warps read that while the next block is summed beside it, and add it, scaled, to sums in registers.
-// Per block and 128 x 256 tile the products take 512 clocks of the tensor core, reading 256 of TMEM and adding 256 of the fp32 units.
+// Per block and 128 x 256 tile the products take 512 clocks of the tensor core, reading 256 of TMEM and adding 256 of the fp32 units, but
+// each of the two accumulators goes from the tensor core to the warps of both CTAs and back, which takes some 1200 clocks by itself: a
+// block takes 590 ns where loads and products alone take 373 (from HBM 550). 65536 rows of 64 experts, 2048 x 2048: 319 us, 1720 TFLOP/s, against
+// 390 us of the 16-bit product; with 1024 or 4096 contraction values 1450 and 1860 TFLOP/s (a tile costs 2 us besides its blocks).
+// What decided it: registers that spill in the loop of sums (a factor 1.5), loads of 16 columns a step ahead of the additions, results by TMA.
+// Barriers of their own for the two halves of a tile cost more than they saved (870 ns a block), so did factors read four blocks ahead.
 #include "fs_experts.cuh"
 #include "fs_pair.cuh"
 #include "fs_tc.cuh"
@@ -113,7 +118,8 @@ __device__ __forceinline__ uint4 sixteen_codes(const uint32_t (&w)[8], float inv
 
 // Rows x[rows[i]] of M rows of K values (zeros for numbers outside; rows null: row i) to codes [R, ldc] and scales [ceil(K / 128)][R]. Eight lanes
 // take a row, sixteen values of a block each, a CTA 32 rows of `span` blocks, so that 32 rows' scales are written side by side. ldc is a
-// multiple of 16; codes past K are zeros. Instructions count as much as bytes: magnitudes are compared in pairs, as whole numbers.
+// multiple of 16; codes past K are zeros. Instructions count as much as bytes: magnitudes are compared in pairs, as whole
+// numbers (65536 gathered rows of 2048: 104 us with 8 values a lane, compared one by one, 47 us so).
 constexpr int kRows8 = 32, kSpan8 = 64;
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) rows8_kernel(const T* x, long long ldx, int M, const int* rows, int R, int K, int span, uint8_t* codes, long long ldc,
@@ -151,7 +157,7 @@ __global__ void __launch_bounds__(256) rows8_kernel(const T* x, long long ldx, i
 }
 
 // Weights w [E, N, K] to codes (rows c_row, matrices c_expert apart) and scales [E][ceil(N / 128)][ceil(K / 128)]: a CTA to a block of
-// 128 x 128, which it holds in registers between the search for the largest magnitude and the codes.
+// 128 x 128, which it holds in registers between the search for the largest magnitude and the codes. Bound by memory: 64 Mi values 30 us, 6.7 TB/s.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) weights8_kernel(const T* w, long long w_expert, long long w_row, int N, int K, uint8_t* codes, long long c_expert,
                                                        long long c_row, float* scales) {
@@ -550,7 +556,8 @@ mm8_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapA, const __gr
 // ------------------------------------------------------------------ short groups
 // Groups of up to a few dozen rows are bound by reading their weights. Here the FEATURES are the M side and the rows N, as in the
 // 16-bit products: a stage is 16 KB of weights and 4 KB of rows, an accumulator kShortRows columns, of which 256 / kShortRows are in use in turn, so that the
-// tensor core does not wait for the sums. Two CTAs to an SM: one's first loads of a tile hide behind the other one's products.
+// tensor core does not wait for the sums. Two CTAs to an SM: one's first loads of a tile hide behind the other one's products. 64 experts of 2048 x 1024
+// with two rows each: 29 us, 4.6 TB/s, some 8 of them launch, first loads and the last, partly filled round; twice the features 50 us, 5.3 TB/s.
 constexpr int kShortRows = 32;                                       // of a tile: a lane's factor is that of one
 constexpr int kShortThreads = 192, kShortFetch = 4, kShortIssue = 5;  // four warps that sum
 constexpr size_t kShortSmem = 112 * 1024;                            // two fit an SM, and no kernel of this library beside one: they take 120 KB
@@ -749,8 +756,8 @@ mm8_short_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapW, cons
 }
 
 // ------------------------------------------------------------------ few rows
-// A single token: bound by reading its experts' weights, so a warp takes one feature of one expert, 16 codes a lane and load, as the
-// 16-bit products do. Each CTA puts the rows into 8 bits itself (a few microseconds less than a launch that does it once).
+// A single token: bound by launch and latency beside its experts' weights, so a warp takes one feature of one expert, 16 codes a lane and load, as the
+// 16-bit products do. Each CTA puts the rows into 8 bits itself, which takes less than a launch that does it once. Two rows of two experts, 2048 x 2048: 6.7 us.
 constexpr int kFewRows8 = 2, kFewWarps8 = 8, kFewMost8 = 8192;  // rows; contraction values that shared memory takes
 
 // Shared memory of a row: what its codes stand for as fp16 (exact), padded to 128, and their scales.
@@ -980,7 +987,8 @@ int launch_short8(Mm8Args a, const uint8_t* x, long long ldx, const uint8_t* w, 
   if (e != cudaSuccess) return report_error(FS_ERR_CUDA, cudaGetErrorString(e));
   const long long most = ((a.R + kShortRows - 1ll) / kShortRows + a.E + 1) * ((a.N + 127) / 128);
   if (most > 0x3fffffffll) return report_error(FS_ERR_UNSUPPORTED, "more than 2^30 tiles");
-  long long grid = 2 * detail::free_ctas();
+  // two to an SM; one, where SMs are to stay free: the second ones would go to those
+  long long grid = detail::free_ctas() * (detail::free_ctas() == detail::sm_count() ? 2ll : 1ll);
   if (grid > most) grid = most;
   if (grid < 1) grid = 1;
   g_mm8_launched.store(true, std::memory_order_relaxed);
@@ -1109,6 +1117,10 @@ int fs_grouped_mm8(const void* x, int type, long long ldx, int M, const int* row
   s = type == FS_TYPE_F16 ? launch_rows8<__half>(x, ldx, M, rows, R, K, codes, ldc, sx, st)
                           : launch_rows8<__nv_bfloat16>(x, ldx, M, rows, R, K, codes, ldc, sx, st);
   if (s != FS_OK) return s;
+  // Up to 40 rows in a mean group its weights' bytes decide, and tiles of 32 rows with the features as M read them fastest; pairs of CTAs pay where
+  // there are tiles of 256 x 256 for all of them, half of every group's last one empty, and a mean group fills one. us with short tiles, 128 x 128 and
+  // 256 x 256: 64 experts 2048 -> 1024, 2 rows each 29, 34, -; 32 experts of 48 rows 24, 22, 31; 64 of 64 rows 44, 40, -; of 128 rows -, 44, 55; 32 of 160 rows,
+  // 1024 -> 2048 -, 35, 34; 32 of 200 rows, 2048 x 2048 -, 64, 54; one of 1024 rows, 1024 x 1024 -, 8.1, 11.6.
   const long long tiles = ((R + 255ll) / 256 + (E < R ? E : R) / 2) * ((N + 255) / 256);
   const bool pairs = tiles * 2 > detail::free_ctas() && N > 128;
   if (transposed) {

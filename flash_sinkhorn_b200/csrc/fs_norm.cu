@@ -3,11 +3,16 @@
 //   m = sum x / F,  v = sum (x - m)^2 / F,  r = 1 / sqrt(v + eps),  n = (x - m) r,  y = n w + b
 //   dx = r (u - mean(u) - n mean(u n)),  u = w dy;   dw = sum over rows of dy n,  db = sum over rows of dy
 //
-// Both passes are bound by memory: x is read and y written, then x and dy read and dx written. A row lies in the registers of
-// a group of warps (the mean first, then the squares of the differences from it: one read, and no cancellation), groups walk
-// over the rows with several rows' loads under way, and in the backward pass each thread adds what its columns contribute
-// to dw and db over all its rows. A CTA leaves one row of sums, which a second launch adds in a fixed order, so every run gives
-// the same bits. Sums are fp32; y, dx, dw and db are rounded once.
+// A row lies in the registers of a group of warps (the mean first, then the squares of the differences from it: one read, and no
+// cancellation), groups walk over the rows with several rows' loads under way (cp.async, each thread what it reads itself), and in the
+// backward pass each thread adds what its columns contribute to dw and db over all its rows. A CTA leaves one row of sums, which a
+// second launch adds in a fixed order, so every run gives the same bits. Rows whose columns are too many for that go without, and a third kernel
+// reads them again. Sums are fp32; y, dx, dw and db are rounded once.
+//
+// Memory is the floor and latency of a row's two or three sums across warps what is seen: 16384 rows of 2048 in bf16 take 30.6 us forward (a copy: 22.7)
+// and 47 + 6 backward (201 MB: 31 at 6.5 TB/s). Measured on the way: a whole row per warp reads w and b from L1 for every row, which takes as long as the
+// row (36 to 40 us); eight warps to a row 36; 84 registers of 512 threads leave one CTA an SM (71 us backward); w, dy and n kept in
+// registers instead of read and unpacked twice 62 -> 47.
 #include "fs_experts.cuh"
 #include "fs_ptx.cuh"
 
