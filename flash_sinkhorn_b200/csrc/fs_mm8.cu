@@ -12,10 +12,12 @@
 // TMEM (fp32); eight warps read that while the next block is summed beside it, and add it, scaled, to sums in registers.
 // Per block and 128 x 256 tile the products take 512 clocks of the tensor core, reading 256 of TMEM and adding 256 of the fp32 units, but
 // each of the two accumulators goes from the tensor core to the warps of both CTAs and back, which takes some 1200 clocks by itself: a
-// block takes 590 ns where loads and products alone take 373 (from HBM 550). 65536 rows of 64 experts, 2048 x 2048: 319 us, 1720 TFLOP/s, against
-// 390 us of the 16-bit product; with 1024 or 4096 contraction values 1450 and 1860 TFLOP/s (a tile costs 2 us besides its blocks).
-// What decided it: registers that spill in the loop of sums (a factor 1.5), loads of 16 columns a step ahead of the additions, results by TMA.
-// Barriers of their own for the two halves of a tile cost more than they saved (870 ns a block), so did factors read four blocks ahead.
+// block takes 550 ns, where loads and products alone take 373 (from HBM 550). 65536 rows of 64 experts, 2048 x 2048: 300 us, 1830 TFLOP/s, against
+// 390 us of the 16-bit product; with 1024 or 4096 contraction values 1510 and 2010 TFLOP/s (a tile costs 2 us besides its blocks).
+// What decided it: registers that spill in the loop of sums (a factor 1.5), loads of 16 columns a step ahead of the additions, results by TMA, and
+// in the wait for a block no more than a look: with its limit handled there in 64 bits, before the first look, the same product took 334 us.
+// Accumulators and barriers of their own for the two halves of a tile cost more than they saved (695 ns a block): products of 128 columns read as much
+// shared memory as it gives. So did factors read four blocks ahead.
 #include "fs_experts.cuh"
 #include "fs_pair.cuh"
 #include "fs_tc.cuh"
@@ -204,7 +206,7 @@ struct Mm8Args {
   int out_type, out_bytes;  // bytes of a store: 16, 4 or 2
   bool boxes;               // whole blocks of 32 rows are written by TMA
   int nstage;
-  long long limit;
+  unsigned limit;  // clocks that the warps which sum wait for a block of products; 0: none at all
 };
 
 template <int CG>
@@ -397,7 +399,8 @@ mm8_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapA, const __gr
     const uint32_t stages = smem_u32(staging + 8192 * (warp - kFirstSum));
     int buf = 0;
     uint32_t acc_ph = 0;
-    bool lost = false;  // a wait of this CTA gave up: NaN from here on
+    bool lost = a.limit == 0;  // a wait of this CTA gave up: NaN from here on
+    if (lost) *abort_flag = 1;
     uint32_t stage = stages;
     auto release = [&](bool whole) {  // the next staging tile: by the copy before last, or by all if no copy follows from this one
       if (a.boxes) {
@@ -659,7 +662,8 @@ mm8_short_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapW, cons
     // A lane has a feature; the rows' factors, a lane's for its row, are read four blocks ahead and handed round in shared memory.
     int buf = 0;
     uint32_t acc_ph = 0;
-    bool lost = false;  // a wait of this CTA gave up: NaN from here on
+    bool lost = a.limit == 0;  // a wait of this CTA gave up: NaN from here on
+    if (lost) *abort_flag = 1;
     float xs[kAhead], ws[kAhead];
     const float *sx = a.sx, *sw = a.sw;
     Tile8 next = {};
@@ -1100,7 +1104,7 @@ int fs_grouped_mm8(const void* x, int type, long long ldx, int M, const int* row
   const long long across = (w_cols + kBlock8 - 1) / kBlock8, down = (w_rows + kBlock8 - 1) / kBlock8;
   if (across * down > 0x7fffffffll) return report_error(FS_ERR_UNSUPPORTED, "too many blocks of 128 x 128 values");
   a.sw_expert = across * down; a.sw_n = transposed ? 1 : (int)across; a.sw_k = transposed ? (int)across : 1;
-  a.limit = product_limit();
+  a.limit = close_limit(product_limit());
   const int width = type_bytes(out_type);
   a.out_bytes = aligned(out, 16) && ldo * width % 16 == 0 && (long long)N * width % 16 == 0 ? 16
                 : aligned(out, 4) && ldo * width % 4 == 0 && (long long)N * width % 4 == 0  ? 4 : 2;

@@ -358,7 +358,8 @@ __device__ __forceinline__ void ortho_product(const OrthoArgs& a, const CUtensor
       }
     };
     int t = p.tiles, b = 0, m0 = 0, n0 = 0;
-    bool lost = *abort_flag != 0;  // a wait of this CTA gave up: NaN from here on
+    if (a.limit == 0) *abort_flag = 1;
+    bool lost = a.limit == 0 || *abort_flag != 0;  // a wait of this CTA gave up: NaN from here on
     if (first < total) {
       tiles.at(first, b, m0, n0);
       if (kFrom) ask(b, m0 + rank * 128 + q * 32, n0 + kCols * side);
@@ -369,7 +370,7 @@ __device__ __forceinline__ void ortho_product(const OrthoArgs& a, const CUtensor
       if (it + stride < total) tiles.at(it + stride, next_b, next_m, next_n);
       if (!lost) {
         lost = !__all_sync(0xffffffffu, CG == 2 ? wait_blocks(bar(ACC_FULL + buf), (t >> 1) & 1, abort_flag, blocks, a.limit)
-                                                : wait_close(bar(ACC_FULL + buf), (t >> 1) & 1, abort_flag, a.limit ? a.limit + 4096ll * blocks : 0));
+                                                : wait_close(bar(ACC_FULL + buf), (t >> 1) & 1, abort_flag, close_limit(a.limit + 4096ll * blocks)));
         tc_fence_after();
       }
 #pragma unroll 1

@@ -71,32 +71,21 @@ __device__ __forceinline__ bool wait_blocks(uint32_t bar, uint32_t parity, volat
   }
   return true;
 }
-// For a wait that ends within a microsecond, many times in a tile: without putting the thread to sleep.
-__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-__device__ __forceinline__ bool wait_close(uint32_t bar, uint32_t parity, volatile int* abort_flag, long long limit) {
-  if (limit == 0) *abort_flag = 1;  // without a look, for tests
-  if (limit == 0) return false;
-  if (mbar_test(bar, parity)) return true;
-  const long long t0 = clock64();
-  while (!mbar_test(bar, parity)) {
+// For a wait that ends within a microsecond, many times in a tile: `limit` clocks at most, which only the slow way looks at.
+__device__ __forceinline__ bool wait_close(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned limit) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const unsigned t0 = (unsigned)clock();
+  while (!mbar_try_wait(bar, parity)) {
     if (*abort_flag) return false;
-    if (clock64() - t0 > limit) {
+    if ((unsigned)clock() - t0 > limit) {
       *abort_flag = 1;
       return false;
     }
   }
   return true;
 }
+// A limit for it; 0: a CTA gives up at its first wait, without a look (for tests).
+__host__ __device__ __forceinline__ unsigned close_limit(long long clocks) { return clocks > (1ll << 30) ? 1u << 30 : (unsigned)clocks; }
 template <int CG>
 __device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
   if (CG == 2)
