@@ -11,14 +11,16 @@
 // 0.2 % for those matrices, below the rounding of a bf16 result. X is held times 2^8, A and P times 2^10, so that small entries
 // keep their bits: entries of X up to 255 and of P up to 63 in magnitude fit.
 //
-// A and P are symmetric: only tiles on and below the diagonal are computed, and written twice. The products are batched over the
+// A and P are symmetric: only tiles on and below the diagonal are computed, and written twice, unless there is a CTA for every tile: writing
+// twice takes 0.5 us then, the other tiles nothing (one matrix of 512 x 512: 106.5 -> 100.5 us). The products are batched over the
 // stack; tiles of 256 x 256 by pairs of CTAs, or 128 x 128 or 128 x 64 by single ones where there are too few. Small matrices go through all
 // products in one launch.
 //
 // 32 matrices of 2048 x 1024, five steps: 1346 us, of which a step's A takes 73, P 45 and P X 129 (without X's lower part 115); their floors are 52, 26 and
 // 83 at the burst rate of the tensor cores, a fifth more under the power cap, and what they lose besides is a partly filled round of tiles (4.3 rounds
-// of A and P count as 5) and 540 MB through HBM in the first steps' P X. One matrix of 512 x 512: 107 us, 15 products of 6 us each, of which 3 are
-// loads (a CTA's 192 KB at 60 bytes a clock), 1 the results and 2.5 the CTAs' meeting.
+// of A and P count as 5) and 540 MB through HBM in the first steps' P X. One matrix of 512 x 512: 86 us, 15 products of 5 us each, of which 2.2 are
+// loads (a CTA's 192 KB, at most 60 bytes a clock), 0.8 the results and 1.5 the CTAs' meeting. Divisions of 64 bits and spilled registers between its
+// products, which every thread waited for, had taken another us of each.
 #include "fs_experts.cuh"
 #include "fs_pair.cuh"
 #include "fs_tc.cuh"
@@ -137,6 +139,7 @@ struct OrthoArgs {
   void* out;  // LAST: [n, k] or, tall, [k, n]
   int out_type, out_bytes;
   bool tall;
+  bool whole;      // tiles of 64 columns: all of A and P are computed, none mirrored
   bool backwards;  // the last matrix first: it is what the product before left in L2
   int nstage;
   long long limit;
@@ -149,22 +152,22 @@ struct TilesO {
   __device__ explicit TilesO(const OrthoArgs& args) : a(args) {
     constexpr int BM = 128 * CG, R = BM / BN > 0 ? BM / BN : 1;
     mt = (a.n + BM - 1) / BM;
-    if (FORM >= APPLY) {
-      nt = (a.k + BN - 1) / BN;
+    nt = ((FORM >= APPLY ? a.k : a.n) + BN - 1) / BN;
+    if (all()) {
       per = mt * nt;
     } else {  // tiles (i, j) with j < (i + 1) R, as far as there are columns
-      nt = (a.n + BN - 1) / BN;
       per = R * mt * (mt - 1) / 2 + nt;
       if (per < 0) per = 0;
     }
   }
+  __device__ bool all() const { return FORM >= APPLY || (CG == 1 && BN == 64 && a.whole); }
   __device__ long long total() const { return (long long)per * a.batch; }
   __device__ void at(long long tile, int& b, int& m0, int& n0) const {
     constexpr int BM = 128 * CG, R = BM / BN > 0 ? BM / BN : 1;
-    b = (int)(tile / per);
+    b = BN == 64 ? (int)((unsigned)tile / (unsigned)per) : (int)(tile / per);  // narrow ones are few, and a division of 64 bits takes 100 clocks
     int rest = (int)(tile - (long long)b * per);
     if (a.backwards) b = a.batch - 1 - b;
-    if (FORM >= APPLY) {
+    if (all()) {
       const int j = rest / mt;
       m0 = (rest - j * mt) * BM;
       n0 = j * BN;
@@ -387,7 +390,7 @@ __device__ __forceinline__ void ortho_product(const OrthoArgs& a, const CUtensor
           else if (it + stride < total) ask(next_b, next_m + rank * 128 + q * 32, next_n + kCols * side);
         }
         if (col < width && row0 < a.n) {
-          const bool across = FORM == LAST ? a.tall : FORM <= SQUARE && n0 + BN <= m0;  // also, or only, written transposed
+          const bool across = FORM == LAST ? a.tall : FORM <= SQUARE && !tiles.all() && n0 + BN <= m0;  // also, or only, written transposed
           uint32_t w[kCols / 2];
 #pragma unroll
           for (int h = 0; h < kCols; h += 32) {
@@ -490,12 +493,13 @@ __device__ __forceinline__ void ortho_product(const OrthoArgs& a, const CUtensor
       n0 = next_n;
     }
   }
-  // every lane goes on from here, whichever one did the work
-  const int done = first < total ? (int)((total - first + stride - 1) / stride) : 0;
-  const long long past = p.s + (long long)done * blocks;
-  p.ph ^= (uint32_t)(past / p.nstage) & 1u;
-  p.s = (int)(past % p.nstage);
-  p.tiles += done;
+  // every lane goes on from here, whichever one did the work (in a chain of products, whose CTAs have few tiles)
+  for (long long it = first; it < total; it += stride) {
+    const unsigned past = p.s + blocks;
+    p.ph ^= past / p.nstage & 1u;
+    p.s = past % p.nstage;
+    ++p.tiles;
+  }
 }
 
 template <int CG, int BN>
@@ -544,7 +548,7 @@ struct OrthoChain {
 struct OrthoMaps {
   CUtensorMap x128[2], x64[2], a128, a64, p128;  // boxes of 128 or 64 rows
 };
-constexpr int kChainBN = 64, kChainTiles = 2;  // columns of a tile, and tiles of a CTA
+constexpr int kChainBN = 64, kChainTiles = 2, kChainStages = 8;  // columns of a tile, tiles of a CTA
 
 // What this CTA has written is there for the loads of all others behind it: the CTA's barrier and one thread's release order all of its
 // writes, and a fence of the thread that releases and of the one that loads orders them before tensor loads (which go another way to
@@ -569,14 +573,14 @@ __global__ void __launch_bounds__(kThreadsO, 1) ortho_chain_kernel(OrthoArgs a, 
   extern __shared__ uint8_t raw[];
   if (threadIdx.x < sizeof(OrthoMaps) / sizeof(CUtensorMap))
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<const CUtensorMap*>(&maps) + threadIdx.x) : "memory");
-  OrthoPipe p = ortho_begin<1, kChainBN>(raw, a.nstage);
+  OrthoPipe p = ortho_begin<1, kChainBN>(raw, kChainStages);
   unsigned target = 0;
 #pragma unroll 1
   for (int i = 0; i < c.steps; ++i) {
-    const int from = i & 1;
-    a.hi = c.x[from];
+    const bool from = i & 1;
+    a.hi = from ? c.x[1] : c.x[0];
     a.lo = i < c.lower_until ? c.lo : nullptr;
-    a.hi_out = c.x[from ^ 1];
+    a.hi_out = from ? c.x[0] : c.x[1];
     a.lo_out = i + 1 < c.lower_until ? c.lo : nullptr;
     a.sym = c.sym;
     ortho_product<GRAM, 1, kChainBN>(a, &maps.x128[from], &maps.x64[from], p);
@@ -633,6 +637,7 @@ int launch_ortho(OrthoArgs a, cudaStream_t st) {
   if (e != cudaSuccess) return report_error(FS_ERR_CUDA, cudaGetErrorString(e));
   const long long mt = (a.n + 128 * CG - 1) / (128 * CG), most = mt * (((FORM >= APPLY ? a.k : a.n) + BN - 1) / BN) * a.batch;
   long long grid = detail::free_ctas() / CG;
+  a.whole = most <= grid;
   if (grid > most) grid = most;
   if (grid < 1) grid = 1;
   cudaLaunchConfig_t cfg{};
@@ -666,8 +671,8 @@ int launch_chain(OrthoArgs a, const OrthoChain& c, cudaStream_t st) {
       !encode_stack(&maps.p128, c.poly, a.n, a.n, a.batch, a.lda, 128))
     return report_error(FS_ERR_CUDA, "cuTensorMapEncodeTiled failed");
   constexpr size_t kStage = 128 * 128 + kChainBN * 128, fixed = 1024 + ortho_staging(kChainBN) + 8 * (2 * 12 + 5) + 8;
-  a.nstage = (int)((kSmemMax - fixed) / kStage);
-  static_assert(fixed + 8 * kStage >= (size_t)kSmemMin && (kSmemMax - fixed) / kStage == 8, "shared memory");
+  constexpr size_t smem = fixed + kChainStages * kStage;
+  static_assert(smem >= (size_t)kSmemMin && smem <= kSmemMax, "shared memory");
   static std::atomic<uint64_t> allowed{0};  // devices on which the kernel may take all shared memory
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -677,11 +682,12 @@ int launch_chain(OrthoArgs a, const OrthoChain& c, cudaStream_t st) {
     if (e == cudaSuccess) allowed.fetch_or(bit, std::memory_order_relaxed);
   }
   if (e != cudaSuccess) return report_error(FS_ERR_CUDA, cudaGetErrorString(e));
-  const long long most = (a.n + 127) / 128 * ((a.k + kChainBN - 1) / kChainBN) * a.batch;
+  const long long high = (a.n + 127) / 128 * a.batch, most = high * ((a.k + kChainBN - 1) / kChainBN);
+  a.whole = high * ((a.n + kChainBN - 1) / kChainBN) <= detail::free_ctas();
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(most < detail::free_ctas() ? most : detail::free_ctas()));
   cfg.blockDim = dim3(kThreadsO);
-  cfg.dynamicSmemBytes = fixed + a.nstage * kStage;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeCooperative;
