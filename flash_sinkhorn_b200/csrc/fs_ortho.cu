@@ -371,11 +371,6 @@ __device__ __forceinline__ void ortho_product(const OrthoArgs& a, const CUtensor
       const int buf = t & 1, row0 = m0 + rank * 128 + q * 32, row = row0 + lane;
       int next_b = 0, next_m = 0, next_n = 0;
       if (it + stride < total) tiles.at(it + stride, next_b, next_m, next_n);
-      if (!lost) {
-        lost = !__all_sync(0xffffffffu, CG == 2 ? wait_blocks(bar(ACC_FULL + buf), (t >> 1) & 1, abort_flag, blocks, a.limit)
-                                                : wait_close(bar(ACC_FULL + buf), (t >> 1) & 1, abort_flag, close_limit(a.limit + 4096ll * blocks)));
-        tc_fence_after();
-      }
 #pragma unroll 1
       for (int c = kCols * side; c < BN; c += 2 * kCols) {
         const int col = n0 + c;
@@ -388,6 +383,11 @@ __device__ __forceinline__ void ortho_product(const OrthoArgs& a, const CUtensor
           __syncwarp();
           if (c + 2 * kCols < BN) ask(b, row0, col + 2 * kCols);
           else if (it + stride < total) ask(next_b, next_m + rank * 128 + q * 32, next_n + kCols * side);
+        }
+        if (c == kCols * side && !lost) {
+          lost = !__all_sync(0xffffffffu, CG == 2 ? wait_blocks(bar(ACC_FULL + buf), (t >> 1) & 1, abort_flag, blocks, a.limit)
+                                                  : wait_close(bar(ACC_FULL + buf), (t >> 1) & 1, abort_flag, close_limit(a.limit + 4096ll * blocks)));
+          tc_fence_after();
         }
         if (col < width && row0 < a.n) {
           const bool across = FORM == LAST ? a.tall : FORM <= SQUARE && !tiles.all() && n0 + BN <= m0;  // also, or only, written transposed
