@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(256) squares_kernel(const T* g, long long g_ma
 template <typename T, int V>
 __global__ void __launch_bounds__(256) begin_kernel(const T* g, long long g_matrix, long long g_row, int rows, int cols, const double* parts, int count,
                                                     float eps, bool tall, __half* hi, __half* lo, long long ldx, unsigned* meeting) {
-  __shared__ float tile[64][65];
+  __shared__ float tile[64][65], factor;
   if (blockIdx.x + blockIdx.y + blockIdx.z + threadIdx.x == 0) *meeting = 0u;
   const int b = blockIdx.z, r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
   constexpr int kLanes = 64 / V;  // to a row of the tile
@@ -93,13 +93,15 @@ __global__ void __launch_bounds__(256) begin_kernel(const T* g, long long g_matr
 #pragma unroll
     for (int j = 0; j < V; ++j) tile[y][x + j] = v[j];
   }
-  // every warp adds the sums of squares in the same order
-  double s = 0.0;
-  for (int i = threadIdx.x & 31; i < count; i += 32) s += parts[b * count + i];
+  if (threadIdx.x < 32) {  // one warp: square roots of 64 bits are dear
+    double s = 0.0;
+    for (int i = threadIdx.x; i < count; i += 32) s += parts[b * count + i];
 #pragma unroll
-  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  const float f = (float)((double)kXScale / (sqrt(s) + (double)eps));
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (threadIdx.x == 0) factor = (float)((double)kXScale / (sqrt(s) + (double)eps));
+  }
   __syncthreads();
+  const float f = factor;
   const int n = tall ? cols : rows, k = tall ? rows : cols, n0 = tall ? c0 : r0, k0 = tall ? r0 : c0;
 #pragma unroll
   for (int y = threadIdx.x >> 3; y < 64; y += 32) {
