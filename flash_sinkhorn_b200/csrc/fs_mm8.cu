@@ -569,6 +569,7 @@ __global__ void __launch_bounds__(kShortThreads, 2)
 mm8_short_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUtensorMap mapX) {
   constexpr uint32_t kStage = kTileA + kShortRows * 128, kColumns = 256;
   constexpr int kBufs = kColumns / kShortRows, kAhead = 4;
+  static_assert(kBufs % 2 == 0, "buffers of factors");
   extern __shared__ uint8_t raw[];
   __shared__ __align__(16) float factors[4][2][kShortRows];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
@@ -690,7 +691,9 @@ mm8_short_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapW, cons
 #pragma unroll
         for (int d = 0; d < kAhead; ++d) {
           if (k0 + d >= t.blocks || lost) continue;
-          float* mine = factors[warp][d & 1];
+          // Two buffers in turn, from tile to tile too (kBufs is even): every lane has passed the other buffer's barrier, behind its last read of
+          // this one, before any writes here again.
+          float* mine = factors[warp][buf & 1];
           mine[lane] = xs[d] * ws[d];
           ask(k0 + d + kAhead, d);
           __syncwarp();
