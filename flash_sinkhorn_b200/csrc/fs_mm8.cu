@@ -286,7 +286,7 @@ mm8_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapA, const __gr
   const int FULL = 0, EMPTY = a.nstage, ACC_FULL = 2 * a.nstage, ACC_EMPTY = ACC_FULL + kBufs, DRAIN = ACC_EMPTY + kBufs;
   uint32_t* slot = reinterpret_cast<uint32_t*>(bars + DRAIN + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(slot + 1);
-  int *gs = reinterpret_cast<int*>(slot + 2), *ts = gs + a.E + 2;
+  int *words = reinterpret_cast<int*>(slot + 2), *gs = words + 4, *ts = gs + a.E + 2;
   auto bar = [&](int i) { return smem_u32(bars + i); };
 
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -306,6 +306,7 @@ mm8_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapA, const __gr
     }
     mbar_init(bar(DRAIN), 1);
     *abort_flag = 0;
+    words[0] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   } else if (warp == kIssueWarp) {
@@ -318,13 +319,11 @@ mm8_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapA, const __gr
   const uint32_t tmem = *slot;
   Tiles8<128 * CG, BN> tiles(a, gs, ts);
   const int total = tiles.total();
-  int issued = 0;  // stages that this CTA's loading thread has started
-
   if (warp < kFirstSum) {
     if (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     // ===================== loads =====================
     if (warp == kFetchWarp && elect_one()) {
-      int s = 0;
+      int s = 0, issued = 0;
       uint32_t ph = 0;
       bool ok = true;
       for (int it = first; ok && it < total; it += stride) {
@@ -352,6 +351,7 @@ mm8_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapA, const __gr
           }
         }
       }
+      words[0] = issued;
     }
     // ===================== products =====================
     if (warp == kIssueWarp && rank == 0 && elect_one()) {
@@ -527,31 +527,7 @@ mm8_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapA, const __gr
     }
     if (a.boxes && lane == 0) bulk_done();
   }
-  __syncwarp();
-  tc_fence_before();
-  __syncthreads();
-  if (*abort_flag) {  // nobody waits any more, and the flag does not change
-    if (warp == kIssueWarp && rank == 0) {  // every product issued here ends before TMEM is freed
-      if (elect_one()) {
-        commit<CG>(bar(DRAIN));
-        mbar_wait_quiet(bar(DRAIN), 0);
-      }
-      __syncwarp();
-    } else if (warp == kFetchWarp) {
-      // The copies in flight land before the CTA ends; those of the second CTA of a pair, which the first one counts, are
-      // given a millisecond, hundreds of times what a copy takes.
-      if (elect_one()) {
-        const long long t0 = clock64();
-        if (rank == 0)
-          for (int j = issued > a.nstage ? issued - a.nstage : 0; j < issued; ++j) wait_landed(bar(FULL + j % a.nstage), (j / a.nstage) & 1, t0);
-        else
-          while (clock64() - t0 < (1ll << 21)) {}
-      }
-      __syncwarp();
-    }
-  }
-  if (CG == 2) cluster_sync_all();
-  tc_fence_after();
+  settle<CG, 1>(abort_flag, words, bar(FULL), bar(DRAIN), a.nstage, warp == kIssueWarp, warp == kFetchWarp);
   if (warp == kIssueWarp) free_columns<CG>(tmem, kColumns);
   if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_mm8_error, 1);
 }
@@ -577,7 +553,7 @@ mm8_short_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapW, cons
   const int FULL = 0, EMPTY = a.nstage, ACC_FULL = 2 * a.nstage, ACC_EMPTY = ACC_FULL + kBufs, DRAIN = ACC_EMPTY + kBufs;
   uint32_t* slot = reinterpret_cast<uint32_t*>(bars + DRAIN + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(slot + 1);
-  int *gs = reinterpret_cast<int*>(slot + 2), *ts = gs + a.E + 2;
+  int *words = reinterpret_cast<int*>(slot + 2), *gs = words + 4, *ts = gs + a.E + 2;
   auto bar = [&](int i) { return smem_u32(bars + i); };
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int first = blockIdx.x, stride = gridDim.x;
@@ -587,6 +563,7 @@ mm8_short_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapW, cons
   } else if (warp == kShortFetch && lane == 0) {
     for (int s = 0; s < 2 * a.nstage + 2 * kBufs + 1; ++s) mbar_init(bar(s), s >= ACC_EMPTY && s < DRAIN ? 4 : 1);
     *abort_flag = 0;
+    words[0] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   } else if (warp == kShortIssue) {
@@ -598,12 +575,11 @@ mm8_short_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapW, cons
   const uint32_t tmem = *slot;
   Tiles8<kShortRows, 128> tiles(a, gs, ts);
   const int total = tiles.total();
-  int issued = 0;
 
   if (warp == kShortFetch) {
     // ===================== loads =====================
     if (elect_one()) {
-      int s = 0;
+      int s = 0, issued = 0;
       uint32_t ph = 0;
       bool ok = true;
       for (int it = first; ok && it < total; it += stride) {
@@ -624,6 +600,7 @@ mm8_short_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapW, cons
           }
         }
       }
+      words[0] = issued;
     }
   } else if (warp == kShortIssue) {
     // ===================== products =====================
@@ -739,25 +716,7 @@ mm8_short_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapW, cons
       }
     }
   }
-  __syncwarp();
-  tc_fence_before();
-  __syncthreads();
-  if (*abort_flag) {  // nobody waits any more, and the flag does not change: products and copies in flight end first
-    if (warp == kShortIssue) {
-      if (elect_one()) {
-        commit<1>(bar(DRAIN));
-        mbar_wait_quiet(bar(DRAIN), 0);
-      }
-      __syncwarp();
-    } else if (warp == kShortFetch) {
-      if (elect_one()) {
-        const long long t0 = clock64();
-        for (int j = issued > a.nstage ? issued - a.nstage : 0; j < issued; ++j) wait_landed(bar(FULL + j % a.nstage), (j / a.nstage) & 1, t0);
-      }
-      __syncwarp();
-    }
-  }
-  tc_fence_after();
+  settle<1, 1>(abort_flag, words, bar(FULL), bar(DRAIN), a.nstage, warp == kShortIssue, warp == kShortFetch);
   if (warp == kShortIssue) free_columns<1>(tmem, kColumns);
   if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_mm8_error, 1);
 }
@@ -936,7 +895,7 @@ int launch_mm8(Mm8Args a, const uint8_t* x, long long ldx, const uint8_t* w, lon
       (a.boxes && !encode_out(&mapC, a.out_type, a.out, a.N, a.R, a.ldo)))
     return report_error(FS_ERR_CUDA, "cuTensorMapEncodeTiled failed");
   constexpr size_t kStage = kTileA + BN / CG * 128;
-  const size_t fixed = 1024 + kStage8 + 8 * (2 * 12 + 9) + 8 + 8 * ((size_t)a.E + 2);
+  const size_t fixed = 1024 + kStage8 + 8 * (2 * 12 + 9) + 24 + 8 * ((size_t)a.E + 2);
   a.nstage = (int)((kSmemMax - fixed) / kStage);
   if (a.nstage > 12) a.nstage = 12;
   size_t smem = fixed + a.nstage * kStage;
@@ -979,9 +938,9 @@ int launch_short8(Mm8Args a, const uint8_t* x, long long ldx, const uint8_t* w, 
   if (!encode8(&mapW, w, 3, {a.K, a.N, a.E}, {w_row, w_expert ? w_expert : w_row}, 128) || !encode8(&mapX, x, 2, {a.K, a.R, 1}, {ldx, 0}, kShortRows))
     return report_error(FS_ERR_CUDA, "cuTensorMapEncodeTiled failed");
   constexpr size_t kStage = kTileA + kShortRows * 128, kStatic = 4 * 2 * kShortRows * sizeof(float);
-  const size_t fixed = 1024 + 8 * (2 * 8 + 2 * (256 / kShortRows) + 1) + 8 + 8 * ((size_t)a.E + 2);
+  const size_t fixed = 1024 + 8 * (2 * 8 + 2 * (256 / kShortRows) + 1) + 24 + 8 * ((size_t)a.E + 2);
   a.nstage = (int)((kShortSmem - kStatic - fixed) / kStage);
-  static_assert((kShortSmem - kStatic - 1024 - 8 * 33 - 8 - 8 * 1026) / kStage >= 4 && (kShortSmem / kStage) <= 8, "stages");
+  static_assert((kShortSmem - kStatic - 1024 - 8 * 33 - 24 - 8 * 1026) / kStage >= 4 && (kShortSmem / kStage) <= 8, "stages");
   const auto kernel = mm8_short_kernel;
   static std::atomic<uint64_t> allowed{0};  // devices on which the kernel may take that much shared memory
   int dev = 0;

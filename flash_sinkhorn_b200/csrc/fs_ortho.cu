@@ -196,6 +196,7 @@ struct OrthoPipe {
   uint8_t *ring, *staging;
   uint64_t* bars;
   volatile int* abort_flag;
+  int* words;  // of settle()
   uint32_t tmem;
   int nstage, warp, lane, rank;
   int s;        // next stage
@@ -220,6 +221,7 @@ __device__ __forceinline__ OrthoPipe ortho_begin(uint8_t* raw, int nstage) {
   p.nstage = nstage;
   uint32_t* slot = reinterpret_cast<uint32_t*>(p.bars + p.drain() + 1);
   p.abort_flag = reinterpret_cast<volatile int*>(slot + 1);
+  p.words = reinterpret_cast<int*>(slot + 2);
   p.warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);
   p.lane = threadIdx.x & 31;
   p.rank = CG == 2 ? (int)cta_rank() : 0;
@@ -235,7 +237,7 @@ __device__ __forceinline__ OrthoPipe ortho_begin(uint8_t* raw, int nstage) {
       mbar_init(p.bar(p.acc_empty() + i), kWriteWarps * CG);  // in CTA 0: all warps of the pair that write
     }
     mbar_init(p.bar(p.drain()), 1);
-    *p.abort_flag = 0;
+    *p.abort_flag = p.words[0] = p.words[1] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   } else if (p.warp == kMulWarp) {
@@ -270,7 +272,7 @@ __device__ __forceinline__ void ortho_product(const OrthoArgs& a, const CUtensor
     // A warp for each operand: one thread takes 150 to 200 clocks for a tensor load, and a stage of P X has three of them for products of 512
     // (32 matrices of 2048 x 1024: 1405 -> 1346 us).
     if (elect_one()) {
-      int s = p.s;
+      int s = p.s, issued = 0;
       uint32_t ph = p.ph;
       bool ok = *abort_flag == 0;  // a CTA that has given up starts nothing more
       for (long long it = first; ok && it < total; it += stride) {
@@ -294,12 +296,14 @@ __device__ __forceinline__ void ortho_product(const OrthoArgs& a, const CUtensor
               load_3d<CG>(dst + kA, mapB, kb * 64, n0 + rank * BNC, b, full);
             }
           }
+          ++issued;
           if (++s == p.nstage) {
             s = 0;
             ph ^= 1;
           }
         }
       }
+      p.words[warp == kGetWarp ? 0 : 1] += issued;
     }
   } else if (warp == kMulWarp) {
     // ===================== products =====================
@@ -509,27 +513,7 @@ __device__ __forceinline__ void ortho_product(const OrthoArgs& a, const CUtensor
 
 template <int CG, int BN>
 __device__ __forceinline__ void ortho_end(const OrthoPipe& p) {
-  __syncwarp();
-  tc_fence_before();
-  __syncthreads();
-  if (*p.abort_flag) {  // nobody waits any more, and the flag does not change
-    if (p.warp == kMulWarp && p.rank == 0) {  // every product issued here ends before TMEM is freed
-      if (elect_one()) {
-        commit<CG>(p.bar(p.drain()));
-        mbar_wait_quiet(p.bar(p.drain()), 0);
-      }
-      __syncwarp();
-    } else if (p.warp == kGetWarp) {
-      // The copies in flight land before the CTA ends: they are given a millisecond, hundreds of times what a copy takes.
-      if (elect_one()) {
-        const long long t0 = clock64();
-        while (clock64() - t0 < (1ll << 21)) {}
-      }
-      __syncwarp();
-    }
-  }
-  if (CG == 2) cluster_sync_all();
-  tc_fence_after();
+  settle<CG, 2>(p.abort_flag, p.words, p.bar(p.full()), p.bar(p.drain()), p.nstage, p.warp == kMulWarp, p.warp == kGetWarp);
   if (p.warp == kMulWarp) free_columns<CG>(p.tmem, 2 * BN);
   if (threadIdx.x == 0 && *p.abort_flag) atomicExch(&g_ortho_error, 1);
 }
@@ -558,7 +542,7 @@ constexpr int kChainBN = 64, kChainTiles = 2, kChainStages = 8;  // columns of a
 // What this CTA has written is there for the loads of all others behind it: the CTA's barrier and one thread's release order all of its
 // writes, and a fence of the thread that releases and of the one that loads orders them before tensor loads (which go another way to
 // memory). The same fences by all threads took 3 us.
-__device__ __forceinline__ void ortho_meet(const OrthoPipe& p, unsigned* meeting, unsigned target) {
+__device__ __forceinline__ void ortho_meet(const OrthoPipe& p, unsigned* meeting, unsigned target, long long limit) {
   __syncthreads();
   if (threadIdx.x == 0 && !*p.abort_flag) {
     unsigned seen;
@@ -567,7 +551,7 @@ __device__ __forceinline__ void ortho_meet(const OrthoPipe& p, unsigned* meeting
     const long long t0 = clock64();
     do {
       asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(meeting) : "memory");
-      if (seen < target && clock64() - t0 > kSpinLimit) *p.abort_flag = 1;
+      if (seen < target && clock64() - t0 > limit) *p.abort_flag = 1;
     } while (seen < target && !*p.abort_flag);
   }
   __syncthreads();
@@ -589,14 +573,14 @@ __global__ void __launch_bounds__(kThreadsO, 1) ortho_chain_kernel(OrthoArgs a, 
     a.lo_out = i + 1 < c.lower_until ? c.lo : nullptr;
     a.sym = c.sym;
     ortho_product<GRAM, 1, kChainBN>(a, &maps.x128[from], &maps.x64[from], p);
-    ortho_meet(p, c.meeting, target += gridDim.x);
+    ortho_meet(p, c.meeting, target += gridDim.x, a.limit);
     a.a = c.sym;
     a.sym = c.poly;
     ortho_product<SQUARE, 1, kChainBN>(a, &maps.a128, &maps.a64, p);
-    ortho_meet(p, c.meeting, target += gridDim.x);
+    ortho_meet(p, c.meeting, target += gridDim.x, a.limit);
     if (i + 1 < c.steps) {
       ortho_product<APPLY, 1, kChainBN>(a, &maps.p128, &maps.x64[from], p);
-      ortho_meet(p, c.meeting, target += gridDim.x);
+      ortho_meet(p, c.meeting, target += gridDim.x, a.limit);
     } else {
       ortho_product<LAST, 1, kChainBN>(a, &maps.p128, &maps.x64[from], p);
     }
@@ -625,7 +609,7 @@ int launch_ortho(OrthoArgs a, cudaStream_t st) {
                        : encode_stack(&mapA, left, a.n, a.n, a.batch, a.lda, 128) && encode_stack(&mapB, a.hi, a.k, a.n, a.batch, a.ldx, 64);
   if (!good) return report_error(FS_ERR_CUDA, "cuTensorMapEncodeTiled failed");
   constexpr size_t kStage = 128 * 128 + BN / CG * 128;
-  constexpr size_t fixed = 1024 + ortho_staging(BN) + 8 * (2 * 12 + 5) + 8;
+  constexpr size_t fixed = 1024 + ortho_staging(BN) + 8 * (2 * 12 + 5) + 32;
   a.nstage = (int)((kSmemMax - fixed) / kStage);
   if (a.nstage > 12) a.nstage = 12;
   size_t smem = fixed + a.nstage * kStage;
@@ -675,7 +659,7 @@ int launch_chain(OrthoArgs a, const OrthoChain& c, cudaStream_t st) {
   if (!encode_stack(&maps.a128, c.sym, a.n, a.n, a.batch, a.lda, 128) || !encode_stack(&maps.a64, c.sym, a.n, a.n, a.batch, a.lda, 64) ||
       !encode_stack(&maps.p128, c.poly, a.n, a.n, a.batch, a.lda, 128))
     return report_error(FS_ERR_CUDA, "cuTensorMapEncodeTiled failed");
-  constexpr size_t kStage = 128 * 128 + kChainBN * 128, fixed = 1024 + ortho_staging(kChainBN) + 8 * (2 * 12 + 5) + 8;
+  constexpr size_t kStage = 128 * 128 + kChainBN * 128, fixed = 1024 + ortho_staging(kChainBN) + 8 * (2 * 12 + 5) + 32;
   constexpr size_t smem = fixed + kChainStages * kStage;
   static_assert(smem >= (size_t)kSmemMin && smem <= kSmemMax, "shared memory");
   static std::atomic<uint64_t> allowed{0};  // devices on which the kernel may take all shared memory

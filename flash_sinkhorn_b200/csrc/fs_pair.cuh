@@ -154,6 +154,54 @@ __device__ __forceinline__ void free_columns(uint32_t addr, uint32_t n) {
   else tmem_dealloc(addr, n);
 }
 
+// The end of a kernel whose waits are bounded, for all threads, behind their roles: if one of them gave up (in either CTA of a pair), the products
+// and tensor loads in flight end before TMEM and shared memory are given back. `words`, in shared memory: the stages that each of LOADERS warps has
+// started, counted over the launch, and with pairs LOADERS + 1 words for what the other CTA says. A stage's full barrier (the leader's, `full` the first)
+// takes one arrival of each loader of each CTA and the bytes of its loads. A loader is at most nstage stages ahead of another one, so those that
+// only some of them have started are all in their barriers' present phases: the leader arrives there for the others and then waits
+// for the bytes. Without anything given up this costs a pair two stores.
+template <int CG, int LOADERS>
+__device__ __forceinline__ void settle(volatile int* abort_flag, int* words, uint32_t full, uint32_t drain, int nstage, bool multiplies, bool loads) {
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();  // nobody waits any more, and the flag does not change
+  bool gave_up = *abort_flag != 0;
+  if (CG == 2) {
+    if (threadIdx.x == 0) {  // while the other CTA is there for certain
+      uint32_t to;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(words + LOADERS)), "r"(cta_rank() ^ 1u));
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"((uint32_t)gave_up) : "memory");
+#pragma unroll
+      for (int i = 0; i < LOADERS; ++i) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to + 4 + 4 * i), "r"(words[i]) : "memory");
+    }
+    __syncwarp();
+    cluster_sync_all();
+    gave_up |= words[LOADERS] != 0;
+  }
+  if (gave_up) {
+    if (CG == 1 || cta_rank() == 0) {
+      if (multiplies) {
+        if (elect_one()) {
+          commit<CG>(drain);
+          mbar_wait_quiet(drain, 0);
+        }
+      } else if (loads) {
+        if (elect_one()) {
+          int last = 0;
+          for (int i = 0; i < CG * LOADERS; ++i) last = max(last, words[i < LOADERS ? i : i + 1]);
+          for (int i = 0; i < CG * LOADERS; ++i)
+            for (int j = words[i < LOADERS ? i : i + 1]; j < last; ++j) mbar_arrive(full + 8 * (j % nstage));
+          const long long t0 = clock64();
+          for (int j = max(last - nstage, 0); j < last; ++j) wait_landed(full + 8 * (j % nstage), (j / nstage) & 1, t0);
+        }
+      }
+      __syncwarp();
+    }
+    if (CG == 2) cluster_sync_all();
+  }
+  tc_fence_after();
+}
+
 // First rows of the groups (running maximum of the offsets within [0, R]), of the rows of no expert (gs[E]) and the end
 // (gs[E + 1]); with TILES the number of tiles before each of them. One warp.
 template <bool TILES>

@@ -511,7 +511,7 @@ int fs_grouped_mm(const void* x, long long ldx, int M, const int* rows, int R, c
                   long long ldo, int type, void* stream);
 
 /* SM clocks that the writers of a product's results wait for it, besides 4096 for each 64 values of its contraction, before the
- * thread block gives up. Negative: the default, 2^28. Holds for the products that the calling thread launches (in a backward
+ * thread block gives up; also those that the blocks of one launch of fs_orthogonalize wait for one another. Negative: the default, 2^28. Holds for the products that the calling thread launches (in a backward
  * pass that is the thread of autograd). Returns the previous value. For tests of that path: with 0 all blocks give up at once. */
 long long fs_set_product_limit(long long clocks);
 
