@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(V * NV <= (V > 1 ? 16 : 8) ? 256 : kMaxNormThr
 // Rows under way, with the one that is worked on, by a thread's bytes of a row and its gradient: two CTAs of 96 KB to an SM, or one of 192 KB.
 __host__ __device__ constexpr int norm_stages(int bytes) { return bytes <= 64 ? 6 : bytes <= 128 ? 3 : bytes <= 256 ? 3 : 1; }
 
-// The gradients, from mean and rstd as the forward pass left them. SUMS: those to w and b as well; up to 16 values of a thread, of which w and what
+// The gradients, from mean and rstd as the forward pass left them, as r u - r mean(u) - n r mean(u n). SUMS: those to w and b as well; up to 16 values of a thread, of which w and what
 // both passes over them need stay in registers (read and unpacked again, they took a third of all instructions).
 template <typename T, typename W, int V, int NV, bool SUMS>
 __global__ void __launch_bounds__(256, SUMS ? 2 : 1) norm_grad_kernel(const NormArgs a) {
@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(256, SUMS ? 2 : 1) norm_grad_kernel(const Norm
   for (int s = 0, turn = 0; left > 0; --left, s = s + 1 == S ? 0 : s + 1, turn ^= 1) {
     ask(s ? s - 1 : S - 1);
     const float r = next_r;
-    const u64 r2 = pk(r, r), shift = pk(-next_mean * r, V == 1 ? 0.f : -next_mean * r);  // n = x r + shift
+    const u64 r2 = pk(r, r), less = pk(-next_mean, V == 1 ? 0.f : -next_mean);
     if (left > 1) {
       mean += stride;
       rstd += stride;
@@ -319,7 +319,7 @@ __global__ void __launch_bounds__(256, SUMS ? 2 : 1) norm_grad_kernel(const Norm
       pairs<T, V>(pg[i * blockDim.x], u[k]);
       if (!SUMS) columns<W, V>(a.w, (i * a.group + t) * V, 1.f, w[0]);
 #pragma unroll
-      for (int j = 0; j < P; ++j) n[k][j] = fma2(n[k][j], r2, shift);
+      for (int j = 0; j < P; ++j) n[k][j] = mul2(add2(n[k][j], less), r2);  // as the forward pass: x r - mean r would round a large mean twice
     };
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -333,15 +333,16 @@ __global__ void __launch_bounds__(256, SUMS ? 2 : 1) norm_grad_kernel(const Norm
           dw[k][j] = fma2(u[k][j], n[k][j], dw[k][j]);
           db[k][j] = add2(db[k][j], u[k][j]);
         }
-        const u64 v = mul2(u[k][j], w[k][j]);
-        su = add2(su, v);
-        sn = fma2(v, n[k][j], sn);
+        u[k][j] = mul2(u[k][j], w[k][j]);
+        su = add2(su, u[k][j]);
+        sn = fma2(u[k][j], n[k][j], sn);
       }
     }
     if (!out) continue;
     float sum[2] = {both(su), both(sn)};
     group_sum(sum, slots[turn][g], warps, 1 + g);
-    const u64 m1 = pk(-sum[0] * per, -sum[0] * per), m2 = pk(-sum[1] * per, -sum[1] * per);
+    const float r1 = -sum[0] * per * r, rn = -sum[1] * per * r;
+    const u64 m1 = pk(r1, r1), m2 = pk(rn, rn);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       constexpr int kOne = SUMS ? 1 : 0;
@@ -349,7 +350,7 @@ __global__ void __launch_bounds__(256, SUMS ? 2 : 1) norm_grad_kernel(const Norm
       if (!in[i]) continue;
       if (!SUMS) read(i, 0);
 #pragma unroll
-      for (int j = 0; j < P; ++j) n[k][j] = mul2(r2, fma2(m2, n[k][j], fma2(u[k][j], w[k][j], m1)));
+      for (int j = 0; j < P; ++j) n[k][j] = fma2(m2, n[k][j], fma2(SUMS ? u[k][j] : mul2(u[k][j], w[k][j]), r2, m1));
       store_pairs<T, V>(out + i * a.group * V, n[k]);
     }
     out += out_step;
@@ -472,7 +473,7 @@ __global__ void __launch_bounds__(256) norm_columns_kernel(const NormArgs a) {
     const long long stride = 8ll * gridDim.y;
     for (long long row = blockIdx.y * 8 + warp; row < a.rows; row += stride * kDeep) {
       Pack<T, V> px[kDeep], pg[kDeep];
-      float r[kDeep], shift[kDeep];
+      float r[kDeep], mean[kDeep];
 #pragma unroll
       for (int d = 0; d < kDeep; ++d) {
         const long long at = row + d * stride;
@@ -480,7 +481,7 @@ __global__ void __launch_bounds__(256) norm_columns_kernel(const NormArgs a) {
         px[d] = read_only<T, V>(static_cast<const T*>(a.x) + at * a.ldx + c);
         pg[d] = read_only<T, V>(static_cast<const T*>(a.dy) + at * a.lddy + c);
         r[d] = __ldg(a.rstd + at);
-        shift[d] = -__ldg(a.mean + at) * r[d];
+        mean[d] = __ldg(a.mean + at);
       }
 #pragma unroll
       for (int d = 0; d < kDeep; ++d) {
@@ -490,7 +491,7 @@ __global__ void __launch_bounds__(256) norm_columns_kernel(const NormArgs a) {
         unpack<T, V>(pg[d], dy);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          dw[j] = fmaf(dy[j], fmaf(x[j], r[d], shift[d]), dw[j]);
+          dw[j] = fmaf(dy[j], (x[j] - mean[d]) * r[d], dw[j]);
           db[j] += dy[j];
         }
       }
