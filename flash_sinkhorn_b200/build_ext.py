@@ -21,7 +21,7 @@ OUT = os.path.join(HERE, "lib", "libflashsinkhorn_b200.so")
 BINDING = os.path.join(HERE, "lib", "fs_torch.so")
 BINDING_SOURCE = "fs_torch.cpp"
 SOURCES = ["fs_api.cu", "fs_simt.cu", "fs_tc.cu", "fs_tck.cu", "fs_sym.cu", "fs_static.cu", "fs_micro.cu",
-           "fs_experts.cu", "fs_group.cu", "fs_norm.cu", "fs_mm8.cu", "fs_ortho.cu"]
+           "fs_experts.cu", "fs_group.cu", "fs_norm.cu", "fs_mm8.cu", "fs_ortho.cu", "fs_health.cu"]
 FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC",

@@ -527,13 +527,9 @@ namespace fs {
 int report_error(int code, const char* msg) { return fail(code, "%s", msg); }
 // Lets them add the kernels they enqueue themselves to the count behind fs_launch_count().
 void count_launches(int k) { g_launches.fetch_add(k, std::memory_order_relaxed); }
-namespace ex {  // fs_group.cu
-int group_error_flag();
-int clear_group_error_flag();
-int mm8_error_flag();
-int clear_mm8_error_flag();
-int ortho_error_flag();
-int clear_ortho_error_flag();
+namespace ex {  // fs_health.cu
+int products_error_flag();
+int clear_products_error_flag();
 }  // namespace ex
 }  // namespace fs
 
@@ -546,18 +542,13 @@ int fs_version(void) { return 200; }  // 0.2.0
 long long fs_launch_count(void) { return g_launches.load(std::memory_order_relaxed); }
 
 int fs_device_error(void) {
-  const int parts[] = {tc::read_error_flag(), sym::read_error_flag(), ex::group_error_flag(), ex::mm8_error_flag(), ex::ortho_error_flag()};
-  int all = 0;
-  for (int p : parts) all = p < 0 || all < 0 ? -1 : all | p;
-  return all;
+  const int a = tc::read_error_flag(), b = sym::read_error_flag(), c = ex::products_error_flag();
+  return a < 0 || b < 0 || c < 0 ? -1 : (a | b | c);
 }
 
 int fs_clear_device_error(void) {
-  const int parts[] = {tc::clear_error_flag(), sym::clear_error_flag(), ex::clear_group_error_flag(), ex::clear_mm8_error_flag(),
-                       ex::clear_ortho_error_flag()};
-  for (int p : parts)
-    if (p) return p;
-  return 0;
+  const int a = tc::clear_error_flag(), b = sym::clear_error_flag(), c = ex::clear_products_error_flag();
+  return a ? a : b ? b : c;
 }
 
 size_t fs_apply_mat_plan_bytes(int n, int m, int d, int dv, int prec) {

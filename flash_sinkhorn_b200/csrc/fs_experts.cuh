@@ -17,6 +17,8 @@ int report_error(int code, const char* msg);  // fs_api.cu: records the calling 
 void count_launches(int k);                   // fs_api.cu: adds to the count behind fs_launch_count()
 
 namespace ex {
+int* products_health();  // fs_health.cu: where a kernel whose bounded wait gave up says so; null after an error
+
 namespace {
 
 __device__ __forceinline__ float to_f32(float v) { return v; }

@@ -36,8 +36,6 @@ namespace {
 
 using namespace fs::tc;
 
-__device__ int g_group_error = 0;  // non-zero once a bounded wait gave up (read by fs_device_error)
-std::atomic<bool> g_launched{false};   // whether this process has launched a product: if not, the word is not looked at
 thread_local long long t_product_limit = kSpinLimit;  // clocks, fs_set_product_limit
 
 enum Form { ROWS_K, ROWS_MN, WEIGHTS };  // rows with W contiguous along the contraction; along the features
@@ -67,6 +65,7 @@ struct GroupArgs {
   const void* x;  // the rows as plain memory, for fetching them one by one
   long long ldx;
   long long limit;  // clocks that the warps which write results wait, besides what the products take; 0: none at all
+  int* health;      // non-zero once a bounded wait gave up (read by fs_device_error)
 };
 
 // ------------------------------------------------------------------ PTX of gathered loads
@@ -543,7 +542,7 @@ group_kernel(const GroupArgs a, const __grid_constant__ CUtensorMap mapA, const 
   if (CG == 2) cluster_sync_all();
   tc_fence_after();
   if (warp == kMmaWarp) free_columns<CG>(tmem, kColumns);
-  if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_group_error, 1);
+  if (threadIdx.x == 0 && *abort_flag) atomicExch(a.health, 1);
 }
 
 // ------------------------------------------------------------------ few rows
@@ -701,7 +700,8 @@ int launch_group(GroupArgs a, const CUtensorMap& mapA, const CUtensorMap& mapB, 
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  g_launched.store(true, std::memory_order_relaxed);
+  a.health = products_health();
+  if (!a.health) return report_error(FS_ERR_CUDA, "cannot find the health word of the current CUDA device");
   e = cudaLaunchKernelEx(&cfg, kernel, a, mapA, mapB);
   if (e != cudaSuccess) return report_error(FS_ERR_CUDA, cudaGetErrorString(e));
   count_launches(1);
@@ -768,20 +768,6 @@ int not_loadable() {
 }  // namespace
 
 long long product_limit() { return t_product_limit; }
-
-// Solvers read the health word where the host waits anyway. A copy of this part takes 12 us, and 10 ms the first time, for the
-// kernels' module to be loaded: not for programs without products.
-int group_error_flag() {
-  if (!g_launched.load(std::memory_order_relaxed)) return 0;
-  int v = 0;
-  if (cudaMemcpyFromSymbol(&v, g_group_error, sizeof(int)) != cudaSuccess) return -1;
-  return v ? 1 : 0;
-}
-int clear_group_error_flag() {
-  if (!g_launched.load(std::memory_order_relaxed)) return 0;
-  const int zero = 0;
-  return cudaMemcpyToSymbol(g_group_error, &zero, sizeof(int)) == cudaSuccess ? 0 : -1;
-}
 
 }  // namespace ex
 }  // namespace fs

@@ -32,9 +32,6 @@ long long product_limit();  // fs_group.cu: of the calling thread
 
 namespace {
 
-__device__ int g_mm8_error = 0;  // non-zero once a bounded wait gave up (read by fs_device_error)
-std::atomic<bool> g_mm8_launched{false};
-
 constexpr int kBlock8 = 128;  // values that share a scale
 constexpr float kTop8 = 448.f;
 
@@ -207,6 +204,7 @@ struct Mm8Args {
   bool boxes;               // whole blocks of 32 rows are written by TMA
   int nstage;
   unsigned limit;  // clocks that the warps which sum wait for a block of products; 0: none at all
+  int* health;     // non-zero once a bounded wait gave up (read by fs_device_error)
 };
 
 template <int CG>
@@ -529,7 +527,7 @@ mm8_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapA, const __gr
   }
   settle<CG, 1>(abort_flag, words, bar(FULL), bar(DRAIN), a.nstage, warp == kIssueWarp, warp == kFetchWarp);
   if (warp == kIssueWarp) free_columns<CG>(tmem, kColumns);
-  if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_mm8_error, 1);
+  if (threadIdx.x == 0 && *abort_flag) atomicExch(a.health, 1);
 }
 
 // ------------------------------------------------------------------ short groups
@@ -718,7 +716,7 @@ mm8_short_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapW, cons
   }
   settle<1, 1>(abort_flag, words, bar(FULL), bar(DRAIN), a.nstage, warp == kShortIssue, warp == kShortFetch);
   if (warp == kShortIssue) free_columns<1>(tmem, kColumns);
-  if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_mm8_error, 1);
+  if (threadIdx.x == 0 && *abort_flag) atomicExch(a.health, 1);
 }
 
 // ------------------------------------------------------------------ few rows
@@ -926,7 +924,8 @@ int launch_mm8(Mm8Args a, const uint8_t* x, long long ldx, const uint8_t* w, lon
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  g_mm8_launched.store(true, std::memory_order_relaxed);
+  a.health = products_health();
+  if (!a.health) return report_error(FS_ERR_CUDA, "cannot find the health word of the current CUDA device");
   e = cudaLaunchKernelEx(&cfg, kernel, a, mapA, mapB, mapC);
   if (e != cudaSuccess) return report_error(FS_ERR_CUDA, cudaGetErrorString(e));
   count_launches(1);
@@ -957,7 +956,8 @@ int launch_short8(Mm8Args a, const uint8_t* x, long long ldx, const uint8_t* w, 
   long long grid = detail::free_ctas() * (detail::free_ctas() == detail::sm_count() ? 2ll : 1ll);
   if (grid > most) grid = most;
   if (grid < 1) grid = 1;
-  g_mm8_launched.store(true, std::memory_order_relaxed);
+  a.health = products_health();
+  if (!a.health) return report_error(FS_ERR_CUDA, "cannot find the health word of the current CUDA device");
   kernel<<<(unsigned)grid, kShortThreads, kShortSmem - kStatic, st>>>(a, mapW, mapX);
   return launched(1);
 }
@@ -1002,19 +1002,6 @@ int check8(int R, int E, int N, int K) {
 bool is16(int type) { return type == FS_TYPE_F16 || type == FS_TYPE_BF16; }
 
 }  // namespace
-
-int mm8_error_flag() {
-  if (!g_mm8_launched.load(std::memory_order_relaxed)) return 0;
-  int v = 0;
-  if (cudaMemcpyFromSymbol(&v, g_mm8_error, sizeof(int)) != cudaSuccess) return -1;
-  return v ? 1 : 0;
-}
-int clear_mm8_error_flag() {
-  if (!g_mm8_launched.load(std::memory_order_relaxed)) return 0;
-  const int zero = 0;
-  return cudaMemcpyToSymbol(g_mm8_error, &zero, sizeof(int)) == cudaSuccess ? 0 : -1;
-}
-
 }  // namespace ex
 }  // namespace fs
 

@@ -33,9 +33,6 @@ long long product_limit();  // fs_group.cu: of the calling thread
 
 namespace {
 
-__device__ int g_ortho_error = 0;  // non-zero once a bounded wait gave up (read by fs_device_error)
-std::atomic<bool> g_ortho_launched{false};
-
 constexpr float kXScale = 256.f, kAScale = 1024.f;  // X and A are held times these
 // X goes without its lower part once what is left of the steps multiplies a rounding along small singular values by no more than this: with the default
 // coefficients before the last step, which leaves 3.4 roundings of 2e-4 in the mean, 0.07 %. At 16, before the last two, matrices that have
@@ -148,6 +145,7 @@ struct OrthoArgs {
   bool backwards;  // the last matrix first: it is what the product before left in L2
   int nstage;
   long long limit;
+  int* health;  // non-zero once a bounded wait gave up (read by fs_device_error)
 };
 
 template <int FORM, int CG, int BN>
@@ -512,10 +510,10 @@ __device__ __forceinline__ void ortho_product(const OrthoArgs& a, const CUtensor
 }
 
 template <int CG, int BN>
-__device__ __forceinline__ void ortho_end(const OrthoPipe& p) {
+__device__ __forceinline__ void ortho_end(const OrthoPipe& p, int* health) {
   settle<CG, 2>(p.abort_flag, p.words, p.bar(p.full()), p.bar(p.drain()), p.nstage, p.warp == kMulWarp, p.warp == kGetWarp);
   if (p.warp == kMulWarp) free_columns<CG>(p.tmem, 2 * BN);
-  if (threadIdx.x == 0 && *p.abort_flag) atomicExch(&g_ortho_error, 1);
+  if (threadIdx.x == 0 && *p.abort_flag) atomicExch(health, 1);
 }
 
 template <int FORM, int CG, int BN>
@@ -524,7 +522,7 @@ ortho_kernel(const OrthoArgs a, const __grid_constant__ CUtensorMap mapA, const 
   extern __shared__ uint8_t raw[];
   OrthoPipe p = ortho_begin<CG, BN>(raw, a.nstage);
   ortho_product<FORM, CG, BN>(a, &mapA, &mapB, p);
-  ortho_end<CG, BN>(p);
+  ortho_end<CG, BN>(p, a.health);
 }
 
 // All products of all steps in one launch, for small matrices, whose products take less than a launch: every CTA does its tiles of
@@ -585,7 +583,7 @@ __global__ void __launch_bounds__(kThreadsO, 1) ortho_chain_kernel(OrthoArgs a, 
       ortho_product<LAST, 1, kChainBN>(a, &maps.p128, &maps.x64[from], p);
     }
   }
-  ortho_end<1, kChainBN>(p);
+  ortho_end<1, kChainBN>(p, a.health);
 }
 
 // ------------------------------------------------------------------ host side
@@ -640,7 +638,8 @@ int launch_ortho(OrthoArgs a, cudaStream_t st) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  g_ortho_launched.store(true, std::memory_order_relaxed);
+  a.health = products_health();
+  if (!a.health) return report_error(FS_ERR_CUDA, "cannot find the health word of the current CUDA device");
   e = cudaLaunchKernelEx(&cfg, kernel, a, mapA, mapB);
   if (e != cudaSuccess) return report_error(FS_ERR_CUDA, cudaGetErrorString(e));
   count_launches(1);
@@ -683,7 +682,8 @@ int launch_chain(OrthoArgs a, const OrthoChain& c, cudaStream_t st) {
   attr.val.cooperative = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  g_ortho_launched.store(true, std::memory_order_relaxed);
+  a.health = products_health();
+  if (!a.health) return report_error(FS_ERR_CUDA, "cannot find the health word of the current CUDA device");
   e = cudaLaunchKernelEx(&cfg, ortho_chain_kernel, a, c, maps);
   if (e != cudaSuccess) return report_error(FS_ERR_CUDA, cudaGetErrorString(e));
   count_launches(1);
@@ -740,19 +740,6 @@ OrthoSpace ortho_space(int batch, int rows, int cols) {
 }
 
 }  // namespace
-
-int ortho_error_flag() {
-  if (!g_ortho_launched.load(std::memory_order_relaxed)) return 0;
-  int v = 0;
-  if (cudaMemcpyFromSymbol(&v, g_ortho_error, sizeof(int)) != cudaSuccess) return -1;
-  return v ? 1 : 0;
-}
-int clear_ortho_error_flag() {
-  if (!g_ortho_launched.load(std::memory_order_relaxed)) return 0;
-  const int zero = 0;
-  return cudaMemcpyToSymbol(g_ortho_error, &zero, sizeof(int)) == cudaSuccess ? 0 : -1;
-}
-
 }  // namespace ex
 }  // namespace fs
 
