@@ -650,6 +650,7 @@ Tensor grouped_mm8(const Tensor& x0, const optional<Tensor>& w0, const optional<
             "scales must be a contiguous float32 tensor of shape (E, ceil(N / 128), ceil(K / 128)) for codes ", shape_of(w), ", got ", type_name(scales), " ",
             shape_of(scales));
     REQUIRE(!scales.requires_grad() && !w.requires_grad(), "codes and scales must not require grad");
+    check_tangent("scales", scales);
   }
   check_cuda("x", x0);
   check_place("weight", w, "x", x0);
