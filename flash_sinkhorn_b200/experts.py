@@ -171,6 +171,9 @@ def expert_mlp(x: torch.Tensor, w_in: Union[torch.Tensor, Blocks8], w_out: Union
     if isinstance(w_in, Blocks8) or isinstance(w_out, Blocks8):
         if not (isinstance(w_in, Blocks8) and isinstance(w_out, Blocks8)):
             raise ValueError("w_in and w_out must both be Blocks8, or neither")
+        n_in, n_out = w_in.codes.shape, w_out.codes.shape
+        if x.ndim != 2 or len(n_in) != 3 or n_in[1:] != (2 * n_out[-1], x.shape[1]) or n_out[:-1] != (n_in[0], x.shape[1]):
+            raise ValueError(f"x must be [T, D], w_in [E, 2 F, D] and w_out [E, D, F], got {tuple(x.shape)}, {tuple(n_in)} and {tuple(n_out)}")
         h = gated_act(grouped_mm8(x, w_in, routing, gather=True), routing, checkpoint=checkpoint)
         return combine_rows(grouped_mm8(h, w_out, routing), routing, weighted=False)
     r = routing

@@ -28,3 +28,13 @@ def test_a_tangent_of_scales_is_refused(ex):
         dual = fwd.make_dual(q.scales, torch.ones_like(q.scales))
         with pytest.raises(ValueError, match="scales must not have a forward-mode tangent"):
             ex.grouped_mm8(x, ex.Blocks8(q.codes, dual), off)
+
+
+@pytest.mark.parametrize("w_in,w_out", [((2, 96, 64), (2, 72, 48)), ((2, 96, 64), (2, 56, 48)), ((2, 96, 64), (3, 64, 48)), ((2, 96, 64), (2, 64, 40)),
+                                        ((2, 96, 72), (2, 64, 48)), ((2, 95, 64), (2, 64, 47))])
+def test_held_weights_of_a_layer_fit_one_another(ex, w_in, w_out):
+    """Also where the sums back into tokens would come out with another width than the rows."""
+    x = torch.zeros(3, 64, dtype=torch.bfloat16)
+    r = ex.Routing(torch.zeros(3, 2), *[torch.zeros(3, 2, dtype=torch.int32)] * 5)
+    with pytest.raises(ValueError, match=r"w_in \[E, 2 F, D\] and w_out \[E, D, F\]"):
+        ex.expert_mlp(x, held(ex, *w_in), held(ex, *w_out), r)
