@@ -1076,8 +1076,11 @@ int fs_grouped_mm8(const void* x, int type, long long ldx, int M, const int* row
   // 1024 -> 2048 -, 35, 34; 32 of 200 rows, 2048 x 2048 -, 64, 54; one of 1024 rows, 1024 x 1024 -, 8.1, 11.6.
   const long long tiles = ((R + 255ll) / 256 + (E < R ? E : R) / 2) * ((N + 255) / 256);
   const bool pairs = tiles * 2 > detail::free_ctas() && N > 128;
+  // The transposed product has no short tiles; its pairs pay from 144 rows on. us with 128 x 128 and 256 x 256, sizes of groups as a skewed routing gives them
+  // (equal ones up to 48): 64 experts, 1024 -> 2048, 2 rows 45, 59; 48 rows 47, 64; 80 rows 54, 67; 130 rows 68, 73; 160 rows 75, 74; 200 rows 88, 80;
+  // 128 experts, 2048 -> 1024, 16 rows 76, 92; 100 rows 108, 110; 145 rows 132, 123; 200 rows 168, 143.
   if (transposed) {
-    if (pairs) return launch_mm8<true, 2, 256>(a, codes, ldc, w, w_expert, w_row, st);
+    if (pairs && R / E >= 144) return launch_mm8<true, 2, 256>(a, codes, ldc, w, w_expert, w_row, st);
     return launch_mm8<true, 1, 128>(a, codes, ldc, w, w_expert, w_row, st);
   }
   if (R / E <= 40) return launch_short8(a, codes, ldc, w, w_expert, w_row, st);

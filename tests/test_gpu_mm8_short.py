@@ -29,3 +29,16 @@ def test_many_tiles_of_odd_numbers_of_blocks(ex, k):
     close(first, want, size, BF16)
     for _ in range(20):
         assert torch.equal(ex.grouped_mm8(x, q, off), first)
+
+
+@pytest.mark.parametrize("mean", [17, 143, 145])
+def test_gradient_to_rows_on_both_sides_of_its_choice(ex, mean):
+    """Enough tiles of 256 x 256 for all CTAs, groups below and above the rows from which pairs take them."""
+    g = gen(mean)
+    e, n, k = 40, 264, 1100
+    counts = [mean - 9, mean + 9] * (e // 2)
+    x, off = normal(g, sum(counts), k, dtype=BF16).requires_grad_(), offsets_of(counts)
+    w, dy = normal(g, e, n, k, scale=k**-0.5, dtype=BF16), normal(g, sum(counts), n, dtype=BF16)
+    codes, scales = blocks8(w)
+    (dx,) = torch.autograd.grad(ex.grouped_mm8(x, w, off), x, dy)
+    close(dx, *grouped(rows8(dy), codes * wide(scales, n, k), off[1:].tolist(), transposed=True), BF16)
