@@ -697,7 +697,11 @@ int launch_form(const OrthoArgs& a, cudaStream_t st) {
     const long long m = (a.n + bm - 1) / bm, n = ((FORM >= APPLY ? a.k : a.n) + bn - 1) / bn;
     return (FORM >= APPLY ? m * n : m * n / 2 + 1) * a.batch;
   };
-  if (tiles(256, 256) * 2 > ctas) return launch_ortho<FORM, 2, 256>(a, st);
+  // Pairs where there are tiles of 256 x 256 for all of them, and rows for both CTAs; then the largest tile with which there is one for every CTA. us of five
+  // steps with tiles of 128 x 64, 128 x 128 and 256 x 256 throughout (as chosen they differ from product to product): 32 matrices of 128 x 2048 198,
+  // 202, 290; 300 of 64 x 72 155, 157, 262; 64 of 128 x 512 147, 145, 196; 32 of 256 x 2048 344, 303, 335; 16 of 300 x 700 180, 165, 233; 32 of 512 x 512 303,
+  // 282, 294; 32 of 1024 x 2048 2362, 1732, 1581; one of 4096 x 4096 2651, 1575, 1230.
+  if (a.n > 128 && tiles(256, 256) * 2 > ctas) return launch_ortho<FORM, 2, 256>(a, st);
   if (tiles(128, 128) > ctas) return launch_ortho<FORM, 1, 128>(a, st);
   return launch_ortho<FORM, 1, 64>(a, st);
 }

@@ -30,3 +30,11 @@ def test_roundings_along_small_singular_values(ortho, n, k):
     g = gen(n)
     m = normal(g, 2, n, 1) @ normal(g, 2, 1, k)
     assert relative(ortho(m, dtype=FP16), plain(m)) <= 1.6e-3
+
+
+@pytest.mark.parametrize("n,k", [(128, 1000), (129, 1000), (1000, 128), (90, 2048)])
+def test_stacks_of_few_rows(ortho, n, k):
+    """Stacks too large for one launch, matrices whose rows fill one CTA of a pair or not even that; the bound is that of all updates."""
+    from test_gpu_orthogonalize import check
+    m = normal(gen(n + k), 40, n, k)
+    check(ortho(m), plain(m))
