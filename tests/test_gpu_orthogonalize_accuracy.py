@@ -38,3 +38,23 @@ def test_stacks_of_few_rows(ortho, n, k):
     from test_gpu_orthogonalize import check
     m = normal(gen(n + k), 40, n, k)
     check(ortho(m), plain(m))
+
+
+@pytest.mark.parametrize("n,k", [(1, 1), (1, 5), (2, 2), (2, 3), (3, 3), (4, 4), (2, 64), (5, 2)])
+def test_few_rows(ortho, n, k):
+    """Nothing averages: one singular value is off by at most 2e-2 (test_gpu_orthogonalize.py), and roundings of several entries, each at most u of
+    its own, are an error matrix whose 2-norm is up to sqrt(rows) times that of one, of which two rows can come together: 2e-2 sqrt(2), with the
+    result's own rounding of 2^-11 less than the 3 % that are documented."""
+    m = normal(gen(n + 10 * k), 100_000, n, k)
+    assert relative(ortho(m, dtype=FP16), plain(m)) <= 3e-2
+
+
+@pytest.mark.parametrize("n,k", [(64, 64), (200, 300), (512, 256), (700, 1024)])
+def test_where_singular_values_go(ortho, n, k):
+    """From 0.003 on to between 0.6818 and 1.2024 in exact arithmetic (extremes of the steps' polynomial there); 0.5 % for roundings."""
+    g, r = gen(n), min(n, k)
+    u, v = torch.linalg.qr(normal(g, n, r))[0], torch.linalg.qr(normal(g, k, r))[0]
+    spread = max(a for a in (0.5, 1.0, 1.5, 2.0) if 10**-a / torch.logspace(-a, 0, r).norm() >= 0.0031)
+    m = (u * torch.logspace(-spread, 0, r, device="cuda")) @ v.T
+    values = torch.linalg.svdvals(ortho(m, dtype=FP16).double())[:r]
+    assert values.max() <= 1.2024 * 1.005 and values.min() >= 0.6818 * 0.995
