@@ -58,3 +58,15 @@ def test_where_singular_values_go(ortho, n, k):
     m = (u * torch.logspace(-spread, 0, r, device="cuda")) @ v.T
     values = torch.linalg.svdvals(ortho(m, dtype=FP16).double())[:r]
     assert values.max() <= 1.2024 * 1.005 and values.min() >= 0.6818 * 0.995
+
+
+@pytest.mark.parametrize("batch,n,k", [(3, 140, 90), (3, 1, 50), (3, 600, 600), (40, 130, 1000), (30, 700, 512)])
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+def test_a_matrix_with_a_value_that_is_not_finite_gives_nan_throughout(ortho, batch, n, k, value):
+    m = normal(gen(n), batch, n, k)
+    want = ortho(m)
+    m[1, n // 2, k - 1] = value
+    for steps in (1, 5):
+        y = ortho(m, steps=steps)
+        assert torch.isnan(y[1]).all() and torch.isfinite(y[[0, 2]]).all()
+    assert torch.equal(y[[0, 2]], want[[0, 2]])
