@@ -12,8 +12,9 @@
 // TMEM (fp32); eight warps read that while the next block is summed beside it, and add it, scaled, to sums in registers.
 // Per block and 128 x 256 tile the products take 512 clocks of the tensor core, reading 256 of TMEM and adding 256 of the fp32 units, but
 // each of the two accumulators goes from the tensor core to the warps of both CTAs and back, which takes some 1200 clocks by itself: a
-// block takes 550 ns, where loads and products alone take 373 (from HBM 550). 65536 rows of 64 experts, 2048 x 2048: 300 us, 1830 TFLOP/s, against
-// 390 us of the 16-bit product; with 1024 or 4096 contraction values 1510 and 2010 TFLOP/s (a tile costs 2 us besides its blocks).
+// block takes 550 ns, where loads and products alone take 373 (from HBM 550). 65536 rows of 64 equal groups, 2048 x 2048: 300 us, 1830 TFLOP/s, against
+// 390 us of the 16-bit product (groups as a routing gives them: 326; under the power cap, after half a second of calls, 15 % more); with 1024 or 4096
+// contraction values 1530 and 2040 TFLOP/s (a tile costs 2 us besides its blocks). The thread that issues waits for sums for 58 % of its clocks, for loads 9.
 // What decided it: registers that spill in the loop of sums (a factor 1.5), loads of 16 columns a step ahead of the additions, results by TMA, and
 // in the wait for a block no more than a look: with its limit handled there in 64 bits, before the first look, the same product took 334 us.
 // Accumulators and barriers of their own for the two halves of a tile cost more than they saved (695 ns a block): products of 128 columns read as much
@@ -534,7 +535,7 @@ mm8_kernel(const Mm8Args a, const __grid_constant__ CUtensorMap mapA, const __gr
 // Groups of up to a few dozen rows are bound by reading their weights. Here the FEATURES are the M side and the rows N, as in the
 // 16-bit products: a stage is 16 KB of weights and 4 KB of rows, an accumulator kShortRows columns, of which 256 / kShortRows are in use in turn, so that the
 // tensor core does not wait for the sums. Two CTAs to an SM: one's first loads of a tile hide behind the other one's products. 64 experts of 2048 x 1024
-// with two rows each: 29 us, 4.6 TB/s, some 8 of them launch, first loads and the last, partly filled round; twice the features 50 us, 5.3 TB/s.
+// with two rows each: 28 us, 4.8 TB/s, some 8 of them launch, first loads and the last, partly filled round; twice the features 49 us, 5.4 TB/s.
 constexpr int kShortRows = 32;                                       // of a tile: a lane's factor is that of one
 constexpr int kShortThreads = 192, kShortFetch = 4, kShortIssue = 5;  // four warps that sum
 constexpr size_t kShortSmem = 112 * 1024;                            // two fit an SM, and no kernel of this library beside one: they take 120 KB

@@ -16,11 +16,12 @@
 // stack; tiles of 256 x 256 by pairs of CTAs, or 128 x 128 or 128 x 64 by single ones where there are too few. Small matrices go through all
 // products in one launch.
 //
-// 32 matrices of 2048 x 1024, five steps: 1346 us, of which a step's A takes 73, P 45 and P X 129 (without X's lower part 115); their floors are 52, 26 and
-// 83 at the burst rate of the tensor cores, a fifth more under the power cap, and what they lose besides is a partly filled round of tiles (4.3 rounds
-// of A and P count as 5) and 540 MB through HBM in the first steps' P X. One matrix of 512 x 512: 86 us, 15 products of 5 us each, of which 2.2 are
-// loads (a CTA's 192 KB, at most 60 bytes a clock), 0.8 the results and 1.5 the CTAs' meeting. Divisions of 64 bits and spilled registers between its
-// products, which every thread waited for, had taken another us of each.
+// 32 matrices of 2048 x 1024, five steps: 1410 us on the device, of which squares and X take 115, a step's A 75, P 46 and P X 139 (the last one, without X's
+// lower part, 124); the products' floors are 52, 26 and 83 at the burst rate of the tensor cores. A call takes 1480 us, and 1690 after half a second of them,
+// under the power cap (1.3 GHz). Without the cap the tensor pipe is busy for 48 (A), 34 (P), 48 (P X) and 56 % (without the lower part) of the time;
+// the thread that issues waits for loads for 46, 38, 36 and 25 % of its clocks and for the writers of results for 1, 6, 18 and 17 %: a partly filled
+// round of tiles (4.3 rounds of A and P count as 5) and X's lower part, 540 MB through HBM in each P X but the last. One matrix of 512 x 512: a call
+// 82 us, 72 in 15 products of 4.8 each, of which 2.2 are loads (a CTA's 192 KB, at most 60 bytes a clock), 0.8 the results and 1.5 the CTAs' meeting.
 #include "fs_experts.cuh"
 #include "fs_pair.cuh"
 #include "fs_tc.cuh"
@@ -268,7 +269,7 @@ __device__ __forceinline__ void ortho_product(const OrthoArgs& a, const CUtensor
   if (warp == kGetWarp || warp == kGetWarpB) {
     // ===================== loads =====================
     // A warp for each operand: one thread takes 150 to 200 clocks for a tensor load, and a stage of P X has three of them for products of 512
-    // (32 matrices of 2048 x 1024: 1405 -> 1346 us).
+    // (32 matrices of 2048 x 1024: 1405 -> 1346 us when it was measured, with X's lower part in three steps).
     if (elect_one()) {
       int s = p.s, issued = 0;
       uint32_t ph = p.ph;
